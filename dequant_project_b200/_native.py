@@ -35,6 +35,15 @@ class L2Spans(ctypes.Structure):
         return s
 
 
+class PagedKV(ctypes.Structure):
+    """``dqg_paged_kv``: two pools of key and value pages."""
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("n_pages", ctypes.c_int64),
+                ("n_kv_heads", ctypes.c_int64), ("page_size", ctypes.c_int64),
+                ("head_dim", ctypes.c_int64), ("page_stride", ctypes.c_int64),
+                ("head_stride", ctypes.c_int64), ("row_stride", ctypes.c_int64),
+                ("dtype", ctypes.c_int32)]
+
+
 def lib() -> ctypes.CDLL:
     """Load (once) and return the C-ABI library."""
     global _lib
@@ -101,6 +110,15 @@ def lib() -> ctypes.CDLL:
     h.dqg_decode_attention_noalloc.argtypes = [vp, vp, vp, vp, i64, i64, i64, i64, i64, i64, vp]
     h.dqg_stream_plan.restype = i32
     h.dqg_stream_plan.argtypes = [i64, i64, i64, i64, i64, i32, ctypes.POINTER(ctypes.c_int32), i32]
+    u64, f32, kv = ctypes.c_uint64, ctypes.c_float, ctypes.POINTER(PagedKV)
+    h.dqg_rope_paged_append.restype = i32
+    h.dqg_rope_paged_append.argtypes = [vp, i64, i64, i64, vp, vp, i64, i64, i32, vp, vp, vp, vp,
+                                        f32, kv, vp, vp]
+    h.dqg_paged_attention_workspace.restype = i32
+    h.dqg_paged_attention_workspace.argtypes = [i64, u64p]
+    h.dqg_paged_attention.restype = i32
+    h.dqg_paged_attention.argtypes = [vp, i64, i64, i64, i64, kv, vp, i64, i64, vp, f32, vp, vp,
+                                      u64, vp]
     _lib = h
     return _lib
 
@@ -113,7 +131,8 @@ EXPORTED = ("dqg_last_error", "dqg_version", "dqg_add_one", "dqg_gemv", "dqg_deq
             "dqg_gemv_allreduce", "dqg_decode_attention_noalloc",
             "dqg_ipc_export", "dqg_ipc_open", "dqg_ipc_close", "dqg_peer_allreduce",
             "dqg_peer_allreduce_add_rms_norm", "dqg_gemv_swiglu",
-            "dqg_gemv_swiglu_supported")
+            "dqg_gemv_swiglu_supported", "dqg_rope_paged_append", "dqg_paged_attention_workspace",
+            "dqg_paged_attention")
 
 
 def check(rc: int) -> None:
@@ -124,7 +143,8 @@ def check(rc: int) -> None:
 
 
 def device_status(device: int, reset: bool = False) -> int:
-    """Read the device-side status word (bit 0: a kernel gave up a bounded wait)."""
+    """Read the device-side status word (bit 0: a kernel gave up a bounded wait;
+    bit 1: a paged operator left out an index out of range)."""
     v = ctypes.c_uint32(0)
     check(lib().dqg_device_status(int(device), ctypes.byref(v), int(reset)))
     return v.value

@@ -15,6 +15,7 @@
 
 #include "../../include/dequant_b200.h"
 #include "gemv.h"
+#include "paged.h"
 
 namespace {
 
@@ -227,6 +228,20 @@ int check_weight_ptrs(const int32_t* qweight, const void* scales, const void* ze
 }
 
 }  // namespace
+
+// The same error message and SM count for the entry points of capi_paged.cu.
+namespace dqg {
+int api_fail(int code, const char* fmt, ...) {
+  va_list ap;
+  va_start(ap, fmt);
+  vsnprintf(g_msg, sizeof(g_msg), fmt, ap);
+  va_end(ap);
+  return code;
+}
+int api_ok() { return ok(); }
+int api_cuda_fail(cudaError_t e, const char* what) { return cuda_fail(e, what); }
+int api_sm_count(int dev) { return sm_count(dev); }
+}  // namespace dqg
 
 extern "C" {
 

@@ -48,6 +48,7 @@
 
 #include "common.cuh"
 #include "gemv.h"
+#include "paged.h"
 
 namespace dqg {
 
@@ -637,7 +638,8 @@ cudaError_t read_device_status(int device, uint32_t* status, bool reset) {
   cudaError_t (*readers[])(uint32_t*, bool) = {read_status_gemv, read_status_stream_b2,
                                                 read_status_stream_b4, read_status_stream_b8,
                                                 read_status_peer,        read_status_direct_b2,
-                                                read_status_direct_b4,   read_status_direct_b8};
+                                                read_status_direct_b4,   read_status_direct_b8,
+                                                read_status_append,      read_status_paged_decode};
   *status = 0;
   for (auto rd : readers) {
     uint32_t v = 0;

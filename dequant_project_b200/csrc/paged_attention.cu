@@ -1,0 +1,550 @@
+// Decode attention over a paged cache: one query token per sequence, lengths
+// on the device, grouped KV heads. No reference counterpart (the reference
+// models the cache's bytes, dequant/byte_model.py:214-219).
+//
+//   o[b, h] = softmax(scale q[b, h] . K_b[:, h / g]^T) V_b[:, h / g]
+//
+// over the lens[b] positions that sequence b's pages hold; zero where there is
+// none. Every key and value row is read once, so HBM bounds it.
+//
+// Work is counted in tiles of 64 positions, sequence by sequence and KV head
+// by KV head, and cut into equal shares, one per CTA (two CTAs per SM), so that
+// lengths of any spread keep every SM streaming to the end; the shares follow
+// from the lengths on the device, so a captured launch serves other lengths.
+// In a CTA one warp copies the tiles' page rows into a ring in shared memory
+// (tensor-map boxes of whole page rows, 128-byte swizzle) and four warps take
+// 16 positions of a tile each: S^T = Q K^T by mma.m16n8k16 with the KV head's
+// query heads as the A rows, online softmax in fp32, O += P V with P (16-bit,
+// as the values are) from the score registers. An item (sequence, head) that
+// lies in one share is finished by its CTA; one that is cut leaves a (max, sum,
+// O) piece per CTA in the workspace, and a second small kernel joins the
+// pieces in order. No atomics: the same lengths give the same bits.
+#include <cstdint>
+
+#include "paged.cuh"
+
+namespace dqg {
+namespace {
+
+constexpr int kTile = 64;              // positions per tile
+constexpr int kWarps = 4;              // consumer warps
+constexpr int kThreads = 32 * (kWarps + 1);
+constexpr int kStages = 3;
+constexpr int kCtasPerSm = 2;
+constexpr int kMergeRows = 4;          // query heads per round of the warps' merge
+
+struct Desc {  // a cut item, by the CTA that holds its first piece
+  int b, hv, pieces, pad;
+};
+
+struct Params {
+  const void* q;
+  void* out;
+  const int32_t* table;
+  const int32_t* lens;
+  float* part;   // [CTA][2][16][D]
+  float* ml;     // [CTA][2][2][16]
+  Desc* desc;    // [CTA]
+  int64_t q_stride_seq, q_stride_head, table_stride, n_pages;
+  int B, hq, hkv, g, nrb, page_shift, len_limit, box_rows;
+  float scale_log2;
+  PrefixPieces prefix;
+};
+
+// Row of a prefix piece that holds query head j of KV head `kvh` in sequence
+// b, and the first of the item's pieces (layout of prompt_attention.cu).
+__device__ __forceinline__ int64_t prefix_first(const PrefixPieces& f, int hkv, int b, int kvh) {
+  return (static_cast<int64_t>(b / (2 * f.tq)) * hkv + kvh) * f.S;
+}
+__device__ __forceinline__ int prefix_row(const PrefixPieces& f, int g, int b, int j) {
+  return ((b / f.tq) & 1) * 128 + (b % f.tq) * g + j;
+}
+
+// Four outputs of one query head from the item's own (max, sum, O) and the
+// shared prefix's pieces, in piece order.
+template <typename E, int D>
+__device__ __forceinline__ void finish(const Params& p, int b, int head, int d4, float mx, float den,
+                                       float4 num) {
+  if (p.prefix.S > 0) {
+    const int kvh = head / p.g, row = prefix_row(p.prefix, p.g, b, head % p.g);
+    const int64_t first = prefix_first(p.prefix, p.hkv, b, kvh);
+    const float* ml = p.prefix.ml + first * 512 + row;
+    float m = mx;
+    for (int s = 0; s < p.prefix.S; ++s) m = fmaxf(m, __ldcg(ml + s * 512));
+    const float mu = m == -INFINITY ? 0.f : m;
+    float f = exp2_approx(mx - mu);
+    den *= f;
+    num.x *= f; num.y *= f; num.z *= f; num.w *= f;
+    const float4* po = reinterpret_cast<const float4*>(p.prefix.o) + (first * (D / 4) + d4) * 256 + row;
+#pragma unroll 4
+    for (int s = 0; s < p.prefix.S; ++s) {
+      f = exp2_approx(__ldcg(ml + s * 512) - mu);
+      den = fmaf(__ldcg(ml + s * 512 + 256), f, den);
+      const float4 v = __ldcg(po + static_cast<int64_t>(s) * (D / 4) * 256);
+      num.x = fmaf(v.x, f, num.x);
+      num.y = fmaf(v.y, f, num.y);
+      num.z = fmaf(v.z, f, num.z);
+      num.w = fmaf(v.w, f, num.w);
+    }
+  }
+  const float inv = den == 0.f ? 0.f : __frcp_rn(den);
+  E* o = static_cast<E*>(p.out) + (static_cast<int64_t>(b) * p.hq + head) * D + d4 * 4;
+  uint2 w;
+  w.x = Elem<E>::pack(num.x * inv, num.y * inv);
+  w.y = Elem<E>::pack(num.z * inv, num.w * inv);
+  *reinterpret_cast<uint2*>(o) = w;
+}
+
+__device__ __forceinline__ int tiles_of(int len) { return len > 0 ? (len + kTile - 1) / kTile : 1; }
+
+// A CTA's share of the tiles: where it starts and how many it takes.
+struct Share {
+  int b, hv, x, ctas;
+  long long count, pos, total;
+};
+
+// Taken by one whole warp.
+__device__ __forceinline__ Share find_share(const Params& p, int cta, int n_ctas) {
+  const int lane = threadIdx.x & 31;
+  const long long hv = static_cast<long long>(p.hkv) * p.nrb;
+  long long total = 0;
+  for (int b0 = 0; b0 < p.B; b0 += 32) {
+    const int b = b0 + lane;
+    total += b < p.B ? tiles_of(clamped_len(p.lens, b, p.len_limit)) : 0;
+  }
+#pragma unroll
+  for (int off = 16; off >= 1; off >>= 1) total += __shfl_xor_sync(0xffffffffu, total, off);
+  total *= hv;
+  Share s;
+  s.total = total;
+  s.ctas = n_ctas < total ? n_ctas : static_cast<int>(total);
+  s.b = s.hv = s.x = 0;
+  s.pos = s.count = 0;
+  if (cta >= s.ctas) return s;
+  s.pos = cta * total / s.ctas;
+  s.count = (cta + 1) * total / s.ctas - s.pos;
+  long long before = 0;
+  for (int b0 = 0; b0 < p.B; b0 += 32) {
+    const int b = b0 + lane;
+    const int nt = b < p.B ? tiles_of(clamped_len(p.lens, b, p.len_limit)) : 0;
+    long long sum = nt * hv;
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+      const long long t = __shfl_up_sync(0xffffffffu, sum, off);
+      if (lane >= off) sum += t;
+    }
+    const unsigned past = __ballot_sync(0xffffffffu, before + sum > s.pos);
+    if (past) {
+      const int l = __ffs(past) - 1;
+      const long long in = s.pos - (before + __shfl_sync(0xffffffffu, sum - nt * hv, l));
+      const int n = __shfl_sync(0xffffffffu, nt, l);
+      s.b = b0 + l;
+      s.hv = static_cast<int>(in / n);
+      s.x = static_cast<int>(in - static_cast<long long>(s.hv) * n);
+      break;
+    }
+    before += __shfl_sync(0xffffffffu, sum, 31);
+  }
+  return s;
+}
+
+__device__ __forceinline__ void ldsm_x4(uint32_t addr, uint32_t* r) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr));
+}
+__device__ __forceinline__ void ldsm_x4_trans(uint32_t addr, uint32_t* r) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr));
+}
+
+// Byte offset of 16-byte chunk `chunk` of row `row` in a tile: halves of 64
+// values, 128-byte rows, swizzled as the tensor map writes them.
+__device__ __forceinline__ uint32_t tile_off(int row, int chunk) {
+  return static_cast<uint32_t>((chunk >> 3) * (kTile * 128) + row * 128 + (((chunk & 7) ^ (row & 7)) << 4));
+}
+
+template <int D>
+struct Layout {
+  static constexpr int kTileBytes = kTile * D * 2;
+  static constexpr int kRing = kStages * 2 * kTileBytes;
+  static constexpr int kMerge = kWarps * kMergeRows * D * 4;
+  static constexpr int kSmem = 1024 + kRing + kMerge + kWarps * 16 * 8 + 2 * kStages * 8 + 64;
+};
+
+template <typename E, int D>
+__global__ void __launch_bounds__(kThreads, kCtasPerSm)
+    paged_decode_kernel(const __grid_constant__ Params p, const __grid_constant__ CUtensorMap kmap,
+                        const __grid_constant__ CUtensorMap vmap) {
+  using L = Layout<D>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
+  float* os = reinterpret_cast<float*>(smem + L::kRing);             // [warp][4][D]
+  float* ms = reinterpret_cast<float*>(smem + L::kRing + L::kMerge);  // [warp][16]
+  float* ls = ms + kWarps * 16;
+  uint64_t* full = reinterpret_cast<uint64_t*>(ls + kWarps * 16);
+  uint64_t* empty = full + kStages;
+  Share* share = reinterpret_cast<Share*>(empty + kStages);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kStages; ++i) {
+      mbar_init(full + i, 1);
+      mbar_init(empty + i, kWarps);
+    }
+    fence_mbar_init();
+    tma_prefetch_map(&kmap);
+    tma_prefetch_map(&vmap);
+  }
+  // After a prefix kernel (which every one of its CTAs lets this one start
+  // from only once its own inputs are complete), the queries, pages and
+  // lengths may be read at once; only the prefix's pieces need the wait.
+  const bool late = p.prefix.S > 0;
+  if (!late) pdl_wait_prior_grid();
+  if (warp == 0) {
+    const Share s = find_share(p, blockIdx.x, gridDim.x);
+    if (lane == 0) *share = s;
+  }
+  __syncthreads();
+  pdl_launch_dependents();
+  Share s = *share;
+  const int n_hv = p.hkv * p.nrb;
+
+  if (warp == kWarps) {
+    // ---- the copying warp: 16-row (or box_rows-row) pieces of page rows.
+    const int per = p.box_rows;                 // rows a box
+    const int boxes = kTile / per * (D / 64);   // K boxes a tile; as many V boxes
+    const int my = lane, half = my % (D / 64), sub = my / (D / 64);
+    int it = 0;
+    bool ok = true;
+    while (s.count > 0 && ok) {
+      const int raw = __ldg(p.lens + s.b);
+      const int len = clamped_len(p.lens, s.b, p.len_limit);
+      if (lane == 0 && raw != len) atomicOr(&g_status, kStatusBadIndex);
+      const int nt = tiles_of(len);
+      const int n = static_cast<int>(min(static_cast<long long>(nt - s.x), s.count));
+      const int32_t* row = p.table + s.b * p.table_stride;
+      const int kvh = s.hv / p.nrb;
+      for (int x = s.x; x < s.x + n; ++x, ++it) {
+        const int st = it % kStages;
+        const int t = x * kTile + sub * per;
+        int page = static_cast<int>(p.n_pages);  // no such page: zeros
+        if (my < boxes && t < len) {
+          page = __ldg(row + (t >> p.page_shift));
+          if (page < 0 || page >= p.n_pages) {
+            page = static_cast<int>(p.n_pages);
+            atomicOr(&g_status, kStatusBadIndex);
+          }
+        }
+        if (it >= kStages && !warp_wait(empty + st, ((it / kStages) & 1) ^ 1)) {
+          ok = false;
+          break;
+        }
+        if (lane == 0) mbar_arrive_expect_tx(full + st, 2 * L::kTileBytes);
+        __syncwarp();
+        if (my < boxes) {
+          const uint32_t dst = smem_u32(smem) + st * 2 * L::kTileBytes + half * (kTile * 128) + sub * per * 128;
+          const int in_page = t & ((1 << p.page_shift) - 1);
+          tma_load_4d(dst, &kmap, full + st, half * 64, in_page, kvh, page);
+          tma_load_4d(dst + L::kTileBytes, &vmap, full + st, half * 64, in_page, kvh, page);
+        }
+      }
+      s.count -= n;
+      s.x = 0;
+      if (++s.hv == n_hv) { s.hv = 0; ++s.b; }
+    }
+    // Copies still in flight land before the CTA's memory goes (bounded).
+    for (int i = it < kStages ? 0 : it - kStages; i < it; ++i)
+      if (!warp_wait(full + i % kStages, (i / kStages) & 1)) break;
+  } else {
+    const int gid = lane >> 2, c = lane & 3;
+    const uint32_t ring = smem_u32(smem);
+    const int p0 = warp * 16;
+    int it = 0;
+    bool ok = true, cut_first = false;
+    while (s.count > 0 && ok) {
+      const int len = clamped_len(p.lens, s.b, p.len_limit);
+      const int nt = tiles_of(len);
+      const int n = static_cast<int>(min(static_cast<long long>(nt - s.x), s.count));
+      const int kvh = s.hv / p.nrb, rb = s.hv - kvh * p.nrb;
+      const int head0 = kvh * p.g + rb * 16;
+      const int rows = min(16, p.g - rb * 16);
+      // Q as A fragments: rows are the KV head's query heads (others zero).
+      uint32_t qa[D / 16][4];
+      const E* qrow = static_cast<const E*>(p.q) + s.b * p.q_stride_seq + head0 * p.q_stride_head;
+#pragma unroll
+      for (int ks = 0; ks < D / 16; ++ks)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int j = gid + 8 * (r & 1), d = ks * 16 + 2 * c + 8 * (r >> 1);
+          qa[ks][r] = j < rows ? __ldg(reinterpret_cast<const uint32_t*>(qrow + j * p.q_stride_head + d)) : 0u;
+        }
+      float o[D / 8][4];
+#pragma unroll
+      for (int nb = 0; nb < D / 8; ++nb) o[nb][0] = o[nb][1] = o[nb][2] = o[nb][3] = 0.f;
+      float m_run[2] = {-INFINITY, -INFINITY}, l_run[2] = {0.f, 0.f};
+      for (int x = s.x; x < s.x + n; ++x, ++it) {
+        const int st = it % kStages;
+        if (!warp_wait(full + st, (it / kStages) & 1)) {
+          ok = false;
+          break;
+        }
+        const uint32_t kst = ring + st * 2 * L::kTileBytes, vst = kst + L::kTileBytes;
+        const int ts = x * kTile + p0;
+        if (ts < len) {
+          if (ts + 16 > len) {
+            // The last page's rows behind the sequence's end hold anything:
+            // zero this warp's part of their values (a zero weight times an
+            // infinity would not be zero).
+            for (int i = lane; i < 16 * (D / 8); i += 32) {
+              const int r = i / (D / 8), ch = i % (D / 8);
+              if (ts + r >= len)
+                *reinterpret_cast<uint4*>(smem + (vst - ring) + tile_off(p0 + r, ch)) = make_uint4(0, 0, 0, 0);
+            }
+            fence_async_shared();  // before the ring's next copy to this place
+            __syncwarp();
+          }
+          float sc[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+          for (int ks = 0; ks < D / 16; ++ks) {
+            uint32_t b[4];
+            ldsm_x4(kst + tile_off(p0 + ((lane >> 4) & 1) * 8 + (lane & 7), ks * 2 + ((lane >> 3) & 1)), b);
+            Elem<E>::mma(sc[0], qa[ks], b[0], b[1]);
+            Elem<E>::mma(sc[1], qa[ks], b[2], b[3]);
+          }
+          float pr[2][4];
+#pragma unroll
+          for (int nb = 0; nb < 2; ++nb)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int t = ts + nb * 8 + 2 * c + (e & 1);
+              sc[nb][e] = t < len ? sc[nb][e] * p.scale_log2 : -INFINITY;
+            }
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            float mx = fmaxf(fmaxf(sc[0][2 * r], sc[0][2 * r + 1]), fmaxf(sc[1][2 * r], sc[1][2 * r + 1]));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+            const float m_new = fmaxf(m_run[r], mx);
+            const float m_use = m_new == -INFINITY ? 0.f : m_new;
+            const float corr = exp2_approx(m_run[r] - m_use);
+            l_run[r] *= corr;
+#pragma unroll
+            for (int nb = 0; nb < D / 8; ++nb) {
+              o[nb][2 * r] *= corr;
+              o[nb][2 * r + 1] *= corr;
+            }
+#pragma unroll
+            for (int nb = 0; nb < 2; ++nb) {
+              pr[nb][2 * r] = exp2_approx(sc[nb][2 * r] - m_use);
+              pr[nb][2 * r + 1] = exp2_approx(sc[nb][2 * r + 1] - m_use);
+              l_run[r] += pr[nb][2 * r] + pr[nb][2 * r + 1];
+            }
+            m_run[r] = m_new;
+          }
+          uint32_t pa[4];
+          pa[0] = Elem<E>::pack(pr[0][0], pr[0][1]);
+          pa[1] = Elem<E>::pack(pr[0][2], pr[0][3]);
+          pa[2] = Elem<E>::pack(pr[1][0], pr[1][1]);
+          pa[3] = Elem<E>::pack(pr[1][2], pr[1][3]);
+#pragma unroll
+          for (int dp = 0; dp < D / 16; ++dp) {
+            uint32_t b[4];
+            ldsm_x4_trans(vst + tile_off(p0 + ((lane >> 3) & 1) * 8 + (lane & 7), dp * 2 + ((lane >> 4) & 1)), b);
+            Elem<E>::mma(o[2 * dp], pa, b[0], b[1]);
+            Elem<E>::mma(o[2 * dp + 1], pa, b[2], b[3]);
+          }
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(empty + st);
+      }
+      if (!ok) break;
+
+      // The item's (or piece's) result: the warps' parts, four heads a round.
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        l_run[r] += __shfl_xor_sync(0xffffffffu, l_run[r], 1);
+        l_run[r] += __shfl_xor_sync(0xffffffffu, l_run[r], 2);
+        if (c == 0) {
+          ms[warp * 16 + gid + 8 * r] = m_run[r];
+          ls[warp * 16 + gid + 8 * r] = l_run[r];
+        }
+      }
+      const bool whole = s.x == 0 && n == nt;
+      const int slot = 2 * blockIdx.x + (s.x > 0 ? 0 : 1);
+      if (!whole && s.x == 0) {
+        cut_first = true;
+        if (threadIdx.x == 0) {
+          const long long end = s.pos + nt;
+          const int last = static_cast<int>((end * s.ctas - 1) / s.total);
+          p.desc[blockIdx.x] = Desc{s.b, s.hv, last - static_cast<int>(blockIdx.x) + 1, 0};
+        }
+      }
+      if (late && whole) pdl_wait_prior_grid();
+      for (int r0 = 0; r0 < rows; r0 += kMergeRows) {
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const int j = gid + 8 * r - r0;
+          if (j >= 0 && j < kMergeRows)
+#pragma unroll
+            for (int nb = 0; nb < D / 8; ++nb)
+              *reinterpret_cast<float2*>(os + (warp * kMergeRows + j) * D + nb * 8 + 2 * c) =
+                  make_float2(o[nb][2 * r], o[nb][2 * r + 1]);
+        }
+        named_sync(1, 32 * kWarps);
+        for (int i = threadIdx.x; i < kMergeRows * (D / 4); i += 32 * kWarps) {
+          const int j = i / (D / 4), d4 = i % (D / 4), row = r0 + j;
+          if (row < rows) {
+            float mx = -INFINITY;
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) mx = fmaxf(mx, ms[w * 16 + row]);
+            const float mu = mx == -INFINITY ? 0.f : mx;
+            float den = 0.f;
+            float4 num = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) {
+              const float f = exp2_approx(ms[w * 16 + row] - mu);
+              const float4 v = *reinterpret_cast<const float4*>(os + (w * kMergeRows + j) * D + d4 * 4);
+              den = fmaf(ls[w * 16 + row], f, den);
+              num.x = fmaf(v.x, f, num.x);
+              num.y = fmaf(v.y, f, num.y);
+              num.z = fmaf(v.z, f, num.z);
+              num.w = fmaf(v.w, f, num.w);
+            }
+            if (whole) {
+              finish<E, D>(p, s.b, head0 + row, d4, mx, den, num);
+            } else {
+              *reinterpret_cast<float4*>(p.part + (static_cast<int64_t>(slot) * 16 + row) * D + d4 * 4) = num;
+              if (d4 == 0) {
+                p.ml[slot * 32 + row] = mx;
+                p.ml[slot * 32 + 16 + row] = den;
+              }
+            }
+          }
+        }
+        named_sync(1, 32 * kWarps);
+      }
+      s.pos += nt - s.x;
+      s.count -= n;
+      s.x = 0;
+      if (++s.hv == n_hv) { s.hv = 0; ++s.b; }
+    }
+    if (threadIdx.x == 0 && !cut_first) p.desc[blockIdx.x] = Desc{0, 0, 0, 0};
+  }
+  if (late) pdl_wait_prior_grid();
+}
+
+// Joins the pieces of the item whose first piece CTA blockIdx.x holds.
+template <typename E, int D>
+__global__ void __launch_bounds__(128)
+    paged_join_kernel(const __grid_constant__ Params p) {
+  pdl_wait_prior_grid();
+  pdl_launch_dependents();
+  const int4 raw = __ldcg(reinterpret_cast<const int4*>(p.desc + blockIdx.x));
+  const Desc d{raw.x, raw.y, raw.z, 0};
+  if (d.pieces == 0) return;
+  const int kvh = d.hv / p.nrb, rb = d.hv - kvh * p.nrb;
+  const int rows = min(16, p.g - rb * 16);
+  // Piece 0 lies in this CTA's second slot, piece i > 0 in CTA + i's first.
+  auto slot_of = [&](int i) {
+    return 2 * (static_cast<int64_t>(blockIdx.x) + i) + (i == 0 ? 1 : 0);
+  };
+  for (int t = threadIdx.x; t < rows * (D / 4); t += 128) {
+    const int row = t / (D / 4), d4 = t % (D / 4);
+    float mx = -INFINITY;
+    for (int i = 0; i < d.pieces; ++i) mx = fmaxf(mx, __ldcg(p.ml + slot_of(i) * 32 + row));
+    const float mu = mx == -INFINITY ? 0.f : mx;
+    float den = 0.f;
+    float4 num = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int i = 0; i < d.pieces; ++i) {
+      const int64_t sl = slot_of(i);
+      const float f = exp2_approx(__ldcg(p.ml + sl * 32 + row) - mu);
+      const float4 v = __ldcg(reinterpret_cast<const float4*>(p.part + (sl * 16 + row) * D + d4 * 4));
+      den = fmaf(__ldcg(p.ml + sl * 32 + 16 + row), f, den);
+      num.x = fmaf(v.x, f, num.x);
+      num.y = fmaf(v.y, f, num.y);
+      num.z = fmaf(v.z, f, num.z);
+      num.w = fmaf(v.w, f, num.w);
+    }
+    finish<E, D>(p, d.b, kvh * p.g + rb * 16 + row, d4, mx, den, num);
+  }
+}
+
+template <typename E, int D>
+cudaError_t launch(const Params& p, const CUtensorMap& kmap, const CUtensorMap& vmap, int num_sms,
+                   cudaStream_t stream) {
+  static int configured[64] = {0};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev < 0 || dev >= 64 || !configured[dev]) {
+    e = cudaFuncSetAttribute(paged_decode_kernel<E, D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             Layout<D>::kSmem);
+    if (e != cudaSuccess) return e;
+    if (dev >= 0 && dev < 64) configured[dev] = 1;
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(kCtasPerSm * num_sms);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = Layout<D>::kSmem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  e = cudaLaunchKernelEx(&cfg, paged_decode_kernel<E, D>, p, kmap, vmap);
+  if (e != cudaSuccess) return e;
+  cfg.blockDim = dim3(128);
+  cfg.dynamicSmemBytes = 0;
+  return cudaLaunchKernelEx(&cfg, paged_join_kernel<E, D>, p);
+}
+
+}  // namespace
+
+int paged_decode_box_rows(int page_size) { return page_size < kTile ? page_size : kTile; }
+
+size_t paged_decode_workspace(int D, int num_sms) {
+  const size_t ctas = static_cast<size_t>(kCtasPerSm) * num_sms;
+  return ctas * (2 * 16 * D * 4 + 2 * 2 * 16 * 4 + sizeof(Desc));
+}
+
+cudaError_t launch_paged_decode(const PagedPool& pool, const CUtensorMap& kmap,
+                                const CUtensorMap& vmap, const DecodeArgs& a, int num_sms,
+                                cudaStream_t stream) {
+  const size_t ctas = static_cast<size_t>(kCtasPerSm) * num_sms;
+  Params p;
+  p.q = a.q;
+  p.out = a.out;
+  p.table = a.table;
+  p.lens = a.lens;
+  p.part = static_cast<float*>(a.workspace);
+  p.ml = p.part + ctas * 2 * 16 * pool.D;
+  p.desc = reinterpret_cast<Desc*>(p.ml + ctas * 2 * 2 * 16);
+  p.q_stride_seq = a.q_stride_seq;
+  p.q_stride_head = a.q_stride_head;
+  p.table_stride = a.table_stride;
+  p.n_pages = pool.n_pages;
+  p.B = a.B;
+  p.hq = a.hq;
+  p.hkv = pool.n_kv_heads;
+  p.g = a.hq / pool.n_kv_heads;
+  p.nrb = (p.g + 15) / 16;
+  p.page_shift = 0;
+  while ((1 << p.page_shift) < pool.page_size) ++p.page_shift;
+  const int64_t limit = static_cast<int64_t>(a.table_width) * pool.page_size;
+  p.len_limit = limit < (1 << 30) ? static_cast<int>(limit) : 1 << 30;
+  p.box_rows = paged_decode_box_rows(pool.page_size);
+  p.scale_log2 = a.scale_log2;
+  p.prefix = a.prefix;
+  if (pool.bf16)
+    return pool.D == 128 ? launch<__nv_bfloat16, 128>(p, kmap, vmap, num_sms, stream)
+                         : launch<__nv_bfloat16, 64>(p, kmap, vmap, num_sms, stream);
+  return pool.D == 128 ? launch<__half, 128>(p, kmap, vmap, num_sms, stream)
+                       : launch<__half, 64>(p, kmap, vmap, num_sms, stream);
+}
+
+}  // namespace dqg
+
+DQG_STATUS_READER(read_status_paged_decode)

@@ -1,0 +1,258 @@
+"""Operators over a key/value cache held in pages: what takes prompts and
+batches of different lengths through the decoder's attention.
+
+A cache is two pools ``k_pages``, ``v_pages`` [pages, kv heads, page size, D]
+(fp16 or bf16; D 64 or 128; page size 16 to 256, a power of two) and, per
+sequence, a row of page numbers in ``block_table``: position t lies in page
+``block_table[b, t // page_size]`` at place ``t % page_size``. The pools may be
+strided views (of one allocation for keys and values, say) as long as both have
+the same strides and D is contiguous.
+
+CUDA tensors go through the sm_100a kernels of libdequant_b200.so on torch's
+current stream; if the library is missing these calls raise. CPU tensors take
+the same formulas in torch: that branch exists for the host-logic tests and is
+never taken for a CUDA tensor.
+
+The reference has none of this; it models the cache's bytes
+(KrishnaI2424/Dequant_Project ``dequant/byte_model.py:214-219``).
+"""
+
+from __future__ import annotations
+
+import contextlib
+import ctypes
+import functools
+import math
+
+import torch
+
+from dequant_project_b200 import _native
+
+_DTYPES = {torch.float16: 0, torch.bfloat16: 1}
+
+
+def _pools(k_pages: torch.Tensor, v_pages: torch.Tensor, *same_type) -> "_native.PagedKV":
+    """The C description of the pools, with the checks that need tensors."""
+    code = _DTYPES.get(k_pages.dtype)
+    if code is None:
+        raise RuntimeError(f"pages must be float16 or bfloat16, got {k_pages.dtype}")
+    if k_pages.dim() != 4:
+        raise RuntimeError("pages must be [pages, kv heads, page size, head dim]")
+    n, h, p, d = k_pages.shape
+    sn, sh, sp, sd = k_pages.stride()
+    if (v_pages.shape != k_pages.shape or v_pages.stride() != (sn, sh, sp, sd)
+            or v_pages.dtype != k_pages.dtype or sd != 1):
+        raise RuntimeError("k_pages and v_pages must have one shape, type and strides, with the "
+                           "head dimension contiguous")
+    device = k_pages.device
+    if v_pages.device != device:
+        raise RuntimeError("k_pages and v_pages must be on the same device")
+    for name, t in same_type:
+        if t.dtype != k_pages.dtype or t.device != device:
+            raise RuntimeError(f"{name} must be {k_pages.dtype} on {device}, as the pages are")
+    return _native.PagedKV(k_pages.data_ptr(), v_pages.data_ptr(), n, h, p, d, sn, sh, sp, code)
+
+
+def _ints(device, *named) -> None:
+    """Contiguous integer tensors of one type and device."""
+    for name, t, dtype, dims in named:
+        if t.dtype != dtype or t.dim() != dims or t.device != device or t.stride(-1) != 1:
+            raise RuntimeError(f"{name} must be a contiguous {dims}-dimensional {dtype} tensor on {device}")
+
+
+def _on(device):
+    """The device as the current one, for callers that have another current."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(device)
+
+
+def _stream(device) -> int:
+    return torch.cuda.current_stream(device).cuda_stream
+
+
+@functools.lru_cache(maxsize=None)
+def _decode_bytes(device_index: int, head_dim: int) -> int:
+    n = ctypes.c_uint64(0)
+    _native.check(_native.lib().dqg_paged_attention_workspace(head_dim, ctypes.byref(n)))
+    return int(n.value)
+
+
+def _workspace(given: torch.Tensor | None, need: int, device) -> torch.Tensor:
+    if given is None:
+        return torch.empty(need, dtype=torch.uint8, device=device)
+    if given.device != device or not given.is_contiguous():
+        raise RuntimeError(f"the workspace must be a contiguous tensor on {device}")
+    return given
+
+
+# ------------------------------------------------------------------- append
+def rope_scaled_tables(head_dim: int, theta: float, positions: int, device, *, rotary_dim: int | None = None,
+                       scaling: dict | None = None) -> tuple:
+    """cos/sin [positions, rotary_dim / 2] (fp32) for ``rope_paged_append``.
+
+    ``rotary_dim`` (default: the whole head) is the part that rotates.
+    ``scaling`` stretches the frequencies for long contexts:
+    ``{"type": "linear", "factor": f}`` divides every frequency by f;
+    ``{"type": "dynamic", "factor": f, "original": n}`` raises theta so that
+    ``positions`` fit where n did; ``{"type": "banded", "factor": f,
+    "original": n, "low": a, "high": b}`` keeps frequencies that turn more than
+    b times within the original length n, divides by f those that turn less
+    than a times, and blends linearly between. Angles are formed in 64 bits."""
+    r = head_dim if rotary_dim is None else rotary_dim
+    if r % 2 or not 2 <= r <= head_dim:
+        raise ValueError(f"rotary_dim must be even and in [2, {head_dim}], got {r}")
+    s = scaling or {"type": "none"}
+    kind = s.get("type")
+    if kind not in ("none", "linear", "dynamic", "banded"):
+        raise ValueError(f"unknown rotary scaling {kind!r}")
+    if kind != "none" and not s["factor"] >= 1.0:
+        raise ValueError(f"the scaling factor must be at least 1, got {s['factor']}")
+    if kind == "dynamic" and positions > s["original"]:
+        if r <= 2:
+            raise ValueError("dynamic scaling needs a rotary_dim above 2")
+        theta = theta * (s["factor"] * positions / s["original"] - (s["factor"] - 1.0)) ** (r / (r - 2))
+    freq = theta ** (-torch.arange(0, r, 2, dtype=torch.float64, device=device) / r)
+    if kind == "linear":
+        freq = freq / s["factor"]
+    elif kind == "banded":
+        if not s["high"] > s["low"] > 0:
+            raise ValueError("banded scaling needs 0 < low < high")
+        turns = s["original"] * freq / (2 * math.pi)
+        keep = ((turns - s["low"]) / (s["high"] - s["low"])).clamp(0.0, 1.0)
+        freq = freq * (keep + (1.0 - keep) / s["factor"])
+    angle = torch.arange(positions, dtype=torch.float64, device=device)[:, None] * freq[None, :]
+    return angle.cos().float(), angle.sin().float()
+
+
+def rope_paged_append(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, positions: torch.Tensor,
+                      slots: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, n_q_heads: int, *,
+                      interleaved: bool = False, q_norm: torch.Tensor | None = None,
+                      k_norm: torch.Tensor | None = None, eps: float = 1e-5) -> torch.Tensor:
+    """Norm (optional), rotate and store a batch of tokens: ``qkv``
+    [T, (Hq + 2 Hkv) D] -> rotated queries [T, Hq, D]; keys and values are
+    written to their pages.
+
+    ``cos``/``sin`` are fp32 [n_positions, R / 2]; token t takes row
+    ``positions[t]`` (int64) and rotates the first R values of each query and
+    key head: pairs (i, i + R/2), or (2i, 2i + 1) with ``interleaved``.
+    ``slots`` (int64 [T]) is page * page_size + place, negative for a token that
+    is not stored; no two tokens may share one. ``q_norm``/``k_norm`` [D]:
+    x * rsqrt(mean(x^2) + eps) * w per head before the rotation. fp32 math, one
+    rounding."""
+    t = qkv.shape[0]
+    hkv, page, d = k_pages.shape[1:]
+    if not qkv.is_cuda:
+        x = qkv.float().view(t, n_q_heads + 2 * hkv, d)
+        q, k, v = x[:, :n_q_heads], x[:, n_q_heads:n_q_heads + hkv], x[:, n_q_heads + hkv:]
+
+        def turn(h, w):
+            if w is not None:
+                h = h * torch.rsqrt(h.square().mean(-1, keepdim=True) + eps) * w.float()
+            n = cos.shape[1]
+            c, s = cos[positions][:, None], sin[positions][:, None]
+            a, b = ((h[..., 0:2 * n:2], h[..., 1:2 * n:2]) if interleaved
+                    else (h[..., :n], h[..., n:2 * n]))
+            lo, hi = a * c - b * s, b * c + a * s
+            part = torch.stack([lo, hi], -1).flatten(-2) if interleaved else torch.cat([lo, hi], -1)
+            return torch.cat([part, h[..., 2 * n:]], -1).to(qkv.dtype)
+
+        kept = slots >= 0
+        at = (slots[kept] // page, slice(None), slots[kept] % page)
+        k_pages[at] = turn(k, k_norm)[kept]
+        v_pages[at] = v.to(qkv.dtype)[kept]
+        return turn(q, q_norm)
+    norms = () if q_norm is None else (("q_norm", q_norm),)
+    norms += () if k_norm is None else (("k_norm", k_norm),)
+    kv = _pools(k_pages, v_pages, ("qkv", qkv), *norms)
+    device = qkv.device
+    if qkv.dim() != 2 or qkv.shape[1] != (n_q_heads + 2 * hkv) * d or qkv.stride(1) != 1:
+        raise RuntimeError(f"qkv must be [T, {(n_q_heads + 2 * hkv) * d}] with contiguous rows")
+    if (cos.dtype != torch.float32 or sin.dtype != torch.float32 or cos.dim() != 2 or sin.shape != cos.shape
+            or cos.device != device or sin.device != device
+            or not (cos.is_contiguous() and sin.is_contiguous())):
+        raise RuntimeError(f"cos and sin must be contiguous float32 [positions, R / 2] on {device}")
+    _ints(device, ("positions", positions, torch.int64, 1), ("slots", slots, torch.int64, 1))
+    if positions.shape[0] != t or slots.shape[0] != t:
+        raise RuntimeError(f"positions and slots must hold one entry for each of the {t} tokens")
+    for name, w in norms:
+        if w.shape != (d,) or w.stride(0) != 1:
+            raise RuntimeError(f"{name} must hold {d} contiguous weights")
+    q = torch.empty((t, n_q_heads, d), dtype=qkv.dtype, device=device)
+    with _on(device):
+        _native.check(_native.lib().dqg_rope_paged_append(
+            qkv.data_ptr(), t, qkv.stride(0) if t > 1 else qkv.shape[1], n_q_heads, cos.data_ptr(),
+            sin.data_ptr(), cos.shape[0], 2 * cos.shape[1], int(interleaved), positions.data_ptr(),
+            slots.data_ptr(), None if q_norm is None else q_norm.data_ptr(),
+            None if k_norm is None else k_norm.data_ptr(), eps, ctypes.byref(kv), q.data_ptr(),
+            _stream(device)))
+    return q
+
+
+# ---------------------------------------------------------------- attention
+def _rows(pages: torch.Tensor, table: torch.Tensor, n: int) -> torch.Tensor:
+    """fp32 [kv heads, n, D]: the first n positions that a table row lists."""
+    page = pages.shape[2]
+    got = pages[table[:-(-n // page)].long()].float()
+    return got.transpose(0, 1).reshape(pages.shape[1], -1, pages.shape[3])[:, :n]
+
+
+def _cpu_attention(q, k, v, ends, scale):
+    """q [rows, Hq, D] fp32 over k, v [Hkv, n, D]; row r sees the first
+    ends[r] keys (zeros where that is none)."""
+    rows, hq, d = q.shape
+    hkv, n, _ = k.shape
+    if n == 0:
+        return torch.zeros_like(q)
+    s = torch.einsum("rkgd,ktd->rkgt", q.view(rows, hkv, hq // hkv, d), k) * scale
+    seen = (torch.arange(n)[None] < ends[:, None])[:, None, None]
+    s = s.masked_fill(~seen, float("-inf"))
+    p = torch.softmax(s, -1).masked_fill(~seen, 0.0)
+    return torch.einsum("rkgt,ktd->rkgd", p, v).reshape(rows, hq, d)
+
+
+def _query(q: torch.Tensor, d: int) -> None:
+    if q.dim() != 3 or q.shape[2] != d or q.stride(2) != 1:
+        raise RuntimeError(f"q must be [rows, heads, {d}] with the head dimension contiguous")
+
+
+def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch.Tensor,
+                    kv_lens: torch.Tensor, *, scale: float | None = None,
+                    workspace: torch.Tensor | None = None) -> torch.Tensor:
+    """One query token per sequence over its cached positions.
+
+    q [B, Hq, D] (strides free, D contiguous), block_table int32
+    [B, pages per sequence], kv_lens int32 [B]. Returns [B, Hq, D]; zeros for a
+    sequence without positions. The lengths stay on the device: a captured call
+    serves other lengths. ``workspace`` (``paged_attention_workspace``) keeps the
+    call from taking scratch memory of its own; calls that share one must not
+    overlap."""
+    b, hq, d = q.shape
+    scale = 1.0 / math.sqrt(d) if scale is None else scale
+    if not q.is_cuda:
+        out = [_cpu_attention(q[i:i + 1].float(), _rows(k_pages, block_table[i], int(kv_lens[i])),
+                              _rows(v_pages, block_table[i], int(kv_lens[i])), kv_lens[i:i + 1], scale)
+               for i in range(b)]
+        return torch.cat(out).to(q.dtype) if out else torch.empty_like(q)
+    kv = _pools(k_pages, v_pages, ("q", q))
+    device = q.device
+    _query(q, kv.head_dim)
+    _ints(device, ("block_table", block_table, torch.int32, 2), ("kv_lens", kv_lens, torch.int32, 1))
+    if block_table.shape[0] != b or kv_lens.shape[0] != b:
+        raise RuntimeError(f"block_table and kv_lens must hold one row for each of the {b} sequences")
+    out = torch.empty((b, hq, d), dtype=q.dtype, device=device)
+    with _on(device):
+        ws = _workspace(workspace, _decode_bytes(device.index, d), device)
+        _native.check(_native.lib().dqg_paged_attention(
+            q.data_ptr(), q.stride(0), q.stride(1), b, hq, ctypes.byref(kv), block_table.data_ptr(),
+            block_table.shape[1], block_table.stride(0) if b > 1 else block_table.shape[1],
+            kv_lens.data_ptr(), scale, out.data_ptr(), ws.data_ptr(), ws.numel() * ws.element_size(),
+            _stream(device)))
+    return out
+
+
+def paged_attention_workspace(head_dim: int, device) -> torch.Tensor:
+    """Scratch memory for ``paged_attention`` calls of any batch and lengths."""
+    device = torch.device(device)
+    with _on(device):
+        return torch.empty(_decode_bytes(device.index, head_dim), dtype=torch.uint8, device=device)

@@ -85,7 +85,8 @@ int dqg_dequantize(const int32_t *qweight, const void *scales, const void *zeros
 
 /*
  * Device-side status of `device` (bit 0: a kernel of this library gave up a
- * bounded wait), the OR of the status words of all its kernels. Synchronous;
+ * bounded wait; bit 1: a paged operator left out an index out of range), the
+ * OR of the status words of all its kernels. Synchronous;
  * for tests and diagnostics, not for the hot path.
  * If reset != 0 the word is cleared after reading. No reference counterpart:
  * the reference kernels have no waits.
@@ -335,6 +336,64 @@ int dqg_gemv_swiglu_supported(int64_t M, int64_t N, int64_t K, int64_t bits, int
  */
 int dqg_silu_mul(const void *gate_up, void *out, int64_t M, int64_t I,
                  const dqg_l2_spans *prefetch, void *stream);
+
+/*
+ * Paged key/value cache (no reference counterpart: the reference only models
+ * the cache's bytes, dequant/byte_model.py:214-219). Keys and values lie in
+ * two pools of [n_pages, n_kv_heads, page_size, head_dim] 16-bit values; a
+ * sequence's positions are spread over the pages that its row of a block
+ * table lists (position t in page table[t / page_size], place t % page_size).
+ * Strides are in elements, the same for both pools, multiples of 8, with
+ * head_dim contiguous; head_dim is 64 or 128, page_size 16, 32, 64, 128 or
+ * 256. The operators below take queries, keys, values and outputs of the
+ * pools' type. A page index, slot, position or length out of range is left
+ * out (read as zeros, not written, held to the table's width) and sets bit 1
+ * of dqg_device_status.
+ */
+enum { DQG_FP16 = 0, DQG_BF16 = 1 };
+typedef struct dqg_paged_kv {
+  void *k;
+  void *v;
+  int64_t n_pages, n_kv_heads, page_size, head_dim;
+  int64_t page_stride, head_stride, row_stride;
+  int32_t dtype;
+} dqg_paged_kv;
+
+/*
+ * Rotation and storing of T tokens. qkv is [T, (Hq + 2 Hkv) * D] (query, key,
+ * value heads; rows qkv_stride elements apart). With q_norm and k_norm (D
+ * weights each, or both NULL) every query and key head is first normed,
+ * x * rsqrt(mean(x^2) + eps) * w; then its first rotary_dim values R are
+ * rotated by token t's row of the fp32 tables [n_positions, R / 2],
+ * row positions[t]: pairs (i, i + R/2), or (2i, 2i + 1) when interleaved.
+ * fp32 math, one rounding. Queries go to q_out [T, Hq, D]; keys and values to
+ * slot slots[t] = page * page_size + place (negative: not stored). Two tokens
+ * of one call must not share a slot.
+ */
+int dqg_rope_paged_append(const void *qkv, int64_t T, int64_t qkv_stride, int64_t n_q_heads,
+                          const float *cos_table, const float *sin_table, int64_t n_positions,
+                          int64_t rotary_dim, int interleaved, const int64_t *positions,
+                          const int64_t *slots, const void *q_norm, const void *k_norm, float eps,
+                          const dqg_paged_kv *kv, void *q_out, void *stream);
+
+/*
+ * Decode attention over the pages: out[b, h] = softmax(scale * q[b, h] .
+ * K^T) V over the kv_lens[b] positions of sequence b, zeros where there is
+ * none; q [n_seqs, Hq, D] with strides in elements (multiples of 8), out
+ * contiguous, up to 128 query heads per KV head, grouped consecutively.
+ * block_table is [n_seqs, table_width], rows table_stride apart; entries
+ * behind a sequence's last page are not read, and what lies in its last page
+ * behind its last position does not matter. The lengths are read on the
+ * device, so a captured launch serves other lengths. workspace: at least
+ * dqg_paged_attention_workspace(D) bytes, 16-byte aligned, of any contents;
+ * calls that share one must not overlap on the GPU. Results do not depend on
+ * anything but the inputs (no atomics).
+ */
+int dqg_paged_attention_workspace(int64_t head_dim, uint64_t *bytes);
+int dqg_paged_attention(const void *q, int64_t q_stride_seq, int64_t q_stride_head, int64_t n_seqs,
+                        int64_t n_q_heads, const dqg_paged_kv *kv, const int32_t *block_table,
+                        int64_t table_width, int64_t table_stride, const int32_t *kv_lens, float scale,
+                        void *out, void *workspace, uint64_t workspace_bytes, void *stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,217 @@
+"""Paged-cache operators on the GPU against plain 64-bit restatements.
+
+Tolerances follow from the kernels' arithmetic. Outputs are rounded once to
+16 bits (unit roundoff u = 2^-11 fp16, 2^-8 bf16). Attention also rounds each
+softmax weight to 16 bits before the product with the values, while the weights'
+sum is taken before rounding: that is at most u * sum_j p_j |v_j| <= u * max|v|
+per output. Exponentials and fp32 sums add below 2^-13 of that scale. So
+|out - ref| <= u |ref| + (u + 2^-13) max|v|.
+"""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+from dequant_project_b200 import _native, paged_ops
+
+pytestmark = pytest.mark.gpu
+
+U = {torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}
+TYPES = [torch.float16, torch.bfloat16]
+
+
+def make_cache(gen, lens, hkv, d, page, dtype, device, width=None, extra=2, fill=None):
+    """Pools and table of scattered pages; whatever no position uses is
+    ``fill`` (random numbers by default)."""
+    counts = [-(-n // page) for n in lens]
+    n_pages = sum(counts) + extra
+    order = torch.randperm(n_pages, generator=gen, device=device).int()
+    table = torch.full((len(lens), max([1, *counts]) if width is None else width), -1, dtype=torch.int32,
+                       device=device)
+    at = 0
+    for i, c in enumerate(counts):
+        table[i, :c] = order[at:at + c]
+        at += c
+    k = torch.randn((n_pages, hkv, page, d), generator=gen, device=device).to(dtype)
+    v = torch.randn((n_pages, hkv, page, d), generator=gen, device=device).to(dtype)
+    if fill is not None:
+        used = torch.zeros((n_pages, page), dtype=torch.bool, device=device)
+        for i, n in enumerate(lens):
+            t = torch.arange(n, device=device)
+            used[table[i].long()[t // page], t % page] = True
+        mask = ~used[:, None, :, None]
+        k.masked_fill_(mask, fill)
+        v.masked_fill_(mask, fill)
+    return k, v, table
+
+
+def rows64(pages, table_row, n):
+    page = pages.shape[2]
+    t = torch.arange(n, device=pages.device)
+    return pages[table_row.long()[t // page], :, t % page].double()  # [n, hkv, d]
+
+
+def attend64(q, k, v, ends, scale):
+    """q [rows, hq, d] over k, v [n, hkv, d] in 64 bits, row by row's end."""
+    rows, hq, d = q.shape
+    n, hkv, _ = k.shape
+    g = hq // hkv
+    out = torch.zeros((rows, hq, d), dtype=torch.float64, device=q.device)
+    if n == 0:
+        return out
+    s = torch.einsum("rkgd,tkd->rkgt", q.double().view(rows, hkv, g, d), k) * scale
+    hidden = torch.arange(n, device=q.device)[None] >= ends[:, None]
+    s = s.masked_fill(hidden[:, None, None], float("-inf"))
+    p = torch.exp(s - s.amax(-1, keepdim=True).clamp(min=-1e300))
+    p = p / p.sum(-1, keepdim=True).clamp(min=1e-300)
+    return torch.einsum("rkgt,tkd->rkgd", p, v).reshape(rows, hq, d)
+
+
+def check_attention(out, ref, v_max, dtype):
+    u = U[dtype]
+    err = (out.double() - ref).abs()
+    lim = u * ref.abs() + (u + 2.0 ** -13) * v_max + 1e-7
+    assert bool((err <= lim).all()), f"max excess {float((err - lim).max()):.3e}, max error {float(err.max()):.3e}"
+
+
+# ------------------------------------------------------------------- append
+def append64(qkv, cos, sin, positions, hq, hkv, d, interleaved, qn, kn, eps):
+    t = qkv.shape[0]
+    x = qkv.double().view(t, hq + 2 * hkv, d)
+    h = x[:, :hq + hkv].clone()
+    if qn is not None:
+        w = torch.cat([qn.double().expand(hq, d), kn.double().expand(hkv, d)])
+        h = h / torch.sqrt((h ** 2).mean(-1, keepdim=True) + eps) * w
+    n = cos.shape[1]
+    i = torch.arange(n, device=qkv.device)
+    a, b = (2 * i, 2 * i + 1) if interleaved else (i, i + n)
+    c, s = cos.double()[positions][:, None], sin.double()[positions][:, None]
+    o = h.clone()
+    o[..., a] = h[..., a] * c - h[..., b] * s
+    o[..., b] = h[..., b] * c + h[..., a] * s
+    return o[:, :hq], o[:, hq:], x[:, hq + hkv:]
+
+
+APPEND = [
+    # tokens, hq, hkv, d, rotary dim, interleaved, norm, page, every n-th skipped
+    (1, 32, 32, 128, 128, False, False, 16, 0),
+    (5, 64, 8, 128, 128, False, True, 64, 0),
+    (33, 6, 2, 64, 64, True, False, 16, 3),
+    (17, 28, 4, 128, 32, False, True, 32, 4),
+    (9, 3, 1, 64, 24, False, True, 16, 0),    # partners cross lanes unevenly
+    (9, 3, 1, 128, 6, False, False, 256, 2),
+    (7, 4, 4, 64, 2, True, True, 128, 0),
+    (700, 32, 8, 128, 64, True, True, 16, 7),  # several heads a lane group
+    (700, 33, 11, 64, 20, False, False, 16, 0),
+]
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("case", APPEND, ids=str)
+def test_append(cuda_device, case, dtype):
+    t, hq, hkv, d, rot, inter, norm, page, skip = case
+    gen = torch.Generator(device=cuda_device).manual_seed(t + hq)
+    k, v, table = make_cache(gen, [t], hkv, d, page, dtype, cuda_device)
+    k0, v0 = k.clone(), v.clone()
+    at = torch.arange(t, device=cuda_device)
+    slots = table[0].long()[at // page] * page + at % page
+    if skip:
+        slots[::skip] = -1
+    positions = torch.randint(0, 4096, (t,), generator=gen, device=cuda_device)
+    cos, sin = paged_ops.rope_scaled_tables(d, 10000.0, 4096, cuda_device, rotary_dim=rot)
+    wide = torch.randn((t, (hq + 2 * hkv) * d + 8), generator=gen, device=cuda_device).to(dtype)
+    qkv = wide[:, :-8]  # rows further apart than they are long
+    qn = kn = None
+    if norm:
+        qn, kn = (1 + 0.1 * torch.randn((2, d), generator=gen, device=cuda_device)).to(dtype)
+    q = paged_ops.rope_paged_append(qkv, cos, sin, positions, slots, k, v, hq, interleaved=inter, q_norm=qn,
+                                    k_norm=kn, eps=1e-5)
+    rq, rk, rv = append64(qkv, cos, sin, positions, hq, hkv, d, inter, qn, kn, 1e-5)
+    # One rounding of a value formed in fp32 from at most six operations on
+    # normed values of size up to |y|: u |ref| + 2^-20 max|y|.
+    u = U[dtype]
+    scale = max(float(rq.abs().max()), float(rk.abs().max()))
+    for got, ref in ((q, rq),):
+        assert bool(((got.double() - ref).abs() <= u * ref.abs() + 2.0 ** -20 * scale).all())
+    kept = slots >= 0
+    ek, ev = k0.double(), v0.double()
+    sl = slots[kept]
+    ek[sl // page, :, sl % page] = rk[kept]
+    ev[sl // page, :, sl % page] = rv[kept]
+    assert bool(((k.double() - ek).abs() <= u * ek.abs() + 2.0 ** -20 * scale).all())
+    assert torch.equal(v.double(), ev)
+    written = torch.zeros((k.shape[0], page), dtype=torch.bool, device=cuda_device)
+    written[sl // page, sl % page] = True
+    untouched = ~written[:, None, :, None].expand_as(k)
+    assert torch.equal(k[untouched], k0[untouched])
+    assert _native.device_status(cuda_device.index) == 0
+
+
+def test_append_leaves_out_what_is_out_of_range(cuda_device):
+    gen = torch.Generator(device=cuda_device).manual_seed(3)
+    k, v, _ = make_cache(gen, [16], 2, 64, 16, torch.float16, cuda_device, extra=1)
+    k0, v0 = k.clone(), v.clone()
+    cos, sin = paged_ops.rope_scaled_tables(64, 1e4, 8, cuda_device)
+    qkv = torch.randn((3, 8 * 64), generator=gen, device=cuda_device).half()
+    slots = torch.tensor([32, 1 << 40, -5], device=cuda_device)  # the pool has 32 slots
+    positions = torch.tensor([0, 9, -1], device=cuda_device)
+    q = paged_ops.rope_paged_append(qkv, cos, sin, positions, slots, k, v, 4)
+    assert torch.isfinite(q.float()).all()
+    assert torch.equal(k, k0) and torch.equal(v, v0)
+    assert _native.device_status(cuda_device.index, reset=True) == 2
+    assert _native.device_status(cuda_device.index) == 0
+
+
+def test_append_on_one_buffer_of_keys_and_values(cuda_device):
+    """Pools that are views of one [pages, 2, heads, page, D] allocation."""
+    gen = torch.Generator(device=cuda_device).manual_seed(4)
+    both = torch.randn((4, 2, 2, 16, 128), generator=gen, device=cuda_device).half()
+    flat = both.clone()
+    k, v = both[:, 0], both[:, 1]
+    cos, sin = paged_ops.rope_scaled_tables(128, 1e4, 64, cuda_device)
+    qkv = torch.randn((20, 8 * 128), generator=gen, device=cuda_device).half()
+    pos = torch.arange(20, device=cuda_device)
+    slots = pos + 16
+    paged_ops.rope_paged_append(qkv, cos, sin, pos, slots, k, v, 4)
+    kc, vc = flat[:, 0].contiguous(), flat[:, 1].contiguous()
+    paged_ops.rope_paged_append(qkv, cos, sin, pos, slots, kc, vc, 4)
+    assert torch.equal(k, kc) and torch.equal(v, vc)
+
+
+# ------------------------------------------------------------------- decode
+DECODE = [
+    # lengths, hq, hkv, d, page
+    ([2049], 32, 32, 128, 16),
+    ([1], 32, 32, 128, 16),
+    ([0, 1, 63, 64, 65, 0, 127, 129], 64, 8, 128, 16),
+    ([300, 17, 0, 5000, 1, 64], 8, 1, 128, 64),
+    ([33, 1000, 257, 256, 255], 28, 4, 128, 128),
+    ([700, 2, 511], 16, 16, 64, 256),
+    ([129, 31, 90], 6, 2, 64, 32),
+    ([100, 2000], 40, 1, 64, 16),      # three row blocks of query heads
+    ([75, 0], 128, 1, 128, 16),
+    ([0, 0, 0], 4, 2, 128, 16),
+    ([40] * 300, 2, 1, 64, 16),        # more sequences than CTAs
+]
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("lens,hq,hkv,d,page", DECODE, ids=lambda v: str(v)[:40])
+def test_decode(cuda_device, lens, hq, hkv, d, page, dtype):
+    gen = torch.Generator(device=cuda_device).manual_seed(len(lens) + hq)
+    k, v, table = make_cache(gen, lens, hkv, d, page, dtype, cuda_device, fill=float("nan"))
+    q = torch.randn((len(lens), hq, d), generator=gen, device=cuda_device).to(dtype)
+    kv_lens = torch.tensor(lens, dtype=torch.int32, device=cuda_device)
+    out = paged_ops.paged_attention(q, k, v, table, kv_lens)
+    scale = 1 / math.sqrt(d)
+    v_max = float(torch.nan_to_num(v.float()).abs().max())
+    ref = torch.cat([attend64(q[i:i + 1], rows64(k, table[i], n), rows64(v, table[i], n),
+                              kv_lens[i:i + 1], scale) for i, n in enumerate(lens)])
+    check_attention(out, ref, v_max, dtype)
+    ws = paged_ops.paged_attention_workspace(d, cuda_device).fill_(255)
+    for _ in range(3):
+        assert torch.equal(paged_ops.paged_attention(q, k, v, table, kv_lens, workspace=ws), out)
+    assert _native.device_status(cuda_device.index) == 0
