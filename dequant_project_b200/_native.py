@@ -119,6 +119,16 @@ def lib() -> ctypes.CDLL:
     h.dqg_paged_attention.restype = i32
     h.dqg_paged_attention.argtypes = [vp, i64, i64, i64, i64, kv, vp, i64, i64, vp, f32, vp, vp,
                                       u64, vp]
+    h.dqg_prompt_attention_workspace.restype = i32
+    h.dqg_prompt_attention_workspace.argtypes = [i64, u64p]
+    h.dqg_prompt_attention.restype = i32
+    h.dqg_prompt_attention.argtypes = [vp, i64, i64, i64, i64, kv, vp, i64, i64, vp, vp, i64, i32,
+                                       f32, vp, vp, u64, vp]
+    h.dqg_shared_prefix_workspace.restype = i32
+    h.dqg_shared_prefix_workspace.argtypes = [i64, i64, i64, i64, i64, u64p]
+    h.dqg_shared_prefix_attention.restype = i32
+    h.dqg_shared_prefix_attention.argtypes = [vp, i64, i64, i64, i64, kv, vp, i64, i64, vp, i64,
+                                              i64, vp, f32, vp, vp, u64, vp]
     _lib = h
     return _lib
 
@@ -132,7 +142,8 @@ EXPORTED = ("dqg_last_error", "dqg_version", "dqg_add_one", "dqg_gemv", "dqg_deq
             "dqg_ipc_export", "dqg_ipc_open", "dqg_ipc_close", "dqg_peer_allreduce",
             "dqg_peer_allreduce_add_rms_norm", "dqg_gemv_swiglu",
             "dqg_gemv_swiglu_supported", "dqg_rope_paged_append", "dqg_paged_attention_workspace",
-            "dqg_paged_attention")
+            "dqg_paged_attention", "dqg_prompt_attention_workspace", "dqg_prompt_attention",
+            "dqg_shared_prefix_workspace", "dqg_shared_prefix_attention")
 
 
 def check(rc: int) -> None:

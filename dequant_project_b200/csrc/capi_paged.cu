@@ -161,6 +161,17 @@ int pool_maps(const dqg::PagedPool& pool, int rows, CUtensorMap* k, CUtensorMap*
   return make_map(v, pool.v, pool.bf16, size, stride, rows, 1, 1, "v_pages");
 }
 
+// Queries [T, kv heads, g, D]: boxes of a tile's tokens, times the KV head's
+// query heads, times 64 values.
+int query_map(const void* q, const dqg::PagedPool& pool, int64_t T, int64_t hq, int64_t stride_row,
+              int64_t stride_head, CUtensorMap* map) {
+  const int64_t g = hq / pool.n_kv_heads;
+  const int64_t size[4] = {pool.D, g, pool.n_kv_heads, T};
+  const int64_t stride[3] = {stride_head, g * stride_head, stride_row};
+  return make_map(map, q, pool.bf16, size, stride, static_cast<int>(g), 1,
+                  dqg::prompt_tokens_per_tile(static_cast<int>(hq), pool.n_kv_heads), "q");
+}
+
 constexpr double kLog2e = 1.4426950408889634;
 
 int current(int* dev, int* sms) {
@@ -274,6 +285,154 @@ int dqg_paged_attention(const void* q, int64_t q_stride_seq, int64_t q_stride_he
   a.scale_log2 = static_cast<float>(scale * kLog2e);
   const cudaError_t e = dqg::launch_paged_decode(pool, kmap, vmap, a, sms, static_cast<cudaStream_t>(stream));
   if (e != cudaSuccess) return api_cuda_fail(e, "paged_attention launch");
+  return api_ok();
+}
+
+int dqg_prompt_attention_workspace(int64_t head_dim, uint64_t* bytes) {
+  if (bytes == nullptr) return api_fail(DQG_ERR_INVALID, "bytes must not be null");
+  if (head_dim != 64 && head_dim != 128)
+    return api_fail(DQG_ERR_UNSUPPORTED, "paged operators handle head_dim 64 and 128, got %lld", (ll)head_dim);
+  int dev = 0, sms = 0;
+  const int rc = current(&dev, &sms);
+  if (rc) return rc;
+  *bytes = dqg::prompt_workspace(static_cast<int>(head_dim), sms);
+  return api_ok();
+}
+
+int dqg_prompt_attention(const void* q, int64_t q_stride_row, int64_t q_stride_head, int64_t T,
+                         int64_t n_q_heads, const dqg_paged_kv* kv, const int32_t* block_table,
+                         int64_t table_width, int64_t table_stride, const int32_t* q_starts,
+                         const int32_t* kv_lens, int64_t n_seqs, int causal, float scale, void* out,
+                         void* workspace, uint64_t workspace_bytes, void* stream) {
+  dqg::PagedPool pool;
+  int rc = check_pool(kv, &pool);
+  if (rc) return rc;
+  if ((rc = check_heads(n_q_heads, pool)) != DQG_OK) return rc;
+  if (T < 0 || T > (1 << 28)) return api_fail(DQG_ERR_INVALID, "T=%lld out of range", (ll)T);
+  if (n_seqs < 0 || n_seqs > (1 << 24))
+    return api_fail(DQG_ERR_INVALID, "n_seqs=%lld out of range", (ll)n_seqs);
+  if (T == 0 || n_seqs == 0) return api_ok();
+  if ((rc = check_query(q, T, n_q_heads, q_stride_row, q_stride_head, pool.D)) != DQG_OK) return rc;
+  if ((rc = check_table(block_table, table_width, table_stride, "block_table")) != DQG_OK) return rc;
+  if ((rc = check_ptr(q_starts, 4, "q_starts")) != DQG_OK) return rc;
+  if ((rc = check_ptr(kv_lens, 4, "kv_lens")) != DQG_OK) return rc;
+  if ((rc = check_ptr(out, 16, "out")) != DQG_OK) return rc;
+  if ((rc = check_scale(scale)) != DQG_OK) return rc;
+  int dev = 0, sms = 0;
+  if ((rc = current(&dev, &sms)) != DQG_OK) return rc;
+  if ((rc = check_workspace(workspace, workspace_bytes, dqg::prompt_workspace(pool.D, sms))) != DQG_OK)
+    return rc;
+  CUtensorMap qmap, kmap, vmap;
+  if ((rc = query_map(q, pool, T, n_q_heads, q_stride_row, q_stride_head, &qmap)) != DQG_OK) return rc;
+  if ((rc = pool_maps(pool, dqg::prompt_box_rows(pool.page_size), &kmap, &vmap)) != DQG_OK) return rc;
+  dqg::PromptArgs a;
+  std::memset(&a, 0, sizeof(a));
+  a.table = block_table;
+  a.table_stride = table_stride;
+  a.table_width = static_cast<int>(table_width);
+  a.q_starts = q_starts;
+  a.kv_lens = kv_lens;
+  a.out = out;
+  a.workspace = workspace;
+  a.B = static_cast<int>(n_seqs);
+  a.T = static_cast<int>(T);
+  a.hq = static_cast<int>(n_q_heads);
+  a.causal = causal != 0;
+  a.scale_log2 = static_cast<float>(scale * kLog2e);
+  const cudaError_t e = dqg::launch_prompt(pool, qmap, kmap, vmap, a, sms, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return api_cuda_fail(e, "prompt_attention launch");
+  return api_ok();
+}
+
+int dqg_shared_prefix_workspace(int64_t n_seqs, int64_t n_q_heads, int64_t n_kv_heads, int64_t head_dim,
+                                int64_t prefix_len, uint64_t* bytes) {
+  if (bytes == nullptr) return api_fail(DQG_ERR_INVALID, "bytes must not be null");
+  if (head_dim != 64 && head_dim != 128)
+    return api_fail(DQG_ERR_UNSUPPORTED, "paged operators handle head_dim 64 and 128, got %lld", (ll)head_dim);
+  if (n_kv_heads < 1 || n_kv_heads > 1024)
+    return api_fail(DQG_ERR_INVALID, "n_kv_heads must be in [1, 1024], got %lld", (ll)n_kv_heads);
+  dqg::PagedPool pool = {};
+  pool.n_kv_heads = static_cast<int>(n_kv_heads);
+  int rc = check_heads(n_q_heads, pool);
+  if (rc) return rc;
+  if (n_seqs < 0 || n_seqs > (1 << 20))
+    return api_fail(DQG_ERR_INVALID, "n_seqs=%lld out of range", (ll)n_seqs);
+  if (prefix_len < 0 || prefix_len > (1 << 30))
+    return api_fail(DQG_ERR_INVALID, "prefix_len=%lld out of range", (ll)prefix_len);
+  int dev = 0, sms = 0;
+  if ((rc = current(&dev, &sms)) != DQG_OK) return rc;
+  *bytes = dqg::paged_decode_workspace(static_cast<int>(head_dim), sms);
+  if (prefix_len > 0 && n_seqs > 0)
+    *bytes += dqg::prefix_workspace(static_cast<int>(n_seqs), static_cast<int>(n_q_heads),
+                                    static_cast<int>(n_kv_heads), static_cast<int>(head_dim),
+                                    static_cast<int>(prefix_len), sms);
+  return api_ok();
+}
+
+int dqg_shared_prefix_attention(const void* q, int64_t q_stride_seq, int64_t q_stride_head, int64_t n_seqs,
+                                int64_t n_q_heads, const dqg_paged_kv* kv, const int32_t* prefix_table,
+                                int64_t prefix_pages, int64_t prefix_len, const int32_t* block_table,
+                                int64_t table_width, int64_t table_stride, const int32_t* kv_lens,
+                                float scale, void* out, void* workspace, uint64_t workspace_bytes,
+                                void* stream) {
+  dqg::PagedPool pool;
+  int rc = check_pool(kv, &pool);
+  if (rc) return rc;
+  uint64_t need = 0;
+  rc = dqg_shared_prefix_workspace(n_seqs, n_q_heads, pool.n_kv_heads, pool.D, prefix_len, &need);
+  if (rc) return rc;
+  if (n_seqs == 0) return api_ok();
+  if ((rc = check_query(q, n_seqs, n_q_heads, q_stride_seq, q_stride_head, pool.D)) != DQG_OK) return rc;
+  if ((rc = check_table(block_table, table_width, table_stride, "block_table")) != DQG_OK) return rc;
+  if (prefix_len > 0) {
+    if ((rc = check_table(prefix_table, prefix_pages, prefix_pages, "prefix_table")) != DQG_OK) return rc;
+    if (prefix_pages * pool.page_size < prefix_len)
+      return api_fail(DQG_ERR_INVALID, "prefix_len=%lld positions exceed the prefix's %lld pages of %d",
+                      (ll)prefix_len, (ll)prefix_pages, pool.page_size);
+  }
+  if ((rc = check_ptr(kv_lens, 4, "kv_lens")) != DQG_OK) return rc;
+  if ((rc = check_ptr(out, 16, "out")) != DQG_OK) return rc;
+  if ((rc = check_scale(scale)) != DQG_OK) return rc;
+  if ((rc = check_workspace(workspace, workspace_bytes, need)) != DQG_OK) return rc;
+  int dev = 0, sms = 0;
+  if ((rc = current(&dev, &sms)) != DQG_OK) return rc;
+  dqg::DecodeArgs d;
+  std::memset(&d, 0, sizeof(d));
+  d.workspace = workspace;
+  CUtensorMap qmap, kmap, vmap;
+  if (prefix_len > 0) {
+    dqg::PromptArgs a;
+    std::memset(&a, 0, sizeof(a));
+    a.table = prefix_table;
+    a.table_stride = prefix_pages;
+    a.table_width = static_cast<int>(prefix_pages);
+    // The decode kernel's scratch has a fixed size: the pieces go behind it.
+    a.workspace = static_cast<uint8_t*>(workspace) + dqg::paged_decode_workspace(pool.D, sms);
+    a.B = 1;
+    a.T = static_cast<int>(n_seqs);
+    a.hq = static_cast<int>(n_q_heads);
+    a.scale_log2 = static_cast<float>(scale * kLog2e);
+    a.prefix_len = static_cast<int>(prefix_len);
+    if ((rc = query_map(q, pool, n_seqs, n_q_heads, q_stride_seq, q_stride_head, &qmap)) != DQG_OK) return rc;
+    if ((rc = pool_maps(pool, dqg::prompt_box_rows(pool.page_size), &kmap, &vmap)) != DQG_OK) return rc;
+    const cudaError_t e = dqg::launch_prompt(pool, qmap, kmap, vmap, a, sms, static_cast<cudaStream_t>(stream));
+    if (e != cudaSuccess) return api_cuda_fail(e, "shared_prefix_attention launch");
+    d.prefix = dqg::prefix_pieces(a, pool, sms);
+  }
+  if ((rc = pool_maps(pool, dqg::paged_decode_box_rows(pool.page_size), &kmap, &vmap)) != DQG_OK) return rc;
+  d.q = q;
+  d.q_stride_seq = q_stride_seq;
+  d.q_stride_head = q_stride_head;
+  d.table = block_table;
+  d.table_stride = table_stride;
+  d.table_width = static_cast<int>(table_width);
+  d.lens = kv_lens;
+  d.out = out;
+  d.B = static_cast<int>(n_seqs);
+  d.hq = static_cast<int>(n_q_heads);
+  d.scale_log2 = static_cast<float>(scale * kLog2e);
+  const cudaError_t e = dqg::launch_paged_decode(pool, kmap, vmap, d, sms, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return api_cuda_fail(e, "shared_prefix_attention launch");
   return api_ok();
 }
 

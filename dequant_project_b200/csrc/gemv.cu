@@ -639,7 +639,8 @@ cudaError_t read_device_status(int device, uint32_t* status, bool reset) {
                                                 read_status_stream_b4, read_status_stream_b8,
                                                 read_status_peer,        read_status_direct_b2,
                                                 read_status_direct_b4,   read_status_direct_b8,
-                                                read_status_append,      read_status_paged_decode};
+                                                read_status_append,      read_status_paged_decode,
+                                                read_status_prompt};
   *status = 0;
   for (auto rd : readers) {
     uint32_t v = 0;

@@ -507,7 +507,7 @@ int paged_decode_box_rows(int page_size) { return page_size < kTile ? page_size 
 
 size_t paged_decode_workspace(int D, int num_sms) {
   const size_t ctas = static_cast<size_t>(kCtasPerSm) * num_sms;
-  return ctas * (2 * 16 * D * 4 + 2 * 2 * 16 * 4 + sizeof(Desc));
+  return (ctas * (2 * 16 * D * 4 + 2 * 2 * 16 * 4 + sizeof(Desc)) + 255) / 256 * 256;
 }
 
 cudaError_t launch_paged_decode(const PagedPool& pool, const CUtensorMap& kmap,

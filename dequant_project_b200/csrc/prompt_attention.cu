@@ -1,0 +1,867 @@
+// Attention of whole prompts (or chunks of them) over a paged cache, and of a
+// batch's queries over a prefix that all of its sequences share. No reference
+// counterpart (the reference models the cache's bytes,
+// dequant/byte_model.py:214-219).
+//
+//   o[t, h] = sum_j p_j v_j / sum_j p_j,   p_j = exp(scale q[t, h] . k_j - m)
+//
+// over the keys that token t sees: of sequence b with q_len new tokens at the
+// end of kv_len cached ones, token i sees keys j < kv_len - q_len + i + 1
+// (all kv_len when not causal); zero where it sees none.
+//
+// Rows are packed: with g query heads per KV head a 128-row tile holds
+// floor(128 / g) tokens times g heads, so that every row of the products uses
+// the same keys, whatever g is. An item is a pair of such tiles (256 rows) of
+// one sequence and KV head; its work is counted in blocks of 128 keys, and all
+// blocks of the call are cut into equal shares, one per SM, whatever the
+// lengths and masks are. An item that lies in one share is finished by its
+// CTA; one that is cut leaves its pieces (max, sum, O) in the workspace, and a
+// second kernel joins them in order (no atomics, the same bits every time).
+//
+// One CTA per SM: one warp copies queries and page rows (tensor-map
+// boxes, 128-byte swizzle, a ring of key and value blocks), one thread issues
+// the products on the tensor cores (tcgen05: S = Q K^T from shared memory,
+// O += P V with P in tensor memory), and each tile has four softmax warps, one
+// thread a row. Tensor memory holds both tiles' S (fp32, 128 columns; P takes
+// the place of S as it is formed) and O (fp32, D columns), so one tile's
+// softmax runs while the other's products do. O stays in tensor memory over
+// all blocks: the maximum that weights refer to is moved, and O rescaled, only
+// when it grows by more than 2^8, which bounds the weights by 2^8; the sums are
+// fp32 and the division by them comes at the end.
+#include <cstdint>
+
+#include "paged.cuh"
+
+namespace dqg {
+namespace {
+
+constexpr int kBlock = 128;         // keys a block; rows a tile
+constexpr int kThreads = 384;       // 2 x 4 softmax warps; products, copies, two idle
+constexpr int kMmaWarp = 8, kCopyWarp = 9;
+constexpr float kMaxGrowth = 8.f;   // log2 of the largest weight
+
+struct Desc {  // a cut item, by the CTA that holds its first piece
+  int tok0, ntok, kvh, pieces;
+};
+
+struct Params {
+  const int32_t* table;
+  const int32_t* q_starts;
+  const int32_t* lens;
+  void* out;
+  float4* part;   // [slot][D / 4][256]
+  float* ml;      // [slot][2][256]
+  Desc* desc;     // [CTA]
+  int64_t table_stride, n_pages;
+  int B, T, hq, hkv, g, tq, page_shift, len_limit, box_rows;
+  bool causal;
+  float scale_log2;
+  int prefix_len, splits, n_pieces;   // a shared prefix: splits > 0
+};
+
+// ------------------------------------------------------------ tensor cores
+__device__ __forceinline__ uint64_t smem_desc(uint32_t addr, uint32_t lead_bytes, uint32_t stride_bytes) {
+  // 128-byte swizzle; `stride` between groups of eight 128-byte rows, `lead`
+  // between 64-value blocks of an operand whose contiguous dimension is not
+  // the summed one.
+  return static_cast<uint64_t>((addr & 0x3ffff) >> 4) | static_cast<uint64_t>(lead_bytes >> 4) << 16 |
+         static_cast<uint64_t>(stride_bytes >> 4) << 32 | uint64_t(1) << 46 | uint64_t(2) << 61;
+}
+// fp32 accumulation of 16-bit operands; m = 128. b_rows: B's contiguous
+// dimension is n (the values), not the summed one.
+__device__ __forceinline__ constexpr uint32_t instr_desc(uint32_t format, uint32_t n, bool b_rows) {
+  return 1u << 4 | format << 7 | format << 10 | (b_rows ? 1u : 0u) << 16 | (n >> 3) << 17 | (128u >> 4) << 24;
+}
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(add ? 1u : 0u)
+      : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(add ? 1u : 0u)
+      : "memory");
+}
+// Arrive on `bar` when every product this thread has issued is complete.
+__device__ __forceinline__ void mma_commit(uint64_t* bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
+               : "memory");
+}
+__device__ __forceinline__ void fence_before_sync() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_after_sync() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+
+// 32 columns of this thread's row of tensor memory.
+#define DQG_R8(a, i) "r"(a[i]), "r"(a[i + 1]), "r"(a[i + 2]), "r"(a[i + 3]), "r"(a[i + 4]), "r"(a[i + 5]), "r"(a[i + 6]), "r"(a[i + 7])
+#define DQG_W8(a, i) "=r"(a[i]), "=r"(a[i + 1]), "=r"(a[i + 2]), "=r"(a[i + 3]), "=r"(a[i + 4]), "=r"(a[i + 5]), "=r"(a[i + 6]), "=r"(a[i + 7])
+#define DQG_U8(a, i) "+r"(a[i]), "+r"(a[i + 1]), "+r"(a[i + 2]), "+r"(a[i + 3]), "+r"(a[i + 4]), "+r"(a[i + 5]), "+r"(a[i + 6]), "+r"(a[i + 7])
+__device__ __forceinline__ void tmem_ld32(uint32_t addr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : DQG_W8(r, 0), DQG_W8(r, 8), DQG_W8(r, 16), DQG_W8(r, 24)
+      : "r"(addr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31};" ::DQG_R8(r, 0),
+      DQG_R8(r, 8), DQG_R8(r, 16), DQG_R8(r, 24), "r"(addr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// Uses of r stay behind the wait that precedes this.
+__device__ __forceinline__ void hold32(uint32_t* r) {
+  asm volatile("" : DQG_U8(r, 0), DQG_U8(r, 8), DQG_U8(r, 16), DQG_U8(r, 24));
+}
+
+// ---------------------------------------------------------------- schedule
+// sum over i in [0, n) of floor((a i + b) / m), by the Euclid-like recursion
+// on (a, m) (lattice points under a line).
+__device__ __forceinline__ long long floor_sum(long long n, long long m, long long a, long long b) {
+  long long sum = 0;
+  while (n > 0) {
+    if (a >= m) {
+      sum += n * (n - 1) / 2 * (a / m);
+      a %= m;
+    }
+    if (b >= m) {
+      sum += n * (b / m);
+      b %= m;
+    }
+    const long long y = a * n + b;
+    if (y < m) break;
+    n = y / m;
+    b = y % m;
+    const long long t = m;
+    m = a;
+    a = t;
+  }
+  return sum;
+}
+
+struct Seq {  // one sequence's rows and keys
+  int q0, ql, kv, pairs;
+};
+__device__ __forceinline__ int blocks_of(int keys) { return keys > 0 ? (keys + kBlock - 1) / kBlock : 1; }
+
+__device__ __forceinline__ Seq load_seq(const Params& p, int b) {
+  Seq s;
+  if (p.splits) {
+    s.q0 = 0;
+    s.ql = p.T;
+    s.kv = p.prefix_len;
+  } else {
+    s.q0 = __ldg(p.q_starts + b);
+    s.ql = __ldg(p.q_starts + b + 1) - s.q0;
+    s.kv = clamped_len(p.lens, b, p.len_limit);
+    // Starts out of order or range: no rows.
+    if (s.q0 < 0 || s.ql < 0 || s.q0 > p.T || s.ql > p.T - s.q0) s.ql = 0;
+  }
+  s.pairs = (s.ql + 2 * p.tq - 1) / (2 * p.tq);
+  return s;
+}
+
+// Keys that a tile whose last token is i sees: its block count follows.
+__device__ __forceinline__ int limit_of(const Params& p, const Seq& s, int i) {
+  if (!p.causal) return s.kv;
+  const int lim = s.kv - s.ql + i + 1;
+  return lim < 0 ? 0 : lim;
+}
+
+// Blocks of a sequence's first n pairs, for one KV head.
+__device__ __forceinline__ long long blocks_before(const Params& p, const Seq& s, int n) {
+  if (n <= 0) return 0;
+  const int last = blocks_of(s.kv);
+  if (!p.causal) return static_cast<long long>(n) * last;
+  const long long tokens = 2 * p.tq, off = s.kv - s.ql;
+  const int full = n < s.pairs ? n : s.pairs - 1;  // the last pair ends at kv
+  long long one = off <= kBlock ? (kBlock - off) / tokens : 0;  // pairs that see one block at most
+  if (one > full) one = full;
+  return one + floor_sum(full - one, kBlock, tokens, off + (one + 1) * tokens + kBlock - 1) +
+         (n == s.pairs ? last : 0);
+}
+
+struct Share {  // a CTA's part of the blocks
+  int b, kvh, pair, x, ctas;
+  long long count, pos, total;
+};
+
+// Taken by one whole warp.
+__device__ __forceinline__ Share find_share(const Params& p, int cta, int n_ctas) {
+  const int lane = threadIdx.x & 31;
+  long long total = 0;
+  for (int b0 = 0; b0 < p.B; b0 += 32) {
+    const int b = b0 + lane;
+    if (b < p.B) {
+      const Seq s = load_seq(p, b);
+      total += blocks_before(p, s, s.pairs);
+    }
+  }
+#pragma unroll
+  for (int off = 16; off >= 1; off >>= 1) total += __shfl_xor_sync(0xffffffffu, total, off);
+  total *= p.hkv;
+  Share r;
+  r.total = total;
+  r.ctas = n_ctas < total ? n_ctas : static_cast<int>(total);
+  r.b = r.kvh = r.pair = r.x = 0;
+  r.pos = r.count = 0;
+  if (cta >= r.ctas) return r;
+  r.pos = cta * total / r.ctas;
+  r.count = (cta + 1) * total / r.ctas - r.pos;
+  long long before = 0;
+  for (int b0 = 0; b0 < p.B; b0 += 32) {
+    const int b = b0 + lane;
+    long long mine = 0;
+    if (b < p.B) {
+      const Seq s = load_seq(p, b);
+      mine = blocks_before(p, s, s.pairs);
+    }
+    long long sum = mine * p.hkv;
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+      const long long t = __shfl_up_sync(0xffffffffu, sum, off);
+      if (lane >= off) sum += t;
+    }
+    const unsigned past = __ballot_sync(0xffffffffu, before + sum > r.pos);
+    if (past) {
+      const int l = __ffs(past) - 1;
+      const long long per = __shfl_sync(0xffffffffu, mine, l);
+      long long in = r.pos - (before + __shfl_sync(0xffffffffu, sum, l) - per * p.hkv);
+      r.b = b0 + l;
+      r.kvh = static_cast<int>(in / per);
+      in -= r.kvh * per;
+      // The pair: 32 probes a round.
+      const Seq s = load_seq(p, r.b);
+      int lo = 0, hi = s.pairs;
+      while (hi - lo > 1) {
+        const int step = (hi - lo + 31) / 32;
+        const int probe = min(lo + (lane + 1) * step, hi);
+        const int f = __ffs(__ballot_sync(0xffffffffu, blocks_before(p, s, probe) > in)) - 1;
+        hi = min(lo + (f + 1) * step, hi);
+        lo = lo + f * step;
+      }
+      r.pair = lo;
+      r.x = static_cast<int>(in - blocks_before(p, s, lo));
+      break;
+    }
+    before += __shfl_sync(0xffffffffu, sum, 31);
+  }
+  return r;
+}
+
+// What a CTA does next: blocks [x0, x1) of one item.
+struct Segment {
+  int b, kvh, tok0, ntok, first, x0, x1, slot;  // first: the pair's first token in its sequence
+  int n0, n1;                                   // the tiles' blocks over the whole item
+  int kv, lim0;                                 // keys; keys that the first token sees (or below 0)
+  bool whole, causal;
+  int pieces;                                   // of the item, where this is the first of several
+  __device__ __forceinline__ int count(int t) const {
+    const int n = t ? n1 : n0, e = x1 < n ? x1 : n;
+    return e > x0 ? e - x0 : 0;
+  }
+};
+
+// Walks a CTA's share; every role of the CTA walks it alike.
+struct Walk {
+  Share r;
+  Seq s;
+  int piece;
+  __device__ __forceinline__ void begin(const Params& p, const Share& share) {
+    r = share;
+    piece = blockIdx.x;
+    if (p.splits || r.count > 0) s = load_seq(p, p.splits ? 0 : r.b);
+  }
+  __device__ __forceinline__ void tiles(const Params& p, Segment& g, int pair) {
+    g.first = pair * 2 * p.tq;
+    g.tok0 = s.q0 + g.first;
+    g.ntok = min(2 * p.tq, s.ql - g.first);
+    g.n0 = blocks_of(limit_of(p, s, g.first + min(p.tq, g.ntok) - 1));
+    g.n1 = g.ntok > p.tq ? blocks_of(limit_of(p, s, g.first + g.ntok - 1)) : 0;
+    g.kv = s.kv;
+    g.causal = p.causal;
+    g.lim0 = s.kv - s.ql + g.first + 1;
+  }
+  __device__ __forceinline__ bool next(const Params& p, Segment& g) {
+    if (p.splits) {
+      if (piece >= p.n_pieces) return false;
+      const int item = piece / p.splits, sp = piece - item * p.splits;
+      const int pair = item / p.hkv;
+      g.b = 0;
+      g.kvh = item - pair * p.hkv;
+      tiles(p, g, pair);
+      const int n = g.n0;  // both tiles see every key
+      g.x0 = static_cast<int>(static_cast<long long>(sp) * n / p.splits);
+      g.x1 = static_cast<int>(static_cast<long long>(sp + 1) * n / p.splits);
+      g.whole = false;
+      g.pieces = 0;
+      g.slot = piece;
+      piece += gridDim.x;
+      return true;
+    }
+    if (r.count <= 0) return false;
+    g.b = r.b;
+    g.kvh = r.kvh;
+    tiles(p, g, r.pair);
+    const int n = max(g.n0, g.n1);
+    g.x0 = r.x;
+    g.x1 = r.x + static_cast<int>(min(static_cast<long long>(n - r.x), r.count));
+    g.whole = g.x0 == 0 && g.x1 == n;
+    g.slot = 2 * blockIdx.x + (g.x0 > 0 ? 0 : 1);
+    g.pieces = 0;
+    if (!g.whole && g.x0 == 0)
+      g.pieces = static_cast<int>(((r.pos + n) * r.ctas - 1) / r.total) - static_cast<int>(blockIdx.x) + 1;
+    r.pos += g.x1 - g.x0;
+    r.count -= g.x1 - g.x0;
+    r.x = 0;
+    if (r.count > 0 && ++r.pair == s.pairs) {
+      r.pair = 0;
+      if (++r.kvh == p.hkv) {
+        r.kvh = 0;
+        do {
+          s = load_seq(p, ++r.b);
+        } while (s.pairs == 0);  // a share never ends in sequences without rows
+      }
+    }
+    return true;
+  }
+};
+
+// ------------------------------------------------------------------ kernel
+template <int D>
+struct Layout {
+  static constexpr int kStages = D == 128 ? 5 : 8;     // key or value blocks in flight
+  static constexpr int kSlot = kBlock * D * 2;
+  static constexpr int kTile = 128 * D * 2;            // a tile's queries
+  static constexpr int kRing = 2 * kTile;              // offset of the ring
+  static constexpr int kBars = kRing + kStages * kSlot;
+  static constexpr int kSmem = 1024 + kBars + 512;
+};
+
+template <typename E, int D>
+__global__ void __launch_bounds__(kThreads, 1)
+    prompt_kernel(const __grid_constant__ Params p, const __grid_constant__ CUtensorMap qmap,
+                  const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
+  using L = Layout<D>;
+  constexpr int kStages = L::kStages;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::kBars);
+  uint64_t* full = bars;                 // ring slots
+  uint64_t* empty = full + kStages;
+  uint64_t* q_full = empty + kStages;
+  uint64_t* q_empty = q_full + 1;
+  uint64_t* s_full = q_empty + 1;        // [2]
+  uint64_t* p_full = s_full + 2;
+  uint64_t* o_full = p_full + 2;
+  uint64_t* drained = o_full + 2;
+  Share* share = reinterpret_cast<Share*>(drained + 1);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(share + 1);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t sbase = smem_u32(smem);
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kStages; ++i) {
+      mbar_init(full + i, 1);
+      mbar_init(empty + i, 1);
+    }
+    mbar_init(q_full, 1);
+    mbar_init(q_empty, 1);
+    for (int t = 0; t < 2; ++t) {
+      mbar_init(s_full + t, 1);
+      mbar_init(p_full + t, 128);
+      mbar_init(o_full + t, 1);
+    }
+    mbar_init(drained, 1);
+    fence_mbar_init();
+    tma_prefetch_map(&qmap);
+    tma_prefetch_map(&kmap);
+    tma_prefetch_map(&vmap);
+  }
+  if (warp == kMmaWarp) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(tmem_slot))
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  // Rows that no (token, head) fills stay zero for the whole kernel.
+  const int used = p.tq * p.g;
+  if (used < 128) {
+    for (int i = threadIdx.x; i < 2 * (D / 64) * (128 - used) * 8; i += kThreads) {
+      const int ch = i & 7, rest = i >> 3;
+      const int r = used + rest % (128 - used), blk = rest / (128 - used);
+      *reinterpret_cast<uint4*>(smem + blk * (128 * 128) + r * 128 + ch * 16) = make_uint4(0, 0, 0, 0);
+    }
+    fence_async_shared();
+  }
+  pdl_wait_prior_grid();
+  if (warp == 0) {
+    Share s = {};
+    if (!p.splits) s = find_share(p, blockIdx.x, gridDim.x);
+    if (lane == 0) *share = s;
+  }
+  fence_before_sync();
+  __syncthreads();
+  fence_after_sync();
+  pdl_launch_dependents();
+  const uint32_t tmem = *tmem_slot;
+  // Registers: a softmax thread holds a row of 128 scores. 384 x 168 at
+  // launch = 256 x 216 + 128 x 72.
+  if (warp >= 8) {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+  if (warp == kCopyWarp) {
+    Walk walk;
+    walk.begin(p, *share);
+    Segment g;
+    // ---- copies: queries per segment, then key and value blocks in turn.
+    const int per = p.box_rows, boxes = kBlock / per * (D / 64);
+    const int half = lane % (D / 64), sub = lane / (D / 64);
+    int seg = 0, pos = 0;
+    bool ok = true;
+    while (ok && walk.next(p, g)) {
+      if (seg > 0 && !warp_wait(q_empty, (seg - 1) & 1)) break;
+      const int tiles = g.n1 > 0 ? 2 : 1;
+      if (lane == 0) mbar_arrive_expect_tx(q_full, tiles * used * D * 2);
+      __syncwarp();
+      if (lane < tiles * (D / 64)) {
+        const int t = lane / (D / 64), h = lane % (D / 64);
+        tma_load_4d(sbase + t * L::kTile + h * (128 * 128), &qmap, q_full, h * 64, 0, g.kvh, g.tok0 + t * p.tq);
+      }
+      ++seg;
+      const int32_t* row = p.table + g.b * p.table_stride;
+      if (!p.splits && lane == 0 && __ldg(p.lens + g.b) != g.kv) atomicOr(&g_status, kStatusBadIndex);
+      for (int x = g.x0; x < g.x1 && ok; ++x) {
+        const int t = x * kBlock + sub * per;
+        int page = static_cast<int>(p.n_pages);  // no such page: zeros
+        if (lane < boxes && t < g.kv) {
+          page = __ldg(row + (t >> p.page_shift));
+          if (page < 0 || page >= p.n_pages) {
+            page = static_cast<int>(p.n_pages);
+            atomicOr(&g_status, kStatusBadIndex);
+          }
+        }
+        const int in_page = t & ((1 << p.page_shift) - 1);
+        for (int w = 0; w < 2; ++w, ++pos) {
+          const int st = pos % kStages;
+          if (pos >= kStages && !warp_wait(empty + st, ((pos / kStages) & 1) ^ 1)) {
+            ok = false;
+            break;
+          }
+          if (lane == 0) mbar_arrive_expect_tx(full + st, L::kSlot);
+          __syncwarp();
+          if (lane < boxes)
+            tma_load_4d(sbase + L::kRing + st * L::kSlot + half * (kBlock * 128) + sub * per * 128,
+                        w ? &vmap : &kmap, full + st, half * 64, in_page, g.kvh, page);
+        }
+      }
+    }
+    // Copies still in flight land before the CTA's memory goes (bounded).
+    if (seg > 0) warp_wait(q_full, (seg - 1) & 1);
+    for (int i = pos < kStages ? 0 : pos - kStages; i < pos; ++i)
+      if (!warp_wait(full + i % kStages, (i / kStages) & 1)) break;
+  } else if (warp == kMmaWarp) {
+    // ---- products: one thread.
+    if (lane == 0) {
+      Walk walk;
+      walk.begin(p, *share);
+      Segment g;
+      constexpr uint32_t kIdS = instr_desc(Elem<E>::kFormat, kBlock, false);
+      constexpr uint32_t kIdO = instr_desc(Elem<E>::kFormat, D, true);
+      auto slot_addr = [&](int pos) { return sbase + L::kRing + (pos % kStages) * L::kSlot; };
+      auto issue_s = [&](int t, int pos) {
+        const uint32_t a = sbase + t * L::kTile, b = slot_addr(pos);
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k) {
+          const uint32_t off = (k / 4) * (128 * 128) + (k % 4) * 32;
+          mma_ss(tmem + t * kBlock, smem_desc(a + off, 16, 1024), smem_desc(b + off, 16, 1024), kIdS, k > 0);
+        }
+        mma_commit(s_full + t);
+      };
+      auto issue_o = [&](int t, int pos, bool add) {
+        const uint32_t b = slot_addr(pos);
+#pragma unroll
+        for (int k = 0; k < kBlock / 16; ++k)
+          mma_ts(tmem + 2 * kBlock + t * D, tmem + t * kBlock + k * 8,
+                 smem_desc(b + k * 16 * 128, kBlock * 128, 1024), kIdO, add || k > 0);
+      };
+      auto wait_full = [&](int pos) {
+        if (!mbar_wait(full + pos % kStages, (pos / kStages) & 1)) return false;
+        fence_after_sync();
+        return true;
+      };
+      int seg = 0, base = 0;
+      uint32_t weights = 0;  // parities of the two p_full barriers
+      bool ok = true;
+      while (ok && walk.next(p, g)) {
+        const int c0 = g.count(0), c1 = g.count(1);
+        const int n = g.x1 - g.x0;
+        ok = mbar_wait(q_full, seg & 1) && wait_full(base);
+        ++seg;
+        if (!ok) break;
+        fence_after_sync();
+        if (c0 > 0) issue_s(0, base);
+        if (c1 > 0) issue_s(1, base);
+        mma_commit(empty + base % kStages);
+        if (n == 1) mma_commit(q_empty);
+        for (int j = 0; j < n && ok; ++j) {
+          const int vpos = base + 2 * j + 1, kpos = vpos + 1;
+          ok = wait_full(vpos) && (j + 1 == n || wait_full(kpos));
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            const int c = t ? c1 : c0;
+            if (!ok || j >= c) continue;
+            ok = mbar_wait(p_full + t, weights >> t & 1);
+            weights ^= 1u << t;
+            if (!ok) continue;
+            fence_after_sync();
+            issue_o(t, vpos, j > 0);
+            if (j + 1 < c) issue_s(t, kpos);
+            else mma_commit(o_full + t);
+          }
+          mma_commit(empty + vpos % kStages);
+          if (j + 1 < n) mma_commit(empty + kpos % kStages);
+          if (j + 2 == n) mma_commit(q_empty);
+        }
+        base += 2 * n;
+      }
+      // Nothing of this CTA is in flight when it ends (bounded).
+      mma_commit(drained);
+      mbar_wait(drained, 0);
+    }
+    __syncwarp();
+  }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+    Walk walk;
+    walk.begin(p, *share);
+    Segment g;
+    // ---- softmax: one thread a row of tile t.
+    const int t = warp >> 2, r = threadIdx.x & 127;
+    const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;  // this warp's 32 lanes
+    const uint32_t ts = tmem + lanes + t * kBlock, to = tmem + lanes + 2 * kBlock + t * D;
+    const int tok = r / p.g, head = r - tok * p.g;  // of the tile
+    int scores = 0, outs = 0, base = 0;
+    bool ok = true, cut_first = false;
+    while (ok && walk.next(p, g)) {
+      const int n = g.count(t);
+      const int tile_n = t ? g.n1 : g.n0;  // 0: a tile without rows
+      const bool live = r < used && t * p.tq + tok < g.ntok;
+      const int limit = g.causal ? min(g.lim0 + t * p.tq + tok, g.kv) : g.kv;
+      // Keys that every row of the tile sees (rows past the end see no fewer).
+      const int seen = g.causal ? g.lim0 + t * p.tq : g.kv;
+      float m = -INFINITY, l = 0.f;
+      for (int j = 0; j < n; ++j) {
+        const int k0 = (g.x0 + j) * kBlock;
+        if (!warp_wait(s_full + t, scores & 1)) {
+          ok = false;
+          break;
+        }
+        ++scores;
+        fence_after_sync();
+        uint32_t raw[128];
+        float* s = reinterpret_cast<float*>(raw);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) tmem_ld32(ts + 32 * q, raw + 32 * q);
+        tmem_wait_ld();
+#pragma unroll
+        for (int q = 0; q < 4; ++q) hold32(raw + 32 * q);
+        if (k0 + kBlock > seen) {
+          const int left = limit - k0;
+#pragma unroll
+          for (int i = 0; i < kBlock; ++i) s[i] = i < left ? s[i] : -INFINITY;
+        }
+        float mx[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+        for (int i = 4; i < kBlock; i += 4)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) mx[q] = fmaxf(mx[q], s[i + q]);
+        const float m_new = fmaxf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])), m);
+        const bool grow = (m_new - m) * p.scale_log2 > kMaxGrowth;
+        if (j == 0) {
+          m = m_new;  // no O yet: the first product overwrites it
+        } else if (__any_sync(0xffffffffu, grow)) {
+          const float f = grow ? exp2_approx((m - m_new) * p.scale_log2) : 1.f;
+#pragma unroll
+          for (int q = 0; q < D / 32; ++q) {
+            uint32_t o[32];
+            tmem_ld32(to + 32 * q, o);
+            tmem_wait_ld();
+            hold32(o);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+            tmem_st32(to + 32 * q, o);
+          }
+          l *= f;
+          if (grow) m = m_new;
+        }
+        const float ref = m == -INFINITY ? 0.f : m * p.scale_log2;
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int hq = 0; hq < 2; ++hq) {
+          uint32_t w[32];
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            const float a = exp2_approx(fmaf(s[64 * hq + 2 * i], p.scale_log2, -ref));
+            const float b = exp2_approx(fmaf(s[64 * hq + 2 * i + 1], p.scale_log2, -ref));
+            sum[(2 * i) & 3] += a;
+            sum[(2 * i + 1) & 3] += b;
+            w[i] = Elem<E>::pack(a, b);
+          }
+          tmem_st32(ts + 32 * hq, w);
+        }
+        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        // Behind the sequence's end its last page holds anything: zero those
+        // values (a zero weight times an infinity would not be zero).
+        if (k0 + kBlock > g.kv && g.kv > k0 && (g.kv & ((1 << p.page_shift) - 1))) {
+          const int vpos = base + 2 * j + 1;
+          if (!warp_wait(full + vpos % kStages, (vpos / kStages) & 1)) {
+            ok = false;
+            break;
+          }
+          const int r0 = g.kv - k0;
+          const int r1 = min(kBlock, ((r0 >> p.page_shift) + 1) << p.page_shift);
+          uint8_t* v = smem + L::kRing + (vpos % kStages) * L::kSlot;
+          for (int i = r; i < (r1 - r0) * (D / 8); i += 128) {
+            const int row = r0 + i / (D / 8), ch = i % (D / 8);
+            *reinterpret_cast<uint4*>(v + (ch >> 3) * (kBlock * 128) + row * 128 + (ch & 7) * 16) =
+                make_uint4(0, 0, 0, 0);
+          }
+          fence_async_shared();
+        }
+        tmem_wait_st();
+        fence_before_sync();
+        mbar_arrive(p_full + t);
+      }
+      base += 2 * (g.x1 - g.x0);
+      if (!ok) break;
+      if (g.pieces && threadIdx.x == 0) p.desc[blockIdx.x] = Desc{g.tok0, g.ntok, g.kvh, g.pieces};
+      cut_first |= g.pieces != 0;
+      if (n > 0) {
+        if (!warp_wait(o_full + t, outs & 1)) break;
+        ++outs;
+        fence_after_sync();
+      }
+      const float inv = l == 0.f ? 0.f : __frcp_rn(l);
+      E* out = static_cast<E*>(p.out) +
+               (static_cast<int64_t>(g.tok0 + t * p.tq + tok) * p.hq + g.kvh * p.g + head) * D;
+      const int64_t slot = g.slot;
+      if (!g.whole && tile_n > 0) {
+        p.ml[slot * 512 + t * 128 + r] = n > 0 && m != -INFINITY ? m * p.scale_log2 : -INFINITY;
+        p.ml[slot * 512 + 256 + t * 128 + r] = l;
+      }
+      if (tile_n > 0) {
+#pragma unroll
+        for (int q = 0; q < D / 32; ++q) {
+          uint32_t o[32];
+          if (n > 0) {
+            tmem_ld32(to + 32 * q, o);
+            tmem_wait_ld();
+            hold32(o);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] = 0u;
+          }
+          if (!g.whole) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              p.part[(slot * (D / 4) + q * 8 + i) * 256 + t * 128 + r] =
+                  make_float4(__uint_as_float(o[4 * i]), __uint_as_float(o[4 * i + 1]),
+                              __uint_as_float(o[4 * i + 2]), __uint_as_float(o[4 * i + 3]));
+          } else if (live) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              uint4 w;
+              uint32_t* ww = reinterpret_cast<uint32_t*>(&w);
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                ww[e] = Elem<E>::pack(__uint_as_float(o[8 * i + 2 * e]) * inv, __uint_as_float(o[8 * i + 2 * e + 1]) * inv);
+              *reinterpret_cast<uint4*>(out + 32 * q + 8 * i) = w;
+            }
+          }
+        }
+      }
+      fence_before_sync();
+    }
+    if (threadIdx.x == 0 && !cut_first && !p.splits) p.desc[blockIdx.x] = Desc{0, 0, 0, 0};
+  }
+  fence_before_sync();
+  __syncthreads();
+  fence_after_sync();
+  if (warp == kMmaWarp)
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+}
+
+// Joins the pieces of the item whose first piece CTA blockIdx.x holds: 32 rows
+// a block, a lane a row.
+template <typename E, int D>
+__global__ void __launch_bounds__(256) prompt_join_kernel(const __grid_constant__ Params p) {
+  pdl_wait_prior_grid();
+  pdl_launch_dependents();
+  const int4 d = __ldcg(reinterpret_cast<const int4*>(p.desc + blockIdx.x));
+  const int tok0 = d.x, ntok = d.y, kvh = d.z, pieces = d.w;
+  if (pieces == 0) return;
+  const int row = blockIdx.y * 32 + (threadIdx.x & 31), r = row & 127;
+  const int tok = (row >> 7) * p.tq + r / p.g;
+  if (r >= p.tq * p.g || tok >= ntok) return;
+  // Piece 0 lies in this CTA's second slot, piece i > 0 in CTA + i's first.
+  auto slot_of = [&](int i) { return 2 * (static_cast<int64_t>(blockIdx.x) + i) + (i == 0 ? 1 : 0); };
+  float m = -INFINITY;
+  for (int i = 0; i < pieces; ++i) m = fmaxf(m, __ldcg(p.ml + slot_of(i) * 512 + row));
+  const float ref = m == -INFINITY ? 0.f : m;
+  E* out = static_cast<E*>(p.out) +
+           (static_cast<int64_t>(tok0 + tok) * p.hq + kvh * p.g + r % p.g) * D;
+  for (int d8 = threadIdx.x >> 5; d8 < D / 8; d8 += 8) {
+    float den = 0.f, acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int i = 0; i < pieces; ++i) {
+      const int64_t sl = slot_of(i);
+      const float f = exp2_approx(__ldcg(p.ml + sl * 512 + row) - ref);
+      den = fmaf(__ldcg(p.ml + sl * 512 + 256 + row), f, den);
+      const float4 a = __ldcg(p.part + (sl * (D / 4) + 2 * d8) * 256 + row);
+      const float4 b = __ldcg(p.part + (sl * (D / 4) + 2 * d8 + 1) * 256 + row);
+      acc[0] = fmaf(a.x, f, acc[0]);
+      acc[1] = fmaf(a.y, f, acc[1]);
+      acc[2] = fmaf(a.z, f, acc[2]);
+      acc[3] = fmaf(a.w, f, acc[3]);
+      acc[4] = fmaf(b.x, f, acc[4]);
+      acc[5] = fmaf(b.y, f, acc[5]);
+      acc[6] = fmaf(b.z, f, acc[6]);
+      acc[7] = fmaf(b.w, f, acc[7]);
+    }
+    const float inv = den == 0.f ? 0.f : __frcp_rn(den);
+    uint4 w;
+    uint32_t* ww = reinterpret_cast<uint32_t*>(&w);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) ww[e] = Elem<E>::pack(acc[2 * e] * inv, acc[2 * e + 1] * inv);
+    *reinterpret_cast<uint4*>(out + 8 * d8) = w;
+  }
+}
+
+template <typename E, int D>
+cudaError_t launch(const Params& p, const CUtensorMap& qmap, const CUtensorMap& kmap,
+                   const CUtensorMap& vmap, int num_sms, cudaStream_t stream) {
+  static int configured[64] = {0};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev < 0 || dev >= 64 || !configured[dev]) {
+    e = cudaFuncSetAttribute(prompt_kernel<E, D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             Layout<D>::kSmem);
+    if (e != cudaSuccess) return e;
+    if (dev >= 0 && dev < 64) configured[dev] = 1;
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(p.splits && p.n_pieces < num_sms ? p.n_pieces : num_sms);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = Layout<D>::kSmem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  e = cudaLaunchKernelEx(&cfg, prompt_kernel<E, D>, p, qmap, kmap, vmap);
+  if (e != cudaSuccess || p.splits) return e;
+  cfg.gridDim = dim3(num_sms, 8);
+  cfg.blockDim = dim3(256);
+  cfg.dynamicSmemBytes = 0;
+  return cudaLaunchKernelEx(&cfg, prompt_join_kernel<E, D>, p);
+}
+
+size_t slot_bytes(int D) { return 256 * static_cast<size_t>(D) * 4 + 512 * 4; }
+int pairs_of(int n, int tq) { return (n + 2 * tq - 1) / (2 * tq); }
+
+}  // namespace
+
+int prompt_box_rows(int page_size) { return page_size < kBlock ? page_size : kBlock; }
+int prompt_tokens_per_tile(int hq, int n_kv_heads) { return 128 / (hq / n_kv_heads); }
+
+size_t prompt_workspace(int D, int num_sms) {
+  return static_cast<size_t>(num_sms) * (2 * slot_bytes(D) + sizeof(Desc));
+}
+
+// Pieces of a prefix: of 1 .. 64 a KV head and pair, those that keep the
+// busiest SM's blocks fewest; half a block counted for each, for the joining.
+int prefix_splits(int n_seqs, int hq, int n_kv_heads, int prefix_len, int num_sms) {
+  const long long items = static_cast<long long>(pairs_of(n_seqs, prompt_tokens_per_tile(hq, n_kv_heads))) * n_kv_heads;
+  const int blocks = (prefix_len + kBlock - 1) / kBlock;
+  int best = 1;
+  long long cost = -1;
+  for (int s = 1; s <= 64 && s <= blocks; ++s) {
+    const long long c = 2 * ((items * s + num_sms - 1) / num_sms * ((blocks + s - 1) / s)) + s;
+    if (cost < 0 || c < cost) {
+      cost = c;
+      best = s;
+    }
+  }
+  return best;
+}
+
+size_t prefix_workspace(int n_seqs, int hq, int n_kv_heads, int D, int prefix_len, int num_sms) {
+  const size_t pieces = static_cast<size_t>(pairs_of(n_seqs, prompt_tokens_per_tile(hq, n_kv_heads))) * n_kv_heads *
+                        prefix_splits(n_seqs, hq, n_kv_heads, prefix_len, num_sms);
+  return pieces * slot_bytes(D);
+}
+
+PrefixPieces prefix_pieces(const PromptArgs& a, const PagedPool& pool, int num_sms) {
+  PrefixPieces f;
+  f.S = prefix_splits(a.T, a.hq, pool.n_kv_heads, a.prefix_len, num_sms);
+  f.tq = prompt_tokens_per_tile(a.hq, pool.n_kv_heads);
+  const size_t pieces = static_cast<size_t>(pairs_of(a.T, f.tq)) * pool.n_kv_heads * f.S;
+  f.o = static_cast<const float*>(a.workspace);
+  f.ml = f.o + pieces * 256 * pool.D;
+  return f;
+}
+
+cudaError_t launch_prompt(const PagedPool& pool, const CUtensorMap& qmap, const CUtensorMap& kmap,
+                          const CUtensorMap& vmap, const PromptArgs& a, int num_sms,
+                          cudaStream_t stream) {
+  Params p;
+  p.table = a.table;
+  p.q_starts = a.q_starts;
+  p.lens = a.kv_lens;
+  p.out = a.out;
+  p.table_stride = a.table_stride;
+  p.n_pages = pool.n_pages;
+  p.B = a.B;
+  p.T = a.T;
+  p.hq = a.hq;
+  p.hkv = pool.n_kv_heads;
+  p.g = a.hq / pool.n_kv_heads;
+  p.tq = prompt_tokens_per_tile(a.hq, pool.n_kv_heads);
+  p.page_shift = 0;
+  while ((1 << p.page_shift) < pool.page_size) ++p.page_shift;
+  const int64_t limit = static_cast<int64_t>(a.table_width) * pool.page_size;
+  p.len_limit = limit < (1 << 30) ? static_cast<int>(limit) : 1 << 30;
+  p.box_rows = prompt_box_rows(pool.page_size);
+  p.causal = a.causal;
+  p.scale_log2 = a.scale_log2;
+  p.prefix_len = a.prefix_len;
+  p.splits = p.n_pieces = 0;
+  size_t slots = 2 * static_cast<size_t>(num_sms);
+  if (a.prefix_len > 0) {
+    p.causal = false;
+    p.splits = prefix_splits(a.T, a.hq, pool.n_kv_heads, a.prefix_len, num_sms);
+    slots = static_cast<size_t>(pairs_of(a.T, p.tq)) * pool.n_kv_heads * p.splits;
+    p.n_pieces = static_cast<int>(slots);
+  }
+  p.part = static_cast<float4*>(a.workspace);
+  p.ml = reinterpret_cast<float*>(p.part + slots * 64 * pool.D);
+  p.desc = reinterpret_cast<Desc*>(p.ml + slots * 512);
+  if (pool.bf16)
+    return pool.D == 128 ? launch<__nv_bfloat16, 128>(p, qmap, kmap, vmap, num_sms, stream)
+                         : launch<__nv_bfloat16, 64>(p, qmap, kmap, vmap, num_sms, stream);
+  return pool.D == 128 ? launch<__half, 128>(p, qmap, kmap, vmap, num_sms, stream)
+                       : launch<__half, 64>(p, qmap, kmap, vmap, num_sms, stream);
+}
+
+}  // namespace dqg
+
+DQG_STATUS_READER(read_status_prompt)

@@ -78,6 +78,21 @@ def _decode_bytes(device_index: int, head_dim: int) -> int:
     return int(n.value)
 
 
+@functools.lru_cache(maxsize=None)
+def _prompt_bytes(device_index: int, head_dim: int) -> int:
+    n = ctypes.c_uint64(0)
+    _native.check(_native.lib().dqg_prompt_attention_workspace(head_dim, ctypes.byref(n)))
+    return int(n.value)
+
+
+@functools.lru_cache(maxsize=256)
+def _prefix_bytes(device_index: int, n_seqs: int, hq: int, hkv: int, head_dim: int, prefix_len: int) -> int:
+    n = ctypes.c_uint64(0)
+    _native.check(_native.lib().dqg_shared_prefix_workspace(n_seqs, hq, hkv, head_dim, prefix_len,
+                                                            ctypes.byref(n)))
+    return int(n.value)
+
+
 def _workspace(given: torch.Tensor | None, need: int, device) -> torch.Tensor:
     if given is None:
         return torch.empty(need, dtype=torch.uint8, device=device)
@@ -256,3 +271,99 @@ def paged_attention_workspace(head_dim: int, device) -> torch.Tensor:
     device = torch.device(device)
     with _on(device):
         return torch.empty(_decode_bytes(device.index, head_dim), dtype=torch.uint8, device=device)
+
+
+def prompt_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch.Tensor,
+                     q_starts: torch.Tensor, kv_lens: torch.Tensor, *, causal: bool = True,
+                     scale: float | None = None, workspace: torch.Tensor | None = None) -> torch.Tensor:
+    """Packed prompts (or chunks at their ends) over their cached positions.
+
+    q [T, Hq, D] holds the new tokens of all sequences one after the other:
+    sequence b has rows ``q_starts[b]`` to ``q_starts[b + 1] - 1`` (int32
+    [B + 1], from 0 to T), and they are the newest of its ``kv_lens[b]`` cached
+    positions (so they were stored first). Row i of q_len sees the keys before
+    kv_len - q_len + i + 1 (all kv_len unless ``causal``); a row that sees none
+    gives zeros. Rows outside every sequence are undefined in the result.
+    Returns [T, Hq, D]. Table, lengths, scale and workspace
+    (``prompt_attention_workspace``) as ``paged_attention``."""
+    t, hq, d = q.shape
+    b = kv_lens.shape[0]
+    scale = 1.0 / math.sqrt(d) if scale is None else scale
+    if not q.is_cuda:
+        out = torch.zeros_like(q)
+        for i in range(b):
+            lo, hi, n = int(q_starts[i]), int(q_starts[i + 1]), int(kv_lens[i])
+            ends = (n - (hi - lo) + torch.arange(hi - lo) + 1 if causal else torch.full((hi - lo,), n))
+            out[lo:hi] = _cpu_attention(q[lo:hi].float(), _rows(k_pages, block_table[i], n),
+                                        _rows(v_pages, block_table[i], n), ends, scale).to(q.dtype)
+        return out
+    kv = _pools(k_pages, v_pages, ("q", q))
+    device = q.device
+    _query(q, kv.head_dim)
+    _ints(device, ("block_table", block_table, torch.int32, 2), ("q_starts", q_starts, torch.int32, 1),
+          ("kv_lens", kv_lens, torch.int32, 1))
+    if block_table.shape[0] != b or q_starts.shape[0] != b + 1:
+        raise RuntimeError(f"block_table and q_starts must hold {b} and {b + 1} rows for {b} sequences")
+    out = torch.empty((t, hq, d), dtype=q.dtype, device=device)
+    with _on(device):
+        ws = _workspace(workspace, _prompt_bytes(device.index, d), device)
+        _native.check(_native.lib().dqg_prompt_attention(
+            q.data_ptr(), q.stride(0), q.stride(1), t, hq, ctypes.byref(kv), block_table.data_ptr(),
+            block_table.shape[1], block_table.stride(0) if b > 1 else block_table.shape[1],
+            q_starts.data_ptr(), kv_lens.data_ptr(), b, int(causal), scale, out.data_ptr(), ws.data_ptr(),
+            ws.numel() * ws.element_size(), _stream(device)))
+    return out
+
+
+def prompt_attention_workspace(head_dim: int, device) -> torch.Tensor:
+    """Scratch memory for ``prompt_attention`` calls of any batch and lengths."""
+    device = torch.device(device)
+    with _on(device):
+        return torch.empty(_prompt_bytes(device.index, head_dim), dtype=torch.uint8, device=device)
+
+
+def shared_prefix_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
+                            prefix_table: torch.Tensor, prefix_len: int, block_table: torch.Tensor,
+                            kv_lens: torch.Tensor, *, scale: float | None = None,
+                            workspace: torch.Tensor | None = None) -> torch.Tensor:
+    """``paged_attention`` for a batch whose sequences share their first
+    ``prefix_len`` positions (a system prompt, a document that is sampled from
+    many times): those lie in the pages of ``prefix_table`` (int32
+    [prefix pages]) and are read once for the whole batch; ``block_table`` and
+    ``kv_lens`` are each sequence's own positions after them (none is fine).
+    ``workspace``: ``shared_prefix_workspace``."""
+    b, hq, d = q.shape
+    scale = 1.0 / math.sqrt(d) if scale is None else scale
+    if not q.is_cuda:
+        out = []
+        for i in range(b):
+            n = int(kv_lens[i])
+            k, v = (torch.cat([_rows(p, prefix_table, prefix_len), _rows(p, block_table[i], n)], 1)
+                    for p in (k_pages, v_pages))
+            out.append(_cpu_attention(q[i:i + 1].float(), k, v, torch.tensor([prefix_len + n]), scale))
+        return torch.cat(out).to(q.dtype) if out else torch.empty_like(q)
+    kv = _pools(k_pages, v_pages, ("q", q))
+    device = q.device
+    _query(q, kv.head_dim)
+    _ints(device, ("prefix_table", prefix_table, torch.int32, 1), ("block_table", block_table, torch.int32, 2),
+          ("kv_lens", kv_lens, torch.int32, 1))
+    if block_table.shape[0] != b or kv_lens.shape[0] != b:
+        raise RuntimeError(f"block_table and kv_lens must hold one row for each of the {b} sequences")
+    out = torch.empty((b, hq, d), dtype=q.dtype, device=device)
+    with _on(device):
+        ws = _workspace(workspace, _prefix_bytes(device.index, b, hq, kv.n_kv_heads, d, prefix_len), device)
+        _native.check(_native.lib().dqg_shared_prefix_attention(
+            q.data_ptr(), q.stride(0), q.stride(1), b, hq, ctypes.byref(kv), prefix_table.data_ptr(),
+            prefix_table.shape[0], prefix_len, block_table.data_ptr(), block_table.shape[1],
+            block_table.stride(0) if b > 1 else block_table.shape[1], kv_lens.data_ptr(), scale,
+            out.data_ptr(), ws.data_ptr(), ws.numel() * ws.element_size(), _stream(device)))
+    return out
+
+
+def shared_prefix_workspace(n_seqs: int, n_q_heads: int, n_kv_heads: int, head_dim: int, prefix_len: int,
+                            device) -> torch.Tensor:
+    """Scratch memory for ``shared_prefix_attention`` calls of these sizes."""
+    device = torch.device(device)
+    with _on(device):
+        return torch.empty(_prefix_bytes(device.index, n_seqs, n_q_heads, n_kv_heads, head_dim, prefix_len),
+                           dtype=torch.uint8, device=device)

@@ -395,6 +395,44 @@ int dqg_paged_attention(const void *q, int64_t q_stride_seq, int64_t q_stride_he
                         int64_t table_width, int64_t table_stride, const int32_t *kv_lens, float scale,
                         void *out, void *workspace, uint64_t workspace_bytes, void *stream);
 
+/*
+ * Attention of whole prompts, or of chunks at their ends, over the pages.
+ * T query tokens are packed: sequence b owns rows q_starts[b] ..
+ * q_starts[b + 1] - 1 of q [T, Hq, D] (q_starts[0] = 0, ascending, the last
+ * one T; sequences may be empty), the newest of its kv_lens[b] cached
+ * positions. Causal: its row i sees the keys before kv_lens[b] - q_len + i + 1;
+ * otherwise all kv_lens[b]. A row that sees none gives zeros. Values at cached
+ * positions must be finite where a causal mask hides them from some rows (a
+ * hidden infinity or NaN among the last 128 positions before a row's own block
+ * ends reaches the row); what lies behind a sequence's end does not matter.
+ * Heads, strides, table, lengths on the device, scale and workspace
+ * (dqg_prompt_attention_workspace(D) bytes) as dqg_paged_attention. Rows of q
+ * outside every sequence leave their rows of out unwritten.
+ */
+int dqg_prompt_attention_workspace(int64_t head_dim, uint64_t *bytes);
+int dqg_prompt_attention(const void *q, int64_t q_stride_row, int64_t q_stride_head, int64_t T,
+                         int64_t n_q_heads, const dqg_paged_kv *kv, const int32_t *block_table,
+                         int64_t table_width, int64_t table_stride, const int32_t *q_starts,
+                         const int32_t *kv_lens, int64_t n_seqs, int causal, float scale, void *out,
+                         void *workspace, uint64_t workspace_bytes, void *stream);
+
+/*
+ * Decode attention of a batch whose sequences share their first prefix_len
+ * positions: out[b, h] is as dqg_paged_attention's over the prefix's keys and
+ * then sequence b's own kv_lens[b]. The prefix's pages (prefix_table
+ * [prefix_pages]) are read once for the whole batch. prefix_len is a host
+ * value (0: no prefix); the sequences' own lengths are read on the device and
+ * may be zero. Everything else as dqg_paged_attention.
+ */
+int dqg_shared_prefix_workspace(int64_t n_seqs, int64_t n_q_heads, int64_t n_kv_heads, int64_t head_dim,
+                                int64_t prefix_len, uint64_t *bytes);
+int dqg_shared_prefix_attention(const void *q, int64_t q_stride_seq, int64_t q_stride_head,
+                                int64_t n_seqs, int64_t n_q_heads, const dqg_paged_kv *kv,
+                                const int32_t *prefix_table, int64_t prefix_pages, int64_t prefix_len,
+                                const int32_t *block_table, int64_t table_width, int64_t table_stride,
+                                const int32_t *kv_lens, float scale, void *out, void *workspace,
+                                uint64_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -215,3 +215,91 @@ def test_decode(cuda_device, lens, hq, hkv, d, page, dtype):
     for _ in range(3):
         assert torch.equal(paged_ops.paged_attention(q, k, v, table, kv_lens, workspace=ws), out)
     assert _native.device_status(cuda_device.index) == 0
+
+
+# ------------------------------------------------------------------- prompt
+def prompt_case(gen, q_lens, kv_lens, hq, hkv, d, page, dtype, device, fill=float("nan")):
+    k, v, table = make_cache(gen, kv_lens, hkv, d, page, dtype, device, fill=fill)
+    starts = torch.tensor([0] + q_lens, device=device).cumsum(0).int()
+    q = torch.randn((int(starts[-1]), hq, d), generator=gen, device=device).to(dtype)
+    return q, k, v, table, starts, torch.tensor(kv_lens, dtype=torch.int32, device=device)
+
+
+def prompt64(q, k, v, table, starts, kv_lens, causal, scale):
+    out = torch.zeros(q.shape, dtype=torch.float64, device=q.device)
+    for i in range(len(kv_lens)):
+        lo, hi, n = int(starts[i]), int(starts[i + 1]), int(kv_lens[i])
+        ends = (n - (hi - lo) + torch.arange(hi - lo, device=q.device) + 1 if causal
+                else torch.full((hi - lo,), n, device=q.device))
+        if hi > lo and n:
+            out[lo:hi] = attend64(q[lo:hi], rows64(k, table[i], n), rows64(v, table[i], n), ends, scale)
+    return out
+
+
+PROMPT = [
+    # query lengths, key lengths, hq, hkv, d, page
+    ([1], [1], 4, 4, 128, 16),
+    ([128], [128], 2, 2, 128, 128),
+    ([257], [257], 3, 3, 128, 64),
+    ([300], [300], 16, 2, 128, 16),
+    ([40], [700], 8, 1, 128, 32),             # a chunk: few rows, many keys
+    ([1], [5000], 64, 8, 128, 64),            # one row, cut over many CTAs
+    ([0, 5, 1, 0, 130, 64], [0, 5, 1, 9, 130, 64], 8, 2, 64, 16),
+    ([7, 200], [3, 150], 4, 2, 128, 16),      # more queries than keys: rows that see none
+    ([3], [0], 4, 2, 128, 16),
+    ([33, 260], [33, 1000], 28, 4, 128, 256),  # 7 heads a group: 126 of a tile's rows
+    ([19], [90], 48, 1, 64, 32),              # 96 of 128 rows
+    ([5], [300], 128, 1, 128, 128),
+    ([9], [40], 100, 1, 128, 16),
+    ([700, 1, 513], [700, 800, 600], 6, 3, 64, 128),
+    ([1] * 200, list(range(1, 201)), 4, 2, 128, 16),
+]
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("causal", [True, False], ids=["causal", "full"])
+@pytest.mark.parametrize("ql,kl,hq,hkv,d,page", PROMPT, ids=lambda v: str(v)[:40])
+def test_prompt(cuda_device, ql, kl, hq, hkv, d, page, causal, dtype):
+    gen = torch.Generator(device=cuda_device).manual_seed(sum(ql) + hq)
+    args = prompt_case(gen, ql, kl, hq, hkv, d, page, dtype, cuda_device)
+    out = paged_ops.prompt_attention(*args, causal=causal)
+    assert _native.device_status(cuda_device.index, reset=True) == 0
+    ref = prompt64(*args, causal, 1 / math.sqrt(d))
+    check_attention(out, ref, float(torch.nan_to_num(args[2].float()).abs().max()), dtype)
+    ws = paged_ops.prompt_attention_workspace(d, cuda_device).fill_(255)
+    for _ in range(3):
+        assert torch.equal(paged_ops.prompt_attention(*args, causal=causal, workspace=ws), out)
+
+
+# ------------------------------------------------------------ shared prefix
+PREFIX = [
+    # prefix, own lengths, hq, hkv, d, page
+    (1, [0, 5, 70], 8, 2, 128, 16),
+    (130, [0, 0], 4, 4, 128, 64),
+    (2000, [1, 300, 0, 64, 65], 32, 32, 128, 16),
+    (777, [30] * 50, 64, 8, 128, 32),
+    (5000, [100, 3], 28, 4, 128, 128),
+    (300, [9, 0, 200], 40, 1, 64, 16),
+    (0, [9, 0, 200], 8, 2, 64, 256),
+    (900, [1], 100, 1, 64, 16),
+    (128, list(range(300)), 2, 2, 64, 16),
+]
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("prefix,lens,hq,hkv,d,page", PREFIX, ids=lambda v: str(v)[:40])
+def test_shared_prefix(cuda_device, prefix, lens, hq, hkv, d, page, dtype):
+    gen = torch.Generator(device=cuda_device).manual_seed(prefix + hq)
+    k, v, table = make_cache(gen, lens + [prefix], hkv, d, page, dtype, cuda_device, fill=float("nan"))
+    own, shared = table[:-1].contiguous(), table[-1].contiguous()
+    q = torch.randn((len(lens), hq, d), generator=gen, device=cuda_device).to(dtype)
+    kv_lens = torch.tensor(lens, dtype=torch.int32, device=cuda_device)
+    out = paged_ops.shared_prefix_attention(q, k, v, shared, prefix, own, kv_lens)
+    assert _native.device_status(cuda_device.index, reset=True) == 0
+    ref = []
+    for i, n in enumerate(lens):
+        kk, vv = (torch.cat([rows64(p, shared, prefix), rows64(p, own[i], n)]) for p in (k, v))
+        ref.append(attend64(q[i:i + 1], kk, vv, kv_lens[i:i + 1] + prefix, 1 / math.sqrt(d)))
+    check_attention(out, torch.cat(ref), float(torch.nan_to_num(v.float()).abs().max()), dtype)
+    for _ in range(3):
+        assert torch.equal(paged_ops.shared_prefix_attention(q, k, v, shared, prefix, own, kv_lens), out)
