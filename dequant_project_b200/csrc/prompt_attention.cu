@@ -39,6 +39,8 @@ constexpr int kBlock = 128;         // keys a block; rows a tile
 constexpr int kThreads = 384;       // 2 x 4 softmax warps; products, copies, two idle
 constexpr int kMmaWarp = 8, kCopyWarp = 9;
 constexpr float kMaxGrowth = 8.f;   // log2 of the largest weight
+constexpr int kItemUnits = 2;       // an item's start and end, in blocks' time
+constexpr int kSegs = 4;            // segments described ahead
 
 struct Desc {  // a cut item, by the CTA that holds its first piece
   int tok0, ntok, kvh, pieces;
@@ -56,6 +58,7 @@ struct Params {
   int B, T, hq, hkv, g, tq, page_shift, len_limit, box_rows;
   bool causal;
   float scale_log2;
+  uint32_t g_magic;                   // ceil(2^32 / g), 0 for g = 1
   int prefix_len, splits, n_pieces;   // a shared prefix: splits > 0
 };
 
@@ -122,6 +125,26 @@ __device__ __forceinline__ void hold32(uint32_t* r) {
   asm volatile("" : DQG_U8(r, 0), DQG_U8(r, 8), DQG_U8(r, 16), DQG_U8(r, 24));
 }
 
+// Two fp32 operations in one instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n\t.reg .b64 a, b, c, d;\n\t"
+      "mov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
+      "fma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 a, b, d;\n\t"
+      "mov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+      "add.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+
 // ---------------------------------------------------------------- schedule
 // sum over i in [0, n) of floor((a i + b) / m), by the Euclid-like recursion
 // on (a, m) (lattice points under a line).
@@ -176,20 +199,21 @@ __device__ __forceinline__ int limit_of(const Params& p, const Seq& s, int i) {
   return lim < 0 ? 0 : lim;
 }
 
-// Blocks of a sequence's first n pairs, for one KV head.
-__device__ __forceinline__ long long blocks_before(const Params& p, const Seq& s, int n) {
+// Units of a sequence's first n pairs, for one KV head: their blocks, and
+// kItemUnits for each pair's start and end.
+__device__ __forceinline__ long long units_before(const Params& p, const Seq& s, int n) {
   if (n <= 0) return 0;
   const int last = blocks_of(s.kv);
-  if (!p.causal) return static_cast<long long>(n) * last;
+  if (!p.causal) return static_cast<long long>(n) * (last + kItemUnits);
   const long long tokens = 2 * p.tq, off = s.kv - s.ql;
   const int full = n < s.pairs ? n : s.pairs - 1;  // the last pair ends at kv
   long long one = off <= kBlock ? (kBlock - off) / tokens : 0;  // pairs that see one block at most
   if (one > full) one = full;
   return one + floor_sum(full - one, kBlock, tokens, off + (one + 1) * tokens + kBlock - 1) +
-         (n == s.pairs ? last : 0);
+         (n == s.pairs ? last : 0) + static_cast<long long>(n) * kItemUnits;
 }
 
-struct Share {  // a CTA's part of the blocks
+struct Share {  // a CTA's part of the units; x: the first one's place in its item
   int b, kvh, pair, x, ctas;
   long long count, pos, total;
 };
@@ -202,7 +226,7 @@ __device__ __forceinline__ Share find_share(const Params& p, int cta, int n_ctas
     const int b = b0 + lane;
     if (b < p.B) {
       const Seq s = load_seq(p, b);
-      total += blocks_before(p, s, s.pairs);
+      total += units_before(p, s, s.pairs);
     }
   }
 #pragma unroll
@@ -222,7 +246,7 @@ __device__ __forceinline__ Share find_share(const Params& p, int cta, int n_ctas
     long long mine = 0;
     if (b < p.B) {
       const Seq s = load_seq(p, b);
-      mine = blocks_before(p, s, s.pairs);
+      mine = units_before(p, s, s.pairs);
     }
     long long sum = mine * p.hkv;
 #pragma unroll
@@ -244,12 +268,12 @@ __device__ __forceinline__ Share find_share(const Params& p, int cta, int n_ctas
       while (hi - lo > 1) {
         const int step = (hi - lo + 31) / 32;
         const int probe = min(lo + (lane + 1) * step, hi);
-        const int f = __ffs(__ballot_sync(0xffffffffu, blocks_before(p, s, probe) > in)) - 1;
+        const int f = __ffs(__ballot_sync(0xffffffffu, units_before(p, s, probe) > in)) - 1;
         hi = min(lo + (f + 1) * step, hi);
         lo = lo + f * step;
       }
       r.pair = lo;
-      r.x = static_cast<int>(in - blocks_before(p, s, lo));
+      r.x = static_cast<int>(in - units_before(p, s, lo));
       break;
     }
     before += __shfl_sync(0xffffffffu, sum, 31);
@@ -257,20 +281,21 @@ __device__ __forceinline__ Share find_share(const Params& p, int cta, int n_ctas
   return r;
 }
 
-// What a CTA does next: blocks [x0, x1) of one item.
+// What a CTA does next: blocks [x0, x1) of one item. The copying warp walks
+// the CTA's share and describes each segment to the other warps.
 struct Segment {
-  int b, kvh, tok0, ntok, first, x0, x1, slot;  // first: the pair's first token in its sequence
-  int n0, n1;                                   // the tiles' blocks over the whole item
-  int kv, lim0;                                 // keys; keys that the first token sees (or below 0)
-  bool whole, causal;
-  int pieces;                                   // of the item, where this is the first of several
-  __device__ __forceinline__ int count(int t) const {
-    const int n = t ? n1 : n0, e = x1 < n ? x1 : n;
-    return e > x0 ? e - x0 : 0;
-  }
+  int kvh, tok0, ntok, x0, x1, slot;  // tok0, ntok: the pair's tokens, rows of q
+  int n0, n1;                         // the tiles' blocks over the whole item; n1 = 0: no second tile
+  int kv, lim0;                       // keys; keys that the first token sees (or below 0)
+  int whole;                          // the item lies in this segment
+  int pieces;                         // of the item, where this is the first of several
 };
+// Blocks of a segment that tile t takes part in.
+__device__ __forceinline__ int tile_count(const Segment& g, int t) {
+  const int n = t ? g.n1 : g.n0;
+  return max(0, min(g.x1, n) - g.x0);
+}
 
-// Walks a CTA's share; every role of the CTA walks it alike.
 struct Walk {
   Share r;
   Seq s;
@@ -281,69 +306,73 @@ struct Walk {
     if (p.splits || r.count > 0) s = load_seq(p, p.splits ? 0 : r.b);
   }
   __device__ __forceinline__ void tiles(const Params& p, Segment& g, int pair) {
-    g.first = pair * 2 * p.tq;
-    g.tok0 = s.q0 + g.first;
-    g.ntok = min(2 * p.tq, s.ql - g.first);
-    g.n0 = blocks_of(limit_of(p, s, g.first + min(p.tq, g.ntok) - 1));
-    g.n1 = g.ntok > p.tq ? blocks_of(limit_of(p, s, g.first + g.ntok - 1)) : 0;
+    const int first = pair * 2 * p.tq;  // the pair's first token in its sequence
+    g.tok0 = s.q0 + first;
+    g.ntok = min(2 * p.tq, s.ql - first);
+    g.n0 = blocks_of(limit_of(p, s, first + min(p.tq, g.ntok) - 1));
+    g.n1 = g.ntok > p.tq ? blocks_of(limit_of(p, s, first + g.ntok - 1)) : 0;
     g.kv = s.kv;
-    g.causal = p.causal;
-    g.lim0 = s.kv - s.ql + g.first + 1;
+    g.lim0 = s.kv - s.ql + first + 1;
   }
-  __device__ __forceinline__ bool next(const Params& p, Segment& g) {
+  __device__ __forceinline__ bool next(const Params& p, Segment& g, int& b) {
     if (p.splits) {
       if (piece >= p.n_pieces) return false;
       const int item = piece / p.splits, sp = piece - item * p.splits;
       const int pair = item / p.hkv;
-      g.b = 0;
+      b = 0;
       g.kvh = item - pair * p.hkv;
       tiles(p, g, pair);
       const int n = g.n0;  // both tiles see every key
       g.x0 = static_cast<int>(static_cast<long long>(sp) * n / p.splits);
       g.x1 = static_cast<int>(static_cast<long long>(sp + 1) * n / p.splits);
-      g.whole = false;
+      g.whole = 0;
       g.pieces = 0;
       g.slot = piece;
       piece += gridDim.x;
       return true;
     }
-    if (r.count <= 0) return false;
-    g.b = r.b;
-    g.kvh = r.kvh;
-    tiles(p, g, r.pair);
-    const int n = max(g.n0, g.n1);
-    g.x0 = r.x;
-    g.x1 = r.x + static_cast<int>(min(static_cast<long long>(n - r.x), r.count));
-    g.whole = g.x0 == 0 && g.x1 == n;
-    g.slot = 2 * blockIdx.x + (g.x0 > 0 ? 0 : 1);
-    g.pieces = 0;
-    if (!g.whole && g.x0 == 0)
-      g.pieces = static_cast<int>(((r.pos + n) * r.ctas - 1) / r.total) - static_cast<int>(blockIdx.x) + 1;
-    r.pos += g.x1 - g.x0;
-    r.count -= g.x1 - g.x0;
-    r.x = 0;
-    if (r.count > 0 && ++r.pair == s.pairs) {
-      r.pair = 0;
-      if (++r.kvh == p.hkv) {
-        r.kvh = 0;
-        do {
-          s = load_seq(p, ++r.b);
-        } while (s.pairs == 0);  // a share never ends in sequences without rows
+    while (r.count > 0) {
+      b = r.b;
+      g.kvh = r.kvh;
+      tiles(p, g, r.pair);
+      const int n = max(g.n0, g.n1);
+      const int end = r.x + static_cast<int>(min(static_cast<long long>(n + kItemUnits - r.x), r.count));
+      g.x0 = max(0, r.x - kItemUnits);
+      g.x1 = max(0, end - kItemUnits);
+      g.whole = g.x0 == 0 && g.x1 == n;
+      g.slot = 2 * blockIdx.x + (g.x0 > 0 ? 0 : 1);
+      g.pieces = 0;
+      const long long item_end = r.pos - r.x + n + kItemUnits;
+      if (!g.whole && g.x0 == 0 && g.x1 > 0)
+        g.pieces = static_cast<int>((item_end * r.ctas - 1) / r.total) - static_cast<int>(blockIdx.x) + 1;
+      r.pos += end - r.x;
+      r.count -= end - r.x;
+      r.x = 0;
+      if (r.count > 0 && ++r.pair == s.pairs) {
+        r.pair = 0;
+        if (++r.kvh == p.hkv) {
+          r.kvh = 0;
+          do {
+            s = load_seq(p, ++r.b);
+          } while (s.pairs == 0);  // a share never ends in sequences without rows
+        }
       }
+      if (g.x1 > g.x0) return true;
     }
-    return true;
+    return false;
   }
 };
 
 // ------------------------------------------------------------------ kernel
 template <int D>
 struct Layout {
-  static constexpr int kStages = D == 128 ? 5 : 8;     // key or value blocks in flight
+  static constexpr int kStages = D == 128 ? 4 : 8;     // key or value blocks in flight
   static constexpr int kSlot = kBlock * D * 2;
   static constexpr int kTile = 128 * D * 2;            // a tile's queries
   static constexpr int kRing = 2 * kTile;              // offset of the ring
-  static constexpr int kBars = kRing + kStages * kSlot;
-  static constexpr int kSmem = 1024 + kBars + 512;
+  static constexpr int kStore = kRing + kStages * kSlot;  // 4 KB a softmax warp, for its stores
+  static constexpr int kBars = kStore + 8 * 4096;
+  static constexpr int kSmem = 1024 + kBars + 768;
 };
 
 template <typename E, int D>
@@ -359,12 +388,16 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* empty = full + kStages;
   uint64_t* q_full = empty + kStages;
   uint64_t* q_empty = q_full + 1;
-  uint64_t* s_full = q_empty + 1;        // [2]
-  uint64_t* p_full = s_full + 2;
+  uint64_t* s_full = q_empty + 1;        // [2], one a tile
+  uint64_t* p_half = s_full + 2;
+  uint64_t* p_full = p_half + 2;
   uint64_t* o_full = p_full + 2;
-  uint64_t* drained = o_full + 2;
+  uint64_t* seg_full = o_full + 2;       // [kSegs]
+  uint64_t* seg_empty = seg_full + kSegs;
+  uint64_t* drained = seg_empty + kSegs;
   Share* share = reinterpret_cast<Share*>(drained + 1);
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(share + 1);
+  Segment* segs = reinterpret_cast<Segment*>(share + 1);  // [kSegs]
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(segs + kSegs);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t sbase = smem_u32(smem);
 
@@ -377,8 +410,13 @@ __global__ void __launch_bounds__(kThreads, 1)
     mbar_init(q_empty, 1);
     for (int t = 0; t < 2; ++t) {
       mbar_init(s_full + t, 1);
+      mbar_init(p_half + t, 128);
       mbar_init(p_full + t, 128);
       mbar_init(o_full + t, 1);
+    }
+    for (int i = 0; i < kSegs; ++i) {
+      mbar_init(seg_full + i, 1);
+      mbar_init(seg_empty + i, 9);
     }
     mbar_init(drained, 1);
     fence_mbar_init();
@@ -417,15 +455,25 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (warp >= 8) {
   asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
   if (warp == kCopyWarp) {
+    // ---- copies: queries per segment, then key and value blocks in turn.
     Walk walk;
     walk.begin(p, *share);
     Segment g;
-    // ---- copies: queries per segment, then key and value blocks in turn.
     const int per = p.box_rows, boxes = kBlock / per * (D / 64);
     const int half = lane % (D / 64), sub = lane / (D / 64);
     int seg = 0, pos = 0;
     bool ok = true;
-    while (ok && walk.next(p, g)) {
+    while (ok) {
+      int b = 0;
+      const bool more = walk.next(p, g, b);
+      const int sg = seg % kSegs;
+      if (seg >= kSegs && !warp_wait(seg_empty + sg, ((seg / kSegs) & 1) ^ 1)) break;
+      if (lane == 0) {
+        if (!more) g.x0 = g.x1 = 0;  // the end
+        segs[sg] = g;
+        mbar_arrive(seg_full + sg);
+      }
+      if (!more) break;
       if (seg > 0 && !warp_wait(q_empty, (seg - 1) & 1)) break;
       const int tiles = g.n1 > 0 ? 2 : 1;
       if (lane == 0) mbar_arrive_expect_tx(q_full, tiles * used * D * 2);
@@ -435,8 +483,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         tma_load_4d(sbase + t * L::kTile + h * (128 * 128), &qmap, q_full, h * 64, 0, g.kvh, g.tok0 + t * p.tq);
       }
       ++seg;
-      const int32_t* row = p.table + g.b * p.table_stride;
-      if (!p.splits && lane == 0 && __ldg(p.lens + g.b) != g.kv) atomicOr(&g_status, kStatusBadIndex);
+      const int32_t* row = p.table + b * p.table_stride;
+      if (!p.splits && lane == 0 && __ldg(p.lens + b) != g.kv) atomicOr(&g_status, kStatusBadIndex);
       for (int x = g.x0; x < g.x1 && ok; ++x) {
         const int t = x * kBlock + sub * per;
         int page = static_cast<int>(p.n_pages);  // no such page: zeros
@@ -469,9 +517,6 @@ __global__ void __launch_bounds__(kThreads, 1)
   } else if (warp == kMmaWarp) {
     // ---- products: one thread.
     if (lane == 0) {
-      Walk walk;
-      walk.begin(p, *share);
-      Segment g;
       constexpr uint32_t kIdS = instr_desc(Elem<E>::kFormat, kBlock, false);
       constexpr uint32_t kIdO = instr_desc(Elem<E>::kFormat, D, true);
       auto slot_addr = [&](int pos) { return sbase + L::kRing + (pos % kStages) * L::kSlot; };
@@ -484,12 +529,14 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         mma_commit(s_full + t);
       };
-      auto issue_o = [&](int t, int pos, bool add) {
+      auto issue_o = [&](int t, int pos, int half, bool add) {
         const uint32_t b = slot_addr(pos);
 #pragma unroll
-        for (int k = 0; k < kBlock / 16; ++k)
+        for (int i = 0; i < kBlock / 32; ++i) {
+          const int k = half * (kBlock / 32) + i;
           mma_ts(tmem + 2 * kBlock + t * D, tmem + t * kBlock + k * 8,
                  smem_desc(b + k * 16 * 128, kBlock * 128, 1024), kIdO, add || k > 0);
+        }
       };
       auto wait_full = [&](int pos) {
         if (!mbar_wait(full + pos % kStages, (pos / kStages) & 1)) return false;
@@ -499,9 +546,13 @@ __global__ void __launch_bounds__(kThreads, 1)
       int seg = 0, base = 0;
       uint32_t weights = 0;  // parities of the two p_full barriers
       bool ok = true;
-      while (ok && walk.next(p, g)) {
-        const int c0 = g.count(0), c1 = g.count(1);
-        const int n = g.x1 - g.x0;
+      while (ok) {
+        const int sg = seg % kSegs;
+        if (!mbar_wait(seg_full + sg, (seg / kSegs) & 1)) break;
+        const int c0 = tile_count(segs[sg], 0), c1 = tile_count(segs[sg], 1);
+        const int n = segs[sg].x1 - segs[sg].x0;
+        if (n == 0) break;
+        mbar_arrive(seg_empty + sg);
         ok = mbar_wait(q_full, seg & 1) && wait_full(base);
         ++seg;
         if (!ok) break;
@@ -517,11 +568,15 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int t = 0; t < 2; ++t) {
             const int c = t ? c1 : c0;
             if (!ok || j >= c) continue;
+            ok = mbar_wait(p_half + t, weights >> t & 1);
+            if (!ok) continue;
+            fence_after_sync();
+            issue_o(t, vpos, 0, j > 0);
             ok = mbar_wait(p_full + t, weights >> t & 1);
             weights ^= 1u << t;
             if (!ok) continue;
             fence_after_sync();
-            issue_o(t, vpos, j > 0);
+            issue_o(t, vpos, 1, true);
             if (j + 1 < c) issue_s(t, kpos);
             else mma_commit(o_full + t);
           }
@@ -539,26 +594,27 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
-    Walk walk;
-    walk.begin(p, *share);
-    Segment g;
     // ---- softmax: one thread a row of tile t.
     const int t = warp >> 2, r = threadIdx.x & 127;
     const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;  // this warp's 32 lanes
     const uint32_t ts = tmem + lanes + t * kBlock, to = tmem + lanes + 2 * kBlock + t * D;
-    const int tok = r / p.g, head = r - tok * p.g;  // of the tile
-    int scores = 0, outs = 0, base = 0;
+    const int tok = t * p.tq + r / p.g;  // of the pair
+    const float2 scale2 = make_float2(p.scale_log2, p.scale_log2);
+    int seg = 0, scores = 0, outs = 0, base = 0;
     bool ok = true, cut_first = false;
-    while (ok && walk.next(p, g)) {
-      const int n = g.count(t);
-      const int tile_n = t ? g.n1 : g.n0;  // 0: a tile without rows
-      const bool live = r < used && t * p.tq + tok < g.ntok;
-      const int limit = g.causal ? min(g.lim0 + t * p.tq + tok, g.kv) : g.kv;
+    while (true) {
+      const int sg = seg % kSegs;
+      if (!warp_wait(seg_full + sg, (seg / kSegs) & 1)) break;
+      const Segment& g = segs[sg];
+      const int x0 = g.x0, kv = g.kv, n = tile_count(g, t), all = g.x1 - x0;
+      if (all == 0) break;
+      ++seg;
+      const int limit = p.causal ? min(g.lim0 + tok, kv) : kv;
       // Keys that every row of the tile sees (rows past the end see no fewer).
-      const int seen = g.causal ? g.lim0 + t * p.tq : g.kv;
+      const int seen = p.causal ? g.lim0 + t * p.tq : kv;
       float m = -INFINITY, l = 0.f;
       for (int j = 0; j < n; ++j) {
-        const int k0 = (g.x0 + j) * kBlock;
+        const int k0 = (x0 + j) * kBlock;
         if (!warp_wait(s_full + t, scores & 1)) {
           ok = false;
           break;
@@ -601,31 +657,15 @@ __global__ void __launch_bounds__(kThreads, 1)
           l *= f;
           if (grow) m = m_new;
         }
-        const float ref = m == -INFINITY ? 0.f : m * p.scale_log2;
-        float sum[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int hq = 0; hq < 2; ++hq) {
-          uint32_t w[32];
-#pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            const float a = exp2_approx(fmaf(s[64 * hq + 2 * i], p.scale_log2, -ref));
-            const float b = exp2_approx(fmaf(s[64 * hq + 2 * i + 1], p.scale_log2, -ref));
-            sum[(2 * i) & 3] += a;
-            sum[(2 * i + 1) & 3] += b;
-            w[i] = Elem<E>::pack(a, b);
-          }
-          tmem_st32(ts + 32 * hq, w);
-        }
-        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
         // Behind the sequence's end its last page holds anything: zero those
         // values (a zero weight times an infinity would not be zero).
-        if (k0 + kBlock > g.kv && g.kv > k0 && (g.kv & ((1 << p.page_shift) - 1))) {
+        if (k0 + kBlock > kv && kv > k0 && (kv & ((1 << p.page_shift) - 1))) {
           const int vpos = base + 2 * j + 1;
           if (!warp_wait(full + vpos % kStages, (vpos / kStages) & 1)) {
             ok = false;
             break;
           }
-          const int r0 = g.kv - k0;
+          const int r0 = kv - k0;
           const int r1 = min(kBlock, ((r0 >> p.page_shift) + 1) << p.page_shift);
           uint8_t* v = smem + L::kRing + (vpos % kStages) * L::kSlot;
           for (int i = r; i < (r1 - r0) * (D / 8); i += 128) {
@@ -635,11 +675,30 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           fence_async_shared();
         }
-        tmem_wait_st();
-        fence_before_sync();
-        mbar_arrive(p_full + t);
+        const float ref = m == -INFINITY ? 0.f : m * p.scale_log2;
+        const float2 ref2 = make_float2(-ref, -ref);
+        float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+        // The products take the first half of the weights while the second is
+        // still being formed.
+#pragma unroll
+        for (int hq = 0; hq < 2; ++hq) {
+          uint32_t w[32];
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            float2 x = fma2(make_float2(s[64 * hq + 2 * i], s[64 * hq + 2 * i + 1]), scale2, ref2);
+            x.x = exp2_approx(x.x);
+            x.y = exp2_approx(x.y);
+            sum[i & 1] = add2(sum[i & 1], x);
+            w[i] = Elem<E>::pack(x.x, x.y);
+          }
+          tmem_st32(ts + 32 * hq, w);
+          tmem_wait_st();
+          fence_before_sync();
+          mbar_arrive((hq ? p_full : p_half) + t);
+        }
+        l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
       }
-      base += 2 * (g.x1 - g.x0);
+      base += 2 * all;
       if (!ok) break;
       if (g.pieces && threadIdx.x == 0) p.desc[blockIdx.x] = Desc{g.tok0, g.ntok, g.kvh, g.pieces};
       cut_first |= g.pieces != 0;
@@ -648,46 +707,69 @@ __global__ void __launch_bounds__(kThreads, 1)
         ++outs;
         fence_after_sync();
       }
-      const float inv = l == 0.f ? 0.f : __frcp_rn(l);
-      E* out = static_cast<E*>(p.out) +
-               (static_cast<int64_t>(g.tok0 + t * p.tq + tok) * p.hq + g.kvh * p.g + head) * D;
-      const int64_t slot = g.slot;
-      if (!g.whole && tile_n > 0) {
-        p.ml[slot * 512 + t * 128 + r] = n > 0 && m != -INFINITY ? m * p.scale_log2 : -INFINITY;
-        p.ml[slot * 512 + 256 + t * 128 + r] = l;
-      }
-      if (tile_n > 0) {
+      if ((t ? g.n1 : g.n0) > 0) {
+        if (g.whole) {
+          // 64 columns at a time through shared memory, so that a warp's
+          // stores are whole 128-byte rows.
+          const float inv = l == 0.f ? 0.f : __frcp_rn(l);
+          uint8_t* st = smem + L::kStore + warp * 4096;
+          E* out = static_cast<E*>(p.out) + static_cast<int64_t>(g.tok0) * p.hq * D + static_cast<int64_t>(g.kvh) * p.g * D;
 #pragma unroll
-        for (int q = 0; q < D / 32; ++q) {
-          uint32_t o[32];
-          if (n > 0) {
-            tmem_ld32(to + 32 * q, o);
+          for (int h = 0; h < D / 64; ++h) {
+            uint32_t o[64];
+            tmem_ld32(to + 64 * h, o);
+            tmem_ld32(to + 64 * h + 32, o + 32);
             tmem_wait_ld();
             hold32(o);
-          } else {
+            hold32(o + 32);
 #pragma unroll
-            for (int i = 0; i < 32; ++i) o[i] = 0u;
+            for (int i = 0; i < 8; ++i) {
+              uint4 w;
+              uint32_t* ww = reinterpret_cast<uint32_t*>(&w);
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                ww[e] = Elem<E>::pack(__uint_as_float(o[8 * i + 2 * e]) * inv,
+                                      __uint_as_float(o[8 * i + 2 * e + 1]) * inv);
+              *reinterpret_cast<uint4*>(st + lane * 128 + ((i ^ (lane & 7)) << 4)) = w;
+            }
+            __syncwarp();
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const int row = i * 4 + (lane >> 3), rr = (warp & 3) * 32 + row;
+              const int tk = fast_div(rr, p.g_magic), head = rr - tk * p.g;
+              if (rr < used && t * p.tq + tk < g.ntok)
+                *reinterpret_cast<uint4*>(out + (static_cast<int64_t>(t * p.tq + tk) * p.hq + head) * D + 64 * h +
+                                          (lane & 7) * 8) =
+                    *reinterpret_cast<const uint4*>(st + row * 128 + (((lane & 7) ^ (row & 7)) << 4));
+            }
+            __syncwarp();
           }
-          if (!g.whole) {
+        } else {
+          const int64_t slot = g.slot;
+          p.ml[slot * 512 + t * 128 + r] = n > 0 && m != -INFINITY ? m * p.scale_log2 : -INFINITY;
+          p.ml[slot * 512 + 256 + t * 128 + r] = l;
+#pragma unroll
+          for (int q = 0; q < D / 32; ++q) {
+            uint32_t o[32];
+            if (n > 0) {
+              tmem_ld32(to + 32 * q, o);
+              tmem_wait_ld();
+              hold32(o);
+            } else {
+#pragma unroll
+              for (int i = 0; i < 32; ++i) o[i] = 0u;
+            }
 #pragma unroll
             for (int i = 0; i < 8; ++i)
               p.part[(slot * (D / 4) + q * 8 + i) * 256 + t * 128 + r] =
                   make_float4(__uint_as_float(o[4 * i]), __uint_as_float(o[4 * i + 1]),
                               __uint_as_float(o[4 * i + 2]), __uint_as_float(o[4 * i + 3]));
-          } else if (live) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              uint4 w;
-              uint32_t* ww = reinterpret_cast<uint32_t*>(&w);
-#pragma unroll
-              for (int e = 0; e < 4; ++e)
-                ww[e] = Elem<E>::pack(__uint_as_float(o[8 * i + 2 * e]) * inv, __uint_as_float(o[8 * i + 2 * e + 1]) * inv);
-              *reinterpret_cast<uint4*>(out + 32 * q + 8 * i) = w;
-            }
           }
         }
       }
       fence_before_sync();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(seg_empty + sg);
     }
     if (threadIdx.x == 0 && !cut_first && !p.splits) p.desc[blockIdx.x] = Desc{0, 0, 0, 0};
   }
@@ -836,6 +918,7 @@ cudaError_t launch_prompt(const PagedPool& pool, const CUtensorMap& qmap, const 
   p.hkv = pool.n_kv_heads;
   p.g = a.hq / pool.n_kv_heads;
   p.tq = prompt_tokens_per_tile(a.hq, pool.n_kv_heads);
+  p.g_magic = p.g > 1 ? static_cast<uint32_t>(((uint64_t(1) << 32) + p.g - 1) / p.g) : 0;
   p.page_shift = 0;
   while ((1 << p.page_shift) < pool.page_size) ++p.page_shift;
   const int64_t limit = static_cast<int64_t>(a.table_width) * pool.page_size;
