@@ -94,6 +94,11 @@ __device__ __forceinline__ void mma_commit(uint64_t* bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
                : "memory");
 }
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+  return p != 0;
+}
 __device__ __forceinline__ void fence_before_sync() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_after_sync() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 
@@ -515,82 +520,98 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int i = pos < kStages ? 0 : pos - kStages; i < pos; ++i)
       if (!warp_wait(full + i % kStages, (i / kStages) & 1)) break;
   } else if (warp == kMmaWarp) {
-    // ---- products: one thread.
-    if (lane == 0) {
-      constexpr uint32_t kIdS = instr_desc(Elem<E>::kFormat, kBlock, false);
-      constexpr uint32_t kIdO = instr_desc(Elem<E>::kFormat, D, true);
-      auto slot_addr = [&](int pos) { return sbase + L::kRing + (pos % kStages) * L::kSlot; };
-      auto issue_s = [&](int t, int pos) {
-        const uint32_t a = sbase + t * L::kTile, b = slot_addr(pos);
+    // ---- products: one thread issues them, the warp walks alike (its
+    // addresses and descriptors then live in uniform registers).
+    constexpr uint32_t kIdS = instr_desc(Elem<E>::kFormat, kBlock, false);
+    constexpr uint32_t kIdO = instr_desc(Elem<E>::kFormat, D, true);
+    const bool one = elect_one();
+    const uint64_t q_desc = smem_desc(sbase, 16, 1024);
+    const uint64_t k_desc = smem_desc(sbase + L::kRing, 16, 1024);
+    const uint64_t v_desc = smem_desc(sbase + L::kRing, kBlock * 128, 1024);
+    auto issue_s = [&](int t, int slot) {
+      if (!one) return;
+      const uint64_t a = q_desc + t * (L::kTile >> 4), b = k_desc + slot * (L::kSlot >> 4);
 #pragma unroll
-        for (int k = 0; k < D / 16; ++k) {
-          const uint32_t off = (k / 4) * (128 * 128) + (k % 4) * 32;
-          mma_ss(tmem + t * kBlock, smem_desc(a + off, 16, 1024), smem_desc(b + off, 16, 1024), kIdS, k > 0);
-        }
-        mma_commit(s_full + t);
-      };
-      auto issue_o = [&](int t, int pos, int half, bool add) {
-        const uint32_t b = slot_addr(pos);
-#pragma unroll
-        for (int i = 0; i < kBlock / 32; ++i) {
-          const int k = half * (kBlock / 32) + i;
-          mma_ts(tmem + 2 * kBlock + t * D, tmem + t * kBlock + k * 8,
-                 smem_desc(b + k * 16 * 128, kBlock * 128, 1024), kIdO, add || k > 0);
-        }
-      };
-      auto wait_full = [&](int pos) {
-        if (!mbar_wait(full + pos % kStages, (pos / kStages) & 1)) return false;
-        fence_after_sync();
-        return true;
-      };
-      int seg = 0, base = 0;
-      uint32_t weights = 0;  // parities of the two p_full barriers
-      bool ok = true;
-      while (ok) {
-        const int sg = seg % kSegs;
-        if (!mbar_wait(seg_full + sg, (seg / kSegs) & 1)) break;
-        const int c0 = tile_count(segs[sg], 0), c1 = tile_count(segs[sg], 1);
-        const int n = segs[sg].x1 - segs[sg].x0;
-        if (n == 0) break;
-        mbar_arrive(seg_empty + sg);
-        ok = mbar_wait(q_full, seg & 1) && wait_full(base);
-        ++seg;
-        if (!ok) break;
-        fence_after_sync();
-        if (c0 > 0) issue_s(0, base);
-        if (c1 > 0) issue_s(1, base);
-        mma_commit(empty + base % kStages);
-        if (n == 1) mma_commit(q_empty);
-        for (int j = 0; j < n && ok; ++j) {
-          const int vpos = base + 2 * j + 1, kpos = vpos + 1;
-          ok = wait_full(vpos) && (j + 1 == n || wait_full(kpos));
-#pragma unroll
-          for (int t = 0; t < 2; ++t) {
-            const int c = t ? c1 : c0;
-            if (!ok || j >= c) continue;
-            ok = mbar_wait(p_half + t, weights >> t & 1);
-            if (!ok) continue;
-            fence_after_sync();
-            issue_o(t, vpos, 0, j > 0);
-            ok = mbar_wait(p_full + t, weights >> t & 1);
-            weights ^= 1u << t;
-            if (!ok) continue;
-            fence_after_sync();
-            issue_o(t, vpos, 1, true);
-            if (j + 1 < c) issue_s(t, kpos);
-            else mma_commit(o_full + t);
-          }
-          mma_commit(empty + vpos % kStages);
-          if (j + 1 < n) mma_commit(empty + kpos % kStages);
-          if (j + 2 == n) mma_commit(q_empty);
-        }
-        base += 2 * n;
+      for (int k = 0; k < D / 16; ++k) {
+        const uint32_t off = ((k / 4) * (128 * 128) + (k % 4) * 32) >> 4;
+        mma_ss(tmem + t * kBlock, a + off, b + off, kIdS, k > 0);
       }
-      // Nothing of this CTA is in flight when it ends (bounded).
-      mma_commit(drained);
-      mbar_wait(drained, 0);
+      mma_commit(s_full + t);
+    };
+    auto issue_o = [&](int t, int slot, int half, bool add) {
+      if (!one) return;
+      const uint64_t b = v_desc + slot * (L::kSlot >> 4);
+#pragma unroll
+      for (int i = 0; i < kBlock / 32; ++i) {
+        const int k = half * (kBlock / 32) + i;
+        mma_ts(tmem + 2 * kBlock + t * D, tmem + t * kBlock + k * 8, b + (k * 16 * 128 >> 4), kIdO, add || k > 0);
+      }
+    };
+    auto commit = [&](uint64_t* bar) {
+      if (one) mma_commit(bar);
+    };
+    auto wait = [&](uint64_t* bar, uint32_t parity) {
+      const bool ok = warp_wait(bar, parity);
+      fence_after_sync();
+      return ok;
+    };
+    int seg = 0, slot = 0;
+    uint32_t ring = 0, weights = 0;  // parities: the ring's, the two tiles' weights
+    auto advance = [&] {
+      if (++slot == kStages) {
+        slot = 0;
+        ring ^= 1;
+      }
+    };
+    bool ok = true;
+    while (ok) {
+      const int sg = seg % kSegs;
+      if (!warp_wait(seg_full + sg, (seg / kSegs) & 1)) break;
+      const int c0 = tile_count(segs[sg], 0), c1 = tile_count(segs[sg], 1);
+      const int n = segs[sg].x1 - segs[sg].x0;
+      if (n == 0) break;
+      __syncwarp();
+      if (one) mbar_arrive(seg_empty + sg);
+      ok = wait(q_full, seg & 1) && wait(full + slot, ring);
+      ++seg;
+      if (!ok) break;
+      if (c0 > 0) issue_s(0, slot);
+      if (c1 > 0) issue_s(1, slot);
+      commit(empty + slot);
+      if (n == 1) commit(q_empty);
+      advance();
+      for (int j = 0; j < n && ok; ++j) {
+        const int vslot = slot;
+        const bool more = j + 1 < n;
+        ok = wait(full + vslot, ring);
+        advance();
+        const int kslot = slot;
+        if (ok && more) {
+          ok = wait(full + kslot, ring);
+          advance();
+        }
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          const int c = t ? c1 : c0;
+          if (!ok || j >= c) continue;
+          ok = wait(p_half + t, weights >> t & 1);
+          if (!ok) continue;
+          issue_o(t, vslot, 0, j > 0);
+          ok = wait(p_full + t, weights >> t & 1);
+          weights ^= 1u << t;
+          if (!ok) continue;
+          issue_o(t, vslot, 1, true);
+          if (j + 1 < c) issue_s(t, kslot);
+          else commit(o_full + t);
+        }
+        commit(empty + vslot);
+        if (more) commit(empty + kslot);
+        if (j + 2 == n) commit(q_empty);
+      }
     }
-    __syncwarp();
+    // Nothing of this CTA is in flight when it ends (bounded).
+    commit(drained);
+    warp_wait(drained, 0);
   }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
