@@ -115,7 +115,7 @@ def lib() -> ctypes.CDLL:
     h.dqg_rope_paged_append.argtypes = [vp, i64, i64, i64, vp, vp, i64, i64, i32, vp, vp, vp, vp,
                                         f32, kv, vp, vp]
     h.dqg_paged_attention_workspace.restype = i32
-    h.dqg_paged_attention_workspace.argtypes = [i64, u64p]
+    h.dqg_paged_attention_workspace.argtypes = [i64, i64, i64, i64, u64p]
     h.dqg_paged_attention.restype = i32
     h.dqg_paged_attention.argtypes = [vp, i64, i64, i64, i64, kv, vp, i64, i64, vp, f32, vp, vp,
                                       u64, vp]

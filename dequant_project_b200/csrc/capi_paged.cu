@@ -236,15 +236,9 @@ int dqg_rope_paged_append(const void* qkv, int64_t T, int64_t qkv_stride, int64_
   return api_ok();
 }
 
-int dqg_paged_attention_workspace(int64_t head_dim, uint64_t* bytes) {
-  if (bytes == nullptr) return api_fail(DQG_ERR_INVALID, "bytes must not be null");
-  if (head_dim != 64 && head_dim != 128)
-    return api_fail(DQG_ERR_UNSUPPORTED, "paged operators handle head_dim 64 and 128, got %lld", (ll)head_dim);
-  int dev = 0, sms = 0;
-  const int rc = current(&dev, &sms);
-  if (rc) return rc;
-  *bytes = dqg::paged_decode_workspace(static_cast<int>(head_dim), sms);
-  return api_ok();
+int dqg_paged_attention_workspace(int64_t n_seqs, int64_t n_q_heads, int64_t n_kv_heads, int64_t head_dim,
+                                  uint64_t* bytes) {
+  return dqg_shared_prefix_workspace(n_seqs, n_q_heads, n_kv_heads, head_dim, 0, bytes);
 }
 
 int dqg_paged_attention(const void* q, int64_t q_stride_seq, int64_t q_stride_head, int64_t n_seqs,
@@ -255,7 +249,7 @@ int dqg_paged_attention(const void* q, int64_t q_stride_seq, int64_t q_stride_he
   int rc = check_pool(kv, &pool);
   if (rc) return rc;
   if ((rc = check_heads(n_q_heads, pool)) != DQG_OK) return rc;
-  if (n_seqs < 0 || n_seqs > (1 << 24))
+  if (n_seqs < 0 || n_seqs > (1 << 20))
     return api_fail(DQG_ERR_INVALID, "n_seqs=%lld out of range", (ll)n_seqs);
   if (n_seqs == 0) return api_ok();
   if ((rc = check_query(q, n_seqs, n_q_heads, q_stride_seq, q_stride_head, pool.D)) != DQG_OK) return rc;
@@ -265,7 +259,8 @@ int dqg_paged_attention(const void* q, int64_t q_stride_seq, int64_t q_stride_he
   if ((rc = check_scale(scale)) != DQG_OK) return rc;
   int dev = 0, sms = 0;
   if ((rc = current(&dev, &sms)) != DQG_OK) return rc;
-  if ((rc = check_workspace(workspace, workspace_bytes, dqg::paged_decode_workspace(pool.D, sms))) != DQG_OK)
+  if ((rc = check_workspace(workspace, workspace_bytes, dqg::paged_decode_workspace(static_cast<int>(n_seqs), static_cast<int>(n_q_heads), pool.n_kv_heads,
+                                                    pool.D, false, sms))) != DQG_OK)
     return rc;
   CUtensorMap kmap, vmap;
   if ((rc = pool_maps(pool, dqg::paged_decode_box_rows(pool.page_size), &kmap, &vmap)) != DQG_OK) return rc;
@@ -361,8 +356,10 @@ int dqg_shared_prefix_workspace(int64_t n_seqs, int64_t n_q_heads, int64_t n_kv_
     return api_fail(DQG_ERR_INVALID, "prefix_len=%lld out of range", (ll)prefix_len);
   int dev = 0, sms = 0;
   if ((rc = current(&dev, &sms)) != DQG_OK) return rc;
-  *bytes = dqg::paged_decode_workspace(static_cast<int>(head_dim), sms);
-  if (prefix_len > 0 && n_seqs > 0)
+  const bool prefix = prefix_len > 0 && n_seqs > 0;
+  *bytes = dqg::paged_decode_workspace(static_cast<int>(n_seqs), static_cast<int>(n_q_heads),
+                                       static_cast<int>(n_kv_heads), static_cast<int>(head_dim), prefix, sms);
+  if (prefix)
     *bytes += dqg::prefix_workspace(static_cast<int>(n_seqs), static_cast<int>(n_q_heads),
                                     static_cast<int>(n_kv_heads), static_cast<int>(head_dim),
                                     static_cast<int>(prefix_len), sms);
@@ -406,8 +403,10 @@ int dqg_shared_prefix_attention(const void* q, int64_t q_stride_seq, int64_t q_s
     a.table = prefix_table;
     a.table_stride = prefix_pages;
     a.table_width = static_cast<int>(prefix_pages);
-    // The decode kernel's scratch has a fixed size: the pieces go behind it.
-    a.workspace = static_cast<uint8_t*>(workspace) + dqg::paged_decode_workspace(pool.D, sms);
+    // The decode kernel's scratch first, the prefix's pieces behind it.
+    a.workspace = static_cast<uint8_t*>(workspace) +
+                  dqg::paged_decode_workspace(static_cast<int>(n_seqs), static_cast<int>(n_q_heads),
+                                              pool.n_kv_heads, pool.D, true, sms);
     a.B = 1;
     a.T = static_cast<int>(n_seqs);
     a.hq = static_cast<int>(n_q_heads);

@@ -58,7 +58,7 @@ struct DecodeArgs {
   float scale_log2;
   PrefixPieces prefix;
 };
-size_t paged_decode_workspace(int D, int num_sms);
+size_t paged_decode_workspace(int B, int hq, int n_kv_heads, int D, bool prefix, int num_sms);
 cudaError_t launch_paged_decode(const PagedPool& pool, const CUtensorMap& kmap,
                                 const CUtensorMap& vmap, const DecodeArgs& a, int num_sms,
                                 cudaStream_t stream);

@@ -18,7 +18,9 @@
 // as the values are) from the score registers. An item (sequence, head) that
 // lies in one share is finished by its CTA; one that is cut leaves a (max, sum,
 // O) piece per CTA in the workspace, and a second small kernel joins the
-// pieces in order. No atomics: the same lengths give the same bits.
+// pieces in order. No atomics: the same lengths give the same bits. Behind a
+// shared prefix every item leaves its result to the second kernel, which joins
+// it with the prefix's pieces: nothing here waits for those.
 #include <cstdint>
 
 #include "paged.cuh"
@@ -31,10 +33,13 @@ constexpr int kWarps = 4;              // consumer warps
 constexpr int kThreads = 32 * (kWarps + 1);
 constexpr int kStages = 3;
 constexpr int kCtasPerSm = 2;
+constexpr int kQuerySlots = 4;         // items whose queries are held at most
 constexpr int kMergeRows = 4;          // query heads per round of the warps' merge
 
-struct Desc {  // a cut item, by the CTA that holds its first piece
-  int b, hv, pieces, pad;
+struct Desc {    // an item that is joined later
+  int b, hv;     // sequence, KV head and 16-row block of its query heads
+  int cta;       // holds the first piece; below 0: the result lies whole in the item's own slot
+  int pieces;    // 0: nothing to join
 };
 
 struct Params {
@@ -42,11 +47,11 @@ struct Params {
   void* out;
   const int32_t* table;
   const int32_t* lens;
-  float* part;   // [CTA][2][16][D]
-  float* ml;     // [CTA][2][2][16]
-  Desc* desc;    // [CTA]
+  float* part;   // [slot][rows][D]; two slots a CTA, then (behind a prefix) one an item
+  float* ml;     // [slot][2][rows]: maximum (log2 units), sum
+  Desc* desc;    // [CTA]; behind a prefix [item]
   int64_t q_stride_seq, q_stride_head, table_stride, n_pages;
-  int B, hq, hkv, g, nrb, page_shift, len_limit, box_rows;
+  int B, hq, hkv, g, nrb, rows, page_shift, len_limit, box_rows, n_ctas;
   float scale_log2;
   PrefixPieces prefix;
 };
@@ -60,33 +65,9 @@ __device__ __forceinline__ int prefix_row(const PrefixPieces& f, int g, int b, i
   return ((b / f.tq) & 1) * 128 + (b % f.tq) * g + j;
 }
 
-// Four outputs of one query head from the item's own (max, sum, O) and the
-// shared prefix's pieces, in piece order.
+// Four outputs of one query head.
 template <typename E, int D>
-__device__ __forceinline__ void finish(const Params& p, int b, int head, int d4, float mx, float den,
-                                       float4 num) {
-  if (p.prefix.S > 0) {
-    const int kvh = head / p.g, row = prefix_row(p.prefix, p.g, b, head % p.g);
-    const int64_t first = prefix_first(p.prefix, p.hkv, b, kvh);
-    const float* ml = p.prefix.ml + first * 512 + row;
-    float m = mx;
-    for (int s = 0; s < p.prefix.S; ++s) m = fmaxf(m, __ldcg(ml + s * 512));
-    const float mu = m == -INFINITY ? 0.f : m;
-    float f = exp2_approx(mx - mu);
-    den *= f;
-    num.x *= f; num.y *= f; num.z *= f; num.w *= f;
-    const float4* po = reinterpret_cast<const float4*>(p.prefix.o) + (first * (D / 4) + d4) * 256 + row;
-#pragma unroll 4
-    for (int s = 0; s < p.prefix.S; ++s) {
-      f = exp2_approx(__ldcg(ml + s * 512) - mu);
-      den = fmaf(__ldcg(ml + s * 512 + 256), f, den);
-      const float4 v = __ldcg(po + static_cast<int64_t>(s) * (D / 4) * 256);
-      num.x = fmaf(v.x, f, num.x);
-      num.y = fmaf(v.y, f, num.y);
-      num.z = fmaf(v.z, f, num.z);
-      num.w = fmaf(v.w, f, num.w);
-    }
-  }
+__device__ __forceinline__ void store4(const Params& p, int b, int head, int d4, float den, float4 num) {
   const float inv = den == 0.f ? 0.f : __frcp_rn(den);
   E* o = static_cast<E*>(p.out) + (static_cast<int64_t>(b) * p.hq + head) * D + d4 * 4;
   uint2 w;
@@ -170,7 +151,8 @@ struct Layout {
   static constexpr int kTileBytes = kTile * D * 2;
   static constexpr int kRing = kStages * 2 * kTileBytes;
   static constexpr int kMerge = kWarps * kMergeRows * D * 4;
-  static constexpr int kSmem = 1024 + kRing + kMerge + kWarps * 16 * 8 + 2 * kStages * 8 + 64;
+  static constexpr int kQuery = 16 * D * 2;
+  static constexpr int kSmem = 1024 + kRing + kMerge + kQuery + kWarps * 16 * 8 + 2 * (kStages + kQuerySlots) * 8 + 64;
 };
 
 template <typename E, int D>
@@ -180,25 +162,39 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
   using L = Layout<D>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
-  float* os = reinterpret_cast<float*>(smem + L::kRing);             // [warp][4][D]
-  float* ms = reinterpret_cast<float*>(smem + L::kRing + L::kMerge);  // [warp][16]
+  // Queries of the items ahead; reads of 16 rows run past a short slot, at
+  // worst into the merge buffer (rows whose results nobody takes).
+  uint8_t* qs = smem + L::kRing;
+  float* os = reinterpret_cast<float*>(qs + L::kQuery);               // [warp][4][D]
+  float* ms = os + L::kMerge / 4;                                     // [warp][16]
   float* ls = ms + kWarps * 16;
   uint64_t* full = reinterpret_cast<uint64_t*>(ls + kWarps * 16);
   uint64_t* empty = full + kStages;
-  Share* share = reinterpret_cast<Share*>(empty + kStages);
+  uint64_t* q_full = empty + kStages;
+  uint64_t* q_empty = q_full + kQuerySlots;
+  Share* share = reinterpret_cast<Share*>(q_empty + kQuerySlots);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int i = 0; i < kStages; ++i) {
       mbar_init(full + i, 1);
       mbar_init(empty + i, kWarps);
     }
+    for (int i = 0; i < kQuerySlots; ++i) {
+      mbar_init(q_full + i, 1);
+      mbar_init(q_empty + i, kWarps);
+    }
     fence_mbar_init();
     tma_prefetch_map(&kmap);
     tma_prefetch_map(&vmap);
   }
+  // Rows that no query head fills stay zero.
+  for (int i = threadIdx.x; i < L::kQuery / 16; i += kThreads) reinterpret_cast<uint4*>(qs)[i] = make_uint4(0, 0, 0, 0);
+  fence_async_shared();
   // After a prefix kernel (which every one of its CTAs lets this one start
   // from only once its own inputs are complete), the queries, pages and
-  // lengths may be read at once; only the prefix's pieces need the wait.
+  // lengths may be read at once; only the end waits (and with it everything
+  // behind this kernel).
+  // waits (and with it everything behind this kernel).
   const bool late = p.prefix.S > 0;
   if (!late) pdl_wait_prior_grid();
   if (warp == 0) {
@@ -209,13 +205,15 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
   pdl_launch_dependents();
   Share s = *share;
   const int n_hv = p.hkv * p.nrb;
+  const int q_slots = min(kQuerySlots, 16 / p.rows);
 
   if (warp == kWarps) {
     // ---- the copying warp: 16-row (or box_rows-row) pieces of page rows.
     const int per = p.box_rows;                 // rows a box
     const int boxes = kTile / per * (D / 64);   // K boxes a tile; as many V boxes
     const int my = lane, half = my % (D / 64), sub = my / (D / 64);
-    int it = 0;
+    const uint64_t policy = policy_evict_last();
+    int it = 0, item = 0;
     bool ok = true;
     while (s.count > 0 && ok) {
       const int raw = __ldg(p.lens + s.b);
@@ -224,7 +222,17 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
       const int nt = tiles_of(len);
       const int n = static_cast<int>(min(static_cast<long long>(nt - s.x), s.count));
       const int32_t* row = p.table + s.b * p.table_stride;
-      const int kvh = s.hv / p.nrb;
+      const int kvh = s.hv / p.nrb, rb = s.hv - kvh * p.nrb;
+      const int rows = min(16, p.g - rb * 16);
+      // The item's queries, a row a lane.
+      const int qi = item % q_slots;
+      if (item >= q_slots && !warp_wait(q_empty + qi, ((item / q_slots) & 1) ^ 1)) break;
+      if (lane == 0) mbar_arrive_expect_tx(q_full + qi, rows * D * 2);
+      __syncwarp();
+      if (lane < rows)
+        bulk_g2s(qs + (qi * p.rows + lane) * D * 2, static_cast<const E*>(p.q) + s.b * p.q_stride_seq +
+                 (kvh * p.g + rb * 16 + lane) * p.q_stride_head, D * 2, q_full + qi, policy);
+      ++item;
       for (int x = s.x; x < s.x + n; ++x, ++it) {
         const int st = it % kStages;
         const int t = x * kTile + sub * per;
@@ -254,13 +262,15 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
       if (++s.hv == n_hv) { s.hv = 0; ++s.b; }
     }
     // Copies still in flight land before the CTA's memory goes (bounded).
+    for (int i = item < q_slots ? 0 : item - q_slots; i < item; ++i)
+      if (!warp_wait(q_full + i % q_slots, (i / q_slots) & 1)) break;
     for (int i = it < kStages ? 0 : it - kStages; i < it; ++i)
       if (!warp_wait(full + i % kStages, (i / kStages) & 1)) break;
   } else {
     const int gid = lane >> 2, c = lane & 3;
     const uint32_t ring = smem_u32(smem);
     const int p0 = warp * 16;
-    int it = 0;
+    int it = 0, item = 0;
     bool ok = true, cut_first = false;
     while (s.count > 0 && ok) {
       const int len = clamped_len(p.lens, s.b, p.len_limit);
@@ -269,16 +279,16 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
       const int kvh = s.hv / p.nrb, rb = s.hv - kvh * p.nrb;
       const int head0 = kvh * p.g + rb * 16;
       const int rows = min(16, p.g - rb * 16);
-      // Q as A fragments: rows are the KV head's query heads (others zero).
+      // Q as A fragments: rows are the KV head's query heads.
       uint32_t qa[D / 16][4];
-      const E* qrow = static_cast<const E*>(p.q) + s.b * p.q_stride_seq + head0 * p.q_stride_head;
+      const int qi = item % q_slots;
+      if (!warp_wait(q_full + qi, (item / q_slots) & 1)) break;
+      ++item;
 #pragma unroll
       for (int ks = 0; ks < D / 16; ++ks)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int j = gid + 8 * (r & 1), d = ks * 16 + 2 * c + 8 * (r >> 1);
-          qa[ks][r] = j < rows ? __ldg(reinterpret_cast<const uint32_t*>(qrow + j * p.q_stride_head + d)) : 0u;
-        }
+        ldsm_x4(smem_u32(qs) + (qi * p.rows + (lane & 15)) * (D * 2) + ks * 32 + (lane >> 4) * 16, qa[ks]);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(q_empty + qi);
       float o[D / 8][4];
 #pragma unroll
       for (int nb = 0; nb < D / 8; ++nb) o[nb][0] = o[nb][1] = o[nb][2] = o[nb][3] = 0.f;
@@ -371,16 +381,17 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
         }
       }
       const bool whole = s.x == 0 && n == nt;
-      const int slot = 2 * blockIdx.x + (s.x > 0 ? 0 : 1);
-      if (!whole && s.x == 0) {
+      const int64_t id = static_cast<int64_t>(s.b) * n_hv + s.hv;
+      const int64_t slot = whole ? 2 * p.n_ctas + id : 2 * blockIdx.x + (s.x > 0 ? 0 : 1);
+      if (s.x == 0 && (late || !whole)) {
         cut_first = true;
         if (threadIdx.x == 0) {
           const long long end = s.pos + nt;
           const int last = static_cast<int>((end * s.ctas - 1) / s.total);
-          p.desc[blockIdx.x] = Desc{s.b, s.hv, last - static_cast<int>(blockIdx.x) + 1, 0};
+          p.desc[late ? id : blockIdx.x] =
+              Desc{s.b, s.hv, whole ? -1 : static_cast<int>(blockIdx.x), last - static_cast<int>(blockIdx.x) + 1};
         }
       }
-      if (late && whole) pdl_wait_prior_grid();
       for (int r0 = 0; r0 < rows; r0 += kMergeRows) {
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
@@ -411,13 +422,13 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
               num.z = fmaf(v.z, f, num.z);
               num.w = fmaf(v.w, f, num.w);
             }
-            if (whole) {
-              finish<E, D>(p, s.b, head0 + row, d4, mx, den, num);
+            if (whole && !late) {
+              store4<E, D>(p, s.b, head0 + row, d4, den, num);
             } else {
-              *reinterpret_cast<float4*>(p.part + (static_cast<int64_t>(slot) * 16 + row) * D + d4 * 4) = num;
+              *reinterpret_cast<float4*>(p.part + (slot * p.rows + row) * D + d4 * 4) = num;
               if (d4 == 0) {
-                p.ml[slot * 32 + row] = mx;
-                p.ml[slot * 32 + 16 + row] = den;
+                p.ml[slot * 2 * p.rows + row] = mx;
+                p.ml[(slot * 2 + 1) * p.rows + row] = den;
               }
             }
           }
@@ -429,46 +440,104 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
       s.x = 0;
       if (++s.hv == n_hv) { s.hv = 0; ++s.b; }
     }
-    if (threadIdx.x == 0 && !cut_first) p.desc[blockIdx.x] = Desc{0, 0, 0, 0};
+    if (threadIdx.x == 0 && !cut_first && !late) p.desc[blockIdx.x] = Desc{0, 0, 0, 0};
   }
   if (late) pdl_wait_prior_grid();
 }
 
-// Joins the pieces of the item whose first piece CTA blockIdx.x holds.
-template <typename E, int D>
-__global__ void __launch_bounds__(128)
+// Joins an item's pieces, R query heads a block: those that the CTAs of the
+// decode kernel left, and the shared prefix's behind them. The pieces are
+// dealt to groups of threads (several loads of each in flight), whose results
+// are joined in order.
+constexpr int kJoinThreads = 256;
+
+template <typename E, int D, int R>
+__global__ void __launch_bounds__(kJoinThreads)
     paged_join_kernel(const __grid_constant__ Params p) {
+  constexpr int kCells = R * (D / 4), kGroups = kJoinThreads / kCells;
+  __shared__ float4 s_num[kGroups][kCells];
+  __shared__ float2 s_ml[kGroups][kCells];
   pdl_wait_prior_grid();
   pdl_launch_dependents();
   const int4 raw = __ldcg(reinterpret_cast<const int4*>(p.desc + blockIdx.x));
-  const Desc d{raw.x, raw.y, raw.z, 0};
-  if (d.pieces == 0) return;
+  const Desc d{raw.x, raw.y, raw.z, raw.w};
   const int kvh = d.hv / p.nrb, rb = d.hv - kvh * p.nrb;
   const int rows = min(16, p.g - rb * 16);
-  // Piece 0 lies in this CTA's second slot, piece i > 0 in CTA + i's first.
-  auto slot_of = [&](int i) {
-    return 2 * (static_cast<int64_t>(blockIdx.x) + i) + (i == 0 ? 1 : 0);
-  };
-  for (int t = threadIdx.x; t < rows * (D / 4); t += 128) {
-    const int row = t / (D / 4), d4 = t % (D / 4);
-    float mx = -INFINITY;
-    for (int i = 0; i < d.pieces; ++i) mx = fmaxf(mx, __ldcg(p.ml + slot_of(i) * 32 + row));
-    const float mu = mx == -INFINITY ? 0.f : mx;
-    float den = 0.f;
-    float4 num = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-    for (int i = 0; i < d.pieces; ++i) {
-      const int64_t sl = slot_of(i);
-      const float f = exp2_approx(__ldcg(p.ml + sl * 32 + row) - mu);
-      const float4 v = __ldcg(reinterpret_cast<const float4*>(p.part + (sl * 16 + row) * D + d4 * 4));
-      den = fmaf(__ldcg(p.ml + sl * 32 + 16 + row), f, den);
+  if (d.pieces == 0 || static_cast<int>(blockIdx.y) * R >= rows) return;
+  const int cell = threadIdx.x % kCells, group = threadIdx.x / kCells;
+  const int row = blockIdx.y * R + cell % R, d4 = cell / R;
+  const int own = d.pieces, all = own + p.prefix.S;
+  const int64_t pre = p.prefix.S ? prefix_first(p.prefix, p.hkv, d.b, kvh) : 0;
+  const int pre_row = p.prefix.S ? prefix_row(p.prefix, p.g, d.b, rb * 16 + row) : 0;
+  float m = -INFINITY, l = 0.f;
+  float4 num = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (row < rows) {
+    constexpr int kBatch = 4;
+    for (int i0 = group; i0 < all; i0 += kBatch * kGroups) {
+      float pm[kBatch], pl[kBatch];
+      float4 v[kBatch];
+#pragma unroll
+      for (int u = 0; u < kBatch; ++u) {
+        const int i = i0 + u * kGroups;
+        pm[u] = -INFINITY;
+        pl[u] = 0.f;
+        v[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (i < own) {
+          // Piece 0 lies in its CTA's second slot, piece i > 0 in CTA + i's
+          // first; a whole result in the item's own.
+          const int64_t slot = d.cta < 0 ? 2 * p.n_ctas + blockIdx.x
+                                         : 2 * (static_cast<int64_t>(d.cta) + i) + (i == 0 ? 1 : 0);
+          pm[u] = __ldcg(p.ml + slot * 2 * p.rows + row);
+          pl[u] = __ldcg(p.ml + (slot * 2 + 1) * p.rows + row);
+          v[u] = __ldcg(reinterpret_cast<const float4*>(p.part + (slot * p.rows + row) * D) + d4);
+        } else if (i < all) {
+          const int64_t s = pre + i - own;
+          pm[u] = __ldcg(p.prefix.ml + s * 512 + pre_row);
+          pl[u] = __ldcg(p.prefix.ml + s * 512 + 256 + pre_row);
+          v[u] = __ldcg(reinterpret_cast<const float4*>(p.prefix.o) + (s * (D / 4) + d4) * 256 + pre_row);
+        }
+      }
+      float mx = m;
+#pragma unroll
+      for (int u = 0; u < kBatch; ++u) mx = fmaxf(mx, pm[u]);
+      const float mu = mx == -INFINITY ? 0.f : mx;
+      float f = exp2_approx(m - mu);
+      l *= f;
+      num.x *= f; num.y *= f; num.z *= f; num.w *= f;
+#pragma unroll
+      for (int u = 0; u < kBatch; ++u) {
+        f = exp2_approx(pm[u] - mu);
+        l = fmaf(pl[u], f, l);
+        num.x = fmaf(v[u].x, f, num.x);
+        num.y = fmaf(v[u].y, f, num.y);
+        num.z = fmaf(v[u].z, f, num.z);
+        num.w = fmaf(v[u].w, f, num.w);
+      }
+      m = mx;
+    }
+  }
+  if (kGroups > 1) {
+    s_num[group][cell] = num;
+    s_ml[group][cell] = make_float2(m, l);
+    __syncthreads();
+    if (group > 0) return;
+#pragma unroll
+    for (int k = 1; k < kGroups; ++k) m = fmaxf(m, s_ml[k][cell].x);
+    const float mu = m == -INFINITY ? 0.f : m;
+    l = 0.f;
+    num = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int k = 0; k < kGroups; ++k) {
+      const float f = exp2_approx(s_ml[k][cell].x - mu);
+      const float4 v = s_num[k][cell];
+      l = fmaf(s_ml[k][cell].y, f, l);
       num.x = fmaf(v.x, f, num.x);
       num.y = fmaf(v.y, f, num.y);
       num.z = fmaf(v.z, f, num.z);
       num.w = fmaf(v.w, f, num.w);
     }
-    finish<E, D>(p, d.b, kvh * p.g + rb * 16 + row, d4, mx, den, num);
   }
+  if (row < rows) store4<E, D>(p, d.b, kvh * p.g + rb * 16 + row, d4, l, num);
 }
 
 template <typename E, int D>
@@ -496,32 +565,55 @@ cudaError_t launch(const Params& p, const CUtensorMap& kmap, const CUtensorMap& 
   cfg.numAttrs = 1;
   e = cudaLaunchKernelEx(&cfg, paged_decode_kernel<E, D>, p, kmap, vmap);
   if (e != cudaSuccess) return e;
-  cfg.blockDim = dim3(128);
+  // Query heads a join block takes: few, so that the pieces of a small batch
+  // spread over many threads, but one where there is one.
+  const int per = p.rows == 1 ? 1 : 4;
+  const int64_t items = p.prefix.S ? static_cast<int64_t>(p.B) * p.hkv * p.nrb : p.n_ctas;
+  if (items > 0x7fffffff) return cudaErrorInvalidValue;
+  cfg.gridDim = dim3(static_cast<unsigned>(items), (p.rows + per - 1) / per);
+  cfg.blockDim = dim3(kJoinThreads);
   cfg.dynamicSmemBytes = 0;
-  return cudaLaunchKernelEx(&cfg, paged_join_kernel<E, D>, p);
+  return per == 1 ? cudaLaunchKernelEx(&cfg, paged_join_kernel<E, D, 1>, p)
+                  : cudaLaunchKernelEx(&cfg, paged_join_kernel<E, D, 4>, p);
 }
 
 }  // namespace
 
 int paged_decode_box_rows(int page_size) { return page_size < kTile ? page_size : kTile; }
 
-size_t paged_decode_workspace(int D, int num_sms) {
+namespace {
+// Slots of pieces, and descriptions, of a launch: two and one a CTA; behind a
+// prefix one and one an item as well.
+struct Scratch {
+  size_t slots, descs, rows;
+};
+Scratch scratch_of(int B, int hq, int n_kv_heads, bool prefix, int num_sms) {
+  const size_t g = hq / n_kv_heads, items = static_cast<size_t>(B) * n_kv_heads * ((g + 15) / 16);
   const size_t ctas = static_cast<size_t>(kCtasPerSm) * num_sms;
-  return (ctas * (2 * 16 * D * 4 + 2 * 2 * 16 * 4 + sizeof(Desc)) + 255) / 256 * 256;
+  return Scratch{2 * ctas + (prefix ? items : 0), prefix ? items : ctas, g < 16 ? g : 16};
+}
+}  // namespace
+
+size_t paged_decode_workspace(int B, int hq, int n_kv_heads, int D, bool prefix, int num_sms) {
+  const Scratch s = scratch_of(B, hq, n_kv_heads, prefix, num_sms);
+  // Descriptions first (16 bytes each), then the pieces.
+  return (s.descs * sizeof(Desc) + s.slots * s.rows * (D + 2) * 4 + 255) / 256 * 256;
 }
 
 cudaError_t launch_paged_decode(const PagedPool& pool, const CUtensorMap& kmap,
                                 const CUtensorMap& vmap, const DecodeArgs& a, int num_sms,
                                 cudaStream_t stream) {
-  const size_t ctas = static_cast<size_t>(kCtasPerSm) * num_sms;
+  const Scratch s = scratch_of(a.B, a.hq, pool.n_kv_heads, a.prefix.S > 0, num_sms);
   Params p;
   p.q = a.q;
   p.out = a.out;
   p.table = a.table;
   p.lens = a.lens;
-  p.part = static_cast<float*>(a.workspace);
-  p.ml = p.part + ctas * 2 * 16 * pool.D;
-  p.desc = reinterpret_cast<Desc*>(p.ml + ctas * 2 * 2 * 16);
+  p.desc = static_cast<Desc*>(a.workspace);
+  p.part = reinterpret_cast<float*>(p.desc + s.descs);
+  p.ml = p.part + s.slots * s.rows * pool.D;
+  p.rows = static_cast<int>(s.rows);
+  p.n_ctas = kCtasPerSm * num_sms;
   p.q_stride_seq = a.q_stride_seq;
   p.q_stride_head = a.q_stride_head;
   p.table_stride = a.table_stride;

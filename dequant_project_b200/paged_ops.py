@@ -72,20 +72,13 @@ def _stream(device) -> int:
 
 
 @functools.lru_cache(maxsize=None)
-def _decode_bytes(device_index: int, head_dim: int) -> int:
-    n = ctypes.c_uint64(0)
-    _native.check(_native.lib().dqg_paged_attention_workspace(head_dim, ctypes.byref(n)))
-    return int(n.value)
-
-
-@functools.lru_cache(maxsize=None)
 def _prompt_bytes(device_index: int, head_dim: int) -> int:
     n = ctypes.c_uint64(0)
     _native.check(_native.lib().dqg_prompt_attention_workspace(head_dim, ctypes.byref(n)))
     return int(n.value)
 
 
-@functools.lru_cache(maxsize=256)
+@functools.lru_cache(maxsize=1024)
 def _prefix_bytes(device_index: int, n_seqs: int, hq: int, hkv: int, head_dim: int, prefix_len: int) -> int:
     n = ctypes.c_uint64(0)
     _native.check(_native.lib().dqg_shared_prefix_workspace(n_seqs, hq, hkv, head_dim, prefix_len,
@@ -257,7 +250,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
         raise RuntimeError(f"block_table and kv_lens must hold one row for each of the {b} sequences")
     out = torch.empty((b, hq, d), dtype=q.dtype, device=device)
     with _on(device):
-        ws = _workspace(workspace, _decode_bytes(device.index, d), device)
+        ws = _workspace(workspace, _prefix_bytes(device.index, b, hq, kv.n_kv_heads, d, 0), device)
         _native.check(_native.lib().dqg_paged_attention(
             q.data_ptr(), q.stride(0), q.stride(1), b, hq, ctypes.byref(kv), block_table.data_ptr(),
             block_table.shape[1], block_table.stride(0) if b > 1 else block_table.shape[1],
@@ -266,11 +259,9 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     return out
 
 
-def paged_attention_workspace(head_dim: int, device) -> torch.Tensor:
-    """Scratch memory for ``paged_attention`` calls of any batch and lengths."""
-    device = torch.device(device)
-    with _on(device):
-        return torch.empty(_decode_bytes(device.index, head_dim), dtype=torch.uint8, device=device)
+def paged_attention_workspace(n_seqs: int, n_q_heads: int, n_kv_heads: int, head_dim: int, device) -> torch.Tensor:
+    """Scratch memory for ``paged_attention`` calls of these sizes and any lengths."""
+    return shared_prefix_workspace(n_seqs, n_q_heads, n_kv_heads, head_dim, 0, device)
 
 
 def prompt_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch.Tensor,

@@ -385,11 +385,12 @@ int dqg_rope_paged_append(const void *qkv, int64_t T, int64_t qkv_stride, int64_
  * behind a sequence's last page are not read, and what lies in its last page
  * behind its last position does not matter. The lengths are read on the
  * device, so a captured launch serves other lengths. workspace: at least
- * dqg_paged_attention_workspace(D) bytes, 16-byte aligned, of any contents;
+ * dqg_paged_attention_workspace's bytes, 16-byte aligned, of any contents;
  * calls that share one must not overlap on the GPU. Results do not depend on
  * anything but the inputs (no atomics).
  */
-int dqg_paged_attention_workspace(int64_t head_dim, uint64_t *bytes);
+int dqg_paged_attention_workspace(int64_t n_seqs, int64_t n_q_heads, int64_t n_kv_heads, int64_t head_dim,
+                                  uint64_t *bytes);
 int dqg_paged_attention(const void *q, int64_t q_stride_seq, int64_t q_stride_head, int64_t n_seqs,
                         int64_t n_q_heads, const dqg_paged_kv *kv, const int32_t *block_table,
                         int64_t table_width, int64_t table_stride, const int32_t *kv_lens, float scale,

@@ -211,7 +211,7 @@ def test_decode(cuda_device, lens, hq, hkv, d, page, dtype):
     ref = torch.cat([attend64(q[i:i + 1], rows64(k, table[i], n), rows64(v, table[i], n),
                               kv_lens[i:i + 1], scale) for i, n in enumerate(lens)])
     check_attention(out, ref, v_max, dtype)
-    ws = paged_ops.paged_attention_workspace(d, cuda_device).fill_(255)
+    ws = paged_ops.paged_attention_workspace(len(lens), hq, hkv, d, cuda_device).fill_(255)
     for _ in range(3):
         assert torch.equal(paged_ops.paged_attention(q, k, v, table, kv_lens, workspace=ws), out)
     assert _native.device_status(cuda_device.index) == 0
