@@ -31,44 +31,46 @@ from dequant_project_b200 import _native
 _DTYPES = {torch.float16: 0, torch.bfloat16: 1}
 
 
-def _pools(k_pages: torch.Tensor, v_pages: torch.Tensor, *same_type) -> "_native.PagedKV":
-    """The C description of the pools, with the checks that need tensors."""
-    code = _DTYPES.get(k_pages.dtype)
-    if code is None:
-        raise RuntimeError(f"pages must be float16 or bfloat16, got {k_pages.dtype}")
-    if k_pages.dim() != 4:
-        raise RuntimeError("pages must be [pages, kv heads, page size, head dim]")
-    n, h, p, d = k_pages.shape
-    sn, sh, sp, sd = k_pages.stride()
-    if (v_pages.shape != k_pages.shape or v_pages.stride() != (sn, sh, sp, sd)
-            or v_pages.dtype != k_pages.dtype or sd != 1):
-        raise RuntimeError("k_pages and v_pages must have one shape, type and strides, with the "
-                           "head dimension contiguous")
-    device = k_pages.device
-    if v_pages.device != device:
-        raise RuntimeError("k_pages and v_pages must be on the same device")
-    for name, t in same_type:
-        if t.dtype != k_pages.dtype or t.device != device:
-            raise RuntimeError(f"{name} must be {k_pages.dtype} on {device}, as the pages are")
-    return _native.PagedKV(k_pages.data_ptr(), v_pages.data_ptr(), n, h, p, d, sn, sh, sp, code)
+def _pools(k: torch.Tensor, v: torch.Tensor, name: str, t: torch.Tensor) -> tuple:
+    """The C description of the pools and their device, with the checks that
+    need tensors; ``t`` (``name`` in messages) must have their type and device."""
+    dtype, shape, strides, dev = k.dtype, k.shape, k.stride(), t.get_device()
+    if (dtype not in _DTYPES or len(shape) != 4 or strides[3] != 1 or v.stride() != strides or v.shape != shape
+            or v.dtype is not dtype or t.dtype is not dtype or k.get_device() != dev or v.get_device() != dev):
+        if dtype not in _DTYPES:
+            raise RuntimeError(f"pages must be float16 or bfloat16, got {dtype}")
+        if len(shape) != 4:
+            raise RuntimeError("pages must be [pages, kv heads, page size, head dim]")
+        if v.stride() != strides or v.shape != shape or v.dtype is not dtype or strides[3] != 1:
+            raise RuntimeError("k_pages and v_pages must have one shape, type and strides, with the "
+                               "head dimension contiguous")
+        if v.device != k.device:
+            raise RuntimeError("k_pages and v_pages must be on the same device")
+        raise RuntimeError(f"{name} must be {dtype} on {k.device}, as the pages are")
+    return _native.PagedKV(k.data_ptr(), v.data_ptr(), *shape, strides[0], strides[1], strides[2],
+                           _DTYPES[dtype]), dev
 
 
-def _ints(device, *named) -> None:
-    """Contiguous integer tensors of one type and device."""
-    for name, t, dtype, dims in named:
-        if t.dtype != dtype or t.dim() != dims or t.device != device or t.stride(-1) != 1:
-            raise RuntimeError(f"{name} must be a contiguous {dims}-dimensional {dtype} tensor on {device}")
+def _ints(name: str, t: torch.Tensor, dtype, dims: int, dev: int) -> None:
+    """An integer tensor whose last dimension is contiguous."""
+    if t.dtype is not dtype or t.dim() != dims or t.get_device() != dev or t.stride()[-1] != 1:
+        raise RuntimeError(f"{name} must be a contiguous {dims}-dimensional {dtype} tensor on cuda:{dev}")
 
 
-def _on(device):
+def _on(dev: int):
     """The device as the current one, for callers that have another current."""
-    if device.index is None or device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(device)
+    return _SAME if dev == torch._C._cuda_getDevice() else torch.cuda.device(dev)
 
 
-def _stream(device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+def _index(device) -> int:
+    index = torch.device(device).index
+    return torch.cuda.current_device() if index is None else index
+
+
+_SAME = contextlib.nullcontext()
+
+
+_stream = torch._C._cuda_getCurrentRawStream if torch.cuda._is_compiled() else None
 
 
 @functools.lru_cache(maxsize=None)
@@ -86,12 +88,14 @@ def _prefix_bytes(device_index: int, n_seqs: int, hq: int, hkv: int, head_dim: i
     return int(n.value)
 
 
-def _workspace(given: torch.Tensor | None, need: int, device) -> torch.Tensor:
+def _workspace(given: torch.Tensor | None, need: int, q: torch.Tensor) -> tuple:
+    """(tensor, pointer, bytes) of the scratch memory of a call on ``q``."""
     if given is None:
-        return torch.empty(need, dtype=torch.uint8, device=device)
-    if given.device != device or not given.is_contiguous():
-        raise RuntimeError(f"the workspace must be a contiguous tensor on {device}")
-    return given
+        given = q.new_empty(need, dtype=torch.uint8)
+        return given, given.data_ptr(), need
+    if given.get_device() != q.get_device() or not given.is_contiguous():
+        raise RuntimeError(f"the workspace must be a contiguous tensor on {q.device}")
+    return given, given.data_ptr(), given.numel() * given.element_size()
 
 
 # ------------------------------------------------------------------- append
@@ -170,30 +174,29 @@ def rope_paged_append(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, p
         k_pages[at] = turn(k, k_norm)[kept]
         v_pages[at] = v.to(qkv.dtype)[kept]
         return turn(q, q_norm)
-    norms = () if q_norm is None else (("q_norm", q_norm),)
-    norms += () if k_norm is None else (("k_norm", k_norm),)
-    kv = _pools(k_pages, v_pages, ("qkv", qkv), *norms)
-    device = qkv.device
+    kv, dev = _pools(k_pages, v_pages, "qkv", qkv)
     if qkv.dim() != 2 or qkv.shape[1] != (n_q_heads + 2 * hkv) * d or qkv.stride(1) != 1:
         raise RuntimeError(f"qkv must be [T, {(n_q_heads + 2 * hkv) * d}] with contiguous rows")
-    if (cos.dtype != torch.float32 or sin.dtype != torch.float32 or cos.dim() != 2 or sin.shape != cos.shape
-            or cos.device != device or sin.device != device
+    shape = cos.shape
+    if (cos.dtype is not torch.float32 or sin.dtype is not torch.float32 or len(shape) != 2 or sin.shape != shape
+            or cos.get_device() != dev or sin.get_device() != dev
             or not (cos.is_contiguous() and sin.is_contiguous())):
-        raise RuntimeError(f"cos and sin must be contiguous float32 [positions, R / 2] on {device}")
-    _ints(device, ("positions", positions, torch.int64, 1), ("slots", slots, torch.int64, 1))
+        raise RuntimeError(f"cos and sin must be contiguous float32 [positions, R / 2] on cuda:{dev}")
+    _ints("positions", positions, torch.int64, 1, dev)
+    _ints("slots", slots, torch.int64, 1, dev)
     if positions.shape[0] != t or slots.shape[0] != t:
         raise RuntimeError(f"positions and slots must hold one entry for each of the {t} tokens")
-    for name, w in norms:
-        if w.shape != (d,) or w.stride(0) != 1:
-            raise RuntimeError(f"{name} must hold {d} contiguous weights")
-    q = torch.empty((t, n_q_heads, d), dtype=qkv.dtype, device=device)
-    with _on(device):
+    for name, w in (("q_norm", q_norm), ("k_norm", k_norm)):
+        if w is not None and (w.shape != (d,) or w.stride(0) != 1 or w.dtype is not qkv.dtype
+                              or w.get_device() != dev):
+            raise RuntimeError(f"{name} must hold {d} contiguous {qkv.dtype} weights on cuda:{dev}")
+    q = qkv.new_empty((t, n_q_heads, d))
+    with _on(dev):
         _native.check(_native.lib().dqg_rope_paged_append(
             qkv.data_ptr(), t, qkv.stride(0) if t > 1 else qkv.shape[1], n_q_heads, cos.data_ptr(),
-            sin.data_ptr(), cos.shape[0], 2 * cos.shape[1], int(interleaved), positions.data_ptr(),
-            slots.data_ptr(), None if q_norm is None else q_norm.data_ptr(),
-            None if k_norm is None else k_norm.data_ptr(), eps, ctypes.byref(kv), q.data_ptr(),
-            _stream(device)))
+            sin.data_ptr(), shape[0], 2 * shape[1], interleaved, positions.data_ptr(), slots.data_ptr(),
+            None if q_norm is None else q_norm.data_ptr(), None if k_norm is None else k_norm.data_ptr(), eps,
+            kv, q.data_ptr(), _stream(dev)))
     return q
 
 
@@ -242,20 +245,19 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
                               _rows(v_pages, block_table[i], int(kv_lens[i])), kv_lens[i:i + 1], scale)
                for i in range(b)]
         return torch.cat(out).to(q.dtype) if out else torch.empty_like(q)
-    kv = _pools(k_pages, v_pages, ("q", q))
-    device = q.device
+    kv, dev = _pools(k_pages, v_pages, "q", q)
     _query(q, kv.head_dim)
-    _ints(device, ("block_table", block_table, torch.int32, 2), ("kv_lens", kv_lens, torch.int32, 1))
+    _ints("block_table", block_table, torch.int32, 2, dev)
+    _ints("kv_lens", kv_lens, torch.int32, 1, dev)
     if block_table.shape[0] != b or kv_lens.shape[0] != b:
         raise RuntimeError(f"block_table and kv_lens must hold one row for each of the {b} sequences")
-    out = torch.empty((b, hq, d), dtype=q.dtype, device=device)
-    with _on(device):
-        ws = _workspace(workspace, _prefix_bytes(device.index, b, hq, kv.n_kv_heads, d, 0), device)
+    out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    with _on(dev):
+        _, ws, size = _workspace(workspace, _prefix_bytes(dev, b, hq, kv.n_kv_heads, d, 0), q)
         _native.check(_native.lib().dqg_paged_attention(
-            q.data_ptr(), q.stride(0), q.stride(1), b, hq, ctypes.byref(kv), block_table.data_ptr(),
+            q.data_ptr(), q.stride(0), q.stride(1), b, hq, kv, block_table.data_ptr(),
             block_table.shape[1], block_table.stride(0) if b > 1 else block_table.shape[1],
-            kv_lens.data_ptr(), scale, out.data_ptr(), ws.data_ptr(), ws.numel() * ws.element_size(),
-            _stream(device)))
+            kv_lens.data_ptr(), scale, out.data_ptr(), ws, size, _stream(dev)))
     return out
 
 
@@ -288,29 +290,29 @@ def prompt_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tens
             out[lo:hi] = _cpu_attention(q[lo:hi].float(), _rows(k_pages, block_table[i], n),
                                         _rows(v_pages, block_table[i], n), ends, scale).to(q.dtype)
         return out
-    kv = _pools(k_pages, v_pages, ("q", q))
-    device = q.device
+    kv, dev = _pools(k_pages, v_pages, "q", q)
     _query(q, kv.head_dim)
-    _ints(device, ("block_table", block_table, torch.int32, 2), ("q_starts", q_starts, torch.int32, 1),
-          ("kv_lens", kv_lens, torch.int32, 1))
+    _ints("block_table", block_table, torch.int32, 2, dev)
+    _ints("q_starts", q_starts, torch.int32, 1, dev)
+    _ints("kv_lens", kv_lens, torch.int32, 1, dev)
     if block_table.shape[0] != b or q_starts.shape[0] != b + 1:
         raise RuntimeError(f"block_table and q_starts must hold {b} and {b + 1} rows for {b} sequences")
-    out = torch.empty((t, hq, d), dtype=q.dtype, device=device)
-    with _on(device):
-        ws = _workspace(workspace, _prompt_bytes(device.index, d), device)
+    out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    with _on(dev):
+        _, ws, size = _workspace(workspace, _prompt_bytes(dev, d), q)
         _native.check(_native.lib().dqg_prompt_attention(
-            q.data_ptr(), q.stride(0), q.stride(1), t, hq, ctypes.byref(kv), block_table.data_ptr(),
+            q.data_ptr(), q.stride(0), q.stride(1), t, hq, kv, block_table.data_ptr(),
             block_table.shape[1], block_table.stride(0) if b > 1 else block_table.shape[1],
-            q_starts.data_ptr(), kv_lens.data_ptr(), b, int(causal), scale, out.data_ptr(), ws.data_ptr(),
-            ws.numel() * ws.element_size(), _stream(device)))
+            q_starts.data_ptr(), kv_lens.data_ptr(), b, causal, scale, out.data_ptr(), ws, size,
+            _stream(dev)))
     return out
 
 
 def prompt_attention_workspace(head_dim: int, device) -> torch.Tensor:
     """Scratch memory for ``prompt_attention`` calls of any batch and lengths."""
-    device = torch.device(device)
-    with _on(device):
-        return torch.empty(_prompt_bytes(device.index, head_dim), dtype=torch.uint8, device=device)
+    dev = _index(device)
+    with _on(dev):
+        return torch.empty(_prompt_bytes(dev, head_dim), dtype=torch.uint8, device=device)
 
 
 def shared_prefix_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
@@ -333,28 +335,28 @@ def shared_prefix_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: tor
                     for p in (k_pages, v_pages))
             out.append(_cpu_attention(q[i:i + 1].float(), k, v, torch.tensor([prefix_len + n]), scale))
         return torch.cat(out).to(q.dtype) if out else torch.empty_like(q)
-    kv = _pools(k_pages, v_pages, ("q", q))
-    device = q.device
+    kv, dev = _pools(k_pages, v_pages, "q", q)
     _query(q, kv.head_dim)
-    _ints(device, ("prefix_table", prefix_table, torch.int32, 1), ("block_table", block_table, torch.int32, 2),
-          ("kv_lens", kv_lens, torch.int32, 1))
+    _ints("prefix_table", prefix_table, torch.int32, 1, dev)
+    _ints("block_table", block_table, torch.int32, 2, dev)
+    _ints("kv_lens", kv_lens, torch.int32, 1, dev)
     if block_table.shape[0] != b or kv_lens.shape[0] != b:
         raise RuntimeError(f"block_table and kv_lens must hold one row for each of the {b} sequences")
-    out = torch.empty((b, hq, d), dtype=q.dtype, device=device)
-    with _on(device):
-        ws = _workspace(workspace, _prefix_bytes(device.index, b, hq, kv.n_kv_heads, d, prefix_len), device)
+    out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    with _on(dev):
+        _, ws, size = _workspace(workspace, _prefix_bytes(dev, b, hq, kv.n_kv_heads, d, prefix_len), q)
         _native.check(_native.lib().dqg_shared_prefix_attention(
-            q.data_ptr(), q.stride(0), q.stride(1), b, hq, ctypes.byref(kv), prefix_table.data_ptr(),
+            q.data_ptr(), q.stride(0), q.stride(1), b, hq, kv, prefix_table.data_ptr(),
             prefix_table.shape[0], prefix_len, block_table.data_ptr(), block_table.shape[1],
             block_table.stride(0) if b > 1 else block_table.shape[1], kv_lens.data_ptr(), scale,
-            out.data_ptr(), ws.data_ptr(), ws.numel() * ws.element_size(), _stream(device)))
+            out.data_ptr(), ws, size, _stream(dev)))
     return out
 
 
 def shared_prefix_workspace(n_seqs: int, n_q_heads: int, n_kv_heads: int, head_dim: int, prefix_len: int,
                             device) -> torch.Tensor:
     """Scratch memory for ``shared_prefix_attention`` calls of these sizes."""
-    device = torch.device(device)
-    with _on(device):
-        return torch.empty(_prefix_bytes(device.index, n_seqs, n_q_heads, n_kv_heads, head_dim, prefix_len),
+    dev = _index(device)
+    with _on(dev):
+        return torch.empty(_prefix_bytes(dev, n_seqs, n_q_heads, n_kv_heads, head_dim, prefix_len),
                            dtype=torch.uint8, device=device)
