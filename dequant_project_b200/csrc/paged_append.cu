@@ -12,10 +12,15 @@
 // positions, so every scaling of the frequencies is the caller's.
 //
 // Bound by HBM: each row is read once and each head written once. A group of
-// D / 8 lanes holds a head, 16 bytes a lane, and a warp takes a few heads of
-// one token, whose table entries then stay in registers; the partner of a
-// rotated value lies in another lane's registers (half layout) or in the lane
-// itself (interleaved), and the sum of squares is one shuffle reduction.
+// D / 16 lanes holds a head, and a lane two runs of eight values: in the half
+// layout those at i and i + R/2, so that both values of a rotated pair lie in
+// one lane and share a table entry; interleaved pairs lie in one lane anyway.
+// A warp takes a few heads of one token, whose table entries stay in
+// registers; the sum of squares is one shuffle reduction. What it measured
+// (B200, 8192 tokens of 64 + 2 x 8 heads of 128, bf16, norms): 69 us, 4.9 TB/s
+// of the 6.4 that a copy reaches. Registers decide: at 80 (three blocks an SM)
+// 69 us, at 128 (two) 79; one, two, three heads a lane group 84, 74, 70 us;
+// runs of four values instead of eight (more, narrower accesses) 84 us.
 #include <cstdint>
 
 #include "paged.cuh"
@@ -24,6 +29,7 @@ namespace dqg {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int kIter = 4;  // heads a lane group takes one after the other
 
 template <typename E>
 struct AppendParams {
@@ -40,16 +46,34 @@ struct AppendParams {
   int64_t qkv_stride, n_positions, n_slots, page_stride, head_stride, row_stride;
   int T, hq, hkv, rot, page_shift, chunks;
   float eps;
-  bool interleaved;
 };
 
-// ALIGNED: the half layout's partner values are whole lanes away (R a
-// multiple of 16), or every pair lies in one lane (interleaved). Otherwise
-// partners are read again from memory, one at a time.
-template <typename E, int D, int ITER, bool ALIGNED>
-__global__ void __launch_bounds__(kThreads)
+enum Layout {
+  kHalf,         // pairs (i, i + R/2), R a multiple of 16
+  kInterleaved,  // pairs (2i, 2i + 1)
+  kUneven        // pairs (i, i + R/2), any R: partners are read again from memory
+};
+
+template <typename E>
+__device__ __forceinline__ void unpack8(uint4 v, float* f) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 t = Elem<E>::unpack(w[i]);
+    f[2 * i] = t.x;
+    f[2 * i + 1] = t.y;
+  }
+}
+template <typename E>
+__device__ __forceinline__ uint4 pack8(const float* f) {
+  return make_uint4(Elem<E>::pack(f[0], f[1]), Elem<E>::pack(f[2], f[3]), Elem<E>::pack(f[4], f[5]),
+                    Elem<E>::pack(f[6], f[7]));
+}
+
+template <typename E, int D, int ITER, int LAYOUT>
+__global__ void __launch_bounds__(kThreads, LAYOUT == kUneven ? 2 : 3)
     paged_append_kernel(const __grid_constant__ AppendParams<E> p) {
-  constexpr int kLanes = D / 8;         // lanes a head
+  constexpr int kLanes = D / 16;        // lanes a head
   constexpr int kGroups = 32 / kLanes;  // heads a warp holds at a time
   const int64_t w = static_cast<int64_t>(blockIdx.x) * (kThreads / 32) + (threadIdx.x >> 5);
   const int64_t token = w / p.chunks;
@@ -58,120 +82,129 @@ __global__ void __launch_bounds__(kThreads)
   pdl_wait_prior_grid();
   pdl_launch_dependents();
   if (token >= p.T) return;
-  const int n_heads = p.hq + 2 * p.hkv;
+  const int rotated = p.hq + p.hkv, n_heads = rotated + p.hkv;
   const int h0 = chunk * ITER * kGroups + grp;
-  const E* row = p.qkv + token * p.qkv_stride + c * 8;
-  uint4 x[ITER];
+  // The lane's two runs of eight values. Half layout: the first R / 16 lanes
+  // hold the pairs, the others what passes.
+  const int rc = p.rot / 16;
+  const bool pairs = LAYOUT != kHalf || c < rc;
+  const int ea = LAYOUT == kHalf ? (pairs ? 8 * c : 16 * c) : 16 * c;
+  const int eb = LAYOUT == kHalf && pairs ? ea + p.rot / 2 : ea + 8;
+  const E* row = p.qkv + token * p.qkv_stride;
+  uint4 xa[ITER], xb[ITER];
 #pragma unroll
   for (int it = 0; it < ITER; ++it) {
     const int h = h0 + it * kGroups;
-    if (h < n_heads) x[it] = *reinterpret_cast<const uint4*>(row + static_cast<int64_t>(h) * D);
+    if (h < n_heads) {
+      xa[it] = __ldcs(reinterpret_cast<const uint4*>(row + static_cast<int64_t>(h) * D + ea));
+      xb[it] = __ldcs(reinterpret_cast<const uint4*>(row + static_cast<int64_t>(h) * D + eb));
+    }
   }
-  int64_t pos = p.positions[token];
-  int64_t slot = p.slots[token];
+  int64_t pos = __ldg(p.positions + token);
+  int64_t slot = __ldg(p.slots + token);
   if (pos < 0 || pos >= p.n_positions || slot >= p.n_slots) {
     if (lane == 0) atomicOr(&g_status, kStatusBadIndex);
     pos = pos < 0 ? 0 : (pos >= p.n_positions ? p.n_positions - 1 : pos);
     if (slot >= p.n_slots) slot = -1;
   }
   const int half = p.rot / 2;
-  // This lane's table entries: the pair that element e belongs to, and the
-  // sign of its partner's term.
-  float cs[8], sn[8];
-  const float* cr = p.cosv + pos * half;
-  const float* sr = p.sinv + pos * half;
-  if (h0 - grp < p.hq + p.hkv) {
+  // Table entries of the lane's eight pairs (uneven: of its sixteen values).
+  constexpr int kTab = LAYOUT == kUneven ? 16 : 8;
+  float cs[kTab], sn[kTab];
+  if (h0 - grp < rotated) {
+    const float* cr = p.cosv + pos * half;
+    const float* sr = p.sinv + pos * half;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const int i = c * 8 + e;
-      cs[e] = 1.f;
-      sn[e] = 0.f;
-      if (i < p.rot) {
-        const bool lo = p.interleaved ? (i & 1) == 0 : i < half;
-        const int pair = p.interleaved ? i >> 1 : (lo ? i : i - half);
-        cs[e] = __ldg(cr + pair);
-        sn[e] = lo ? -__ldg(sr + pair) : __ldg(sr + pair);
-      }
+    for (int e = 0; e < kTab; ++e) {
+      const int i = LAYOUT == kUneven ? (ea + e < half ? ea + e : ea + e - half) : 8 * c + e;
+      const bool in = LAYOUT == kUneven ? ea + e < p.rot : i < half;
+      cs[e] = in ? __ldg(cr + i) : 1.f;
+      sn[e] = in ? __ldg(sr + i) : 0.f;
     }
   }
   const int64_t page = slot >> p.page_shift;
   const int64_t place = slot & ((int64_t(1) << p.page_shift) - 1);
-  const int64_t base = page * p.page_stride + place * p.row_stride + c * 8;
+  const int64_t base = page * p.page_stride + place * p.row_stride;
 #pragma unroll
   for (int it = 0; it < ITER; ++it) {
     const int h = h0 + it * kGroups;
-    // A group's lanes hold one head and a warp's groups neighbouring ones: the
-    // shuffles below are taken by the whole warp.
-    const bool rotated = h < p.hq + p.hkv;
     const bool is_k = h >= p.hq;
-    float f[8], o[8];
-    const uint32_t* xw = reinterpret_cast<const uint32_t*>(&x[it]);
+    // (Warp-uniform: the shuffles below are taken by the whole warp.)
+    if (h - grp < rotated) {
+      float a[8], b[8];
+      unpack8<E>(h < n_heads ? xa[it] : make_uint4(0u, 0u, 0u, 0u), a);
+      unpack8<E>(h < n_heads ? xb[it] : make_uint4(0u, 0u, 0u, 0u), b);
+      float r = 1.f;
+      if (p.q_norm) {
+        float ss = 0.f;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const float2 t = h < n_heads ? Elem<E>::unpack(xw[e]) : make_float2(0.f, 0.f);
-      f[2 * e] = t.x;
-      f[2 * e + 1] = t.y;
-    }
-    const E* nw = is_k ? p.k_norm : p.q_norm;
-    float r = 1.f;
-    if (p.q_norm) {
-      float ss = 0.f;
+        for (int e = 0; e < 8; ++e) ss = fmaf(a[e], a[e], fmaf(b[e], b[e], ss));
 #pragma unroll
-      for (int e = 0; e < 8; ++e) ss = fmaf(f[e], f[e], ss);
+        for (int off = kLanes / 2; off >= 1; off >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, off);
+        r = rsqrtf(fmaf(ss, 1.f / D, p.eps));
+        float wa[8], wb[8];
+        const E* nw = is_k ? p.k_norm : p.q_norm;
+        unpack8<E>(__ldg(reinterpret_cast<const uint4*>(nw + ea)), wa);
+        unpack8<E>(__ldg(reinterpret_cast<const uint4*>(nw + eb)), wb);
 #pragma unroll
-      for (int off = kLanes / 2; off >= 1; off >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, off);
-      r = rsqrtf(ss * (1.f / D) + p.eps);
-      const uint4 wv = *reinterpret_cast<const uint4*>(nw + c * 8);
-      const uint32_t* ww = reinterpret_cast<const uint32_t*>(&wv);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float2 t = Elem<E>::unpack(ww[e]);
-        f[2 * e] *= r * t.x;
-        f[2 * e + 1] *= r * t.y;
-      }
-    }
-    if (ALIGNED && !p.interleaved) {
-      // Lane c + half / 8 (or c - half / 8) of the group holds the partners.
-      const int dist = half >> 3;
-      const int src = c * 8 < half ? c + dist : (c * 8 < p.rot ? c - dist : c);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) o[e] = __shfl_sync(0xffffffffu, f[e], src, kLanes);
-    } else if (p.interleaved) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) o[e] = f[e ^ 1];
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int i = c * 8 + e;
-        o[e] = 0.f;
-        if (rotated && i < p.rot) {
-          const int j = i < half ? i + half : i - half;
-          o[e] = Elem<E>::load(row + static_cast<int64_t>(h) * D - c * 8 + j);
-          if (p.q_norm) o[e] *= r * Elem<E>::load(nw + j);
+        for (int e = 0; e < 8; ++e) {
+          a[e] *= r * wa[e];
+          b[e] *= r * wb[e];
         }
+      }
+      if (h < rotated) {
+        if (LAYOUT == kHalf) {
+          if (pairs) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const float x = a[e], y = b[e];
+              a[e] = fmaf(x, cs[e], -(y * sn[e]));
+              b[e] = fmaf(y, cs[e], x * sn[e]);
+            }
+          }
+        } else if (LAYOUT == kInterleaved) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            float* t = e < 4 ? a + 2 * e : b + 2 * (e - 4);
+            if (8 * c + e < half) {
+              const float x = t[0], y = t[1];
+              t[0] = fmaf(x, cs[e], -(y * sn[e]));
+              t[1] = fmaf(y, cs[e], x * sn[e]);
+            }
+          }
+        } else {
+          const E* head = row + static_cast<int64_t>(h) * D;
+          const E* nw = is_k ? p.k_norm : p.q_norm;
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const int i = ea + e, j = i < half ? i + half : i - half;
+            float* t = e < 8 ? a + e : b + e - 8;
+            if (i < p.rot) {
+              float y = Elem<E>::load(head + j);
+              if (p.q_norm) y *= r * Elem<E>::load(nw + j);
+              *t = fmaf(*t, cs[e % kTab], i < half ? -(y * sn[e % kTab]) : y * sn[e % kTab]);
+            }
+          }
+        }
+        xa[it] = pack8<E>(a);
+        xb[it] = pack8<E>(b);
       }
     }
     if (h >= n_heads) continue;
-    uint4 y = x[it];
-    if (rotated) {
-      uint32_t* yw = reinterpret_cast<uint32_t*>(&y);
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (c * 8 + e < p.rot) f[e] = fmaf(o[e], sn[e], f[e] * cs[e]);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) yw[e] = Elem<E>::pack(f[2 * e], f[2 * e + 1]);
-    }
+    E* dst;
     if (!is_k) {
-      *reinterpret_cast<uint4*>(p.q_out + (token * p.hq + h) * D + c * 8) = y;
-    } else if (slot >= 0) {
-      const int kh = rotated ? h - p.hq : h - p.hq - p.hkv;
-      *reinterpret_cast<uint4*>((rotated ? p.k : p.v) + base + kh * p.head_stride) = y;
+      dst = p.q_out + (token * p.hq + h) * D;
+    } else {
+      if (slot < 0) continue;
+      dst = h < rotated ? p.k + base + (h - p.hq) * p.head_stride : p.v + base + (h - rotated) * p.head_stride;
     }
+    *reinterpret_cast<uint4*>(dst + ea) = xa[it];
+    *reinterpret_cast<uint4*>(dst + eb) = xb[it];
   }
 }
 
 template <typename E, int D, int ITER>
-cudaError_t launch(const PagedPool& pool, const AppendArgs& a, bool aligned, cudaStream_t stream) {
+cudaError_t launch(const PagedPool& pool, const AppendArgs& a, cudaStream_t stream) {
   AppendParams<E> p;
   p.qkv = static_cast<const E*>(a.qkv);
   p.cosv = a.cosv;
@@ -196,8 +229,7 @@ cudaError_t launch(const PagedPool& pool, const AppendArgs& a, bool aligned, cud
   p.page_shift = 0;
   while ((1 << p.page_shift) < pool.page_size) ++p.page_shift;
   p.eps = a.eps;
-  p.interleaved = a.interleaved;
-  constexpr int kPer = ITER * 32 / (D / 8);
+  constexpr int kPer = ITER * 32 / (D / 16);
   p.chunks = (a.hq + 2 * pool.n_kv_heads + kPer - 1) / kPer;
   const int64_t warps = static_cast<int64_t>(a.T) * p.chunks;
   const int64_t blocks = (warps + kThreads / 32 - 1) / (kThreads / 32);
@@ -211,30 +243,30 @@ cudaError_t launch(const PagedPool& pool, const AppendArgs& a, bool aligned, cud
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return aligned ? cudaLaunchKernelEx(&cfg, paged_append_kernel<E, D, ITER, true>, p)
-                 : cudaLaunchKernelEx(&cfg, paged_append_kernel<E, D, ITER, false>, p);
+  if (a.interleaved) return cudaLaunchKernelEx(&cfg, paged_append_kernel<E, D, ITER, kInterleaved>, p);
+  if (a.rot % 16 == 0) return cudaLaunchKernelEx(&cfg, paged_append_kernel<E, D, ITER, kHalf>, p);
+  return cudaLaunchKernelEx(&cfg, paged_append_kernel<E, D, ITER, kUneven>, p);
 }
 
 template <typename E, int D>
-cudaError_t launch_iter(const PagedPool& pool, const AppendArgs& a, int num_sms, bool aligned,
+cudaError_t launch_iter(const PagedPool& pool, const AppendArgs& a, int num_sms,
                         cudaStream_t stream) {
-  // Four heads a lane group once that still fills the GPU's warps; below it
+  // kIter heads a lane group once that still fills the GPU's warps; below it
   // one, so that a few tokens spread over the SMs.
-  const int64_t groups = static_cast<int64_t>(a.T) * (a.hq + 2 * pool.n_kv_heads) * (D / 8) / 32;
-  if (groups >= 4 * 64 * static_cast<int64_t>(num_sms)) return launch<E, D, 4>(pool, a, aligned, stream);
-  return launch<E, D, 1>(pool, a, aligned, stream);
+  const int64_t groups = static_cast<int64_t>(a.T) * (a.hq + 2 * pool.n_kv_heads) * (D / 16) / 32;
+  if (groups >= kIter * 64 * static_cast<int64_t>(num_sms)) return launch<E, D, kIter>(pool, a, stream);
+  return launch<E, D, 1>(pool, a, stream);
 }
 
 }  // namespace
 
 cudaError_t launch_paged_append(const PagedPool& pool, const AppendArgs& a, int num_sms,
                                 cudaStream_t stream) {
-  const bool aligned = a.interleaved || a.rot % 16 == 0;
   if (pool.bf16)
-    return pool.D == 128 ? launch_iter<__nv_bfloat16, 128>(pool, a, num_sms, aligned, stream)
-                         : launch_iter<__nv_bfloat16, 64>(pool, a, num_sms, aligned, stream);
-  return pool.D == 128 ? launch_iter<__half, 128>(pool, a, num_sms, aligned, stream)
-                       : launch_iter<__half, 64>(pool, a, num_sms, aligned, stream);
+    return pool.D == 128 ? launch_iter<__nv_bfloat16, 128>(pool, a, num_sms, stream)
+                         : launch_iter<__nv_bfloat16, 64>(pool, a, num_sms, stream);
+  return pool.D == 128 ? launch_iter<__half, 128>(pool, a, num_sms, stream)
+                       : launch_iter<__half, 64>(pool, a, num_sms, stream);
 }
 
 }  // namespace dqg
