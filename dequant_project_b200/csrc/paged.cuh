@@ -80,6 +80,30 @@ __device__ __forceinline__ void fence_async_shared() {
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
 }
 
+// a / b of non-negative values; short where both fit 32 bits, as they mostly do.
+__device__ __forceinline__ long long quotient(long long a, long long b) {
+  if (((a | b) >> 32) == 0) return static_cast<uint32_t>(a) / static_cast<uint32_t>(b);
+  return a / b;
+}
+// `total` units of work in `ctas` equal shares: share c begins at unit
+// floor(c total / ctas).
+struct Shares {
+  long long total, each;
+  int ctas, rest;
+  __device__ __forceinline__ void set(long long units, int n) {
+    total = units;
+    ctas = n < units ? n : static_cast<int>(units);
+    each = ctas ? quotient(total, ctas) : 0;
+    rest = static_cast<int>(total - each * ctas);
+  }
+  __device__ __forceinline__ long long begin(int c) const {
+    return c * each + static_cast<uint32_t>(c * rest) / static_cast<uint32_t>(ctas);
+  }
+  __device__ __forceinline__ int holder(long long unit) const {  // the share that holds a unit
+    return static_cast<int>(quotient((unit + 1) * ctas - 1, total));
+  }
+};
+
 // A sequence's length, held to what its row of the table can address.
 __device__ __forceinline__ int clamped_len(const int32_t* lens, int b, int limit) {
   const int n = __ldg(lens + b);

@@ -80,8 +80,9 @@ __device__ __forceinline__ int tiles_of(int len) { return len > 0 ? (len + kTile
 
 // A CTA's share of the tiles: where it starts and how many it takes.
 struct Share {
-  int b, hv, x, ctas;
-  long long count, pos, total;
+  Shares all;
+  long long count, pos;
+  int b, hv, x;
 };
 
 // Taken by one whole warp.
@@ -95,15 +96,13 @@ __device__ __forceinline__ Share find_share(const Params& p, int cta, int n_ctas
   }
 #pragma unroll
   for (int off = 16; off >= 1; off >>= 1) total += __shfl_xor_sync(0xffffffffu, total, off);
-  total *= hv;
   Share s;
-  s.total = total;
-  s.ctas = n_ctas < total ? n_ctas : static_cast<int>(total);
+  s.all.set(total * hv, n_ctas);
   s.b = s.hv = s.x = 0;
   s.pos = s.count = 0;
-  if (cta >= s.ctas) return s;
-  s.pos = cta * total / s.ctas;
-  s.count = (cta + 1) * total / s.ctas - s.pos;
+  if (cta >= s.all.ctas) return s;
+  s.pos = s.all.begin(cta);
+  s.count = s.all.begin(cta + 1) - s.pos;
   long long before = 0;
   for (int b0 = 0; b0 < p.B; b0 += 32) {
     const int b = b0 + lane;
@@ -120,7 +119,7 @@ __device__ __forceinline__ Share find_share(const Params& p, int cta, int n_ctas
       const long long in = s.pos - (before + __shfl_sync(0xffffffffu, sum - nt * hv, l));
       const int n = __shfl_sync(0xffffffffu, nt, l);
       s.b = b0 + l;
-      s.hv = static_cast<int>(in / n);
+      s.hv = static_cast<int>(quotient(in, n));
       s.x = static_cast<int>(in - static_cast<long long>(s.hv) * n);
       break;
     }
@@ -152,7 +151,7 @@ struct Layout {
   static constexpr int kRing = kStages * 2 * kTileBytes;
   static constexpr int kMerge = kWarps * kMergeRows * D * 4;
   static constexpr int kQuery = 16 * D * 2;
-  static constexpr int kSmem = 1024 + kRing + kMerge + kQuery + kWarps * 16 * 8 + 2 * (kStages + kQuerySlots) * 8 + 64;
+  static constexpr int kSmem = 1024 + kRing + kMerge + kQuery + kWarps * 16 * 8 + 2 * (kStages + kQuerySlots) * 8 + 80;
 };
 
 template <typename E, int D>
@@ -386,8 +385,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
       if (s.x == 0 && (late || !whole)) {
         cut_first = true;
         if (threadIdx.x == 0) {
-          const long long end = s.pos + nt;
-          const int last = static_cast<int>((end * s.ctas - 1) / s.total);
+          const int last = s.all.holder(s.pos + nt - 1);
           p.desc[late ? id : blockIdx.x] =
               Desc{s.b, s.hv, whole ? -1 : static_cast<int>(blockIdx.x), last - static_cast<int>(blockIdx.x) + 1};
         }

@@ -39,7 +39,7 @@ constexpr int kBlock = 128;         // keys a block; rows a tile
 constexpr int kThreads = 384;       // 2 x 4 softmax warps; products, copies, two idle
 constexpr int kMmaWarp = 8, kCopyWarp = 9;
 constexpr float kMaxGrowth = 8.f;   // log2 of the largest weight
-constexpr int kItemUnits = 2;       // an item's start and end, in blocks' time
+constexpr int kItemKeys = 2 * kBlock;  // an item's start and end, in keys' time
 constexpr int kSegs = 4;            // segments described ahead
 
 struct Desc {  // a cut item, by the CTA that holds its first piece
@@ -151,30 +151,6 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
 }
 
 // ---------------------------------------------------------------- schedule
-// sum over i in [0, n) of floor((a i + b) / m), by the Euclid-like recursion
-// on (a, m) (lattice points under a line).
-__device__ __forceinline__ long long floor_sum(long long n, long long m, long long a, long long b) {
-  long long sum = 0;
-  while (n > 0) {
-    if (a >= m) {
-      sum += n * (n - 1) / 2 * (a / m);
-      a %= m;
-    }
-    if (b >= m) {
-      sum += n * (b / m);
-      b %= m;
-    }
-    const long long y = a * n + b;
-    if (y < m) break;
-    n = y / m;
-    b = y % m;
-    const long long t = m;
-    m = a;
-    a = t;
-  }
-  return sum;
-}
-
 struct Seq {  // one sequence's rows and keys
   int q0, ql, kv, pairs;
 };
@@ -204,23 +180,30 @@ __device__ __forceinline__ int limit_of(const Params& p, const Seq& s, int i) {
   return lim < 0 ? 0 : lim;
 }
 
-// Units of a sequence's first n pairs, for one KV head: their blocks, and
-// kItemUnits for each pair's start and end.
-__device__ __forceinline__ long long units_before(const Params& p, const Seq& s, int n) {
+// The cost of an item: the keys that its last token sees, and kItemKeys for its
+// start and end. (Keys, not blocks: their sum over a causal sequence's pairs is
+// a plain quadratic, which every CTA evaluates to find its share.)
+// Cost of a sequence's first n pairs, for one KV head.
+__device__ __forceinline__ long long cost_before(const Params& p, const Seq& s, int n) {
+  const long long start = static_cast<long long>(n) * kItemKeys;
   if (n <= 0) return 0;
-  const int last = blocks_of(s.kv);
-  if (!p.causal) return static_cast<long long>(n) * (last + kItemUnits);
-  const long long tokens = 2 * p.tq, off = s.kv - s.ql;
+  if (!p.causal) return start + static_cast<long long>(n) * s.kv;
+  const int tokens = 2 * p.tq, off = s.kv - s.ql;
   const int full = n < s.pairs ? n : s.pairs - 1;  // the last pair ends at kv
-  long long one = off <= kBlock ? (kBlock - off) / tokens : 0;  // pairs that see one block at most
-  if (one > full) one = full;
-  return one + floor_sum(full - one, kBlock, tokens, off + (one + 1) * tokens + kBlock - 1) +
-         (n == s.pairs ? last : 0) + static_cast<long long>(n) * kItemUnits;
+  const int none = off < 0 ? min(full, -off / tokens) : 0;  // pairs that see no key
+  const long long k = full - none;
+  const long long first = off + static_cast<long long>(none) * tokens;
+  return start + k * first + k * (k + 1) / 2 * tokens + (n == s.pairs ? s.kv : 0);
+}
+// The block where a cut `unit` units into an item falls.
+__device__ __forceinline__ int cut_block(int unit) {
+  return unit < kItemKeys ? 0 : (unit - kItemKeys + kBlock / 2) / kBlock;
 }
 
 struct Share {  // a CTA's part of the units; x: the first one's place in its item
-  int b, kvh, pair, x, ctas;
-  long long count, pos, total;
+  Shares all;
+  long long count, pos;
+  int b, kvh, pair, x;
 };
 
 // Taken by one whole warp.
@@ -231,27 +214,27 @@ __device__ __forceinline__ Share find_share(const Params& p, int cta, int n_ctas
     const int b = b0 + lane;
     if (b < p.B) {
       const Seq s = load_seq(p, b);
-      total += units_before(p, s, s.pairs);
+      total += cost_before(p, s, s.pairs);
     }
   }
 #pragma unroll
   for (int off = 16; off >= 1; off >>= 1) total += __shfl_xor_sync(0xffffffffu, total, off);
-  total *= p.hkv;
   Share r;
-  r.total = total;
-  r.ctas = n_ctas < total ? n_ctas : static_cast<int>(total);
+  // Shares of a block at least, so that none inside an item comes to nothing.
+  total *= p.hkv;
+  r.all.set(total, static_cast<int>(max(1ll, min(static_cast<long long>(n_ctas), total / kBlock))));
   r.b = r.kvh = r.pair = r.x = 0;
   r.pos = r.count = 0;
-  if (cta >= r.ctas) return r;
-  r.pos = cta * total / r.ctas;
-  r.count = (cta + 1) * total / r.ctas - r.pos;
+  if (cta >= r.all.ctas) return r;
+  r.pos = r.all.begin(cta);
+  r.count = r.all.begin(cta + 1) - r.pos;
   long long before = 0;
   for (int b0 = 0; b0 < p.B; b0 += 32) {
     const int b = b0 + lane;
     long long mine = 0;
     if (b < p.B) {
       const Seq s = load_seq(p, b);
-      mine = units_before(p, s, s.pairs);
+      mine = cost_before(p, s, s.pairs);
     }
     long long sum = mine * p.hkv;
 #pragma unroll
@@ -265,20 +248,20 @@ __device__ __forceinline__ Share find_share(const Params& p, int cta, int n_ctas
       const long long per = __shfl_sync(0xffffffffu, mine, l);
       long long in = r.pos - (before + __shfl_sync(0xffffffffu, sum, l) - per * p.hkv);
       r.b = b0 + l;
-      r.kvh = static_cast<int>(in / per);
+      r.kvh = static_cast<int>(quotient(in, per));
       in -= r.kvh * per;
       // The pair: 32 probes a round.
       const Seq s = load_seq(p, r.b);
       int lo = 0, hi = s.pairs;
       while (hi - lo > 1) {
-        const int step = (hi - lo + 31) / 32;
+        const int step = (hi - lo + 31) >> 5;
         const int probe = min(lo + (lane + 1) * step, hi);
-        const int f = __ffs(__ballot_sync(0xffffffffu, units_before(p, s, probe) > in)) - 1;
+        const int f = __ffs(__ballot_sync(0xffffffffu, cost_before(p, s, probe) > in)) - 1;
         hi = min(lo + (f + 1) * step, hi);
         lo = lo + f * step;
       }
       r.pair = lo;
-      r.x = static_cast<int>(in - units_before(p, s, lo));
+      r.x = static_cast<int>(in - cost_before(p, s, lo));
       break;
     }
     before += __shfl_sync(0xffffffffu, sum, 31);
@@ -305,8 +288,8 @@ struct Walk {
   Share r;
   Seq s;
   int piece;
-  __device__ __forceinline__ void begin(const Params& p, const Share& share) {
-    r = share;
+  __device__ __forceinline__ void begin(const Params& p) {
+    if (!p.splits) r = find_share(p, blockIdx.x, gridDim.x);
     piece = blockIdx.x;
     if (p.splits || r.count > 0) s = load_seq(p, p.splits ? 0 : r.b);
   }
@@ -341,15 +324,22 @@ struct Walk {
       g.kvh = r.kvh;
       tiles(p, g, r.pair);
       const int n = max(g.n0, g.n1);
-      const int end = r.x + static_cast<int>(min(static_cast<long long>(n + kItemUnits - r.x), r.count));
-      g.x0 = max(0, r.x - kItemUnits);
-      g.x1 = max(0, end - kItemUnits);
+      const int seen = max(0, limit_of(p, s, g.tok0 - s.q0 + g.ntok - 1));
+      const int cost = seen + kItemKeys;
+      const int end = static_cast<int>(min(static_cast<long long>(cost), r.x + r.count));
+      g.x0 = min(n, cut_block(r.x));
+      g.x1 = end == cost ? n : min(n, cut_block(end));
       g.whole = g.x0 == 0 && g.x1 == n;
       g.slot = 2 * blockIdx.x + (g.x0 > 0 ? 0 : 1);
       g.pieces = 0;
-      const long long item_end = r.pos - r.x + n + kItemUnits;
-      if (!g.whole && g.x0 == 0 && g.x1 > 0)
-        g.pieces = static_cast<int>((item_end * r.ctas - 1) / r.total) - static_cast<int>(blockIdx.x) + 1;
+      if (!g.whole && g.x0 == 0 && g.x1 > 0) {
+        // The last piece lies with the holder of the item's last unit, unless
+        // that one's cut falls behind the last block.
+        const long long start = r.pos - r.x;
+        const int last = r.all.holder(start + cost - 1);
+        g.pieces = last - static_cast<int>(blockIdx.x) + 1 -
+                   (cut_block(static_cast<int>(r.all.begin(last) - start)) >= n ? 1 : 0);
+      }
       r.pos += end - r.x;
       r.count -= end - r.x;
       r.x = 0;
@@ -400,8 +390,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* seg_full = o_full + 2;       // [kSegs]
   uint64_t* seg_empty = seg_full + kSegs;
   uint64_t* drained = seg_empty + kSegs;
-  Share* share = reinterpret_cast<Share*>(drained + 1);
-  Segment* segs = reinterpret_cast<Segment*>(share + 1);  // [kSegs]
+  Segment* segs = reinterpret_cast<Segment*>(drained + 1);  // [kSegs]
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(segs + kSegs);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t sbase = smem_u32(smem);
@@ -444,15 +433,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     fence_async_shared();
   }
-  pdl_wait_prior_grid();
-  if (warp == 0) {
-    Share s = {};
-    if (!p.splits) s = find_share(p, blockIdx.x, gridDim.x);
-    if (lane == 0) *share = s;
-  }
   fence_before_sync();
   __syncthreads();
   fence_after_sync();
+  pdl_wait_prior_grid();
   pdl_launch_dependents();
   const uint32_t tmem = *tmem_slot;
   // Registers: a softmax thread holds a row of 128 scores. 384 x 168 at
@@ -462,7 +446,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (warp == kCopyWarp) {
     // ---- copies: queries per segment, then key and value blocks in turn.
     Walk walk;
-    walk.begin(p, *share);
+    walk.begin(p);
     Segment g;
     const int per = p.box_rows, boxes = kBlock / per * (D / 64);
     const int half = lane % (D / 64), sub = lane / (D / 64);
@@ -802,49 +786,62 @@ __global__ void __launch_bounds__(kThreads, 1)
 }
 
 // Joins the pieces of the item whose first piece CTA blockIdx.x holds: 32 rows
-// a block, a lane a row.
+// a block, a lane a row, a warp eight columns.
 template <typename E, int D>
-__global__ void __launch_bounds__(256) prompt_join_kernel(const __grid_constant__ Params p) {
+__global__ void __launch_bounds__(32 * (D / 8)) prompt_join_kernel(const __grid_constant__ Params p) {
   pdl_wait_prior_grid();
   pdl_launch_dependents();
   const int4 d = __ldcg(reinterpret_cast<const int4*>(p.desc + blockIdx.x));
   const int tok0 = d.x, ntok = d.y, kvh = d.z, pieces = d.w;
   if (pieces == 0) return;
-  const int row = blockIdx.y * 32 + (threadIdx.x & 31), r = row & 127;
+  const int row = blockIdx.y * 32 + (threadIdx.x & 31), r = row & 127, d8 = threadIdx.x >> 5;
   const int tok = (row >> 7) * p.tq + r / p.g;
   if (r >= p.tq * p.g || tok >= ntok) return;
-  // Piece 0 lies in this CTA's second slot, piece i > 0 in CTA + i's first.
-  auto slot_of = [&](int i) { return 2 * (static_cast<int64_t>(blockIdx.x) + i) + (i == 0 ? 1 : 0); };
-  float m = -INFINITY;
-  for (int i = 0; i < pieces; ++i) m = fmaxf(m, __ldcg(p.ml + slot_of(i) * 512 + row));
-  const float ref = m == -INFINITY ? 0.f : m;
-  E* out = static_cast<E*>(p.out) +
-           (static_cast<int64_t>(tok0 + tok) * p.hq + kvh * p.g + r % p.g) * D;
-  for (int d8 = threadIdx.x >> 5; d8 < D / 8; d8 += 8) {
-    float den = 0.f, acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-    for (int i = 0; i < pieces; ++i) {
-      const int64_t sl = slot_of(i);
-      const float f = exp2_approx(__ldcg(p.ml + sl * 512 + row) - ref);
-      den = fmaf(__ldcg(p.ml + sl * 512 + 256 + row), f, den);
-      const float4 a = __ldcg(p.part + (sl * (D / 4) + 2 * d8) * 256 + row);
-      const float4 b = __ldcg(p.part + (sl * (D / 4) + 2 * d8 + 1) * 256 + row);
-      acc[0] = fmaf(a.x, f, acc[0]);
-      acc[1] = fmaf(a.y, f, acc[1]);
-      acc[2] = fmaf(a.z, f, acc[2]);
-      acc[3] = fmaf(a.w, f, acc[3]);
-      acc[4] = fmaf(b.x, f, acc[4]);
-      acc[5] = fmaf(b.y, f, acc[5]);
-      acc[6] = fmaf(b.z, f, acc[6]);
-      acc[7] = fmaf(b.w, f, acc[7]);
-    }
-    const float inv = den == 0.f ? 0.f : __frcp_rn(den);
-    uint4 w;
-    uint32_t* ww = reinterpret_cast<uint32_t*>(&w);
+  constexpr int kBatch = 4;  // pieces whose loads are in flight together
+  float m = -INFINITY, den = 0.f, acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  for (int i0 = 0; i0 < pieces; i0 += kBatch) {
+    float pm[kBatch], pl[kBatch];
+    float4 a[kBatch], b[kBatch];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) ww[e] = Elem<E>::pack(acc[2 * e] * inv, acc[2 * e + 1] * inv);
-    *reinterpret_cast<uint4*>(out + 8 * d8) = w;
+    for (int u = 0; u < kBatch; ++u) {
+      const int i = i0 + u;
+      pm[u] = -INFINITY;
+      pl[u] = 0.f;
+      a[u] = b[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (i < pieces) {
+        // Piece 0 lies in this CTA's second slot, piece i > 0 in CTA + i's first.
+        const int64_t sl = 2 * (static_cast<int64_t>(blockIdx.x) + i) + (i == 0 ? 1 : 0);
+        pm[u] = __ldcg(p.ml + sl * 512 + row);
+        pl[u] = __ldcg(p.ml + sl * 512 + 256 + row);
+        a[u] = __ldcg(p.part + (sl * (D / 4) + 2 * d8) * 256 + row);
+        b[u] = __ldcg(p.part + (sl * (D / 4) + 2 * d8 + 1) * 256 + row);
+      }
+    }
+    float mx = m;
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) mx = fmaxf(mx, pm[u]);
+    const float ref = mx == -INFINITY ? 0.f : mx;
+    float f = exp2_approx(m - ref);
+    m = mx;
+    den *= f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) acc[e] *= f;
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+      f = exp2_approx(pm[u] - ref);
+      den = fmaf(pl[u], f, den);
+      const float v[8] = {a[u].x, a[u].y, a[u].z, a[u].w, b[u].x, b[u].y, b[u].z, b[u].w};
+#pragma unroll
+      for (int e = 0; e < 8; ++e) acc[e] = fmaf(v[e], f, acc[e]);
+    }
   }
+  const float inv = den == 0.f ? 0.f : __frcp_rn(den);
+  uint4 w;
+  uint32_t* ww = reinterpret_cast<uint32_t*>(&w);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) ww[e] = Elem<E>::pack(acc[2 * e] * inv, acc[2 * e + 1] * inv);
+  *reinterpret_cast<uint4*>(static_cast<E*>(p.out) +
+                            (static_cast<int64_t>(tok0 + tok) * p.hq + kvh * p.g + r % p.g) * D + 8 * d8) = w;
 }
 
 template <typename E, int D>
@@ -873,7 +870,7 @@ cudaError_t launch(const Params& p, const CUtensorMap& qmap, const CUtensorMap& 
   e = cudaLaunchKernelEx(&cfg, prompt_kernel<E, D>, p, qmap, kmap, vmap);
   if (e != cudaSuccess || p.splits) return e;
   cfg.gridDim = dim3(num_sms, 8);
-  cfg.blockDim = dim3(256);
+  cfg.blockDim = dim3(32 * (D / 8));
   cfg.dynamicSmemBytes = 0;
   return cudaLaunchKernelEx(&cfg, prompt_join_kernel<E, D>, p);
 }
