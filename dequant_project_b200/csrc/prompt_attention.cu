@@ -39,6 +39,7 @@ constexpr int kBlock = 128;         // keys a block; rows a tile
 constexpr int kThreads = 384;       // 2 x 4 softmax warps; products, copies, two idle
 constexpr int kMmaWarp = 8, kCopyWarp = 9;
 constexpr float kMaxGrowth = 8.f;   // log2 of the largest weight
+constexpr int kEarly = 96;          // keys whose weights are handed over first
 constexpr int kItemKeys = 2 * kBlock;  // an item's start and end, in keys' time
 constexpr int kSegs = 4;            // segments described ahead
 
@@ -121,6 +122,13 @@ __device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t* r) {
       "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
       "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31};" ::DQG_R8(r, 0),
       DQG_R8(r, 8), DQG_R8(r, 16), DQG_R8(r, 24), "r"(addr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15};" ::DQG_R8(r, 0),
+      DQG_R8(r, 8), "r"(addr)
       : "memory");
 }
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
@@ -522,13 +530,13 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       mma_commit(s_full + t);
     };
-    auto issue_o = [&](int t, int slot, int half, bool add) {
+    auto issue_o = [&](int t, int slot, bool late, bool add) {
       if (!one) return;
       const uint64_t b = v_desc + slot * (L::kSlot >> 4);
 #pragma unroll
-      for (int i = 0; i < kBlock / 32; ++i) {
-        const int k = half * (kBlock / 32) + i;
-        mma_ts(tmem + 2 * kBlock + t * D, tmem + t * kBlock + k * 8, b + (k * 16 * 128 >> 4), kIdO, add || k > 0);
+      for (int k = 0; k < kBlock / 16; ++k) {
+        if ((k < kEarly / 16) != late)
+          mma_ts(tmem + 2 * kBlock + t * D, tmem + t * kBlock + k * 8, b + (k * 16 * 128 >> 4), kIdO, add || k > 0);
       }
     };
     auto commit = [&](uint64_t* bar) {
@@ -580,11 +588,11 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (!ok || j >= c) continue;
           ok = wait(p_half + t, weights >> t & 1);
           if (!ok) continue;
-          issue_o(t, vslot, 0, j > 0);
+          issue_o(t, vslot, false, j > 0);
           ok = wait(p_full + t, weights >> t & 1);
           weights ^= 1u << t;
           if (!ok) continue;
-          issue_o(t, vslot, 1, true);
+          issue_o(t, vslot, true, true);
           if (j + 1 < c) issue_s(t, kslot);
           else commit(o_full + t);
         }
@@ -683,23 +691,33 @@ __global__ void __launch_bounds__(kThreads, 1)
         const float ref = m == -INFINITY ? 0.f : m * p.scale_log2;
         const float2 ref2 = make_float2(-ref, -ref);
         float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-        // The products take the first half of the weights while the second is
-        // still being formed.
+        // The products take the first kEarly weights while the rest is formed.
+        auto weigh = [&](int from, uint32_t* w, int n) {
 #pragma unroll
-        for (int hq = 0; hq < 2; ++hq) {
-          uint32_t w[32];
-#pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            float2 x = fma2(make_float2(s[64 * hq + 2 * i], s[64 * hq + 2 * i + 1]), scale2, ref2);
+          for (int i = 0; i < n / 2; ++i) {
+            float2 x = fma2(make_float2(s[from + 2 * i], s[from + 2 * i + 1]), scale2, ref2);
             x.x = exp2_approx(x.x);
             x.y = exp2_approx(x.y);
             sum[i & 1] = add2(sum[i & 1], x);
             w[i] = Elem<E>::pack(x.x, x.y);
           }
-          tmem_st32(ts + 32 * hq, w);
+        };
+        {
+          uint32_t w[kEarly / 2];
+          weigh(0, w, kEarly);
+          tmem_st32(ts, w);
+          tmem_st16(ts + 32, w + 32);
           tmem_wait_st();
           fence_before_sync();
-          mbar_arrive((hq ? p_full : p_half) + t);
+          mbar_arrive(p_half + t);
+        }
+        {
+          uint32_t w[(kBlock - kEarly) / 2];
+          weigh(kEarly, w, kBlock - kEarly);
+          tmem_st16(ts + kEarly / 2, w);
+          tmem_wait_st();
+          fence_before_sync();
+          mbar_arrive(p_full + t);
         }
         l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
       }
