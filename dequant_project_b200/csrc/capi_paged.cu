@@ -260,7 +260,7 @@ int dqg_paged_attention(const void* q, int64_t q_stride_seq, int64_t q_stride_he
   int dev = 0, sms = 0;
   if ((rc = current(&dev, &sms)) != DQG_OK) return rc;
   if ((rc = check_workspace(workspace, workspace_bytes, dqg::paged_decode_workspace(static_cast<int>(n_seqs), static_cast<int>(n_q_heads), pool.n_kv_heads,
-                                                    pool.D, false, sms))) != DQG_OK)
+                                                    pool.D, 0, sms))) != DQG_OK)
     return rc;
   CUtensorMap kmap, vmap;
   if ((rc = pool_maps(pool, dqg::paged_decode_box_rows(pool.page_size), &kmap, &vmap)) != DQG_OK) return rc;
@@ -356,10 +356,13 @@ int dqg_shared_prefix_workspace(int64_t n_seqs, int64_t n_q_heads, int64_t n_kv_
     return api_fail(DQG_ERR_INVALID, "prefix_len=%lld out of range", (ll)prefix_len);
   int dev = 0, sms = 0;
   if ((rc = current(&dev, &sms)) != DQG_OK) return rc;
-  const bool prefix = prefix_len > 0 && n_seqs > 0;
+  const bool pieces = prefix_len > 0 && n_seqs > 0 &&
+                      !dqg::prefix_streamed(static_cast<int>(n_seqs), static_cast<int>(n_q_heads),
+                                            static_cast<int>(n_kv_heads));
   *bytes = dqg::paged_decode_workspace(static_cast<int>(n_seqs), static_cast<int>(n_q_heads),
-                                       static_cast<int>(n_kv_heads), static_cast<int>(head_dim), prefix, sms);
-  if (prefix)
+                                       static_cast<int>(n_kv_heads), static_cast<int>(head_dim),
+                                       static_cast<int>(prefix_len), sms);
+  if (pieces)
     *bytes += dqg::prefix_workspace(static_cast<int>(n_seqs), static_cast<int>(n_q_heads),
                                     static_cast<int>(n_kv_heads), static_cast<int>(head_dim),
                                     static_cast<int>(prefix_len), sms);
@@ -396,8 +399,10 @@ int dqg_shared_prefix_attention(const void* q, int64_t q_stride_seq, int64_t q_s
   dqg::DecodeArgs d;
   std::memset(&d, 0, sizeof(d));
   d.workspace = workspace;
+  d.prefix_len = static_cast<int>(prefix_len);
+  d.prefix_table = prefix_table;
   CUtensorMap qmap, kmap, vmap;
-  if (prefix_len > 0) {
+  if (prefix_len > 0 && !dqg::prefix_streamed(static_cast<int>(n_seqs), static_cast<int>(n_q_heads), pool.n_kv_heads)) {
     dqg::PromptArgs a;
     std::memset(&a, 0, sizeof(a));
     a.table = prefix_table;
@@ -406,7 +411,7 @@ int dqg_shared_prefix_attention(const void* q, int64_t q_stride_seq, int64_t q_s
     // The decode kernel's scratch first, the prefix's pieces behind it.
     a.workspace = static_cast<uint8_t*>(workspace) +
                   dqg::paged_decode_workspace(static_cast<int>(n_seqs), static_cast<int>(n_q_heads),
-                                              pool.n_kv_heads, pool.D, true, sms);
+                                              pool.n_kv_heads, pool.D, static_cast<int>(prefix_len), sms);
     a.B = 1;
     a.T = static_cast<int>(n_seqs);
     a.hq = static_cast<int>(n_q_heads);

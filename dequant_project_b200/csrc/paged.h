@@ -56,9 +56,14 @@ struct DecodeArgs {
   void* workspace;
   int B, hq;
   float scale_log2;
-  PrefixPieces prefix;
+  int prefix_len;               // a shared prefix: 0 for none
+  const int32_t* prefix_table;
+  PrefixPieces prefix;          // its pieces, where the prompt kernel took it
 };
-size_t paged_decode_workspace(int B, int hq, int n_kv_heads, int D, bool prefix, int num_sms);
+size_t paged_decode_workspace(int B, int hq, int n_kv_heads, int D, int prefix_len, int num_sms);
+// Whether the decode kernel streams a prefix itself (else the prompt kernel
+// takes it, and DecodeArgs::prefix its pieces).
+bool prefix_streamed(int n_seqs, int hq, int n_kv_heads);
 cudaError_t launch_paged_decode(const PagedPool& pool, const CUtensorMap& kmap,
                                 const CUtensorMap& vmap, const DecodeArgs& a, int num_sms,
                                 cudaStream_t stream);

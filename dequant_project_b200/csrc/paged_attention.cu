@@ -21,6 +21,11 @@
 // pieces in order. No atomics: the same lengths give the same bits. Behind a
 // shared prefix every item leaves its result to the second kernel, which joins
 // it with the prefix's pieces: nothing here waits for those.
+//
+// A prefix whose rows (sequences times query heads of a KV head) fit two 16-row
+// tiles is streamed by this kernel itself, as items of its own ahead of the
+// sequences' (kStreamed in PrefixPieces); one with more rows is left to the
+// prompt kernel, which reads it once for 256 rows.
 #include <cstdint>
 
 #include "paged.cuh"
@@ -47,11 +52,14 @@ struct Params {
   void* out;
   const int32_t* table;
   const int32_t* lens;
-  float* part;   // [slot][rows][D]; two slots a CTA, then (behind a prefix) one an item
-  float* ml;     // [slot][2][rows]: maximum (log2 units), sum
-  Desc* desc;    // [CTA]; behind a prefix [item]
+  float* part;   // [row][D]: two pieces of `rows` rows a CTA, then (behind a prefix) whole results
+  float* m;      // [row]: maximum (log2 units)
+  float* l;      // [row]: sum
+  Desc* desc;    // [CTA]; behind a prefix [item], then [prefix item]
+  const int32_t* pre_table;
   int64_t q_stride_seq, q_stride_head, table_stride, n_pages;
   int B, hq, hkv, g, nrb, rows, page_shift, len_limit, box_rows, n_ctas;
+  int pre_len, pre_seqs, pre_tiles, pre_items;  // a streamed prefix: sequences an item; tiles; items
   float scale_log2;
   PrefixPieces prefix;
 };
@@ -97,13 +105,20 @@ __device__ __forceinline__ Share find_share(const Params& p, int cta, int n_ctas
 #pragma unroll
   for (int off = 16; off >= 1; off >>= 1) total += __shfl_xor_sync(0xffffffffu, total, off);
   Share s;
-  s.all.set(total * hv, n_ctas);
+  const long long pre = static_cast<long long>(p.pre_items) * p.pre_tiles;
+  s.all.set(total * hv + pre, n_ctas);
   s.b = s.hv = s.x = 0;
   s.pos = s.count = 0;
   if (cta >= s.all.ctas) return s;
   s.pos = s.all.begin(cta);
   s.count = s.all.begin(cta + 1) - s.pos;
-  long long before = 0;
+  if (s.pos < pre) {  // prefix items come first, as sequence -1
+    s.b = -1;
+    s.hv = static_cast<int>(quotient(s.pos, p.pre_tiles));
+    s.x = static_cast<int>(s.pos - static_cast<long long>(s.hv) * p.pre_tiles);
+    return s;
+  }
+  long long before = pre;
   for (int b0 = 0; b0 < p.B; b0 += 32) {
     const int b = b0 + lane;
     const int nt = b < p.B ? tiles_of(clamped_len(p.lens, b, p.len_limit)) : 0;
@@ -126,6 +141,52 @@ __device__ __forceinline__ Share find_share(const Params& p, int cta, int n_ctas
     before += __shfl_sync(0xffffffffu, sum, 31);
   }
   return s;
+}
+
+// An item as the share walks over it.
+struct Item {
+  const int32_t* table;
+  int len, tiles, kvh, head0, rows, first;  // first: the prefix's first sequence
+};
+__device__ __forceinline__ Item item_of(const Params& p, const Share& s) {
+  Item i;
+  if (s.b < 0) {
+    const int blocks = p.pre_items / p.hkv;
+    i.kvh = s.hv / blocks;
+    i.first = (s.hv - i.kvh * blocks) * p.pre_seqs;
+    i.len = p.pre_len;
+    i.tiles = p.pre_tiles;
+    i.table = p.pre_table;
+    i.head0 = i.kvh * p.g;
+    i.rows = min(p.pre_seqs, p.B - i.first) * p.g;
+  } else {
+    i.len = clamped_len(p.lens, s.b, p.len_limit);
+    i.tiles = tiles_of(i.len);
+    i.table = p.table + s.b * p.table_stride;
+    i.kvh = s.hv / p.nrb;
+    const int rb = s.hv - i.kvh * p.nrb;
+    i.head0 = i.kvh * p.g + rb * 16;
+    i.rows = min(16, p.g - rb * 16);
+    i.first = 0;
+  }
+  return i;
+}
+// Behind n tiles of the item at hand.
+__device__ __forceinline__ void advance(const Params& p, Share& s, int n) {
+  s.pos += n;
+  s.count -= n;
+  s.x = 0;
+  if (++s.hv == (s.b < 0 ? p.pre_items : p.hkv * p.nrb)) {
+    s.hv = 0;
+    ++s.b;
+  }
+}
+// First row of an item's whole result (see Params::part).
+__device__ __forceinline__ int64_t whole_row(const Params& p, int b, int hv) {
+  const int64_t cut = 2 * static_cast<int64_t>(p.n_ctas) * p.rows;
+  if (b < 0) return cut + static_cast<int64_t>(hv) * 16;
+  return cut + static_cast<int64_t>(p.pre_items) * 16 +
+         (static_cast<int64_t>(b) * p.hkv * p.nrb + hv) * min(16, p.g);
 }
 
 __device__ __forceinline__ void ldsm_x4(uint32_t addr, uint32_t* r) {
@@ -151,7 +212,7 @@ struct Layout {
   static constexpr int kRing = kStages * 2 * kTileBytes;
   static constexpr int kMerge = kWarps * kMergeRows * D * 4;
   static constexpr int kQuery = 16 * D * 2;
-  static constexpr int kSmem = 1024 + kRing + kMerge + kQuery + kWarps * 16 * 8 + 2 * (kStages + kQuerySlots) * 8 + 80;
+  static constexpr int kSmem = 1024 + kRing + kMerge + kQuery + kWarps * 16 * 8 + 2 * (kStages + kQuerySlots + 1) * 8 + 80;
 };
 
 template <typename E, int D>
@@ -171,7 +232,9 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
   uint64_t* empty = full + kStages;
   uint64_t* q_full = empty + kStages;
   uint64_t* q_empty = q_full + kQuerySlots;
-  Share* share = reinterpret_cast<Share*>(q_empty + kQuerySlots);
+  uint64_t* pre_full = q_empty + kQuerySlots;  // a streamed prefix's queries take all slots
+  uint64_t* pre_empty = pre_full + 1;
+  Share* share = reinterpret_cast<Share*>(pre_empty + 1);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int i = 0; i < kStages; ++i) {
@@ -182,6 +245,8 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
       mbar_init(q_full + i, 1);
       mbar_init(q_empty + i, kWarps);
     }
+    mbar_init(pre_full, 1);
+    mbar_init(pre_empty, kWarps);
     fence_mbar_init();
     tma_prefetch_map(&kmap);
     tma_prefetch_map(&vmap);
@@ -195,6 +260,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
   // behind this kernel).
   // waits (and with it everything behind this kernel).
   const bool late = p.prefix.S > 0;
+  const bool joined = late || p.pre_items > 0;  // results are joined with a prefix's
   if (!late) pdl_wait_prior_grid();
   if (warp == 0) {
     const Share s = find_share(p, blockIdx.x, gridDim.x);
@@ -203,8 +269,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
   __syncthreads();
   pdl_launch_dependents();
   Share s = *share;
-  const int n_hv = p.hkv * p.nrb;
-  const int q_slots = min(kQuerySlots, 16 / p.rows);
+  const int q_rows = min(16, p.g), q_slots = min(kQuerySlots, 16 / q_rows);
 
   if (warp == kWarps) {
     // ---- the copying warp: 16-row (or box_rows-row) pieces of page rows.
@@ -212,32 +277,38 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
     const int boxes = kTile / per * (D / 64);   // K boxes a tile; as many V boxes
     const int my = lane, half = my % (D / 64), sub = my / (D / 64);
     const uint64_t policy = policy_evict_last();
-    int it = 0, item = 0;
+    int it = 0, item = 0, pre = 0;
     bool ok = true;
     while (s.count > 0 && ok) {
-      const int raw = __ldg(p.lens + s.b);
-      const int len = clamped_len(p.lens, s.b, p.len_limit);
-      if (lane == 0 && raw != len) atomicOr(&g_status, kStatusBadIndex);
-      const int nt = tiles_of(len);
-      const int n = static_cast<int>(min(static_cast<long long>(nt - s.x), s.count));
-      const int32_t* row = p.table + s.b * p.table_stride;
-      const int kvh = s.hv / p.nrb, rb = s.hv - kvh * p.nrb;
-      const int rows = min(16, p.g - rb * 16);
+      const Item i = item_of(p, s);
+      const int n = static_cast<int>(min(static_cast<long long>(i.tiles - s.x), s.count));
       // The item's queries, a row a lane.
-      const int qi = item % q_slots;
-      if (item >= q_slots && !warp_wait(q_empty + qi, ((item / q_slots) & 1) ^ 1)) break;
-      if (lane == 0) mbar_arrive_expect_tx(q_full + qi, rows * D * 2);
-      __syncwarp();
-      if (lane < rows)
-        bulk_g2s(qs + (qi * p.rows + lane) * D * 2, static_cast<const E*>(p.q) + s.b * p.q_stride_seq +
-                 (kvh * p.g + rb * 16 + lane) * p.q_stride_head, D * 2, q_full + qi, policy);
-      ++item;
+      if (s.b < 0) {
+        if (pre > 0 && !warp_wait(pre_empty, (pre - 1) & 1)) break;
+        if (lane == 0) mbar_arrive_expect_tx(pre_full, i.rows * D * 2);
+        __syncwarp();
+        if (lane < i.rows)
+          bulk_g2s(qs + lane * D * 2, static_cast<const E*>(p.q) + (i.first + lane / p.g) * p.q_stride_seq +
+                   (i.head0 + lane % p.g) * p.q_stride_head, D * 2, pre_full, policy);
+        ++pre;
+      } else {
+        if (lane == 0 && __ldg(p.lens + s.b) != i.len) atomicOr(&g_status, kStatusBadIndex);
+        if (item == 0 && pre > 0 && !warp_wait(pre_empty, (pre - 1) & 1)) break;
+        const int qi = item % q_slots;
+        if (item >= q_slots && !warp_wait(q_empty + qi, ((item / q_slots) & 1) ^ 1)) break;
+        if (lane == 0) mbar_arrive_expect_tx(q_full + qi, i.rows * D * 2);
+        __syncwarp();
+        if (lane < i.rows)
+          bulk_g2s(qs + (qi * q_rows + lane) * D * 2, static_cast<const E*>(p.q) + s.b * p.q_stride_seq +
+                   (i.head0 + lane) * p.q_stride_head, D * 2, q_full + qi, policy);
+        ++item;
+      }
       for (int x = s.x; x < s.x + n; ++x, ++it) {
         const int st = it % kStages;
         const int t = x * kTile + sub * per;
         int page = static_cast<int>(p.n_pages);  // no such page: zeros
-        if (my < boxes && t < len) {
-          page = __ldg(row + (t >> p.page_shift));
+        if (my < boxes && t < i.len) {
+          page = __ldg(i.table + (t >> p.page_shift));
           if (page < 0 || page >= p.n_pages) {
             page = static_cast<int>(p.n_pages);
             atomicOr(&g_status, kStatusBadIndex);
@@ -252,15 +323,14 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
         if (my < boxes) {
           const uint32_t dst = smem_u32(smem) + st * 2 * L::kTileBytes + half * (kTile * 128) + sub * per * 128;
           const int in_page = t & ((1 << p.page_shift) - 1);
-          tma_load_4d(dst, &kmap, full + st, half * 64, in_page, kvh, page);
-          tma_load_4d(dst + L::kTileBytes, &vmap, full + st, half * 64, in_page, kvh, page);
+          tma_load_4d(dst, &kmap, full + st, half * 64, in_page, i.kvh, page);
+          tma_load_4d(dst + L::kTileBytes, &vmap, full + st, half * 64, in_page, i.kvh, page);
         }
       }
-      s.count -= n;
-      s.x = 0;
-      if (++s.hv == n_hv) { s.hv = 0; ++s.b; }
+      advance(p, s, n);
     }
     // Copies still in flight land before the CTA's memory goes (bounded).
+    if (pre > 0) warp_wait(pre_full, (pre - 1) & 1);
     for (int i = item < q_slots ? 0 : item - q_slots; i < item; ++i)
       if (!warp_wait(q_full + i % q_slots, (i / q_slots) & 1)) break;
     for (int i = it < kStages ? 0 : it - kStages; i < it; ++i)
@@ -269,25 +339,24 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
     const int gid = lane >> 2, c = lane & 3;
     const uint32_t ring = smem_u32(smem);
     const int p0 = warp * 16;
-    int it = 0, item = 0;
+    int it = 0, item = 0, pre = 0;
     bool ok = true, cut_first = false;
     while (s.count > 0 && ok) {
-      const int len = clamped_len(p.lens, s.b, p.len_limit);
-      const int nt = tiles_of(len);
+      const Item i = item_of(p, s);
+      const int len = i.len, nt = i.tiles, head0 = i.head0, rows = i.rows;
       const int n = static_cast<int>(min(static_cast<long long>(nt - s.x), s.count));
-      const int kvh = s.hv / p.nrb, rb = s.hv - kvh * p.nrb;
-      const int head0 = kvh * p.g + rb * 16;
-      const int rows = min(16, p.g - rb * 16);
-      // Q as A fragments: rows are the KV head's query heads.
+      // Q as A fragments: rows are the KV head's query heads (of several
+      // sequences, in a prefix).
       uint32_t qa[D / 16][4];
-      const int qi = item % q_slots;
-      if (!warp_wait(q_full + qi, (item / q_slots) & 1)) break;
-      ++item;
+      const int qi = s.b < 0 ? 0 : item % q_slots;
+      if (!(s.b < 0 ? warp_wait(pre_full, pre & 1) : warp_wait(q_full + qi, (item / q_slots) & 1))) break;
 #pragma unroll
       for (int ks = 0; ks < D / 16; ++ks)
-        ldsm_x4(smem_u32(qs) + (qi * p.rows + (lane & 15)) * (D * 2) + ks * 32 + (lane >> 4) * 16, qa[ks]);
+        ldsm_x4(smem_u32(qs) + (qi * q_rows + (lane & 15)) * (D * 2) + ks * 32 + (lane >> 4) * 16, qa[ks]);
       __syncwarp();
-      if (lane == 0) mbar_arrive(q_empty + qi);
+      if (lane == 0) mbar_arrive(s.b < 0 ? pre_empty : q_empty + qi);
+      if (s.b < 0) ++pre;
+      else ++item;
       float o[D / 8][4];
 #pragma unroll
       for (int nb = 0; nb < D / 8; ++nb) o[nb][0] = o[nb][1] = o[nb][2] = o[nb][3] = 0.f;
@@ -380,13 +449,15 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
         }
       }
       const bool whole = s.x == 0 && n == nt;
-      const int64_t id = static_cast<int64_t>(s.b) * n_hv + s.hv;
-      const int64_t slot = whole ? 2 * p.n_ctas + id : 2 * blockIdx.x + (s.x > 0 ? 0 : 1);
-      if (s.x == 0 && (late || !whole)) {
+      const int64_t row0 = whole ? whole_row(p, s.b, s.hv)
+                                 : (2 * static_cast<int64_t>(blockIdx.x) + (s.x > 0 ? 0 : 1)) * p.rows;
+      if (s.x == 0 && (joined || !whole)) {
         cut_first = true;
         if (threadIdx.x == 0) {
+          const int64_t items = static_cast<int64_t>(p.B) * p.hkv * p.nrb;
+          const int64_t id = s.b < 0 ? items + s.hv : static_cast<int64_t>(s.b) * p.hkv * p.nrb + s.hv;
           const int last = s.all.holder(s.pos + nt - 1);
-          p.desc[late ? id : blockIdx.x] =
+          p.desc[joined ? id : blockIdx.x] =
               Desc{s.b, s.hv, whole ? -1 : static_cast<int>(blockIdx.x), last - static_cast<int>(blockIdx.x) + 1};
         }
       }
@@ -420,25 +491,22 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
               num.z = fmaf(v.z, f, num.z);
               num.w = fmaf(v.w, f, num.w);
             }
-            if (whole && !late) {
+            if (whole && !joined) {
               store4<E, D>(p, s.b, head0 + row, d4, den, num);
             } else {
-              *reinterpret_cast<float4*>(p.part + (slot * p.rows + row) * D + d4 * 4) = num;
+              *reinterpret_cast<float4*>(p.part + (row0 + row) * D + d4 * 4) = num;
               if (d4 == 0) {
-                p.ml[slot * 2 * p.rows + row] = mx;
-                p.ml[(slot * 2 + 1) * p.rows + row] = den;
+                p.m[row0 + row] = mx;
+                p.l[row0 + row] = den;
               }
             }
           }
         }
         named_sync(1, 32 * kWarps);
       }
-      s.pos += nt - s.x;
-      s.count -= n;
-      s.x = 0;
-      if (++s.hv == n_hv) { s.hv = 0; ++s.b; }
+      advance(p, s, n);
     }
-    if (threadIdx.x == 0 && !cut_first && !late) p.desc[blockIdx.x] = Desc{0, 0, 0, 0};
+    if (threadIdx.x == 0 && !cut_first && !joined) p.desc[blockIdx.x] = Desc{0, 0, 0, 0};
   }
   if (late) pdl_wait_prior_grid();
 }
@@ -464,7 +532,22 @@ __global__ void __launch_bounds__(kJoinThreads)
   if (d.pieces == 0 || static_cast<int>(blockIdx.y) * R >= rows) return;
   const int cell = threadIdx.x % kCells, group = threadIdx.x / kCells;
   const int row = blockIdx.y * R + cell % R, d4 = cell / R;
-  const int own = d.pieces, all = own + p.prefix.S;
+  // A streamed prefix's pieces are described as an item's are.
+  Desc f{0, 0, 0, 0};
+  int f_row = 0;
+  if (p.pre_items) {
+    const int pid = kvh * (p.pre_items / p.hkv) + d.b / p.pre_seqs;
+    const int4 t = __ldcg(reinterpret_cast<const int4*>(p.desc + gridDim.x + pid));
+    f = Desc{t.x, t.y, t.z, t.w};
+    f_row = d.b % p.pre_seqs * p.g + row;
+  }
+  const int own = d.pieces, all = own + p.prefix.S + f.pieces;
+  // Piece 0 lies in its CTA's second place, piece i > 0 in CTA + i's first; a
+  // whole result in the item's own.
+  auto row_of = [&](const Desc& e, int i) {
+    return e.cta < 0 ? whole_row(p, e.b, e.hv)
+                     : (2 * (static_cast<int64_t>(e.cta) + i) + (i == 0 ? 1 : 0)) * p.rows;
+  };
   const int64_t pre = p.prefix.S ? prefix_first(p.prefix, p.hkv, d.b, kvh) : 0;
   const int pre_row = p.prefix.S ? prefix_row(p.prefix, p.g, d.b, rb * 16 + row) : 0;
   float m = -INFINITY, l = 0.f;
@@ -480,14 +563,11 @@ __global__ void __launch_bounds__(kJoinThreads)
         pm[u] = -INFINITY;
         pl[u] = 0.f;
         v[u] = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (i < own) {
-          // Piece 0 lies in its CTA's second slot, piece i > 0 in CTA + i's
-          // first; a whole result in the item's own.
-          const int64_t slot = d.cta < 0 ? 2 * p.n_ctas + blockIdx.x
-                                         : 2 * (static_cast<int64_t>(d.cta) + i) + (i == 0 ? 1 : 0);
-          pm[u] = __ldcg(p.ml + slot * 2 * p.rows + row);
-          pl[u] = __ldcg(p.ml + (slot * 2 + 1) * p.rows + row);
-          v[u] = __ldcg(reinterpret_cast<const float4*>(p.part + (slot * p.rows + row) * D) + d4);
+        if (i < own || (i < all && p.pre_items)) {
+          const int64_t at = i < own ? row_of(d, i) + row : row_of(f, i - own) + f_row;
+          pm[u] = __ldcg(p.m + at);
+          pl[u] = __ldcg(p.l + at);
+          v[u] = __ldcg(reinterpret_cast<const float4*>(p.part + at * D) + d4);
         } else if (i < all) {
           const int64_t s = pre + i - own;
           pm[u] = __ldcg(p.prefix.ml + s * 512 + pre_row);
@@ -565,10 +645,10 @@ cudaError_t launch(const Params& p, const CUtensorMap& kmap, const CUtensorMap& 
   if (e != cudaSuccess) return e;
   // Query heads a join block takes: few, so that the pieces of a small batch
   // spread over many threads, but one where there is one.
-  const int per = p.rows == 1 ? 1 : 4;
-  const int64_t items = p.prefix.S ? static_cast<int64_t>(p.B) * p.hkv * p.nrb : p.n_ctas;
+  const int rows = p.g < 16 ? p.g : 16, per = rows == 1 ? 1 : 4;
+  const int64_t items = p.prefix.S || p.pre_items ? static_cast<int64_t>(p.B) * p.hkv * p.nrb : p.n_ctas;
   if (items > 0x7fffffff) return cudaErrorInvalidValue;
-  cfg.gridDim = dim3(static_cast<unsigned>(items), (p.rows + per - 1) / per);
+  cfg.gridDim = dim3(static_cast<unsigned>(items), (rows + per - 1) / per);
   cfg.blockDim = dim3(kJoinThreads);
   cfg.dynamicSmemBytes = 0;
   return per == 1 ? cudaLaunchKernelEx(&cfg, paged_join_kernel<E, D, 1>, p)
@@ -580,28 +660,49 @@ cudaError_t launch(const Params& p, const CUtensorMap& kmap, const CUtensorMap& 
 int paged_decode_box_rows(int page_size) { return page_size < kTile ? page_size : kTile; }
 
 namespace {
-// Slots of pieces, and descriptions, of a launch: two and one a CTA; behind a
-// prefix one and one an item as well.
+// What a launch leaves between its kernels: rows of pieces and whole results,
+// and descriptions (see Params).
 struct Scratch {
-  size_t slots, descs, rows;
+  size_t rows, descs;
+  int per_piece, pre_items, pre_seqs;
 };
-Scratch scratch_of(int B, int hq, int n_kv_heads, bool prefix, int num_sms) {
-  const size_t g = hq / n_kv_heads, items = static_cast<size_t>(B) * n_kv_heads * ((g + 15) / 16);
+Scratch scratch_of(int B, int hq, int n_kv_heads, int prefix_len, int num_sms) {
+  const int g = hq / n_kv_heads, g16 = g < 16 ? g : 16;
+  const size_t items = static_cast<size_t>(B) * n_kv_heads * ((g + 15) / 16);
   const size_t ctas = static_cast<size_t>(kCtasPerSm) * num_sms;
-  return Scratch{2 * ctas + (prefix ? items : 0), prefix ? items : ctas, g < 16 ? g : 16};
+  Scratch s{2 * ctas * g16, ctas, g16, 0, 1};
+  if (prefix_len > 0) {
+    if (prefix_streamed(B, hq, n_kv_heads)) {
+      s.pre_seqs = 16 / g;
+      s.pre_items = (B + s.pre_seqs - 1) / s.pre_seqs * n_kv_heads;
+      s.per_piece = 16;
+      s.rows = 2 * ctas * 16 + static_cast<size_t>(s.pre_items) * 16;
+    }
+    s.rows += items * g16;
+    s.descs = items + s.pre_items;
+  }
+  return s;
 }
 }  // namespace
 
-size_t paged_decode_workspace(int B, int hq, int n_kv_heads, int D, bool prefix, int num_sms) {
-  const Scratch s = scratch_of(B, hq, n_kv_heads, prefix, num_sms);
-  // Descriptions first (16 bytes each), then the pieces.
-  return (s.descs * sizeof(Desc) + s.slots * s.rows * (D + 2) * 4 + 255) / 256 * 256;
+// At most two 16-row tiles: streaming the prefix once or twice beats the prompt
+// kernel's start and its mostly empty 128-row tiles (16 sequences, 32 heads,
+// 2000 positions: VS us against 35 us).
+bool prefix_streamed(int n_seqs, int hq, int n_kv_heads) {
+  const int g = hq / n_kv_heads;
+  return g <= 16 && n_seqs <= 2 * (16 / g);
+}
+
+size_t paged_decode_workspace(int B, int hq, int n_kv_heads, int D, int prefix_len, int num_sms) {
+  const Scratch s = scratch_of(B, hq, n_kv_heads, prefix_len, num_sms);
+  // Descriptions first (16 bytes each), then the rows.
+  return (s.descs * sizeof(Desc) + s.rows * (D + 2) * 4 + 255) / 256 * 256;
 }
 
 cudaError_t launch_paged_decode(const PagedPool& pool, const CUtensorMap& kmap,
                                 const CUtensorMap& vmap, const DecodeArgs& a, int num_sms,
                                 cudaStream_t stream) {
-  const Scratch s = scratch_of(a.B, a.hq, pool.n_kv_heads, a.prefix.S > 0, num_sms);
+  const Scratch s = scratch_of(a.B, a.hq, pool.n_kv_heads, a.prefix_len, num_sms);
   Params p;
   p.q = a.q;
   p.out = a.out;
@@ -609,8 +710,14 @@ cudaError_t launch_paged_decode(const PagedPool& pool, const CUtensorMap& kmap,
   p.lens = a.lens;
   p.desc = static_cast<Desc*>(a.workspace);
   p.part = reinterpret_cast<float*>(p.desc + s.descs);
-  p.ml = p.part + s.slots * s.rows * pool.D;
-  p.rows = static_cast<int>(s.rows);
+  p.m = p.part + s.rows * pool.D;
+  p.l = p.m + s.rows;
+  p.rows = s.per_piece;
+  p.pre_table = a.prefix_table;
+  p.pre_len = a.prefix_len;
+  p.pre_seqs = s.pre_seqs;
+  p.pre_items = s.pre_items;
+  p.pre_tiles = s.pre_items ? (a.prefix_len + kTile - 1) / kTile : 0;
   p.n_ctas = kCtasPerSm * num_sms;
   p.q_stride_seq = a.q_stride_seq;
   p.q_stride_head = a.q_stride_head;
