@@ -6,7 +6,9 @@ Each ``csrc/*.cu`` is compiled by nvcc for ``arch=compute_100a,code=sm_100a``
 with ``-lineinfo`` and linked into ``dequant_project_b200/libdequant_b200.so``
 next to this file (static CUDA runtime, no torch dependency). The shared
 library is the product's C ABI (include/dequant_b200.h); the Python package
-loads it with ctypes.
+loads it with ctypes. The paged-cache operators' calls are also bound natively
+(``binding/paged_binding.cpp``, built against the installed torch into
+``_paged_binding.so``).
 """
 
 from __future__ import annotations
@@ -23,6 +25,8 @@ CSRC = PKG / "csrc"
 INCLUDE = PKG.parent / "include"
 OUT = PKG / "libdequant_b200.so"
 OBJ_DIR = PKG / "_build"
+BINDING = PKG / "binding" / "paged_binding.cpp"
+BINDING_OUT = PKG / "_paged_binding.so"
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 
@@ -59,7 +63,34 @@ def _compile(src: Path, verbose_ptxas: bool) -> Path:
     return obj
 
 
+def build_binding(force: bool = False) -> Path:
+    """The native binding of the paged operators (g++, torch's headers)."""
+    deps = [BINDING, *INCLUDE.glob("*.h")]
+    if not force and BINDING_OUT.exists():
+        t = BINDING_OUT.stat().st_mtime
+        if all(p.stat().st_mtime <= t for p in deps):
+            return BINDING_OUT
+    import sysconfig
+
+    import torch
+    root = Path(torch.__file__).resolve().parent
+    tmp = BINDING_OUT.with_suffix(".so.tmp")
+    cuda = Path(nvcc()).resolve().parent.parent / "include"
+    inc = [INCLUDE, root / "include", root / "include/torch/csrc/api/include", cuda,
+           sysconfig.get_paths()["include"]]
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           *[f"-I{p}" for p in inc], str(BINDING), "-o", str(tmp), f"-L{root / 'lib'}",
+           "-ltorch_python", "-ltorch_cpu", "-ltorch", "-lc10", "-lc10_cuda"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"{BINDING.name} failed to build:\n{r.stdout}\n{r.stderr}")
+    os.replace(tmp, BINDING_OUT)
+    return BINDING_OUT
+
+
 def build(force: bool = False, verbose_ptxas: bool = False) -> Path:
+    build_binding(force)
     srcs = sources()
     if not force and not _stale(srcs):
         return OUT
