@@ -85,22 +85,20 @@ __device__ __forceinline__ long long quotient(long long a, long long b) {
   if (((a | b) >> 32) == 0) return static_cast<uint32_t>(a) / static_cast<uint32_t>(b);
   return a / b;
 }
-// `total` units of work in `ctas` equal shares: share c begins at unit
-// floor(c total / ctas).
+// `total` units of work in shares of `each`, the last one shorter; at most n.
 struct Shares {
   long long total, each;
-  int ctas, rest;
-  __device__ __forceinline__ void set(long long units, int n) {
+  __device__ __forceinline__ void set(long long units, int n, int least) {
     total = units;
-    ctas = n < units ? n : static_cast<int>(units);
-    each = ctas ? quotient(total, ctas) : 0;
-    rest = static_cast<int>(total - each * ctas);
+    each = quotient(units + n - 1, n);
+    if (each < least) each = least;
   }
   __device__ __forceinline__ long long begin(int c) const {
-    return c * each + static_cast<uint32_t>(c * rest) / static_cast<uint32_t>(ctas);
+    const long long b = c * each;
+    return b < total ? b : total;
   }
   __device__ __forceinline__ int holder(long long unit) const {  // the share that holds a unit
-    return static_cast<int>(quotient((unit + 1) * ctas - 1, total));
+    return static_cast<int>(quotient(unit, each));
   }
 };
 

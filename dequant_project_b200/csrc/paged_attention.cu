@@ -39,6 +39,7 @@ constexpr int kThreads = 32 * (kWarps + 1);
 constexpr int kStages = 3;
 constexpr int kCtasPerSm = 2;
 constexpr int kQuerySlots = 4;         // items whose queries are held at most
+constexpr int kItemTiles = 1;         // an item's start and end, in tiles' time
 constexpr int kMergeRows = 4;          // query heads per round of the warps' merge
 
 struct Desc {    // an item that is joined later
@@ -86,7 +87,8 @@ __device__ __forceinline__ void store4(const Params& p, int b, int head, int d4,
 
 __device__ __forceinline__ int tiles_of(int len) { return len > 0 ? (len + kTile - 1) / kTile : 1; }
 
-// A CTA's share of the tiles: where it starts and how many it takes.
+// A CTA's share of the units (an item's tiles, and kItemTiles for its start and
+// end): where it starts, how many it takes; x: the first one's place in its item.
 struct Share {
   Shares all;
   long long count, pos;
@@ -96,50 +98,49 @@ struct Share {
 // Taken by one whole warp.
 __device__ __forceinline__ Share find_share(const Params& p, int cta, int n_ctas) {
   const int lane = threadIdx.x & 31;
-  const long long hv = static_cast<long long>(p.hkv) * p.nrb;
+  const int hv = p.hkv * p.nrb;
+  const long long pre = static_cast<long long>(p.pre_items) * (p.pre_tiles + kItemTiles);
+  auto cost = [&](int b) {
+    return b < p.B ? tiles_of(clamped_len(p.lens, b, p.len_limit)) + kItemTiles : 0;
+  };
   long long total = 0;
-  for (int b0 = 0; b0 < p.B; b0 += 32) {
-    const int b = b0 + lane;
-    total += b < p.B ? tiles_of(clamped_len(p.lens, b, p.len_limit)) : 0;
-  }
-#pragma unroll
+#pragma unroll 1
+  for (int b = lane; b < p.B; b += 32) total += cost(b);
+#pragma unroll 1
   for (int off = 16; off >= 1; off >>= 1) total += __shfl_xor_sync(0xffffffffu, total, off);
   Share s;
-  const long long pre = static_cast<long long>(p.pre_items) * p.pre_tiles;
-  s.all.set(total * hv + pre, n_ctas);
-  s.b = s.hv = s.x = 0;
-  s.pos = s.count = 0;
-  if (cta >= s.all.ctas) return s;
+  s.all.set(total * hv + pre, n_ctas, 1);
   s.pos = s.all.begin(cta);
   s.count = s.all.begin(cta + 1) - s.pos;
-  if (s.pos < pre) {  // prefix items come first, as sequence -1
-    s.b = -1;
-    s.hv = static_cast<int>(quotient(s.pos, p.pre_tiles));
-    s.x = static_cast<int>(s.pos - static_cast<long long>(s.hv) * p.pre_tiles);
-    return s;
-  }
-  long long before = pre;
-  for (int b0 = 0; b0 < p.B; b0 += 32) {
-    const int b = b0 + lane;
-    const int nt = b < p.B ? tiles_of(clamped_len(p.lens, b, p.len_limit)) : 0;
-    long long sum = nt * hv;
-#pragma unroll
-    for (int off = 1; off < 32; off <<= 1) {
-      const long long t = __shfl_up_sync(0xffffffffu, sum, off);
-      if (lane >= off) sum += t;
+  s.b = -1;
+  s.hv = s.x = 0;
+  if (s.count == 0) return s;
+  long long before = 0;
+  int per = p.pre_tiles + kItemTiles;
+  if (s.pos >= pre) {  // (prefix items come first, as sequence -1)
+    before = pre;
+#pragma unroll 1
+    for (int b0 = 0; b0 < p.B; b0 += 32) {
+      const int c = cost(b0 + lane);
+      long long sum = static_cast<long long>(c) * hv;
+#pragma unroll 1
+      for (int off = 1; off < 32; off <<= 1) {
+        const long long t = __shfl_up_sync(0xffffffffu, sum, off);
+        if (lane >= off) sum += t;
+      }
+      const unsigned past = __ballot_sync(0xffffffffu, before + sum > s.pos);
+      if (past) {
+        const int l = __ffs(past) - 1;
+        per = __shfl_sync(0xffffffffu, c, l);
+        before += __shfl_sync(0xffffffffu, sum, l) - static_cast<long long>(per) * hv;
+        s.b = b0 + l;
+        break;
+      }
+      before += __shfl_sync(0xffffffffu, sum, 31);
     }
-    const unsigned past = __ballot_sync(0xffffffffu, before + sum > s.pos);
-    if (past) {
-      const int l = __ffs(past) - 1;
-      const long long in = s.pos - (before + __shfl_sync(0xffffffffu, sum - nt * hv, l));
-      const int n = __shfl_sync(0xffffffffu, nt, l);
-      s.b = b0 + l;
-      s.hv = static_cast<int>(quotient(in, n));
-      s.x = static_cast<int>(in - static_cast<long long>(s.hv) * n);
-      break;
-    }
-    before += __shfl_sync(0xffffffffu, sum, 31);
   }
+  s.hv = static_cast<int>(quotient(s.pos - before, per));
+  s.x = static_cast<int>(s.pos - before - static_cast<long long>(s.hv) * per);
   return s;
 }
 
@@ -147,6 +148,7 @@ __device__ __forceinline__ Share find_share(const Params& p, int cta, int n_ctas
 struct Item {
   const int32_t* table;
   int len, tiles, kvh, head0, rows, first;  // first: the prefix's first sequence
+  int units, x0, x1;                        // of the share that the item takes; tiles in it
 };
 __device__ __forceinline__ Item item_of(const Params& p, const Share& s) {
   Item i;
@@ -169,9 +171,12 @@ __device__ __forceinline__ Item item_of(const Params& p, const Share& s) {
     i.rows = min(16, p.g - rb * 16);
     i.first = 0;
   }
+  i.units = static_cast<int>(min(static_cast<long long>(i.tiles + kItemTiles - s.x), s.count));
+  i.x0 = max(0, s.x - kItemTiles);
+  i.x1 = max(0, s.x + i.units - kItemTiles);
   return i;
 }
-// Behind n tiles of the item at hand.
+// Behind n units of the item at hand.
 __device__ __forceinline__ void advance(const Params& p, Share& s, int n) {
   s.pos += n;
   s.count -= n;
@@ -281,7 +286,10 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
     bool ok = true;
     while (s.count > 0 && ok) {
       const Item i = item_of(p, s);
-      const int n = static_cast<int>(min(static_cast<long long>(i.tiles - s.x), s.count));
+      if (i.x1 == i.x0) {  // the cut falls before its first tile
+        advance(p, s, i.units);
+        continue;
+      }
       // The item's queries, a row a lane.
       if (s.b < 0) {
         if (pre > 0 && !warp_wait(pre_empty, (pre - 1) & 1)) break;
@@ -303,7 +311,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
                    (i.head0 + lane) * p.q_stride_head, D * 2, q_full + qi, policy);
         ++item;
       }
-      for (int x = s.x; x < s.x + n; ++x, ++it) {
+      for (int x = i.x0; x < i.x1; ++x, ++it) {
         const int st = it % kStages;
         const int t = x * kTile + sub * per;
         int page = static_cast<int>(p.n_pages);  // no such page: zeros
@@ -327,7 +335,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
           tma_load_4d(dst + L::kTileBytes, &vmap, full + st, half * 64, in_page, i.kvh, page);
         }
       }
-      advance(p, s, n);
+      advance(p, s, i.units);
     }
     // Copies still in flight land before the CTA's memory goes (bounded).
     if (pre > 0) warp_wait(pre_full, (pre - 1) & 1);
@@ -343,8 +351,11 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
     bool ok = true, cut_first = false;
     while (s.count > 0 && ok) {
       const Item i = item_of(p, s);
-      const int len = i.len, nt = i.tiles, head0 = i.head0, rows = i.rows;
-      const int n = static_cast<int>(min(static_cast<long long>(nt - s.x), s.count));
+      const int len = i.len, head0 = i.head0, rows = i.rows;
+      if (i.x1 == i.x0) {
+        advance(p, s, i.units);
+        continue;
+      }
       // Q as A fragments: rows are the KV head's query heads (of several
       // sequences, in a prefix).
       uint32_t qa[D / 16][4];
@@ -361,7 +372,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
 #pragma unroll
       for (int nb = 0; nb < D / 8; ++nb) o[nb][0] = o[nb][1] = o[nb][2] = o[nb][3] = 0.f;
       float m_run[2] = {-INFINITY, -INFINITY}, l_run[2] = {0.f, 0.f};
-      for (int x = s.x; x < s.x + n; ++x, ++it) {
+      for (int x = i.x0; x < i.x1; ++x, ++it) {
         const int st = it % kStages;
         if (!warp_wait(full + st, (it / kStages) & 1)) {
           ok = false;
@@ -448,15 +459,15 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
           ls[warp * 16 + gid + 8 * r] = l_run[r];
         }
       }
-      const bool whole = s.x == 0 && n == nt;
+      const bool whole = i.x0 == 0 && i.x1 == i.tiles;
       const int64_t row0 = whole ? whole_row(p, s.b, s.hv)
-                                 : (2 * static_cast<int64_t>(blockIdx.x) + (s.x > 0 ? 0 : 1)) * p.rows;
-      if (s.x == 0 && (joined || !whole)) {
+                                 : (2 * static_cast<int64_t>(blockIdx.x) + (i.x0 > 0 ? 0 : 1)) * p.rows;
+      if (i.x0 == 0 && (joined || !whole)) {
         cut_first = true;
         if (threadIdx.x == 0) {
           const int64_t items = static_cast<int64_t>(p.B) * p.hkv * p.nrb;
           const int64_t id = s.b < 0 ? items + s.hv : static_cast<int64_t>(s.b) * p.hkv * p.nrb + s.hv;
-          const int last = s.all.holder(s.pos + nt - 1);
+          const int last = s.all.holder(s.pos - s.x + i.tiles + kItemTiles - 1);
           p.desc[joined ? id : blockIdx.x] =
               Desc{s.b, s.hv, whole ? -1 : static_cast<int>(blockIdx.x), last - static_cast<int>(blockIdx.x) + 1};
         }
@@ -504,7 +515,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
         }
         named_sync(1, 32 * kWarps);
       }
-      advance(p, s, n);
+      advance(p, s, i.units);
     }
     if (threadIdx.x == 0 && !cut_first && !joined) p.desc[blockIdx.x] = Desc{0, 0, 0, 0};
   }

@@ -230,12 +230,11 @@ __device__ __forceinline__ Share find_share(const Params& p, int cta, int n_ctas
   Share r;
   // Shares of a block at least, so that none inside an item comes to nothing.
   total *= p.hkv;
-  r.all.set(total, static_cast<int>(max(1ll, min(static_cast<long long>(n_ctas), total / kBlock))));
+  r.all.set(total, n_ctas, kBlock);
   r.b = r.kvh = r.pair = r.x = 0;
-  r.pos = r.count = 0;
-  if (cta >= r.all.ctas) return r;
   r.pos = r.all.begin(cta);
   r.count = r.all.begin(cta + 1) - r.pos;
+  if (r.count == 0) return r;
   long long before = 0;
   for (int b0 = 0; b0 < p.B; b0 += 32) {
     const int b = b0 + lane;
