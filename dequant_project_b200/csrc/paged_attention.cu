@@ -62,6 +62,7 @@ struct Params {
   int B, hq, hkv, g, nrb, rows, page_shift, len_limit, box_rows, n_ctas;
   int pre_len, pre_seqs, pre_tiles, pre_items;  // a streamed prefix: sequences an item; tiles; items
   float scale_log2;
+  bool n_units32;   // the units of any lengths fit 31 bits
   PrefixPieces prefix;
 };
 
@@ -103,12 +104,39 @@ __device__ __forceinline__ Share find_share(const Params& p, int cta, int n_ctas
   auto cost = [&](int b) {
     return b < p.B ? tiles_of(clamped_len(p.lens, b, p.len_limit)) + kItemTiles : 0;
   };
+  Share s;
+  if (p.B <= 32 && p.pre_items == 0 && p.n_units32) {
+    // Up to 32 sequences and 2^31 units: one scan, and little code (a launch
+    // fetches it from the L2 cache at first use, which is most of the time
+    // that a short call takes here).
+    const uint32_t c = cost(lane);
+    uint32_t sum = c;
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+      const uint32_t t = __shfl_up_sync(0xffffffffu, sum, off);
+      if (lane >= off) sum += t;
+    }
+    const uint32_t total = __shfl_sync(0xffffffffu, sum, 31) * hv;
+    const uint32_t each = (total + n_ctas - 1) / n_ctas;
+    const uint32_t pos = min(total, cta * each);
+    s.all.total = total;
+    s.all.each = each;
+    s.pos = pos;
+    s.count = min(total, pos + each) - pos;
+    const unsigned past = __ballot_sync(0xffffffffu, sum * hv > pos);
+    const int l = past ? __ffs(past) - 1 : 0;
+    const uint32_t per = max(1u, __shfl_sync(0xffffffffu, c, l));
+    const uint32_t in = pos - (__shfl_sync(0xffffffffu, sum, l) - per) * hv;
+    s.b = l;
+    s.hv = in / per;
+    s.x = in - s.hv * per;
+    return s;
+  }
   long long total = 0;
 #pragma unroll 1
   for (int b = lane; b < p.B; b += 32) total += cost(b);
 #pragma unroll 1
   for (int off = 16; off >= 1; off >>= 1) total += __shfl_xor_sync(0xffffffffu, total, off);
-  Share s;
   s.all.set(total * hv + pre, n_ctas, 1);
   s.pos = s.all.begin(cta);
   s.count = s.all.begin(cta + 1) - s.pos;
@@ -745,6 +773,7 @@ cudaError_t launch_paged_decode(const PagedPool& pool, const CUtensorMap& kmap,
   p.len_limit = limit < (1 << 30) ? static_cast<int>(limit) : 1 << 30;
   p.box_rows = paged_decode_box_rows(pool.page_size);
   p.scale_log2 = a.scale_log2;
+  p.n_units32 = static_cast<double>(a.B) * p.hkv * p.nrb * (p.len_limit / kTile + 2 + kItemTiles) < 2147483648.0;
   p.prefix = a.prefix;
   if (pool.bf16)
     return pool.D == 128 ? launch<__nv_bfloat16, 128>(p, kmap, vmap, num_sms, stream)
