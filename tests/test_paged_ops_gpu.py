@@ -303,3 +303,284 @@ def test_shared_prefix(cuda_device, prefix, lens, hq, hkv, d, page, dtype):
     check_attention(out, torch.cat(ref), float(torch.nan_to_num(v.float()).abs().max()), dtype)
     for _ in range(3):
         assert torch.equal(paged_ops.shared_prefix_attention(q, k, v, shared, prefix, own, kv_lens), out)
+
+
+# ------------------------------------------- values, layouts, streams, limits
+def _growing(k, table, lens, page, per_block):
+    """Keys whose size grows along each sequence, so that the running maximum
+    moves in every block."""
+    for i, n in enumerate(lens):
+        t = torch.arange(n, device=k.device)
+        f = (per_block ** (t // 64)).to(k.dtype)
+        k[table[i].long()[t // page], :, t % page] *= f[:, None, None]
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+def test_a_maximum_that_keeps_growing(cuda_device, dtype):
+    """Scores grow from block to block by more than the factor at which the
+    accumulators are rescaled. Scores up to |s| = 2^6 carry an error of about
+    2^-19 of fp32 sums, so the bound above holds as it is."""
+    gen = torch.Generator(device=cuda_device).manual_seed(5)
+    lens, hq, hkv, d, page = [700, 130], 8, 2, 128, 16
+    args = list(prompt_case(gen, [300, 130], lens, hq, hkv, d, page, dtype, cuda_device))
+    _growing(args[1], args[3], lens, page, 1.2)
+    q, k, v, table, starts, kv_lens = args
+    v_max = float(torch.nan_to_num(v.float()).abs().max())
+    out = paged_ops.prompt_attention(*args)
+    check_attention(out, prompt64(*args, True, 1 / math.sqrt(d)), v_max, dtype)
+    qd = q[:2].contiguous()
+    ref = torch.cat([attend64(qd[i:i + 1], rows64(k, table[i], n), rows64(v, table[i], n), kv_lens[i:i + 1],
+                              1 / math.sqrt(d)) for i, n in enumerate(lens)])
+    check_attention(paged_ops.paged_attention(qd, k, v, table, kv_lens), ref, v_max, dtype)
+
+
+def test_scale_is_taken(cuda_device):
+    gen = torch.Generator(device=cuda_device).manual_seed(6)
+    args = prompt_case(gen, [70], [200], 4, 2, 64, 16, torch.float16, cuda_device)
+    q, k, v, table, starts, lens = args
+    out = paged_ops.prompt_attention(*args, scale=0.4)
+    check_attention(out, prompt64(*args, True, 0.4), 6.0, torch.float16)
+    out = paged_ops.paged_attention(q[:1], k, v, table, lens, scale=0.4)
+    ref = attend64(q[:1], rows64(k, table[0], 200), rows64(v, table[0], 200), lens, 0.4)
+    check_attention(out, ref, 6.0, torch.float16)
+
+
+def test_non_finite_keys_and_values(cuda_device):
+    """A NaN or infinity that a row sees reaches it as in the formula; other
+    sequences, and rows whose mask hides a NaN key, do not notice."""
+    gen = torch.Generator(device=cuda_device).manual_seed(7)
+    lens = [90, 90, 90, 150]
+    args = prompt_case(gen, [90, 90, 90, 150], lens, 2, 2, 128, 16, torch.float16, cuda_device)
+    q, k, v, table, starts, kv_lens = args
+    clean = paged_ops.prompt_attention(*args)
+    k2, v2 = k.clone(), v.clone()
+    k2[table[0, 40 // 16], :, 40 % 16] = float("nan")   # seen by rows 40.. of sequence 0
+    v2[table[1, 0], :, 0, 5] = float("inf")             # seen by every row of sequence 1
+    out = paged_ops.prompt_attention(q, k2, v2, table, starts, kv_lens)
+    assert torch.equal(out[:40], clean[:40])
+    assert torch.isnan(out[40:90]).all()
+    assert torch.isinf(out[90:180, :, 5]).all()
+    keep = [i for i in range(128) if i != 5]
+    assert torch.equal(out[90:180][..., keep], clean[90:180][..., keep])
+    assert torch.equal(out[180:], clean[180:])
+    qd = q[[0, 90, 180, 270]].contiguous()
+    plain = paged_ops.paged_attention(qd, k, v, table, kv_lens)
+    out = paged_ops.paged_attention(qd, k2, v2, table, kv_lens)
+    assert torch.isnan(out[0]).all() and torch.isinf(out[1, :, 5]).all()
+    assert torch.equal(out[2:], plain[2:])
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_strided_inputs(cuda_device, d):
+    """Queries as a view of a wider projection, keys and values as views of one
+    buffer with rows further apart, a table that is part of a wider one."""
+    gen = torch.Generator(device=cuda_device).manual_seed(8)
+    hq, hkv, page, lens, ql = 8, 2, 16, [100, 37, 64], [30, 37, 1]
+    k, v, table = make_cache(gen, lens, hkv, d, page, torch.float16, cuda_device, width=12)
+    both = torch.randn((k.shape[0], page, 2 * hkv, d + 8), generator=gen, device=cuda_device).half()
+    kv, vv = (both[:, :, i * hkv:(i + 1) * hkv, :d].permute(0, 2, 1, 3) for i in (0, 1))
+    kv.copy_(k)
+    vv.copy_(v)
+    wide = torch.randn((sum(ql), hq * d + 64), generator=gen, device=cuda_device).half()
+    q = wide[:, 64:].unflatten(1, (hq, d))
+    starts = torch.tensor([0, 30, 67, 68], dtype=torch.int32, device=cuda_device)
+    kv_lens = torch.tensor(lens, dtype=torch.int32, device=cuda_device)
+    part = table[:, :7]
+    want = paged_ops.prompt_attention(q.contiguous(), k, v, table, starts, kv_lens)
+    assert torch.equal(paged_ops.prompt_attention(q, kv, vv, part, starts, kv_lens), want)
+    want = paged_ops.paged_attention(q[:3].contiguous(), k, v, table, kv_lens)
+    assert torch.equal(paged_ops.paged_attention(q[:3], kv, vv, part, kv_lens), want)
+    pre = table[0, :3].contiguous()
+    for n in (3, 60):  # streamed with the sequences; by the prompt kernel
+        rows = q[:n] if n == 3 else q
+        tab = part if n == 3 else part[:1].expand(68, 7).contiguous()
+        ln = kv_lens if n == 3 else kv_lens[:1].expand(68).contiguous()
+        want = paged_ops.shared_prefix_attention(rows.contiguous(), k, v, pre, 40, tab, ln)
+        assert torch.equal(paged_ops.shared_prefix_attention(rows, kv, vv, pre, 40, tab, ln), want)
+
+
+def test_offsets_past_32_bits(cuda_device):
+    """Pages 2^28 elements apart: offsets past 2^31 elements and 2^32 bytes."""
+    gen = torch.Generator(device=cuda_device).manual_seed(9)
+    hkv, page, d, n = 2, 16, 128, 12
+    k, v, table = make_cache(gen, [150], hkv, d, page, torch.float16, cuda_device)
+    span = 1 << 28
+    big = torch.empty(n * span, dtype=torch.float16, device=cuda_device)
+    strides = (span, page * d, d, 1)
+    kb = torch.as_strided(big, (n, hkv, page, d), strides)
+    vb = torch.as_strided(big, (n, hkv, page, d), strides, 1 << 20)
+    kb[:k.shape[0]].copy_(k)
+    vb[:k.shape[0]].copy_(v)
+    move = torch.arange(n - 1, -1, -1, dtype=torch.int32, device=cuda_device)  # the far end holds page 0
+    kb.copy_(kb.clone()[move.long()])
+    vb.copy_(vb.clone()[move.long()])
+    far = move[table.long().clamp(min=0)]
+    lens = torch.tensor([150], dtype=torch.int32, device=cuda_device)
+    starts = torch.tensor([0, 20], dtype=torch.int32, device=cuda_device)
+    q = torch.randn((20, 4, d), generator=gen, device=cuda_device).half()
+    assert torch.equal(paged_ops.prompt_attention(q, kb, vb, far, starts, lens),
+                       paged_ops.prompt_attention(q, k, v, table, starts, lens))
+    assert torch.equal(paged_ops.paged_attention(q[:1], kb, vb, far, lens),
+                       paged_ops.paged_attention(q[:1], k, v, table, lens))
+    cos, sin = paged_ops.rope_scaled_tables(d, 1e4, 64, cuda_device)
+    qkv = torch.randn((16, 8 * d), generator=gen, device=cuda_device).half()
+    pos = torch.arange(16, device=cuda_device)
+    paged_ops.rope_paged_append(qkv, cos, sin, pos, pos + 16 * (n - 1), kb, vb, 4)
+    paged_ops.rope_paged_append(qkv, cos, sin, pos, pos, k, v, 4)
+    assert torch.equal(kb[n - 1], k[0]) and torch.equal(vb[n - 1], v[0])
+
+
+def test_pages_may_lie_anywhere(cuda_device):
+    """The same sequence through other pages, another page size and another
+    place in the batch gives the same bits where the shares are cut alike."""
+    gen = torch.Generator(device=cuda_device).manual_seed(10)
+    k, v, table = make_cache(gen, [200, 200], 2, 128, 16, torch.bfloat16, cuda_device)
+    t = torch.arange(200, device=cuda_device)
+    for pool in (k, v):  # the second sequence holds what the first does
+        pool[table[1].long()[t // 16], :, t % 16] = pool[table[0].long()[t // 16], :, t % 16]
+    q = torch.randn((1, 8, 128), generator=gen, device=cuda_device).bfloat16()
+    one = torch.tensor([200], dtype=torch.int32, device=cuda_device)
+    a = paged_ops.paged_attention(q, k, v, table[:1], one)
+    assert torch.equal(paged_ops.paged_attention(q, k, v, table[1:], one), a)
+
+
+def test_captured_calls_serve_other_lengths(cuda_device):
+    gen = torch.Generator(device=cuda_device).manual_seed(11)
+    lens = [500, 300, 800]
+    k, v, table = make_cache(gen, lens, 2, 128, 16, torch.float16, cuda_device)
+    q = torch.randn((3, 8, 128), generator=gen, device=cuda_device).half()
+    kv_lens = torch.tensor(lens, dtype=torch.int32, device=cuda_device)
+    starts = torch.tensor([0, 1, 1, 3], dtype=torch.int32, device=cuda_device)
+    pre = table[2, :4].contiguous()
+
+    def calls():
+        return (paged_ops.paged_attention(q, k, v, table, kv_lens),
+                paged_ops.prompt_attention(q, k, v, table, starts, kv_lens),
+                paged_ops.shared_prefix_attention(q, k, v, pre, 60, table, kv_lens))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        calls()
+        side.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            got = calls()
+    for new in ([500, 300, 800], [1, 0, 799], [64, 65, 63]):
+        kv_lens.copy_(torch.tensor(new, dtype=torch.int32))
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(got, calls()):
+            assert torch.equal(a, b), new
+
+
+def test_on_another_stream(cuda_device):
+    """Work is queued on torch's current stream: behind what fills the inputs
+    there, and not on the default stream."""
+    gen = torch.Generator(device=cuda_device).manual_seed(12)
+    k, v, table = make_cache(gen, [600], 2, 128, 16, torch.float16, cuda_device)
+    q = torch.randn((1, 4, 128), generator=gen, device=cuda_device).half()
+    lens = torch.tensor([600], dtype=torch.int32, device=cuda_device)
+    want = paged_ops.paged_attention(q, k, v, table, lens)
+    late = torch.zeros_like(q)
+    big = torch.randn((4096, 4096), device=cuda_device)
+    torch.cuda.synchronize()
+    s = torch.cuda.Stream()
+    with torch.cuda.stream(s):
+        for _ in range(4):
+            big = big @ big
+            big = big / big.abs().max()
+        late.copy_(q)
+        out = paged_ops.paged_attention(late, k, v, table, lens)
+    s.synchronize()
+    assert torch.equal(out, want)
+
+
+def test_indexes_out_of_range_are_left_out(cuda_device):
+    """A page number no page has reads as zeros, a length past the table ends at
+    it; both are reported, and nothing else is touched."""
+    gen = torch.Generator(device=cuda_device).manual_seed(13)
+    k, v, table = make_cache(gen, [64, 64], 2, 128, 16, torch.float16, cuda_device)
+    q = torch.randn((2, 4, 128), generator=gen, device=cuda_device).half()
+    lens = torch.tensor([64, 64], dtype=torch.int32, device=cuda_device)
+    starts = torch.tensor([0, 1, 2], dtype=torch.int32, device=cuda_device)
+    calls = [lambda t, n: paged_ops.paged_attention(q, k, v, t, n),
+             lambda t, n: paged_ops.prompt_attention(q, k, v, t, starts, n)]
+    for call in calls:
+        good = call(table, lens)
+        for bad in (-7, 1 << 30, k.shape[0]):
+            t = table.clone()
+            t[0, 2] = bad
+            out = call(t, lens)
+            assert torch.equal(out[1], good[1]) and torch.isfinite(out).all()
+            assert _native.device_status(cuda_device.index, reset=True) == 2
+        for n in (65, 1 << 30, -3):
+            out = call(table, torch.tensor([n, 64], dtype=torch.int32, device=cuda_device))
+            assert torch.equal(out[1], good[1])
+            assert torch.equal(out[0], good[0] if n > 0 else torch.zeros_like(out[0]))
+            assert _native.device_status(cuda_device.index, reset=True) == 2
+    # Starts out of order: those sequences have no rows.
+    wrong = torch.tensor([0, 5, 2], dtype=torch.int32, device=cuda_device)
+    paged_ops.prompt_attention(q, k, v, table, wrong, lens)
+    torch.cuda.synchronize()
+    assert _native.device_status(cuda_device.index, reset=True) in (0, 2)
+
+
+def test_empty_calls(cuda_device):
+    k = torch.zeros((2, 1, 16, 64), dtype=torch.float16, device=cuda_device)
+    q = torch.zeros((0, 2, 64), dtype=torch.float16, device=cuda_device)
+    none = torch.zeros((0, 1), dtype=torch.int32, device=cuda_device)
+    lens = torch.zeros(0, dtype=torch.int32, device=cuda_device)
+    starts = torch.zeros(1, dtype=torch.int32, device=cuda_device)
+    assert paged_ops.paged_attention(q, k, k, none, lens).shape == (0, 2, 64)
+    assert paged_ops.prompt_attention(q, k, k, none, starts, lens).shape == (0, 2, 64)
+    pre = torch.zeros(1, dtype=torch.int32, device=cuda_device)
+    assert paged_ops.shared_prefix_attention(q, k, k, pre, 3, none, lens).shape == (0, 2, 64)
+
+
+def test_binding_rejects_bad_tensors(cuda_device):
+    def z(*shape, dtype=torch.float16, device=cuda_device):
+        return torch.zeros(shape, dtype=dtype, device=device)
+
+    k, q, t, n = z(2, 1, 16, 64), z(3, 2, 64), z(3, 2, dtype=torch.int32), z(3, dtype=torch.int32)
+    cases = [
+        ((q.float(), k, k, t, n), "q must be float16"),
+        ((q.bfloat16(), k, k, t, n), "q must be float16"),
+        ((q, k.float(), k.float(), t, n), "pages must be float16 or bfloat16"),
+        ((q, k[0], k[0], t, n), "pages must be"),
+        ((q, k, z(2, 1, 32, 64), t, n), "one shape, type and strides"),
+        ((q, k, k.transpose(2, 3).contiguous().transpose(2, 3), t, n), "one shape, type and strides"),
+        ((q, k, k.cpu(), t, n), "same device"),
+        ((q, k, k, t.cpu(), n), "block_table must be"),
+        ((q, k, k, t.long(), n), "block_table must be"),
+        ((q, k, k, t[:2], n), "block_table must hold 3 rows"),
+        ((q, k, k, t, n.long()), "kv_lens must be"),
+        ((q, k, k, t, n[:1]), "kv_lens must hold 3 rows"),
+        ((q[:, :, :32], k, k, t, n), "q must be"),
+        ((q.transpose(1, 2).contiguous().transpose(1, 2), k, k, t, n), "head dimension contiguous"),
+        ((z(3, 2, 96), z(2, 1, 16, 96), z(2, 1, 16, 96), t, n), "head_dim 64 and 128"),
+        ((q, z(2, 1, 24, 64), z(2, 1, 24, 64), t, n), "page_size must be"),
+        ((q, z(2, 3, 16, 64), z(2, 3, 16, 64), t, n), "query heads per KV head"),
+    ]
+    for args, msg in cases:
+        with pytest.raises(RuntimeError, match=msg):
+            paged_ops.paged_attention(*args)
+    with pytest.raises(RuntimeError, match="workspace of"):
+        paged_ops.paged_attention(q, k, k, t, n, workspace=z(64))
+    with pytest.raises(RuntimeError, match="scale must be positive"):
+        paged_ops.paged_attention(q, k, k, t, n, scale=-1.0)
+    with pytest.raises(RuntimeError, match="q_starts must hold 4 rows"):
+        paged_ops.prompt_attention(q, k, k, t, n, n)
+    with pytest.raises(RuntimeError, match="prefix_len=33 positions exceed"):
+        paged_ops.shared_prefix_attention(q, k, k, z(2, dtype=torch.int32), 33, t, n)
+    i64 = torch.int64
+    good = dict(qkv=z(3, 4 * 64), cos=z(8, 32, dtype=torch.float32), sin=z(8, 32, dtype=torch.float32),
+                positions=z(3, dtype=i64), slots=z(3, dtype=i64), k_pages=k, v_pages=k, n_q_heads=2)
+    for change, msg in ((dict(qkv=z(3, 200)), "qkv must be"), (dict(cos=z(8, 32)), "cos and sin"),
+                        (dict(sin=z(8, 16, dtype=torch.float32)), "cos and sin"),
+                        (dict(positions=z(2, dtype=i64)), "positions must hold 3"),
+                        (dict(slots=z(3, dtype=torch.int32)), "slots must be"),
+                        (dict(q_norm=z(64)), "given together"), (dict(q_norm=z(32), k_norm=z(64)), "q_norm must hold"),
+                        (dict(cos=z(8, 33, dtype=torch.float32), sin=z(8, 33, dtype=torch.float32)), "rotary_dim")):
+        with pytest.raises(RuntimeError, match=msg):
+            paged_ops.rope_paged_append(**{**good, **change})
