@@ -515,12 +515,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     // addresses and descriptors then live in uniform registers).
     constexpr uint32_t kIdS = instr_desc(Elem<E>::kFormat, kBlock, false);
     constexpr uint32_t kIdO = instr_desc(Elem<E>::kFormat, D, true);
-    const bool one = elect_one();
+    if (elect_one()) {
     const uint64_t q_desc = smem_desc(sbase, 16, 1024);
     const uint64_t k_desc = smem_desc(sbase + L::kRing, 16, 1024);
     const uint64_t v_desc = smem_desc(sbase + L::kRing, kBlock * 128, 1024);
     auto issue_s = [&](int t, int slot) {
-      if (!one) return;
       const uint64_t a = q_desc + t * (L::kTile >> 4), b = k_desc + slot * (L::kSlot >> 4);
 #pragma unroll
       for (int k = 0; k < D / 16; ++k) {
@@ -530,7 +529,6 @@ __global__ void __launch_bounds__(kThreads, 1)
       mma_commit(s_full + t);
     };
     auto issue_o = [&](int t, int slot, bool late, bool add) {
-      if (!one) return;
       const uint64_t b = v_desc + slot * (L::kSlot >> 4);
 #pragma unroll
       for (int k = 0; k < kBlock / 16; ++k) {
@@ -539,10 +537,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     };
     auto commit = [&](uint64_t* bar) {
-      if (one) mma_commit(bar);
+      mma_commit(bar);
     };
     auto wait = [&](uint64_t* bar, uint32_t parity) {
-      const bool ok = warp_wait(bar, parity);
+      const bool ok = mbar_wait(bar, parity);
       fence_after_sync();
       return ok;
     };
@@ -557,12 +555,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     bool ok = true;
     while (ok) {
       const int sg = seg % kSegs;
-      if (!warp_wait(seg_full + sg, (seg / kSegs) & 1)) break;
+      if (!mbar_wait(seg_full + sg, (seg / kSegs) & 1)) break;
       const int c0 = tile_count(segs[sg], 0), c1 = tile_count(segs[sg], 1);
       const int n = segs[sg].x1 - segs[sg].x0;
       if (n == 0) break;
-      __syncwarp();
-      if (one) mbar_arrive(seg_empty + sg);
+      mbar_arrive(seg_empty + sg);
       ok = wait(q_full, seg & 1) && wait(full + slot, ring);
       ++seg;
       if (!ok) break;
@@ -602,7 +599,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     // Nothing of this CTA is in flight when it ends (bounded).
     commit(drained);
-    warp_wait(drained, 0);
+    mbar_wait(drained, 0);
+    }
+    __syncwarp();
   }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
