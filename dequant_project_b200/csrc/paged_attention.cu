@@ -39,7 +39,6 @@ constexpr int kThreads = 32 * (kWarps + 1);
 constexpr int kStages = 3;
 constexpr int kCtasPerSm = 2;
 constexpr int kQuerySlots = 4;         // items whose queries are held at most
-constexpr int kItemTiles = 1;         // an item's start and end, in tiles' time
 constexpr int kMergeRows = 4;          // query heads per round of the warps' merge
 
 struct Desc {    // an item that is joined later
@@ -60,6 +59,7 @@ struct Params {
   const int32_t* pre_table;
   int64_t q_stride_seq, q_stride_head, table_stride, n_pages;
   int B, hq, hkv, g, nrb, rows, page_shift, len_limit, box_rows, n_ctas;
+  int item_tiles;                                // an item's start and end, in tiles' time
   int pre_len, pre_seqs, pre_tiles, pre_items;  // a streamed prefix: sequences an item; tiles; items
   float scale_log2;
   bool n_units32;   // the units of any lengths fit 31 bits
@@ -88,7 +88,7 @@ __device__ __forceinline__ void store4(const Params& p, int b, int head, int d4,
 
 __device__ __forceinline__ int tiles_of(int len) { return len > 0 ? (len + kTile - 1) / kTile : 1; }
 
-// A CTA's share of the units (an item's tiles, and kItemTiles for its start and
+// A CTA's share of the units (an item's tiles, and item_tiles for its start and
 // end): where it starts, how many it takes; x: the first one's place in its item.
 struct Share {
   Shares all;
@@ -100,9 +100,9 @@ struct Share {
 __device__ __forceinline__ Share find_share(const Params& p, int cta, int n_ctas) {
   const int lane = threadIdx.x & 31;
   const int hv = p.hkv * p.nrb;
-  const long long pre = static_cast<long long>(p.pre_items) * (p.pre_tiles + kItemTiles);
+  const long long pre = static_cast<long long>(p.pre_items) * (p.pre_tiles + p.item_tiles);
   auto cost = [&](int b) {
-    return b < p.B ? tiles_of(clamped_len(p.lens, b, p.len_limit)) + kItemTiles : 0;
+    return b < p.B ? tiles_of(clamped_len(p.lens, b, p.len_limit)) + p.item_tiles : 0;
   };
   Share s;
   if (p.B <= 32 && p.pre_items == 0 && p.n_units32) {
@@ -144,7 +144,7 @@ __device__ __forceinline__ Share find_share(const Params& p, int cta, int n_ctas
   s.hv = s.x = 0;
   if (s.count == 0) return s;
   long long before = 0;
-  int per = p.pre_tiles + kItemTiles;
+  int per = p.pre_tiles + p.item_tiles;
   if (s.pos >= pre) {  // (prefix items come first, as sequence -1)
     before = pre;
 #pragma unroll 1
@@ -199,9 +199,9 @@ __device__ __forceinline__ Item item_of(const Params& p, const Share& s) {
     i.rows = min(16, p.g - rb * 16);
     i.first = 0;
   }
-  i.units = static_cast<int>(min(static_cast<long long>(i.tiles + kItemTiles - s.x), s.count));
-  i.x0 = max(0, s.x - kItemTiles);
-  i.x1 = max(0, s.x + i.units - kItemTiles);
+  i.units = static_cast<int>(min(static_cast<long long>(i.tiles + p.item_tiles - s.x), s.count));
+  i.x0 = max(0, s.x - p.item_tiles);
+  i.x1 = max(0, s.x + i.units - p.item_tiles);
   return i;
 }
 // Behind n units of the item at hand.
@@ -495,7 +495,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
         if (threadIdx.x == 0) {
           const int64_t items = static_cast<int64_t>(p.B) * p.hkv * p.nrb;
           const int64_t id = s.b < 0 ? items + s.hv : static_cast<int64_t>(s.b) * p.hkv * p.nrb + s.hv;
-          const int last = s.all.holder(s.pos - s.x + i.tiles + kItemTiles - 1);
+          const int last = s.all.holder(s.pos - s.x + i.tiles + p.item_tiles - 1);
           p.desc[joined ? id : blockIdx.x] =
               Desc{s.b, s.hv, whole ? -1 : static_cast<int>(blockIdx.x), last - static_cast<int>(blockIdx.x) + 1};
         }
@@ -773,7 +773,10 @@ cudaError_t launch_paged_decode(const PagedPool& pool, const CUtensorMap& kmap,
   p.len_limit = limit < (1 << 30) ? static_cast<int>(limit) : 1 << 30;
   p.box_rows = paged_decode_box_rows(pool.page_size);
   p.scale_log2 = a.scale_log2;
-  p.n_units32 = static_cast<double>(a.B) * p.hkv * p.nrb * (p.len_limit / kTile + 2 + kItemTiles) < 2147483648.0;
+  // With more query heads the warps' merge takes more rounds (128 sequences of
+  // 8 heads a KV head behind a prefix: 116 us with 1, 111 with 2, 108.5 with 3).
+  p.item_tiles = p.g > kMergeRows ? 3 : 1;
+  p.n_units32 = static_cast<double>(a.B) * p.hkv * p.nrb * (p.len_limit / kTile + 2 + p.item_tiles) < 2147483648.0;
   p.prefix = a.prefix;
   if (pool.bf16)
     return pool.D == 128 ? launch<__nv_bfloat16, 128>(p, kmap, vmap, num_sms, stream)
