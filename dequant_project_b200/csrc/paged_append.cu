@@ -17,10 +17,11 @@
 // one lane and share a table entry; interleaved pairs lie in one lane anyway.
 // A warp takes a few heads of one token, whose table entries stay in
 // registers; the sum of squares is one shuffle reduction. What it measured
-// (B200, 8192 tokens of 64 + 2 x 8 heads of 128, bf16, norms): 69 us, 4.9 TB/s
-// of the 6.4 that a copy reaches. Registers decide: at 80 (three blocks an SM)
-// 69 us, at 128 (two) 79; one, two, three heads a lane group 84, 74, 70 us;
-// runs of four values instead of eight (more, narrower accesses) 84 us.
+// (B200, 8192 tokens of 64 + 2 x 8 heads of 128, bf16, norms): 59 us, 5.7 TB/s
+// of the 6.4 that a copy reaches. Registers and stores decide: 128 registers
+// (two blocks of 256 an SM) 79 us, 80 (three) 69; with stores that do not stay
+// in the L2 cache 62, in blocks of 128 threads 59. Runs of four values instead
+// of eight (more, narrower accesses) 84 us; one head a lane group at a time 84.
 #include <cstdint>
 
 #include "paged.cuh"
@@ -28,7 +29,7 @@
 namespace dqg {
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 128;
 constexpr int kIter = 4;  // heads a lane group takes one after the other
 
 template <typename E>
@@ -71,7 +72,7 @@ __device__ __forceinline__ uint4 pack8(const float* f) {
 }
 
 template <typename E, int D, int ITER, int LAYOUT>
-__global__ void __launch_bounds__(kThreads, LAYOUT == kUneven ? 2 : 3)
+__global__ void __launch_bounds__(kThreads, LAYOUT == kUneven ? 4 : 5)
     paged_append_kernel(const __grid_constant__ AppendParams<E> p) {
   constexpr int kLanes = D / 16;        // lanes a head
   constexpr int kGroups = 32 / kLanes;  // heads a warp holds at a time
@@ -198,8 +199,8 @@ __global__ void __launch_bounds__(kThreads, LAYOUT == kUneven ? 2 : 3)
       if (slot < 0) continue;
       dst = h < rotated ? p.k + base + (h - p.hq) * p.head_stride : p.v + base + (h - rotated) * p.head_stride;
     }
-    *reinterpret_cast<uint4*>(dst + ea) = xa[it];
-    *reinterpret_cast<uint4*>(dst + eb) = xb[it];
+    __stcs(reinterpret_cast<uint4*>(dst + ea), xa[it]);
+    __stcs(reinterpret_cast<uint4*>(dst + eb), xb[it]);
   }
 }
 

@@ -24,8 +24,14 @@
 //
 // A prefix whose rows (sequences times query heads of a KV head) fit two 16-row
 // tiles is streamed by this kernel itself, as items of its own ahead of the
-// sequences' (kStreamed in PrefixPieces); one with more rows is left to the
-// prompt kernel, which reads it once for 256 rows.
+// sequences' (prefix_streamed below); one with more rows is left to the prompt
+// kernel, which reads it once for 256 rows.
+//
+// Measured (B200): 64 sequences of 900 to 16000 positions, 64 query and 8 KV
+// heads, bf16, 1.25 GB: 200 us, 6.27 TB/s, 0.97 of the rate that a copy
+// reaches; HBM bounds it. Short calls are bound by latency: one sequence of 2049
+// positions, 32 heads (33.5 MB): 11.5 us, about 4 of them before the first tile
+// has come (shares, table, copies), 4.5 streaming, 3 for the second kernel.
 #include <cstdint>
 
 #include "paged.cuh"
@@ -726,7 +732,7 @@ Scratch scratch_of(int B, int hq, int n_kv_heads, int prefix_len, int num_sms) {
 
 // At most two 16-row tiles: streaming the prefix once or twice beats the prompt
 // kernel's start and its mostly empty 128-row tiles (16 sequences, 32 heads,
-// 2000 positions: VS us against 35 us).
+// 2000 positions: 23 us against 35).
 bool prefix_streamed(int n_seqs, int hq, int n_kv_heads) {
   const int g = hq / n_kv_heads;
   return g <= 16 && n_seqs <= 2 * (16 / g);
