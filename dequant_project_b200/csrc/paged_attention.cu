@@ -111,7 +111,7 @@ __device__ __forceinline__ Share find_share(const Params& p, int cta, int n_ctas
     return b < p.B ? tiles_of(clamped_len(p.lens, b, p.len_limit)) + p.item_tiles : 0;
   };
   Share s;
-  if (p.B <= 32 && p.pre_items == 0 && p.n_units32) {
+  if (p.B <= 32 && p.n_units32) {
     // Up to 32 sequences and 2^31 units: one scan, and little code (a launch
     // fetches it from the L2 cache at first use, which is most of the time
     // that a short call takes here).
@@ -122,18 +122,23 @@ __device__ __forceinline__ Share find_share(const Params& p, int cta, int n_ctas
       const uint32_t t = __shfl_up_sync(0xffffffffu, sum, off);
       if (lane >= off) sum += t;
     }
-    const uint32_t total = __shfl_sync(0xffffffffu, sum, 31) * hv;
+    const uint32_t ahead = static_cast<uint32_t>(pre);  // prefix items come first, as sequence -1
+    const uint32_t total = __shfl_sync(0xffffffffu, sum, 31) * hv + ahead;
     const uint32_t each = (total + n_ctas - 1) / n_ctas;
     const uint32_t pos = min(total, cta * each);
     s.all.total = total;
     s.all.each = each;
     s.pos = pos;
     s.count = min(total, pos + each) - pos;
-    const unsigned past = __ballot_sync(0xffffffffu, sum * hv > pos);
-    const int l = past ? __ffs(past) - 1 : 0;
-    const uint32_t per = max(1u, __shfl_sync(0xffffffffu, c, l));
-    const uint32_t in = pos - (__shfl_sync(0xffffffffu, sum, l) - per) * hv;
-    s.b = l;
+    uint32_t per = p.pre_tiles + p.item_tiles, in = pos;
+    s.b = -1;
+    if (pos >= ahead) {
+      const unsigned past = __ballot_sync(0xffffffffu, sum * hv > pos - ahead);
+      const int l = past ? __ffs(past) - 1 : 0;
+      per = max(1u, __shfl_sync(0xffffffffu, c, l));
+      in = pos - ahead - (__shfl_sync(0xffffffffu, sum, l) - per) * hv;
+      s.b = l;
+    }
     s.hv = in / per;
     s.x = in - s.hv * per;
     return s;
@@ -782,7 +787,8 @@ cudaError_t launch_paged_decode(const PagedPool& pool, const CUtensorMap& kmap,
   // With more query heads the warps' merge takes more rounds (128 sequences of
   // 8 heads a KV head behind a prefix: 116 us with 1, 111 with 2, 108.5 with 3).
   p.item_tiles = p.g > kMergeRows ? 3 : 1;
-  p.n_units32 = static_cast<double>(a.B) * p.hkv * p.nrb * (p.len_limit / kTile + 2 + p.item_tiles) < 2147483648.0;
+  p.n_units32 = static_cast<double>(a.B) * p.hkv * p.nrb * (p.len_limit / kTile + 2 + p.item_tiles) +
+                    static_cast<double>(p.pre_items) * (p.pre_tiles + p.item_tiles) < 2147483648.0;
   p.prefix = a.prefix;
   if (pool.bf16)
     return pool.D == 128 ? launch<__nv_bfloat16, 128>(p, kmap, vmap, num_sms, stream)
