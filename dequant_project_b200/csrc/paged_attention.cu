@@ -403,10 +403,6 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
 #pragma unroll
       for (int ks = 0; ks < D / 16; ++ks)
         ldsm_x4(smem_u32(qs) + (qi * q_rows + (lane & 15)) * (D * 2) + ks * 32 + (lane >> 4) * 16, qa[ks]);
-      __syncwarp();
-      if (lane == 0) mbar_arrive(s.b < 0 ? pre_empty : q_empty + qi);
-      if (s.b < 0) ++pre;
-      else ++item;
       float o[D / 8][4];
 #pragma unroll
       for (int nb = 0; nb < D / 8; ++nb) o[nb][0] = o[nb][1] = o[nb][2] = o[nb][3] = 0.f;
@@ -487,6 +483,19 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
         if (lane == 0) mbar_arrive(empty + st);
       }
       if (!ok) break;
+      // The queries' place is free once their reads have come back, not once
+      // they are issued: here every fragment is used (by the products, or, in a
+      // warp whose slices all lay behind the end, by this).
+      if (i.x0 * kTile + p0 >= len) {
+        uint32_t x = 0;
+#pragma unroll
+        for (int ks = 0; ks < D / 16; ++ks) x ^= qa[ks][0] ^ qa[ks][1] ^ qa[ks][2] ^ qa[ks][3];
+        asm volatile("" ::"r"(x) : "memory");
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(s.b < 0 ? pre_empty : q_empty + qi);
+      if (s.b < 0) ++pre;
+      else ++item;
 
       // The item's (or piece's) result: the warps' parts, four heads a round.
 #pragma unroll

@@ -195,6 +195,9 @@ DECODE = [
     ([75, 0], 128, 1, 128, 16),
     ([0, 0, 0], 4, 2, 128, 16),
     ([40] * 300, 2, 1, 64, 16),        # more sequences than CTAs
+    ([40] * 128, 64, 8, 128, 64),      # many items of one tile: queries' places are soon reused
+    ([64, 17] * 64, 128, 8, 128, 16),
+    ([33] * 200, 24, 4, 64, 32),
 ]
 
 
