@@ -302,7 +302,6 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
   // from only once its own inputs are complete), the queries, pages and
   // lengths may be read at once; only the end waits (and with it everything
   // behind this kernel).
-  // waits (and with it everything behind this kernel).
   const bool late = p.prefix.S > 0;
   const bool joined = late || p.pre_items > 0;  // results are joined with a prefix's
   if (!late) pdl_wait_prior_grid();

@@ -81,6 +81,7 @@ struct Params {
   bool causal;
   float scale_log2;
   uint32_t g_magic;                   // ceil(2^32 / g), 0 for g = 1
+  bool n_units32;                     // the units of any lengths fit 31 bits
   int prefix_len, splits, n_pieces;   // a shared prefix: splits > 0
 };
 
@@ -235,65 +236,100 @@ struct Share {  // a CTA's part of the units; x: the first one's place in its it
   int b, kvh, pair, x;
 };
 
-// Taken by one whole warp.
-__device__ __forceinline__ Share find_share(const Params& p, int cta, int n_ctas) {
+// Taken by one whole warp; *s: the sequence where the share starts.
+__device__ __forceinline__ Share find_share(const Params& p, int cta, int n_ctas, Seq* s) {
   const int lane = threadIdx.x & 31;
-  long long total = 0;
-  for (int b0 = 0; b0 < p.B; b0 += 32) {
-    const int b = b0 + lane;
-    if (b < p.B) {
-      const Seq s = load_seq(p, b);
-      total += cost_before(p, s, s.pairs);
-    }
-  }
-#pragma unroll
-  for (int off = 16; off >= 1; off >>= 1) total += __shfl_xor_sync(0xffffffffu, total, off);
   Share r;
-  // Shares of a block at least, so that none inside an item comes to nothing.
-  total *= p.hkv;
-  r.all.set(total, n_ctas, kBlock);
   r.b = r.kvh = r.pair = r.x = 0;
-  r.pos = r.all.begin(cta);
-  r.count = r.all.begin(cta + 1) - r.pos;
-  if (r.count == 0) return r;
-  long long before = 0;
-  for (int b0 = 0; b0 < p.B; b0 += 32) {
-    const int b = b0 + lane;
-    long long mine = 0;
-    if (b < p.B) {
-      const Seq s = load_seq(p, b);
-      mine = cost_before(p, s, s.pairs);
-    }
-    long long sum = mine * p.hkv;
+  long long in;
+  if (p.B <= 32 && p.n_units32) {
+    // Up to 32 sequences and 2^31 units: one scan, and little code (a launch
+    // fetches it from the L2 cache at first use, which is most of the time
+    // that a short call takes here).
+    Seq mine = {0, 0, 0, 0};
+    if (lane < p.B) mine = load_seq(p, lane);
+    const uint32_t c = static_cast<uint32_t>(cost_before(p, mine, mine.pairs));
+    uint32_t sum = c;
 #pragma unroll
     for (int off = 1; off < 32; off <<= 1) {
-      const long long t = __shfl_up_sync(0xffffffffu, sum, off);
+      const uint32_t t = __shfl_up_sync(0xffffffffu, sum, off);
       if (lane >= off) sum += t;
     }
-    const unsigned past = __ballot_sync(0xffffffffu, before + sum > r.pos);
-    if (past) {
-      const int l = __ffs(past) - 1;
-      const long long per = __shfl_sync(0xffffffffu, mine, l);
-      long long in = r.pos - (before + __shfl_sync(0xffffffffu, sum, l) - per * p.hkv);
-      r.b = b0 + l;
-      r.kvh = static_cast<int>(quotient(in, per));
-      in -= r.kvh * per;
-      // The pair: 32 probes a round.
-      const Seq s = load_seq(p, r.b);
-      int lo = 0, hi = s.pairs;
-      while (hi - lo > 1) {
-        const int step = (hi - lo + 31) >> 5;
-        const int probe = min(lo + (lane + 1) * step, hi);
-        const int f = __ffs(__ballot_sync(0xffffffffu, cost_before(p, s, probe) > in)) - 1;
-        hi = min(lo + (f + 1) * step, hi);
-        lo = lo + f * step;
-      }
-      r.pair = lo;
-      r.x = static_cast<int>(in - cost_before(p, s, lo));
-      break;
+    const uint32_t total = __shfl_sync(0xffffffffu, sum, 31) * p.hkv;
+    const uint32_t each = max((total + n_ctas - 1) / n_ctas, static_cast<uint32_t>(kBlock));
+    const uint32_t pos = min(total, cta * each);
+    r.all.total = total;
+    r.all.each = each;
+    r.pos = pos;
+    r.count = min(total, pos + each) - pos;
+    const unsigned past = __ballot_sync(0xffffffffu, sum * p.hkv > pos);
+    const int l = past ? __ffs(past) - 1 : 0;
+    const uint32_t per = max(1u, __shfl_sync(0xffffffffu, c, l));
+    const uint32_t rest = pos - (__shfl_sync(0xffffffffu, sum, l) - per) * p.hkv;
+    r.b = l;
+    r.kvh = rest / per;
+    in = rest - r.kvh * per;
+    s->q0 = __shfl_sync(0xffffffffu, mine.q0, l);
+    s->ql = __shfl_sync(0xffffffffu, mine.ql, l);
+    s->kv = __shfl_sync(0xffffffffu, mine.kv, l);
+    s->pairs = __shfl_sync(0xffffffffu, mine.pairs, l);
+    if (r.count == 0) return r;
+  } else {
+    long long total = 0;
+#pragma unroll 1
+    for (int b = lane; b < p.B; b += 32) {
+      const Seq t = load_seq(p, b);
+      total += cost_before(p, t, t.pairs);
     }
-    before += __shfl_sync(0xffffffffu, sum, 31);
+#pragma unroll 1
+    for (int off = 16; off >= 1; off >>= 1) total += __shfl_xor_sync(0xffffffffu, total, off);
+    // Shares of a block at least, so that none inside an item comes to nothing.
+    r.all.set(total * p.hkv, n_ctas, kBlock);
+    r.pos = r.all.begin(cta);
+    r.count = r.all.begin(cta + 1) - r.pos;
+    if (r.count == 0) return r;
+    long long before = 0, per = 1;
+#pragma unroll 1
+    for (int b0 = 0; b0 < p.B; b0 += 32) {
+      const int b = b0 + lane;
+      long long mine = 0;
+      if (b < p.B) {
+        const Seq t = load_seq(p, b);
+        mine = cost_before(p, t, t.pairs);
+      }
+      long long sum = mine * p.hkv;
+#pragma unroll 1
+      for (int off = 1; off < 32; off <<= 1) {
+        const long long t = __shfl_up_sync(0xffffffffu, sum, off);
+        if (lane >= off) sum += t;
+      }
+      const unsigned past = __ballot_sync(0xffffffffu, before + sum > r.pos);
+      if (past) {
+        const int l = __ffs(past) - 1;
+        per = __shfl_sync(0xffffffffu, mine, l);
+        before += __shfl_sync(0xffffffffu, sum, l) - per * p.hkv;
+        r.b = b0 + l;
+        break;
+      }
+      before += __shfl_sync(0xffffffffu, sum, 31);
+    }
+    in = r.pos - before;
+    r.kvh = static_cast<int>(quotient(in, per));
+    in -= r.kvh * per;
+    *s = load_seq(p, r.b);
   }
+  // The pair: 32 probes a round.
+  int lo = 0, hi = s->pairs;
+#pragma unroll 1
+  while (hi - lo > 1) {
+    const int step = (hi - lo + 31) >> 5;
+    const int probe = min(lo + (lane + 1) * step, hi);
+    const int f = __ffs(__ballot_sync(0xffffffffu, cost_before(p, *s, probe) > in)) - 1;
+    hi = min(lo + (f + 1) * step, hi);
+    lo = lo + f * step;
+  }
+  r.pair = lo;
+  r.x = static_cast<int>(in - cost_before(p, *s, lo));
   return r;
 }
 
@@ -317,9 +353,11 @@ struct Walk {
   Seq s;
   int piece;
   __device__ __forceinline__ void begin(const Params& p) {
-    if (!p.splits) r = find_share(p, blockIdx.x, gridDim.x);
     piece = blockIdx.x;
-    if (p.splits || r.count > 0) s = load_seq(p, p.splits ? 0 : r.b);
+    if (p.splits)
+      s = load_seq(p, 0);
+    else
+      r = find_share(p, blockIdx.x, gridDim.x, &s);
   }
   __device__ __forceinline__ void tiles(const Params& p, Segment& g, int pair) {
     const int first = pair * 2 * p.tq;  // the pair's first token in its sequence
@@ -980,6 +1018,8 @@ cudaError_t launch_prompt(const PagedPool& pool, const CUtensorMap& qmap, const 
   p.len_limit = limit < (1 << 30) ? static_cast<int>(limit) : 1 << 30;
   p.box_rows = prompt_box_rows(pool.page_size);
   p.causal = a.causal;
+  p.n_units32 = (static_cast<double>(a.T) / (2 * p.tq) + a.B) * (static_cast<double>(p.len_limit) + kItemKeys) *
+                    pool.n_kv_heads < 2147483648.0;
   p.scale_log2 = a.scale_log2;
   p.prefix_len = a.prefix_len;
   p.splits = p.n_pieces = 0;
