@@ -22,8 +22,8 @@
 // boxes, 128-byte swizzle, a ring of key and value blocks), one thread issues
 // the products on the tensor cores (tcgen05: S = Q K^T from shared memory,
 // O += P V with P in tensor memory), and each tile has four softmax warps, one
-// thread a row. Tensor memory holds both tiles' S (fp32, 128 columns; P takes
-// the place of S as it is formed) and O (fp32, D columns), so one tile's
+// thread a row. Tensor memory holds both tiles' S (fp32, 128 columns; with D =
+// 128 P takes the place of S as it is formed) and O (fp32, D columns), so one tile's
 // softmax runs while the other's products do. O stays in tensor memory over
 // all blocks: the maximum that weights refer to is moved, and O rescaled, only
 // when it grows by more than 2^8, which bounds the weights by 2^8; the sums are
@@ -429,6 +429,9 @@ template <int D>
 struct Layout {
   static constexpr int kStages = D == 128 ? 4 : 8;     // key or value blocks in flight
   static constexpr int kSlot = kBlock * D * 2;
+  // With D = 64 tensor memory has room for P beside S: the next block's scores
+  // are formed while a block's weights still are.
+  static constexpr bool kApart = D == 64;
   static constexpr int kTile = 128 * D * 2;            // a tile's queries
   static constexpr int kRing = 2 * kTile;              // offset of the ring
   static constexpr int kStore = kRing + kStages * kSlot;  // 4 KB a softmax warp, for its stores
@@ -587,12 +590,15 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       mma_commit(s_full + t);
     };
+    const uint32_t weights_at = L::kApart ? tmem + 2 * kBlock + 2 * D : tmem;
+    constexpr uint32_t weights_step = L::kApart ? kBlock / 2 : kBlock;
     auto issue_o = [&](int t, int slot, bool late, bool add) {
       const uint64_t b = v_desc + slot * (L::kSlot >> 4);
 #pragma unroll
       for (int k = 0; k < kBlock / 16; ++k) {
         if ((k < kEarly / 16) != late)
-          mma_ts(tmem + 2 * kBlock + t * D, tmem + t * kBlock + k * 8, b + (k * 16 * 128 >> 4), kIdO, add || k > 0);
+          mma_ts(tmem + 2 * kBlock + t * D, weights_at + t * weights_step + k * 8, b + (k * 16 * 128 >> 4), kIdO,
+                 add || k > 0);
       }
     };
     auto commit = [&](uint64_t* bar) {
@@ -643,12 +649,14 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (!ok || j >= c) continue;
           ok = wait(p_half + t, weights >> t & 1);
           if (!ok) continue;
+          // (Early weights also say that the block's scores have been read.)
+          if (L::kApart && j + 1 < c) issue_s(t, kslot);
           issue_o(t, vslot, false, j > 0);
           ok = wait(p_full + t, weights >> t & 1);
           weights ^= 1u << t;
           if (!ok) continue;
           issue_o(t, vslot, true, true);
-          if (j + 1 < c) issue_s(t, kslot);
+          if (!L::kApart && j + 1 < c) issue_s(t, kslot);
           else commit(o_full + t);
         }
         commit(empty + vslot);
@@ -668,6 +676,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int t = warp >> 2, r = threadIdx.x & 127;
     const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;  // this warp's 32 lanes
     const uint32_t ts = tmem + lanes + t * kBlock, to = tmem + lanes + 2 * kBlock + t * D;
+    const uint32_t tp = L::kApart ? tmem + lanes + 2 * kBlock + 2 * D + t * (kBlock / 2) : ts;  // weights
     const int tok = t * p.tq + r / p.g;  // of the pair
     const float2 scale2 = make_float2(p.scale_log2, p.scale_log2);
     int seg = 0, scores = 0, outs = 0, base = 0;
@@ -710,6 +719,16 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int q = 0; q < 4; ++q) mx[q] = fmaxf(mx[q], s[i + q]);
         const float m_new = fmaxf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])), m);
         const bool grow = (m_new - m) * p.scale_log2 > kMaxGrowth;
+        if (L::kApart && j > 0) {
+          // The block before has to be in O, and its weights read, before
+          // either changes (with P in the place of S its scores say so).
+          if (!warp_wait(o_full + t, outs & 1)) {
+            ok = false;
+            break;
+          }
+          ++outs;
+          fence_after_sync();
+        }
         if (j == 0) {
           m = m_new;  // no O yet: the first product overwrites it
         } else if (__any_sync(0xffffffffu, grow)) {
@@ -762,8 +781,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         {
           uint32_t w[kEarly / 2];
           weigh(0, w, kEarly);
-          tmem_st32(ts, w);
-          tmem_st16(ts + 32, w + 32);
+          tmem_st32(tp, w);
+          tmem_st16(tp + 32, w + 32);
           tmem_wait_st();
           fence_before_sync();
           mbar_arrive(p_half + t);
@@ -771,7 +790,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         {
           uint32_t w[(kBlock - kEarly) / 2];
           weigh(kEarly, w, kBlock - kEarly);
-          tmem_st16(ts + kEarly / 2, w);
+          tmem_st16(tp + kEarly / 2, w);
           tmem_wait_st();
           fence_before_sync();
           mbar_arrive(p_full + t);
