@@ -46,7 +46,9 @@
 // maximum is known (1012), two threads a row (1166), blocks of 64 keys with the
 // scores one block ahead (1114: a product of 64 columns reads its operands at
 // 2/3 of the rate, and its one issuing thread becomes the bound), a product
-// warp for each tile (1182).
+// warp for each tile (1182). With D = 64 the products are half as long and P has
+// columns of its own, so the softmax alone bounds it: 13 packed prompts, 6858
+// tokens, 32 and 8 heads: 104 us (115 with P in the place of S).
 #include <cstdint>
 
 #include "paged.cuh"

@@ -186,7 +186,9 @@ def prompt_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tens
     [B + 1], from 0 to T), and they are the newest of its ``kv_lens[b]`` cached
     positions (so they were stored first). Row i of q_len sees the keys before
     kv_len - q_len + i + 1 (all kv_len unless ``causal``); a row that sees none
-    gives zeros. Rows outside every sequence are undefined in the result.
+    gives zeros. Rows outside every sequence are undefined in the result, and a
+    non-finite value that the mask hides from a row reaches it where both fall
+    into one block of 128 positions.
     Returns [T, Hq, D]. Table, lengths, scale and workspace
     (``prompt_attention_workspace``) as ``paged_attention``."""
     if q.is_cuda:

@@ -402,10 +402,10 @@ int dqg_paged_attention(const void *q, int64_t q_stride_seq, int64_t q_stride_he
  * q_starts[b + 1] - 1 of q [T, Hq, D] (q_starts[0] = 0, ascending, the last
  * one T; sequences may be empty), the newest of its kv_lens[b] cached
  * positions. Causal: its row i sees the keys before kv_lens[b] - q_len + i + 1;
- * otherwise all kv_lens[b]. A row that sees none gives zeros. Values at cached
- * positions must be finite where a causal mask hides them from some rows (a
- * hidden infinity or NaN among the last 128 positions before a row's own block
- * ends reaches the row); what lies behind a sequence's end does not matter.
+ * otherwise all kv_lens[b]. A row that sees none gives zeros. What lies behind
+ * a sequence's end does not matter; a non-finite value at a cached position that
+ * the mask hides from a row reaches the row all the same when the position and
+ * the last key that the row sees fall into one block of 128 positions.
  * Heads, strides, table, lengths on the device, scale and workspace
  * (dqg_prompt_attention_workspace(D) bytes) as dqg_paged_attention. Rows of q
  * outside every sequence leave their rows of out unwritten.
