@@ -149,3 +149,37 @@ def test_rope_tables_reject_bad_arguments():
                {"scaling": {"type": "linear", "factor": 0.5}}):
         with pytest.raises(ValueError):
             paged_ops.rope_scaled_tables(64, 1e4, 8, "cpu", **kw)
+
+
+def _serve(world):
+    import socket
+
+    import torch.multiprocessing as mp
+
+    import paged_workers
+    with socket.socket() as s:
+        s.bind(("127.0.0.1", 0))
+        port = s.getsockname()[1]
+    ctx = mp.get_context("spawn")
+    queue = ctx.Queue()
+    procs = [ctx.Process(target=paged_workers.serve, args=(r, world, port, queue)) for r in range(world)]
+    for p in procs:
+        p.start()
+    got = {}
+    for _ in procs:
+        rank, logits, err = queue.get(timeout=120)
+        assert err is None, err
+        got[rank] = torch.from_numpy(logits)
+    for p in procs:
+        p.join(timeout=60)
+        assert p.exitcode == 0
+    return got
+
+
+def test_two_ranks_serve_what_one_does():
+    """Heads, intermediate and vocabulary split over two gloo ranks: every rank
+    gathers the logits of the single-rank run (sums of two partials instead of
+    one: the decoder tests' bound)."""
+    one, two = _serve(1)[0], _serve(2)
+    assert torch.equal(two[0], two[1])
+    assert max_rel_err(two[0], one) < 5e-3
