@@ -24,6 +24,10 @@ struct Elem<__half> {
     return *reinterpret_cast<const uint32_t*>(&h);
   }
   static __device__ __forceinline__ float load(const __half* p) { return __half2float(*p); }
+  // a b + c, two values at a time.
+  static __device__ __forceinline__ uint32_t fma2(uint32_t a, uint32_t b, uint32_t c) { return hfma2_u32(a, b, c); }
+  // All ones in each half that holds an infinity or a NaN.
+  static __device__ __forceinline__ uint32_t non_finite(uint32_t v) { return __vcmpeq2(v & 0x7c007c00u, 0x7c007c00u); }
   // d += a b for one 16x16 by 16x8 tile (fp32 accumulators).
   static __device__ __forceinline__ void mma(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 "
@@ -45,6 +49,12 @@ struct Elem<__nv_bfloat16> {
   static __device__ __forceinline__ float load(const __nv_bfloat16* p) {
     return __bfloat162float(*p);
   }
+  static __device__ __forceinline__ uint32_t fma2(uint32_t a, uint32_t b, uint32_t c) {
+    uint32_t d;
+    asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
+    return d;
+  }
+  static __device__ __forceinline__ uint32_t non_finite(uint32_t v) { return __vcmpeq2(v & 0x7f807f80u, 0x7f807f80u); }
   static __device__ __forceinline__ void mma(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 "
         "{%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"

@@ -18,6 +18,13 @@
 // CTA; one that is cut leaves its pieces (max, sum, O) in the workspace, and a
 // second kernel joins them in order (no atomics, the same bits every time).
 //
+// The products run over whole blocks of keys for a whole tile, with weights of
+// zero where a row sees nothing. A zero weight times an infinity would not be
+// zero, so the values that some row of the pair does not see are looked at first,
+// by two warps of their own beside the softmax: non-finite ones become zeros in
+// shared memory (finite ones cost one fused multiply-add each), and rows that do
+// see one take it from memory when the segment ends.
+//
 // One CTA per SM: one warp copies queries and page rows (tensor-map
 // boxes, 128-byte swizzle, a ring of key and value blocks), one thread issues
 // the products on the tensor cores (tcgen05: S = Q K^T from shared memory,
@@ -57,8 +64,8 @@ namespace dqg {
 namespace {
 
 constexpr int kBlock = 128;         // keys a block; rows a tile
-constexpr int kThreads = 384;       // 2 x 4 softmax warps; products, copies, two idle
-constexpr int kMmaWarp = 8, kCopyWarp = 9;
+constexpr int kThreads = 384;       // 2 x 4 softmax warps; products, copies, 2 value warps
+constexpr int kMmaWarp = 8, kCopyWarp = 9, kValueWarp = 10, kValueWarps = 2;
 constexpr float kMaxGrowth = 8.f;   // log2 of the largest weight
 constexpr int kEarly = 96;          // keys whose weights are handed over first
 // An item's start and end, in keys' time (8192 tokens, 64/8 heads: 1019 us with
@@ -71,6 +78,7 @@ struct Desc {  // a cut item, by the CTA that holds its first piece
 };
 
 struct Params {
+  const void* v;  // the pool of value pages
   const int32_t* table;
   const int32_t* q_starts;
   const int32_t* lens;
@@ -78,7 +86,7 @@ struct Params {
   float4* part;   // [slot][D / 4][256]
   float* ml;      // [slot][2][256]
   Desc* desc;     // [CTA]
-  int64_t table_stride, n_pages;
+  int64_t table_stride, n_pages, page_stride, head_stride, row_stride;
   int B, T, hq, hkv, g, tq, page_shift, len_limit, box_rows;
   bool causal;
   float scale_log2;
@@ -343,6 +351,9 @@ struct Segment {
   int kv, lim0;                       // keys; keys that the first token sees (or below 0)
   int whole;                          // the item lies in this segment
   int pieces;                         // of the item, where this is the first of several
+  int b;                              // sequence
+  int from, check;                    // the value warps look at keys >= from, in blocks >= check
+  int tainted;                        // such a key's values were not finite (set by the value warps)
 };
 // Blocks of a segment that tile t takes part in.
 __device__ __forceinline__ int tile_count(const Segment& g, int t) {
@@ -438,8 +449,98 @@ struct Layout {
   static constexpr int kRing = 2 * kTile;              // offset of the ring
   static constexpr int kStore = kRing + kStages * kSlot;  // 4 KB a softmax warp, for its stores
   static constexpr int kBars = kStore + 8 * 4096;
-  static constexpr int kSmem = 1024 + kBars + 768;
+  static constexpr int kBarBytes = (4 * kStages + 11 + 2 * kSegs) * 8 + kSegs * static_cast<int>(sizeof(Segment)) + 8;
+  static constexpr int kSmem = 1024 + kBars + kBarBytes;
 };
+
+// Zeros in place of the non-finite values in rows [r0, r1) of a block in shared
+// memory (128 rows in halves of 64 values); whether one of the first `rows` rows
+// held one. r0 is a multiple of 4. Taken by the value warps, `part` of them each.
+template <typename E, int D>
+__device__ __forceinline__ bool clean_values(uint8_t* v, int r0, int r1, int rows, int part) {
+  const int lane = threadIdx.x & 31;
+  uint32_t acc[4] = {0u, 0u, 0u, 0u};  // 0 x = 0 for every finite x, NaN otherwise
+#pragma unroll 4
+  for (int r = r0 + 4 * part; r < r1; r += 4 * kValueWarps) {
+#pragma unroll
+    for (int h = 0; h < D / 64; ++h) {
+      const uint4 w = *reinterpret_cast<const uint4*>(v + h * (kBlock * 128) + r * 128 + lane * 16);
+      acc[0] = Elem<E>::fma2(w.x, 0u, acc[0]);
+      acc[1] = Elem<E>::fma2(w.y, 0u, acc[1]);
+      acc[2] = Elem<E>::fma2(w.z, 0u, acc[2]);
+      acc[3] = Elem<E>::fma2(w.w, 0u, acc[3]);
+    }
+  }
+  if (!__any_sync(0xffffffffu, (acc[0] | acc[1] | acc[2] | acc[3]) != 0u)) return false;
+  bool seen = false;
+#pragma unroll 1
+  for (int i = 0; i < D / 64 * kBlock; i += 4) {  // (rows of both halves)
+    const int r = i % kBlock;
+    if (r < r0 || r >= r1 || (r / 4) % kValueWarps != (r0 / 4 + part) % kValueWarps) continue;
+    uint4* at = reinterpret_cast<uint4*>(v + i * 128 + lane * 16);
+    uint4 w = *at;
+    uint32_t* ww = reinterpret_cast<uint32_t*>(&w);
+    bool any = false;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const uint32_t bad = Elem<E>::non_finite(ww[e]);
+      any |= bad != 0u;
+      ww[e] &= ~bad;
+    }
+    if (any) {
+      *at = w;
+      seen |= r + (lane >> 3) < rows;
+    }
+  }
+  return __any_sync(0xffffffffu, seen);
+}
+
+// Adds to this thread's row of tile `tile` the non-finite values, among the keys
+// that it sees, which clean_values took out of a segment's products. (A key that
+// a row sees has a positive weight, whatever a 16-bit type makes of it.) Taken by
+// the tile's softmax warps; rare, and out of line, where it takes no registers
+// from them.
+template <typename E, int D>
+__device__ __noinline__ void take_non_finite(const Params& p, const Segment& g, int tile, uint32_t tmem) {
+  const uint32_t to = tmem + (((threadIdx.x >> 5) & 3) << 21) + 2 * kBlock + tile * D;
+  const int token = tile * p.tq + (threadIdx.x & 127) / p.g;
+  const int limit = p.causal ? min(g.lim0 + token, g.kv) : g.kv;
+  const int from = max(g.from, g.x0 * kBlock), end = min(g.kv, (g.x0 + tile_count(g, tile)) * kBlock);
+  const int32_t* table = p.table + g.b * p.table_stride;
+  const E* pool = static_cast<const E*>(p.v) + g.kvh * p.head_stride;
+  const int in_page = (1 << p.page_shift) - 1;
+#pragma unroll 1
+  for (int q = 0; q < D / 32; ++q) {
+    uint32_t o[32];
+    tmem_ld32(to + 32 * q, o);
+    tmem_wait_ld();
+    hold32(o);
+#pragma unroll 1
+    for (int t = from; t < end; ++t) {
+      const int page = __ldg(table + (t >> p.page_shift));
+      if (page < 0 || page >= p.n_pages) continue;
+      const uint4* row =
+          reinterpret_cast<const uint4*>(pool + page * p.page_stride + (t & in_page) * p.row_stride + 32 * q);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint4 w = row[i];
+        const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const uint32_t bad = Elem<E>::non_finite(ww[e]);
+          if (bad != 0u && t < limit) {
+            const float2 x = Elem<E>::unpack(ww[e] & bad);
+            o[8 * i + 2 * e] = __float_as_uint(__uint_as_float(o[8 * i + 2 * e]) + x.x);
+            o[8 * i + 2 * e + 1] = __float_as_uint(__uint_as_float(o[8 * i + 2 * e + 1]) + x.y);
+          }
+        }
+      }
+    }
+    __syncwarp();
+    tmem_st32(to + 32 * q, o);
+  }
+  tmem_wait_st();
+}
 
 template <typename E, int D>
 __global__ void __launch_bounds__(kThreads, 1)
@@ -461,7 +562,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* seg_full = o_full + 2;       // [kSegs]
   uint64_t* seg_empty = seg_full + kSegs;
   uint64_t* drained = seg_empty + kSegs;
-  Segment* segs = reinterpret_cast<Segment*>(drained + 1);  // [kSegs]
+  uint64_t* asked = drained + 1;         // [kStages], in the order of the checked blocks:
+  uint64_t* checked = asked + kStages;   // values on their way; values checked
+  Segment* segs = reinterpret_cast<Segment*>(checked + kStages);  // [kSegs]
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(segs + kSegs);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t sbase = smem_u32(smem);
@@ -470,6 +573,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int i = 0; i < kStages; ++i) {
       mbar_init(full + i, 1);
       mbar_init(empty + i, 1);
+      mbar_init(asked + i, 1);
+      mbar_init(checked + i, kValueWarps);
     }
     mbar_init(q_full, 1);
     mbar_init(q_empty, 1);
@@ -481,7 +586,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     for (int i = 0; i < kSegs; ++i) {
       mbar_init(seg_full + i, 1);
-      mbar_init(seg_empty + i, 9);
+      mbar_init(seg_empty + i, 9 + kValueWarps);
     }
     mbar_init(drained, 1);
     fence_mbar_init();
@@ -521,15 +626,19 @@ __global__ void __launch_bounds__(kThreads, 1)
     Segment g;
     const int per = p.box_rows, boxes = kBlock / per * (D / 64);
     const int half = lane % (D / 64), sub = lane / (D / 64);
-    int seg = 0, pos = 0;
+    int seg = 0, pos = 0, checks = 0;
     bool ok = true;
     while (ok) {
       int b = 0;
       const bool more = walk.next(p, g, b);
       const int sg = seg % kSegs;
       if (seg >= kSegs && !warp_wait(seg_empty + sg, ((seg / kSegs) & 1) ^ 1)) break;
+      g.from = max(0, p.causal ? g.lim0 : g.kv) & ~3;
+      g.check = max(g.x0, g.from / kBlock);
       if (lane == 0) {
         if (!more) g.x0 = g.x1 = 0;  // the end
+        g.b = b;
+        g.tainted = 0;
         segs[sg] = g;
         mbar_arrive(seg_full + sg);
       }
@@ -567,6 +676,10 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (lane < boxes)
             tma_load_4d(sbase + L::kRing + st * L::kSlot + half * (kBlock * 128) + sub * per * 128,
                         w ? &vmap : &kmap, full + st, half * 64, in_page, g.kvh, page);
+        }
+        if (ok && x >= g.check) {
+          if (lane == 0) mbar_arrive(asked + checks % kStages);
+          ++checks;
         }
       }
     }
@@ -671,6 +784,39 @@ __global__ void __launch_bounds__(kThreads, 1)
     mbar_wait(drained, 0);
     }
     __syncwarp();
+  } else {
+    // ---- values that not every row sees. Blocks that need no look are not
+    // waited for, so the copies say when one that does is on its way: the phase
+    // of its ring slot is then the current one, and stays so until the products
+    // have taken it, which these warps have to let them first. (For the same reason
+    // no phase of `asked` or `checked` is ever overrun.)
+    int seg = 0, base = 0, n = 0;
+    bool ok = true;
+    while (ok) {
+      const int sg = seg % kSegs;
+      if (!warp_wait(seg_full + sg, (seg / kSegs) & 1)) break;
+      Segment& g = segs[sg];
+      const int x0 = g.x0, x1 = g.x1, kv = g.kv;
+      if (x1 == x0) break;
+      ++seg;
+      for (int x = g.check; x < x1; ++x, ++n) {
+        const int pos = base + 2 * (x - x0) + 1;
+        if (!warp_wait(asked + n % kStages, (n / kStages) & 1) || !warp_wait(full + pos % kStages, (pos / kStages) & 1)) {
+          ok = false;
+          break;
+        }
+        // Rows of the last page behind the end hold anything, those of no page zeros.
+        const int rows = kv - x * kBlock, end = ((rows - 1) | ((1 << p.page_shift) - 1)) + 1;
+        if (clean_values<E, D>(smem + L::kRing + (pos % kStages) * L::kSlot, max(0, g.from - x * kBlock),
+                               min(kBlock, end), rows, warp - kValueWarp))
+          g.tainted = 1;
+        fence_async_shared();  // before the products read them
+        __syncwarp();
+        if (lane == 0) mbar_arrive(checked + n % kStages);
+      }
+      base += 2 * (x1 - x0);
+      if (ok && lane == 0) mbar_arrive(seg_empty + sg);
+    }
   }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
@@ -681,7 +827,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t tp = L::kApart ? tmem + lanes + 2 * kBlock + 2 * D + t * (kBlock / 2) : ts;  // weights
     const int tok = t * p.tq + r / p.g;  // of the pair
     const float2 scale2 = make_float2(p.scale_log2, p.scale_log2);
-    int seg = 0, scores = 0, outs = 0, base = 0;
+    int seg = 0, scores = 0, outs = 0, checks = 0;
     bool ok = true, cut_first = false;
     while (true) {
       const int sg = seg % kSegs;
@@ -748,24 +894,6 @@ __global__ void __launch_bounds__(kThreads, 1)
           l *= f;
           if (grow) m = m_new;
         }
-        // Behind the sequence's end its last page holds anything: zero those
-        // values (a zero weight times an infinity would not be zero).
-        if (k0 + kBlock > kv && kv > k0 && (kv & ((1 << p.page_shift) - 1))) {
-          const int vpos = base + 2 * j + 1;
-          if (!warp_wait(full + vpos % kStages, (vpos / kStages) & 1)) {
-            ok = false;
-            break;
-          }
-          const int r0 = kv - k0;
-          const int r1 = min(kBlock, ((r0 >> p.page_shift) + 1) << p.page_shift);
-          uint8_t* v = smem + L::kRing + (vpos % kStages) * L::kSlot;
-          for (int i = r; i < (r1 - r0) * (D / 8); i += 128) {
-            const int row = r0 + i / (D / 8), ch = i % (D / 8);
-            *reinterpret_cast<uint4*>(v + (ch >> 3) * (kBlock * 128) + row * 128 + (ch & 7) * 16) =
-                make_uint4(0, 0, 0, 0);
-          }
-          fence_async_shared();
-        }
         const float ref = m == -INFINITY ? 0.f : m * p.scale_log2;
         const float2 ref2 = make_float2(-ref, -ref);
         float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
@@ -785,6 +913,13 @@ __global__ void __launch_bounds__(kThreads, 1)
           weigh(0, w, kEarly);
           tmem_st32(tp, w);
           tmem_st16(tp + 32, w + 32);
+          if (x0 + j >= g.check) {
+            const int c = checks + x0 + j - g.check;
+            if (!warp_wait(checked + c % kStages, (c / kStages) & 1)) {
+              ok = false;
+              break;
+            }
+          }
           tmem_wait_st();
           fence_before_sync();
           mbar_arrive(p_half + t);
@@ -799,7 +934,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
       }
-      base += 2 * all;
+      checks += max(0, x0 + all - g.check);
       if (!ok) break;
       if (g.pieces && threadIdx.x == 0) p.desc[blockIdx.x] = Desc{g.tok0, g.ntok, g.kvh, g.pieces};
       cut_first |= g.pieces != 0;
@@ -807,6 +942,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!warp_wait(o_full + t, outs & 1)) break;
         ++outs;
         fence_after_sync();
+        if (g.tainted) take_non_finite<E, D>(p, g, t, tmem);
       }
       if ((t ? g.n1 : g.n0) > 0) {
         if (g.whole) {
@@ -1020,6 +1156,10 @@ cudaError_t launch_prompt(const PagedPool& pool, const CUtensorMap& qmap, const 
                           const CUtensorMap& vmap, const PromptArgs& a, int num_sms,
                           cudaStream_t stream) {
   Params p;
+  p.v = pool.v;
+  p.page_stride = pool.page_stride;
+  p.head_stride = pool.head_stride;
+  p.row_stride = pool.row_stride;
   p.table = a.table;
   p.q_starts = a.q_starts;
   p.lens = a.kv_lens;

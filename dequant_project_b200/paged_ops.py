@@ -147,7 +147,14 @@ def _cpu_attention(q, k, v, ends, scale):
     seen = (torch.arange(n)[None] < ends[:, None])[:, None, None]
     s = s.masked_fill(~seen, float("-inf"))
     p = torch.softmax(s, -1).masked_fill(~seen, 0.0)
-    return torch.einsum("rkgt,ktd->rkgd", p, v).reshape(rows, hq, d)
+    fine = torch.isfinite(v)
+    out = torch.einsum("rkgt,ktd->rkgd", p, torch.where(fine, v, 0.0))
+    # A weight of zero times an infinity is not zero: rows take the non-finite
+    # values that they see, and no others.
+    for t in torch.nonzero(~fine.all(-1).all(0))[:, 0].tolist():
+        x = torch.where(fine[:, t], 0.0, v[:, t])[None, :, None]
+        out = out + torch.where(seen[..., t, None], x, 0.0)
+    return out.reshape(rows, hq, d)
 
 
 def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch.Tensor,
@@ -186,9 +193,8 @@ def prompt_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tens
     [B + 1], from 0 to T), and they are the newest of its ``kv_lens[b]`` cached
     positions (so they were stored first). Row i of q_len sees the keys before
     kv_len - q_len + i + 1 (all kv_len unless ``causal``); a row that sees none
-    gives zeros. Rows outside every sequence are undefined in the result, and a
-    non-finite value that the mask hides from a row reaches it where both fall
-    into one block of 128 positions.
+    gives zeros, and what a row does not see does not matter to it, non-finite
+    values included. Rows outside every sequence are undefined in the result.
     Returns [T, Hq, D]. Table, lengths, scale and workspace
     (``prompt_attention_workspace``) as ``paged_attention``."""
     if q.is_cuda:

@@ -402,10 +402,8 @@ int dqg_paged_attention(const void *q, int64_t q_stride_seq, int64_t q_stride_he
  * q_starts[b + 1] - 1 of q [T, Hq, D] (q_starts[0] = 0, ascending, the last
  * one T; sequences may be empty), the newest of its kv_lens[b] cached
  * positions. Causal: its row i sees the keys before kv_lens[b] - q_len + i + 1;
- * otherwise all kv_lens[b]. A row that sees none gives zeros. What lies behind
- * a sequence's end does not matter; a non-finite value at a cached position that
- * the mask hides from a row reaches the row all the same when the position and
- * the last key that the row sees fall into one block of 128 positions.
+ * otherwise all kv_lens[b]. A row that sees none gives zeros. What a row does
+ * not see, behind the sequence's end or hidden by the mask, does not matter to it.
  * Heads, strides, table, lengths on the device, scale and workspace
  * (dqg_prompt_attention_workspace(D) bytes) as dqg_paged_attention. Rows of q
  * outside every sequence leave their rows of out unwritten.
