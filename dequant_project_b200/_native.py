@@ -129,6 +129,9 @@ def lib() -> ctypes.CDLL:
     h.dqg_shared_prefix_attention.restype = i32
     h.dqg_shared_prefix_attention.argtypes = [vp, i64, i64, i64, i64, kv, vp, i64, i64, vp, i64,
                                               i64, vp, f32, vp, vp, u64, vp]
+    h.dqg_debug_paged_starved.restype = i32
+    h.dqg_debug_paged_starved.argtypes = [*h.dqg_shared_prefix_attention.argtypes[:-1],
+                                          ctypes.c_uint32, u64, vp]
     _lib = h
     return _lib
 
@@ -143,7 +146,7 @@ EXPORTED = ("dqg_last_error", "dqg_version", "dqg_add_one", "dqg_gemv", "dqg_deq
             "dqg_peer_allreduce_add_rms_norm", "dqg_gemv_swiglu",
             "dqg_gemv_swiglu_supported", "dqg_rope_paged_append", "dqg_paged_attention_workspace",
             "dqg_paged_attention", "dqg_prompt_attention_workspace", "dqg_prompt_attention",
-            "dqg_shared_prefix_workspace", "dqg_shared_prefix_attention")
+            "dqg_shared_prefix_workspace", "dqg_shared_prefix_attention", "dqg_debug_paged_starved")
 
 
 def check(rc: int) -> None:

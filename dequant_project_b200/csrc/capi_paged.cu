@@ -369,12 +369,14 @@ int dqg_shared_prefix_workspace(int64_t n_seqs, int64_t n_q_heads, int64_t n_kv_
   return api_ok();
 }
 
-int dqg_shared_prefix_attention(const void* q, int64_t q_stride_seq, int64_t q_stride_head, int64_t n_seqs,
-                                int64_t n_q_heads, const dqg_paged_kv* kv, const int32_t* prefix_table,
-                                int64_t prefix_pages, int64_t prefix_len, const int32_t* block_table,
-                                int64_t table_width, int64_t table_stride, const int32_t* kv_lens,
-                                float scale, void* out, void* workspace, uint64_t workspace_bytes,
-                                void* stream) {
+}  // extern "C"
+
+namespace {
+int shared_prefix(const void* q, int64_t q_stride_seq, int64_t q_stride_head, int64_t n_seqs,
+                  int64_t n_q_heads, const dqg_paged_kv* kv, const int32_t* prefix_table,
+                  int64_t prefix_pages, int64_t prefix_len, const int32_t* block_table, int64_t table_width,
+                  int64_t table_stride, const int32_t* kv_lens, float scale, void* out, void* workspace,
+                  uint64_t workspace_bytes, uint32_t starved, uint64_t wait_ns, void* stream) {
   dqg::PagedPool pool;
   int rc = check_pool(kv, &pool);
   if (rc) return rc;
@@ -399,6 +401,8 @@ int dqg_shared_prefix_attention(const void* q, int64_t q_stride_seq, int64_t q_s
   dqg::DecodeArgs d;
   std::memset(&d, 0, sizeof(d));
   d.workspace = workspace;
+  d.starved = starved;
+  d.wait_ns = wait_ns;
   d.prefix_len = static_cast<int>(prefix_len);
   d.prefix_table = prefix_table;
   CUtensorMap qmap, kmap, vmap;
@@ -438,6 +442,35 @@ int dqg_shared_prefix_attention(const void* q, int64_t q_stride_seq, int64_t q_s
   const cudaError_t e = dqg::launch_paged_decode(pool, kmap, vmap, d, sms, static_cast<cudaStream_t>(stream));
   if (e != cudaSuccess) return api_cuda_fail(e, "shared_prefix_attention launch");
   return api_ok();
+}
+}  // namespace
+
+extern "C" {
+
+int dqg_shared_prefix_attention(const void* q, int64_t q_stride_seq, int64_t q_stride_head, int64_t n_seqs,
+                                int64_t n_q_heads, const dqg_paged_kv* kv, const int32_t* prefix_table,
+                                int64_t prefix_pages, int64_t prefix_len, const int32_t* block_table,
+                                int64_t table_width, int64_t table_stride, const int32_t* kv_lens,
+                                float scale, void* out, void* workspace, uint64_t workspace_bytes,
+                                void* stream) {
+  return shared_prefix(q, q_stride_seq, q_stride_head, n_seqs, n_q_heads, kv, prefix_table, prefix_pages,
+                       prefix_len, block_table, table_width, table_stride, kv_lens, scale, out, workspace,
+                       workspace_bytes, 0, 0, stream);
+}
+
+int dqg_debug_paged_starved(const void* q, int64_t q_stride_seq, int64_t q_stride_head, int64_t n_seqs,
+                            int64_t n_q_heads, const dqg_paged_kv* kv, const int32_t* prefix_table,
+                            int64_t prefix_pages, int64_t prefix_len, const int32_t* block_table,
+                            int64_t table_width, int64_t table_stride, const int32_t* kv_lens, float scale,
+                            void* out, void* workspace, uint64_t workspace_bytes, uint32_t starved,
+                            uint64_t wait_ns, void* stream) {
+  if (wait_ns < 1000000ull || wait_ns > 1000000000ull)
+    return api_fail(DQG_ERR_INVALID, "wait_ns must be in [1 ms, 1 s], got %llu", (unsigned long long)wait_ns);
+  if (starved < 1 || starved > 31)
+    return api_fail(DQG_ERR_INVALID, "starved must be in [1, 31], got %u", starved);
+  return shared_prefix(q, q_stride_seq, q_stride_head, n_seqs, n_q_heads, kv, prefix_table, prefix_pages,
+                       prefix_len, block_table, table_width, table_stride, kv_lens, scale, out, workspace,
+                       workspace_bytes, starved, wait_ns, stream);
 }
 
 }  // extern "C"

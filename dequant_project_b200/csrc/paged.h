@@ -59,6 +59,8 @@ struct DecodeArgs {
   int prefix_len;               // a shared prefix: 0 for none
   const int32_t* prefix_table;
   PrefixPieces prefix;          // its pieces, where the prompt kernel took it
+  uint64_t wait_ns;             // limit of a wait; 0: the library's
+  uint32_t starved;             // diagnostic: bit w < 4, consumer warp w gives up at once; bit 4, nothing is copied
 };
 size_t paged_decode_workspace(int B, int hq, int n_kv_heads, int D, int prefix_len, int num_sms);
 // Whether the decode kernel streams a prefix itself (else the prompt kernel

@@ -22,6 +22,10 @@
 // shared prefix every item leaves its result to the second kernel, which joins
 // it with the prefix's pieces: nothing here waits for those.
 //
+// Waits are bounded. A consumer warp whose wait ran out goes on through its
+// items without data and makes their results NaN, so that the barriers among
+// the warps are always met and every item is described to the second kernel.
+//
 // A prefix whose rows (sequences times query heads of a KV head) fit two 16-row
 // tiles is streamed by this kernel itself, as items of its own ahead of the
 // sequences' (prefix_streamed below); one with more rows is left to the prompt
@@ -68,6 +72,8 @@ struct Params {
   int item_tiles;                                // an item's start and end, in tiles' time
   int pre_len, pre_seqs, pre_tiles, pre_items;  // a streamed prefix: sequences an item; tiles; items
   float scale_log2;
+  uint32_t starved;  // see DecodeArgs
+  uint64_t wait_ns;
   bool n_units32;   // the units of any lengths fit 31 bits
   PrefixPieces prefix;
 };
@@ -321,7 +327,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
     const int my = lane, half = my % (D / 64), sub = my / (D / 64);
     const uint64_t policy = policy_evict_last();
     int it = 0, item = 0, pre = 0;
-    bool ok = true;
+    bool ok = !(p.starved >> kWarps & 1);
     while (s.count > 0 && ok) {
       const Item i = item_of(p, s);
       if (i.x1 == i.x0) {  // the cut falls before its first tile
@@ -330,7 +336,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
       }
       // The item's queries, a row a lane.
       if (s.b < 0) {
-        if (pre > 0 && !warp_wait(pre_empty, (pre - 1) & 1)) break;
+        if (pre > 0 && !warp_wait(pre_empty, (pre - 1) & 1, p.wait_ns)) break;
         if (lane == 0) mbar_arrive_expect_tx(pre_full, i.rows * D * 2);
         __syncwarp();
         if (lane < i.rows)
@@ -339,9 +345,9 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
         ++pre;
       } else {
         if (lane == 0 && __ldg(p.lens + s.b) != i.len) atomicOr(&g_status, kStatusBadIndex);
-        if (item == 0 && pre > 0 && !warp_wait(pre_empty, (pre - 1) & 1)) break;
+        if (item == 0 && pre > 0 && !warp_wait(pre_empty, (pre - 1) & 1, p.wait_ns)) break;
         const int qi = item % q_slots;
-        if (item >= q_slots && !warp_wait(q_empty + qi, ((item / q_slots) & 1) ^ 1)) break;
+        if (item >= q_slots && !warp_wait(q_empty + qi, ((item / q_slots) & 1) ^ 1, p.wait_ns)) break;
         if (lane == 0) mbar_arrive_expect_tx(q_full + qi, i.rows * D * 2);
         __syncwarp();
         if (lane < i.rows)
@@ -360,7 +366,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
             atomicOr(&g_status, kStatusBadIndex);
           }
         }
-        if (it >= kStages && !warp_wait(empty + st, ((it / kStages) & 1) ^ 1)) {
+        if (it >= kStages && !warp_wait(empty + st, ((it / kStages) & 1) ^ 1, p.wait_ns)) {
           ok = false;
           break;
         }
@@ -376,18 +382,20 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
       advance(p, s, i.units);
     }
     // Copies still in flight land before the CTA's memory goes (bounded).
-    if (pre > 0) warp_wait(pre_full, (pre - 1) & 1);
+    if (pre > 0) warp_wait(pre_full, (pre - 1) & 1, p.wait_ns);
     for (int i = item < q_slots ? 0 : item - q_slots; i < item; ++i)
-      if (!warp_wait(q_full + i % q_slots, (i / q_slots) & 1)) break;
+      if (!warp_wait(q_full + i % q_slots, (i / q_slots) & 1, p.wait_ns)) break;
     for (int i = it < kStages ? 0 : it - kStages; i < it; ++i)
-      if (!warp_wait(full + i % kStages, (i / kStages) & 1)) break;
+      if (!warp_wait(full + i % kStages, (i / kStages) & 1, p.wait_ns)) break;
   } else {
     const int gid = lane >> 2, c = lane & 3;
     const uint32_t ring = smem_u32(smem);
     const int p0 = warp * 16;
     int it = 0, item = 0, pre = 0;
-    bool ok = true, cut_first = false;
-    while (s.count > 0 && ok) {
+    // Once a wait has run out no later one is taken.
+    bool ok = !(p.starved >> warp & 1), cut_first = false;
+    auto await = [&](uint64_t* bar, uint32_t parity) { return ok = ok && warp_wait(bar, parity, p.wait_ns); };
+    while (s.count > 0) {
       const Item i = item_of(p, s);
       const int len = i.len, head0 = i.head0, rows = i.rows;
       if (i.x1 == i.x0) {
@@ -398,7 +406,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
       // sequences, in a prefix).
       uint32_t qa[D / 16][4];
       const int qi = s.b < 0 ? 0 : item % q_slots;
-      if (!(s.b < 0 ? warp_wait(pre_full, pre & 1) : warp_wait(q_full + qi, (item / q_slots) & 1))) break;
+      await(s.b < 0 ? pre_full : q_full + qi, (s.b < 0 ? pre : item / q_slots) & 1);
 #pragma unroll
       for (int ks = 0; ks < D / 16; ++ks)
         ldsm_x4(smem_u32(qs) + (qi * q_rows + (lane & 15)) * (D * 2) + ks * 32 + (lane >> 4) * 16, qa[ks]);
@@ -408,10 +416,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
       float m_run[2] = {-INFINITY, -INFINITY}, l_run[2] = {0.f, 0.f};
       for (int x = i.x0; x < i.x1; ++x, ++it) {
         const int st = it % kStages;
-        if (!warp_wait(full + st, (it / kStages) & 1)) {
-          ok = false;
-          break;
-        }
+        if (!await(full + st, (it / kStages) & 1)) continue;
         const uint32_t kst = ring + st * 2 * L::kTileBytes, vst = kst + L::kTileBytes;
         const int ts = x * kTile + p0;
         if (ts < len) {
@@ -481,7 +486,6 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
         __syncwarp();
         if (lane == 0) mbar_arrive(empty + st);
       }
-      if (!ok) break;
       // The queries' place is free once their reads have come back, not once
       // they are issued: here every fragment is used (by the products, or, in a
       // warp whose slices all lay behind the end, by this).
@@ -492,7 +496,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
         asm volatile("" ::"r"(x) : "memory");
       }
       __syncwarp();
-      if (lane == 0) mbar_arrive(s.b < 0 ? pre_empty : q_empty + qi);
+      if (ok && lane == 0) mbar_arrive(s.b < 0 ? pre_empty : q_empty + qi);
       if (s.b < 0) ++pre;
       else ++item;
 
@@ -503,7 +507,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
         l_run[r] += __shfl_xor_sync(0xffffffffu, l_run[r], 2);
         if (c == 0) {
           ms[warp * 16 + gid + 8 * r] = m_run[r];
-          ls[warp * 16 + gid + 8 * r] = l_run[r];
+          ls[warp * 16 + gid + 8 * r] = ok ? l_run[r] : NAN;
         }
       }
       const bool whole = i.x0 == 0 && i.x1 == i.tiles;
@@ -792,6 +796,8 @@ cudaError_t launch_paged_decode(const PagedPool& pool, const CUtensorMap& kmap,
   p.len_limit = limit < (1 << 30) ? static_cast<int>(limit) : 1 << 30;
   p.box_rows = paged_decode_box_rows(pool.page_size);
   p.scale_log2 = a.scale_log2;
+  p.starved = a.starved;
+  p.wait_ns = a.wait_ns ? a.wait_ns : kWaitLimitNs;
   // With more query heads the warps' merge takes more rounds (128 sequences of
   // 8 heads a KV head behind a prefix: 116 us with 1, 111 with 2, 108.5 with 3).
   p.item_tiles = p.g > kMergeRows ? 3 : 1;

@@ -432,6 +432,21 @@ int dqg_shared_prefix_attention(const void *q, int64_t q_stride_seq, int64_t q_s
                                 const int32_t *kv_lens, float scale, void *out, void *workspace,
                                 uint64_t workspace_bytes, void *stream);
 
+/*
+ * Diagnostic for the bounded waits of dqg_paged_attention (prefix_len 0) and
+ * dqg_shared_prefix_attention: their decode kernel with warps that do nothing
+ * (starved, bits 0 to 3: a consumer warp that gives up before its first wait;
+ * bit 4: the copying warp), so that the other warps' waits give up after
+ * wait_ns (1 ms to 1 s). The kernels return, results that were given up are
+ * NaN, and where a wait ran out bit 0 of dqg_device_status is set. For tests.
+ */
+int dqg_debug_paged_starved(const void *q, int64_t q_stride_seq, int64_t q_stride_head, int64_t n_seqs,
+                            int64_t n_q_heads, const dqg_paged_kv *kv, const int32_t *prefix_table,
+                            int64_t prefix_pages, int64_t prefix_len, const int32_t *block_table,
+                            int64_t table_width, int64_t table_stride, const int32_t *kv_lens, float scale,
+                            void *out, void *workspace, uint64_t workspace_bytes, uint32_t starved,
+                            uint64_t wait_ns, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
