@@ -41,7 +41,7 @@ cudaError_t launch_paged_append(const PagedPool& pool, const AppendArgs& a, int 
 // result by the decode kernels. S == 0: no prefix.
 struct PrefixPieces {
   const float* o;     // [pair][kv head][S][D / 4][256] float4
-  const float* ml;    // [pair][kv head][S][2][256]: maximum (log2 units), sum
+  const float* ml;    // [pair][kv head][S][2][256]: reference of the weights (log2 units), sum
   int S, tq;          // pieces; sequences per 128-row tile
 };
 

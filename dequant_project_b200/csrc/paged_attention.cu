@@ -50,6 +50,11 @@ constexpr int kStages = 3;
 constexpr int kCtasPerSm = 2;
 constexpr int kQuerySlots = 4;         // items whose queries are held at most
 constexpr int kMergeRows = 4;          // query heads per round of the warps' merge
+// Weights are formed for the values' 16-bit type, relative to a reference 2^15
+// below the running maximum: of fp16's range (2^-24 to 2^16) all that lies above
+// 1 is used too, so that what a weight loses at the lower end is below 2^-40 of
+// the largest one. References are in log2 units, and with every piece its own.
+constexpr float kHeadroom = 15.f;
 
 struct Desc {    // an item that is joined later
   int b, hv;     // sequence, KV head and 16-row block of its query heads
@@ -63,7 +68,7 @@ struct Params {
   const int32_t* table;
   const int32_t* lens;
   float* part;   // [row][D]: two pieces of `rows` rows a CTA, then (behind a prefix) whole results
-  float* m;      // [row]: maximum (log2 units)
+  float* m;      // [row]: reference of the weights (log2 units)
   float* l;      // [row]: sum
   Desc* desc;    // [CTA]; behind a prefix [item], then [prefix item]
   const int32_t* pre_table;
@@ -455,7 +460,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
             const float m_new = fmaxf(m_run[r], mx);
             const float m_use = m_new == -INFINITY ? 0.f : m_new;
-            const float corr = exp2_approx(m_run[r] - m_use);
+            const float corr = exp2_approx(m_run[r] - m_use), ref = m_use - kHeadroom;
             l_run[r] *= corr;
 #pragma unroll
             for (int nb = 0; nb < D / 8; ++nb) {
@@ -464,8 +469,8 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
             }
 #pragma unroll
             for (int nb = 0; nb < 2; ++nb) {
-              pr[nb][2 * r] = exp2_approx(sc[nb][2 * r] - m_use);
-              pr[nb][2 * r + 1] = exp2_approx(sc[nb][2 * r + 1] - m_use);
+              pr[nb][2 * r] = exp2_approx(sc[nb][2 * r] - ref);
+              pr[nb][2 * r + 1] = exp2_approx(sc[nb][2 * r + 1] - ref);
               l_run[r] += pr[nb][2 * r] + pr[nb][2 * r + 1];
             }
             m_run[r] = m_new;
@@ -506,7 +511,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
         l_run[r] += __shfl_xor_sync(0xffffffffu, l_run[r], 1);
         l_run[r] += __shfl_xor_sync(0xffffffffu, l_run[r], 2);
         if (c == 0) {
-          ms[warp * 16 + gid + 8 * r] = m_run[r];
+          ms[warp * 16 + gid + 8 * r] = m_run[r] - kHeadroom;
           ls[warp * 16 + gid + 8 * r] = ok ? l_run[r] : NAN;
         }
       }

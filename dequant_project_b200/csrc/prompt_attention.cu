@@ -33,7 +33,7 @@
 // 128 P takes the place of S as it is formed) and O (fp32, D columns), so one tile's
 // softmax runs while the other's products do. O stays in tensor memory over
 // all blocks: the maximum that weights refer to is moved, and O rescaled, only
-// when it grows by more than 2^8, which bounds the weights by 2^8; the sums are
+// when it grows by more than 2^8, which bounds the weights; the sums are
 // fp32 and the division by them comes at the end. P is rounded to the values'
 // 16-bit type for the second product (the tensor cores take both operands in
 // one type); the sum is taken before the rounding.
@@ -66,7 +66,11 @@ namespace {
 constexpr int kBlock = 128;         // keys a block; rows a tile
 constexpr int kThreads = 384;       // 2 x 4 softmax warps; products, copies, 2 value warps
 constexpr int kMmaWarp = 8, kCopyWarp = 9, kValueWarp = 10, kValueWarps = 2;
-constexpr float kMaxGrowth = 8.f;   // log2 of the largest weight
+// Weights are relative to a reference kHeadroom below a maximum that the true one
+// exceeds by kMaxGrowth at most (log2 units): 2^15 at most, so that of fp16's
+// range (2^-24 to 2^16) what lies above 1 is used too, and what a weight loses at
+// the lower end is below 2^-32 of the largest one.
+constexpr float kMaxGrowth = 8.f, kHeadroom = 7.f;
 constexpr int kEarly = 96;          // keys whose weights are handed over first
 // An item's start and end, in keys' time (8192 tokens, 64/8 heads: 1019 us with
 // 128, 982 with 256, 982 with 512).
@@ -894,7 +898,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           l *= f;
           if (grow) m = m_new;
         }
-        const float ref = m == -INFINITY ? 0.f : m * p.scale_log2;
+        const float ref = m == -INFINITY ? 0.f : fmaf(m, p.scale_log2, -kHeadroom);
         const float2 ref2 = make_float2(-ref, -ref);
         float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
         // The products take the first kEarly weights while the rest is formed.
@@ -983,7 +987,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         } else {
           const int64_t slot = g.slot;
-          p.ml[slot * 512 + t * 128 + r] = n > 0 && m != -INFINITY ? m * p.scale_log2 : -INFINITY;
+          p.ml[slot * 512 + t * 128 + r] = n > 0 && m != -INFINITY ? fmaf(m, p.scale_log2, -kHeadroom) : -INFINITY;
           p.ml[slot * 512 + 256 + t * 128 + r] = l;
 #pragma unroll
           for (int q = 0; q < D / 32; ++q) {
