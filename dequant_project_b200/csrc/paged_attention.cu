@@ -54,6 +54,11 @@ constexpr int kMergeRows = 4;          // query heads per round of the warps' me
 // below the running maximum: of fp16's range (2^-24 to 2^16) all that lies above
 // 1 is used too, so that what a weight loses at the lower end is below 2^-40 of
 // the largest one. References are in log2 units, and with every piece its own.
+// (One rounding of a weight, to the type that the product's two operands share,
+// adds up to a quarter to the output's own error. Weights as a sum of two 16-bit
+// numbers and a second product left the output's alone: large batches took the
+// same 201 us, but short calls 12.9 us instead of 12.3, small prefixes 25.6
+// instead of 24.3.)
 constexpr float kHeadroom = 15.f;
 
 struct Desc {    // an item that is joined later
