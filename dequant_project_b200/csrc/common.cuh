@@ -14,7 +14,7 @@ namespace dqg {
 // the host reads it with dqg_device_status().
 enum : uint32_t {
   kStatusWaitTimeout = 1u << 0,   // an mbarrier wait ran past its time limit
-  kStatusBadIndex = 1u << 1,      // a page, slot, position or length out of range was left out
+  kStatusBadIndex = 1u << 1,      // a page, slot, position, length or start out of range was left out
 };
 
 // One status word per translation unit that includes this header (internal

@@ -211,7 +211,10 @@ __device__ __forceinline__ Seq load_seq(const Params& p, int b) {
     s.ql = __ldg(p.q_starts + b + 1) - s.q0;
     s.kv = clamped_len(p.lens, b, p.len_limit);
     // Starts out of order or range: no rows.
-    if (s.q0 < 0 || s.ql < 0 || s.q0 > p.T || s.ql > p.T - s.q0) s.ql = 0;
+    if (s.q0 < 0 || s.ql < 0 || s.q0 > p.T || s.ql > p.T - s.q0) {
+      s.ql = 0;
+      atomicOr(&g_status, kStatusBadIndex);
+    }
   }
   s.pairs = (s.ql + 2 * p.tq - 1) / (2 * p.tq);
   return s;
@@ -1183,7 +1186,8 @@ cudaError_t launch_prompt(const PagedPool& pool, const CUtensorMap& qmap, const 
   p.len_limit = limit < (1 << 30) ? static_cast<int>(limit) : 1 << 30;
   p.box_rows = prompt_box_rows(pool.page_size);
   p.causal = a.causal;
-  p.n_units32 = (static_cast<double>(a.T) / (2 * p.tq) + a.B) * (static_cast<double>(p.len_limit) + kItemKeys) *
+  // (Each sequence for itself: starts that are out of order may count rows twice.)
+  p.n_units32 = (static_cast<double>(a.T) / (2 * p.tq) + 1.0) * a.B * (static_cast<double>(p.len_limit) + kItemKeys) *
                     pool.n_kv_heads < 2147483648.0;
   p.scale_log2 = a.scale_log2;
   p.prefix_len = a.prefix_len;

@@ -346,9 +346,9 @@ int dqg_silu_mul(const void *gate_up, void *out, int64_t M, int64_t I,
  * Strides are in elements, the same for both pools, multiples of 8, with
  * head_dim contiguous; head_dim is 64 or 128, page_size 16, 32, 64, 128 or
  * 256. The operators below take queries, keys, values and outputs of the
- * pools' type. A page index, slot, position or length out of range is left
- * out (read as zeros, not written, held to the table's width) and sets bit 1
- * of dqg_device_status.
+ * pools' type. A page index, slot, position, length or row start out of range
+ * or order is left out (read as zeros, not written, held to the table's width)
+ * and sets bit 1 of dqg_device_status.
  */
 enum { DQG_FP16 = 0, DQG_BF16 = 1 };
 typedef struct dqg_paged_kv {
@@ -406,7 +406,8 @@ int dqg_paged_attention(const void *q, int64_t q_stride_seq, int64_t q_stride_he
  * not see, behind the sequence's end or hidden by the mask, does not matter to it.
  * Heads, strides, table, lengths on the device, scale and workspace
  * (dqg_prompt_attention_workspace(D) bytes) as dqg_paged_attention. Rows of q
- * outside every sequence leave their rows of out unwritten.
+ * outside every sequence, or of one whose starts are out of order or range,
+ * leave their rows of out unwritten.
  */
 int dqg_prompt_attention_workspace(int64_t head_dim, uint64_t *bytes);
 int dqg_prompt_attention(const void *q, int64_t q_stride_row, int64_t q_stride_head, int64_t T,
