@@ -8,6 +8,7 @@
 // copy of the library, the one that _native.py loaded.
 #include <Python.h>
 #include <ATen/ATen.h>
+#include <ATen/core/grad_mode.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
@@ -55,6 +56,15 @@ const at::Tensor& tensor(PyObject* o, const char* name) {
 
 const char* type_name(at::ScalarType t) { return t == at::kHalf ? "float16" : "bfloat16"; }
 
+// The operators have no backward pass: what autograd would record is refused
+// instead of left out.
+void forward_only(std::initializer_list<const at::Tensor*> inputs) {
+  if (!at::GradMode::is_enabled()) return;
+  for (const at::Tensor* t : inputs)
+    if (t->requires_grad())
+      reject("the paged operators are forward only: an input requires a gradient (call them under torch.no_grad())");
+}
+
 struct Pools {
   dqg_paged_kv kv;
   at::ScalarType type;
@@ -94,7 +104,8 @@ void ints(const Pools& p, const at::Tensor& t, const char* name, at::ScalarType 
 // A block table's row length and stride.
 int64_t row_stride(const at::Tensor& table) { return table.size(0) > 1 ? table.stride(0) : table.size(1); }
 
-void query(const Pools& p, const at::Tensor& q) {
+void query(const Pools& p, const at::Tensor& q, PyObject* k, PyObject* v) {
+  forward_only({&q, &THPVariable_Unpack(k), &THPVariable_Unpack(v)});
   same(p, q, "q");
   if (q.dim() != 3 || q.size(2) != p.kv.head_dim || q.stride(2) != 1)
     reject("q must be [rows, heads, %d] with the head dimension contiguous", static_cast<int>(p.kv.head_dim));
@@ -148,7 +159,9 @@ at::Tensor append(PyObject* const* a, Py_ssize_t n) {
   const at::Tensor &qkv = tensor(a[0], "qkv"), &cos = tensor(a[1], "cos"), &sin = tensor(a[2], "sin");
   const at::Tensor &positions = tensor(a[3], "positions"), &slots = tensor(a[4], "slots");
   const Pools p = pools(tensor(a[5], "k_pages"), tensor(a[6], "v_pages"));
+  const at::Tensor &k = tensor(a[5], "k_pages"), &v = tensor(a[6], "v_pages");
   const int64_t hq = integer(a[7]), d = p.kv.head_dim;
+  forward_only({&qkv, &cos, &sin, &k, &v});
   same(p, qkv, "qkv");
   const int64_t width = (hq + 2 * p.kv.n_kv_heads) * d;
   if (qkv.dim() != 2 || qkv.size(1) != width || qkv.stride(1) != 1)
@@ -165,6 +178,7 @@ at::Tensor append(PyObject* const* a, Py_ssize_t n) {
   for (int i = 0; i < 2; ++i) {
     if (a[9 + i] == Py_None) continue;
     const at::Tensor& w = tensor(a[9 + i], names[i]);
+    forward_only({&w});
     same(p, w, names[i]);
     if (w.dim() != 1 || w.size(0) != d || w.stride(0) != 1)
       reject("%s must hold %lld contiguous weights", names[i], static_cast<long long>(d));
@@ -179,6 +193,9 @@ at::Tensor append(PyObject* const* a, Py_ssize_t n) {
                  sin.data_ptr<float>(), cos.size(0), 2 * cos.size(1), interleaved, positions.data_ptr<int64_t>(),
                  slots.data_ptr<int64_t>(), norms[0], norms[1], static_cast<float>(eps), &p.kv, q.data_ptr(),
                  stream_of(p.device)));
+  // Written in place: what autograd has saved of the pages is out of date.
+  for (const at::Tensor* x : {&k, &v})
+    if (!x->is_inference()) x->unsafeGetTensorImpl()->bump_version();
   return q;
 }
 
@@ -187,7 +204,7 @@ at::Tensor decode(PyObject* const* a, Py_ssize_t n) {
   arguments(n, 7);
   const at::Tensor &q = tensor(a[0], "q"), &table = tensor(a[3], "block_table"), &lens = tensor(a[4], "kv_lens");
   const Pools p = pools(tensor(a[1], "k_pages"), tensor(a[2], "v_pages"));
-  query(p, q);
+  query(p, q, a[1], a[2]);
   const int64_t b = q.size(0), hq = q.size(1), d = q.size(2);
   ints(p, table, "block_table", at::kInt, 2, b);
   ints(p, lens, "kv_lens", at::kInt, 1, b);
@@ -209,7 +226,7 @@ at::Tensor prompt(PyObject* const* a, Py_ssize_t n) {
   const at::Tensor &q = tensor(a[0], "q"), &table = tensor(a[3], "block_table");
   const at::Tensor &starts = tensor(a[4], "q_starts"), &lens = tensor(a[5], "kv_lens");
   const Pools p = pools(tensor(a[1], "k_pages"), tensor(a[2], "v_pages"));
-  query(p, q);
+  query(p, q, a[1], a[2]);
   const int64_t t = q.size(0), hq = q.size(1), d = q.size(2);
   ints(p, lens, "kv_lens", at::kInt, 1, -1);
   const int64_t b = lens.size(0);
@@ -236,7 +253,7 @@ at::Tensor prefix(PyObject* const* a, Py_ssize_t n) {
   const at::Tensor &table = tensor(a[5], "block_table"), &lens = tensor(a[6], "kv_lens");
   const Pools p = pools(tensor(a[1], "k_pages"), tensor(a[2], "v_pages"));
   const int64_t len = integer(a[4]);
-  query(p, q);
+  query(p, q, a[1], a[2]);
   const int64_t b = q.size(0), hq = q.size(1), d = q.size(2);
   ints(p, pre, "prefix_table", at::kInt, 1, -1);
   ints(p, table, "block_table", at::kInt, 2, b);

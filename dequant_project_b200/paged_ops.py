@@ -8,6 +8,10 @@ sequence, a row of page numbers in ``block_table``: position t lies in page
 strided views (of one allocation for keys and values, say) as long as both have
 the same strides and D is contiguous.
 
+Forward only: an input that requires a gradient is refused while gradients are
+recorded (``torch.no_grad()`` allows it). ``rope_paged_append`` writes the pages
+in place.
+
 CUDA tensors go through the sm_100a kernels of libdequant_b200.so on torch's
 current stream (checked and called by the native binding,
 ``binding/paged_binding.cpp``); if either is missing these calls raise. CPU tensors take
@@ -46,6 +50,13 @@ def _binding():
             "dqg_shared_prefix_workspace", "dqg_shared_prefix_attention")))
         _bound = _paged_binding
     return _bound
+
+
+def _forward_only(*inputs) -> None:
+    """The binding's refusal, for CPU tensors."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in inputs):
+        raise RuntimeError("the paged operators are forward only: an input requires a gradient "
+                           "(call them under torch.no_grad())")
 
 
 # ------------------------------------------------------------------- append
@@ -103,6 +114,7 @@ def rope_paged_append(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, p
     x * rsqrt(mean(x^2) + eps) * w per head before the rotation. fp32 math, one
     rounding."""
     if not qkv.is_cuda:
+        _forward_only(qkv, cos, sin, k_pages, v_pages, q_norm, k_norm)
         t = qkv.shape[0]
         hkv, page, d = k_pages.shape[1:]
         x = qkv.float().view(t, n_q_heads + 2 * hkv, d)
@@ -170,6 +182,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     overlap."""
     if q.is_cuda:
         return _binding().paged_attention(q, k_pages, v_pages, block_table, kv_lens, scale, workspace)
+    _forward_only(q, k_pages, v_pages)
     b, _, d = q.shape
     scale = 1.0 / math.sqrt(d) if scale is None else scale
     out = [_cpu_attention(q[i:i + 1].float(), _rows(k_pages, block_table[i], int(kv_lens[i])),
@@ -200,6 +213,7 @@ def prompt_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tens
     if q.is_cuda:
         return _binding().prompt_attention(q, k_pages, v_pages, block_table, q_starts, kv_lens, causal, scale,
                                            workspace)
+    _forward_only(q, k_pages, v_pages)
     scale = 1.0 / math.sqrt(q.shape[2]) if scale is None else scale
     out = torch.zeros_like(q)
     for i in range(kv_lens.shape[0]):
@@ -235,6 +249,7 @@ def shared_prefix_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: tor
     if q.is_cuda:
         return _binding().shared_prefix_attention(q, k_pages, v_pages, prefix_table, prefix_len, block_table,
                                                   kv_lens, scale, workspace)
+    _forward_only(q, k_pages, v_pages)
     b, _, d = q.shape
     scale = 1.0 / math.sqrt(d) if scale is None else scale
     out = []
