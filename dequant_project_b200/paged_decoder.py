@@ -154,12 +154,17 @@ class PagedDecoder:
             raise ValueError(f"a prefix holds whole pages of {self.page} and leaves room in "
                              f"{self.max_positions} positions, got {n}")
         pages = self.pages.take(n // self.page)
-        self._prompts([tokens], [pages], [0])
+        try:
+            self._prompts([tokens], [pages], [0])
+        except BaseException:
+            self.pages.give(pages)
+            raise
         self.prefix_pages, self.prefix_len = pages, n
 
     def add(self, prompts: list[torch.Tensor]) -> tuple[list[int], torch.Tensor]:
         """Run new sequences' prompts (int64, at least one token each) in one
-        packed pass. Returns their ids and their last tokens' logits."""
+        packed pass. Returns their ids and their last tokens' logits. A pass
+        that raises adds nothing."""
         for p in prompts:
             if p.dim() != 1 or p.shape[0] < 1 or self.prefix_len + p.shape[0] > self.max_positions:
                 raise ValueError(f"a prompt holds 1 to {self.max_positions - self.prefix_len} tokens")
@@ -167,11 +172,11 @@ class PagedDecoder:
         try:
             for p in prompts:
                 taken.append(self.pages.take(-(-int(p.shape[0]) // self.page)))
-        except RuntimeError:
-            for t in taken:
+            logits = self._prompts(prompts, [self.prefix_pages + t for t in taken], [self.prefix_len] * len(prompts))
+        except BaseException:
+            for t in reversed(taken):
                 self.pages.give(t)
             raise
-        logits = self._prompts(prompts, [self.prefix_pages + t for t in taken], [self.prefix_len] * len(prompts))
         ids = []
         for p, t in zip(prompts, taken):
             self.seqs[self._next] = {"pages": t, "len": int(p.shape[0])}
@@ -181,7 +186,8 @@ class PagedDecoder:
 
     def step(self, ids: list[int], tokens: torch.Tensor) -> torch.Tensor:
         """One token of each of the sequences ``ids`` (int64 [len(ids)]): its
-        logits [len(ids), vocab]."""
+        logits [len(ids), vocab]. A step that raises leaves the sequences as
+        they were, so that it can be taken again."""
         if tokens.shape != (len(ids),) or len(set(ids)) != len(ids):
             raise ValueError("step takes one token for each of different sequences")
         seqs = [self.seqs[i] for i in ids]
@@ -189,13 +195,24 @@ class PagedDecoder:
             if self.prefix_len + s["len"] >= self.max_positions:
                 raise ValueError(f"a sequence has reached {self.max_positions} positions")
         short = [s for s in seqs if s["len"] == len(s["pages"]) * self.page]
-        for s, page in zip(short, self.pages.take(len(short))):
+        more = self.pages.take(len(short))
+        for s, page in zip(short, more):
             s["pages"].append(page)
-        positions = self._ints([self.prefix_len + s["len"] for s in seqs], torch.int64)
-        slots = self._ints([self._slots(s["pages"], s["len"], 1)[0] for s in seqs], torch.int64)
+        try:
+            logits = self._step(seqs, tokens)
+        except BaseException:
+            for s in short:
+                s["pages"].pop()
+            self.pages.give(more)
+            raise
         for s in seqs:
             s["len"] += 1
-        table, lens = self._table([s["pages"] for s in seqs]), self._ints([s["len"] for s in seqs])
+        return logits
+
+    def _step(self, seqs: list[dict], tokens: torch.Tensor) -> torch.Tensor:
+        positions = self._ints([self.prefix_len + s["len"] for s in seqs], torch.int64)
+        slots = self._ints([self._slots(s["pages"], s["len"], 1)[0] for s in seqs], torch.int64)
+        table, lens = self._table([s["pages"] for s in seqs]), self._ints([s["len"] + 1 for s in seqs])
         if self.prefix_len:
             prefix = self._ints(self.prefix_pages)
 
@@ -213,12 +230,16 @@ class PagedDecoder:
 
     def generate(self, prompts: list[torch.Tensor], steps: int) -> torch.Tensor:
         """Greedy: the prompts' next ``steps`` tokens, [len(prompts), steps]."""
+        if steps < 1:
+            return torch.empty((len(prompts), 0), dtype=torch.int64, device=self.dec.device)
         ids, logits = self.add(prompts)
-        out = [logits.argmax(-1)]
-        while len(out) < steps:
-            out.append(self.step(ids, out[-1]).argmax(-1))
-        for i in ids:
-            self.free(i)
+        try:
+            out = [logits.argmax(-1)]
+            while len(out) < steps:
+                out.append(self.step(ids, out[-1]).argmax(-1))
+        finally:
+            for i in ids:
+                self.free(i)
         return torch.stack(out, 1)
 
 
