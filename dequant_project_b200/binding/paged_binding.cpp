@@ -320,4 +320,12 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_paged_binding", nullptr, -1, meth
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__paged_binding(void) { return PyModule_Create(&module); }
+// `built_for`: the torch that this was compiled against, whose layouts it knows.
+PyMODINIT_FUNC PyInit__paged_binding(void) {
+  PyObject* m = PyModule_Create(&module);
+  if (m != nullptr && PyModule_AddStringConstant(m, "built_for", DQG_BUILT_FOR) != 0) {
+    Py_DECREF(m);
+    return nullptr;
+  }
+  return m;
+}

@@ -42,8 +42,11 @@ def _binding():
         try:
             from dequant_project_b200 import _paged_binding
         except ImportError as exc:
-            raise ImportError("_paged_binding.so is not built. Build it once with:\n"
-                              "    python -m dequant_project_b200.build") from exc
+            raise ImportError(f"_paged_binding.so is not built, or not for this torch and Python ({exc}). "
+                              "Build it once with:\n    python -m dequant_project_b200.build") from exc
+        if _paged_binding.built_for != torch.__version__:
+            raise ImportError(f"_paged_binding.so is built for torch {_paged_binding.built_for}, this is "
+                              f"{torch.__version__}. Build it again with:\n    python -m dequant_project_b200.build")
         _paged_binding.bind(*(ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in (
             "dqg_last_error", "dqg_rope_paged_append", "dqg_paged_attention_workspace",
             "dqg_paged_attention", "dqg_prompt_attention_workspace", "dqg_prompt_attention",
