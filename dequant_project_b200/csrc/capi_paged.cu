@@ -358,7 +358,8 @@ int dqg_shared_prefix_workspace(int64_t n_seqs, int64_t n_q_heads, int64_t n_kv_
   if ((rc = current(&dev, &sms)) != DQG_OK) return rc;
   const bool pieces = prefix_len > 0 && n_seqs > 0 &&
                       !dqg::prefix_streamed(static_cast<int>(n_seqs), static_cast<int>(n_q_heads),
-                                            static_cast<int>(n_kv_heads));
+                                            static_cast<int>(n_kv_heads), static_cast<int>(head_dim),
+                                            static_cast<int>(prefix_len));
   *bytes = dqg::paged_decode_workspace(static_cast<int>(n_seqs), static_cast<int>(n_q_heads),
                                        static_cast<int>(n_kv_heads), static_cast<int>(head_dim),
                                        static_cast<int>(prefix_len), sms);
@@ -406,7 +407,8 @@ int shared_prefix(const void* q, int64_t q_stride_seq, int64_t q_stride_head, in
   d.prefix_len = static_cast<int>(prefix_len);
   d.prefix_table = prefix_table;
   CUtensorMap qmap, kmap, vmap;
-  if (prefix_len > 0 && !dqg::prefix_streamed(static_cast<int>(n_seqs), static_cast<int>(n_q_heads), pool.n_kv_heads)) {
+  if (prefix_len > 0 && !dqg::prefix_streamed(static_cast<int>(n_seqs), static_cast<int>(n_q_heads), pool.n_kv_heads,
+                                              pool.D, static_cast<int>(prefix_len))) {
     dqg::PromptArgs a;
     std::memset(&a, 0, sizeof(a));
     a.table = prefix_table;

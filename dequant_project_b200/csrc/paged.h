@@ -65,7 +65,7 @@ struct DecodeArgs {
 size_t paged_decode_workspace(int B, int hq, int n_kv_heads, int D, int prefix_len, int num_sms);
 // Whether the decode kernel streams a prefix itself (else the prompt kernel
 // takes it, and DecodeArgs::prefix its pieces).
-bool prefix_streamed(int n_seqs, int hq, int n_kv_heads);
+bool prefix_streamed(int n_seqs, int hq, int n_kv_heads, int D, int prefix_len);
 cudaError_t launch_paged_decode(const PagedPool& pool, const CUtensorMap& kmap,
                                 const CUtensorMap& vmap, const DecodeArgs& a, int num_sms,
                                 cudaStream_t stream);

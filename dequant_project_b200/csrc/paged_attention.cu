@@ -26,8 +26,8 @@
 // items without data and makes their results NaN, so that the barriers among
 // the warps are always met and every item is described to the second kernel.
 //
-// A prefix whose rows (sequences times query heads of a KV head) fit two 16-row
-// tiles is streamed by this kernel itself, as items of its own ahead of the
+// A prefix whose rows (sequences times query heads of a KV head) fit one or two
+// 16-row tiles is streamed by this kernel itself, as items of its own ahead of the
 // sequences' (prefix_streamed below); one with more rows is left to the prompt
 // kernel, which reads it once for 256 rows.
 //
@@ -738,13 +738,13 @@ struct Scratch {
   size_t rows, descs;
   int per_piece, pre_items, pre_seqs;
 };
-Scratch scratch_of(int B, int hq, int n_kv_heads, int prefix_len, int num_sms) {
+Scratch scratch_of(int B, int hq, int n_kv_heads, int D, int prefix_len, int num_sms) {
   const int g = hq / n_kv_heads, g16 = g < 16 ? g : 16;
   const size_t items = static_cast<size_t>(B) * n_kv_heads * ((g + 15) / 16);
   const size_t ctas = static_cast<size_t>(kCtasPerSm) * num_sms;
   Scratch s{2 * ctas * g16, ctas, g16, 0, 1};
   if (prefix_len > 0) {
-    if (prefix_streamed(B, hq, n_kv_heads)) {
+    if (prefix_streamed(B, hq, n_kv_heads, D, prefix_len)) {
       s.pre_seqs = 16 / g;
       s.pre_items = (B + s.pre_seqs - 1) / s.pre_seqs * n_kv_heads;
       s.per_piece = 16;
@@ -757,16 +757,23 @@ Scratch scratch_of(int B, int hq, int n_kv_heads, int prefix_len, int num_sms) {
 }
 }  // namespace
 
-// At most two 16-row tiles: streaming the prefix once or twice beats the prompt
-// kernel's start and its mostly empty 128-row tiles (16 sequences, 32 heads,
-// 2000 positions: 23 us against 35).
-bool prefix_streamed(int n_seqs, int hq, int n_kv_heads) {
+// One 16-row tile, or two of a prefix of up to 96 MiB: streaming the prefix once
+// or twice beats the prompt kernel's start and its mostly empty 128-row tiles,
+// until the second reading costs more. Streamed and by the prompt kernel, 32 query
+// and KV heads: 16 sequences behind 2000 positions 24.2 and 34.5 us, behind 16000
+// 58.4 and 71.1; 32 sequences (two tiles) behind 2000 (33 MB) 35.4 and 42.7, but
+// behind 16000 (262 MB) 98.6 and 81.9. 64 and 8 heads, 4 sequences (two tiles):
+// behind 2000 12.8 and 15.5, behind 16000 (66 MB) 26.6 and 30.7; four tiles behind
+// 16000 39.1 and 31.3.
+bool prefix_streamed(int n_seqs, int hq, int n_kv_heads, int D, int prefix_len) {
   const int g = hq / n_kv_heads;
-  return g <= 16 && n_seqs <= 2 * (16 / g);
+  if (g > 16) return false;
+  const int64_t bytes = static_cast<int64_t>(prefix_len) * n_kv_heads * D * 4;
+  return n_seqs <= (bytes <= (int64_t(96) << 20) ? 2 : 1) * (16 / g);
 }
 
 size_t paged_decode_workspace(int B, int hq, int n_kv_heads, int D, int prefix_len, int num_sms) {
-  const Scratch s = scratch_of(B, hq, n_kv_heads, prefix_len, num_sms);
+  const Scratch s = scratch_of(B, hq, n_kv_heads, D, prefix_len, num_sms);
   // Descriptions first (16 bytes each), then the rows.
   return (s.descs * sizeof(Desc) + s.rows * (D + 2) * 4 + 255) / 256 * 256;
 }
@@ -774,7 +781,7 @@ size_t paged_decode_workspace(int B, int hq, int n_kv_heads, int D, int prefix_l
 cudaError_t launch_paged_decode(const PagedPool& pool, const CUtensorMap& kmap,
                                 const CUtensorMap& vmap, const DecodeArgs& a, int num_sms,
                                 cudaStream_t stream) {
-  const Scratch s = scratch_of(a.B, a.hq, pool.n_kv_heads, a.prefix_len, num_sms);
+  const Scratch s = scratch_of(a.B, a.hq, pool.n_kv_heads, pool.D, a.prefix_len, num_sms);
   Params p;
   p.q = a.q;
   p.out = a.out;
@@ -808,8 +815,11 @@ cudaError_t launch_paged_decode(const PagedPool& pool, const CUtensorMap& kmap,
   p.scale_log2 = a.scale_log2;
   p.starved = a.starved;
   p.wait_ns = a.wait_ns ? a.wait_ns : kWaitLimitNs;
-  // With more query heads the warps' merge takes more rounds (128 sequences of
-  // 8 heads a KV head behind a prefix: 116 us with 1, 111 with 2, 108.5 with 3).
+  // With more query heads the warps' merge takes more rounds: 128 sequences of 8
+  // heads a KV head behind a prefix 116 us with 1, 111 with 2, 108.5 with 3; 32 of
+  // 16 heads, 4000 positions, 22.1 with 1, 21.2 with 3; 64 of 8 heads, 900 to 16000
+  // positions, 202.1 and 201.6. (One the other way: 128 of 8 heads, 700 positions,
+  // 18.3 and 19.2. With one head a KV head both within 2 %.)
   p.item_tiles = p.g > kMergeRows ? 3 : 1;
   p.n_units32 = static_cast<double>(a.B) * p.hkv * p.nrb * (p.len_limit / kTile + 2 + p.item_tiles) +
                     static_cast<double>(p.pre_items) * (p.pre_tiles + p.item_tiles) < 2147483648.0;
