@@ -143,6 +143,15 @@ class PagedDecoder:
         tokens = torch.cat([p.to(self.dec.device) for p in prompts])
         return self._forward(tokens, positions, slots, attend, self._ints([b - 1 for b in bounds[1:]], torch.int64))
 
+    def _check_tokens(self, tokens: torch.Tensor) -> None:
+        """Tokens on the host are looked at: one outside the vocabulary would be
+        another token's row (negative) or a fault on the GPU. (Those on the GPU
+        come from logits, and looking at them would wait for it.)"""
+        if not tokens.is_cuda and tokens.numel():
+            lo, hi = int(tokens.min()), int(tokens.max())
+            if lo < 0 or hi >= self.dec.cfg.vocab:
+                raise ValueError(f"tokens must be in [0, {self.dec.cfg.vocab}), got {lo if lo < 0 else hi}")
+
     # ------------------------------------------------------------- the calls
     def set_prefix(self, tokens: torch.Tensor) -> None:
         """Cache ``tokens`` once as the beginning of every sequence added from
@@ -153,6 +162,7 @@ class PagedDecoder:
         if n < 1 or n % self.page or n >= self.max_positions:
             raise ValueError(f"a prefix holds whole pages of {self.page} and leaves room in "
                              f"{self.max_positions} positions, got {n}")
+        self._check_tokens(tokens)
         pages = self.pages.take(n // self.page)
         try:
             self._prompts([tokens], [pages], [0])
@@ -168,6 +178,7 @@ class PagedDecoder:
         for p in prompts:
             if p.dim() != 1 or p.shape[0] < 1 or self.prefix_len + p.shape[0] > self.max_positions:
                 raise ValueError(f"a prompt holds 1 to {self.max_positions - self.prefix_len} tokens")
+            self._check_tokens(p)
         taken: list[list[int]] = []
         try:
             for p in prompts:
@@ -190,6 +201,7 @@ class PagedDecoder:
         they were, so that it can be taken again."""
         if tokens.shape != (len(ids),) or len(set(ids)) != len(ids):
             raise ValueError("step takes one token for each of different sequences")
+        self._check_tokens(tokens)
         seqs = [self.seqs[i] for i in ids]
         for s in seqs:
             if self.prefix_len + s["len"] >= self.max_positions:

@@ -79,3 +79,16 @@ def test_generate():
     assert len(serve.pages.free) == 3 and not serve.seqs
     assert serve.generate(prompts_of(3, 2), 0).shape == (2, 0)
     assert len(serve.pages.free) == 3 and not serve.seqs
+
+
+@pytest.mark.parametrize("bad", [-1, TINY.vocab])
+def test_tokens_outside_the_vocabulary(bad):
+    serve, _ = make()
+    tok = torch.tensor([3, bad, 5, 6, 7, 8, 9, 10])
+    for call in (lambda: serve.set_prefix(tok), lambda: serve.add([tok[:1], tok])):
+        with pytest.raises(ValueError, match=f"tokens must be in .*, got {bad}"):
+            call()
+    ids, _ = serve.add([tok[:1]])
+    with pytest.raises(ValueError, match=f"got {bad}"):
+        serve.step(ids, tok[1:2])
+    assert serve.seqs[ids[0]]["len"] == 1 and len(serve.pages.free) == 11
