@@ -17,8 +17,9 @@
 // one lane and share a table entry; interleaved pairs lie in one lane anyway.
 // A warp takes a few heads of one token, whose table entries stay in
 // registers; the sum of squares is one shuffle reduction. What it measured
-// (B200, 8192 tokens of 64 + 2 x 8 heads of 128, bf16, norms): 59 us, 5.7 TB/s
-// of the 6.4 that a copy reaches. Registers and stores decide: 128 registers
+// (B200, 8192 tokens of 64 + 2 x 8 heads of 128, bf16, norms): 62.5 us a call,
+// 5.4 TB/s of the 6.4 that a copy reaches (58.5 us and 5.8 replayed from a graph,
+// which the following figures are). Registers and stores decide: 128 registers
 // (two blocks of 256 an SM) 79 us, 80 (three) 69; with stores that do not stay
 // in the L2 cache 62, in blocks of 128 threads 59. Runs of four values instead
 // of eight (more, narrower accesses) 84 us; one head a lane group at a time 84.

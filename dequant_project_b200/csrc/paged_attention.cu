@@ -5,7 +5,10 @@
 //   o[b, h] = softmax(scale q[b, h] . K_b[:, h / g]^T) V_b[:, h / g]
 //
 // over the lens[b] positions that sequence b's pages hold; zero where there is
-// none. Every key and value row is read once, so HBM bounds it.
+// none. Every key and value row is read once for every 16 query heads of its KV
+// head (8 times at most, by CTAs that share the L2 cache), so HBM bounds it up to
+// 16: 32 sequences of 4000 positions and one KV head take 21 us with 16 query
+// heads, 28 with 32, 74 with 128 (65 MB, 10 us at the copy rate).
 //
 // Work is counted in tiles of 64 positions, sequence by sequence and KV head
 // by KV head, and cut into equal shares, one per CTA (two CTAs per SM), so that
@@ -31,11 +34,13 @@
 // sequences' (prefix_streamed below); one with more rows is left to the prompt
 // kernel, which reads it once for 256 rows.
 //
-// Measured (B200): 64 sequences of 900 to 16000 positions, 64 query and 8 KV
-// heads, bf16, 1.25 GB: 200 us, 6.27 TB/s, 0.97 of the rate that a copy
-// reaches; HBM bounds it. Short calls are bound by latency: one sequence of 2049
-// positions, 32 heads (33.5 MB): 11.5 us, about 4 of them before the first tile
-// has come (shares, table, copies), 4.5 streaming, 3 for the second kernel.
+// Measured (B200, a stream of calls whose inputs alternate between three sets):
+// 64 sequences of 900 to 16000 positions, 64 query and 8 KV heads, bf16, 1.25 GB:
+// 206 us, 6.08 TB/s, 0.94 of the rate that a copy reaches (both kernels; the first
+// alone 200 us, 6.27); HBM bounds it. Short calls are bound by latency: one
+// sequence of 2049 positions, 32 heads (33.5 MB): 13 us (12.4 replayed from a
+// graph), about 4 of them before the first tile has come (shares, table, copies),
+// 4.5 streaming, 3 for the second kernel.
 #include <cstdint>
 
 #include "paged.cuh"

@@ -38,9 +38,12 @@
 // 16-bit type for the second product (the tensor cores take both operands in
 // one type); the sum is taken before the rounding.
 //
-// Measured (B200, bf16, causal): 8192 tokens, 64 query and 8 KV heads of 128:
-// 965 us, 1.14 PFLOP/s, 0.67 of a cuBLAS product's burst rate; fp16, 2048
-// tokens, 32 heads: 52 us. What bounds it: a block pair (256 rows, 128 keys)
+// Measured (B200, a stream of calls whose inputs alternate between three sets):
+// bf16, causal, 8192 tokens, 64 query and 8 KV heads of 128: 1005 us, 1.09
+// PFLOP/s, 0.64 of a cuBLAS product's burst rate and 0.78 of its sustained one (the
+// power cap holds the clock at 1.55 GHz; one launch alone, at 1.62, takes 887);
+// fp16, 2048 tokens, 32 heads: 60 us (54 where the inputs stay in the L2 cache).
+// What bounds it: a block pair (256 rows, 128 keys)
 // takes 3220 cycles where its products take 2048 on the tensor cores and its
 // exponentials 2048 on their unit. A tile's chain is its softmax, 1980 cycles
 // (490 until its scores are read, 1420 for the weights at 11 cycles each where
@@ -48,14 +51,16 @@
 // there (products of the late weights and of the next block, 768, and the
 // signals between the warps); the other tile runs between, but not for free. An
 // item's start and end cost about 3 us more. Tried and slower (8192 tokens, 989
-// us then): every fourth weight by a polynomial on the fp32 pipe (1062: a lone
+// us on that GPU): every fourth weight by a polynomial on the fp32 pipe (1062: a lone
 // warp is bound by issue, not by the unit), weights formed before the block's
 // maximum is known (1012), two threads a row (1166), blocks of 64 keys with the
 // scores one block ahead (1114: a product of 64 columns reads its operands at
 // 2/3 of the rate, and its one issuing thread becomes the bound), a product
 // warp for each tile (1182). With D = 64 the products are half as long and P has
-// columns of its own, so the softmax alone bounds it: 13 packed prompts, 6858
-// tokens, 32 and 8 heads: 104 us (115 with P in the place of S).
+// columns of its own, so the softmax alone bounds it (in a long prompt the
+// exponential unit is busy 0.74 of the time, the tensor cores 0.37): 13 packed
+// prompts, 6858 tokens, 32 and 8 heads: 107 us, 103 on warm inputs (115 with P in
+// the place of S).
 #include <cstdint>
 
 #include "paged.cuh"
@@ -627,206 +632,203 @@ __global__ void __launch_bounds__(kThreads, 1)
   // Registers: a softmax thread holds a row of 128 scores. 384 x 168 at
   // launch = 256 x 216 + 128 x 72.
   if (warp >= 8) {
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
-  if (warp == kCopyWarp) {
-    // ---- copies: queries per segment, then key and value blocks in turn.
-    Walk walk;
-    walk.begin(p);
-    Segment g;
-    const int per = p.box_rows, boxes = kBlock / per * (D / 64);
-    const int half = lane % (D / 64), sub = lane / (D / 64);
-    int seg = 0, pos = 0, checks = 0;
-    bool ok = true;
-    while (ok) {
-      int b = 0;
-      const bool more = walk.next(p, g, b);
-      const int sg = seg % kSegs;
-      if (seg >= kSegs && !warp_wait(seg_empty + sg, ((seg / kSegs) & 1) ^ 1)) break;
-      g.from = max(0, p.causal ? g.lim0 : g.kv) & ~3;
-      g.check = max(g.x0, g.from / kBlock);
-      if (lane == 0) {
-        if (!more) g.x0 = g.x1 = 0;  // the end
-        g.b = b;
-        g.tainted = 0;
-        segs[sg] = g;
-        mbar_arrive(seg_full + sg);
-      }
-      if (!more) break;
-      if (seg > 0 && !warp_wait(q_empty, (seg - 1) & 1)) break;
-      const int tiles = g.n1 > 0 ? 2 : 1;
-      if (lane == 0) mbar_arrive_expect_tx(q_full, tiles * used * D * 2);
-      __syncwarp();
-      if (lane < tiles * (D / 64)) {
-        const int t = lane / (D / 64), h = lane % (D / 64);
-        tma_load_4d(sbase + t * L::kTile + h * (128 * 128), &qmap, q_full, h * 64, 0, g.kvh, g.tok0 + t * p.tq);
-      }
-      ++seg;
-      const int32_t* row = p.table + b * p.table_stride;
-      if (!p.splits && lane == 0 && __ldg(p.lens + b) != g.kv) atomicOr(&g_status, kStatusBadIndex);
-      for (int x = g.x0; x < g.x1 && ok; ++x) {
-        const int t = x * kBlock + sub * per;
-        int page = static_cast<int>(p.n_pages);  // no such page: zeros
-        if (lane < boxes && t < g.kv) {
-          page = __ldg(row + (t >> p.page_shift));
-          if (page < 0 || page >= p.n_pages) {
-            page = static_cast<int>(p.n_pages);
-            atomicOr(&g_status, kStatusBadIndex);
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    if (warp == kCopyWarp) {
+      // ---- copies: queries per segment, then key and value blocks in turn.
+      Walk walk;
+      walk.begin(p);
+      Segment g;
+      const int per = p.box_rows, boxes = kBlock / per * (D / 64);
+      const int half = lane % (D / 64), sub = lane / (D / 64);
+      int seg = 0, pos = 0, checks = 0;
+      bool ok = true;
+      while (ok) {
+        int b = 0;
+        const bool more = walk.next(p, g, b);
+        const int sg = seg % kSegs;
+        if (seg >= kSegs && !warp_wait(seg_empty + sg, ((seg / kSegs) & 1) ^ 1)) break;
+        g.from = max(0, p.causal ? g.lim0 : g.kv) & ~3;
+        g.check = max(g.x0, g.from / kBlock);
+        if (lane == 0) {
+          if (!more) g.x0 = g.x1 = 0;  // the end
+          g.b = b;
+          g.tainted = 0;
+          segs[sg] = g;
+          mbar_arrive(seg_full + sg);
+        }
+        if (!more) break;
+        if (seg > 0 && !warp_wait(q_empty, (seg - 1) & 1)) break;
+        const int tiles = g.n1 > 0 ? 2 : 1;
+        if (lane == 0) mbar_arrive_expect_tx(q_full, tiles * used * D * 2);
+        __syncwarp();
+        if (lane < tiles * (D / 64)) {
+          const int t = lane / (D / 64), h = lane % (D / 64);
+          tma_load_4d(sbase + t * L::kTile + h * (128 * 128), &qmap, q_full, h * 64, 0, g.kvh, g.tok0 + t * p.tq);
+        }
+        ++seg;
+        const int32_t* row = p.table + b * p.table_stride;
+        if (!p.splits && lane == 0 && __ldg(p.lens + b) != g.kv) atomicOr(&g_status, kStatusBadIndex);
+        for (int x = g.x0; x < g.x1 && ok; ++x) {
+          const int t = x * kBlock + sub * per;
+          int page = static_cast<int>(p.n_pages);  // no such page: zeros
+          if (lane < boxes && t < g.kv) {
+            page = __ldg(row + (t >> p.page_shift));
+            if (page < 0 || page >= p.n_pages) {
+              page = static_cast<int>(p.n_pages);
+              atomicOr(&g_status, kStatusBadIndex);
+            }
+          }
+          const int in_page = t & ((1 << p.page_shift) - 1);
+          for (int w = 0; w < 2; ++w, ++pos) {
+            const int st = pos % kStages;
+            if (pos >= kStages && !warp_wait(empty + st, ((pos / kStages) & 1) ^ 1)) {
+              ok = false;
+              break;
+            }
+            if (lane == 0) mbar_arrive_expect_tx(full + st, L::kSlot);
+            __syncwarp();
+            if (lane < boxes)
+              tma_load_4d(sbase + L::kRing + st * L::kSlot + half * (kBlock * 128) + sub * per * 128,
+                          w ? &vmap : &kmap, full + st, half * 64, in_page, g.kvh, page);
+          }
+          if (ok && x >= g.check) {
+            if (lane == 0) mbar_arrive(asked + checks % kStages);
+            ++checks;
           }
         }
-        const int in_page = t & ((1 << p.page_shift) - 1);
-        for (int w = 0; w < 2; ++w, ++pos) {
-          const int st = pos % kStages;
-          if (pos >= kStages && !warp_wait(empty + st, ((pos / kStages) & 1) ^ 1)) {
+      }
+      // Copies still in flight land before the CTA's memory goes (bounded).
+      if (seg > 0) warp_wait(q_full, (seg - 1) & 1);
+      for (int i = pos < kStages ? 0 : pos - kStages; i < pos; ++i)
+        if (!warp_wait(full + i % kStages, (i / kStages) & 1)) break;
+    } else if (warp == kMmaWarp) {
+      // ---- products: one elected thread waits for what they need and issues them.
+      constexpr uint32_t kIdS = instr_desc(Elem<E>::kFormat, kBlock, false);
+      constexpr uint32_t kIdO = instr_desc(Elem<E>::kFormat, D, true);
+      if (elect_one()) {
+        const uint64_t q_desc = smem_desc(sbase, 16, 1024);
+        const uint64_t k_desc = smem_desc(sbase + L::kRing, 16, 1024);
+        const uint64_t v_desc = smem_desc(sbase + L::kRing, kBlock * 128, 1024);
+        auto issue_s = [&](int t, int slot) {
+          const uint64_t a = q_desc + t * (L::kTile >> 4), b = k_desc + slot * (L::kSlot >> 4);
+    #pragma unroll
+          for (int k = 0; k < D / 16; ++k) {
+            const uint32_t off = ((k / 4) * (128 * 128) + (k % 4) * 32) >> 4;
+            mma_ss(tmem + t * kBlock, a + off, b + off, kIdS, k > 0);
+          }
+          mma_commit(s_full + t);
+        };
+        const uint32_t weights_at = L::kApart ? tmem + 2 * kBlock + 2 * D : tmem;
+        constexpr uint32_t weights_step = L::kApart ? kBlock / 2 : kBlock;
+        auto issue_o = [&](int t, int slot, bool late, bool add) {
+          const uint64_t b = v_desc + slot * (L::kSlot >> 4);
+    #pragma unroll
+          for (int k = 0; k < kBlock / 16; ++k) {
+            if ((k < kEarly / 16) != late)
+              mma_ts(tmem + 2 * kBlock + t * D, weights_at + t * weights_step + k * 8, b + (k * 16 * 128 >> 4), kIdO,
+                     add || k > 0);
+          }
+        };
+        auto wait = [&](uint64_t* bar, uint32_t parity) {
+          const bool ok = mbar_wait(bar, parity);
+          fence_after_sync();
+          return ok;
+        };
+        int seg = 0, slot = 0;
+        uint32_t ring = 0, weights = 0;  // parities: the ring's, the two tiles' weights
+        auto advance = [&] {
+          if (++slot == kStages) {
+            slot = 0;
+            ring ^= 1;
+          }
+        };
+        bool ok = true;
+        while (ok) {
+          const int sg = seg % kSegs;
+          if (!mbar_wait(seg_full + sg, (seg / kSegs) & 1)) break;
+          const int c0 = tile_count(segs[sg], 0), c1 = tile_count(segs[sg], 1);
+          const int n = segs[sg].x1 - segs[sg].x0;
+          if (n == 0) break;
+          mbar_arrive(seg_empty + sg);
+          ok = wait(q_full, seg & 1) && wait(full + slot, ring);
+          ++seg;
+          if (!ok) break;
+          if (c0 > 0) issue_s(0, slot);
+          if (c1 > 0) issue_s(1, slot);
+          mma_commit(empty + slot);
+          if (n == 1) mma_commit(q_empty);
+          advance();
+          for (int j = 0; j < n && ok; ++j) {
+            const int vslot = slot;
+            const bool more = j + 1 < n;
+            ok = wait(full + vslot, ring);
+            advance();
+            const int kslot = slot;
+            if (ok && more) {
+              ok = wait(full + kslot, ring);
+              advance();
+            }
+    #pragma unroll
+            for (int t = 0; t < 2; ++t) {
+              const int c = t ? c1 : c0;
+              if (!ok || j >= c) continue;
+              ok = wait(p_half + t, weights >> t & 1);
+              if (!ok) continue;
+              // (Early weights also say that the block's scores have been read.)
+              if (L::kApart && j + 1 < c) issue_s(t, kslot);
+              issue_o(t, vslot, false, j > 0);
+              ok = wait(p_full + t, weights >> t & 1);
+              weights ^= 1u << t;
+              if (!ok) continue;
+              issue_o(t, vslot, true, true);
+              if (!L::kApart && j + 1 < c) issue_s(t, kslot);
+              else mma_commit(o_full + t);
+            }
+            mma_commit(empty + vslot);
+            if (more) mma_commit(empty + kslot);
+            if (j + 2 == n) mma_commit(q_empty);
+          }
+        }
+        // Nothing of this CTA is in flight when it ends (bounded).
+        mma_commit(drained);
+        mbar_wait(drained, 0);
+      }
+      __syncwarp();
+    } else {
+      // ---- values that not every row sees. Blocks that need no look are not
+      // waited for, so the copies say when one that does is on its way: the phase
+      // of its ring slot is then the current one, and stays so until the products
+      // have taken it, which these warps have to let them first. (For the same reason
+      // no phase of `asked` or `checked` is ever overrun.)
+      int seg = 0, base = 0, n = 0;
+      bool ok = true;
+      while (ok) {
+        const int sg = seg % kSegs;
+        if (!warp_wait(seg_full + sg, (seg / kSegs) & 1)) break;
+        Segment& g = segs[sg];
+        const int x0 = g.x0, x1 = g.x1, kv = g.kv;
+        if (x1 == x0) break;
+        ++seg;
+        for (int x = g.check; x < x1; ++x, ++n) {
+          const int pos = base + 2 * (x - x0) + 1;
+          if (!warp_wait(asked + n % kStages, (n / kStages) & 1) ||
+              !warp_wait(full + pos % kStages, (pos / kStages) & 1)) {
             ok = false;
             break;
           }
-          if (lane == 0) mbar_arrive_expect_tx(full + st, L::kSlot);
+          // Rows of the last page behind the end hold anything, those of no page zeros.
+          const int rows = kv - x * kBlock, end = ((rows - 1) | ((1 << p.page_shift) - 1)) + 1;
+          if (clean_values<E, D>(smem + L::kRing + (pos % kStages) * L::kSlot, max(0, g.from - x * kBlock),
+                                 min(kBlock, end), rows, warp - kValueWarp))
+            g.tainted = 1;
+          fence_async_shared();  // before the products read them
           __syncwarp();
-          if (lane < boxes)
-            tma_load_4d(sbase + L::kRing + st * L::kSlot + half * (kBlock * 128) + sub * per * 128,
-                        w ? &vmap : &kmap, full + st, half * 64, in_page, g.kvh, page);
+          if (lane == 0) mbar_arrive(checked + n % kStages);
         }
-        if (ok && x >= g.check) {
-          if (lane == 0) mbar_arrive(asked + checks % kStages);
-          ++checks;
-        }
+        base += 2 * (x1 - x0);
+        if (ok && lane == 0) mbar_arrive(seg_empty + sg);
       }
     }
-    // Copies still in flight land before the CTA's memory goes (bounded).
-    if (seg > 0) warp_wait(q_full, (seg - 1) & 1);
-    for (int i = pos < kStages ? 0 : pos - kStages; i < pos; ++i)
-      if (!warp_wait(full + i % kStages, (i / kStages) & 1)) break;
-  } else if (warp == kMmaWarp) {
-    // ---- products: one thread issues them, the warp walks alike (its
-    // addresses and descriptors then live in uniform registers).
-    constexpr uint32_t kIdS = instr_desc(Elem<E>::kFormat, kBlock, false);
-    constexpr uint32_t kIdO = instr_desc(Elem<E>::kFormat, D, true);
-    if (elect_one()) {
-    const uint64_t q_desc = smem_desc(sbase, 16, 1024);
-    const uint64_t k_desc = smem_desc(sbase + L::kRing, 16, 1024);
-    const uint64_t v_desc = smem_desc(sbase + L::kRing, kBlock * 128, 1024);
-    auto issue_s = [&](int t, int slot) {
-      const uint64_t a = q_desc + t * (L::kTile >> 4), b = k_desc + slot * (L::kSlot >> 4);
-#pragma unroll
-      for (int k = 0; k < D / 16; ++k) {
-        const uint32_t off = ((k / 4) * (128 * 128) + (k % 4) * 32) >> 4;
-        mma_ss(tmem + t * kBlock, a + off, b + off, kIdS, k > 0);
-      }
-      mma_commit(s_full + t);
-    };
-    const uint32_t weights_at = L::kApart ? tmem + 2 * kBlock + 2 * D : tmem;
-    constexpr uint32_t weights_step = L::kApart ? kBlock / 2 : kBlock;
-    auto issue_o = [&](int t, int slot, bool late, bool add) {
-      const uint64_t b = v_desc + slot * (L::kSlot >> 4);
-#pragma unroll
-      for (int k = 0; k < kBlock / 16; ++k) {
-        if ((k < kEarly / 16) != late)
-          mma_ts(tmem + 2 * kBlock + t * D, weights_at + t * weights_step + k * 8, b + (k * 16 * 128 >> 4), kIdO,
-                 add || k > 0);
-      }
-    };
-    auto commit = [&](uint64_t* bar) {
-      mma_commit(bar);
-    };
-    auto wait = [&](uint64_t* bar, uint32_t parity) {
-      const bool ok = mbar_wait(bar, parity);
-      fence_after_sync();
-      return ok;
-    };
-    int seg = 0, slot = 0;
-    uint32_t ring = 0, weights = 0;  // parities: the ring's, the two tiles' weights
-    auto advance = [&] {
-      if (++slot == kStages) {
-        slot = 0;
-        ring ^= 1;
-      }
-    };
-    bool ok = true;
-    while (ok) {
-      const int sg = seg % kSegs;
-      if (!mbar_wait(seg_full + sg, (seg / kSegs) & 1)) break;
-      const int c0 = tile_count(segs[sg], 0), c1 = tile_count(segs[sg], 1);
-      const int n = segs[sg].x1 - segs[sg].x0;
-      if (n == 0) break;
-      mbar_arrive(seg_empty + sg);
-      ok = wait(q_full, seg & 1) && wait(full + slot, ring);
-      ++seg;
-      if (!ok) break;
-      if (c0 > 0) issue_s(0, slot);
-      if (c1 > 0) issue_s(1, slot);
-      commit(empty + slot);
-      if (n == 1) commit(q_empty);
-      advance();
-      for (int j = 0; j < n && ok; ++j) {
-        const int vslot = slot;
-        const bool more = j + 1 < n;
-        ok = wait(full + vslot, ring);
-        advance();
-        const int kslot = slot;
-        if (ok && more) {
-          ok = wait(full + kslot, ring);
-          advance();
-        }
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          const int c = t ? c1 : c0;
-          if (!ok || j >= c) continue;
-          ok = wait(p_half + t, weights >> t & 1);
-          if (!ok) continue;
-          // (Early weights also say that the block's scores have been read.)
-          if (L::kApart && j + 1 < c) issue_s(t, kslot);
-          issue_o(t, vslot, false, j > 0);
-          ok = wait(p_full + t, weights >> t & 1);
-          weights ^= 1u << t;
-          if (!ok) continue;
-          issue_o(t, vslot, true, true);
-          if (!L::kApart && j + 1 < c) issue_s(t, kslot);
-          else commit(o_full + t);
-        }
-        commit(empty + vslot);
-        if (more) commit(empty + kslot);
-        if (j + 2 == n) commit(q_empty);
-      }
-    }
-    // Nothing of this CTA is in flight when it ends (bounded).
-    commit(drained);
-    mbar_wait(drained, 0);
-    }
-    __syncwarp();
-  } else {
-    // ---- values that not every row sees. Blocks that need no look are not
-    // waited for, so the copies say when one that does is on its way: the phase
-    // of its ring slot is then the current one, and stays so until the products
-    // have taken it, which these warps have to let them first. (For the same reason
-    // no phase of `asked` or `checked` is ever overrun.)
-    int seg = 0, base = 0, n = 0;
-    bool ok = true;
-    while (ok) {
-      const int sg = seg % kSegs;
-      if (!warp_wait(seg_full + sg, (seg / kSegs) & 1)) break;
-      Segment& g = segs[sg];
-      const int x0 = g.x0, x1 = g.x1, kv = g.kv;
-      if (x1 == x0) break;
-      ++seg;
-      for (int x = g.check; x < x1; ++x, ++n) {
-        const int pos = base + 2 * (x - x0) + 1;
-        if (!warp_wait(asked + n % kStages, (n / kStages) & 1) || !warp_wait(full + pos % kStages, (pos / kStages) & 1)) {
-          ok = false;
-          break;
-        }
-        // Rows of the last page behind the end hold anything, those of no page zeros.
-        const int rows = kv - x * kBlock, end = ((rows - 1) | ((1 << p.page_shift) - 1)) + 1;
-        if (clean_values<E, D>(smem + L::kRing + (pos % kStages) * L::kSlot, max(0, g.from - x * kBlock),
-                               min(kBlock, end), rows, warp - kValueWarp))
-          g.tainted = 1;
-        fence_async_shared();  // before the products read them
-        __syncwarp();
-        if (lane == 0) mbar_arrive(checked + n % kStages);
-      }
-      base += 2 * (x1 - x0);
-      if (ok && lane == 0) mbar_arrive(seg_empty + sg);
-    }
-  }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
     // ---- softmax: one thread a row of tile t.

@@ -246,7 +246,8 @@ def shared_prefix_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: tor
     """``paged_attention`` for a batch whose sequences share their first
     ``prefix_len`` positions (a system prompt, a document that is sampled from
     many times): those lie in the pages of ``prefix_table`` (int32
-    [prefix pages]) and are read once for the whole batch; ``block_table`` and
+    [prefix pages]) and are read once for many sequences (once or twice for a
+    small batch, once for every 256 / (Hq / Hkv) of a larger one); ``block_table`` and
     ``kv_lens`` are each sequence's own positions after them (none is fine).
     ``workspace``: ``shared_prefix_workspace``."""
     if q.is_cuda:

@@ -420,7 +420,8 @@ int dqg_prompt_attention(const void *q, int64_t q_stride_row, int64_t q_stride_h
  * Decode attention of a batch whose sequences share their first prefix_len
  * positions: out[b, h] is as dqg_paged_attention's over the prefix's keys and
  * then sequence b's own kv_lens[b]. The prefix's pages (prefix_table
- * [prefix_pages]) are read once for the whole batch. prefix_len is a host
+ * [prefix_pages]) are read once or twice for a small batch, and once for every
+ * 2 * floor(128 / (Hq / Hkv)) sequences of a larger one. prefix_len is a host
  * value (0: no prefix); the sequences' own lengths are read on the device and
  * may be zero. Everything else as dqg_paged_attention.
  */
