@@ -1,22 +1,14 @@
 // Rotation and storing of a batch of tokens' queries, keys and values: one
 // pass over the QKV projection's rows that norms the query and key heads
 // (optional), rotates them by their positions and writes queries to a dense
-// tensor and keys and values into their pages. No reference counterpart: the
-// reference only models the cache's bytes (dequant/byte_model.py:214-219).
+// tensor and keys and values into their pages (formulas and a lane's part of
+// them: paged_rope.cuh). No reference counterpart: the reference only models the
+// cache's bytes (dequant/byte_model.py:214-219). fp32 with one rounding at the
+// end; cos and sin come from a table of positions, so every scaling of the
+// frequencies is the caller's.
 //
-//   y     = x * rsqrt(mean(x^2) + eps) * w           (with a norm; per head)
-//   (a,b) = (y_i, y_j),  j = i + R/2  or  (i, j) = (2p, 2p + 1)
-//   a'    = a cos - b sin,  b' = b cos + a sin       (first R values; the rest pass)
-//
-// in fp32 with one rounding at the end; cos and sin come from a table of
-// positions, so every scaling of the frequencies is the caller's.
-//
-// Bound by HBM: each row is read once and each head written once. A group of
-// D / 16 lanes holds a head, and a lane two runs of eight values: in the half
-// layout those at i and i + R/2, so that both values of a rotated pair lie in
-// one lane and share a table entry; interleaved pairs lie in one lane anyway.
-// A warp takes a few heads of one token, whose table entries stay in
-// registers; the sum of squares is one shuffle reduction. What it measured
+// Bound by HBM: each row is read once and each head written once. A warp takes a
+// few heads of one token, whose table entries stay in registers; the sum of squares is one shuffle reduction. What it measured
 // (B200, 8192 tokens of 64 + 2 x 8 heads of 128, bf16, norms): 62.5 us a call,
 // 5.4 TB/s of the 6.4 that a copy reaches (58.5 us and 5.8 replayed from a graph,
 // which the following figures are). Registers and stores decide: 128 registers
@@ -25,7 +17,7 @@
 // of eight (more, narrower accesses) 84 us; one head a lane group at a time 84.
 #include <cstdint>
 
-#include "paged.cuh"
+#include "paged_rope.cuh"
 
 namespace dqg {
 namespace {
@@ -50,56 +42,30 @@ struct AppendParams {
   float eps;
 };
 
-enum Layout {
-  kHalf,         // pairs (i, i + R/2), R a multiple of 16
-  kInterleaved,  // pairs (2i, 2i + 1)
-  kUneven        // pairs (i, i + R/2), any R: partners are read again from memory
-};
-
-template <typename E>
-__device__ __forceinline__ void unpack8(uint4 v, float* f) {
-  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float2 t = Elem<E>::unpack(w[i]);
-    f[2 * i] = t.x;
-    f[2 * i + 1] = t.y;
-  }
-}
-template <typename E>
-__device__ __forceinline__ uint4 pack8(const float* f) {
-  return make_uint4(Elem<E>::pack(f[0], f[1]), Elem<E>::pack(f[2], f[3]), Elem<E>::pack(f[4], f[5]),
-                    Elem<E>::pack(f[6], f[7]));
-}
-
 template <typename E, int D, int ITER, int LAYOUT>
 __global__ void __launch_bounds__(kThreads, LAYOUT == kUneven ? 4 : 5)
     paged_append_kernel(const __grid_constant__ AppendParams<E> p) {
-  constexpr int kLanes = D / 16;        // lanes a head
+  using Lane = RopeLane<E, D, LAYOUT>;
+  constexpr int kLanes = Lane::kLanes;
   constexpr int kGroups = 32 / kLanes;  // heads a warp holds at a time
   const int64_t w = static_cast<int64_t>(blockIdx.x) * (kThreads / 32) + (threadIdx.x >> 5);
   const int64_t token = w / p.chunks;
   const int chunk = static_cast<int>(w - token * p.chunks);
-  const int lane = threadIdx.x & 31, c = lane % kLanes, grp = lane / kLanes;
+  const int lane = threadIdx.x & 31, grp = lane / kLanes;
   pdl_wait_prior_grid();
   pdl_launch_dependents();
   if (token >= p.T) return;
   const int rotated = p.hq + p.hkv, n_heads = rotated + p.hkv;
   const int h0 = chunk * ITER * kGroups + grp;
-  // The lane's two runs of eight values. Half layout: the first R / 16 lanes
-  // hold the pairs, the others what passes.
-  const int rc = p.rot / 16;
-  const bool pairs = LAYOUT != kHalf || c < rc;
-  const int ea = LAYOUT == kHalf ? (pairs ? 8 * c : 16 * c) : 16 * c;
-  const int eb = LAYOUT == kHalf && pairs ? ea + p.rot / 2 : ea + 8;
+  Lane part(lane % kLanes, p.rot);
   const E* row = p.qkv + token * p.qkv_stride;
   uint4 xa[ITER], xb[ITER];
 #pragma unroll
   for (int it = 0; it < ITER; ++it) {
     const int h = h0 + it * kGroups;
     if (h < n_heads) {
-      xa[it] = __ldcs(reinterpret_cast<const uint4*>(row + static_cast<int64_t>(h) * D + ea));
-      xb[it] = __ldcs(reinterpret_cast<const uint4*>(row + static_cast<int64_t>(h) * D + eb));
+      xa[it] = __ldcs(reinterpret_cast<const uint4*>(row + static_cast<int64_t>(h) * D + part.ea));
+      xb[it] = __ldcs(reinterpret_cast<const uint4*>(row + static_cast<int64_t>(h) * D + part.eb));
     }
   }
   int64_t pos = __ldg(p.positions + token);
@@ -109,21 +75,7 @@ __global__ void __launch_bounds__(kThreads, LAYOUT == kUneven ? 4 : 5)
     pos = pos < 0 ? 0 : (pos >= p.n_positions ? p.n_positions - 1 : pos);
     if (slot >= p.n_slots) slot = -1;
   }
-  const int half = p.rot / 2;
-  // Table entries of the lane's eight pairs (uneven: of its sixteen values).
-  constexpr int kTab = LAYOUT == kUneven ? 16 : 8;
-  float cs[kTab], sn[kTab];
-  if (h0 - grp < rotated) {
-    const float* cr = p.cosv + pos * half;
-    const float* sr = p.sinv + pos * half;
-#pragma unroll
-    for (int e = 0; e < kTab; ++e) {
-      const int i = LAYOUT == kUneven ? (ea + e < half ? ea + e : ea + e - half) : 8 * c + e;
-      const bool in = LAYOUT == kUneven ? ea + e < p.rot : i < half;
-      cs[e] = in ? __ldg(cr + i) : 1.f;
-      sn[e] = in ? __ldg(sr + i) : 0.f;
-    }
-  }
+  if (h0 - grp < rotated) part.entries(p.cosv + pos * part.half, p.sinv + pos * part.half);
   const int64_t page = slot >> p.page_shift;
   const int64_t place = slot & ((int64_t(1) << p.page_shift) - 1);
   const int64_t base = page * p.page_stride + place * p.row_stride;
@@ -131,63 +83,15 @@ __global__ void __launch_bounds__(kThreads, LAYOUT == kUneven ? 4 : 5)
   for (int it = 0; it < ITER; ++it) {
     const int h = h0 + it * kGroups;
     const bool is_k = h >= p.hq;
-    // (Warp-uniform: the shuffles below are taken by the whole warp.)
+    // (Warp-uniform: the norm's shuffles are taken by the whole warp.)
     if (h - grp < rotated) {
       float a[8], b[8];
       unpack8<E>(h < n_heads ? xa[it] : make_uint4(0u, 0u, 0u, 0u), a);
       unpack8<E>(h < n_heads ? xb[it] : make_uint4(0u, 0u, 0u, 0u), b);
-      float r = 1.f;
-      if (p.q_norm) {
-        float ss = 0.f;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) ss = fmaf(a[e], a[e], fmaf(b[e], b[e], ss));
-#pragma unroll
-        for (int off = kLanes / 2; off >= 1; off >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, off);
-        r = rsqrtf(fmaf(ss, 1.f / D, p.eps));
-        float wa[8], wb[8];
-        const E* nw = is_k ? p.k_norm : p.q_norm;
-        unpack8<E>(__ldg(reinterpret_cast<const uint4*>(nw + ea)), wa);
-        unpack8<E>(__ldg(reinterpret_cast<const uint4*>(nw + eb)), wb);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          a[e] *= r * wa[e];
-          b[e] *= r * wb[e];
-        }
-      }
+      const E* nw = is_k ? p.k_norm : p.q_norm;
+      const float r = part.norm(a, b, nw, p.eps);
       if (h < rotated) {
-        if (LAYOUT == kHalf) {
-          if (pairs) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              const float x = a[e], y = b[e];
-              a[e] = fmaf(x, cs[e], -(y * sn[e]));
-              b[e] = fmaf(y, cs[e], x * sn[e]);
-            }
-          }
-        } else if (LAYOUT == kInterleaved) {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            float* t = e < 4 ? a + 2 * e : b + 2 * (e - 4);
-            if (8 * c + e < half) {
-              const float x = t[0], y = t[1];
-              t[0] = fmaf(x, cs[e], -(y * sn[e]));
-              t[1] = fmaf(y, cs[e], x * sn[e]);
-            }
-          }
-        } else {
-          const E* head = row + static_cast<int64_t>(h) * D;
-          const E* nw = is_k ? p.k_norm : p.q_norm;
-#pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const int i = ea + e, j = i < half ? i + half : i - half;
-            float* t = e < 8 ? a + e : b + e - 8;
-            if (i < p.rot) {
-              float y = Elem<E>::load(head + j);
-              if (p.q_norm) y *= r * Elem<E>::load(nw + j);
-              *t = fmaf(*t, cs[e % kTab], i < half ? -(y * sn[e % kTab]) : y * sn[e % kTab]);
-            }
-          }
-        }
+        part.rotate(a, b, row + static_cast<int64_t>(h) * D, nw, r);
         xa[it] = pack8<E>(a);
         xb[it] = pack8<E>(b);
       }
@@ -200,8 +104,8 @@ __global__ void __launch_bounds__(kThreads, LAYOUT == kUneven ? 4 : 5)
       if (slot < 0) continue;
       dst = h < rotated ? p.k + base + (h - p.hq) * p.head_stride : p.v + base + (h - rotated) * p.head_stride;
     }
-    __stcs(reinterpret_cast<uint4*>(dst + ea), xa[it]);
-    __stcs(reinterpret_cast<uint4*>(dst + eb), xb[it]);
+    __stcs(reinterpret_cast<uint4*>(dst + part.ea), xa[it]);
+    __stcs(reinterpret_cast<uint4*>(dst + part.eb), xb[it]);
   }
 }
 
