@@ -44,6 +44,22 @@ class PagedKV(ctypes.Structure):
                 ("dtype", ctypes.c_int32)]
 
 
+class QuantizedKV(ctypes.Structure):
+    """``dqg_quantized_kv``: pools of codes, their scales and open blocks."""
+    _fields_ = [*((n, ctypes.c_void_p) for n in ("k", "v", "k_scale", "v_scale", "k_open", "v_open")),
+                *((n, ctypes.c_int64) for n in (
+                    "n_pages", "n_kv_heads", "page_size", "head_dim", "block", "n_open", "page_stride", "head_stride",
+                    "row_stride", "scale_page_stride", "scale_head_stride", "open_stride", "open_head_stride")),
+                ("codes", ctypes.c_int32), ("dtype", ctypes.c_int32)]
+
+
+class Sampling(ctypes.Structure):
+    """``dqg_sampling``: a value a row on the device, or one for all."""
+    _fields_ = [*((n, ctypes.c_void_p) for n in ("temperatures", "top_ks", "top_ps", "min_ps")),
+                ("temperature", ctypes.c_float), ("top_k", ctypes.c_int32), ("top_p", ctypes.c_float),
+                ("min_p", ctypes.c_float)]
+
+
 def lib() -> ctypes.CDLL:
     """Load (once) and return the C-ABI library."""
     global _lib
@@ -132,6 +148,18 @@ def lib() -> ctypes.CDLL:
     h.dqg_debug_paged_starved.restype = i32
     h.dqg_debug_paged_starved.argtypes = [*h.dqg_shared_prefix_attention.argtypes[:-1],
                                           ctypes.c_uint32, u64, vp]
+    qkv = ctypes.POINTER(QuantizedKV)
+    h.dqg_rope_quantized_append.restype = i32
+    h.dqg_rope_quantized_append.argtypes = [vp, i64, i64, i64, vp, vp, i64, i64, i32, vp, vp, vp, f32, qkv, vp,
+                                            i64, i64, vp, vp, vp, i64, vp, vp]
+    h.dqg_expand_pages.restype = i32
+    h.dqg_expand_pages.argtypes = [qkv, vp, i64, i64, vp, vp, i64, i64, vp, vp, vp, vp]
+    h.dqg_quantized_attention_workspace.restype = i32
+    h.dqg_quantized_attention_workspace.argtypes = [i64, i64, i64, i64, u64p]
+    h.dqg_quantized_attention.restype = i32
+    h.dqg_quantized_attention.argtypes = [vp, i64, i64, i64, i64, qkv, vp, i64, i64, vp, vp, f32, vp, vp, u64, vp]
+    h.dqg_sample_tokens.restype = i32
+    h.dqg_sample_tokens.argtypes = [vp, ctypes.c_int32, i64, i64, i64, vp, ctypes.POINTER(Sampling), vp, vp, vp]
     _lib = h
     return _lib
 
@@ -146,7 +174,9 @@ EXPORTED = ("dqg_last_error", "dqg_version", "dqg_add_one", "dqg_gemv", "dqg_deq
             "dqg_peer_allreduce_add_rms_norm", "dqg_gemv_swiglu",
             "dqg_gemv_swiglu_supported", "dqg_rope_paged_append", "dqg_paged_attention_workspace",
             "dqg_paged_attention", "dqg_prompt_attention_workspace", "dqg_prompt_attention",
-            "dqg_shared_prefix_workspace", "dqg_shared_prefix_attention", "dqg_debug_paged_starved")
+            "dqg_shared_prefix_workspace", "dqg_shared_prefix_attention", "dqg_debug_paged_starved",
+            "dqg_rope_quantized_append", "dqg_expand_pages", "dqg_quantized_attention_workspace",
+            "dqg_quantized_attention", "dqg_sample_tokens")
 
 
 def check(rc: int) -> None:

@@ -1,0 +1,305 @@
+// Rotation and storing of a batch of tokens in a cache held in 8 bits: queries
+// as in paged_append.cu (formulas: paged_rope.cuh), keys and values in blocks
+// of 16, 32 or 64 positions of one head with one fp32 scale:
+//
+//   x = E(rotated key) or value, in the 16-bit type E, as a 16-bit cache holds it
+//   s = max(max |x| / L, 2^-126),  code = round(x / s)      (L = 127 or 448)
+//
+// A block is quantised once, when its last position comes: until then its rows
+// wait in 16 bits in the sequence's open block. (Codes that were rounded again
+// whenever a later row raises the block's maximum would save that memory and
+// lose up to half a step each time, and would depend on how a prompt was cut
+// into calls.) 2^-126 keeps 1 / s finite; a value that is not finite makes s
+// NaN, and with it all of the block.
+//
+// The first blocks of the grid take queries, the others a block of positions
+// of one KV head each: keys, then values, sixteen values of a row a thread.
+// The block that completes a sequence's open block also stores the new open
+// rows, whose place it has read before; no other reads or writes them.
+#include <cstdint>
+
+#include "paged_rope.cuh"
+#include "quantized.cuh"
+
+namespace dqg {
+namespace {
+
+constexpr int kThreads = 128;
+constexpr int kMaxBlock = 64;
+
+template <typename E>
+struct Params {
+  const E* qkv;
+  const float* cosv;
+  const float* sinv;
+  const int64_t* positions;
+  const E* q_norm;
+  const E* k_norm;
+  E* q_out;
+  QuantizedPool pool;
+  QuantizedSeqs seqs;
+  int64_t qkv_stride, n_positions, q_blocks;
+  int T, hq, hkv, rot, page_shift, block_shift, chunks;
+  float eps;
+};
+
+struct Seq {
+  int q0, n, end;  // first row of qkv, new rows, length with them
+};
+// A sequence's rows; none where its description is out of order or range.
+template <typename E>
+__device__ __forceinline__ Seq load_seq(const Params<E>& p, int b, bool report) {
+  Seq s;
+  s.q0 = __ldg(p.seqs.q_starts + b);
+  s.end = __ldg(p.seqs.lens + b);
+  const int64_t n = static_cast<int64_t>(__ldg(p.seqs.q_starts + b + 1)) - s.q0;
+  const int64_t limit = static_cast<int64_t>(p.seqs.table_width) << p.page_shift;
+  const int slot = __ldg(p.seqs.open_slots + b);
+  const bool good = s.q0 >= 0 && n >= 0 && s.q0 + n <= p.T && (n == 0 || (n <= s.end && s.end <= limit && slot >= 0 &&
+                                                                          slot < p.pool.n_open));
+  if (!good && report) atomicOr(&g_status, kStatusBadIndex);
+  s.n = good ? static_cast<int>(n) : 0;
+  return s;
+}
+// Blocks of positions that a sequence's new rows touch on, the open one at its
+// end counted with the first.
+template <typename E>
+__device__ __forceinline__ uint32_t units_of(const Params<E>& p, const Seq& s) {
+  if (s.n == 0) return 0;
+  const int first = (s.end - s.n) >> p.block_shift, done = s.end >> p.block_shift;
+  return done > first ? done - first : 1;
+}
+
+__device__ __forceinline__ int64_t clamped_position(int64_t pos, int64_t n, bool report) {
+  if (pos < 0 || pos >= n) {
+    if (report) atomicOr(&g_status, kStatusBadIndex);
+    return pos < 0 ? 0 : n - 1;
+  }
+  return pos;
+}
+
+template <typename E, int D, int LAYOUT>
+__device__ __forceinline__ void store_queries(const Params<E>& p) {
+  using Lane = RopeLane<E, D, LAYOUT>;
+  constexpr int kGroups = 32 / Lane::kLanes;  // heads a warp holds
+  const int64_t w = static_cast<int64_t>(blockIdx.x) * (kThreads / 32) + (threadIdx.x >> 5);
+  const int64_t token = w / p.chunks;
+  const int lane = threadIdx.x & 31, h = static_cast<int>(w - token * p.chunks) * kGroups + lane / Lane::kLanes;
+  if (token >= p.T) return;
+  Lane part(lane % Lane::kLanes, p.rot);
+  const E* head = p.qkv + token * p.qkv_stride + static_cast<int64_t>(h) * D;
+  uint4 xa = make_uint4(0, 0, 0, 0), xb = xa;
+  if (h < p.hq) {
+    xa = __ldcs(reinterpret_cast<const uint4*>(head + part.ea));
+    xb = __ldcs(reinterpret_cast<const uint4*>(head + part.eb));
+  }
+  const int64_t pos = clamped_position(__ldg(p.positions + token), p.n_positions, lane == 0);
+  part.entries(p.cosv + pos * part.half, p.sinv + pos * part.half);
+  float a[8], b[8];
+  unpack8<E>(xa, a);
+  unpack8<E>(xb, b);
+  const float r = part.norm(a, b, p.q_norm, p.eps);
+  if (h >= p.hq) return;
+  part.rotate(a, b, head, p.q_norm, r);
+  E* dst = p.q_out + (token * p.hq + h) * D;
+  __stcs(reinterpret_cast<uint4*>(dst + part.ea), pack8<E>(a));
+  __stcs(reinterpret_cast<uint4*>(dst + part.eb), pack8<E>(b));
+}
+
+// Largest magnitude among 16-bit values, as bits (an infinity or NaN is larger
+// than any finite value).
+__device__ __forceinline__ uint32_t magnitude(uint4 v, uint32_t m) {
+  m = __vmaxu2(m, v.x & 0x7fff7fffu);
+  m = __vmaxu2(m, v.y & 0x7fff7fffu);
+  m = __vmaxu2(m, v.z & 0x7fff7fffu);
+  return __vmaxu2(m, v.w & 0x7fff7fffu);
+}
+
+template <typename E, int D, int LAYOUT, class Code>
+__device__ __forceinline__ void store_block(const Params<E>& p, int b, const Seq& s, int j, int kvh, uint32_t* scratch) {
+  using Lane = RopeLane<E, D, LAYOUT>;
+  constexpr int kRows = kThreads / Lane::kLanes;       // rows at a time
+  constexpr int kPasses = (kMaxBlock + kRows - 1) / kRows;
+  const int row0 = threadIdx.x / Lane::kLanes;
+  const int base = j << p.block_shift, block = 1 << p.block_shift, start = s.end - s.n;
+  const bool whole = base + block <= s.end;
+  const int64_t slot = __ldg(p.seqs.open_slots + b);
+  int page = whole ? __ldg(p.seqs.table + b * p.seqs.table_stride + (base >> p.page_shift)) : 0;
+  if (page < 0 || page >= p.pool.n_pages) {
+    if (threadIdx.x == 0) atomicOr(&g_status, kStatusBadIndex);
+    page = -1;
+  }
+  for (int which = 0; which < 2; ++which) {
+    E* open = static_cast<E*>(which ? p.pool.v_open : p.pool.k_open) + slot * p.pool.open_stride +
+              kvh * p.pool.open_head_stride;
+    const E* nw = which ? nullptr : p.k_norm;
+    uint4 xa[kPasses], xb[kPasses];
+    uint32_t most = 0;
+#pragma unroll
+    for (int i = 0; i < kPasses; ++i) {
+      xa[i] = xb[i] = make_uint4(0, 0, 0, 0);
+      if (i * kRows >= block) continue;
+      const int row = row0 + i * kRows, t = base + row;
+      const bool fresh = row < block && t >= start && t < s.end;
+      const int64_t token = s.q0 + (fresh ? t - start : 0);
+      Lane part(threadIdx.x % Lane::kLanes, which ? 0 : p.rot);
+      const E* head = p.qkv + token * p.qkv_stride + static_cast<int64_t>(p.hq + (which ? p.hkv : 0) + kvh) * D;
+      if (fresh) {
+        xa[i] = __ldcs(reinterpret_cast<const uint4*>(head + part.ea));
+        xb[i] = __ldcs(reinterpret_cast<const uint4*>(head + part.eb));
+      }
+      if (!which) {
+        const int64_t pos = clamped_position(__ldg(p.positions + token), p.n_positions, false);
+        part.entries(p.cosv + pos * part.half, p.sinv + pos * part.half);
+        float x[8], y[8];
+        unpack8<E>(xa[i], x);
+        unpack8<E>(xb[i], y);
+        const float r = part.norm(x, y, nw, p.eps);
+        if (fresh) {
+          part.rotate(x, y, head, nw, r);
+          xa[i] = pack8<E>(x);
+          xb[i] = pack8<E>(y);
+        }
+      }
+      if (whole && row < block && t < start) {  // stored by an earlier call
+        xa[i] = *reinterpret_cast<const uint4*>(open + row * D + part.ea);
+        xb[i] = *reinterpret_cast<const uint4*>(open + row * D + part.eb);
+      }
+      if (!whole && fresh) {
+        *reinterpret_cast<uint4*>(open + row * D + part.ea) = xa[i];
+        *reinterpret_cast<uint4*>(open + row * D + part.eb) = xb[i];
+      }
+      most = magnitude(xb[i], magnitude(xa[i], most));
+    }
+    if (!whole) continue;
+#pragma unroll
+    for (int off = 16; off >= 1; off >>= 1) most = __vmaxu2(most, __shfl_xor_sync(0xffffffffu, most, off));
+    if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = most;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kThreads / 32; ++w) most = __vmaxu2(most, scratch[w]);
+    __syncthreads();
+    const float2 two = Elem<E>::unpack(most);
+    const bool finite = Elem<E>::non_finite(most) == 0u;
+    const float scale = finite ? fmaxf(fmaxf(two.x, two.y) / Code::kMost, 1.17549435e-38f) : NAN;
+    const float inv = 1.f / scale;
+    if (page < 0) continue;
+    if (threadIdx.x == 0) {
+      float* to = (which ? p.pool.v_scale : p.pool.k_scale) + page * p.pool.scale_page_stride +
+                  kvh * p.pool.scale_head_stride;
+      to[(base & ((1 << p.page_shift) - 1)) >> p.block_shift] = scale;
+    }
+    uint8_t* codes = static_cast<uint8_t*>(which ? p.pool.v : p.pool.k) + page * p.pool.page_stride +
+                     kvh * p.pool.head_stride + (base & ((1 << p.page_shift) - 1)) * p.pool.row_stride;
+#pragma unroll
+    for (int i = 0; i < kPasses; ++i) {
+      const int row = row0 + i * kRows;
+      if (row >= block) continue;
+      const Lane part(threadIdx.x % Lane::kLanes, which ? 0 : p.rot);
+      float x[8];
+#pragma unroll
+      for (int run = 0; run < 2; ++run) {
+        unpack8<E>(run ? xb[i] : xa[i], x);
+        uint2 w = make_uint2(0, 0);
+        if (finite) {
+          w.x = Code::pack4(x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
+          w.y = Code::pack4(x[4] * inv, x[5] * inv, x[6] * inv, x[7] * inv);
+        }
+        __stcs(reinterpret_cast<uint2*>(codes + row * p.pool.row_stride + (run ? part.eb : part.ea)), w);
+      }
+    }
+  }
+}
+
+template <typename E, int D, int LAYOUT, class Code>
+__global__ void __launch_bounds__(kThreads)
+    quantized_append_kernel(const __grid_constant__ Params<E> p) {
+  __shared__ uint32_t scratch[kThreads / 32 + 2];
+  pdl_wait_prior_grid();
+  pdl_launch_dependents();
+  if (blockIdx.x < p.q_blocks) {
+    store_queries<E, D, LAYOUT>(p);
+    return;
+  }
+  const int64_t u = blockIdx.x - p.q_blocks;
+  const int kvh = static_cast<int>(u % p.hkv);
+  int64_t in = 0;
+  // (The last block's unit is behind all others: it looks at every sequence.)
+  const bool report = blockIdx.x == gridDim.x - 1;
+  const int b = find_unit(p.seqs.B, u / p.hkv, [&](int i) { return units_of(p, load_seq(p, i, report)); }, scratch, &in);
+  if (b < 0) return;
+  const Seq s = load_seq(p, b, false);
+  const int first = (s.end - s.n) >> p.block_shift, last = (s.end - 1) >> p.block_shift;
+  __syncthreads();
+  store_block<E, D, LAYOUT, Code>(p, b, s, first + static_cast<int>(in), kvh, scratch);
+  if (in == 0 && last > first && (s.end & ((1 << p.block_shift) - 1))) {
+    __syncthreads();  // the open rows have been read
+    store_block<E, D, LAYOUT, Code>(p, b, s, last, kvh, scratch);
+  }
+}
+
+template <typename E, int D, class Code>
+cudaError_t launch(const QuantizedPool& pool, const QuantizedSeqs& seqs, const QuantizedAppendArgs& a,
+                   cudaStream_t stream) {
+  Params<E> p;
+  p.qkv = static_cast<const E*>(a.qkv);
+  p.cosv = a.cosv;
+  p.sinv = a.sinv;
+  p.positions = a.positions;
+  p.q_norm = static_cast<const E*>(a.q_norm);
+  p.k_norm = static_cast<const E*>(a.k_norm);
+  p.q_out = static_cast<E*>(a.q_out);
+  p.pool = pool;
+  p.seqs = seqs;
+  p.qkv_stride = a.qkv_stride;
+  p.n_positions = a.n_positions;
+  p.T = a.T;
+  p.hq = a.hq;
+  p.hkv = pool.n_kv_heads;
+  p.rot = a.rot;
+  p.eps = a.eps;
+  p.page_shift = p.block_shift = 0;
+  while ((1 << p.page_shift) < pool.page_size) ++p.page_shift;
+  while ((1 << p.block_shift) < pool.block) ++p.block_shift;
+  constexpr int kPer = 32 / (D / 16);
+  p.chunks = (a.hq + kPer - 1) / kPer;
+  p.q_blocks = (static_cast<int64_t>(a.T) * p.chunks + kThreads / 32 - 1) / (kThreads / 32);
+  // n new rows make (n - 1) / block + 1 units at most; and one more than all.
+  const int64_t units = a.T / pool.block + (a.T < seqs.B ? a.T : seqs.B) + 1;
+  const int64_t blocks = p.q_blocks + units * pool.n_kv_heads;
+  if (blocks > 0x7fffffff) return cudaErrorInvalidValue;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(blocks));
+  cfg.blockDim = dim3(kThreads);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (a.interleaved) return cudaLaunchKernelEx(&cfg, quantized_append_kernel<E, D, kInterleaved, Code>, p);
+  if (a.rot % 16 == 0) return cudaLaunchKernelEx(&cfg, quantized_append_kernel<E, D, kHalf, Code>, p);
+  return cudaLaunchKernelEx(&cfg, quantized_append_kernel<E, D, kUneven, Code>, p);
+}
+
+template <typename E, int D>
+cudaError_t launch_code(const QuantizedPool& pool, const QuantizedSeqs& seqs, const QuantizedAppendArgs& a,
+                        cudaStream_t stream) {
+  return pool.e4m3 ? launch<E, D, E4m3>(pool, seqs, a, stream) : launch<E, D, Int8>(pool, seqs, a, stream);
+}
+
+}  // namespace
+
+cudaError_t launch_quantized_append(const QuantizedPool& pool, const QuantizedSeqs& seqs, const QuantizedAppendArgs& a,
+                                    int num_sms, cudaStream_t stream) {
+  (void)num_sms;
+  if (pool.bf16)
+    return pool.D == 128 ? launch_code<__nv_bfloat16, 128>(pool, seqs, a, stream)
+                         : launch_code<__nv_bfloat16, 64>(pool, seqs, a, stream);
+  return pool.D == 128 ? launch_code<__half, 128>(pool, seqs, a, stream)
+                       : launch_code<__half, 64>(pool, seqs, a, stream);
+}
+
+}  // namespace dqg
+
+DQG_STATUS_READER(read_status_quantized_append)

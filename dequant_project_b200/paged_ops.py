@@ -50,7 +50,9 @@ def _binding():
         _paged_binding.bind(*(ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in (
             "dqg_last_error", "dqg_rope_paged_append", "dqg_paged_attention_workspace",
             "dqg_paged_attention", "dqg_prompt_attention_workspace", "dqg_prompt_attention",
-            "dqg_shared_prefix_workspace", "dqg_shared_prefix_attention")))
+            "dqg_shared_prefix_workspace", "dqg_shared_prefix_attention", "dqg_rope_quantized_append",
+            "dqg_expand_pages", "dqg_quantized_attention_workspace", "dqg_quantized_attention",
+            "dqg_sample_tokens")))
         _bound = _paged_binding
     return _bound
 

@@ -449,6 +449,117 @@ int dqg_debug_paged_starved(const void *q, int64_t q_stride_seq, int64_t q_strid
                             void *out, void *workspace, uint64_t workspace_bytes, uint32_t starved,
                             uint64_t wait_ns, void *stream);
 
+/*
+ * Key/value cache in 8 bits (no reference counterpart, as above). Keys and
+ * values are codes, int8 or e4m3, in two pools of [n_pages, n_kv_heads,
+ * page_size, head_dim] bytes, with an fp32 scale for every `block` positions
+ * (16, 32 or 64, at most a page) of a head: k_scale and v_scale are [n_pages,
+ * n_kv_heads, page_size / block], the blocks contiguous. A value is code *
+ * scale. A block is quantised once, when its last position is stored: until
+ * then its rows wait in 16 bits in the sequence's open block, a row of the
+ * pools k_open and v_open [n_open, n_kv_heads, block, head_dim] (the last two
+ * dimensions contiguous), so that what the cache holds does not depend on how
+ * a prompt was cut into calls. A sequence's positions are its complete blocks,
+ * through its row of a block table as above, and then len % block rows of the
+ * open block open_slots[b] (no two sequences share one). Strides of the codes
+ * are multiples of 16 bytes, of the open pools of 8 elements; page sizes, head
+ * dimensions, and what is done about indexes out of range, as above. Queries,
+ * outputs and open rows have the type `dtype`.
+ */
+enum { DQG_INT8 = 0, DQG_E4M3 = 1 };
+typedef struct dqg_quantized_kv {
+  void *k, *v;
+  float *k_scale, *v_scale;
+  void *k_open, *v_open;
+  int64_t n_pages, n_kv_heads, page_size, head_dim, block, n_open;
+  int64_t page_stride, head_stride, row_stride;
+  int64_t scale_page_stride, scale_head_stride;
+  int64_t open_stride, open_head_stride;
+  int32_t codes, dtype;
+} dqg_quantized_kv;
+
+/*
+ * dqg_rope_paged_append for such a cache. T tokens are packed by sequence as
+ * in dqg_prompt_attention: rows q_starts[b] .. q_starts[b + 1] - 1 are the
+ * newest of sequence b's kv_lens[b] positions, these included. Norms,
+ * rotation (by positions[t], a row of the tables) and q_out as there, for
+ * every row of qkv; rows outside every sequence are not stored. Keys and
+ * values are rounded to `dtype` first, as a 16-bit cache holds them; a block
+ * that is complete then (its earlier rows taken from the open block) gets
+ * scale = max(max |x| / L, 2^-126), L = 127 or 448, and codes x / scale
+ * rounded to nearest; rows of a block that is not go to the open block. A
+ * block that holds a value that is not finite gets the scale NaN. A sequence
+ * whose rows are out of order or range, or more than its length, is not
+ * stored, and sets bit 1 of dqg_device_status.
+ */
+int dqg_rope_quantized_append(const void *qkv, int64_t T, int64_t qkv_stride, int64_t n_q_heads,
+                              const float *cos_table, const float *sin_table, int64_t n_positions,
+                              int64_t rotary_dim, int interleaved, const int64_t *positions,
+                              const void *q_norm, const void *k_norm, float eps,
+                              const dqg_quantized_kv *kv, const int32_t *block_table,
+                              int64_t table_width, int64_t table_stride, const int32_t *open_slots,
+                              const int32_t *q_starts, const int32_t *kv_lens, int64_t n_seqs,
+                              void *q_out, void *stream);
+
+/*
+ * The listed sequences' positions as 16-bit pages: k_out and v_out [n_pages,
+ * n_kv_heads, page_size, head_dim] (contiguous, of the type `dtype`) take one
+ * sequence's pages after the other's, each value rounded once and zeros behind
+ * a sequence's end, and table_out [n_seqs, table_width] (contiguous) says
+ * where they lie, so that the operators over 16-bit pages can read them.
+ * n_pages is what the caller has room for: pages beyond it are left out (-1 in
+ * table_out), which sets bit 1 of dqg_device_status; pages that no sequence
+ * takes are left as they were.
+ */
+int dqg_expand_pages(const dqg_quantized_kv *kv, const int32_t *block_table, int64_t table_width,
+                     int64_t table_stride, const int32_t *open_slots, const int32_t *kv_lens,
+                     int64_t n_seqs, int64_t n_pages, void *k_out, void *v_out, int32_t *table_out,
+                     void *stream);
+
+/*
+ * dqg_paged_attention over such a cache. Products use the codes as they are
+ * (exact in 16 bits); scales are applied to scores and weights in fp32.
+ */
+int dqg_quantized_attention_workspace(int64_t n_seqs, int64_t n_q_heads, int64_t n_kv_heads,
+                                      int64_t head_dim, uint64_t *bytes);
+int dqg_quantized_attention(const void *q, int64_t q_stride_seq, int64_t q_stride_head,
+                            int64_t n_seqs, int64_t n_q_heads, const dqg_quantized_kv *kv,
+                            const int32_t *block_table, int64_t table_width, int64_t table_stride,
+                            const int32_t *open_slots, const int32_t *kv_lens, float scale,
+                            void *out, void *workspace, uint64_t workspace_bytes, void *stream);
+
+/*
+ * Draws a token from each row of logits [rows, vocab] (fp16, bf16 or fp32;
+ * rows row_stride elements apart), from one given random number in [0, 1) a
+ * row. With m the row's largest logit and T its temperature, w_i =
+ * exp((l_i - m) / T); tokens rank by logit, the lower index first. Kept are
+ * those of rank below top_k (0 or less: all), with min_p <= w_i, and with the
+ * w of those that top_k keeps and that rank before them below top_p of top_k's
+ * sum (1 or more: all). The token is the first, by index, whose running sum of
+ * kept w exceeds uniform * their sum (the last kept one if none does), and
+ * logprob the logarithm of its w over that sum. A temperature of 0 (or less,
+ * or NaN) takes the largest logit of lowest index, with logprob 0. NaN counts
+ * as -inf; where the largest logit is +inf only such are kept; a row without
+ * a logit above -inf gives token -1 and logprob NaN. The sums are taken over
+ * 64-bit integers (w in units of 2^-44), so that they do not depend on an
+ * order. Each parameter is an array of `rows` (temperatures, top_ks, top_ps,
+ * min_ps on the device) or, where that is NULL, the value beside it.
+ */
+enum { DQG_FP32 = 2 };
+typedef struct dqg_sampling {
+  const float *temperatures;
+  const int32_t *top_ks;
+  const float *top_ps;
+  const float *min_ps;
+  float temperature;
+  int32_t top_k;
+  float top_p;
+  float min_p;
+} dqg_sampling;
+int dqg_sample_tokens(const void *logits, int32_t dtype, int64_t rows, int64_t vocab,
+                      int64_t row_stride, const float *uniform, const dqg_sampling *params,
+                      int64_t *tokens, float *logprobs, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
