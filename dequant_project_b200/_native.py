@@ -158,6 +158,8 @@ def lib() -> ctypes.CDLL:
     h.dqg_quantized_attention_workspace.argtypes = [i64, i64, i64, i64, u64p]
     h.dqg_quantized_attention.restype = i32
     h.dqg_quantized_attention.argtypes = [vp, i64, i64, i64, i64, qkv, vp, i64, i64, vp, vp, f32, vp, vp, u64, vp]
+    h.dqg_debug_quantized_starved.restype = i32
+    h.dqg_debug_quantized_starved.argtypes = [*h.dqg_quantized_attention.argtypes[:-1], ctypes.c_uint32, u64, vp]
     h.dqg_sample_tokens.restype = i32
     h.dqg_sample_tokens.argtypes = [vp, ctypes.c_int32, i64, i64, i64, vp, ctypes.POINTER(Sampling), vp, vp, vp]
     _lib = h
@@ -176,7 +178,7 @@ EXPORTED = ("dqg_last_error", "dqg_version", "dqg_add_one", "dqg_gemv", "dqg_deq
             "dqg_paged_attention", "dqg_prompt_attention_workspace", "dqg_prompt_attention",
             "dqg_shared_prefix_workspace", "dqg_shared_prefix_attention", "dqg_debug_paged_starved",
             "dqg_rope_quantized_append", "dqg_expand_pages", "dqg_quantized_attention_workspace",
-            "dqg_quantized_attention", "dqg_sample_tokens")
+            "dqg_quantized_attention", "dqg_debug_quantized_starved", "dqg_sample_tokens")
 
 
 def check(rc: int) -> None:

@@ -91,10 +91,11 @@ inline EncodeFn encode_fn() {
 }
 
 // A 4-dimensional map of `bytes`-byte values: sizes innermost first, strides in
-// elements of the three outer dimensions, 128-byte swizzled boxes of `values`
-// values by `rows1` by `rows2` by `rows3`.
+// elements of the three outer dimensions, swizzled boxes of `values` values by
+// `rows1` by `rows2` by `rows3`.
 inline int make_map(CUtensorMap* map, const void* base, CUtensorMapDataType type, int bytes, const int64_t (&size)[4],
-             const int64_t (&stride)[3], int values, int rows1, int rows2, int rows3, const char* name) {
+             const int64_t (&stride)[3], int values, int rows1, int rows2, int rows3,
+                    CUtensorMapSwizzle swizzle, const char* name) {
   const EncodeFn fn = encode_fn();
   if (fn == nullptr) return api_fail(DQG_ERR_UNSUPPORTED, "the driver has no cuTensorMapEncodeTiled");
   cuuint64_t dims[4], strides[3];
@@ -104,7 +105,7 @@ inline int make_map(CUtensorMap* map, const void* base, CUtensorMapDataType type
                              static_cast<cuuint32_t>(rows2), static_cast<cuuint32_t>(rows3)};
   const cuuint32_t one[4] = {1, 1, 1, 1};
   const CUresult r = fn(map, type, 4, const_cast<void*>(base), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS)
     return api_fail(DQG_ERR_INVALID, "%s: no tensor map for these sizes and strides (%d)", name,

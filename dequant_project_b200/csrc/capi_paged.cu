@@ -54,7 +54,7 @@ int check_pool(const dqg_paged_kv* kv, dqg::PagedPool* pool) {
 int pool_map(CUtensorMap* map, const void* base, const dqg::PagedPool& pool, const int64_t (&size)[4],
              const int64_t (&stride)[3], int rows1, int rows2, int rows3, const char* name) {
   return make_map(map, base, pool.bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, size,
-                  stride, 64, rows1, rows2, rows3, name);
+                  stride, 64, rows1, rows2, rows3, CU_TENSOR_MAP_SWIZZLE_128B, name);
 }
 
 int pool_maps(const dqg::PagedPool& pool, int rows, CUtensorMap* k, CUtensorMap* v) {

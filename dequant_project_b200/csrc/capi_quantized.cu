@@ -191,16 +191,18 @@ int dqg_quantized_attention_workspace(int64_t n_seqs, int64_t n_q_heads, int64_t
   if (n_seqs < 0 || n_seqs > (1 << 20)) return api_fail(DQG_ERR_INVALID, "n_seqs=%lld out of range", (ll)n_seqs);
   int dev = 0, sms = 0;
   if ((rc = current(&dev, &sms)) != DQG_OK) return rc;
-  *bytes = dqg::quantized_attention_workspace(static_cast<int>(n_seqs), static_cast<int>(n_q_heads),
-                                              static_cast<int>(n_kv_heads), static_cast<int>(head_dim), sms);
+  *bytes = dqg::quantized_attention_workspace(static_cast<int>(n_q_heads), static_cast<int>(n_kv_heads),
+                                              static_cast<int>(head_dim), sms);
   return api_ok();
 }
 
-int dqg_quantized_attention(const void* q, int64_t q_stride_seq, int64_t q_stride_head, int64_t n_seqs,
-                            int64_t n_q_heads, const dqg_quantized_kv* kv, const int32_t* block_table,
-                            int64_t table_width, int64_t table_stride, const int32_t* open_slots,
-                            const int32_t* kv_lens, float scale, void* out, void* workspace, uint64_t workspace_bytes,
-                            void* stream) {
+}  // extern "C"
+
+namespace {
+int quantized_attention(const void* q, int64_t q_stride_seq, int64_t q_stride_head, int64_t n_seqs, int64_t n_q_heads,
+                        const dqg_quantized_kv* kv, const int32_t* block_table, int64_t table_width,
+                        int64_t table_stride, const int32_t* open_slots, const int32_t* kv_lens, float scale, void* out,
+                        void* workspace, uint64_t workspace_bytes, uint32_t starved, uint64_t wait_ns, void* stream) {
   dqg::QuantizedPool pool;
   dqg::QuantizedSeqs seqs;
   int rc = check_quantized(kv, &pool);
@@ -215,9 +217,18 @@ int dqg_quantized_attention(const void* q, int64_t q_stride_seq, int64_t q_strid
   if ((rc = check_scale(scale)) != DQG_OK) return rc;
   int dev = 0, sms = 0;
   if ((rc = current(&dev, &sms)) != DQG_OK) return rc;
-  const uint64_t need = dqg::quantized_attention_workspace(seqs.B, static_cast<int>(n_q_heads), pool.n_kv_heads,
-                                                           pool.D, sms);
+  const uint64_t need = dqg::quantized_attention_workspace(static_cast<int>(n_q_heads), pool.n_kv_heads, pool.D, sms);
   if ((rc = check_workspace(workspace, workspace_bytes, need)) != DQG_OK) return rc;
+  const int64_t size[4] = {pool.D, pool.page_size, pool.n_kv_heads, pool.n_pages};
+  const int64_t stride[3] = {pool.row_stride, pool.head_stride, pool.page_stride};
+  const int rows = dqg::quantized_box_rows(pool.page_size);
+  const CUtensorMapSwizzle swizzle = pool.D == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B;
+  CUtensorMap kmap, vmap;
+  if ((rc = make_map(&kmap, pool.k, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, size, stride, pool.D, rows, 1, 1, swizzle, "k")) !=
+          DQG_OK ||
+      (rc = make_map(&vmap, pool.v, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, size, stride, pool.D, rows, 1, 1, swizzle, "v")) !=
+          DQG_OK)
+    return rc;
   dqg::QuantizedAttentionArgs a;
   a.q = q;
   a.q_stride_seq = q_stride_seq;
@@ -226,9 +237,37 @@ int dqg_quantized_attention(const void* q, int64_t q_stride_seq, int64_t q_strid
   a.workspace = workspace;
   a.hq = static_cast<int>(n_q_heads);
   a.scale = scale;
-  const cudaError_t e = dqg::launch_quantized_attention(pool, seqs, a, sms, static_cast<cudaStream_t>(stream));
+  a.starved = starved;
+  a.wait_ns = wait_ns;
+  const cudaError_t e =
+      dqg::launch_quantized_attention(pool, seqs, kmap, vmap, a, sms, static_cast<cudaStream_t>(stream));
   if (e != cudaSuccess) return api_cuda_fail(e, "quantized_attention launch");
   return api_ok();
+}
+}  // namespace
+
+extern "C" {
+
+int dqg_quantized_attention(const void* q, int64_t q_stride_seq, int64_t q_stride_head, int64_t n_seqs,
+                            int64_t n_q_heads, const dqg_quantized_kv* kv, const int32_t* block_table,
+                            int64_t table_width, int64_t table_stride, const int32_t* open_slots,
+                            const int32_t* kv_lens, float scale, void* out, void* workspace, uint64_t workspace_bytes,
+                            void* stream) {
+  return quantized_attention(q, q_stride_seq, q_stride_head, n_seqs, n_q_heads, kv, block_table, table_width,
+                             table_stride, open_slots, kv_lens, scale, out, workspace, workspace_bytes, 0, 0, stream);
+}
+
+int dqg_debug_quantized_starved(const void* q, int64_t q_stride_seq, int64_t q_stride_head, int64_t n_seqs,
+                                int64_t n_q_heads, const dqg_quantized_kv* kv, const int32_t* block_table,
+                                int64_t table_width, int64_t table_stride, const int32_t* open_slots,
+                                const int32_t* kv_lens, float scale, void* out, void* workspace,
+                                uint64_t workspace_bytes, uint32_t starved, uint64_t wait_ns, void* stream) {
+  if (wait_ns < 1000000ull || wait_ns > 1000000000ull)
+    return api_fail(DQG_ERR_INVALID, "wait_ns must be in [1 ms, 1 s], got %llu", (unsigned long long)wait_ns);
+  if (starved < 1 || starved > 511) return api_fail(DQG_ERR_INVALID, "starved must be in [1, 511], got %u", starved);
+  return quantized_attention(q, q_stride_seq, q_stride_head, n_seqs, n_q_heads, kv, block_table, table_width,
+                             table_stride, open_slots, kv_lens, scale, out, workspace, workspace_bytes, starved,
+                             wait_ns, stream);
 }
 
 }  // extern "C"

@@ -63,10 +63,15 @@ struct QuantizedAttentionArgs {
   void* workspace;
   int hq;
   float scale;
+  uint64_t wait_ns;  // limit of a wait; 0: the library's
+  uint32_t starved;  // diagnostic: bit w < 8, consumer warp w gives up at once; bit 8, nothing is copied
 };
-size_t quantized_attention_workspace(int B, int hq, int n_kv_heads, int D, int num_sms);
-cudaError_t launch_quantized_attention(const QuantizedPool& pool, const QuantizedSeqs& seqs,
-                                       const QuantizedAttentionArgs& a, int num_sms, cudaStream_t stream);
+// Rows of the tensor maps' boxes for the kernel's tiles.
+int quantized_box_rows(int page_size);
+size_t quantized_attention_workspace(int hq, int n_kv_heads, int D, int num_sms);
+cudaError_t launch_quantized_attention(const QuantizedPool& pool, const QuantizedSeqs& seqs, const CUtensorMap& kmap,
+                                       const CUtensorMap& vmap, const QuantizedAttentionArgs& a, int num_sms,
+                                       cudaStream_t stream);
 
 cudaError_t read_status_quantized_append(uint32_t* status, bool reset);
 cudaError_t read_status_expand(uint32_t* status, bool reset);

@@ -1,5 +1,6 @@
 // Decode attention over a cache held in 8 bits: one query token per sequence,
-// lengths on the device, grouped KV heads.
+// lengths on the device, grouped KV heads. No reference counterpart (the
+// reference models the cache's bytes, dequant/byte_model.py:214-219).
 //
 //   o[b, h] = sum_t p_t s_v(t) code_v(t) / sum_t p_t,
 //   p_t = exp(scale s_k(t) q[b, h] . code_k(t) - m)
@@ -7,139 +8,719 @@
 // over the complete blocks of sequence b and then the 16-bit rows of its open
 // block (s = 1); zero where there is none.
 //
-// A block takes one query head of one sequence, its warps every fourth
-// position; a lane holds D / 32 values of the query and of the sum.
+// The work is cut as in paged_attention.cu (paged_decode.cuh): equal shares of
+// tiles of 128 positions, pieces of cut items joined in order by a second
+// kernel. One warp copies a tile's code rows by tensor-map boxes and its
+// scales by cp.async into a ring; eight warps take 16 positions each, which
+// lie in one block, so that a warp's scales are two numbers. Positions are the
+// m side of mma.m16n8k16 and query heads its n side (8 of them, or 16 in two
+// products): S = K Q^T, then O^T += V^T P, with the weights transposed between
+// by movmatrix. With heads on the m side, as in the 16-bit kernel, half or more
+// of the products' rows and of the accumulators would be empty for the usual
+// one to eight heads a KV head.
+//
+// Codes are read from shared memory sixteen bytes a lane and become fp16 in
+// registers, exactly (int8: the byte in the mantissa of 1024, less 1152; e4m3:
+// one conversion for two), in whatever order of the summed index that gives,
+// the queries' being the same. bf16 queries become fp16 times a power of two
+// for each head, the largest between 2^14 and 2^15: what that loses is below
+// 2^-39 of the largest. Scores are scaled in fp32. So are the weights: besides
+// the softmax's reference (of the scores) the sum over values has one of its
+// own, of the score plus log2 s_v, so that a 16-bit weight is relative to the
+// largest p s_v met, whatever the blocks' scales are. Both references move, and
+// the sums are rescaled, only when a slice exceeds one by more than 2^kMaxGrowth;
+// of fp16's range (2^-24 to 2^16) a weight loses below 2^-32 of the largest.
+// Open rows go through products of their own type.
+//
+// Waits are bounded, as in paged_attention.cu: a consumer warp whose wait ran
+// out goes on without data and makes its results NaN.
 #include <cstdint>
 
+#include "paged_decode.cuh"
 #include "quantized.cuh"
 
 namespace dqg {
 namespace {
 
-constexpr int kWarps = 4;
+constexpr int kTile = 128;             // positions per tile
+constexpr int kWarps = 8;              // consumer warps, 16 positions each
+constexpr int kThreads = 32 * (kWarps + 1);
+constexpr int kQuerySlots = 4;         // items whose queries are held at most
+constexpr int kMergeRows = 2;          // query heads per round of the warps' merge
+constexpr int kScales = kTile / 16;    // scales a tile, of keys; as many of values
+constexpr float kMaxGrowth = 8.f, kHeadroom = 7.f;  // log2 units
 
-struct Params {
-  QuantizedPool pool;
-  QuantizedSeqs seqs;
-  const void* q;
-  void* out;
-  int64_t q_stride_seq, q_stride_head;
-  int hq, g, page_shift, block_shift, len_limit;
-  float scale_log2;
+struct Params : DecodeParams {
+  const float* k_scale;
+  const float* v_scale;
+  const void* k_open;
+  const void* v_open;
+  const int32_t* open_slots;
+  int64_t scale_page_stride, scale_head_stride, open_stride, open_head_stride, n_open;
+  int block_shift;
 };
 
-template <typename E, class Code, int D>
-__global__ void __launch_bounds__(32 * kWarps) quantized_attention_kernel(const __grid_constant__ Params p) {
-  constexpr int kPer = D / 32;
-  __shared__ float s_o[kWarps][D], s_m[kWarps], s_l[kWarps];
-  pdl_wait_prior_grid();
-  pdl_launch_dependents();
-  const int b = blockIdx.y, h = blockIdx.x, kvh = h / p.g, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int len = clamped_len(p.seqs.lens, b, p.len_limit), done = len >> p.block_shift << p.block_shift;
-  if (threadIdx.x == 0 && __ldg(p.seqs.lens + b) != len) atomicOr(&g_status, kStatusBadIndex);
-  const int64_t slot = __ldg(p.seqs.open_slots + b);
-  const bool open = slot >= 0 && slot < p.pool.n_open;
-  if (threadIdx.x == 0 && !open && done < len) atomicOr(&g_status, kStatusBadIndex);
-  const E* q = static_cast<const E*>(p.q) + b * p.q_stride_seq + h * p.q_stride_head + lane * kPer;
-  float qv[kPer], o[kPer], m = -INFINITY, l = 0.f;
-  for (int i = 0; i < kPer; ++i) {
-    qv[i] = Elem<E>::load(q + i) * p.scale_log2;
-    o[i] = 0.f;
+// Tiles of complete blocks, and one of the open block's rows.
+__device__ __forceinline__ int tiles_of(const Params& p, int len) {
+  const int open = len & ((1 << p.block_shift) - 1);
+  return max(1, (len - open + kTile - 1) / kTile + (open ? 1 : 0));
+}
+
+__device__ __forceinline__ uint4 lds128(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
+  return v;
+}
+__device__ __forceinline__ uint2 lds64(uint32_t addr) {
+  uint2 v;
+  asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr));
+  return v;
+}
+__device__ __forceinline__ uint32_t transposed(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+__device__ __forceinline__ float log2_approx(float x) {
+  float y;
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
+// Arrives once this thread's earlier cp.async copies are complete.
+__device__ __forceinline__ void cp_async_arrive(uint64_t* bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+
+// Four codes as two pairs of fp16 values: bytes (0, 2) and (1, 3) where
+// kStride is 2, (0, 1) and (2, 3) where it is 1. kUnit: what the values have to
+// be multiplied by.
+template <class Code>
+struct Pairs;
+template <>
+struct Pairs<Int8> {
+  static constexpr int kStride = 2;
+  static __device__ __forceinline__ void expand(uint32_t w, uint32_t& a, uint32_t& b) {
+    constexpr uint32_t kLess1152 = 0xe480e480u;  // 1024 + 128, of codes taken as unsigned
+    a = hadd2_u32((w & 0x00ff00ffu) ^ 0x64806480u, kLess1152);
+    b = hadd2_u32(((w >> 8) & 0x00ff00ffu) ^ 0x64806480u, kLess1152);
   }
-  for (int t = warp; t < len; t += kWarps) {
-    float k[kPer], v[kPer];
-    if (t < done) {
-      const int page = __ldg(p.seqs.table + b * p.seqs.table_stride + (t >> p.page_shift));
-      const int row = t & ((1 << p.page_shift) - 1);
-      const bool good = page >= 0 && page < p.pool.n_pages;
-      if (!good && lane == 0) atomicOr(&g_status, kStatusBadIndex);
-      const int64_t at = page * p.pool.page_stride + kvh * p.pool.head_stride + row * p.pool.row_stride + lane * kPer;
-      const int64_t sc = page * p.pool.scale_page_stride + kvh * p.pool.scale_head_stride + (row >> p.block_shift);
-      float f[4];
-      for (int which = 0; which < 2; ++which) {
-        const uint8_t* codes = static_cast<const uint8_t*>(which ? p.pool.v : p.pool.k);
-        const float s = good ? __ldg((which ? p.pool.v_scale : p.pool.k_scale) + sc) : 0.f;
-        uint32_t w = 0;
-        if (good)
-          for (int i = 0; i < kPer; ++i) w |= static_cast<uint32_t>(codes[at + i]) << (8 * i);
-        Code::unpack4(w, f);
-        for (int i = 0; i < kPer; ++i) (which ? v : k)[i] = f[i] * s;
-      }
-    } else {
-      const int64_t at = slot * p.pool.open_stride + kvh * p.pool.open_head_stride + (t - done) * D + lane * kPer;
-      for (int i = 0; i < kPer; ++i) {
-        k[i] = open ? Elem<E>::load(static_cast<const E*>(p.pool.k_open) + at + i) : 0.f;
-        v[i] = open ? Elem<E>::load(static_cast<const E*>(p.pool.v_open) + at + i) : 0.f;
-      }
+};
+template <>
+struct Pairs<E4m3> {
+  static constexpr int kStride = 1;
+  static __device__ __forceinline__ void expand(uint32_t w, uint32_t& a, uint32_t& b) {
+    a = E4m3::half2(w);
+    b = E4m3::half2(w >> 16);
+  }
+};
+
+// Row of a tile that row n of a product takes: conflict-free reads of sixteen
+// bytes a lane by eight rows of four lanes (keys) as by four of eight (values).
+__device__ __forceinline__ int row_of(int n) { return n ^ ((n & 1) << 2); }
+
+// Byte offset of 16-byte chunk `chunk` of code row `row`, swizzled as the
+// tensor map writes it (128 bytes for rows of 128, 64 for rows of 64).
+template <int D>
+__device__ __forceinline__ uint32_t code_off(int row, int chunk) {
+  return D == 128 ? row * 128 + ((chunk ^ (row & 7)) << 4) : row * 64 + ((chunk ^ ((row >> 1) & 3)) << 4);
+}
+
+template <int D, int NB>
+struct Layout {
+  static constexpr int kCtasPerSm = NB == 1 ? 2 : 1;
+  static constexpr int kStages = NB == 1 ? 3 : 6;
+  static constexpr int kTileBytes = kTile * D;  // and as many hold 64 open rows
+  static constexpr int kRing = kStages * 2 * kTileBytes;
+  static constexpr int kQuery = 16 * D * 2;
+  static constexpr int kMerge = kWarps * kMergeRows * D * 4;
+  static constexpr int kStats = 3 * kWarps * 16 * 4;
+  static constexpr int kScaleBytes = kStages * 2 * kScales * 4;
+  static constexpr int kSmem =
+      1024 + kRing + kQuery + kMerge + kStats + kScaleBytes + 2 * (kStages + kQuerySlots) * 8 + static_cast<int>(sizeof(Share));
+};
+
+template <typename E, class Code, int D, int NB>
+__global__ void __launch_bounds__(kThreads, Layout<D, NB>::kCtasPerSm)
+    quantized_decode_kernel(const __grid_constant__ Params p, const __grid_constant__ CUtensorMap kmap,
+                            const __grid_constant__ CUtensorMap vmap) {
+  using L = Layout<D, NB>;
+  constexpr int kStages = L::kStages;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
+  // Queries of the items ahead; reads of 8 or 16 rows run past a short slot, at
+  // worst into the merge buffer (columns whose results nobody takes).
+  uint8_t* qs = smem + L::kRing;
+  float* os = reinterpret_cast<float*>(qs + L::kQuery);          // [warp][kMergeRows][D]
+  float* ms = os + L::kMerge / 4;                                // [warp][16]: the scores' reference,
+  float* vs = ms + kWarps * 16;                                  // the values',
+  float* ls = vs + kWarps * 16;                                  // and the sum
+  float* scales = ls + kWarps * 16;                              // [stage][2][kScales]
+  uint64_t* full = reinterpret_cast<uint64_t*>(scales + L::kScaleBytes / 4);
+  uint64_t* empty = full + kStages;
+  uint64_t* q_full = empty + kStages;
+  uint64_t* q_empty = q_full + kQuerySlots;
+  Share* share = reinterpret_cast<Share*>(q_empty + kQuerySlots);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kStages; ++i) {
+      mbar_init(full + i, 1 + 2 * kScales);
+      mbar_init(empty + i, kWarps);
     }
-    float s = 0.f;
-    for (int i = 0; i < kPer; ++i) s = fmaf(qv[i], k[i], s);
-    for (int off = 16; off >= 1; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
-    const float mx = fmaxf(m, s), f = exp2f(m - mx), w = exp2f(s - mx);
-    l = fmaf(l, f, w);
-    for (int i = 0; i < kPer; ++i) o[i] = fmaf(o[i], f, w * v[i]);
-    m = mx;
+    for (int i = 0; i < kQuerySlots; ++i) {
+      mbar_init(q_full + i, 1);
+      mbar_init(q_empty + i, kWarps);
+    }
+    fence_mbar_init();
+    tma_prefetch_map(&kmap);
+    tma_prefetch_map(&vmap);
   }
-  for (int i = 0; i < kPer; ++i) s_o[warp][lane * kPer + i] = o[i];
-  if (lane == 0) {
-    s_m[warp] = m;
-    s_l[warp] = l;
+  pdl_wait_prior_grid();
+  if (warp == 0) {
+    const Share s = find_share(p, blockIdx.x, gridDim.x);
+    if (lane == 0) *share = s;
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < D; i += 32 * kWarps) {
-    float mx = -INFINITY, den = 0.f, num = 0.f;
-    for (int w = 0; w < kWarps; ++w) mx = fmaxf(mx, s_m[w]);
-    for (int w = 0; w < kWarps; ++w) {
-      const float f = s_l[w] == 0.f ? 0.f : exp2f(s_m[w] - mx);
-      den = fmaf(s_l[w], f, den);
-      num = fmaf(s_o[w][i], f, num);
+  pdl_launch_dependents();
+  Share s = *share;
+  const int q_rows = min(16, p.g), q_slots = min(kQuerySlots, 16 / q_rows);
+  const int block = 1 << p.block_shift;
+
+  if (warp == kWarps) {
+    // ---- the copying warp.
+    const int per = p.box_rows, boxes = kTile / per;  // rows a box; boxes a tile, of keys and of values
+    const uint64_t policy = policy_evict_last();
+    int it = 0, item = 0;
+    bool ok = !(p.starved >> kWarps & 1);
+    while (s.count > 0 && ok) {
+      const Item i = item_of(p, s);
+      if (i.x1 == i.x0) {  // the cut falls before its first tile
+        advance(p, s, i.units);
+        continue;
+      }
+      const int done = i.len & ~(block - 1), whole = (done + kTile - 1) / kTile;
+      if (lane == 0 && __ldg(p.lens + s.b) != i.len) atomicOr(&g_status, kStatusBadIndex);
+      const int qi = item % q_slots;
+      if (item >= q_slots && !warp_wait(q_empty + qi, ((item / q_slots) & 1) ^ 1, p.wait_ns)) break;
+      if (lane == 0) mbar_arrive_expect_tx(q_full + qi, i.rows * D * 2);
+      __syncwarp();
+      if (lane < i.rows)
+        bulk_g2s(qs + (qi * q_rows + lane) * D * 2, static_cast<const E*>(p.q) + s.b * p.q_stride_seq +
+                 (i.head0 + lane) * p.q_stride_head, D * 2, q_full + qi, policy);
+      ++item;
+      for (int x = i.x0; x < i.x1; ++x, ++it) {
+        const int st = it % kStages;
+        uint8_t* dst = smem + st * 2 * L::kTileBytes;
+        if (x < whole || i.len == done) {
+          auto page_at = [&](int t) {
+            int page = static_cast<int>(p.n_pages);  // no such page: zeros
+            if (t < done) {
+              page = __ldg(i.table + (t >> p.page_shift));
+              if (page < 0 || page >= p.n_pages) {
+                page = static_cast<int>(p.n_pages);
+                atomicOr(&g_status, kStatusBadIndex);
+              }
+            }
+            return page;
+          };
+          const int t = x * kTile + lane * per;
+          const int page = lane < boxes ? page_at(t) : 0;
+          // A lane a scale: of keys, then of values.
+          const int j = lane % kScales, ts = x * kTile + (j << p.block_shift);
+          const bool scaled = lane < 2 * kScales && j < kTile >> p.block_shift;
+          const int sp = scaled ? page_at(ts) : static_cast<int>(p.n_pages);
+          if (it >= kStages && !warp_wait(empty + st, ((it / kStages) & 1) ^ 1, p.wait_ns)) {
+            ok = false;
+            break;
+          }
+          if (lane == 0) mbar_arrive_expect_tx(full + st, 2 * L::kTileBytes);
+          __syncwarp();
+          if (lane < boxes) {
+            const int in_page = t & ((1 << p.page_shift) - 1);
+            tma_load_4d(smem_u32(dst) + lane * per * D, &kmap, full + st, 0, in_page, i.kvh, page);
+            tma_load_4d(smem_u32(dst) + L::kTileBytes + lane * per * D, &vmap, full + st, 0, in_page, i.kvh, page);
+          }
+          if (lane < 2 * kScales) {
+            float* to = scales + st * 2 * kScales + lane;
+            if (sp < p.n_pages) {
+              cp_async4(smem_u32(to), (lane < kScales ? p.k_scale : p.v_scale) + sp * p.scale_page_stride +
+                        i.kvh * p.scale_head_stride + ((ts & ((1 << p.page_shift) - 1)) >> p.block_shift));
+            } else {
+              *to = 0.f;
+            }
+            cp_async_arrive(full + st);
+          }
+        } else {
+          // The open rows, as they are.
+          const int rows = i.len - done;
+          const int64_t slot = __ldg(p.open_slots + s.b);
+          const bool good = slot >= 0 && slot < p.n_open;
+          if (it >= kStages && !warp_wait(empty + st, ((it / kStages) & 1) ^ 1, p.wait_ns)) {
+            ok = false;
+            break;
+          }
+          if (!good) {
+            for (int c = lane; c < 2 * L::kTileBytes / 16; c += 32) reinterpret_cast<uint4*>(dst)[c] = make_uint4(0, 0, 0, 0);
+            if (lane == 0) atomicOr(&g_status, kStatusBadIndex);
+            __syncwarp();
+            fence_async_shared();  // before the ring's next copy to this place
+          }
+          if (lane == 0) {
+            mbar_arrive_expect_tx(full + st, good ? 2 * rows * D * 2 : 0);
+            if (good) {
+              const int64_t at = slot * p.open_stride + i.kvh * p.open_head_stride;
+              bulk_g2s(dst, static_cast<const E*>(p.k_open) + at, rows * D * 2, full + st, policy);
+              bulk_g2s(dst + L::kTileBytes, static_cast<const E*>(p.v_open) + at, rows * D * 2, full + st, policy);
+            }
+          }
+          __syncwarp();
+          if (lane < 2 * kScales) mbar_arrive(full + st);
+        }
+      }
+      advance(p, s, i.units);
     }
-    const float x = den == 0.f ? 0.f : num / den;
-    static_cast<E*>(p.out)[(static_cast<int64_t>(b) * p.hq + h) * D + i] =
-        reinterpret_cast<const E&>(static_cast<const uint16_t&>(static_cast<uint16_t>(Elem<E>::pack(x, 0.f))));
+    // Copies still in flight land before the CTA's memory goes (bounded).
+    for (int i = item < q_slots ? 0 : item - q_slots; i < item; ++i)
+      if (!warp_wait(q_full + i % q_slots, (i / q_slots) & 1, p.wait_ns)) break;
+    for (int i = it < kStages ? 0 : it - kStages; i < it; ++i)
+      if (!warp_wait(full + i % kStages, (i / kStages) & 1, p.wait_ns)) break;
+  } else {
+    const int gid = lane >> 2, c = lane & 3;
+    const uint32_t ring = smem_u32(smem);
+    const int p0 = warp * 16;
+    int it = 0, item = 0;
+    // Once a wait has run out no later one is taken.
+    bool ok = !(p.starved >> warp & 1), cut_first = false;
+    auto await = [&](uint64_t* bar, uint32_t parity) { return ok = ok && warp_wait(bar, parity, p.wait_ns); };
+    while (s.count > 0) {
+      const Item i = item_of(p, s);
+      if (i.x1 == i.x0) {
+        advance(p, s, i.units);
+        continue;
+      }
+      const int done = i.len & ~(block - 1), whole = (done + kTile - 1) / kTile;
+      const int qi = item % q_slots;
+      await(q_full + qi, (item / q_slots) & 1);
+      // Queries as B fragments: columns are heads; a lane holds the values at
+      // 64 h + 16 c to + 15, four a product.
+      uint32_t qf[NB][D / 16][2];
+      float unit[NB][2];  // what scores of heads 2 c and 2 c + 1 are multiplied by, but for the block's scale
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) {
+        const uint32_t row = smem_u32(qs) + (qi * q_rows + nb * 8 + gid) * (D * 2) + c * 32;
+        uint32_t w[D / 8];
+        uint32_t most = 0;
+#pragma unroll
+        for (int h = 0; h < D / 32; ++h) {
+          const uint4 v = lds128(row + (h >> 1) * 128 + (h & 1) * 16);
+          w[4 * h] = v.x;
+          w[4 * h + 1] = v.y;
+          w[4 * h + 2] = v.z;
+          w[4 * h + 3] = v.w;
+        }
+        float f = p.scale_log2;
+        if (Elem<E>::kFormat == 1) {
+          // bf16 to fp16, times a power of two for the head.
+#pragma unroll
+          for (int h = 0; h < D / 8; ++h) most = __vmaxu2(most, w[h] & 0x7fff7fffu);
+          most = max(most & 0xffffu, most >> 16);
+          most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
+          most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
+          const int e = min(max(static_cast<int>(most >> 7), 20), 240);  // exponent of the largest, biased
+          const float up = __uint_as_float(static_cast<uint32_t>(127 + 14 + 127 - e) << 23);  // 2^(14 - (e - 127))
+#pragma unroll
+          for (int h = 0; h < D / 8; ++h) {
+            const float2 x = Elem<E>::unpack(w[h]);
+            w[h] = Elem<__half>::pack(x.x * up, x.y * up);
+          }
+          f *= __uint_as_float(static_cast<uint32_t>(e - 14) << 23);  // 2^((e - 127) - 14)
+        }
+        unit[nb][0] = __shfl_sync(0xffffffffu, f, 8 * c);  // of lanes with gid = 2 c
+        unit[nb][1] = __shfl_sync(0xffffffffu, f, 8 * c + 4);
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k) {
+          qf[nb][k][0] = Pairs<Code>::kStride == 2 ? prmt(w[2 * k], w[2 * k + 1], 0x5410) : w[2 * k];
+          qf[nb][k][1] = Pairs<Code>::kStride == 2 ? prmt(w[2 * k], w[2 * k + 1], 0x7632) : w[2 * k + 1];
+        }
+      }
+      float o[NB][D / 16][4];
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k) o[nb][k][0] = o[nb][k][1] = o[nb][k][2] = o[nb][k][3] = 0.f;
+      float m[NB][2], mv[NB][2], l[NB][2];  // of heads 2 c and 2 c + 1 (l: this lane's part)
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          m[nb][e] = mv[nb][e] = -INFINITY;
+          l[nb][e] = 0.f;
+        }
+      // Weights of a slice's scores sc (log2 units; entries 2 r + e: row gid + 8 r,
+      // head 2 c + e), for the softmax's sum (into l) and for the values, whose
+      // scale is 2^lv (in place of sc).
+      auto weigh = [&](float (&sc)[NB][4], float lv) {
+        bool grow = false;
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            grow |= sc[nb][e] - m[nb][e & 1] > kMaxGrowth || sc[nb][e] + lv - mv[nb][e & 1] > kMaxGrowth;
+        if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+          for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              float mx = fmaxf(sc[nb][e], sc[nb][e + 2]);
+              mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+              mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+              mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+              // (Each column by itself: those of no head hold anything.)
+              if (mx - m[nb][e] > kMaxGrowth) {
+                l[nb][e] *= exp2_approx(m[nb][e] - mx);
+                m[nb][e] = mx;
+              }
+              if (mx + lv - mv[nb][e] > kMaxGrowth) {
+                const float f = exp2_approx(mv[nb][e] - (mx + lv));
+                mv[nb][e] = mx + lv;
+#pragma unroll
+                for (int k = 0; k < D / 16; ++k) {
+                  o[nb][k][e] *= f;
+                  o[nb][k][e + 2] *= f;
+                }
+              }
+            }
+        }
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const float ref = (m[nb][e] == -INFINITY ? 0.f : m[nb][e]) - kHeadroom;
+            const float ref_v = (mv[nb][e] == -INFINITY ? 0.f : mv[nb][e]) - kHeadroom - lv;
+            l[nb][e] += exp2_approx(sc[nb][e] - ref) + exp2_approx(sc[nb][e + 2] - ref);
+            sc[nb][e] = exp2_approx(sc[nb][e] - ref_v);
+            sc[nb][e + 2] = exp2_approx(sc[nb][e + 2] - ref_v);
+          }
+      };
+      for (int x = i.x0; x < i.x1; ++x, ++it) {
+        const int st = it % kStages;
+        if (!await(full + st, (it / kStages) & 1)) continue;
+        const uint32_t kst = ring + st * 2 * L::kTileBytes, vst = kst + L::kTileBytes;
+        if (x < whole || i.len == done) {
+          if (x * kTile + p0 < done) {
+            const float* sl = scales + st * 2 * kScales + (p0 >> p.block_shift);
+            const float ks = sl[0], lv = log2_approx(sl[kScales]);
+            float sc[NB][4];
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb) sc[nb][0] = sc[nb][1] = sc[nb][2] = sc[nb][3] = 0.f;
+#pragma unroll
+            for (int h = 0; h < D / 64; ++h) {
+              const uint4 a = lds128(kst + code_off<D>(p0 + row_of(gid), c + 4 * h));
+              const uint4 b = lds128(kst + code_off<D>(p0 + 8 + row_of(gid), c + 4 * h));
+              const uint32_t aw[4] = {a.x, a.y, a.z, a.w}, bw[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                uint32_t f[4];
+                Pairs<Code>::expand(aw[k], f[0], f[2]);
+                Pairs<Code>::expand(bw[k], f[1], f[3]);
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb) Elem<__half>::mma(sc[nb], f, qf[nb][4 * h + k][0], qf[nb][4 * h + k][1]);
+              }
+            }
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) sc[nb][e] *= unit[nb][e & 1] * ks;
+            weigh(sc, lv);
+            uint32_t pf[NB][2];
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb) {
+              pf[nb][0] = transposed(Elem<__half>::pack(sc[nb][0], sc[nb][1]));
+              pf[nb][1] = transposed(Elem<__half>::pack(sc[nb][2], sc[nb][3]));
+            }
+            // A lane's D / 8 values of four rows: a word of each gives two
+            // products' halves.
+            constexpr uint32_t kLow = Pairs<Code>::kStride == 2 ? 0x5410 : 0x5140;
+            constexpr uint32_t kHigh = Pairs<Code>::kStride == 2 ? 0x7632 : 0x7362;
+            const int r0 = row_of(2 * c), r1 = row_of(2 * c + 1);
+            uint32_t vw[4][D / 32];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              const int row = p0 + (r & 1 ? r1 : r0) + (r & 2 ? 8 : 0);
+              if (D == 128) {
+                const uint4 v = lds128(vst + code_off<D>(row, gid));
+                vw[r][0] = v.x;
+                vw[r][1] = v.y;
+                vw[r][2 % (D / 32)] = v.z;
+                vw[r][3 % (D / 32)] = v.w;
+              } else {
+                const uint2 v = lds64(vst + code_off<D>(row, gid >> 1) + (gid & 1) * 8);
+                vw[r][0] = v.x;
+                vw[r][1] = v.y;
+              }
+            }
+#pragma unroll
+            for (int k = 0; k < D / 16; ++k) {
+              const uint32_t sel = k & 1 ? kHigh : kLow;
+              uint32_t f[4];
+              Pairs<Code>::expand(prmt(vw[0][k / 2], vw[1][k / 2], sel), f[0], f[1]);
+              Pairs<Code>::expand(prmt(vw[2][k / 2], vw[3][k / 2], sel), f[2], f[3]);
+#pragma unroll
+              for (int nb = 0; nb < NB; ++nb) Elem<__half>::mma(o[nb][k], f, pf[nb][0], pf[nb][1]);
+            }
+          }
+        } else if (p0 < i.len - done) {
+          // Open rows, in their own type: rows of the products are the tile's.
+          const int rows = i.len - done - p0;  // of this warp's 16, or more
+          float sc[NB][4];
+#pragma unroll
+          for (int nb = 0; nb < NB; ++nb) sc[nb][0] = sc[nb][1] = sc[nb][2] = sc[nb][3] = 0.f;
+#pragma unroll
+          for (int k = 0; k < D / 16; ++k) {
+            const uint32_t at = (k / 4) * 128 + c * 32 + (k % 4) * 8;
+            const uint2 a = lds64(kst + (p0 + gid) * (D * 2) + at), b = lds64(kst + (p0 + 8 + gid) * (D * 2) + at);
+            const uint32_t f[4] = {a.x, b.x, a.y, b.y};
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb) {
+              const uint2 w = lds64(smem_u32(qs) + (qi * q_rows + nb * 8 + gid) * (D * 2) + at);
+              Elem<E>::mma(sc[nb], f, w.x, w.y);
+            }
+          }
+#pragma unroll
+          for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sc[nb][e] = gid + 8 * (e >> 1) < rows ? sc[nb][e] * p.scale_log2 : -INFINITY;
+          weigh(sc, 0.f);
+          uint32_t pf[NB][2];
+#pragma unroll
+          for (int nb = 0; nb < NB; ++nb) {
+            pf[nb][0] = transposed(Elem<E>::pack(sc[nb][0], sc[nb][1]));
+            pf[nb][1] = transposed(Elem<E>::pack(sc[nb][2], sc[nb][3]));
+          }
+#pragma unroll
+          for (int k = 0; k < D / 16; ++k) {
+            uint32_t w[4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              // What lies behind the last row may be anything: a zero weight
+              // times an infinity would not be zero.
+              const int row = 2 * c + (r & 1) + (r & 2 ? 8 : 0);
+              w[r] = 0;
+              if (row < rows)
+                asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w[r]) : "r"(vst + (p0 + row) * (D * 2) + gid * (D / 4) + k * 4));
+            }
+            const uint32_t f[4] = {prmt(w[0], w[1], 0x5410), prmt(w[0], w[1], 0x7632), prmt(w[2], w[3], 0x5410),
+                                   prmt(w[2], w[3], 0x7632)};
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb) Elem<E>::mma(o[nb][k], f, pf[nb][0], pf[nb][1]);
+          }
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(empty + st);
+      }
+      // The queries' place is free once their reads have come back, not once
+      // they are issued: here every fragment is used.
+      {
+        uint32_t x = 0;
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+          for (int k = 0; k < D / 16; ++k) x ^= qf[nb][k][0] ^ qf[nb][k][1];
+        asm volatile("" ::"r"(x) : "memory");
+      }
+      __syncwarp();
+      if (ok && lane == 0) mbar_arrive(q_empty + qi);
+      ++item;
+
+      // The item's (or piece's) result: the warps' parts, two heads a round.
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          l[nb][e] += __shfl_xor_sync(0xffffffffu, l[nb][e], 4);
+          l[nb][e] += __shfl_xor_sync(0xffffffffu, l[nb][e], 8);
+          l[nb][e] += __shfl_xor_sync(0xffffffffu, l[nb][e], 16);
+          if (gid == 0) {
+            const int at = warp * 16 + nb * 8 + 2 * c + e;
+            ms[at] = m[nb][e];
+            vs[at] = mv[nb][e];
+            ls[at] = ok ? l[nb][e] : NAN;
+          }
+        }
+      const bool all = i.x0 == 0 && i.x1 == i.tiles;
+      const int64_t row0 = (2 * static_cast<int64_t>(blockIdx.x) + (i.x0 > 0 ? 0 : 1)) * p.rows;
+      if (i.x0 == 0 && !all) {
+        cut_first = true;
+        if (threadIdx.x == 0) {
+          const int last = s.all.holder(s.pos - s.x + i.tiles + p.item_tiles - 1);
+          p.desc[blockIdx.x] = Desc{s.b, s.hv, static_cast<int>(blockIdx.x), last - static_cast<int>(blockIdx.x) + 1};
+        }
+      }
+#pragma unroll
+      for (int r = 0; r < 4 * NB; ++r) {
+        if (2 * r >= i.rows) break;
+        if (c == r % 4) {
+          // Sixteen (or eight) values of a head a lane; their chunks are
+          // swizzled by gid against bank conflicts.
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+#pragma unroll
+            for (int k = 0; k < D / 32; ++k)
+              *reinterpret_cast<float4*>(os + (warp * kMergeRows + e) * D + gid * (D / 8) + (k ^ ((gid >> 1) & (D / 32 - 1))) * 4) =
+                  make_float4(o[r / 4][2 * k][e], o[r / 4][2 * k][e + 2], o[r / 4][2 * k + 1][e], o[r / 4][2 * k + 1][e + 2]);
+        }
+        named_sync(1, 32 * kWarps);
+        for (int cell = threadIdx.x; cell < kMergeRows * (D / 4); cell += 32 * kWarps) {
+          const int j = cell / (D / 4), d4 = cell % (D / 4), row = 2 * r + j;
+          if (row < i.rows) {
+            const int g8 = d4 / (D / 32), at = g8 * (D / 8) + ((d4 ^ ((g8 >> 1) & (D / 32 - 1))) & (D / 32 - 1)) * 4;
+            float mx = -INFINITY;
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) mx = fmaxf(mx, ms[w * 16 + row]);
+            const float mu = mx == -INFINITY ? 0.f : mx;
+            float den = 0.f;
+            float4 num = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) {
+              den = fmaf(ls[w * 16 + row], exp2_approx(ms[w * 16 + row] - mu), den);
+              const float f = exp2_approx(vs[w * 16 + row] - mu);
+              const float4 v = *reinterpret_cast<const float4*>(os + (w * kMergeRows + j) * D + at);
+              num.x = fmaf(v.x, f, num.x);
+              num.y = fmaf(v.y, f, num.y);
+              num.z = fmaf(v.z, f, num.z);
+              num.w = fmaf(v.w, f, num.w);
+            }
+            if (all) {
+              store4<E, D>(p, s.b, i.head0 + row, d4, den, num);
+            } else {
+              *reinterpret_cast<float4*>(p.part + (row0 + row) * D + d4 * 4) = num;
+              if (d4 == 0) {
+                p.m[row0 + row] = mx;
+                p.l[row0 + row] = den;
+              }
+            }
+          }
+        }
+        named_sync(1, 32 * kWarps);
+      }
+      advance(p, s, i.units);
+    }
+    if (threadIdx.x == 0 && !cut_first) p.desc[blockIdx.x] = Desc{0, 0, 0, 0};
   }
 }
 
-template <typename E, class Code>
-cudaError_t launch(const Params& p, cudaStream_t stream) {
+template <typename E, class Code, int D, int NB>
+cudaError_t launch(Params p, const CUtensorMap& kmap, const CUtensorMap& vmap, int num_sms, cudaStream_t stream) {
+  using L = Layout<D, NB>;
+  static int configured[64] = {0};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev < 0 || dev >= 64 || !configured[dev]) {
+    e = cudaFuncSetAttribute(quantized_decode_kernel<E, Code, D, NB>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             L::kSmem);
+    if (e != cudaSuccess) return e;
+    if (dev >= 0 && dev < 64) configured[dev] = 1;
+  }
+  p.n_ctas = L::kCtasPerSm * num_sms;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(p.hq, p.seqs.B);
-  cfg.blockDim = dim3(32 * kWarps);
+  cfg.gridDim = dim3(p.n_ctas);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = L::kSmem;
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return p.pool.D == 128 ? cudaLaunchKernelEx(&cfg, quantized_attention_kernel<E, Code, 128>, p)
-                         : cudaLaunchKernelEx(&cfg, quantized_attention_kernel<E, Code, 64>, p);
+  e = cudaLaunchKernelEx(&cfg, quantized_decode_kernel<E, Code, D, NB>, p, kmap, vmap);
+  if (e != cudaSuccess) return e;
+  return launch_join<E, D>(p, cfg);
+}
+
+template <typename E, class Code>
+cudaError_t launch_for(const Params& p, int D, const CUtensorMap& kmap, const CUtensorMap& vmap, int num_sms,
+                       cudaStream_t stream) {
+  // Heads of a KV head: one product's eight columns, or two's sixteen (and row
+  // blocks of sixteen beyond).
+  if (p.g <= 8)
+    return D == 128 ? launch<E, Code, 128, 1>(p, kmap, vmap, num_sms, stream)
+                    : launch<E, Code, 64, 1>(p, kmap, vmap, num_sms, stream);
+  return D == 128 ? launch<E, Code, 128, 2>(p, kmap, vmap, num_sms, stream)
+                  : launch<E, Code, 64, 2>(p, kmap, vmap, num_sms, stream);
+}
+
+struct Scratch {
+  size_t rows, descs;
+  int per_piece;
+};
+Scratch scratch_of(int hq, int n_kv_heads, int num_sms) {
+  const int g = hq / n_kv_heads, g16 = g < 16 ? g : 16;
+  const size_t ctas = 2 * static_cast<size_t>(num_sms);
+  return Scratch{2 * ctas * g16, ctas, g16};
 }
 
 }  // namespace
 
-size_t quantized_attention_workspace(int, int, int, int, int) { return 16; }
+int quantized_box_rows(int page_size) { return page_size < kTile ? page_size : kTile; }
 
-cudaError_t launch_quantized_attention(const QuantizedPool& pool, const QuantizedSeqs& seqs,
-                                       const QuantizedAttentionArgs& a, int num_sms, cudaStream_t stream) {
-  (void)num_sms;
-  Params p;
-  p.pool = pool;
-  p.seqs = seqs;
+size_t quantized_attention_workspace(int hq, int n_kv_heads, int D, int num_sms) {
+  const Scratch s = scratch_of(hq, n_kv_heads, num_sms);
+  // Descriptions first (16 bytes each), then the rows.
+  return (s.descs * sizeof(Desc) + s.rows * (D + 2) * 4 + 255) / 256 * 256;
+}
+
+cudaError_t launch_quantized_attention(const QuantizedPool& pool, const QuantizedSeqs& seqs, const CUtensorMap& kmap,
+                                       const CUtensorMap& vmap, const QuantizedAttentionArgs& a, int num_sms,
+                                       cudaStream_t stream) {
+  const Scratch s = scratch_of(a.hq, pool.n_kv_heads, num_sms);
+  Params p = {};
   p.q = a.q;
   p.out = a.out;
+  p.table = seqs.table;
+  p.lens = seqs.lens;
+  p.desc = static_cast<Desc*>(a.workspace);
+  p.part = reinterpret_cast<float*>(p.desc + s.descs);
+  p.m = p.part + s.rows * pool.D;
+  p.l = p.m + s.rows;
+  p.rows = s.per_piece;
+  p.pre_seqs = 1;
   p.q_stride_seq = a.q_stride_seq;
   p.q_stride_head = a.q_stride_head;
+  p.table_stride = seqs.table_stride;
+  p.n_pages = pool.n_pages;
+  p.B = seqs.B;
   p.hq = a.hq;
+  p.hkv = pool.n_kv_heads;
   p.g = a.hq / pool.n_kv_heads;
-  p.page_shift = p.block_shift = 0;
+  p.nrb = (p.g + 15) / 16;
   while ((1 << p.page_shift) < pool.page_size) ++p.page_shift;
   while ((1 << p.block_shift) < pool.block) ++p.block_shift;
   const int64_t limit = static_cast<int64_t>(seqs.table_width) * pool.page_size;
   p.len_limit = limit < (1 << 30) ? static_cast<int>(limit) : 1 << 30;
-  p.scale_log2 = a.scale * 1.44269504f;
+  p.box_rows = quantized_box_rows(pool.page_size);
+  p.scale_log2 = static_cast<float>(a.scale * 1.4426950408889634);
+  p.starved = a.starved;
+  p.wait_ns = a.wait_ns ? a.wait_ns : kWaitLimitNs;
+  p.item_tiles = 1;
+  p.n_units32 = static_cast<double>(p.B) * p.hkv * p.nrb * (p.len_limit / kTile + 2 + p.item_tiles) < 2147483648.0;
+  p.k_scale = pool.k_scale;
+  p.v_scale = pool.v_scale;
+  p.k_open = pool.k_open;
+  p.v_open = pool.v_open;
+  p.open_slots = seqs.open_slots;
+  p.scale_page_stride = pool.scale_page_stride;
+  p.scale_head_stride = pool.scale_head_stride;
+  p.open_stride = pool.open_stride;
+  p.open_head_stride = pool.open_head_stride;
+  p.n_open = pool.n_open;
   if (pool.bf16)
-    return pool.e4m3 ? launch<__nv_bfloat16, E4m3>(p, stream) : launch<__nv_bfloat16, Int8>(p, stream);
-  return pool.e4m3 ? launch<__half, E4m3>(p, stream) : launch<__half, Int8>(p, stream);
+    return pool.e4m3 ? launch_for<__nv_bfloat16, E4m3>(p, pool.D, kmap, vmap, num_sms, stream)
+                     : launch_for<__nv_bfloat16, Int8>(p, pool.D, kmap, vmap, num_sms, stream);
+  return pool.e4m3 ? launch_for<__half, E4m3>(p, pool.D, kmap, vmap, num_sms, stream)
+                   : launch_for<__half, Int8>(p, pool.D, kmap, vmap, num_sms, stream);
 }
 
 }  // namespace dqg

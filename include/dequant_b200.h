@@ -529,6 +529,19 @@ int dqg_quantized_attention(const void *q, int64_t q_stride_seq, int64_t q_strid
                             void *out, void *workspace, uint64_t workspace_bytes, void *stream);
 
 /*
+ * Diagnostic for the bounded waits of dqg_quantized_attention, as
+ * dqg_debug_paged_starved (starved, bits 0 to 7: a consumer warp; bit 8: the
+ * copying warp). For tests.
+ */
+int dqg_debug_quantized_starved(const void *q, int64_t q_stride_seq, int64_t q_stride_head,
+                                int64_t n_seqs, int64_t n_q_heads, const dqg_quantized_kv *kv,
+                                const int32_t *block_table, int64_t table_width,
+                                int64_t table_stride, const int32_t *open_slots,
+                                const int32_t *kv_lens, float scale, void *out, void *workspace,
+                                uint64_t workspace_bytes, uint32_t starved, uint64_t wait_ns,
+                                void *stream);
+
+/*
  * Draws a token from each row of logits [rows, vocab] (fp16, bf16 or fp32;
  * rows row_stride elements apart), from one given random number in [0, 1) a
  * row. With m the row's largest logit and T its temperature, w_i =
