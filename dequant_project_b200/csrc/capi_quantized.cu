@@ -221,7 +221,7 @@ int quantized_attention(const void* q, int64_t q_stride_seq, int64_t q_stride_he
   if ((rc = check_workspace(workspace, workspace_bytes, need)) != DQG_OK) return rc;
   const int64_t size[4] = {pool.D, pool.page_size, pool.n_kv_heads, pool.n_pages};
   const int64_t stride[3] = {pool.row_stride, pool.head_stride, pool.page_stride};
-  const int rows = dqg::quantized_box_rows(pool.page_size);
+  constexpr int rows = dqg::kQuantizedBoxRows;
   const CUtensorMapSwizzle swizzle = pool.D == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B;
   CUtensorMap kmap, vmap;
   if ((rc = make_map(&kmap, pool.k, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, size, stride, pool.D, rows, 1, 1, swizzle, "k")) !=
@@ -264,7 +264,7 @@ int dqg_debug_quantized_starved(const void* q, int64_t q_stride_seq, int64_t q_s
                                 uint64_t workspace_bytes, uint32_t starved, uint64_t wait_ns, void* stream) {
   if (wait_ns < 1000000ull || wait_ns > 1000000000ull)
     return api_fail(DQG_ERR_INVALID, "wait_ns must be in [1 ms, 1 s], got %llu", (unsigned long long)wait_ns);
-  if (starved < 1 || starved > 511) return api_fail(DQG_ERR_INVALID, "starved must be in [1, 511], got %u", starved);
+  if (starved < 1 || starved > 255) return api_fail(DQG_ERR_INVALID, "starved must be in [1, 255], got %u", starved);
   return quantized_attention(q, q_stride_seq, q_stride_head, n_seqs, n_q_heads, kv, block_table, table_width,
                              table_stride, open_slots, kv_lens, scale, out, workspace, workspace_bytes, starved,
                              wait_ns, stream);

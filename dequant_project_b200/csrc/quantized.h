@@ -64,10 +64,9 @@ struct QuantizedAttentionArgs {
   int hq;
   float scale;
   uint64_t wait_ns;  // limit of a wait; 0: the library's
-  uint32_t starved;  // diagnostic: bit w < 8, consumer warp w gives up at once; bit 8, nothing is copied
+  uint32_t starved;  // diagnostic: bit w < 7, consumer warp w gives up at once; bit 7, nothing is copied
 };
-// Rows of the tensor maps' boxes for the kernel's tiles.
-int quantized_box_rows(int page_size);
+constexpr int kQuantizedBoxRows = 16;  // of the tensor maps' boxes
 size_t quantized_attention_workspace(int hq, int n_kv_heads, int D, int num_sms);
 cudaError_t launch_quantized_attention(const QuantizedPool& pool, const QuantizedSeqs& seqs, const CUtensorMap& kmap,
                                        const CUtensorMap& vmap, const QuantizedAttentionArgs& a, int num_sms,

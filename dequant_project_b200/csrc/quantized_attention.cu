@@ -9,10 +9,11 @@
 // block (s = 1); zero where there is none.
 //
 // The work is cut as in paged_attention.cu (paged_decode.cuh): equal shares of
-// tiles of 128 positions, pieces of cut items joined in order by a second
-// kernel. One warp copies a tile's code rows by tensor-map boxes and its
-// scales by cp.async into a ring; eight warps take 16 positions each, which
-// lie in one block, so that a warp's scales are two numbers. Positions are the
+// tiles of 112 positions, pieces of cut items joined in order by a second
+// kernel. One warp copies a tile's code rows by tensor-map boxes of 16 and its
+// scales by cp.async into a ring; seven warps take 16 positions each, which
+// lie in one block, so that a warp's scales are two numbers (eight warps in
+// all, two CTAs per SM: 128 registers a thread). Positions are the
 // m side of mma.m16n8k16 and query heads its n side (8 of them, or 16 in two
 // products): S = K Q^T, then O^T += V^T P, with the weights transposed between
 // by movmatrix. With heads on the m side, as in the 16-bit kernel, half or more
@@ -20,8 +21,7 @@
 // one to eight heads a KV head.
 //
 // Codes are read from shared memory sixteen bytes a lane and become fp16 in
-// registers, exactly (int8: the byte in the mantissa of 1024, less 1152; e4m3:
-// one conversion for two), in whatever order of the summed index that gives,
+// registers, exactly (Pairs), in whatever order of the summed index that gives,
 // the queries' being the same. bf16 queries become fp16 times a power of two
 // for each head, the largest between 2^14 and 2^15: what that loses is below
 // 2^-39 of the largest. Scores are scaled in fp32. So are the weights: besides
@@ -42,12 +42,12 @@
 namespace dqg {
 namespace {
 
-constexpr int kTile = 128;             // positions per tile
-constexpr int kWarps = 8;              // consumer warps, 16 positions each
+constexpr int kWarps = 7;              // consumer warps, 16 positions each
+constexpr int kTile = 16 * kWarps;     // positions per tile
+constexpr int kOpen = 48;              // open rows per tile: their keys fit the codes' place
 constexpr int kThreads = 32 * (kWarps + 1);
 constexpr int kQuerySlots = 4;         // items whose queries are held at most
 constexpr int kMergeRows = 2;          // query heads per round of the warps' merge
-constexpr int kScales = kTile / 16;    // scales a tile, of keys; as many of values
 constexpr float kMaxGrowth = 8.f, kHeadroom = 7.f;  // log2 units
 
 struct Params : DecodeParams {
@@ -60,10 +60,10 @@ struct Params : DecodeParams {
   int block_shift;
 };
 
-// Tiles of complete blocks, and one of the open block's rows.
+// Tiles of complete blocks, and of the open block's rows.
 __device__ __forceinline__ int tiles_of(const Params& p, int len) {
   const int open = len & ((1 << p.block_shift) - 1);
-  return max(1, (len - open + kTile - 1) / kTile + (open ? 1 : 0));
+  return max(1, (len - open + kTile - 1) / kTile + (open + kOpen - 1) / kOpen);
 }
 
 __device__ __forceinline__ uint4 lds128(uint32_t addr) {
@@ -94,23 +94,31 @@ __device__ __forceinline__ void cp_async_arrive(uint64_t* bar) {
   asm volatile("cp.async.mbarrier.arrive.noinc.shared.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
 
-// Four codes as two pairs of fp16 values: bytes (0, 2) and (1, 3) where
-// kStride is 2, (0, 1) and (2, 3) where it is 1. kUnit: what the values have to
-// be multiplied by.
+// Four codes as two pairs of fp16 numbers: bytes (0, 2) and (1, 3) where
+// kStride is 2, (0, 1) and (2, 3) where it is 1. A number is (code + kBias) /
+// 2^kUnit: an int8 code is taken with its sign bit turned over, as the
+// fraction of a subnormal number, at one or two integer instructions a pair.
+// The bias goes out of the products' sums again: S starts at -kBias sum(q), and
+// a product more per slice sums kBias p beside the values. (Bytes put into the
+// fraction of 1024 and made small again by an addition: 64 more instructions of
+// about 430 a slice.)
 template <class Code>
 struct Pairs;
 template <>
 struct Pairs<Int8> {
-  static constexpr int kStride = 2;
+  static constexpr int kStride = 2, kUnit = 24;
+  static constexpr bool kBiased = true;
+  static constexpr uint32_t kBias = 0x00800080u;  // 128 / 2^24, twice
   static __device__ __forceinline__ void expand(uint32_t w, uint32_t& a, uint32_t& b) {
-    constexpr uint32_t kLess1152 = 0xe480e480u;  // 1024 + 128, of codes taken as unsigned
-    a = hadd2_u32((w & 0x00ff00ffu) ^ 0x64806480u, kLess1152);
-    b = hadd2_u32(((w >> 8) & 0x00ff00ffu) ^ 0x64806480u, kLess1152);
+    a = (w & 0x00ff00ffu) ^ kBias;
+    b = ((w >> 8) & 0x00ff00ffu) ^ kBias;
   }
 };
 template <>
 struct Pairs<E4m3> {
-  static constexpr int kStride = 1;
+  static constexpr int kStride = 1, kUnit = 0;
+  static constexpr bool kBiased = false;
+  static constexpr uint32_t kBias = 0;
   static __device__ __forceinline__ void expand(uint32_t w, uint32_t& a, uint32_t& b) {
     a = E4m3::half2(w);
     b = E4m3::half2(w >> 16);
@@ -132,12 +140,13 @@ template <int D, int NB>
 struct Layout {
   static constexpr int kCtasPerSm = NB == 1 ? 2 : 1;
   static constexpr int kStages = NB == 1 ? 3 : 6;
-  static constexpr int kTileBytes = kTile * D;  // and as many hold 64 open rows
+  static constexpr int kTileBytes = kTile * D;
+  static_assert(kOpen * D * 2 <= kTileBytes, "open rows");
   static constexpr int kRing = kStages * 2 * kTileBytes;
   static constexpr int kQuery = 16 * D * 2;
   static constexpr int kMerge = kWarps * kMergeRows * D * 4;
   static constexpr int kStats = 3 * kWarps * 16 * 4;
-  static constexpr int kScaleBytes = kStages * 2 * kScales * 4;
+  static constexpr int kScaleBytes = kStages * 2 * kWarps * 4;
   static constexpr int kSmem =
       1024 + kRing + kQuery + kMerge + kStats + kScaleBytes + 2 * (kStages + kQuerySlots) * 8 + static_cast<int>(sizeof(Share));
 };
@@ -157,7 +166,7 @@ __global__ void __launch_bounds__(kThreads, Layout<D, NB>::kCtasPerSm)
   float* ms = os + L::kMerge / 4;                                // [warp][16]: the scores' reference,
   float* vs = ms + kWarps * 16;                                  // the values',
   float* ls = vs + kWarps * 16;                                  // and the sum
-  float* scales = ls + kWarps * 16;                              // [stage][2][kScales]
+  float* scales = ls + kWarps * 16;                              // [stage][2][kWarps]
   uint64_t* full = reinterpret_cast<uint64_t*>(scales + L::kScaleBytes / 4);
   uint64_t* empty = full + kStages;
   uint64_t* q_full = empty + kStages;
@@ -166,7 +175,7 @@ __global__ void __launch_bounds__(kThreads, Layout<D, NB>::kCtasPerSm)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int i = 0; i < kStages; ++i) {
-      mbar_init(full + i, 1 + 2 * kScales);
+      mbar_init(full + i, 1 + 2 * kWarps);
       mbar_init(empty + i, kWarps);
     }
     for (int i = 0; i < kQuerySlots; ++i) {
@@ -190,7 +199,6 @@ __global__ void __launch_bounds__(kThreads, Layout<D, NB>::kCtasPerSm)
 
   if (warp == kWarps) {
     // ---- the copying warp.
-    const int per = p.box_rows, boxes = kTile / per;  // rows a box; boxes a tile, of keys and of values
     const uint64_t policy = policy_evict_last();
     int it = 0, item = 0;
     bool ok = !(p.starved >> kWarps & 1);
@@ -210,43 +218,39 @@ __global__ void __launch_bounds__(kThreads, Layout<D, NB>::kCtasPerSm)
         bulk_g2s(qs + (qi * q_rows + lane) * D * 2, static_cast<const E*>(p.q) + s.b * p.q_stride_seq +
                  (i.head0 + lane) * p.q_stride_head, D * 2, q_full + qi, policy);
       ++item;
-      for (int x = i.x0; x < i.x1; ++x, ++it) {
+      // A lane a slice of 16 positions, of keys and then of values: its box and
+      // its block's scale. Pages are read from the table one tile ahead: their
+      // latency would be a tile's time.
+      constexpr int kNone = -0x7fffffff - 1;
+      const int slice = lane % kWarps, n_pages = static_cast<int>(p.n_pages);
+      const bool values = lane >= kWarps;
+      auto page_of = [&](int x) {
+        const int t = x * kTile + slice * 16;
+        return lane < 2 * kWarps && t < done ? __ldg(i.table + (t >> p.page_shift)) : kNone;
+      };
+      int page = page_of(i.x0), next = kNone;
+      for (int x = i.x0; x < i.x1; ++x, ++it, page = next) {
         const int st = it % kStages;
         uint8_t* dst = smem + st * 2 * L::kTileBytes;
+        if (x + 1 < i.x1) next = page_of(x + 1);
         if (x < whole || i.len == done) {
-          auto page_at = [&](int t) {
-            int page = static_cast<int>(p.n_pages);  // no such page: zeros
-            if (t < done) {
-              page = __ldg(i.table + (t >> p.page_shift));
-              if (page < 0 || page >= p.n_pages) {
-                page = static_cast<int>(p.n_pages);
-                atomicOr(&g_status, kStatusBadIndex);
-              }
-            }
-            return page;
-          };
-          const int t = x * kTile + lane * per;
-          const int page = lane < boxes ? page_at(t) : 0;
-          // A lane a scale: of keys, then of values.
-          const int j = lane % kScales, ts = x * kTile + (j << p.block_shift);
-          const bool scaled = lane < 2 * kScales && j < kTile >> p.block_shift;
-          const int sp = scaled ? page_at(ts) : static_cast<int>(p.n_pages);
           if (it >= kStages && !warp_wait(empty + st, ((it / kStages) & 1) ^ 1, p.wait_ns)) {
             ok = false;
             break;
           }
+          // No such page: zeros.
+          const bool good = page >= 0 && page < n_pages;
+          if (!good && page != kNone) atomicOr(&g_status, kStatusBadIndex);
           if (lane == 0) mbar_arrive_expect_tx(full + st, 2 * L::kTileBytes);
           __syncwarp();
-          if (lane < boxes) {
-            const int in_page = t & ((1 << p.page_shift) - 1);
-            tma_load_4d(smem_u32(dst) + lane * per * D, &kmap, full + st, 0, in_page, i.kvh, page);
-            tma_load_4d(smem_u32(dst) + L::kTileBytes + lane * per * D, &vmap, full + st, 0, in_page, i.kvh, page);
-          }
-          if (lane < 2 * kScales) {
-            float* to = scales + st * 2 * kScales + lane;
-            if (sp < p.n_pages) {
-              cp_async4(smem_u32(to), (lane < kScales ? p.k_scale : p.v_scale) + sp * p.scale_page_stride +
-                        i.kvh * p.scale_head_stride + ((ts & ((1 << p.page_shift) - 1)) >> p.block_shift));
+          if (lane < 2 * kWarps) {
+            const int in_page = (x * kTile + slice * 16) & ((1 << p.page_shift) - 1);
+            tma_load_4d(smem_u32(dst) + lane * (16 * D), values ? &vmap : &kmap, full + st, 0, in_page, i.kvh,
+                        good ? page : n_pages);
+            float* to = scales + st * 2 * kWarps + lane;
+            if (good) {
+              cp_async4(smem_u32(to), (values ? p.v_scale : p.k_scale) + page * p.scale_page_stride +
+                        i.kvh * p.scale_head_stride + (in_page >> p.block_shift));
             } else {
               *to = 0.f;
             }
@@ -254,7 +258,7 @@ __global__ void __launch_bounds__(kThreads, Layout<D, NB>::kCtasPerSm)
           }
         } else {
           // The open rows, as they are.
-          const int rows = i.len - done;
+          const int first = (x - whole) * kOpen, rows = min(kOpen, i.len - done - first);
           const int64_t slot = __ldg(p.open_slots + s.b);
           const bool good = slot >= 0 && slot < p.n_open;
           if (it >= kStages && !warp_wait(empty + st, ((it / kStages) & 1) ^ 1, p.wait_ns)) {
@@ -270,13 +274,13 @@ __global__ void __launch_bounds__(kThreads, Layout<D, NB>::kCtasPerSm)
           if (lane == 0) {
             mbar_arrive_expect_tx(full + st, good ? 2 * rows * D * 2 : 0);
             if (good) {
-              const int64_t at = slot * p.open_stride + i.kvh * p.open_head_stride;
+              const int64_t at = slot * p.open_stride + i.kvh * p.open_head_stride + first * D;
               bulk_g2s(dst, static_cast<const E*>(p.k_open) + at, rows * D * 2, full + st, policy);
               bulk_g2s(dst + L::kTileBytes, static_cast<const E*>(p.v_open) + at, rows * D * 2, full + st, policy);
             }
           }
           __syncwarp();
-          if (lane < 2 * kScales) mbar_arrive(full + st);
+          if (lane < 2 * kWarps) mbar_arrive(full + st);
         }
       }
       advance(p, s, i.units);
@@ -287,13 +291,25 @@ __global__ void __launch_bounds__(kThreads, Layout<D, NB>::kCtasPerSm)
     for (int i = it < kStages ? 0 : it - kStages; i < it; ++i)
       if (!warp_wait(full + i % kStages, (i / kStages) & 1, p.wait_ns)) break;
   } else {
+    using Pair = Pairs<Code>;
+    constexpr int kSums = D / 16 + (Pair::kBiased ? 1 : 0);  // products a slice; the last one sums the bias
     const int gid = lane >> 2, c = lane & 3;
     const uint32_t ring = smem_u32(smem);
     const int p0 = warp * 16;
-    int it = 0, item = 0;
+    // Where this lane reads in a stage's keys and values; rows 8 further lie
+    // 8 rows' bytes behind.
+    uint32_t k_at[D / 64], v_at[2];
+#pragma unroll
+    for (int h = 0; h < D / 64; ++h) k_at[h] = ring + code_off<D>(p0 + row_of(gid), c + 4 * h);
+#pragma unroll
+    for (int r = 0; r < 2; ++r)
+      v_at[r] = ring + L::kTileBytes + (D == 128 ? code_off<D>(p0 + row_of(2 * c + r), gid)
+                                                 : code_off<D>(p0 + row_of(2 * c + r), gid >> 1) + (gid & 1) * 8);
+    int stage = 0, item = 0;
+    uint32_t parity = 0;
     // Once a wait has run out no later one is taken.
     bool ok = !(p.starved >> warp & 1), cut_first = false;
-    auto await = [&](uint64_t* bar, uint32_t parity) { return ok = ok && warp_wait(bar, parity, p.wait_ns); };
+    auto await = [&](uint64_t* bar, uint32_t phase) { return ok = ok && warp_wait(bar, phase, p.wait_ns); };
     while (s.count > 0) {
       const Item i = item_of(p, s);
       if (i.x1 == i.x0) {
@@ -306,12 +322,12 @@ __global__ void __launch_bounds__(kThreads, Layout<D, NB>::kCtasPerSm)
       // Queries as B fragments: columns are heads; a lane holds the values at
       // 64 h + 16 c to + 15, four a product.
       uint32_t qf[NB][D / 16][2];
-      float unit[NB][2];  // what scores of heads 2 c and 2 c + 1 are multiplied by, but for the block's scale
+      float unit[NB][2];   // what scores of heads 2 c and 2 c + 1 are multiplied by, but for the block's scale
+      float begin[NB][2];  // where their sums begin
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb) {
         const uint32_t row = smem_u32(qs) + (qi * q_rows + nb * 8 + gid) * (D * 2) + c * 32;
         uint32_t w[D / 8];
-        uint32_t most = 0;
 #pragma unroll
         for (int h = 0; h < D / 32; ++h) {
           const uint4 v = lds128(row + (h >> 1) * 128 + (h & 1) * 16);
@@ -320,9 +336,10 @@ __global__ void __launch_bounds__(kThreads, Layout<D, NB>::kCtasPerSm)
           w[4 * h + 2] = v.z;
           w[4 * h + 3] = v.w;
         }
-        float f = p.scale_log2;
+        float f = p.scale_log2 * (1 << Pair::kUnit);
         if (Elem<E>::kFormat == 1) {
           // bf16 to fp16, times a power of two for the head.
+          uint32_t most = 0;
 #pragma unroll
           for (int h = 0; h < D / 8; ++h) most = __vmaxu2(most, w[h] & 0x7fff7fffu);
           most = max(most & 0xffffu, most >> 16);
@@ -341,184 +358,223 @@ __global__ void __launch_bounds__(kThreads, Layout<D, NB>::kCtasPerSm)
         unit[nb][1] = __shfl_sync(0xffffffffu, f, 8 * c + 4);
 #pragma unroll
         for (int k = 0; k < D / 16; ++k) {
-          qf[nb][k][0] = Pairs<Code>::kStride == 2 ? prmt(w[2 * k], w[2 * k + 1], 0x5410) : w[2 * k];
-          qf[nb][k][1] = Pairs<Code>::kStride == 2 ? prmt(w[2 * k], w[2 * k + 1], 0x7632) : w[2 * k + 1];
+          qf[nb][k][0] = Pair::kStride == 2 ? prmt(w[2 * k], w[2 * k + 1], 0x5410) : w[2 * k];
+          qf[nb][k][1] = Pair::kStride == 2 ? prmt(w[2 * k], w[2 * k + 1], 0x7632) : w[2 * k + 1];
         }
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+        if (Pair::kBiased) {
+          const uint32_t ones[4] = {Pair::kBias, Pair::kBias, Pair::kBias, Pair::kBias};
+#pragma unroll
+          for (int k = 0; k < D / 16; ++k) Elem<__half>::mma(sum, ones, qf[nb][k][0], qf[nb][k][1]);
+        }
+        begin[nb][0] = -sum[0];
+        begin[nb][1] = -sum[1];
       }
-      float o[NB][D / 16][4];
+      float o[NB][kSums][4];
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-        for (int k = 0; k < D / 16; ++k) o[nb][k][0] = o[nb][k][1] = o[nb][k][2] = o[nb][k][3] = 0.f;
-      float m[NB][2], mv[NB][2], l[NB][2];  // of heads 2 c and 2 c + 1 (l: this lane's part)
+        for (int k = 0; k < kSums; ++k) o[nb][k][0] = o[nb][k][1] = o[nb][k][2] = o[nb][k][3] = 0.f;
+      // References of heads 2 c and 2 c + 1, kHeadroom below a maximum that the
+      // true one exceeds by kMaxGrowth at most, of the scores and of what the
+      // values are weighed with; l: this lane's part of the sum.
+      float ref[NB][2], ref_v[NB][2], l[NB][2];
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          m[nb][e] = mv[nb][e] = -INFINITY;
+          ref[nb][e] = ref_v[nb][e] = -3.4e38f;
           l[nb][e] = 0.f;
         }
-      // Weights of a slice's scores sc (log2 units; entries 2 r + e: row gid + 8 r,
-      // head 2 c + e), for the softmax's sum (into l) and for the values, whose
-      // scale is 2^lv (in place of sc).
-      auto weigh = [&](float (&sc)[NB][4], float lv) {
-        bool grow = false;
+      // Weights of a slice, whose scores are sc * f (log2 units; entries 2 r + e:
+      // row gid + 8 r, head 2 c + e): for the softmax's sum into l, and for the
+      // values, whose scale is 2^lv, in place of sc.
+      auto weigh = [&](float (&sc)[NB][4], const float (&f)[NB][2], float lv) {
+        float a[NB][4], b[NB][4], most = -INFINITY;
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            grow |= sc[nb][e] - m[nb][e & 1] > kMaxGrowth || sc[nb][e] + lv - mv[nb][e & 1] > kMaxGrowth;
-        if (__any_sync(0xffffffffu, grow)) {
+          for (int e = 0; e < 4; ++e) {
+            a[nb][e] = fmaf(sc[nb][e], f[nb][e & 1], -ref[nb][e & 1]);
+            b[nb][e] = fmaf(sc[nb][e], f[nb][e & 1], lv - ref_v[nb][e & 1]);
+            most = fmaxf(most, fmaxf(a[nb][e], b[nb][e]));
+          }
+        if (__any_sync(0xffffffffu, most > kHeadroom + kMaxGrowth)) {
 #pragma unroll
           for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-              float mx = fmaxf(sc[nb][e], sc[nb][e + 2]);
+              float mx = fmaxf(sc[nb][e] * f[nb][e], sc[nb][e + 2] * f[nb][e]);
               mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
               mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
-              mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+              mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16)) - kHeadroom;
               // (Each column by itself: those of no head hold anything.)
-              if (mx - m[nb][e] > kMaxGrowth) {
-                l[nb][e] *= exp2_approx(m[nb][e] - mx);
-                m[nb][e] = mx;
+              if (mx - ref[nb][e] > kMaxGrowth) {
+                l[nb][e] *= exp2_approx(ref[nb][e] - mx);
+                ref[nb][e] = mx;
               }
-              if (mx + lv - mv[nb][e] > kMaxGrowth) {
-                const float f = exp2_approx(mv[nb][e] - (mx + lv));
-                mv[nb][e] = mx + lv;
+              if (mx + lv - ref_v[nb][e] > kMaxGrowth) {
+                const float g = exp2_approx(ref_v[nb][e] - (mx + lv));
+                ref_v[nb][e] = mx + lv;
 #pragma unroll
-                for (int k = 0; k < D / 16; ++k) {
-                  o[nb][k][e] *= f;
-                  o[nb][k][e + 2] *= f;
+                for (int k = 0; k < kSums; ++k) {
+                  o[nb][k][e] *= g;
+                  o[nb][k][e + 2] *= g;
                 }
+              }
+#pragma unroll
+              for (int r = 0; r < 4; r += 2) {
+                a[nb][e + r] = fmaf(sc[nb][e + r], f[nb][e], -ref[nb][e]);
+                b[nb][e + r] = fmaf(sc[nb][e + r], f[nb][e], lv - ref_v[nb][e]);
               }
             }
         }
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const float ref = (m[nb][e] == -INFINITY ? 0.f : m[nb][e]) - kHeadroom;
-            const float ref_v = (mv[nb][e] == -INFINITY ? 0.f : mv[nb][e]) - kHeadroom - lv;
-            l[nb][e] += exp2_approx(sc[nb][e] - ref) + exp2_approx(sc[nb][e + 2] - ref);
-            sc[nb][e] = exp2_approx(sc[nb][e] - ref_v);
-            sc[nb][e + 2] = exp2_approx(sc[nb][e + 2] - ref_v);
+          for (int e = 0; e < 4; ++e) {
+            l[nb][e & 1] += exp2_approx(a[nb][e]);
+            sc[nb][e] = exp2_approx(b[nb][e]);
           }
       };
-      for (int x = i.x0; x < i.x1; ++x, ++it) {
-        const int st = it % kStages;
-        if (!await(full + st, (it / kStages) & 1)) continue;
-        const uint32_t kst = ring + st * 2 * L::kTileBytes, vst = kst + L::kTileBytes;
-        if (x < whole || i.len == done) {
-          if (x * kTile + p0 < done) {
-            const float* sl = scales + st * 2 * kScales + (p0 >> p.block_shift);
-            const float ks = sl[0], lv = log2_approx(sl[kScales]);
-            float sc[NB][4];
+      for (int x = i.x0; x < i.x1; ++x) {
+        const uint32_t at = stage * 2 * L::kTileBytes;
+        if (await(full + stage, parity)) {
+          if (x < whole || i.len == done) {
+            if (x * kTile + p0 < done) {
+              const float ks = scales[stage * 2 * kWarps + warp];
+              const float lv = log2_approx(scales[stage * 2 * kWarps + kWarps + warp]) + Pair::kUnit;
+              float sc[NB][4], f[NB][2];
 #pragma unroll
-            for (int nb = 0; nb < NB; ++nb) sc[nb][0] = sc[nb][1] = sc[nb][2] = sc[nb][3] = 0.f;
+              for (int nb = 0; nb < NB; ++nb) {
+                f[nb][0] = unit[nb][0] * ks;
+                f[nb][1] = unit[nb][1] * ks;
+                sc[nb][0] = sc[nb][2] = begin[nb][0];
+                sc[nb][1] = sc[nb][3] = begin[nb][1];
+              }
 #pragma unroll
-            for (int h = 0; h < D / 64; ++h) {
-              const uint4 a = lds128(kst + code_off<D>(p0 + row_of(gid), c + 4 * h));
-              const uint4 b = lds128(kst + code_off<D>(p0 + 8 + row_of(gid), c + 4 * h));
-              const uint32_t aw[4] = {a.x, a.y, a.z, a.w}, bw[4] = {b.x, b.y, b.z, b.w};
+              for (int h = 0; h < D / 64; ++h) {
+                const uint4 a = lds128(k_at[h] + at), b = lds128(k_at[h] + at + 8 * D);
+                const uint32_t aw[4] = {a.x, a.y, a.z, a.w}, bw[4] = {b.x, b.y, b.z, b.w};
 #pragma unroll
-              for (int k = 0; k < 4; ++k) {
-                uint32_t f[4];
-                Pairs<Code>::expand(aw[k], f[0], f[2]);
-                Pairs<Code>::expand(bw[k], f[1], f[3]);
+                for (int k = 0; k < 4; ++k) {
+                  uint32_t w[4];
+                  Pair::expand(aw[k], w[0], w[2]);
+                  Pair::expand(bw[k], w[1], w[3]);
 #pragma unroll
-                for (int nb = 0; nb < NB; ++nb) Elem<__half>::mma(sc[nb], f, qf[nb][4 * h + k][0], qf[nb][4 * h + k][1]);
+                  for (int nb = 0; nb < NB; ++nb)
+                    Elem<__half>::mma(sc[nb], w, qf[nb][4 * h + k][0], qf[nb][4 * h + k][1]);
+                }
+              }
+              // A lane's D / 8 values of four rows: a word of each gives two
+              // products' halves.
+              constexpr uint32_t kLow = Pair::kStride == 2 ? 0x5410 : 0x5140;
+              constexpr uint32_t kHigh = Pair::kStride == 2 ? 0x7632 : 0x7362;
+              uint32_t vw[4][D / 32];
+#pragma unroll
+              for (int r = 0; r < 4; ++r) {
+                const uint32_t from = v_at[r & 1] + at + (r & 2 ? 8 * D : 0);
+                if (D == 128) {
+                  const uint4 v = lds128(from);
+                  vw[r][0] = v.x;
+                  vw[r][1] = v.y;
+                  vw[r][2 % (D / 32)] = v.z;
+                  vw[r][3 % (D / 32)] = v.w;
+                } else {
+                  const uint2 v = lds64(from);
+                  vw[r][0] = v.x;
+                  vw[r][1] = v.y;
+                }
+              }
+              weigh(sc, f, lv);
+              uint32_t pf[NB][2];
+#pragma unroll
+              for (int nb = 0; nb < NB; ++nb) {
+                pf[nb][0] = transposed(Elem<__half>::pack(sc[nb][0], sc[nb][1]));
+                pf[nb][1] = transposed(Elem<__half>::pack(sc[nb][2], sc[nb][3]));
+              }
+#pragma unroll
+              for (int k = 0; k < D / 16; ++k) {
+                const uint32_t sel = k & 1 ? kHigh : kLow;
+                uint32_t w[4];
+                Pair::expand(prmt(vw[0][k / 2], vw[1][k / 2], sel), w[0], w[1]);
+                Pair::expand(prmt(vw[2][k / 2], vw[3][k / 2], sel), w[2], w[3]);
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb) Elem<__half>::mma(o[nb][k], w, pf[nb][0], pf[nb][1]);
+              }
+              if (Pair::kBiased) {
+                const uint32_t ones[4] = {Pair::kBias, Pair::kBias, Pair::kBias, Pair::kBias};
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb) Elem<__half>::mma(o[nb][kSums - 1], ones, pf[nb][0], pf[nb][1]);
+              }
+            }
+          } else if (p0 < min(kOpen, i.len - done - (x - whole) * kOpen)) {
+            // Open rows, in their own type: rows of the products are the tile's.
+            const uint32_t kst = ring + at, vst = kst + L::kTileBytes;
+            const int rows = i.len - done - (x - whole) * kOpen - p0;  // of this warp's 16, or more
+            float sc[NB][4], f[NB][2];
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb) {
+              sc[nb][0] = sc[nb][1] = sc[nb][2] = sc[nb][3] = 0.f;
+              f[nb][0] = f[nb][1] = p.scale_log2;
+            }
+#pragma unroll
+            for (int k = 0; k < D / 16; ++k) {
+              const uint32_t off = (k / 4) * 128 + c * 32 + (k % 4) * 8;
+              const uint2 a = lds64(kst + (p0 + gid) * (D * 2) + off), b = lds64(kst + (p0 + 8 + gid) * (D * 2) + off);
+              const uint32_t w[4] = {a.x, b.x, a.y, b.y};
+#pragma unroll
+              for (int nb = 0; nb < NB; ++nb) {
+                const uint2 q = lds64(smem_u32(qs) + (qi * q_rows + nb * 8 + gid) * (D * 2) + off);
+                Elem<E>::mma(sc[nb], w, q.x, q.y);
               }
             }
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-              for (int e = 0; e < 4; ++e) sc[nb][e] *= unit[nb][e & 1] * ks;
-            weigh(sc, lv);
+              for (int e = 0; e < 4; ++e) sc[nb][e] = gid + 8 * (e >> 1) < rows ? sc[nb][e] : -INFINITY;
+            weigh(sc, f, 0.f);
             uint32_t pf[NB][2];
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb) {
-              pf[nb][0] = transposed(Elem<__half>::pack(sc[nb][0], sc[nb][1]));
-              pf[nb][1] = transposed(Elem<__half>::pack(sc[nb][2], sc[nb][3]));
-            }
-            // A lane's D / 8 values of four rows: a word of each gives two
-            // products' halves.
-            constexpr uint32_t kLow = Pairs<Code>::kStride == 2 ? 0x5410 : 0x5140;
-            constexpr uint32_t kHigh = Pairs<Code>::kStride == 2 ? 0x7632 : 0x7362;
-            const int r0 = row_of(2 * c), r1 = row_of(2 * c + 1);
-            uint32_t vw[4][D / 32];
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-              const int row = p0 + (r & 1 ? r1 : r0) + (r & 2 ? 8 : 0);
-              if (D == 128) {
-                const uint4 v = lds128(vst + code_off<D>(row, gid));
-                vw[r][0] = v.x;
-                vw[r][1] = v.y;
-                vw[r][2 % (D / 32)] = v.z;
-                vw[r][3 % (D / 32)] = v.w;
-              } else {
-                const uint2 v = lds64(vst + code_off<D>(row, gid >> 1) + (gid & 1) * 8);
-                vw[r][0] = v.x;
-                vw[r][1] = v.y;
-              }
+              pf[nb][0] = transposed(Elem<E>::pack(sc[nb][0], sc[nb][1]));
+              pf[nb][1] = transposed(Elem<E>::pack(sc[nb][2], sc[nb][3]));
             }
 #pragma unroll
             for (int k = 0; k < D / 16; ++k) {
-              const uint32_t sel = k & 1 ? kHigh : kLow;
-              uint32_t f[4];
-              Pairs<Code>::expand(prmt(vw[0][k / 2], vw[1][k / 2], sel), f[0], f[1]);
-              Pairs<Code>::expand(prmt(vw[2][k / 2], vw[3][k / 2], sel), f[2], f[3]);
+              uint32_t w[4];
 #pragma unroll
-              for (int nb = 0; nb < NB; ++nb) Elem<__half>::mma(o[nb][k], f, pf[nb][0], pf[nb][1]);
+              for (int r = 0; r < 4; ++r) {
+                // What lies behind the last row may be anything: a zero weight
+                // times an infinity would not be zero.
+                const int row = 2 * c + (r & 1) + (r & 2 ? 8 : 0);
+                w[r] = 0;
+                if (row < rows)
+                  asm volatile("ld.shared.b32 %0, [%1];"
+                               : "=r"(w[r])
+                               : "r"(vst + (p0 + row) * (D * 2) + gid * (D / 4) + k * 4));
+              }
+              const uint32_t v[4] = {prmt(w[0], w[1], 0x5410), prmt(w[0], w[1], 0x7632), prmt(w[2], w[3], 0x5410),
+                                     prmt(w[2], w[3], 0x7632)};
+#pragma unroll
+              for (int nb = 0; nb < NB; ++nb) Elem<E>::mma(o[nb][k], v, pf[nb][0], pf[nb][1]);
             }
           }
-        } else if (p0 < i.len - done) {
-          // Open rows, in their own type: rows of the products are the tile's.
-          const int rows = i.len - done - p0;  // of this warp's 16, or more
-          float sc[NB][4];
-#pragma unroll
-          for (int nb = 0; nb < NB; ++nb) sc[nb][0] = sc[nb][1] = sc[nb][2] = sc[nb][3] = 0.f;
-#pragma unroll
-          for (int k = 0; k < D / 16; ++k) {
-            const uint32_t at = (k / 4) * 128 + c * 32 + (k % 4) * 8;
-            const uint2 a = lds64(kst + (p0 + gid) * (D * 2) + at), b = lds64(kst + (p0 + 8 + gid) * (D * 2) + at);
-            const uint32_t f[4] = {a.x, b.x, a.y, b.y};
-#pragma unroll
-            for (int nb = 0; nb < NB; ++nb) {
-              const uint2 w = lds64(smem_u32(qs) + (qi * q_rows + nb * 8 + gid) * (D * 2) + at);
-              Elem<E>::mma(sc[nb], f, w.x, w.y);
-            }
-          }
-#pragma unroll
-          for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) sc[nb][e] = gid + 8 * (e >> 1) < rows ? sc[nb][e] * p.scale_log2 : -INFINITY;
-          weigh(sc, 0.f);
-          uint32_t pf[NB][2];
-#pragma unroll
-          for (int nb = 0; nb < NB; ++nb) {
-            pf[nb][0] = transposed(Elem<E>::pack(sc[nb][0], sc[nb][1]));
-            pf[nb][1] = transposed(Elem<E>::pack(sc[nb][2], sc[nb][3]));
-          }
-#pragma unroll
-          for (int k = 0; k < D / 16; ++k) {
-            uint32_t w[4];
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-              // What lies behind the last row may be anything: a zero weight
-              // times an infinity would not be zero.
-              const int row = 2 * c + (r & 1) + (r & 2 ? 8 : 0);
-              w[r] = 0;
-              if (row < rows)
-                asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w[r]) : "r"(vst + (p0 + row) * (D * 2) + gid * (D / 4) + k * 4));
-            }
-            const uint32_t f[4] = {prmt(w[0], w[1], 0x5410), prmt(w[0], w[1], 0x7632), prmt(w[2], w[3], 0x5410),
-                                   prmt(w[2], w[3], 0x7632)};
-#pragma unroll
-            for (int nb = 0; nb < NB; ++nb) Elem<E>::mma(o[nb][k], f, pf[nb][0], pf[nb][1]);
-          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(empty + stage);
         }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(empty + st);
+        if (++stage == kStages) {
+          stage = 0;
+          parity ^= 1;
+        }
+      }
+      if (Pair::kBiased) {
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+          for (int k = 0; k < D / 16; ++k)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[nb][k][e] -= o[nb][kSums - 1][e & 1];
       }
       // The queries' place is free once their reads have come back, not once
       // they are issued: here every fragment is used.
@@ -544,8 +600,9 @@ __global__ void __launch_bounds__(kThreads, Layout<D, NB>::kCtasPerSm)
           l[nb][e] += __shfl_xor_sync(0xffffffffu, l[nb][e], 16);
           if (gid == 0) {
             const int at = warp * 16 + nb * 8 + 2 * c + e;
-            ms[at] = m[nb][e];
-            vs[at] = mv[nb][e];
+            // (-inf: no position yet, as in the pieces.)
+            ms[at] = ref[nb][e] == -3.4e38f ? -INFINITY : ref[nb][e];
+            vs[at] = ref_v[nb][e] == -3.4e38f ? -INFINITY : ref_v[nb][e];
             ls[at] = ok ? l[nb][e] : NAN;
           }
         }
@@ -664,8 +721,6 @@ Scratch scratch_of(int hq, int n_kv_heads, int num_sms) {
 
 }  // namespace
 
-int quantized_box_rows(int page_size) { return page_size < kTile ? page_size : kTile; }
-
 size_t quantized_attention_workspace(int hq, int n_kv_heads, int D, int num_sms) {
   const Scratch s = scratch_of(hq, n_kv_heads, num_sms);
   // Descriptions first (16 bytes each), then the rows.
@@ -700,7 +755,6 @@ cudaError_t launch_quantized_attention(const QuantizedPool& pool, const Quantize
   while ((1 << p.block_shift) < pool.block) ++p.block_shift;
   const int64_t limit = static_cast<int64_t>(seqs.table_width) * pool.page_size;
   p.len_limit = limit < (1 << 30) ? static_cast<int>(limit) : 1 << 30;
-  p.box_rows = quantized_box_rows(pool.page_size);
   p.scale_log2 = static_cast<float>(a.scale * 1.4426950408889634);
   p.starved = a.starved;
   p.wait_ns = a.wait_ns ? a.wait_ns : kWaitLimitNs;

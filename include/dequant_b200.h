@@ -530,7 +530,7 @@ int dqg_quantized_attention(const void *q, int64_t q_stride_seq, int64_t q_strid
 
 /*
  * Diagnostic for the bounded waits of dqg_quantized_attention, as
- * dqg_debug_paged_starved (starved, bits 0 to 7: a consumer warp; bit 8: the
+ * dqg_debug_paged_starved (starved, bits 0 to 6: a consumer warp; bit 7: the
  * copying warp). For tests.
  */
 int dqg_debug_quantized_starved(const void *q, int64_t q_stride_seq, int64_t q_stride_head,
