@@ -20,11 +20,11 @@
 // of the products' rows and of the accumulators would be empty for the usual
 // one to eight heads a KV head.
 //
-// Codes are read from shared memory sixteen bytes a lane and become fp16 in
+// Codes are read from shared memory sixteen bytes a lane and become operands in
 // registers, exactly (Pairs), in whatever order of the summed index that gives,
-// the queries' being the same. bf16 queries become fp16 times a power of two
-// for each head, the largest between 2^14 and 2^15: what that loses is below
-// 2^-39 of the largest. Scores are scaled in fp32. So are the weights: besides
+// the queries' being the same. Beside e4m3 codes bf16 queries become fp16 times
+// a power of two for each head, the largest between 2^14 and 2^15: what that
+// loses is below 2^-39 of the largest. Scores are scaled in fp32. So are the weights: besides
 // the softmax's reference (of the scores) the sum over values has one of its
 // own, of the score plus log2 s_v, so that a 16-bit weight is relative to the
 // largest p s_v met, whatever the blocks' scales are. Both references move, and
@@ -47,7 +47,7 @@ constexpr int kTile = 16 * kWarps;     // positions per tile
 constexpr int kOpen = 48;              // open rows per tile: their keys fit the codes' place
 constexpr int kThreads = 32 * (kWarps + 1);
 constexpr int kQuerySlots = 4;         // items whose queries are held at most
-constexpr int kMergeRows = 2;          // query heads per round of the warps' merge
+constexpr int kMergeRows = 4;          // query heads per round of the warps' merge
 constexpr float kMaxGrowth = 8.f, kHeadroom = 7.f;  // log2 units
 
 struct Params : DecodeParams {
@@ -66,14 +66,18 @@ __device__ __forceinline__ int tiles_of(const Params& p, int len) {
   return max(1, (len - open + kTile - 1) / kTile + (open + kOpen - 1) / kOpen);
 }
 
+template <int kOff = 0>
 __device__ __forceinline__ uint4 lds128(uint32_t addr) {
   uint4 v;
-  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4 + %5];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "r"(addr), "n"(kOff));
   return v;
 }
+template <int kOff = 0>
 __device__ __forceinline__ uint2 lds64(uint32_t addr) {
   uint2 v;
-  asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr));
+  asm volatile("ld.shared.v2.b32 {%0, %1}, [%2 + %3];" : "=r"(v.x), "=r"(v.y) : "r"(addr), "n"(kOff));
   return v;
 }
 __device__ __forceinline__ uint32_t transposed(uint32_t x) {
@@ -94,20 +98,24 @@ __device__ __forceinline__ void cp_async_arrive(uint64_t* bar) {
   asm volatile("cp.async.mbarrier.arrive.noinc.shared.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
 
-// Four codes as two pairs of fp16 numbers: bytes (0, 2) and (1, 3) where
-// kStride is 2, (0, 1) and (2, 3) where it is 1. A number is (code + kBias) /
-// 2^kUnit: an int8 code is taken with its sign bit turned over, as the
-// fraction of a subnormal number, at one or two integer instructions a pair.
-// The bias goes out of the products' sums again: S starts at -kBias sum(q), and
-// a product more per slice sums kBias p beside the values. (Bytes put into the
-// fraction of 1024 and made small again by an addition: 64 more instructions of
-// about 430 a slice.)
+// Codes as operands. Values, four codes a word, become two pairs of fp16
+// numbers: bytes (0, 2) and (1, 3) where kStride is 2, (0, 1) and (2, 3) where
+// it is 1. e4m3: one conversion for two. int8: the byte with its sign bit turned
+// over, as the fraction of a subnormal number, (code + 128) / 2^24: one or two
+// integer instructions a pair; the bias goes out of the sums again (a product
+// more per slice sums 128 p). Bytes put into the fraction of 1024 and made small
+// again by an addition took 64 more instructions of about 430 a slice.
+// Keys: e4m3 the same way. int8 codes enter integer products as they are; the
+// queries are rounded to 15 bits of their head's largest, in two int8 digits.
+// That is 2^-16 of the largest a value, a tenth of what the weights' rounding to
+// fp16 does to a score of usual size, and takes all instructions but the
+// products away.
 template <class Code>
 struct Pairs;
 template <>
 struct Pairs<Int8> {
   static constexpr int kStride = 2, kUnit = 24;
-  static constexpr bool kBiased = true;
+  static constexpr bool kInteger = true;
   static constexpr uint32_t kBias = 0x00800080u;  // 128 / 2^24, twice
   static __device__ __forceinline__ void expand(uint32_t w, uint32_t& a, uint32_t& b) {
     a = (w & 0x00ff00ffu) ^ kBias;
@@ -117,13 +125,23 @@ struct Pairs<Int8> {
 template <>
 struct Pairs<E4m3> {
   static constexpr int kStride = 1, kUnit = 0;
-  static constexpr bool kBiased = false;
+  static constexpr bool kInteger = false;
   static constexpr uint32_t kBias = 0;
   static __device__ __forceinline__ void expand(uint32_t w, uint32_t& a, uint32_t& b) {
     a = E4m3::half2(w);
     b = E4m3::half2(w >> 16);
   }
 };
+// d += a b of int8 values, one 16x32 by 32x8 tile. Sums below 2^22 that begin at
+// kIntZero are the bits of that float plus the sum.
+__device__ __forceinline__ void mma_s8(int* d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                       uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+constexpr int kIntZero = 0x4b400000;  // 1.5 * 2^23
+__device__ __forceinline__ float int_sum(int bits) { return __int_as_float(bits) - 12582912.f; }
 
 // Row of a tile that row n of a product takes: conflict-free reads of sixteen
 // bytes a lane by eight rows of four lanes (keys) as by four of eight (values).
@@ -292,7 +310,7 @@ __global__ void __launch_bounds__(kThreads, Layout<D, NB>::kCtasPerSm)
       if (!warp_wait(full + i % kStages, (i / kStages) & 1, p.wait_ns)) break;
   } else {
     using Pair = Pairs<Code>;
-    constexpr int kSums = D / 16 + (Pair::kBiased ? 1 : 0);  // products a slice; the last one sums the bias
+    constexpr int kSums = D / 16 + (Pair::kInteger ? 1 : 0);  // products a slice; the last one sums the bias
     const int gid = lane >> 2, c = lane & 3;
     const uint32_t ring = smem_u32(smem);
     const int p0 = warp * 16;
@@ -320,14 +338,14 @@ __global__ void __launch_bounds__(kThreads, Layout<D, NB>::kCtasPerSm)
       const int qi = item % q_slots;
       await(q_full + qi, (item / q_slots) & 1);
       // Queries as B fragments: columns are heads; a lane holds the values at
-      // 64 h + 16 c to + 15, four a product.
-      uint32_t qf[NB][D / 16][2];
-      float unit[NB][2];   // what scores of heads 2 c and 2 c + 1 are multiplied by, but for the block's scale
-      float begin[NB][2];  // where their sums begin
+      // 64 h + 16 c to + 15, four a product (fp16) or eight (digits).
+      uint32_t qf[NB][D / 16][2];  // digits: [word][high, low]
+      float unit[NB][2];           // what scores of heads 2 c and 2 c + 1 are multiplied by, but for the block's scale
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb) {
         const uint32_t row = smem_u32(qs) + (qi * q_rows + nb * 8 + gid) * (D * 2) + c * 32;
         uint32_t w[D / 8];
+        uint32_t most = 0;
 #pragma unroll
         for (int h = 0; h < D / 32; ++h) {
           const uint4 v = lds128(row + (h >> 1) * 128 + (h & 1) * 16);
@@ -336,39 +354,50 @@ __global__ void __launch_bounds__(kThreads, Layout<D, NB>::kCtasPerSm)
           w[4 * h + 2] = v.z;
           w[4 * h + 3] = v.w;
         }
-        float f = p.scale_log2 * (1 << Pair::kUnit);
-        if (Elem<E>::kFormat == 1) {
-          // bf16 to fp16, times a power of two for the head.
-          uint32_t most = 0;
 #pragma unroll
-          for (int h = 0; h < D / 8; ++h) most = __vmaxu2(most, w[h] & 0x7fff7fffu);
-          most = max(most & 0xffffu, most >> 16);
-          most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
-          most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
-          const int e = min(max(static_cast<int>(most >> 7), 20), 240);  // exponent of the largest, biased
-          const float up = __uint_as_float(static_cast<uint32_t>(127 + 14 + 127 - e) << 23);  // 2^(14 - (e - 127))
+        for (int h = 0; h < D / 8; ++h) most = __vmaxu2(most, w[h] & 0x7fff7fffu);
+        most = max(most & 0xffffu, most >> 16);
+        most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
+        most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
+        float f = p.scale_log2;
+        if constexpr (Pair::kInteger) {
+          // (A largest value that is not finite makes the head's unit so.)
+          const float largest = Elem<E>::unpack(most).x, up = fminf(16319.f / largest, 1e38f);
+          f *= largest > 1e-30f ? largest / 16319.f : (largest == largest ? 1e-38f : NAN);
 #pragma unroll
-          for (int h = 0; h < D / 8; ++h) {
-            const float2 x = Elem<E>::unpack(w[h]);
-            w[h] = Elem<__half>::pack(x.x * up, x.y * up);
+          for (int k = 0; k < D / 16; ++k) {
+            const float2 x = Elem<E>::unpack(w[2 * k]), y = Elem<E>::unpack(w[2 * k + 1]);
+            const float v[4] = {x.x, x.y, y.x, y.y};
+            int high[4], low[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int n = __float2int_rn(v[e] * up);
+              high[e] = (n + 64) >> 7;
+              low[e] = n - high[e] * 128;
+            }
+            qf[nb][k][0] = prmt(prmt(high[0], high[1], 0x0040), prmt(high[2], high[3], 0x0040), 0x5410);
+            qf[nb][k][1] = prmt(prmt(low[0], low[1], 0x0040), prmt(low[2], low[3], 0x0040), 0x5410);
           }
-          f *= __uint_as_float(static_cast<uint32_t>(e - 14) << 23);  // 2^((e - 127) - 14)
+        } else {
+          if (Elem<E>::kFormat == 1) {
+            // bf16 to fp16, times a power of two for the head.
+            const int e = min(max(static_cast<int>(most >> 7), 20), 240);  // exponent of the largest, biased
+            const float up = __uint_as_float(static_cast<uint32_t>(127 + 14 + 127 - e) << 23);  // 2^(14 - (e - 127))
+#pragma unroll
+            for (int h = 0; h < D / 8; ++h) {
+              const float2 x = Elem<E>::unpack(w[h]);
+              w[h] = Elem<__half>::pack(x.x * up, x.y * up);
+            }
+            f *= __uint_as_float(static_cast<uint32_t>(e - 14) << 23);  // 2^((e - 127) - 14)
+          }
+#pragma unroll
+          for (int k = 0; k < D / 16; ++k) {
+            qf[nb][k][0] = w[2 * k];
+            qf[nb][k][1] = w[2 * k + 1];
+          }
         }
         unit[nb][0] = __shfl_sync(0xffffffffu, f, 8 * c);  // of lanes with gid = 2 c
         unit[nb][1] = __shfl_sync(0xffffffffu, f, 8 * c + 4);
-#pragma unroll
-        for (int k = 0; k < D / 16; ++k) {
-          qf[nb][k][0] = Pair::kStride == 2 ? prmt(w[2 * k], w[2 * k + 1], 0x5410) : w[2 * k];
-          qf[nb][k][1] = Pair::kStride == 2 ? prmt(w[2 * k], w[2 * k + 1], 0x7632) : w[2 * k + 1];
-        }
-        float sum[4] = {0.f, 0.f, 0.f, 0.f};
-        if (Pair::kBiased) {
-          const uint32_t ones[4] = {Pair::kBias, Pair::kBias, Pair::kBias, Pair::kBias};
-#pragma unroll
-          for (int k = 0; k < D / 16; ++k) Elem<__half>::mma(sum, ones, qf[nb][k][0], qf[nb][k][1]);
-        }
-        begin[nb][0] = -sum[0];
-        begin[nb][1] = -sum[1];
       }
       float o[NB][kSums][4];
 #pragma unroll
@@ -445,26 +474,48 @@ __global__ void __launch_bounds__(kThreads, Layout<D, NB>::kCtasPerSm)
               const float ks = scales[stage * 2 * kWarps + warp];
               const float lv = log2_approx(scales[stage * 2 * kWarps + kWarps + warp]) + Pair::kUnit;
               float sc[NB][4], f[NB][2];
+              int sums[NB][2][4];
 #pragma unroll
               for (int nb = 0; nb < NB; ++nb) {
                 f[nb][0] = unit[nb][0] * ks;
                 f[nb][1] = unit[nb][1] * ks;
-                sc[nb][0] = sc[nb][2] = begin[nb][0];
-                sc[nb][1] = sc[nb][3] = begin[nb][1];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  sc[nb][e] = 0.f;
+                  sums[nb][0][e] = sums[nb][1][e] = kIntZero;
+                }
               }
 #pragma unroll
               for (int h = 0; h < D / 64; ++h) {
-                const uint4 a = lds128(k_at[h] + at), b = lds128(k_at[h] + at + 8 * D);
+                const uint4 a = lds128(k_at[h] + at), b = lds128<8 * D>(k_at[h] + at);
                 const uint32_t aw[4] = {a.x, a.y, a.z, a.w}, bw[4] = {b.x, b.y, b.z, b.w};
+                if constexpr (Pair::kInteger) {
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                  uint32_t w[4];
-                  Pair::expand(aw[k], w[0], w[2]);
-                  Pair::expand(bw[k], w[1], w[3]);
+                  for (int k = 0; k < 4; k += 2)
 #pragma unroll
-                  for (int nb = 0; nb < NB; ++nb)
-                    Elem<__half>::mma(sc[nb], w, qf[nb][4 * h + k][0], qf[nb][4 * h + k][1]);
+                    for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                      for (int e = 0; e < 2; ++e)
+                        mma_s8(sums[nb][e], aw[k], bw[k], aw[k + 1], bw[k + 1], qf[nb][4 * h + k][e],
+                               qf[nb][4 * h + k + 1][e]);
+                } else {
+#pragma unroll
+                  for (int k = 0; k < 4; ++k) {
+                    uint32_t w[4];
+                    Pair::expand(aw[k], w[0], w[2]);
+                    Pair::expand(bw[k], w[1], w[3]);
+#pragma unroll
+                    for (int nb = 0; nb < NB; ++nb)
+                      Elem<__half>::mma(sc[nb], w, qf[nb][4 * h + k][0], qf[nb][4 * h + k][1]);
+                  }
                 }
+              }
+              if constexpr (Pair::kInteger) {
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                  for (int e = 0; e < 4; ++e)
+                    sc[nb][e] = fmaf(int_sum(sums[nb][0][e]), 128.f, int_sum(sums[nb][1][e]));
               }
               // A lane's D / 8 values of four rows: a word of each gives two
               // products' halves.
@@ -473,15 +524,15 @@ __global__ void __launch_bounds__(kThreads, Layout<D, NB>::kCtasPerSm)
               uint32_t vw[4][D / 32];
 #pragma unroll
               for (int r = 0; r < 4; ++r) {
-                const uint32_t from = v_at[r & 1] + at + (r & 2 ? 8 * D : 0);
+                const uint32_t from = v_at[r & 1] + at;
                 if (D == 128) {
-                  const uint4 v = lds128(from);
+                  const uint4 v = r & 2 ? lds128<8 * D>(from) : lds128(from);
                   vw[r][0] = v.x;
                   vw[r][1] = v.y;
                   vw[r][2 % (D / 32)] = v.z;
                   vw[r][3 % (D / 32)] = v.w;
                 } else {
-                  const uint2 v = lds64(from);
+                  const uint2 v = r & 2 ? lds64<8 * D>(from) : lds64(from);
                   vw[r][0] = v.x;
                   vw[r][1] = v.y;
                 }
@@ -502,7 +553,7 @@ __global__ void __launch_bounds__(kThreads, Layout<D, NB>::kCtasPerSm)
 #pragma unroll
                 for (int nb = 0; nb < NB; ++nb) Elem<__half>::mma(o[nb][k], w, pf[nb][0], pf[nb][1]);
               }
-              if (Pair::kBiased) {
+              if (Pair::kInteger) {
                 const uint32_t ones[4] = {Pair::kBias, Pair::kBias, Pair::kBias, Pair::kBias};
 #pragma unroll
                 for (int nb = 0; nb < NB; ++nb) Elem<__half>::mma(o[nb][kSums - 1], ones, pf[nb][0], pf[nb][1]);
@@ -568,7 +619,7 @@ __global__ void __launch_bounds__(kThreads, Layout<D, NB>::kCtasPerSm)
           parity ^= 1;
         }
       }
-      if (Pair::kBiased) {
+      if (Pair::kInteger) {
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
@@ -590,7 +641,8 @@ __global__ void __launch_bounds__(kThreads, Layout<D, NB>::kCtasPerSm)
       if (ok && lane == 0) mbar_arrive(q_empty + qi);
       ++item;
 
-      // The item's (or piece's) result: the warps' parts, two heads a round.
+      // The item's (or piece's) result: the warps' references and sums first,
+      // then their parts, four heads a round.
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
@@ -606,8 +658,27 @@ __global__ void __launch_bounds__(kThreads, Layout<D, NB>::kCtasPerSm)
             ls[at] = ok ? l[nb][e] : NAN;
           }
         }
+      named_sync(1, 32 * kWarps);
       const bool all = i.x0 == 0 && i.x1 == i.tiles;
       const int64_t row0 = (2 * static_cast<int64_t>(blockIdx.x) + (i.x0 > 0 ? 0 : 1)) * p.rows;
+      if (threadIdx.x < i.rows) {
+        // A head's maximum, its sum, and what each warp's part is multiplied by.
+        const int row = threadIdx.x;
+        float mx = -INFINITY, den = 0.f;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) mx = fmaxf(mx, ms[w * 16 + row]);
+        const float mu = mx == -INFINITY ? 0.f : mx;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+          den = fmaf(ls[w * 16 + row], exp2_approx(ms[w * 16 + row] - mu), den);
+          vs[w * 16 + row] = exp2_approx(vs[w * 16 + row] - mu);
+        }
+        ls[row] = den;
+        if (!all) {
+          p.m[row0 + row] = mx;
+          p.l[row0 + row] = den;
+        }
+      }
       if (i.x0 == 0 && !all) {
         cut_first = true;
         if (threadIdx.x == 0) {
@@ -616,48 +687,38 @@ __global__ void __launch_bounds__(kThreads, Layout<D, NB>::kCtasPerSm)
         }
       }
 #pragma unroll
-      for (int r = 0; r < 4 * NB; ++r) {
-        if (2 * r >= i.rows) break;
-        if (c == r % 4) {
+      for (int r = 0; r < 2 * NB; ++r) {
+        if (kMergeRows * r >= i.rows) break;
+        if (c / 2 == r % 2) {
           // Sixteen (or eight) values of a head a lane; their chunks are
           // swizzled by gid against bank conflicts.
 #pragma unroll
           for (int e = 0; e < 2; ++e)
 #pragma unroll
             for (int k = 0; k < D / 32; ++k)
-              *reinterpret_cast<float4*>(os + (warp * kMergeRows + e) * D + gid * (D / 8) + (k ^ ((gid >> 1) & (D / 32 - 1))) * 4) =
-                  make_float4(o[r / 4][2 * k][e], o[r / 4][2 * k][e + 2], o[r / 4][2 * k + 1][e], o[r / 4][2 * k + 1][e + 2]);
+              *reinterpret_cast<float4*>(os + (warp * kMergeRows + 2 * (c % 2) + e) * D + gid * (D / 8) +
+                                         (k ^ ((gid >> 1) & (D / 32 - 1))) * 4) =
+                  make_float4(o[r / 2][2 * k][e], o[r / 2][2 * k][e + 2], o[r / 2][2 * k + 1][e], o[r / 2][2 * k + 1][e + 2]);
         }
         named_sync(1, 32 * kWarps);
         for (int cell = threadIdx.x; cell < kMergeRows * (D / 4); cell += 32 * kWarps) {
-          const int j = cell / (D / 4), d4 = cell % (D / 4), row = 2 * r + j;
+          const int j = cell / (D / 4), d4 = cell % (D / 4), row = kMergeRows * r + j;
           if (row < i.rows) {
-            const int g8 = d4 / (D / 32), at = g8 * (D / 8) + ((d4 ^ ((g8 >> 1) & (D / 32 - 1))) & (D / 32 - 1)) * 4;
-            float mx = -INFINITY;
-#pragma unroll
-            for (int w = 0; w < kWarps; ++w) mx = fmaxf(mx, ms[w * 16 + row]);
-            const float mu = mx == -INFINITY ? 0.f : mx;
-            float den = 0.f;
+            const int g8 = d4 / (D / 32), at = g8 * (D / 8) + ((d4 ^ (g8 >> 1)) & (D / 32 - 1)) * 4;
             float4 num = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
             for (int w = 0; w < kWarps; ++w) {
-              den = fmaf(ls[w * 16 + row], exp2_approx(ms[w * 16 + row] - mu), den);
-              const float f = exp2_approx(vs[w * 16 + row] - mu);
+              const float f = vs[w * 16 + row];
               const float4 v = *reinterpret_cast<const float4*>(os + (w * kMergeRows + j) * D + at);
               num.x = fmaf(v.x, f, num.x);
               num.y = fmaf(v.y, f, num.y);
               num.z = fmaf(v.z, f, num.z);
               num.w = fmaf(v.w, f, num.w);
             }
-            if (all) {
-              store4<E, D>(p, s.b, i.head0 + row, d4, den, num);
-            } else {
+            if (all)
+              store4<E, D>(p, s.b, i.head0 + row, d4, ls[row], num);
+            else
               *reinterpret_cast<float4*>(p.part + (row0 + row) * D + d4 * 4) = num;
-              if (d4 == 0) {
-                p.m[row0 + row] = mx;
-                p.l[row0 + row] = den;
-              }
-            }
           }
         }
         named_sync(1, 32 * kWarps);
@@ -758,7 +819,10 @@ cudaError_t launch_quantized_attention(const QuantizedPool& pool, const Quantize
   p.scale_log2 = static_cast<float>(a.scale * 1.4426950408889634);
   p.starved = a.starved;
   p.wait_ns = a.wait_ns ? a.wait_ns : kWaitLimitNs;
-  p.item_tiles = 1;
+  // An item's start and end, in tiles' time: 64 sequences of 900 to 16000
+  // positions, 64 and 8 heads, 137 us with 1, 121 with 2 and 3, 122 with 4, 127
+  // with 6; 8 sequences of 4000 of 8 heads on one 13.8 and 14.5.
+  p.item_tiles = 2;
   p.n_units32 = static_cast<double>(p.B) * p.hkv * p.nrb * (p.len_limit / kTile + 2 + p.item_tiles) < 2147483648.0;
   p.k_scale = pool.k_scale;
   p.v_scale = pool.v_scale;

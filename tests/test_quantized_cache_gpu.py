@@ -12,7 +12,10 @@ Attention: outputs are rounded once to 16 bits (unit roundoff u = 2^-11 fp16,
 2^-8 bf16) and each softmax weight once to 16 bits before the product with the
 values, while the weights' sum is taken before: at most u * sum_j p_j |v_j| <= u
 * max|v| per output. Exponentials and fp32 sums add below 2^-13 of that scale.
-So |out - ref| <= u |ref| + (u + 2^-13) max|v|.
+So |out - ref| <= u |ref| + (u + 2^-13) max|v|. Beside int8 codes the decode
+step rounds queries to 2^-16 of their head's largest: a score changes by e <=
+scale 2^-16 max|q| sum|k| (the sum over a key's values), a weight by a factor
+within exp(2 e), an output by expm1(2 e) max|v| at most.
 """
 
 from __future__ import annotations
@@ -98,10 +101,10 @@ def attend64(q, k, v, ends, scale):
     return torch.einsum("rkgt,tkd->rkgd", p, v).reshape(rows, hq, d)
 
 
-def check_attention(out, ref, v_max, dtype):
+def check_attention(out, ref, v_max, dtype, e=0.0):
     u = U[dtype]
     err = (out.double() - ref).abs()
-    lim = u * ref.abs() + (u + 2.0 ** -13) * v_max + 1e-7
+    lim = u * ref.abs() + (u + 2.0 ** -13 + math.expm1(2 * e)) * v_max + 1e-7
     assert bool((err <= lim).all()), f"max excess {float((err - lim).max()):.3e}, max error {float(err.max()):.3e}"
 
 
@@ -381,6 +384,15 @@ def largest_value(cache, table, slots, lens):
                default=0.0)
 
 
+def query_rounding(q, cache, table, slots, lens):
+    """The bound e of how far rounded queries move a score."""
+    if cache.k.dtype != torch.int8:
+        return 0.0
+    k = max([float(rows64(cache, 0, table[b], slots[b].long(), n).abs().sum(-1).max()) for b, n in enumerate(lens) if n],
+            default=0.0)
+    return 2.0 ** -16 * float(q.float().abs().max()) * k / math.sqrt(q.shape[2])
+
+
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
 @pytest.mark.parametrize("codes", CODES, ids=str)
 @pytest.mark.parametrize("lens,hq,hkv,d,page,block", DECODE, ids=lambda v: str(v)[:40])
@@ -392,7 +404,7 @@ def test_decode(cuda_device, lens, hq, hkv, d, page, block, codes, dtype):
     out = qc.quantized_attention(q, cache, table, slots, kv_lens)
     assert _native.device_status(cuda_device.index, reset=True) == 0
     ref = reference(q, cache, table, slots, lens, 1 / math.sqrt(d))
-    check_attention(out, ref, largest_value(cache, table, slots, lens), dtype)
+    check_attention(out, ref, largest_value(cache, table, slots, lens), dtype, query_rounding(q, cache, table, slots, lens))
     ws = qc.quantized_attention_workspace(len(lens), hq, hkv, d, cuda_device).fill_(255)
     for _ in range(3):
         assert torch.equal(qc.quantized_attention(q, cache, table, slots, kv_lens, workspace=ws), out)
