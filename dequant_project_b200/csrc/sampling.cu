@@ -18,8 +18,9 @@
 // a sum that every CTA has, so that one barrier of the cluster is enough. What
 // lies far below a cut stays out of the histograms: top-k's cut is above what
 // the k-th largest of the threads' maxima is above, and top-p's above the
-// largest of four weights that has top_p of the sum above it. The tokens that
-// are left, mostly a few, are listed once and read from there.
+// largest of five weights that has top_p of the sum from it on. The tokens that
+// are left, mostly a few, are listed once and read from there; up to 256 of them
+// are not searched at all, but ranked by one CTA that compares each with all.
 #include <cstdint>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -40,8 +41,8 @@ constexpr int kMaxCtas = 8;
 constexpr int kBins = 1024;
 constexpr int kPer = kBins / kThreads;  // bins a thread
 constexpr int kListed = 2048;           // tokens that a CTA's list holds
-constexpr int kLevels = 4;              // weights 2^-4, 2^-8, 2^-12, 2^-16
-constexpr u64 kOne = u64(1) << 44;
+constexpr int kDirect = 256;            // tokens of a row's lists that one CTA ranks
+constexpr int kLevels = 5;              // weights 2^-4, 2^-7, 2^-10, 2^-13, 2^-16
 
 struct Params {
   SampleArgs a;
@@ -102,28 +103,40 @@ __device__ __forceinline__ float value_of(uint32_t key) {
 struct Shared {
   Power powers[64];
   uint32_t own[3][kBins];     // this CTA's histogram: numbers, or 16 bits of the weights each
-  uint32_t sum[2][3][kBins];  // the cluster's, in turn: numbers, or 24 bits of the weights each
-  float list[kListed];
+  // The cluster's, of the bins that this CTA holds (every ctas-th; a CTA alone
+  // has its own histogram), in turn: numbers, or 24 bits of the weights each.
+  uint32_t sum[3][3][kBins / 2];
+  float list[kListed];        // logits,
+  uint16_t places[kListed];   // and their places in the CTA's part of the row
   u64 scratch[kWarps];
-  u64 parts[kLevels + 1];     // of sums, read by the peers
+  u64 wide[kLevels + 2][kWarps];
+  u64 parts[kLevels + 2];     // of sums and of a number of ties, read by the peers
   float largest;
-  uint32_t first, ties, cut_ties, listed;
+  uint32_t first, cut_ties, listed;
+  int limit;                  // place of the last token at the cut that is kept
   u64 total;
   uint32_t bin;               // of the cut
   u64 before, inside;         // ahead of it, and in it
 };
 
+struct Ranked {  // a token of a row's lists
+  u64 w;
+  float v;
+  uint32_t place;
+};
+struct Ranks {  // of half of a row's tokens: those ahead of one
+  u64 w;
+  uint32_t greater, ties;
+};
+
 struct Weights {
   float m, high, low;  // the largest logit; log2(e) / T in two parts
-  bool inf;            // m is +inf
   const Power* powers;
-  // W of a logit.
+  // W of a logit (m finite). No branches: several tokens' chains run together.
   __device__ __forceinline__ u64 operator()(float v) const {
-    if (inf) return v == INFINITY ? kOne : 0;
     // s + err = v - m and p + e = (v - m) log2(e) / T, in twice the precision.
     const float s = v - m, back = s - v;
-    const float p = s * high;
-    if (!(p >= -46.f)) return 0;
+    const float p = fmaxf(s * high, -48.f);
     const float err = (v - (s - back)) + (-m - back);
     const float e = fmaf(err, high, fmaf(s, low, fmaf(s, high, -p)));
     const float t = fmaf(p, 64.f, 12582912.f);  // 1.5 * 2^23: the fraction's last bit is one
@@ -133,8 +146,7 @@ struct Weights {
     const float q = r * fmaf(r, fmaf(r, fmaf(r, 9.6181291e-3f, 5.5504109e-2f), 2.4022651e-1f), 6.9314718e-1f);
     const Power w = powers[n & 63];
     const u64 one = w.fixed + (static_cast<long long>(__float2int_rn(q * w.scaled)) << 13);
-    const int down = -(n >> 6);
-    return down ? (one + (u64(1) << (down - 1))) >> down : one;
+    return p >= -46.f ? (((one << 1) >> -(n >> 6)) + 1) >> 1 : 0;
   }
 };
 
@@ -168,6 +180,21 @@ __device__ __forceinline__ V block_reduce(V v, u64* scratch, F f) {
   __syncthreads();
   return v;
 }
+// f over what the cluster's CTAs have at p, and of the CTAs before `rank` alone
+// (*before), `none` standing for no value. A lane a CTA.
+template <typename V, class F>
+__device__ __forceinline__ V cluster_reduce(const V* p, int ctas, V none, F f, int rank = 0, V* before = nullptr) {
+  static_assert(kMaxCtas == 8, "eight lanes");
+  const int r = threadIdx.x & 7;
+  V v = r < ctas ? peer(p, r) : none, b = r < rank ? v : none;
+#pragma unroll
+  for (int off = 4; off >= 1; off >>= 1) {
+    v = f(v, __shfl_xor_sync(0xffffffffu, v, off));
+    if (before) b = f(b, __shfl_xor_sync(0xffffffffu, b, off));
+  }
+  if (before) *before = b;
+  return v;
+}
 // Sum of v over the threads before this one; *all: over the block.
 __device__ __forceinline__ u64 block_scan(u64 v, u64* scratch, u64* all) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -193,43 +220,56 @@ __device__ __forceinline__ u64 block_scan(u64 v, u64* scratch, u64* all) {
 // One round of a cut's search: histograms over bins that add() fills (tokens'
 // numbers, or their weights), added up over the cluster; the bin that
 // take(sum before it) takes last, from the highest down, goes to sh->bin, with
-// sh->before and sh->inside. The buffers of sh->sum take turns; the next
-// round's is zeroed here.
+// sh->before and sh->inside. Three buffers of the cluster's sums take turns:
+// a round's is read by the peers until they come to the next one's barrier, and
+// zeroed in the round after that, before the barrier behind which it is used.
 template <bool kWeighed, class Add, class Take>
-__device__ __forceinline__ void search_round(Shared* sh, int turn, int ctas, Add add, Take take) {
+__device__ __forceinline__ void search_round(Shared* sh, int round, int ctas, Add add, Take take) {
   constexpr int kArrays = kWeighed ? 3 : 1;
+  auto& sum = sh->sum[round % 3];
   for (int i = threadIdx.x; i < kArrays * kBins; i += kThreads) (&sh->own[0][0])[i] = 0;
-  for (int i = threadIdx.x; i < 3 * kBins; i += kThreads) (&sh->sum[turn ^ 1][0][0])[i] = 0;
   if (threadIdx.x == 0) sh->bin = 0;
   __syncthreads();
   add();
   __syncthreads();
+  u64 in[kPer], mine = 0, all;
+  // A thread's bins, the highest first.
+  const int top = kBins - 1 - threadIdx.x * kPer;
+  if (ctas == 1) {
 #pragma unroll
-  for (int k = 0; k < kPer; ++k) {
-    const int bin = threadIdx.x + k * kThreads;
-    if (kWeighed) {
-      const u64 w = sh->own[0][bin] + (static_cast<u64>(sh->own[1][bin]) << 16) + (static_cast<u64>(sh->own[2][bin]) << 32);
-      if (w == 0) continue;
-      for (int r = 0; r < ctas; ++r)
+    for (int k = 0; k < kPer; ++k) {
+      in[k] = sh->own[0][top - k];
+      if (kWeighed) in[k] += (static_cast<u64>(sh->own[1][top - k]) << 16) + (static_cast<u64>(sh->own[2][top - k]) << 32);
+    }
+  } else {
+    const int share = __ffs(ctas) - 1;
+    for (int i = threadIdx.x; i < 3 * (kBins >> share); i += kThreads)
+      sh->sum[(round + 1) % 3][i / (kBins >> share)][i % (kBins >> share)] = 0;
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) {
+      const int bin = threadIdx.x + k * kThreads, owner = bin & (ctas - 1), at = bin >> share;
+      if (kWeighed) {
+        const u64 w = sh->own[0][bin] + (static_cast<u64>(sh->own[1][bin]) << 16) + (static_cast<u64>(sh->own[2][bin]) << 32);
 #pragma unroll
         for (int j = 0; j < 3; ++j) {
           const uint32_t part = static_cast<uint32_t>(w >> (24 * j)) & 0xffffffu;
-          if (part) peer_add(&sh->sum[turn][j][bin], r, part);
+          if (part) peer_add(&sum[j][at], owner, part);
         }
-    } else if (sh->own[0][bin]) {
-      for (int r = 0; r < ctas; ++r) peer_add(&sh->sum[turn][0][bin], r, sh->own[0][bin]);
+      } else if (sh->own[0][bin]) {
+        peer_add(&sum[0][at], owner, sh->own[0][bin]);
+      }
+    }
+    cluster_sync();
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) {
+      const int owner = (top - k) & (ctas - 1), at = (top - k) >> share;
+      in[k] = peer(&sum[0][at], owner);
+      if (kWeighed)
+        in[k] += (static_cast<u64>(peer(&sum[1][at], owner)) << 24) + (static_cast<u64>(peer(&sum[2][at], owner)) << 48);
     }
   }
-  cluster_sync();
-  // A thread's bins, the highest first.
-  const int top = kBins - 1 - threadIdx.x * kPer;
-  u64 in[kPer], mine = 0, all;
 #pragma unroll
-  for (int k = 0; k < kPer; ++k) {
-    in[k] = sh->sum[turn][0][top - k];
-    if (kWeighed) in[k] += (static_cast<u64>(sh->sum[turn][1][top - k]) << 24) + (static_cast<u64>(sh->sum[turn][2][top - k]) << 48);
-    mine += in[k];
-  }
+  for (int k = 0; k < kPer; ++k) mine += in[k];
   u64 before = block_scan(mine, sh->scratch, &all);
   uint32_t best = 0;  // places from the top, and one
   u64 best_before = 0, best_in = 0;
@@ -265,7 +305,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
   const int lane = threadIdx.x & 31;
   const int slice = q.run * kThreads, base = rank * slice, n = max(0, min(slice, p.vocab - base));
   if (threadIdx.x < 64) sh->powers[threadIdx.x] = kPowers.at[threadIdx.x];
-  for (int i = threadIdx.x; i < 3 * kBins; i += kThreads) (&sh->sum[0][0][0])[i] = 0;
+  for (int i = threadIdx.x; i < 9 * (kBins / 2); i += kThreads) (&sh->sum[0][0][0])[i] = 0;
   pdl_wait_prior_grid();
   pdl_launch_dependents();
   const float heat = p.temperatures ? __ldg(p.temperatures + row) : p.temperature;
@@ -301,7 +341,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
     sh->listed = 0;
   }
   cluster_sync();
-  for (int r = 0; r < ctas; ++r) m = fmaxf(m, peer(&sh->largest, r));
+  m = cluster_reduce(&sh->largest, ctas, -INFINITY, [](float a, float b) { return fmaxf(a, b); });
 
   const int first = threadIdx.x * q.run;  // of this thread's tokens
   if (m == -INFINITY) {
@@ -319,24 +359,40 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
     at = block_reduce(at, sh->scratch, [](uint32_t a, uint32_t b) { return min(a, b); });
     if (threadIdx.x == 0) sh->first = at;
     cluster_sync();
+    at = cluster_reduce(&sh->first, ctas, 0xffffffffu, [](uint32_t a, uint32_t b) { return min(a, b); });
     if (rank == 0 && threadIdx.x == 0) {
-      for (int r = 1; r < ctas; ++r) at = min(at, peer(&sh->first, r));
       p.tokens[row] = at;
       p.logprobs[row] = 0.f;
     }
     cluster_sync();
     return;
   }
+  if (m == INFINITY) {
+    // Tokens at +inf weigh one and all others nothing, whatever the temperature.
+    for (int i = threadIdx.x; i < slice; i += kThreads) x[i] = x[i] == INFINITY ? 0.f : -INFINITY;
+    largest = largest == INFINITY ? 0.f : -INFINITY;
+    m = 0.f;
+    __syncthreads();
+  }
   const double per_t = 1.4426950408889634 / fmax(static_cast<double>(heat), 1e-37);
-  Weights weight{m, static_cast<float>(per_t), 0.f, m == INFINITY, sh->powers};
+  Weights weight{m, static_cast<float>(per_t), 0.f, sh->powers};
   weight.low = static_cast<float>(per_t - weight.high);
+
+  const u64 least_w = min_p > 0.f ? static_cast<u64>(ceil(static_cast<double>(min_p) * 17592186044416.0)) : 0;
+  // The token is the first whose running sum exceeds this integer: u total, held
+  // below total.
+  const float u = fmaxf(__ldg(p.uniform + row), 0.f);
+  auto goal_of = [&](u64 total) {
+    const u64 goal = static_cast<u64>(fmin(static_cast<double>(u) * static_cast<double>(total), 9.0e18));
+    return goal < total ? goal : total - 1;
+  };
 
   // Kept: logits above `cut`, and the first `room` of those at it (or all).
   float cut = -INFINITY;
   uint32_t room = 0;
   bool all_at = true;
   bool listed = false;  // the tokens that a cut may fall on are in the list
-  int turn = 0;
+  int round = 0;
   auto each = [&](auto f) {
     if (listed) {
       for (int i = threadIdx.x, c = sh->listed; i < c; i += kThreads) f(sh->list[i]);
@@ -346,14 +402,94 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
   };
   // Lists this CTA's tokens from `least` on; a list that they do not fit is not used.
   auto make_list = [&](float least) {
-    for (int i = threadIdx.x; i < n; i += kThreads) {
-      const float v = x[i];
-      if (v < least) continue;
-      const uint32_t at = atomicAdd(&sh->listed, 1u);
-      if (at < kListed) sh->list[at] = v;
+    // (Counted first, so that a warp takes its places in the list at once.)
+    uint32_t c = 0;
+#pragma unroll 4
+    for (int i = threadIdx.x; i < slice; i += kThreads) c += x[i] >= least;
+    uint32_t sum = c, at = 0;
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+      const uint32_t t = __shfl_up_sync(0xffffffffu, sum, off);
+      if (lane >= off) sum += t;
     }
+    if (lane == 31) at = atomicAdd(&sh->listed, sum);
+    at = __shfl_sync(0xffffffffu, at, 31) + sum - c;
+    if (c && at + c <= kListed)
+#pragma unroll 4
+      for (int i = threadIdx.x; i < slice; i += kThreads)
+        if (const float v = x[i]; v >= least) {
+          sh->places[at] = static_cast<uint16_t>(i);
+          sh->list[at++] = v;
+        }
     __syncthreads();
     listed = sh->listed <= kListed;
+  };
+  // Where the row's lists hold kDirect tokens at most, the first CTA ranks them
+  // by comparing each with all, and draws: whether that was done. top_k counts
+  // where `sum` (over what top-k keeps) is not known yet.
+  auto draw_listed = [&](u64 sum) {
+    cluster_sync();
+    uint32_t before;
+    const uint32_t c = cluster_reduce(&sh->listed, ctas, 0u, [](uint32_t a, uint32_t b) { return a + b; }, rank, &before);
+    if (c > kDirect) return false;
+    Ranked* all = reinterpret_cast<Ranked*>(&sh->own[0][0]);
+    Ranks* half = reinterpret_cast<Ranks*>(all + kDirect);
+    static_assert(kDirect * (sizeof(Ranked) + sizeof(Ranks)) <= sizeof(sh->own), "lists");
+    for (uint32_t i = threadIdx.x; i < sh->listed; i += kThreads) {
+      const float v = sh->list[i];
+      const uint32_t to = map_to_rank(all + before + i, 0);
+      asm volatile("st.shared::cluster.v2.b64 [%0], {%1, %2};" ::"r"(to), "l"(weight(v)),
+                   "l"(static_cast<u64>(base + sh->places[i]) << 32 | __float_as_uint(v))
+                   : "memory");
+    }
+    cluster_sync();
+    if (rank > 0) return true;
+    // A token's half of the others, by two threads each.
+    const uint32_t me = threadIdx.x & (kDirect - 1), from = threadIdx.x >= kDirect ? c / 2 : 0;
+    const uint32_t to = threadIdx.x >= kDirect ? c : c / 2;
+    const Ranked mine = all[me < c ? me : 0];
+    Ranks r{0, 0, 0};
+    if (me < c)
+      for (uint32_t j = from; j < to; ++j) {
+        const Ranked t = all[j];
+        r.w += t.v > mine.v ? t.w : 0;
+        r.greater += t.v > mine.v;
+        r.ties += t.v == mine.v && t.place < mine.place;
+      }
+    if (threadIdx.x >= kDirect) half[me] = r;
+    __syncthreads();
+    const bool in = threadIdx.x < c;  // (of the first half of the threads: a token each)
+    if (in) {
+      r.w += half[me].w;
+      r.greater += half[me].greater;
+      r.ties += half[me].ties;
+    }
+    const auto plus = [](u64 a, u64 b) { return a + b; };
+    const u64 ahead = r.w + r.ties * mine.w;  // the sum ranked before it
+    bool keep = in && (sum > 0 || r.greater + r.ties < static_cast<uint32_t>(top_k));
+    if (sum == 0) sum = block_reduce(keep ? mine.w : 0, sh->scratch, plus);
+    if (top_p < 1.f)
+      keep &= r.greater + r.ties == 0 || static_cast<double>(ahead) < static_cast<double>(top_p) * static_cast<double>(sum);
+    keep &= mine.w >= least_w;
+    const u64 w = keep ? mine.w : 0;
+    const u64 total = block_reduce(w, sh->scratch, plus);
+    if (threadIdx.x < kDirect) all[me] = Ranked{w, mine.v, in ? mine.place : 0xffffffffu};
+    __syncthreads();
+    // Running sums in the order of the places.
+    u64 upto = 0;
+    if (me < c)
+      for (uint32_t j = from; j < to; ++j) upto += all[j].place <= mine.place ? all[j].w : 0;
+    if (threadIdx.x >= kDirect) half[me].w = upto;
+    __syncthreads();
+    if (w) {
+      upto += half[me].w;
+      const u64 goal = goal_of(total);
+      if (goal < upto && upto - w <= goal) {
+        p.tokens[row] = mine.place;
+        p.logprobs[row] = static_cast<float>(log(static_cast<double>(w) / static_cast<double>(total)));
+      }
+    }
+    return true;
   };
   // Finds the key where take(sum before) is last true among those from `low`
   // up to the largest; leaves the sums before it and at it.
@@ -363,13 +499,13 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
     while (true) {
       int shift = 0;
       while ((high - low) >> shift >= kBins) ++shift;
-      search_round<decltype(weighed)::value>(sh, turn, ctas, [&] {
+      search_round<decltype(weighed)::value>(sh, round, ctas, [&] {
         each([&](float v) {
           const uint32_t key = key_of<kDrop>(v);
           if (key >= low && key <= high) add(v, &sh->own[0][(key - low) >> shift]);
         });
       }, [&](u64 in) { return take(*before + in); });
-      turn ^= 1;
+      ++round;
       *before += sh->before;
       *inside = sh->inside;
       low += sh->bin << shift;
@@ -389,15 +525,21 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
       const uint32_t low = key_of<kDrop>(m > 0.f ? m * 0.125f : m * 8.f), high = key_of<kDrop>(m);
       int shift = 0;
       while ((high - low) >> shift >= kBins) ++shift;
-      search_round<false>(sh, turn, ctas, [&] {
+      search_round<false>(sh, round, ctas, [&] {
         const uint32_t key = key_of<kDrop>(largest);
         atomicAdd(&sh->own[0][key > low ? (key - low) >> shift : 0], 1u);
       }, [&](u64 before) { return before < static_cast<u64>(top_k); });
-      turn ^= 1;
+      ++round;
       if (sh->bin) least = value_of<kDrop>(low + (sh->bin << shift));
       __syncthreads();
     }
-    if (least > -INFINITY) make_list(least);
+    if (least > -INFINITY) {
+      make_list(least);
+      if (draw_listed(0)) {
+        cluster_sync();
+        return;
+      }
+    }
     u64 before, inside;
     cut = value_of<kDrop>(search(std::false_type(), key_of<kDrop>(least), [](float, uint32_t* bin) { atomicAdd(bin, 1u); },
                                  [&](u64 ahead) { return ahead < static_cast<u64>(top_k); }, &before, &inside));
@@ -405,46 +547,57 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
     all_at = room == inside;
   }
   if (top_p < 1.f) {
-    // The sum over what top-k keeps (all of those at its cut first), and the
-    // sums above four weights.
-    u64 sums[kLevels + 1] = {};
-    uint32_t ties = 0;
-    each([&](float v) {
-      if (v < cut) return;
-      const u64 w = weight(v);
-      ties += v == cut;
+    // The sum over what top-k keeps (all of those at its cut first), the sums
+    // above five weights, and the number of those at the cut.
+    u64 sums[kLevels + 2] = {};
+    const auto plus = [](u64 a, u64 b) { return a + b; };
+    auto take = [&](float v) {
+      const u64 w = v >= cut ? weight(v) : 0;
       sums[kLevels] += w;
+      sums[kLevels + 1] += v == cut;
 #pragma unroll
       for (int k = 0; k < kLevels; ++k)
-        if (w >= kOne >> (4 * k + 4)) sums[k] += w;
-    });
-    const u64 at_cut = cut > -INFINITY ? weight(cut) : 0;
-#pragma unroll
-    for (int k = 0; k <= kLevels; ++k) {
-      const u64 t = block_reduce(sums[k], sh->scratch, [](u64 a, u64 b) { return a + b; });
-      if (threadIdx.x == 0) sh->parts[k] = t;
+        if (w >= u64(1) << (40 - 3 * k)) sums[k] += w;
+    };
+    if (listed) {
+      each(take);
+    } else {
+#pragma unroll 4
+      for (int i = threadIdx.x; i < slice; i += kThreads) take(x[i]);
     }
-    ties = block_reduce(ties, sh->scratch, [](uint32_t a, uint32_t b) { return a + b; });
-    if (threadIdx.x == 0) sh->ties = ties;
+#pragma unroll
+    for (int k = 0; k < kLevels + 2; ++k) {
+#pragma unroll
+      for (int off = 16; off >= 1; off >>= 1) sums[k] += __shfl_xor_sync(0xffffffffu, sums[k], off);
+      if (lane == 0) sh->wide[k][threadIdx.x >> 5] = sums[k];
+    }
+    __syncthreads();
+    if (threadIdx.x < 32 * (kLevels + 2)) {
+      u64 v = lane < kWarps ? sh->wide[threadIdx.x >> 5][lane] : 0;
+#pragma unroll
+      for (int off = kWarps / 2; off >= 1; off >>= 1) v += __shfl_xor_sync(0xffffffffu, v, off);
+      if (lane == 0) sh->parts[threadIdx.x >> 5] = v;
+    }
     cluster_sync();
-    ties = 0;
 #pragma unroll
-    for (int k = 0; k <= kLevels; ++k) sums[k] = 0;
-    for (int r = 0; r < ctas; ++r) {
-#pragma unroll
-      for (int k = 0; k <= kLevels; ++k) sums[k] += peer(&sh->parts[k], r);
-      ties += peer(&sh->ties, r);
-    }
-    const u64 left_out = all_at ? 0 : (ties - room) * at_cut;
+    for (int k = 0; k < kLevels + 2; ++k) sums[k] = cluster_reduce(&sh->parts[k], ctas, u64(0), plus);
+    const u64 left_out = all_at ? 0 : (sums[kLevels + 1] - room) * weight(cut);
     const double target = static_cast<double>(top_p) * static_cast<double>(sums[kLevels] - left_out);
     float least = cut;
-    if (!listed && !weight.inf) {
+    if (!listed) {
       // Some room for the rounding of the logit that goes with a weight.
 #pragma unroll
       for (int k = kLevels - 1; k >= 0; --k)
         if (static_cast<double>(sums[k]) >= target)
-          least = fmaxf(cut, m - heat * (2.7725887f * 1.0001f) * (k + 1) - fabsf(m) * 1e-5f);
-      if (least > cut) make_list(least);
+          least = fmaxf(cut, m - heat * (0.6931472f * 1.0001f) * (3 * k + 4) - fabsf(m) * 1e-5f);
+      if (least > cut) {
+        make_list(least);
+        // (Behind a top-k that is not the whole row's its ties would count too.)
+        if (cut == -INFINITY && draw_listed(sums[kLevels])) {
+          cluster_sync();
+          return;
+        }
+      }
     }
     u64 before, inside;
     const float low = value_of<kDrop>(search(std::true_type(), key_of<kDrop>(least), [&](float v, uint32_t* bin) {
@@ -456,67 +609,99 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
     // All tokens at this logit weigh the same: of them those that have less than
     // the target before them, and one at least where nothing is before.
     const u64 w = weight(low);
-    const u64 here = low == cut && !all_at ? room : inside / w;
-    const double most = (target - static_cast<double>(before)) / static_cast<double>(w);
+    const double per = 1.0 / static_cast<double>(w), most = (target - static_cast<double>(before)) * per;
+    const u64 at_low = static_cast<u64>(static_cast<double>(inside) * per + 0.5);  // (below 2^18: exact)
+    const u64 here = low == cut && !all_at ? room : at_low;
     u64 few = most >= static_cast<double>(here) ? here : (most < 0.0 ? 0 : static_cast<u64>(most));
     while (few < here && static_cast<double>(before + few * w) < target) ++few;
     while (few > 0 && !(static_cast<double>(before + (few - 1) * w) < target)) --few;
     if (before == 0 && few == 0) few = 1;
     cut = low;
     room = static_cast<uint32_t>(few);
-    all_at = few == inside / w;
+    all_at = few == at_low;
   }
 
-  // Tokens at the cut that this thread's come behind, where not all are kept.
-  uint32_t ahead = 0;
+  // Where not all tokens at the cut are kept: the place of the last one that is.
+  int limit = slice;
   if (!all_at) {
     uint32_t ties = 0;
-    for (int j = 0; j < q.run; ++j) ties += x[first + j] == cut;
+    if (listed) {
+      for (int i = threadIdx.x; i < kThreads; i += kThreads) sh->own[0][i] = 0;
+      __syncthreads();
+      for (int i = threadIdx.x, c = sh->listed; i < c; i += kThreads)
+        if (sh->list[i] == cut) atomicAdd(&sh->own[0][sh->places[i] / q.run], 1u);
+      __syncthreads();
+      ties = sh->own[0][threadIdx.x];
+    } else {
+      for (int j = 0; j < q.run; ++j) ties += x[first + j] == cut;
+    }
     u64 all;
-    ahead = static_cast<uint32_t>(block_scan(ties, sh->scratch, &all));
+    uint32_t ahead = static_cast<uint32_t>(block_scan(ties, sh->scratch, &all)), before;
     if (threadIdx.x == 0) sh->cut_ties = static_cast<uint32_t>(all);
     cluster_sync();
-    for (int i = 0; i < rank; ++i) ahead += peer(&sh->cut_ties, i);
+    cluster_reduce(&sh->cut_ties, ctas, 0u, [](uint32_t a, uint32_t b) { return a + b; }, rank, &before);
+    ahead += before;
+    if (threadIdx.x == 0) sh->limit = before < room ? slice : -1;
+    __syncthreads();
+    if (ahead < room && room < ahead + ties) {
+      uint32_t left = room - ahead;
+      for (int j = 0; left > 0; ++j)
+        if (x[first + j] == cut && --left == 0) sh->limit = first + j;
+    } else if (ahead == room && ties > 0 && ahead > before) {
+      // The last one kept lies in an earlier run of this CTA, which ends with it.
+      atomicMin(&sh->limit, first - 1);
+    }
+    __syncthreads();
+    limit = sh->limit;
   }
-  // W of a token if it is kept; *tie: tokens at the cut before it.
-  const u64 least_w = min_p > 0.f ? static_cast<u64>(ceil(static_cast<double>(min_p) * 17592186044416.0)) : 0;
-  auto kept = [&](float v, uint32_t* tie) -> u64 {
-    if (v < cut) return 0;
-    if (v == cut && !all_at && (*tie)++ >= room) return 0;
+  // W of a token, by its place, if it is kept.
+  auto kept = [&](float v, int place) -> u64 {
+    if (v < cut || (v == cut && place > limit)) return 0;
     const u64 w = weight(v);
     return w >= least_w ? w : 0;
   };
   u64 mine = 0, total = 0;
-  {
-    uint32_t tie = ahead;
-    for (int j = 0; j < q.run; ++j) mine += kept(x[first + j], &tie);
+  if (cut == -INFINITY) {
+#pragma unroll 4
+    for (int j = 0; j < q.run; ++j) {
+      const u64 w = weight(x[first + j]);
+      mine += w >= least_w ? w : 0;
+    }
+  } else if (listed) {
+    // From the list: a run's sum in 16 bits of the weights each.
+    for (int i = threadIdx.x; i < 3 * kThreads; i += kThreads) (&sh->own[0][0])[i] = 0;
+    __syncthreads();
+    for (int i = threadIdx.x, c = sh->listed; i < c; i += kThreads) {
+      const u64 w = kept(sh->list[i], sh->places[i]);
+      uint32_t* run = &sh->own[0][sh->places[i] / q.run];
+      if (const uint32_t part = static_cast<uint32_t>(w) & 0xffffu) atomicAdd(run, part);
+      if (const uint32_t part = static_cast<uint32_t>(w >> 16) & 0xffffu) atomicAdd(run + kThreads, part);
+      if (const uint32_t part = static_cast<uint32_t>(w >> 32)) atomicAdd(run + 2 * kThreads, part);
+    }
+    __syncthreads();
+    const uint32_t* run = &sh->own[0][threadIdx.x];
+    mine = run[0] + (static_cast<u64>(run[kThreads]) << 16) + (static_cast<u64>(run[2 * kThreads]) << 32);
+  } else {
+    for (int j = 0; j < q.run; ++j) mine += kept(x[first + j], first + j);
   }
   u64 before = block_scan(mine, sh->scratch, &total);
   if (threadIdx.x == 0) sh->total = total;
   cluster_sync();
-  total = 0;
-  for (int i = 0; i < ctas; ++i) {
-    const u64 t = peer(&sh->total, i);
-    if (i < rank) before += t;
-    total += t;
+  {
+    u64 ahead_of;
+    total = cluster_reduce(&sh->total, ctas, u64(0), [](u64 a, u64 b) { return a + b; }, rank, &ahead_of);
+    before += ahead_of;
   }
-  // The first token whose running sum exceeds this integer (u total, held below total).
-  const double u = fmaxf(__ldg(p.uniform + row), 0.f);
-  u64 goal = static_cast<u64>(fmin(u * static_cast<double>(total), 9.0e18));
-  if (goal >= total) goal = total - 1;
+  const u64 goal = goal_of(total);
   const unsigned found = __ballot_sync(0xffffffffu, before <= goal && goal < before + mine);
   if (found) {
     // The warp looks through the one thread's tokens, 32 at a time.
     const int src = __ffs(found) - 1;
     before = __shfl_sync(0xffffffffu, before, src);
-    uint32_t tie = __shfl_sync(0xffffffffu, ahead, src);
     const int from = __shfl_sync(0xffffffffu, first, src);
     for (int j0 = 0; j0 < q.run; j0 += 32) {
       const float v = j0 + lane < q.run ? x[from + j0 + lane] : -INFINITY;
-      const unsigned at_cut = __ballot_sync(0xffffffffu, j0 + lane < q.run && v == cut);
-      uint32_t mine_tie = tie + __popc(at_cut & ((1u << lane) - 1));
-      const u64 w = kept(v, &mine_tie);
-      tie += __popc(at_cut);
+      const u64 w = kept(v, from + j0 + lane);
       u64 sum = w;
 #pragma unroll
       for (int off = 1; off < 32; off <<= 1) {
