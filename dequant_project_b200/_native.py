@@ -154,6 +154,11 @@ def lib() -> ctypes.CDLL:
                                             i64, i64, vp, vp, vp, i64, vp, vp]
     h.dqg_expand_pages.restype = i32
     h.dqg_expand_pages.argtypes = [qkv, vp, i64, i64, vp, vp, i64, i64, vp, vp, vp, vp]
+    h.dqg_quantized_prompt_workspace.restype = i32
+    h.dqg_quantized_prompt_workspace.argtypes = [qkv, i64, i64, i64, u64p]
+    h.dqg_quantized_prompt_attention.restype = i32
+    h.dqg_quantized_prompt_attention.argtypes = [vp, i64, i64, i64, i64, qkv, vp, i64, i64, vp, vp, vp, i64, i64, i32,
+                                                 f32, vp, vp, u64, vp]
     h.dqg_quantized_attention_workspace.restype = i32
     h.dqg_quantized_attention_workspace.argtypes = [i64, i64, i64, i64, u64p]
     h.dqg_quantized_attention.restype = i32
@@ -177,7 +182,8 @@ EXPORTED = ("dqg_last_error", "dqg_version", "dqg_add_one", "dqg_gemv", "dqg_deq
             "dqg_gemv_swiglu_supported", "dqg_rope_paged_append", "dqg_paged_attention_workspace",
             "dqg_paged_attention", "dqg_prompt_attention_workspace", "dqg_prompt_attention",
             "dqg_shared_prefix_workspace", "dqg_shared_prefix_attention", "dqg_debug_paged_starved",
-            "dqg_rope_quantized_append", "dqg_expand_pages", "dqg_quantized_attention_workspace",
+            "dqg_rope_quantized_append", "dqg_expand_pages", "dqg_quantized_prompt_workspace",
+            "dqg_quantized_prompt_attention", "dqg_quantized_attention_workspace",
             "dqg_quantized_attention", "dqg_debug_quantized_starved", "dqg_sample_tokens")
 
 

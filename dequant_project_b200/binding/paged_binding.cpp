@@ -36,6 +36,8 @@ decltype(&dqg_rope_quantized_append) p_quantized_append = nullptr;
 decltype(&dqg_expand_pages) p_expand = nullptr;
 decltype(&dqg_quantized_attention_workspace) p_quantized_bytes = nullptr;
 decltype(&dqg_quantized_attention) p_quantized = nullptr;
+decltype(&dqg_quantized_prompt_workspace) p_quantized_prompt_bytes = nullptr;
+decltype(&dqg_quantized_prompt_attention) p_quantized_prompt = nullptr;
 decltype(&dqg_sample_tokens) p_sample = nullptr;
 
 // A rejected argument: becomes RuntimeError with this message.
@@ -438,6 +440,39 @@ at::Tensor quantized_decode(PyObject* const* a, Py_ssize_t n) {
   return out;
 }
 
+// (q, cache: 6, block_table, open_slots, q_starts, kv_lens, n_pages, causal,
+//  scale, workspace)
+at::Tensor quantized_prompt(PyObject* const* a, Py_ssize_t n) {
+  arguments(n, 15);
+  const at::Tensor& q = tensor(a[0], "q");
+  const Quantized c = quantized(a + 1);
+  const at::Tensor &table = tensor(a[7], "block_table"), &open = tensor(a[8], "open_slots");
+  const at::Tensor &starts = tensor(a[9], "q_starts"), &lens = tensor(a[10], "kv_lens");
+  const int64_t pages = integer(a[11]);
+  const int causal = PyObject_IsTrue(a[12]);
+  forward_only_cache(q, c);
+  same(c, q, "q");
+  if (q.dim() != 3 || q.size(2) != c.kv.head_dim || q.stride(2) != 1)
+    reject("q must be [rows, heads, %d] with the head dimension contiguous", static_cast<int>(c.kv.head_dim));
+  const int64_t t = q.size(0), hq = q.size(1), d = q.size(2);
+  ints(c, lens, "kv_lens", at::kInt, 1, -1);
+  const int64_t b = lens.size(0);
+  ints(c, table, "block_table", at::kInt, 2, b);
+  ints(c, open, "open_slots", at::kInt, 1, b);
+  ints(c, starts, "q_starts", at::kInt, 1, b + 1);
+  const float scale = scale_of(a[13], d);
+  c10::cuda::CUDAGuard guard(static_cast<c10::DeviceIndex>(c.device));
+  uint64_t need = 0;
+  check(p_quantized_prompt_bytes(&c.kv, b, table.size(1), pages, &need));
+  const Scratch ws = scratch(a[14], need, q);
+  at::Tensor out = at::empty({t, hq, d}, q.options());
+  check(p_quantized_prompt(q.data_ptr(), q.stride(0), q.stride(1), t, hq, &c.kv, table.data_ptr<int32_t>(),
+                           table.size(1), row_stride(table), open.data_ptr<int32_t>(), starts.data_ptr<int32_t>(),
+                           lens.data_ptr<int32_t>(), b, pages, causal, scale, out.data_ptr(), ws.ptr, ws.bytes,
+                           stream_of(c.device)));
+  return out;
+}
+
 // A parameter of the draw: a number for all rows, or a tensor of one a row.
 template <typename T>
 void parameter(PyObject* o, const at::Tensor& logits, const char* name, const T** each, T* all) {
@@ -520,7 +555,7 @@ void set(F*& entry, void* address) {
 
 // Addresses of the library's entry points, in the order below.
 PyObject* bind(PyObject*, PyObject* const* args, Py_ssize_t n) {
-  constexpr int kEntries = 13;
+  constexpr int kEntries = 15;
   void* at[kEntries];
   if (n != kEntries) {
     PyErr_Format(PyExc_TypeError, "bind takes %d addresses", kEntries);
@@ -545,6 +580,8 @@ PyObject* bind(PyObject*, PyObject* const* args, Py_ssize_t n) {
   set(p_quantized_bytes, at[10]);
   set(p_quantized, at[11]);
   set(p_sample, at[12]);
+  set(p_quantized_prompt_bytes, at[13]);
+  set(p_quantized_prompt, at[14]);
   set(p_last_error, at[0]);
   Py_RETURN_NONE;
 }
@@ -558,6 +595,7 @@ PyMethodDef methods[] = {METHOD("bind", bind),
                          METHOD("rope_quantized_append", call<quantized_append>),
                          METHOD("expand_pages", call<expand>),
                          METHOD("quantized_attention", call<quantized_decode>),
+                         METHOD("quantized_prompt_attention", call<quantized_prompt>),
                          METHOD("sample_tokens", call<sample>),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_paged_binding", nullptr, -1, methods,

@@ -113,6 +113,32 @@ inline int make_map(CUtensorMap* map, const void* base, CUtensorMapDataType type
   return DQG_OK;
 }
 
+// A map of values of the pools' type, in boxes of 64 values a row.
+inline int pool_map(CUtensorMap* map, const void* base, const dqg::PagedPool& pool, const int64_t (&size)[4],
+             const int64_t (&stride)[3], int rows1, int rows2, int rows3, const char* name) {
+  return make_map(map, base, pool.bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, size,
+                  stride, 64, rows1, rows2, rows3, CU_TENSOR_MAP_SWIZZLE_128B, name);
+}
+
+inline int pool_maps(const dqg::PagedPool& pool, int rows, CUtensorMap* k, CUtensorMap* v) {
+  const int64_t size[4] = {pool.D, pool.page_size, pool.n_kv_heads, pool.n_pages};
+  const int64_t stride[3] = {pool.row_stride, pool.head_stride, pool.page_stride};
+  int rc = pool_map(k, pool.k, pool, size, stride, rows, 1, 1, "k_pages");
+  if (rc) return rc;
+  return pool_map(v, pool.v, pool, size, stride, rows, 1, 1, "v_pages");
+}
+
+// Queries [T, kv heads, g, D]: boxes of a tile's tokens, times the KV head's
+// query heads, times 64 values.
+inline int query_map(const void* q, const dqg::PagedPool& pool, int64_t T, int64_t hq, int64_t stride_row,
+              int64_t stride_head, CUtensorMap* map) {
+  const int64_t g = hq / pool.n_kv_heads;
+  const int64_t size[4] = {pool.D, g, pool.n_kv_heads, T};
+  const int64_t stride[3] = {stride_head, g * stride_head, stride_row};
+  return pool_map(map, q, pool, size, stride, static_cast<int>(g), 1,
+                  dqg::prompt_tokens_per_tile(static_cast<int>(hq), pool.n_kv_heads), "q");
+}
+
 constexpr double kLog2e = 1.4426950408889634;
 
 inline int current(int* dev, int* sms) {

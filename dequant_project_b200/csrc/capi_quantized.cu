@@ -79,6 +79,12 @@ int check_quantized(const dqg_quantized_kv* kv, dqg::QuantizedPool* pool) {
   return DQG_OK;
 }
 
+int check_expanded(int64_t n_seqs, int64_t n_pages) {
+  if (n_seqs < 0 || n_seqs > (1 << 20)) return api_fail(DQG_ERR_INVALID, "n_seqs=%lld out of range", (ll)n_seqs);
+  if (n_pages < 0 || n_pages > (1 << 24)) return api_fail(DQG_ERR_INVALID, "n_pages=%lld out of range", (ll)n_pages);
+  return DQG_OK;
+}
+
 int check_seqs(const int32_t* table, int64_t width, int64_t stride, const int32_t* open_slots, const int32_t* lens,
                int64_t n_seqs, dqg::QuantizedSeqs* seqs) {
   int rc = check_table(table, width, stride, "block_table");
@@ -165,8 +171,7 @@ int dqg_expand_pages(const dqg_quantized_kv* kv, const int32_t* block_table, int
   dqg::QuantizedSeqs seqs;
   int rc = check_quantized(kv, &pool);
   if (rc) return rc;
-  if (n_seqs < 0 || n_seqs > (1 << 20)) return api_fail(DQG_ERR_INVALID, "n_seqs=%lld out of range", (ll)n_seqs);
-  if (n_pages < 0 || n_pages > (1 << 24)) return api_fail(DQG_ERR_INVALID, "n_pages=%lld out of range", (ll)n_pages);
+  if ((rc = check_expanded(n_seqs, n_pages)) != DQG_OK) return rc;
   if (n_seqs == 0) return api_ok();
   if ((rc = check_seqs(block_table, table_width, table_stride, open_slots, kv_lens, n_seqs, &seqs)) != DQG_OK)
     return rc;
@@ -174,8 +179,116 @@ int dqg_expand_pages(const dqg_quantized_kv* kv, const int32_t* block_table, int
   if (n_pages > 0 && ((rc = check_ptr(k_out, 16, "k_out")) != DQG_OK || (rc = check_ptr(v_out, 16, "v_out")) != DQG_OK))
     return rc;
   const cudaError_t e =
-      dqg::launch_expand_pages(pool, seqs, n_pages, k_out, v_out, table_out, static_cast<cudaStream_t>(stream));
+      dqg::launch_expand_pages(pool, seqs, n_pages, k_out, v_out, table_out, nullptr, 0, static_cast<cudaStream_t>(stream));
   if (e != cudaSuccess) return api_cuda_fail(e, "expand_pages launch");
+  return api_ok();
+}
+
+}  // extern "C"
+
+namespace {
+// What a prompt call leaves between its kernels.
+struct PromptScratch {
+  uint64_t k, v, table, scales, pieces, bytes;  // offsets, and all of it
+  int64_t scale_stride, n_pages;
+};
+PromptScratch prompt_scratch(const dqg::QuantizedPool& pool, int64_t n_seqs, int64_t table_width, int64_t n_pages,
+                             int sms) {
+  if (n_pages == 0) n_pages = 1;  // no position at all: a page for the maps, which nothing reads
+  const auto up = [](uint64_t n) { return (n + 255) / 256 * 256; };
+  const uint64_t pages = up(static_cast<uint64_t>(n_pages) * pool.n_kv_heads * pool.page_size * pool.D * 2);
+  PromptScratch s;
+  s.n_pages = n_pages;
+  s.scale_stride = (n_pages * (pool.page_size / 16) + 7) / 8 * 8 + 8 * (n_seqs + 1);
+  s.k = 0;
+  s.v = pages;
+  s.table = 2 * pages;
+  s.scales = s.table + up(static_cast<uint64_t>(n_seqs) * table_width * 4);
+  s.pieces = s.scales + up(static_cast<uint64_t>(s.scale_stride) * pool.n_kv_heads * 4);
+  s.bytes = s.pieces + dqg::prompt_workspace(pool.D, sms);
+  return s;
+}
+}  // namespace
+
+extern "C" {
+
+int dqg_quantized_prompt_workspace(const dqg_quantized_kv* kv, int64_t n_seqs, int64_t table_width, int64_t n_pages,
+                                   uint64_t* bytes) {
+  if (bytes == nullptr) return api_fail(DQG_ERR_INVALID, "bytes must not be null");
+  dqg::QuantizedPool pool;
+  int rc = check_quantized(kv, &pool);
+  if (rc) return rc;
+  if ((rc = check_expanded(n_seqs, n_pages)) != DQG_OK) return rc;
+  if (table_width < 1 || table_width > (int64_t(1) << 26))
+    return api_fail(DQG_ERR_INVALID, "table_width=%lld out of range", (ll)table_width);
+  int dev = 0, sms = 0;
+  if ((rc = current(&dev, &sms)) != DQG_OK) return rc;
+  *bytes = prompt_scratch(pool, n_seqs, table_width, n_pages, sms).bytes;
+  return api_ok();
+}
+
+int dqg_quantized_prompt_attention(const void* q, int64_t q_stride_row, int64_t q_stride_head, int64_t T,
+                                   int64_t n_q_heads, const dqg_quantized_kv* kv, const int32_t* block_table,
+                                   int64_t table_width, int64_t table_stride, const int32_t* open_slots,
+                                   const int32_t* q_starts, const int32_t* kv_lens, int64_t n_seqs, int64_t n_pages,
+                                   int causal, float scale, void* out, void* workspace, uint64_t workspace_bytes,
+                                   void* stream) {
+  dqg::QuantizedPool pool;
+  dqg::QuantizedSeqs seqs;
+  int rc = check_quantized(kv, &pool);
+  if (rc) return rc;
+  if ((rc = check_heads(n_q_heads, pool.n_kv_heads)) != DQG_OK) return rc;
+  if (T < 0 || T > (1 << 28)) return api_fail(DQG_ERR_INVALID, "T=%lld out of range", (ll)T);
+  if ((rc = check_expanded(n_seqs, n_pages)) != DQG_OK) return rc;
+  if (T == 0 || n_seqs == 0) return api_ok();
+  if ((rc = check_query(q, T, n_q_heads, q_stride_row, q_stride_head, pool.D)) != DQG_OK) return rc;
+  if ((rc = check_seqs(block_table, table_width, table_stride, open_slots, kv_lens, n_seqs, &seqs)) != DQG_OK)
+    return rc;
+  if ((rc = check_ptr(q_starts, 4, "q_starts")) != DQG_OK) return rc;
+  if ((rc = check_ptr(out, 16, "out")) != DQG_OK) return rc;
+  if ((rc = check_scale(scale)) != DQG_OK) return rc;
+  int dev = 0, sms = 0;
+  if ((rc = current(&dev, &sms)) != DQG_OK) return rc;
+  const PromptScratch s = prompt_scratch(pool, n_seqs, table_width, n_pages, sms);
+  if ((rc = check_workspace(workspace, workspace_bytes, s.bytes)) != DQG_OK) return rc;
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  int32_t* table = reinterpret_cast<int32_t*>(ws + s.table);
+  dqg::PagedPool pages;
+  pages.k = ws + s.k;
+  pages.v = ws + s.v;
+  pages.n_pages = s.n_pages;
+  pages.row_stride = pool.D;
+  pages.head_stride = static_cast<int64_t>(pool.page_size) * pool.D;
+  pages.page_stride = pool.n_kv_heads * pages.head_stride;
+  pages.n_kv_heads = pool.n_kv_heads;
+  pages.page_size = pool.page_size;
+  pages.D = pool.D;
+  pages.bf16 = pool.bf16;
+  CUtensorMap qmap, kmap, vmap;
+  if ((rc = query_map(q, pages, T, n_q_heads, q_stride_row, q_stride_head, &qmap)) != DQG_OK) return rc;
+  if ((rc = pool_maps(pages, dqg::prompt_box_rows(pages.page_size), &kmap, &vmap)) != DQG_OK) return rc;
+  float* scales = reinterpret_cast<float*>(ws + s.scales);
+  cudaError_t e = dqg::launch_expand_pages(pool, seqs, s.n_pages, ws + s.k, ws + s.v, table, scales, s.scale_stride,
+                                           static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return api_cuda_fail(e, "quantized_prompt_attention launch");
+  dqg::PromptArgs a;
+  std::memset(&a, 0, sizeof(a));
+  a.table = table;
+  a.table_stride = table_width;
+  a.table_width = static_cast<int>(table_width);
+  a.q_starts = q_starts;
+  a.kv_lens = kv_lens;
+  a.out = out;
+  a.workspace = ws + s.pieces;
+  a.B = static_cast<int>(n_seqs);
+  a.T = static_cast<int>(T);
+  a.hq = static_cast<int>(n_q_heads);
+  a.causal = causal != 0;
+  a.scale_log2 = static_cast<float>(scale * kLog2e);
+  a.k_scales = scales;
+  a.scale_stride = s.scale_stride;
+  e = dqg::launch_prompt(pages, qmap, kmap, vmap, a, sms, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return api_cuda_fail(e, "quantized_prompt_attention launch");
   return api_ok();
 }
 

@@ -5,9 +5,11 @@
 //   zeros behind a sequence's end
 //
 // so that the operators over 16-bit pages can read them. Attention of prompts
-// goes this way: in its product loop the codes would be expanded once for
-// every 256 rows (and by warps that share their issue slots with the softmax
-// that bounds it), here once for all.
+// goes this way too, with keys as codes (exact in 16 bits) whose scales the
+// prompt kernel applies to its scores: key values rounded to bf16 would move a
+// score by 2^-9 of itself. In the product loop the codes would be expanded once
+// for every 256 rows (and by warps that share their issue slots with the
+// softmax that bounds it), here once for all.
 //
 // Bound by HBM: a byte read and two written a value. A block takes one page of
 // one head, sixteen values a thread at a time.
@@ -27,6 +29,8 @@ struct Params {
   void* k_out;
   void* v_out;
   int32_t* table_out;
+  float* k_scales;       // keys as codes: their scales (see PromptArgs), or null
+  int64_t scale_stride;
   int64_t n_pages;
   int page_shift, block_shift, len_limit;
 };
@@ -96,6 +100,14 @@ __global__ void __launch_bounds__(kThreads) expand_pages_kernel(const __grid_con
   }
   const int n8 = bad_page ? 0 : min(page_size, max(0, done - base));  // rows in 8 bits
   const int n16 = bad_slot ? n8 : min(page_size, len - base);         // and open ones behind them
+  const bool raw = p.k_scales != nullptr;
+  if (raw) {
+    float* to = p.k_scales + kvh * p.scale_stride + scaled_keys_begin(static_cast<int>(u - in), page_size, b) + base / 16;
+    for (int i = threadIdx.x; i < page_size / 16; i += kThreads)
+      to[i] = 16 * i < n8 ? __ldg(p.pool.k_scale + page * p.pool.scale_page_stride + kvh * p.pool.scale_head_stride +
+                                  (16 * i >> p.block_shift))
+                          : 1.f;
+  }
   for (int which = 0; which < 2; ++which) {
     const uint8_t* codes = static_cast<const uint8_t*>(which ? p.pool.v : p.pool.k) + page * p.pool.page_stride +
                            kvh * p.pool.head_stride;
@@ -109,7 +121,7 @@ __global__ void __launch_bounds__(kThreads) expand_pages_kernel(const __grid_con
       uint4 lo = make_uint4(0, 0, 0, 0), hi = lo;
       if (row < n8) {
         const uint4 w = __ldcs(reinterpret_cast<const uint4*>(codes + row * p.pool.row_stride + c * 16));
-        const float scale = __ldg(scales + (row >> p.block_shift));
+        const float scale = raw && !which ? 1.f : __ldg(scales + (row >> p.block_shift));
         const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
         float f[16];
 #pragma unroll
@@ -150,8 +162,11 @@ cudaError_t launch(const Params& p, cudaStream_t stream) {
 }  // namespace
 
 cudaError_t launch_expand_pages(const QuantizedPool& pool, const QuantizedSeqs& seqs, int64_t n_pages, void* k_out,
-                                void* v_out, int32_t* table_out, cudaStream_t stream) {
+                                void* v_out, int32_t* table_out, float* k_scales, int64_t scale_stride,
+                                cudaStream_t stream) {
   Params p;
+  p.k_scales = k_scales;
+  p.scale_stride = scale_stride;
   p.pool = pool;
   p.seqs = seqs;
   p.k_out = k_out;

@@ -86,7 +86,16 @@ struct PromptArgs {
   // A prefix: T rows see the same prefix_len keys of one table row; the
   // pieces go to the workspace as PrefixPieces describes. 0: a prompt.
   int prefix_len;
+  // Keys that are codes: fp32 scales, one for every sixteen positions, of KV
+  // head h at h * scale_stride and of sequence b from
+  // scaled_keys_begin(table[b][0], page size, b) on. Null: none.
+  const float* k_scales;
+  int64_t scale_stride;
 };
+// (Multiples of eight, and apart for sequences whose pages follow one another.)
+inline __host__ __device__ int scaled_keys_begin(int first_page, int page_size, int b) {
+  return (first_page * (page_size / 16) + 7) / 8 * 8 + 8 * b;
+}
 size_t prompt_workspace(int D, int num_sms);
 size_t prefix_workspace(int n_seqs, int hq, int n_kv_heads, int D, int prefix_len, int num_sms);
 int prefix_splits(int n_seqs, int hq, int n_kv_heads, int prefix_len, int num_sms);

@@ -104,6 +104,8 @@ struct Params {
   uint32_t g_magic;                   // ceil(2^32 / g), 0 for g = 1
   bool n_units32;                     // the units of any lengths fit 31 bits
   int prefix_len, splits, n_pieces;   // a shared prefix: splits > 0
+  const float* k_scales;              // scaled keys: see PromptArgs
+  int64_t scale_stride;
 };
 
 // ------------------------------------------------------------ tensor cores
@@ -189,6 +191,15 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
       "fma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
       : "=f"(d.x), "=f"(d.y)
       : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 a, b, d;\n\t"
+      "mov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+      "mul.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
   return d;
 }
 __device__ __forceinline__ float2 add2(float2 a, float2 b) {
@@ -368,6 +379,7 @@ struct Segment {
   int b;                              // sequence
   int from, check;                    // the value warps look at keys >= from, in blocks >= check
   int tainted;                        // such a key's values were not finite (set by the value warps)
+  int scales;                         // scaled keys: where the sequence's scales begin
 };
 // Blocks of a segment that tile t takes part in.
 __device__ __forceinline__ int tile_count(const Segment& g, int t) {
@@ -556,7 +568,7 @@ __device__ __noinline__ void take_non_finite(const Params& p, const Segment& g, 
   tmem_wait_st();
 }
 
-template <typename E, int D>
+template <typename E, int D, bool kScaled>
 __global__ void __launch_bounds__(kThreads, 1)
     prompt_kernel(const __grid_constant__ Params p, const __grid_constant__ CUtensorMap qmap,
                   const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
@@ -652,6 +664,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (lane == 0) {
           if (!more) g.x0 = g.x1 = 0;  // the end
           g.b = b;
+          if (kScaled && more)
+            g.scales = g.kv > 0 ? scaled_keys_begin(__ldg(p.table + b * p.table_stride), 1 << p.page_shift, b) : 0;
           g.tainted = 0;
           segs[sg] = g;
           mbar_arrive(seg_full + sg);
@@ -853,6 +867,17 @@ __global__ void __launch_bounds__(kThreads, 1)
       float m = -INFINITY, l = 0.f;
       for (int j = 0; j < n; ++j) {
         const int k0 = (x0 + j) * kBlock;
+        float4 ks[2] = {};
+        if (kScaled) {
+          // Keys are codes: their scales, one for every sixteen, go to the scores.
+          // (A sequence whose pages found no room may point anywhere.)
+          const int64_t at = static_cast<int64_t>(g.scales) + k0 / 16;
+          if (at >= 0 && at + 8 <= p.scale_stride) {
+            const float4* from = reinterpret_cast<const float4*>(p.k_scales + g.kvh * p.scale_stride + at);
+            ks[0] = __ldg(from);
+            ks[1] = __ldg(from + 1);
+          }
+        }
         if (!warp_wait(s_full + t, scores & 1)) {
           ok = false;
           break;
@@ -866,6 +891,19 @@ __global__ void __launch_bounds__(kThreads, 1)
         tmem_wait_ld();
 #pragma unroll
         for (int q = 0; q < 4; ++q) hold32(raw + 32 * q);
+        if (kScaled) {
+          // (Before any score is hidden: a block that the row does not see may
+          // have any scale. Applied to groups' maxima and in the weights' first
+          // product instead, the scales would be fewer instructions, but more
+          // registers than there are: 2048 tokens 82 us instead of 74.)
+          const float f[8] = {ks[0].x, ks[0].y, ks[0].z, ks[0].w, ks[1].x, ks[1].y, ks[1].z, ks[1].w};
+#pragma unroll
+          for (int i = 0; i < kBlock; i += 2) {
+            const float2 x = mul2(make_float2(s[i], s[i + 1]), make_float2(f[i / 16], f[i / 16]));
+            s[i] = x.x;
+            s[i + 1] = x.y;
+          }
+        }
         if (k0 + kBlock > seen) {
           const int left = limit - k0;
 #pragma unroll
@@ -1087,7 +1125,7 @@ __global__ void __launch_bounds__(32 * (D / 8)) prompt_join_kernel(const __grid_
                             (static_cast<int64_t>(tok0 + tok) * p.hq + kvh * p.g + r % p.g) * D + 8 * d8) = w;
 }
 
-template <typename E, int D>
+template <typename E, int D, bool kScaled>
 cudaError_t launch(const Params& p, const CUtensorMap& qmap, const CUtensorMap& kmap,
                    const CUtensorMap& vmap, int num_sms, cudaStream_t stream) {
   static int configured[64] = {0};
@@ -1095,7 +1133,7 @@ cudaError_t launch(const Params& p, const CUtensorMap& qmap, const CUtensorMap& 
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
   if (dev < 0 || dev >= 64 || !configured[dev]) {
-    e = cudaFuncSetAttribute(prompt_kernel<E, D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    e = cudaFuncSetAttribute(prompt_kernel<E, D, kScaled>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                              Layout<D>::kSmem);
     if (e != cudaSuccess) return e;
     if (dev >= 0 && dev < 64) configured[dev] = 1;
@@ -1110,12 +1148,22 @@ cudaError_t launch(const Params& p, const CUtensorMap& qmap, const CUtensorMap& 
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  e = cudaLaunchKernelEx(&cfg, prompt_kernel<E, D>, p, qmap, kmap, vmap);
+  e = cudaLaunchKernelEx(&cfg, prompt_kernel<E, D, kScaled>, p, qmap, kmap, vmap);
   if (e != cudaSuccess || p.splits) return e;
   cfg.gridDim = dim3(num_sms, 8);
   cfg.blockDim = dim3(32 * (D / 8));
   cfg.dynamicSmemBytes = 0;
   return cudaLaunchKernelEx(&cfg, prompt_join_kernel<E, D>, p);
+}
+
+template <bool kScaled>
+cudaError_t launch_for(const Params& p, const PagedPool& pool, const CUtensorMap& qmap, const CUtensorMap& kmap,
+                       const CUtensorMap& vmap, int num_sms, cudaStream_t stream) {
+  if (pool.bf16)
+    return pool.D == 128 ? launch<__nv_bfloat16, 128, kScaled>(p, qmap, kmap, vmap, num_sms, stream)
+                         : launch<__nv_bfloat16, 64, kScaled>(p, qmap, kmap, vmap, num_sms, stream);
+  return pool.D == 128 ? launch<__half, 128, kScaled>(p, qmap, kmap, vmap, num_sms, stream)
+                       : launch<__half, 64, kScaled>(p, qmap, kmap, vmap, num_sms, stream);
 }
 
 size_t slot_bytes(int D) { return 256 * static_cast<size_t>(D) * 4 + 512 * 4; }
@@ -1206,11 +1254,10 @@ cudaError_t launch_prompt(const PagedPool& pool, const CUtensorMap& qmap, const 
   p.part = static_cast<float4*>(a.workspace);
   p.ml = reinterpret_cast<float*>(p.part + slots * 64 * pool.D);
   p.desc = reinterpret_cast<Desc*>(p.ml + slots * 512);
-  if (pool.bf16)
-    return pool.D == 128 ? launch<__nv_bfloat16, 128>(p, qmap, kmap, vmap, num_sms, stream)
-                         : launch<__nv_bfloat16, 64>(p, qmap, kmap, vmap, num_sms, stream);
-  return pool.D == 128 ? launch<__half, 128>(p, qmap, kmap, vmap, num_sms, stream)
-                       : launch<__half, 64>(p, qmap, kmap, vmap, num_sms, stream);
+  p.k_scales = a.k_scales;
+  p.scale_stride = a.scale_stride;
+  return a.k_scales ? launch_for<true>(p, pool, qmap, kmap, vmap, num_sms, stream)
+                    : launch_for<false>(p, pool, qmap, kmap, vmap, num_sms, stream);
 }
 
 }  // namespace dqg

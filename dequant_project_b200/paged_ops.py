@@ -52,7 +52,7 @@ def _binding():
             "dqg_paged_attention", "dqg_prompt_attention_workspace", "dqg_prompt_attention",
             "dqg_shared_prefix_workspace", "dqg_shared_prefix_attention", "dqg_rope_quantized_append",
             "dqg_expand_pages", "dqg_quantized_attention_workspace", "dqg_quantized_attention",
-            "dqg_sample_tokens")))
+            "dqg_sample_tokens", "dqg_quantized_prompt_workspace", "dqg_quantized_prompt_attention")))
         _bound = _paged_binding
     return _bound
 

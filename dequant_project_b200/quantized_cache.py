@@ -27,6 +27,7 @@ The reference has none of this; it models the cache's bytes
 
 from __future__ import annotations
 
+import ctypes
 import math
 from typing import NamedTuple
 
@@ -208,8 +209,30 @@ def quantized_prompt_attention(q: torch.Tensor, cache: QuantizedCache, block_tab
                                *, causal: bool = True, scale: float | None = None,
                                workspace: torch.Tensor | None = None) -> torch.Tensor:
     """``paged_ops.prompt_attention`` over an 8-bit cache, whose positions are
-    first expanded once to 16-bit pages (``expanded_pages``, which says what
-    ``n_pages`` is; they take n_pages * 4 * Hkv * page size * D bytes while the
-    call runs). Everything else as ``prompt_attention``."""
-    k, v, table = expanded_pages(cache, block_table, open_slots, kv_lens, n_pages)
-    return paged.prompt_attention(q, k, v, table, q_starts, kv_lens, causal=causal, scale=scale, workspace=workspace)
+    first expanded once to 16-bit pages (as ``expanded_pages``, which says what
+    ``n_pages`` is; but keys stay codes, and their scales go to the scores).
+    ``workspace``: ``quantized_prompt_workspace``, mostly n_pages * 4 * Hkv *
+    page size * D bytes; calls that share one must not overlap. Everything else
+    as ``prompt_attention``."""
+    if q.is_cuda:
+        return paged._binding().quantized_prompt_attention(q, *cache, block_table, open_slots, q_starts, kv_lens,
+                                                           n_pages, causal, scale, workspace)
+    paged._forward_only(q, *cache)
+    scale = 1.0 / math.sqrt(q.shape[2]) if scale is None else scale
+    out = torch.zeros_like(q)
+    for b in range(kv_lens.shape[0]):
+        lo, hi, n = int(q_starts[b]), int(q_starts[b + 1]), int(kv_lens[b])
+        ends = n - (hi - lo) + torch.arange(hi - lo) + 1 if causal else torch.full((hi - lo,), n)
+        k, v = (_rows(cache, w, block_table[b], int(open_slots[b]), n) for w in (0, 1))
+        out[lo:hi] = paged._cpu_attention(q[lo:hi].float(), k, v.to(q.dtype).float(), ends, scale).to(q.dtype)
+    return out
+
+
+def quantized_prompt_workspace(cache: QuantizedCache, n_seqs: int, table_width: int, n_pages: int) -> torch.Tensor:
+    """Scratch memory for ``quantized_prompt_attention`` calls of these sizes
+    (``table_width``: block_table's) and any lengths."""
+    kv = _native.QuantizedKV(*(t.data_ptr() for t in cache), *cache.k.shape, cache.block, cache.k_open.shape[0],
+                             *cache.k.stride()[:3], *cache.k_scale.stride()[:2], *cache.k_open.stride()[:2],
+                             int(cache.k.dtype == torch.float8_e4m3fn), int(cache.k_open.dtype == torch.bfloat16))
+    return paged._bytes(cache.k.device, _native.lib().dqg_quantized_prompt_workspace, ctypes.byref(kv), n_seqs,
+                        table_width, n_pages)

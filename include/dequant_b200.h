@@ -517,6 +517,25 @@ int dqg_expand_pages(const dqg_quantized_kv *kv, const int32_t *block_table, int
                      void *stream);
 
 /*
+ * dqg_prompt_attention over such a cache. The sequences' positions are first
+ * expanded once, into the workspace, as dqg_expand_pages does, but with keys as
+ * codes, which are exact in 16 bits; their scales are applied to the scores in
+ * fp32. n_pages as there; what sequences give that it leaves pages of out is
+ * undefined. Workspace: dqg_quantized_prompt_workspace's bytes (mostly n_pages
+ * pages of n_kv_heads * page_size * head_dim * 4 bytes), 16-byte aligned, of any
+ * contents; calls that share one must not overlap.
+ */
+int dqg_quantized_prompt_workspace(const dqg_quantized_kv *kv, int64_t n_seqs, int64_t table_width,
+                                   int64_t n_pages, uint64_t *bytes);
+int dqg_quantized_prompt_attention(const void *q, int64_t q_stride_row, int64_t q_stride_head,
+                                   int64_t T, int64_t n_q_heads, const dqg_quantized_kv *kv,
+                                   const int32_t *block_table, int64_t table_width,
+                                   int64_t table_stride, const int32_t *open_slots,
+                                   const int32_t *q_starts, const int32_t *kv_lens, int64_t n_seqs,
+                                   int64_t n_pages, int causal, float scale, void *out,
+                                   void *workspace, uint64_t workspace_bytes, void *stream);
+
+/*
  * dqg_paged_attention over such a cache. Products use the codes as they are
  * (exact in 16 bits); scales are applied to scores and weights in fp32.
  */

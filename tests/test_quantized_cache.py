@@ -54,11 +54,11 @@ def test_prompt_cut_in_any_way_gives_the_same_cache_and_attention(block, page, c
         assert bool(((a - b).float().abs() <= (rel + 2.0 ** -10) * a.float().abs() + 0.51 * step).all())
     out = qc.quantized_prompt_attention(queries[0], caches[0], table, ints(1), ints(0, n), ints(n), -(-n // page))
     want = paged_ops.prompt_attention(queries[0], ek, ev, et, ints(0, n), ints(n))
-    assert torch.equal(out, want)
     last = qc.quantized_attention(queries[0][-1:], caches[0], table, ints(1), ints(n))
     # (The expanded pages' values are rounded to fp16 once more: 2^-11 of each, and of the scores' keys.)
-    e = 2.0 ** -11 * float(queries[0][-1].float().norm(dim=-1).max() * ek.float().norm(dim=-1).max()) / math.sqrt(d)
-    assert float((last[0] - out[-1]).abs().max()) <= (2.0 ** -10 + math.expm1(2 * e)) * float(ev.abs().max())
+    e = 2.0 ** -11 * float(queries[0].float().norm(dim=-1).max() * ek.float().norm(dim=-1).max()) / math.sqrt(d)
+    assert float((out - want).abs().max()) <= (2.0 ** -10 + math.expm1(2 * e)) * float(ev.abs().max())
+    assert float((last[0] - out[-1]).abs().max()) <= 2.0 ** -9 * float(ev.abs().max())
 
 
 def test_a_block_with_a_value_that_is_not_finite_reads_as_nan():

@@ -422,10 +422,9 @@ def test_decode(cuda_device, lens, hq, hkv, d, page, block, codes, dtype):
     ([33, 260], [33, 1000], 28, 4, 128, 256, 64, torch.int8),
 ], ids=lambda v: str(v)[:30])
 def test_prompt(cuda_device, ql, kl, hq, hkv, d, page, block, codes, causal, dtype):
-    """As the decode step, with keys and values rounded to 16 bits once more:
-    a value by u of itself, below u max|v| in the output, and a key so that its
-    score changes by u |q||k| / sqrt(d) at most: with e = that, an output by (exp(2e) - 1)
-    max|v| at most."""
+    """As the decode step, with exact queries, but values rounded to 16 bits:
+    by u of themselves (or half of fp16's smallest step), below u max|v| in the
+    output."""
     gen = torch.Generator(device=cuda_device).manual_seed(sum(ql) + hq)
     cache, table, slots = make_cache(gen, kl, hkv, d, page, block, codes, dtype, cuda_device)
     starts = ints([0] + torch.tensor(ql).cumsum(0).tolist(), cuda_device)
@@ -433,6 +432,10 @@ def test_prompt(cuda_device, ql, kl, hq, hkv, d, page, block, codes, causal, dty
     n_pages = sum(-(-n // page) for n in kl)
     out = qc.quantized_prompt_attention(q, cache, table, slots, starts, ints(kl, cuda_device), n_pages, causal=causal)
     assert _native.device_status(cuda_device.index, reset=True) == 0
+    ws = qc.quantized_prompt_workspace(cache, len(kl), table.shape[1], n_pages).fill_(255)
+    for _ in range(3):
+        assert torch.equal(qc.quantized_prompt_attention(q, cache, table, slots, starts, ints(kl, cuda_device), n_pages,
+                                                         causal=causal, workspace=ws), out)
     u = U[dtype]
     for b, (n_q, n) in enumerate(zip(ql, kl)):
         if n_q == 0:
@@ -443,23 +446,47 @@ def test_prompt(cuda_device, ql, kl, hq, hkv, d, page, block, codes, causal, dty
                 else torch.full((n_q,), n, device=cuda_device))
         ref = attend64(q[lo:lo + n_q], k, v, ends, 1 / math.sqrt(d))
         v_max = float(v.abs().max()) if n else 0.0
-        k_max = float(k.norm(dim=-1).max()) if n else 0.0
-        e = u * float(q[lo:lo + n_q].float().norm(dim=-1).max()) * k_max / math.sqrt(d)
-        lim = u * ref.abs() + (2 * u + 2.0 ** -13 + math.expm1(2 * e)) * v_max + 1e-7
+        lim = u * ref.abs() + (2 * u + 2.0 ** -13) * v_max + 2e-7
         assert bool(((out[lo:lo + n_q].double() - ref).abs() <= lim).all())
 
 
-def test_prompt_is_the_16_bit_operator_over_expanded_pages(cuda_device):
+def test_operators_over_expanded_pages(cuda_device):
+    """The 16-bit operators over expanded pages: keys rounded to 16 bits move a
+    score by e <= u |q||k| / sqrt(d), and an output by expm1(2 e) max|v| at
+    most; queries of the decode step as above."""
     gen = torch.Generator(device=cuda_device).manual_seed(12)
-    cache, table, slots = make_cache(gen, [300, 77], 2, 128, 32, 16, torch.int8, torch.float16, cuda_device)
-    starts, lens = ints([0, 200, 250], cuda_device), ints([300, 77], cuda_device)
+    kl = [300, 77]
+    cache, table, slots = make_cache(gen, kl, 2, 128, 32, 16, torch.int8, torch.float16, cuda_device)
+    starts, lens = ints([0, 200, 250], cuda_device), ints(kl, cuda_device)
     q = torch.randn((250, 8, 128), generator=gen, device=cuda_device).half()
     k, v, t = qc.expanded_pages(cache, table, slots, lens, 13)
+    u, v_max = 2.0 ** -11, largest_value(cache, table, slots, kl)
+    e = u * float(q.float().norm(dim=-1).max()) * float(k.float().norm(dim=-1).max()) / math.sqrt(128)
     want = paged_ops.prompt_attention(q, k, v, t, starts, lens)
-    assert torch.equal(qc.quantized_prompt_attention(q, cache, table, slots, starts, lens, 13), want)
+    out = qc.quantized_prompt_attention(q, cache, table, slots, starts, lens, 13)
+    assert float((out.float() - want.float()).abs().max()) <= (6 * u + 2.0 ** -12 + math.expm1(2 * e)) * v_max
     one = q[:2].contiguous()
-    # The decode step takes codes as they are, the 16-bit one rounded values: see test_prompt.
+    e += query_rounding(one, cache, table, slots, kl)
     a, b = qc.quantized_attention(one, cache, table, slots, lens), paged_ops.paged_attention(one, k, v, t, lens)
-    e = 2.0 ** -11 * float(one.float().norm(dim=-1).max()) * float(k.float().norm(dim=-1).max()) / math.sqrt(128)
-    assert float((a.float() - b.float()).abs().max()) <= (4 * 2.0 ** -11 + 2.0 ** -12 + math.expm1(2 * e)) * float(
-        v.float().abs().max())
+    assert float((a.float() - b.float()).abs().max()) <= (6 * u + 2.0 ** -12 + math.expm1(2 * e)) * v_max
+
+
+def test_prompts_without_room_or_positions(cuda_device):
+    """Pages that there is no room for are reported, and the other sequences are
+    as they were; sequences without positions give zeros."""
+    gen = torch.Generator(device=cuda_device).manual_seed(13)
+    kl = [40, 3000, 0]
+    cache, table, slots = make_cache(gen, kl, 2, 64, 16, 16, torch.int8, torch.float16, cuda_device)
+    starts, lens = ints([0, 30, 60, 64], cuda_device), ints(kl, cuda_device)
+    q = torch.randn((64, 4, 64), generator=gen, device=cuda_device).half()
+    full = qc.quantized_prompt_attention(q, cache, table, slots, starts, lens, 191)
+    assert _native.device_status(cuda_device.index, reset=True) == 0
+    assert bool((full[60:] == 0).all())
+    for n_pages in (3, 20):
+        ws = qc.quantized_prompt_workspace(cache, 3, table.shape[1], n_pages).fill_(255)
+        out = qc.quantized_prompt_attention(q, cache, table, slots, starts, lens, n_pages, workspace=ws)
+        assert _native.device_status(cuda_device.index, reset=True) == 2
+        assert torch.equal(out[:30], full[:30]) and bool((out[60:] == 0).all())
+    none = qc.quantized_prompt_attention(q, cache, table, slots, starts, ints([0, 0, 0], cuda_device), 0)
+    assert bool((none == 0).all())
+    assert _native.device_status(cuda_device.index, reset=True) == 0

@@ -72,6 +72,15 @@ def decode(kv=None, **kw):
     return _native.lib().dqg_quantized_attention(*a.values(), cache() if kv is None else kv, *b.values(), None)
 
 
+def prompt(kv=None, **kw):
+    a = dict(q=16, qs=512, qh=128, T=5, hq=4)
+    b = dict(table=16, width=3, tstride=3, open=16, starts=16, lens=16, seqs=2, pages=6, causal=1, scale=0.1, out=16, ws=256,
+             bytes=1 << 40)
+    for k, v in kw.items():
+        (a if k in a else b)[k] = v
+    return _native.lib().dqg_quantized_prompt_attention(*a.values(), cache() if kv is None else kv, *b.values(), None)
+
+
 def sample(params=None, **kw):
     a = dict(logits=16, dtype=0, rows=2, vocab=100, stride=100, uniform=16)
     b = dict(tokens=16, logprobs=16)
@@ -81,7 +90,7 @@ def sample(params=None, **kw):
     return _native.lib().dqg_sample_tokens(*a.values(), p, *b.values(), None)
 
 
-@pytest.mark.parametrize("call", [append, expand, decode], ids=lambda f: f.__name__)
+@pytest.mark.parametrize("call", [append, expand, decode, prompt], ids=lambda f: f.__name__)
 @pytest.mark.parametrize("kw,code,msg", CACHES, ids=lambda v: str(v))
 def test_caches(call, kw, code, msg):
     rejected(call(cache(**kw)), code, msg)
@@ -97,7 +106,7 @@ SEQS = [
 ]
 
 
-@pytest.mark.parametrize("call", [append, expand, decode], ids=lambda f: f.__name__)
+@pytest.mark.parametrize("call", [append, expand, decode, prompt], ids=lambda f: f.__name__)
 @pytest.mark.parametrize("kw,msg", SEQS, ids=lambda v: str(v))
 def test_sequences(call, kw, msg):
     rejected(call(**kw), 1, msg)
@@ -132,8 +141,15 @@ def test_append(kw, msg):
     (dict(scale=float("nan")), "scale must be positive"),
     (dict(out=8), "out must be 16-byte aligned"),
 ], ids=lambda v: str(v))
-def test_decode(kw, msg):
+def test_attention(kw, msg):
     rejected(decode(**kw), 1, msg)
+    rejected(prompt(**kw), 1, msg)
+
+
+def test_prompt():
+    rejected(prompt(T=-1), 1, "T=-1 out of range")
+    rejected(prompt(pages=-1), 1, "n_pages=-1 out of range")
+    rejected(prompt(starts=None), 1, "q_starts must not be null")
 
 
 @pytest.mark.parametrize("kw,code,msg", [
@@ -167,7 +183,7 @@ def test_sample(kw, params, code, msg):
 
 
 def test_empty_calls_launch_nothing():
-    assert append(T=0) == 0 and expand(seqs=0) == 0 and decode(seqs=0) == 0 and sample(rows=0) == 0
+    assert append(T=0) == 0 and expand(seqs=0) == 0 and decode(seqs=0) == 0 and prompt(T=0) == 0 and sample(rows=0) == 0
     rejected(_native.lib().dqg_sample_tokens(16, 0, 1, 1, 1, 16, None, 16, 16, None), 1, "params must not be null")
 
 
@@ -176,6 +192,9 @@ def test_workspace_queries():
     rejected(lib.dqg_quantized_attention_workspace(2, 4, 2, 96, ctypes.byref(n)), 2, "head_dim 64 and 128")
     rejected(lib.dqg_quantized_attention_workspace(2, 4, 3, 128, ctypes.byref(n)), 1, "query heads per KV head")
     rejected(lib.dqg_quantized_attention_workspace(2, 4, 2, 128, None), 1, "bytes must not be null")
+    rejected(lib.dqg_quantized_prompt_workspace(cache(block=8), 2, 3, 6, ctypes.byref(n)), 2, "block must be 16")
+    rejected(lib.dqg_quantized_prompt_workspace(cache(), 2, 0, 6, ctypes.byref(n)), 1, "table_width=0")
+    rejected(lib.dqg_quantized_prompt_workspace(cache(), 2, 3, -1, ctypes.byref(n)), 1, "n_pages=-1")
 
 
 def test_struct_layouts():
