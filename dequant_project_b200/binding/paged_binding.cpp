@@ -302,6 +302,14 @@ at::Tensor prefix(PyObject* const* a, Py_ssize_t n) {
   return out;
 }
 
+PyObject* tuple(std::initializer_list<at::Tensor> tensors) {
+  PyObject* t = PyTuple_New(static_cast<Py_ssize_t>(tensors.size()));
+  if (t == nullptr) throw python_error();
+  Py_ssize_t i = 0;
+  for (const at::Tensor& x : tensors) PyTuple_SET_ITEM(t, i++, THPVariable_Wrap(x));
+  return t;
+}
+
 // A cache held in 8 bits: k, v, k_scale, v_scale, k_open, v_open.
 struct Quantized {
   dqg_quantized_kv kv;
@@ -385,32 +393,28 @@ at::Tensor quantized_append(PyObject* const* a, Py_ssize_t n) {
   return q;
 }
 
-// (cache: 6, block_table, open_slots, kv_lens, k_out, v_out, table_out)
-at::Tensor expand(PyObject* const* a, Py_ssize_t n) {
-  arguments(n, 12);
+// (cache: 6, block_table, open_slots, kv_lens, n_pages) -> (k_pages, v_pages,
+// table)
+PyObject* expand(PyObject* const* a, Py_ssize_t n) {
+  arguments(n, 10);
   const Quantized c = quantized(a);
   const at::Tensor &table = tensor(a[6], "block_table"), &open = tensor(a[7], "open_slots");
-  const at::Tensor &lens = tensor(a[8], "kv_lens"), &k = tensor(a[9], "k_out"), &v = tensor(a[10], "v_out");
-  const at::Tensor& out = tensor(a[11], "table_out");
-  forward_only_cache(k, c);
+  const at::Tensor& lens = tensor(a[8], "kv_lens");
+  const int64_t pages = integer(a[9]);
+  forward_only_cache(*c.t[0], c);
   ints(c, lens, "kv_lens", at::kInt, 1, -1);
   const int64_t b = lens.size(0);
   ints(c, table, "block_table", at::kInt, 2, b);
   ints(c, open, "open_slots", at::kInt, 1, b);
-  ints(c, out, "table_out", at::kInt, 2, b);
-  for (const at::Tensor* x : {&k, &v}) {
-    same(c, *x, "an expanded pool");
-    if (x->dim() != 4 || x->size(1) != c.kv.n_kv_heads || x->size(2) != c.kv.page_size ||
-        x->size(3) != c.kv.head_dim || x->sizes() != k.sizes() || !x->is_contiguous())
-      reject("expanded pools must be contiguous [pages, kv heads, page size, head dim]");
-  }
-  if (out.size(1) != table.size(1) || !out.is_contiguous()) reject("table_out must be contiguous and as block_table");
+  if (pages < 0) reject("n_pages=%lld out of range", static_cast<long long>(pages));
   c10::cuda::CUDAGuard guard(static_cast<c10::DeviceIndex>(c.device));
+  const at::TensorOptions options = c.t[4]->options();
+  at::Tensor k = at::empty({pages, c.kv.n_kv_heads, c.kv.page_size, c.kv.head_dim}, options), v = at::empty_like(k);
+  at::Tensor out = at::empty({b, table.size(1)}, table.options());
   check(p_expand(&c.kv, table.data_ptr<int32_t>(), table.size(1), row_stride(table), open.data_ptr<int32_t>(),
-                 lens.data_ptr<int32_t>(), b, k.size(0), k.data_ptr(), v.data_ptr(), out.data_ptr<int32_t>(),
+                 lens.data_ptr<int32_t>(), b, pages, k.data_ptr(), v.data_ptr(), out.data_ptr<int32_t>(),
                  stream_of(c.device)));
-  changed({&k, &v, &out});
-  return out;
+  return tuple({k, v, out});
 }
 
 // (q, cache: 6, block_table, open_slots, kv_lens, scale, workspace)
@@ -525,11 +529,7 @@ PyObject* sample(PyObject* const* a, Py_ssize_t n) {
   check(p_sample(logits.data_ptr(), type == at::kHalf ? DQG_FP16 : (type == at::kFloat ? DQG_FP32 : DQG_BF16), rows,
                  vocab, rows > 1 ? logits.stride(0) : vocab, uniform.data_ptr<float>(), &s, tokens.data_ptr<int64_t>(),
                  logprobs.data_ptr<float>(), stream_of(logits.get_device())));
-  PyObject* pair = PyTuple_New(2);
-  if (pair == nullptr) throw python_error();
-  PyTuple_SET_ITEM(pair, 0, THPVariable_Wrap(tokens));
-  PyTuple_SET_ITEM(pair, 1, THPVariable_Wrap(logprobs));
-  return pair;
+  return tuple({tokens, logprobs});
 }
 
 PyObject* wrapped(at::Tensor t) { return THPVariable_Wrap(t); }

@@ -16,10 +16,12 @@ struct Int8 {
     const uint32_t cd = prmt(__float2int_rn(c), __float2int_rn(d), 0x0040);
     return prmt(ab, cd, 0x5410);
   }
-  // Four codes to four values.
+  // Four codes to four values: bytes plus 128 in the last bits of 2^23. (The
+  // conversion instruction runs at an eighth of this rate.)
   static __device__ __forceinline__ void unpack4(uint32_t w, float* f) {
+    w ^= 0x80808080u;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) f[i] = static_cast<float>(static_cast<int8_t>(w >> (8 * i)));
+    for (int i = 0; i < 4; ++i) f[i] = __uint_as_float(prmt(w, 0x4b000000u, 0x7440 + i)) - 8388736.f;
   }
 };
 struct E4m3 {

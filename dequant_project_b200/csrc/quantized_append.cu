@@ -25,7 +25,7 @@ namespace dqg {
 namespace {
 
 constexpr int kThreads = 128;
-constexpr int kMaxBlock = 64;
+constexpr int kIter = 4;  // heads a lane group takes one after the other, at most
 
 template <typename E>
 struct Params {
@@ -39,7 +39,7 @@ struct Params {
   QuantizedPool pool;
   QuantizedSeqs seqs;
   int64_t qkv_stride, n_positions, q_blocks;
-  int T, hq, hkv, rot, page_shift, block_shift, chunks;
+  int T, hq, hkv, rot, page_shift, block_shift, chunks, iter;
   float eps;
 };
 
@@ -81,29 +81,39 @@ __device__ __forceinline__ int64_t clamped_position(int64_t pos, int64_t n, bool
 template <typename E, int D, int LAYOUT>
 __device__ __forceinline__ void store_queries(const Params<E>& p) {
   using Lane = RopeLane<E, D, LAYOUT>;
-  constexpr int kGroups = 32 / Lane::kLanes;  // heads a warp holds
+  constexpr int kGroups = 32 / Lane::kLanes;  // heads a warp holds at a time
   const int64_t w = static_cast<int64_t>(blockIdx.x) * (kThreads / 32) + (threadIdx.x >> 5);
   const int64_t token = w / p.chunks;
-  const int lane = threadIdx.x & 31, h = static_cast<int>(w - token * p.chunks) * kGroups + lane / Lane::kLanes;
+  const int lane = threadIdx.x & 31, grp = lane / Lane::kLanes;
+  const int h0 = static_cast<int>(w - token * p.chunks) * p.iter * kGroups + grp;
   if (token >= p.T) return;
   Lane part(lane % Lane::kLanes, p.rot);
-  const E* head = p.qkv + token * p.qkv_stride + static_cast<int64_t>(h) * D;
-  uint4 xa = make_uint4(0, 0, 0, 0), xb = xa;
-  if (h < p.hq) {
-    xa = __ldcs(reinterpret_cast<const uint4*>(head + part.ea));
-    xb = __ldcs(reinterpret_cast<const uint4*>(head + part.eb));
+  const E* row = p.qkv + token * p.qkv_stride;
+  uint4 xa[kIter], xb[kIter];
+#pragma unroll
+  for (int it = 0; it < kIter; ++it) {
+    const int h = h0 + it * kGroups;
+    if (it < p.iter && h < p.hq) {
+      xa[it] = __ldcs(reinterpret_cast<const uint4*>(row + static_cast<int64_t>(h) * D + part.ea));
+      xb[it] = __ldcs(reinterpret_cast<const uint4*>(row + static_cast<int64_t>(h) * D + part.eb));
+    }
   }
   const int64_t pos = clamped_position(__ldg(p.positions + token), p.n_positions, lane == 0);
   part.entries(p.cosv + pos * part.half, p.sinv + pos * part.half);
-  float a[8], b[8];
-  unpack8<E>(xa, a);
-  unpack8<E>(xb, b);
-  const float r = part.norm(a, b, p.q_norm, p.eps);
-  if (h >= p.hq) return;
-  part.rotate(a, b, head, p.q_norm, r);
-  E* dst = p.q_out + (token * p.hq + h) * D;
-  __stcs(reinterpret_cast<uint4*>(dst + part.ea), pack8<E>(a));
-  __stcs(reinterpret_cast<uint4*>(dst + part.eb), pack8<E>(b));
+#pragma unroll
+  for (int it = 0; it < kIter; ++it) {
+    const int h = h0 + it * kGroups;
+    if (it >= p.iter || h - grp >= p.hq) break;  // (by whole warps)
+    float a[8], b[8];
+    unpack8<E>(h < p.hq ? xa[it] : make_uint4(0, 0, 0, 0), a);
+    unpack8<E>(h < p.hq ? xb[it] : make_uint4(0, 0, 0, 0), b);
+    const float r = part.norm(a, b, p.q_norm, p.eps);
+    if (h >= p.hq) continue;
+    part.rotate(a, b, row + static_cast<int64_t>(h) * D, p.q_norm, r);
+    E* dst = p.q_out + (token * p.hq + h) * D;
+    __stcs(reinterpret_cast<uint4*>(dst + part.ea), pack8<E>(a));
+    __stcs(reinterpret_cast<uint4*>(dst + part.eb), pack8<E>(b));
+  }
 }
 
 // Largest magnitude among 16-bit values, as bits (an infinity or NaN is larger
@@ -115,11 +125,11 @@ __device__ __forceinline__ uint32_t magnitude(uint4 v, uint32_t m) {
   return __vmaxu2(m, v.w & 0x7fff7fffu);
 }
 
-template <typename E, int D, int LAYOUT, class Code>
+// kPasses: a block's rows over those that the threads hold at a time.
+template <typename E, int D, int LAYOUT, int kPasses>
 __device__ __forceinline__ void store_block(const Params<E>& p, int b, const Seq& s, int j, int kvh, uint32_t* scratch) {
   using Lane = RopeLane<E, D, LAYOUT>;
   constexpr int kRows = kThreads / Lane::kLanes;       // rows at a time
-  constexpr int kPasses = (kMaxBlock + kRows - 1) / kRows;
   const int row0 = threadIdx.x / Lane::kLanes;
   const int base = j << p.block_shift, block = 1 << p.block_shift, start = s.end - s.n;
   const bool whole = base + block <= s.end;
@@ -138,7 +148,6 @@ __device__ __forceinline__ void store_block(const Params<E>& p, int b, const Seq
 #pragma unroll
     for (int i = 0; i < kPasses; ++i) {
       xa[i] = xb[i] = make_uint4(0, 0, 0, 0);
-      if (i * kRows >= block) continue;
       const int row = row0 + i * kRows, t = base + row;
       const bool fresh = row < block && t >= start && t < s.end;
       const int64_t token = s.q0 + (fresh ? t - start : 0);
@@ -181,7 +190,8 @@ __device__ __forceinline__ void store_block(const Params<E>& p, int b, const Seq
     __syncthreads();
     const float2 two = Elem<E>::unpack(most);
     const bool finite = Elem<E>::non_finite(most) == 0u;
-    const float scale = finite ? fmaxf(fmaxf(two.x, two.y) / Code::kMost, 1.17549435e-38f) : NAN;
+    const bool e4m3 = p.pool.e4m3;
+    const float scale = finite ? fmaxf(fmaxf(two.x, two.y) / (e4m3 ? E4m3::kMost : Int8::kMost), 1.17549435e-38f) : NAN;
     const float inv = 1.f / scale;
     if (page < 0) continue;
     if (threadIdx.x == 0) {
@@ -201,9 +211,12 @@ __device__ __forceinline__ void store_block(const Params<E>& p, int b, const Seq
       for (int run = 0; run < 2; ++run) {
         unpack8<E>(run ? xb[i] : xa[i], x);
         uint2 w = make_uint2(0, 0);
-        if (finite) {
-          w.x = Code::pack4(x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
-          w.y = Code::pack4(x[4] * inv, x[5] * inv, x[6] * inv, x[7] * inv);
+        if (finite && e4m3) {
+          w.x = E4m3::pack4(x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
+          w.y = E4m3::pack4(x[4] * inv, x[5] * inv, x[6] * inv, x[7] * inv);
+        } else if (finite) {
+          w.x = Int8::pack4(x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
+          w.y = Int8::pack4(x[4] * inv, x[5] * inv, x[6] * inv, x[7] * inv);
         }
         __stcs(reinterpret_cast<uint2*>(codes + row * p.pool.row_stride + (run ? part.eb : part.ea)), w);
       }
@@ -211,8 +224,8 @@ __device__ __forceinline__ void store_block(const Params<E>& p, int b, const Seq
   }
 }
 
-template <typename E, int D, int LAYOUT, class Code>
-__global__ void __launch_bounds__(kThreads)
+template <typename E, int D, int LAYOUT, int kPasses>
+__global__ void __launch_bounds__(kThreads, kPasses == 4 || LAYOUT == kUneven ? 4 : 5)
     quantized_append_kernel(const __grid_constant__ Params<E> p) {
   __shared__ uint32_t scratch[kThreads / 32 + 2];
   pdl_wait_prior_grid();
@@ -231,15 +244,15 @@ __global__ void __launch_bounds__(kThreads)
   const Seq s = load_seq(p, b, false);
   const int first = (s.end - s.n) >> p.block_shift, last = (s.end - 1) >> p.block_shift;
   __syncthreads();
-  store_block<E, D, LAYOUT, Code>(p, b, s, first + static_cast<int>(in), kvh, scratch);
+  store_block<E, D, LAYOUT, kPasses>(p, b, s, first + static_cast<int>(in), kvh, scratch);
   if (in == 0 && last > first && (s.end & ((1 << p.block_shift) - 1))) {
     __syncthreads();  // the open rows have been read
-    store_block<E, D, LAYOUT, Code>(p, b, s, last, kvh, scratch);
+    store_block<E, D, LAYOUT, kPasses>(p, b, s, last, kvh, scratch);
   }
 }
 
-template <typename E, int D, class Code>
-cudaError_t launch(const QuantizedPool& pool, const QuantizedSeqs& seqs, const QuantizedAppendArgs& a,
+template <typename E, int D, int kPasses>
+cudaError_t launch(const QuantizedPool& pool, const QuantizedSeqs& seqs, const QuantizedAppendArgs& a, int num_sms,
                    cudaStream_t stream) {
   Params<E> p;
   p.qkv = static_cast<const E*>(a.qkv);
@@ -261,8 +274,11 @@ cudaError_t launch(const QuantizedPool& pool, const QuantizedSeqs& seqs, const Q
   p.page_shift = p.block_shift = 0;
   while ((1 << p.page_shift) < pool.page_size) ++p.page_shift;
   while ((1 << p.block_shift) < pool.block) ++p.block_shift;
-  constexpr int kPer = 32 / (D / 16);
-  p.chunks = (a.hq + kPer - 1) / kPer;
+  // kIter heads a lane group once that still fills the GPU's warps; below it
+  // one, so that a few tokens spread over the SMs.
+  constexpr int kGroups = 32 / (D / 16);
+  p.iter = static_cast<int64_t>(a.T) * a.hq / kGroups >= kIter * 64 * static_cast<int64_t>(num_sms) ? kIter : 1;
+  p.chunks = (a.hq + kGroups * p.iter - 1) / (kGroups * p.iter);
   p.q_blocks = (static_cast<int64_t>(a.T) * p.chunks + kThreads / 32 - 1) / (kThreads / 32);
   // n new rows make (n - 1) / block + 1 units at most; and one more than all.
   const int64_t units = a.T / pool.block + (a.T < seqs.B ? a.T : seqs.B) + 1;
@@ -277,27 +293,30 @@ cudaError_t launch(const QuantizedPool& pool, const QuantizedSeqs& seqs, const Q
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  if (a.interleaved) return cudaLaunchKernelEx(&cfg, quantized_append_kernel<E, D, kInterleaved, Code>, p);
-  if (a.rot % 16 == 0) return cudaLaunchKernelEx(&cfg, quantized_append_kernel<E, D, kHalf, Code>, p);
-  return cudaLaunchKernelEx(&cfg, quantized_append_kernel<E, D, kUneven, Code>, p);
+  if (a.interleaved) return cudaLaunchKernelEx(&cfg, quantized_append_kernel<E, D, kInterleaved, kPasses>, p);
+  if (a.rot % 16 == 0) return cudaLaunchKernelEx(&cfg, quantized_append_kernel<E, D, kHalf, kPasses>, p);
+  return cudaLaunchKernelEx(&cfg, quantized_append_kernel<E, D, kUneven, kPasses>, p);
 }
 
 template <typename E, int D>
-cudaError_t launch_code(const QuantizedPool& pool, const QuantizedSeqs& seqs, const QuantizedAppendArgs& a,
-                        cudaStream_t stream) {
-  return pool.e4m3 ? launch<E, D, E4m3>(pool, seqs, a, stream) : launch<E, D, Int8>(pool, seqs, a, stream);
+cudaError_t launch_passes(const QuantizedPool& pool, const QuantizedSeqs& seqs, const QuantizedAppendArgs& a, int num_sms,
+                          cudaStream_t stream) {
+  const int rows = kThreads / (D / 16);  // that the threads hold at a time
+  if (pool.block <= rows) return launch<E, D, 1>(pool, seqs, a, num_sms, stream);
+  if (pool.block <= 2 * rows) return launch<E, D, 2>(pool, seqs, a, num_sms, stream);
+  if constexpr (D == 128) return launch<E, D, 4>(pool, seqs, a, num_sms, stream);
+  return cudaErrorInvalidValue;
 }
 
 }  // namespace
 
 cudaError_t launch_quantized_append(const QuantizedPool& pool, const QuantizedSeqs& seqs, const QuantizedAppendArgs& a,
                                     int num_sms, cudaStream_t stream) {
-  (void)num_sms;
   if (pool.bf16)
-    return pool.D == 128 ? launch_code<__nv_bfloat16, 128>(pool, seqs, a, stream)
-                         : launch_code<__nv_bfloat16, 64>(pool, seqs, a, stream);
-  return pool.D == 128 ? launch_code<__half, 128>(pool, seqs, a, stream)
-                       : launch_code<__half, 64>(pool, seqs, a, stream);
+    return pool.D == 128 ? launch_passes<__nv_bfloat16, 128>(pool, seqs, a, num_sms, stream)
+                         : launch_passes<__nv_bfloat16, 64>(pool, seqs, a, num_sms, stream);
+  return pool.D == 128 ? launch_passes<__half, 128>(pool, seqs, a, num_sms, stream)
+                       : launch_passes<__half, 64>(pool, seqs, a, num_sms, stream);
 }
 
 }  // namespace dqg

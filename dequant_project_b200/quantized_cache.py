@@ -184,15 +184,12 @@ def expanded_pages(cache: QuantizedCache, block_table: torch.Tensor, open_slots:
     zeros. ``n_pages`` is the number that the sequences take (sum of
     ceil(len / page size)) or more; what has no room is left out and reported,
     pages that nothing takes are undefined."""
-    shape = (n_pages, cache.k.shape[1], cache.page_size, cache.k.shape[3])
-    k, v = (torch.empty(shape, dtype=cache.k_open.dtype, device=cache.k.device) for _ in range(2))
-    table = torch.empty((block_table.shape[0], block_table.shape[1]), dtype=torch.int32, device=cache.k.device)
     if cache.k.is_cuda:
-        paged._binding().expand_pages(*cache, block_table, open_slots, kv_lens, k, v, table)
-        return k, v, table
+        return paged._binding().expand_pages(*cache, block_table, open_slots, kv_lens, n_pages)
     paged._forward_only(*cache)
     at, page = 0, cache.page_size
-    table.fill_(-1)
+    k, v = (torch.empty((n_pages, cache.k.shape[1], page, cache.k.shape[3]), dtype=cache.k_open.dtype) for _ in range(2))
+    table = torch.full_like(block_table, -1)
     for b, n in enumerate(kv_lens.tolist()):
         taken = -(-n // page)
         table[b, :taken] = torch.arange(at, at + taken)
