@@ -239,14 +239,13 @@ __global__ void __launch_bounds__(kThreads, Layout<D, NB>::kCtasPerSm)
       // A lane a slice of 16 positions, of keys and then of values: its box and
       // its block's scale. Pages are read from the table one tile ahead: their
       // latency would be a tile's time.
-      constexpr int kNone = -0x7fffffff - 1;
       const int slice = lane % kWarps, n_pages = static_cast<int>(p.n_pages);
       const bool values = lane >= kWarps;
       auto page_of = [&](int x) {
         const int t = x * kTile + slice * 16;
-        return lane < 2 * kWarps && t < done ? __ldg(i.table + (t >> p.page_shift)) : kNone;
+        return lane < 2 * kWarps && t < done ? __ldg(i.table + (t >> p.page_shift)) : 0;
       };
-      int page = page_of(i.x0), next = kNone;
+      int page = page_of(i.x0), next = 0;
       for (int x = i.x0; x < i.x1; ++x, ++it, page = next) {
         const int st = it % kStages;
         uint8_t* dst = smem + st * 2 * L::kTileBytes;
@@ -256,9 +255,9 @@ __global__ void __launch_bounds__(kThreads, Layout<D, NB>::kCtasPerSm)
             ok = false;
             break;
           }
-          // No such page: zeros.
-          const bool good = page >= 0 && page < n_pages;
-          if (!good && page != kNone) atomicOr(&g_status, kStatusBadIndex);
+          // No position, or no such page: zeros.
+          const bool some = x * kTile + slice * 16 < done, good = some && page >= 0 && page < n_pages;
+          if (some && !good) atomicOr(&g_status, kStatusBadIndex);
           if (lane == 0) mbar_arrive_expect_tx(full + st, 2 * L::kTileBytes);
           __syncwarp();
           if (lane < 2 * kWarps) {

@@ -8,7 +8,9 @@ prompts of any lengths through every layer at once (``rope_paged_append``, then
 ``prompt_attention``), ``step`` decodes one token of every sequence
 (``paged_attention``, or ``shared_prefix_attention`` where the sequences begin
 with the prefix that ``set_prefix`` has cached once), ``free`` returns a
-sequence's pages. Linear layers go through the fused GEMV up to eight rows and
+sequence's pages, ``sample`` draws the next tokens (``sample_tokens``). With
+``codes`` the cache is held in 8 bits (``quantized_cache``: half the bytes a
+decode step reads, twice the positions in the same memory). Linear layers go through the fused GEMV up to eight rows and
 through dequantize and a matrix product above, as ``QuantLinear`` does.
 
 The reference models the decode step's bytes
@@ -26,18 +28,22 @@ import torch
 
 from dequant_project_b200 import decode_ops as ops
 from dequant_project_b200 import paged_ops as paged
+from dequant_project_b200 import quantized_cache as quantized
 from dequant_project_b200.decoder import TPDecoder
+from dequant_project_b200.sampling import sample_tokens
 
 
 class PageAllocator:
-    """Page numbers of a pool, handed out and taken back on the host."""
+    """Page numbers of a pool (or other things' numbers), handed out and taken
+    back on the host."""
 
-    def __init__(self, n_pages: int):
+    def __init__(self, n_pages: int, what: str = "pages"):
         self.free = list(range(n_pages - 1, -1, -1))
+        self.what = what
 
     def take(self, n: int) -> list[int]:
         if n > len(self.free):
-            raise RuntimeError(f"{n} pages needed, {len(self.free)} free")
+            raise RuntimeError(f"{n} {self.what} needed, {len(self.free)} free")
         got = self.free[len(self.free) - n:][::-1]
         del self.free[len(self.free) - n:]
         return got
@@ -49,19 +55,31 @@ class PageAllocator:
 class PagedDecoder:
     """A decoder's weights over a paged cache of ``n_pages`` pages a layer
     (this rank's heads), ``page_size`` positions each, for sequences of up to
-    ``max_positions`` positions. At world > 1 every rank makes the same calls."""
+    ``max_positions`` positions. ``codes`` (int8 or float8_e4m3fn; default: 16
+    bits) holds the cache in 8 bits, with a scale for every ``block`` positions
+    of a head and open blocks for ``max_seqs`` sequences. At world > 1 every
+    rank makes the same calls."""
 
     def __init__(self, dec: TPDecoder, n_pages: int, page_size: int = 16, max_positions: int = 4096,
-                 rope_scaling: dict | None = None):
+                 rope_scaling: dict | None = None, *, codes: torch.dtype | None = None, block: int = 16,
+                 max_seqs: int = 64):
         cfg = dec.cfg
         self.dec, self.page, self.max_positions = dec, page_size, max_positions
-        shape = (n_pages, dec.hkv, page_size, cfg.head_dim)
-        self.k = [torch.zeros(shape, dtype=torch.float16, device=dec.device) for _ in range(cfg.n_layers)]
-        self.v = [torch.zeros(shape, dtype=torch.float16, device=dec.device) for _ in range(cfg.n_layers)]
+        self.codes = codes
+        if codes is None:
+            shape = (n_pages, dec.hkv, page_size, cfg.head_dim)
+            self.k = [torch.zeros(shape, dtype=torch.float16, device=dec.device) for _ in range(cfg.n_layers)]
+            self.v = [torch.zeros(shape, dtype=torch.float16, device=dec.device) for _ in range(cfg.n_layers)]
+        else:
+            # (One open block more than sequences: a prefix passes through it.)
+            self.cache = [quantized.QuantizedCache.empty(n_pages, dec.hkv, page_size, cfg.head_dim, max_seqs + 1,
+                                                         block=block, codes=codes, device=dec.device)
+                          for _ in range(cfg.n_layers)]
+            self.open = PageAllocator(max_seqs, "open blocks")
         self.cos, self.sin = paged.rope_scaled_tables(cfg.head_dim, cfg.rope_theta, max_positions, dec.device,
                                                       scaling=rope_scaling)
         self.pages = PageAllocator(n_pages)
-        self.seqs: dict[int, dict] = {}  # id -> own pages, own length
+        self.seqs: dict[int, dict] = {}  # id -> own pages, own length (and open block)
         self.prefix_pages: list[int] = []
         self.prefix_len = 0
         self._next = 0
@@ -88,17 +106,16 @@ class PagedDecoder:
         both = self._linear(x, gu).view(x.shape[0], -1, 2, 8)
         return ops.silu_mul(both.transpose(1, 2).reshape(x.shape[0], -1))
 
-    def _forward(self, tokens, positions, slots, attend, last) -> torch.Tensor:
-        """All layers over packed tokens, whose keys and values go to
-        ``slots``; ``attend(layer, q)`` is the attention. Logits of rows ``last``."""
+    def _forward(self, tokens, store, attend, last) -> torch.Tensor:
+        """All layers over packed tokens: ``store(layer, qkv)`` rotates, puts
+        keys and values into the cache and gives the queries, ``attend(layer,
+        q)`` is the attention. Logits of rows ``last``."""
         dec, cfg = self.dec, self.dec.cfg
         h = dec.embed[tokens]
         pending = None
         for layer, w in enumerate(dec.layers):
             x = ops.add_rms_norm(h, pending, dec.attn_norm[layer], cfg.eps)
-            q = paged.rope_paged_append(self._linear(x, w["qkv"]), self.cos, self.sin, positions, slots,
-                                        self.k[layer], self.v[layer], dec.hq)
-            a = attend(layer, q).reshape(tokens.shape[0], -1)
+            a = attend(layer, store(layer, self._linear(x, w["qkv"]))).reshape(tokens.shape[0], -1)
             x = ops.add_rms_norm(h, self._reduce(self._linear(a, w["o"])), dec.mlp_norm[layer], cfg.eps)
             pending = self._reduce(self._linear(self._mlp(x, w["gu"]), w["down"]))
         x = ops.add_rms_norm(h, pending, dec.final_norm, cfg.eps)[last].contiguous()
@@ -124,24 +141,54 @@ class PagedDecoder:
     def _slots(self, pages: list[int], start: int, n: int) -> list[int]:
         return [pages[t // self.page] * self.page + t % self.page for t in range(start, start + n)]
 
-    def _prompts(self, prompts, tables, starts) -> torch.Tensor:
+    def _store(self, positions, slots):
+        """What puts tokens into 16-bit pages, at ``slots``."""
+        def store(layer, qkv):
+            return paged.rope_paged_append(qkv, self.cos, self.sin, positions, slots, self.k[layer], self.v[layer],
+                                           self.dec.hq)
+        return store
+
+    def _store_quantized(self, positions, table, open_slots, q_starts, kv_lens):
+        """What puts tokens into 8-bit pages, as the newest of the sequences."""
+        def store(layer, qkv):
+            return quantized.rope_quantized_append(qkv, self.cos, self.sin, positions, self.cache[layer], table,
+                                                   open_slots, q_starts, kv_lens, self.dec.hq)
+        return store
+
+    def _prompts(self, prompts, tables, starts, opens) -> torch.Tensor:
         """Packed prompts whose rows continue cached sequences: ``tables`` their
-        pages, ``starts`` the positions already cached."""
+        pages, ``starts`` the positions already cached, ``opens`` their open
+        blocks."""
         lens = [int(p.shape[0]) for p in prompts]
         ends = [s + n for s, n in zip(starts, lens)]
         bounds = [0]
         for n in lens:
             bounds.append(bounds[-1] + n)
         positions = self._ints([t for s, e in zip(starts, ends) for t in range(s, e)], torch.int64)
-        slots = self._ints([t for pages, s, n in zip(tables, starts, lens) for t in self._slots(pages, s, n)],
-                           torch.int64)
         table, q_starts, kv_lens = self._table(tables), self._ints(bounds), self._ints(ends)
+        if self.codes is None:
+            store = self._store(positions, self._ints([t for pages, s, n in zip(tables, starts, lens)
+                                                       for t in self._slots(pages, s, n)], torch.int64))
 
-        def attend(layer, q):
-            return paged.prompt_attention(q, self.k[layer], self.v[layer], table, q_starts, kv_lens)
+            def attend(layer, q):
+                return paged.prompt_attention(q, self.k[layer], self.v[layer], table, q_starts, kv_lens)
+        else:
+            open_slots, n_pages = self._ints(opens), sum(-(-n // self.page) for n in ends)
+            store = self._store_quantized(positions, table, open_slots, q_starts, kv_lens)
+
+            def attend(layer, q):
+                return quantized.quantized_prompt_attention(q, self.cache[layer], table, open_slots, q_starts, kv_lens,
+                                                            n_pages)
 
         tokens = torch.cat([p.to(self.dec.device) for p in prompts])
-        return self._forward(tokens, positions, slots, attend, self._ints([b - 1 for b in bounds[1:]], torch.int64))
+        return self._forward(tokens, store, attend, self._ints([b - 1 for b in bounds[1:]], torch.int64))
+
+    def _take_open(self, n: int) -> list[int]:
+        return [0] * n if self.codes is None else self.open.take(n)
+
+    def _give_open(self, opens: list[int]) -> None:
+        if self.codes is not None:
+            self.open.give(opens)
 
     def _check_tokens(self, tokens: torch.Tensor) -> None:
         """Tokens on the host are looked at: one outside the vocabulary would be
@@ -165,7 +212,7 @@ class PagedDecoder:
         self._check_tokens(tokens)
         pages = self.pages.take(n // self.page)
         try:
-            self._prompts([tokens], [pages], [0])
+            self._prompts([tokens], [pages], [0], [len(self.open.free)] if self.codes is not None else [0])
         except BaseException:
             self.pages.give(pages)
             raise
@@ -180,17 +227,20 @@ class PagedDecoder:
                 raise ValueError(f"a prompt holds 1 to {self.max_positions - self.prefix_len} tokens")
             self._check_tokens(p)
         taken: list[list[int]] = []
+        opens = self._take_open(len(prompts))
         try:
             for p in prompts:
                 taken.append(self.pages.take(-(-int(p.shape[0]) // self.page)))
-            logits = self._prompts(prompts, [self.prefix_pages + t for t in taken], [self.prefix_len] * len(prompts))
+            logits = self._prompts(prompts, [self.prefix_pages + t for t in taken], [self.prefix_len] * len(prompts),
+                                   opens)
         except BaseException:
             for t in reversed(taken):
                 self.pages.give(t)
+            self._give_open(opens)
             raise
         ids = []
-        for p, t in zip(prompts, taken):
-            self.seqs[self._next] = {"pages": t, "len": int(p.shape[0])}
+        for p, t, o in zip(prompts, taken, opens):
+            self.seqs[self._next] = {"pages": t, "len": int(p.shape[0]), "open": o}
             ids.append(self._next)
             self._next += 1
         return ids, logits
@@ -223,7 +273,18 @@ class PagedDecoder:
 
     def _step(self, seqs: list[dict], tokens: torch.Tensor) -> torch.Tensor:
         positions = self._ints([self.prefix_len + s["len"] for s in seqs], torch.int64)
-        slots = self._ints([self._slots(s["pages"], s["len"], 1)[0] for s in seqs], torch.int64)
+        if self.codes is not None:
+            # (The prefix is read as every sequence's own beginning.)
+            table = self._table([self.prefix_pages + s["pages"] for s in seqs])
+            lens = self._ints([self.prefix_len + s["len"] + 1 for s in seqs])
+            open_slots, starts = self._ints([s["open"] for s in seqs]), self._ints(range(len(seqs) + 1))
+
+            def attend(layer, q):
+                return quantized.quantized_attention(q, self.cache[layer], table, open_slots, lens)
+
+            return self._forward(tokens.to(self.dec.device),
+                                 self._store_quantized(positions, table, open_slots, starts, lens), attend, slice(None))
+        store = self._store(positions, self._ints([self._slots(s["pages"], s["len"], 1)[0] for s in seqs], torch.int64))
         table, lens = self._table([s["pages"] for s in seqs]), self._ints([s["len"] + 1 for s in seqs])
         if self.prefix_len:
             prefix = self._ints(self.prefix_pages)
@@ -234,21 +295,37 @@ class PagedDecoder:
         else:
             def attend(layer, q):
                 return paged.paged_attention(q, self.k[layer], self.v[layer], table, lens)
-        return self._forward(tokens.to(self.dec.device), positions, slots, attend, slice(None))
+        return self._forward(tokens.to(self.dec.device), store, attend, slice(None))
 
     def free(self, seq: int) -> None:
         """Forget a sequence and return its pages."""
-        self.pages.give(self.seqs.pop(seq)["pages"])
+        s = self.seqs.pop(seq)
+        self.pages.give(s["pages"])
+        self._give_open([s["open"]])
 
-    def generate(self, prompts: list[torch.Tensor], steps: int) -> torch.Tensor:
-        """Greedy: the prompts' next ``steps`` tokens, [len(prompts), steps]."""
+    def sample(self, logits: torch.Tensor, generator: torch.Generator | None = None, **params) -> torch.Tensor:
+        """The next tokens of rows of logits: ``sample_tokens`` with ``params``
+        (temperature, top_k, top_p, min_p) and random numbers of ``generator``
+        (of the model's device; at world > 1 one is needed that every rank has
+        seeded alike). Without params the largest logits."""
+        if not params:
+            return logits.argmax(-1)
+        if self.dec.world > 1 and generator is None:
+            raise ValueError("sampling on several ranks needs a generator that all have seeded alike")
+        uniform = torch.rand(logits.shape[0], generator=generator, device=logits.device)
+        return sample_tokens(logits, uniform, **params)[0]
+
+    def generate(self, prompts: list[torch.Tensor], steps: int, generator: torch.Generator | None = None,
+                 **params) -> torch.Tensor:
+        """The prompts' next ``steps`` tokens, [len(prompts), steps]: greedy, or
+        drawn as ``sample`` draws them."""
         if steps < 1:
             return torch.empty((len(prompts), 0), dtype=torch.int64, device=self.dec.device)
         ids, logits = self.add(prompts)
         try:
-            out = [logits.argmax(-1)]
+            out = [self.sample(logits, generator, **params)]
             while len(out) < steps:
-                out.append(self.step(ids, out[-1]).argmax(-1))
+                out.append(self.sample(self.step(ids, out[-1]), generator, **params))
         finally:
             for i in ids:
                 self.free(i)
@@ -269,26 +346,34 @@ def main() -> None:
     ap.add_argument("--prefix", type=int, default=0, help="tokens that all sequences share (whole pages)")
     ap.add_argument("--steps", type=int, default=32)
     ap.add_argument("--page", type=int, default=16)
+    ap.add_argument("--cache", choices=("fp16", "int8", "e4m3"), default="fp16")
+    ap.add_argument("--temperature", type=float, default=0.0, help="0: the largest logit")
+    ap.add_argument("--top-k", type=int, default=0)
+    ap.add_argument("--top-p", type=float, default=1.0)
+    ap.add_argument("--min-p", type=float, default=0.0)
     args = ap.parse_args()
     base = D.LLAMA2_7B
     cfg = D.DecoderConfig(args.layers, base.hidden, base.n_heads, base.n_kv_heads, base.intermediate, base.vocab)
     dec = TPDecoder(cfg, QuantConfig(4, 128, False), device="cuda", kv_len=0, batch=min(args.seqs, 8))
     longest = args.prefix + args.prompt + args.steps
     pages = args.seqs * -(-(args.prompt + args.steps) // args.page) + args.prefix // args.page
-    serve = PagedDecoder(dec, pages, args.page, longest)
+    serve = PagedDecoder(dec, pages, args.page, longest, max_seqs=args.seqs,
+                         codes={"fp16": None, "int8": torch.int8, "e4m3": torch.float8_e4m3fn}[args.cache])
+    params = {} if args.temperature == 0 else dict(temperature=args.temperature, top_k=args.top_k, top_p=args.top_p,
+                                                   min_p=args.min_p)
     gen = torch.Generator().manual_seed(0)
     if args.prefix:
         serve.set_prefix(torch.randint(0, cfg.vocab, (args.prefix,), generator=gen))
     prompts = [torch.randint(0, cfg.vocab, (max(1, args.prompt * (i + 1) // args.seqs),), generator=gen)
                for i in range(args.seqs)]
-    serve.generate(prompts, 2)  # warm-up
+    serve.generate(prompts, 2, **params)  # warm-up
     torch.cuda.synchronize()
     t0 = time.perf_counter()
     ids, logits = serve.add(prompts)
     torch.cuda.synchronize()
     t1 = time.perf_counter()
     for _ in range(args.steps):
-        logits = serve.step(ids, logits.argmax(-1))
+        logits = serve.step(ids, serve.sample(logits, **params))
     torch.cuda.synchronize()
     t2 = time.perf_counter()
     total = sum(int(p.shape[0]) for p in prompts)
