@@ -191,8 +191,15 @@ __device__ __forceinline__ void store_block(const Params<E>& p, int b, const Seq
     const float2 two = Elem<E>::unpack(most);
     const bool finite = Elem<E>::non_finite(most) == 0u;
     const bool e4m3 = p.pool.e4m3;
-    const float scale = finite ? fmaxf(fmaxf(two.x, two.y) / (e4m3 ? E4m3::kMost : Int8::kMost), 1.17549435e-38f) : NAN;
-    const float inv = 1.f / scale;
+    // code = round(x / s), formed as (L x) / max |x|: the product is exact, and
+    // the quotient too where it is a number of few bits (a reciprocal's product,
+    // and one Newton step on the quotient), so that a value halfway between two
+    // codes is seen to be. Without that 1.5 times the rounding errors of codes,
+    // with a division 73 instead of 67 us for 8192 tokens.
+    const float largest = fmaxf(two.x, two.y), range = e4m3 ? E4m3::kMost : Int8::kMost;
+    const bool tiny = largest / range < 1.17549435e-38f;
+    const float scale = finite ? (tiny ? 1.17549435e-38f : largest / range) : NAN;
+    const float up = tiny ? 8.50705917e37f : range, down = tiny ? 1.f : largest, inv = 1.f / down;  // (2^126)
     if (page < 0) continue;
     if (threadIdx.x == 0) {
       float* to = (which ? p.pool.v_scale : p.pool.k_scale) + page * p.pool.scale_page_stride +
@@ -211,12 +218,14 @@ __device__ __forceinline__ void store_block(const Params<E>& p, int b, const Seq
       for (int run = 0; run < 2; ++run) {
         unpack8<E>(run ? xb[i] : xa[i], x);
         uint2 w = make_uint2(0, 0);
-        if (finite && e4m3) {
-          w.x = E4m3::pack4(x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
-          w.y = E4m3::pack4(x[4] * inv, x[5] * inv, x[6] * inv, x[7] * inv);
-        } else if (finite) {
-          w.x = Int8::pack4(x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
-          w.y = Int8::pack4(x[4] * inv, x[5] * inv, x[6] * inv, x[7] * inv);
+        if (finite) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const float t = x[e] * up, y = t * inv;
+            x[e] = fmaf(fmaf(-y, down, t), inv, y);
+          }
+          w = e4m3 ? make_uint2(E4m3::pack4(x[0], x[1], x[2], x[3]), E4m3::pack4(x[4], x[5], x[6], x[7]))
+                   : make_uint2(Int8::pack4(x[0], x[1], x[2], x[3]), Int8::pack4(x[4], x[5], x[6], x[7]));
         }
         __stcs(reinterpret_cast<uint2*>(codes + row * p.pool.row_stride + (run ? part.eb : part.ea)), w);
       }

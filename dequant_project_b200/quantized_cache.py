@@ -84,7 +84,10 @@ def quantize_block(x: torch.Tensor, codes: torch.dtype) -> tuple:
     x = x.float()
     most = x.abs().amax((-1, -2))
     scale = torch.where(torch.isfinite(most), (most / MOST[codes]).clamp(min=LEAST_SCALE), float("nan"))
-    y = torch.where(torch.isfinite(scale)[..., None, None], x / scale[..., None, None], 0.0)
+    # (L x) / max |x|, the product exact: x / scale without the scale's rounding.
+    tiny = (scale <= LEAST_SCALE)[..., None, None]
+    y = torch.where(tiny, x * 2.0 ** 126, x * MOST[codes] / most[..., None, None])
+    y = torch.where(torch.isfinite(scale)[..., None, None], y, 0.0)
     if codes == torch.int8:
         return torch.round(y).clamp(-127, 127).to(torch.int8), scale
     return y.clamp(-448, 448).to(codes), scale

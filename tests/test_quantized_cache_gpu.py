@@ -3,10 +3,10 @@ restatements.
 
 Stored blocks: the 16-bit values that the codes stand for are those that
 ``rope_paged_append`` writes for the same tokens (bit for bit). A scale is
-max(fp32(max|x| / L), 2^-126) exactly. A code is x * fp32(1 / scale) rounded to
-nearest: two fp32 roundings of a number of at most L before it, so |code - x /
-scale| <= half a step + 2^-22 |x / scale|, a step being 1 (int8) or, for e4m3,
-2^-3 of the power of two at or below |x / scale|, 2^-9 at least.
+max(fp32(max|x| / L), 2^-126) exactly. A code is fp32(L x / max|x|) rounded to
+nearest, which is x / scale but for two fp32 roundings (the scale's and this), so
+|code - x / scale| <= half a step + 2^-22 |x / scale|, a step being 1 (int8) or,
+for e4m3, 2^-3 of the power of two at or below |x / scale|, 2^-9 at least.
 
 Attention: outputs are rounded once to 16 bits (unit roundoff u = 2^-11 fp16,
 2^-8 bf16) and each softmax weight once to 16 bits before the product with the
