@@ -85,6 +85,11 @@ __device__ __forceinline__ uint32_t transposed(uint32_t x) {
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
 }
+__device__ __forceinline__ float max3(float x, float y, float z) {
+  float m;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(m) : "f"(x), "f"(y), "f"(z));
+  return m;
+}
 __device__ __forceinline__ float log2_approx(float x) {
   float y;
   asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -184,7 +189,7 @@ __global__ void __launch_bounds__(kThreads, Layout<D, NB>::kCtasPerSm)
   float* ms = os + L::kMerge / 4;                                // [warp][16]: the scores' reference,
   float* vs = ms + kWarps * 16;                                  // the values',
   float* ls = vs + kWarps * 16;                                  // and the sum
-  float* scales = ls + kWarps * 16;                              // [stage][2][kWarps]
+  float* scales = ls + kWarps * 16;                              // [stage][slice][key, value]
   uint64_t* full = reinterpret_cast<uint64_t*>(scales + L::kScaleBytes / 4);
   uint64_t* empty = full + kStages;
   uint64_t* q_full = empty + kStages;
@@ -264,7 +269,7 @@ __global__ void __launch_bounds__(kThreads, Layout<D, NB>::kCtasPerSm)
             const int in_page = (x * kTile + slice * 16) & ((1 << p.page_shift) - 1);
             tma_load_4d(smem_u32(dst) + lane * (16 * D), values ? &vmap : &kmap, full + st, 0, in_page, i.kvh,
                         good ? page : n_pages);
-            float* to = scales + st * 2 * kWarps + lane;
+            float* to = scales + (st * kWarps + slice) * 2 + (values ? 1 : 0);
             if (good) {
               cp_async4(smem_u32(to), (values ? p.v_scale : p.k_scale) + page * p.scale_page_stride +
                         i.kvh * p.scale_head_stride + (in_page >> p.block_shift));
@@ -425,7 +430,7 @@ __global__ void __launch_bounds__(kThreads, Layout<D, NB>::kCtasPerSm)
           for (int e = 0; e < 4; ++e) {
             a[nb][e] = fmaf(sc[nb][e], f[nb][e & 1], -ref[nb][e & 1]);
             b[nb][e] = fmaf(sc[nb][e], f[nb][e & 1], lv - ref_v[nb][e & 1]);
-            most = fmaxf(most, fmaxf(a[nb][e], b[nb][e]));
+            most = max3(most, a[nb][e], b[nb][e]);
           }
         if (__any_sync(0xffffffffu, most > kHeadroom + kMaxGrowth)) {
 #pragma unroll
@@ -470,8 +475,8 @@ __global__ void __launch_bounds__(kThreads, Layout<D, NB>::kCtasPerSm)
         if (await(full + stage, parity)) {
           if (x < whole || i.len == done) {
             if (x * kTile + p0 < done) {
-              const float ks = scales[stage * 2 * kWarps + warp];
-              const float lv = log2_approx(scales[stage * 2 * kWarps + kWarps + warp]) + Pair::kUnit;
+              const float2 both = *reinterpret_cast<const float2*>(scales + (stage * kWarps + warp) * 2);
+              const float ks = both.x, lv = log2_approx(both.y) + Pair::kUnit;
               float sc[NB][4], f[NB][2];
               int sums[NB][2][4];
 #pragma unroll
