@@ -21,6 +21,16 @@
 // largest of five weights that has top_p of the sum from it on. The tokens that
 // are left, mostly a few, are listed once and read from there; up to 256 of them
 // are not searched at all, but ranked by one CTA that compares each with all.
+//
+// Neither HBM nor arithmetic bounds it, but the chain of steps that each need
+// the whole row's last (barriers are the largest stall: 6.8 cycles a warp's
+// instruction): 64 rows of 128256 in fp16 with all parameters 31 us (16.4 MB,
+// 2.5 us), up to 50 where the cuts fall in flat places, one row of 32000 13 us,
+// 256 rows of 32000 in fp32 33 us. Top-k alone (50) takes 18 us for the 64 rows;
+// top-p of 0.9 over normal logits (deviation 3), whose cut lies among tens of
+// thousands of tokens, 114. A row a CTA with a 64-bit exp took 412 us, clusters
+// 116, weights in pairs 61, short lists 42; rows kept in their own type, so that
+// half the CTAs hold one and all 64 rows run at once, 31.
 #include <cstdint>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -47,7 +57,7 @@ constexpr int kLevels = 5;              // weights 2^-4, 2^-7, 2^-10, 2^-13, 2^-
 struct Params {
   SampleArgs a;
   int ctas;  // a row
-  int run;   // tokens a thread: odd, so that reads of shared memory do not conflict
+  int run;   // tokens a thread: an odd number of words, so that reads of shared memory do not conflict
 };
 
 // 2^(j / 64), as an integer of 44 fractional bits and as a float times 2^31.
@@ -70,23 +80,63 @@ constexpr Powers powers() {
 }
 __device__ const Powers kPowers = powers();
 
+// Types of logits, as a row is kept in shared memory: words of one or two.
 template <typename T>
 struct Logit;
 template <>
 struct Logit<float> {
   static constexpr int kDrop = 0;  // low bits of an fp32 value that these never use
+  static constexpr uint32_t kLowest = 0xff800000u;
   static __device__ __forceinline__ float load(float v) { return v; }
+  static __device__ __forceinline__ float store(float v) { return v; }
+  // The larger of two words' values; NaN loses.
+  static __device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b) {
+    return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b)));
+  }
+  static __device__ __forceinline__ float2 both(uint32_t w) { return make_float2(__uint_as_float(w), -INFINITY); }
 };
 template <>
 struct Logit<__half> {
   static constexpr int kDrop = 13;
+  static constexpr uint32_t kLowest = 0xfc00fc00u;
   static __device__ __forceinline__ float load(__half v) { return __half2float(v); }
+  static __device__ __forceinline__ __half store(float v) { return __float2half_rn(v); }
+  static __device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b) {
+    const __half2 m = __hmax2(reinterpret_cast<const __half2&>(a), reinterpret_cast<const __half2&>(b));
+    return reinterpret_cast<const uint32_t&>(m);
+  }
+  static __device__ __forceinline__ float2 both(uint32_t w) {
+    return __half22float2(reinterpret_cast<const __half2&>(w));
+  }
 };
 template <>
 struct Logit<__nv_bfloat16> {
   static constexpr int kDrop = 16;
+  static constexpr uint32_t kLowest = 0xff80ff80u;
   static __device__ __forceinline__ float load(__nv_bfloat16 v) { return __bfloat162float(v); }
+  static __device__ __forceinline__ __nv_bfloat16 store(float v) { return __float2bfloat16_rn(v); }
+  static __device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b) {
+    const __nv_bfloat162 m =
+        __hmax2(reinterpret_cast<const __nv_bfloat162&>(a), reinterpret_cast<const __nv_bfloat162&>(b));
+    return reinterpret_cast<const uint32_t&>(m);
+  }
+  static __device__ __forceinline__ float2 both(uint32_t w) {
+    return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+  }
 };
+
+// f(logit, place) for the words from, from + step, ... of the first `count`
+// tokens at x; kEven: count fills its words.
+template <typename T, bool kEven, class F>
+__device__ __forceinline__ void each_word(const T* x, int from, int step, int count, F f) {
+  constexpr int kPack = 4 / sizeof(T);
+#pragma unroll 4
+  for (int i = from * kPack; i < count; i += step * kPack) {
+    const float2 v = Logit<T>::both(*reinterpret_cast<const uint32_t*>(x + i));
+    f(v.x, i);
+    if (kPack == 2 && (kEven || i + 1 < count)) f(v.y, i + 1);
+  }
+}
 
 // Integers whose order is the values' (both zeros alike), and back.
 template <int kDrop>
@@ -100,7 +150,7 @@ __device__ __forceinline__ float value_of(uint32_t key) {
   return __uint_as_float(u >> 31 ? u & 0x7fffffffu : ~(u | ((1u << kDrop) - 1)));
 }
 
-struct Shared {
+struct alignas(16) Shared {
   Power powers[64];
   uint32_t own[3][kBins];     // this CTA's histogram: numbers, or 16 bits of the weights each
   // The cluster's, of the bins that this CTA holds (every ctas-th; a CTA alone
@@ -300,7 +350,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
   extern __shared__ __align__(16) uint8_t smem_raw[];
   const SampleArgs& p = q.a;
   Shared* sh = reinterpret_cast<Shared*>(smem_raw);
-  float* x = reinterpret_cast<float*>(sh + 1);
+  T* x = reinterpret_cast<T*>(sh + 1);
   const int ctas = q.ctas, rank = static_cast<int>(cluster_ctarank()), row = blockIdx.x / ctas;
   const int lane = threadIdx.x & 31;
   const int slice = q.run * kThreads, base = rank * slice, n = max(0, min(slice, p.vocab - base));
@@ -315,25 +365,29 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
   min_p = min_p > 0.f ? fminf(min_p, 1.f) : 0.f;
 
   // The row's part into shared memory; NaN becomes -inf.
-  float largest = -INFINITY;
+  float largest;
   {
+    using L = Logit<T>;
     const T* from = static_cast<const T*>(p.logits) + row * p.row_stride + base;
     constexpr int kVec = 16 / sizeof(T);
     const int whole = reinterpret_cast<uintptr_t>(from) % 16 ? 0 : n / kVec * kVec;
-    auto put = [&](int i, float v) {
-      v = v == v ? v : -INFINITY;
-      largest = fmaxf(largest, v);
-      x[i] = v;
-    };
+    uint32_t most = L::kLowest;
 #pragma unroll 4
     for (int i = threadIdx.x * kVec; i < whole; i += kThreads * kVec) {
-      const uint4 raw = __ldg(reinterpret_cast<const uint4*>(from + i));
-      const T* v = reinterpret_cast<const T*>(&raw);
-#pragma unroll
-      for (int k = 0; k < kVec; ++k) put(i + k, Logit<T>::load(v[k]));
+      uint4 w = __ldg(reinterpret_cast<const uint4*>(from + i));
+      w = make_uint4(L::larger(w.x, L::kLowest), L::larger(w.y, L::kLowest), L::larger(w.z, L::kLowest),
+                     L::larger(w.w, L::kLowest));
+      most = L::larger(L::larger(L::larger(most, w.x), L::larger(w.y, w.z)), w.w);
+      *reinterpret_cast<uint4*>(x + i) = w;
     }
-    for (int i = whole + threadIdx.x; i < n; i += kThreads) put(i, Logit<T>::load(from[i]));
-    for (int i = n + threadIdx.x; i < slice; i += kThreads) x[i] = -INFINITY;
+    const float2 two = L::both(most);
+    largest = fmaxf(two.x, two.y);
+    for (int i = whole + threadIdx.x; i < slice; i += kThreads) {
+      float v = i < n ? L::load(from[i]) : -INFINITY;
+      v = v == v ? v : -INFINITY;
+      largest = fmaxf(largest, v);
+      x[i] = L::store(v);
+    }
   }
   float m = block_reduce(largest, sh->scratch, [](float a, float b) { return fmaxf(a, b); });
   if (threadIdx.x == 0) {
@@ -355,7 +409,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
   if (!(heat > 0.f)) {
     uint32_t at = 0xffffffffu;
     for (int j = q.run - 1; j >= 0; --j)
-      if (x[first + j] == m) at = base + first + j;
+      if (Logit<T>::load(x[first + j]) == m) at = base + first + j;
     at = block_reduce(at, sh->scratch, [](uint32_t a, uint32_t b) { return min(a, b); });
     if (threadIdx.x == 0) sh->first = at;
     cluster_sync();
@@ -369,7 +423,8 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
   }
   if (m == INFINITY) {
     // Tokens at +inf weigh one and all others nothing, whatever the temperature.
-    for (int i = threadIdx.x; i < slice; i += kThreads) x[i] = x[i] == INFINITY ? 0.f : -INFINITY;
+    for (int i = threadIdx.x; i < slice; i += kThreads)
+      x[i] = Logit<T>::store(Logit<T>::load(x[i]) == INFINITY ? 0.f : -INFINITY);
     largest = largest == INFINITY ? 0.f : -INFINITY;
     m = 0.f;
     __syncthreads();
@@ -397,15 +452,14 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
     if (listed) {
       for (int i = threadIdx.x, c = sh->listed; i < c; i += kThreads) f(sh->list[i]);
     } else {
-      for (int i = threadIdx.x; i < n; i += kThreads) f(x[i]);
+      each_word<T, false>(x, threadIdx.x, kThreads, n, [&](float v, int) { f(v); });
     }
   };
   // Lists this CTA's tokens from `least` on; a list that they do not fit is not used.
   auto make_list = [&](float least) {
     // (Counted first, so that a warp takes its places in the list at once.)
     uint32_t c = 0;
-#pragma unroll 4
-    for (int i = threadIdx.x; i < slice; i += kThreads) c += x[i] >= least;
+    each_word<T, true>(x, threadIdx.x, kThreads, slice, [&](float v, int) { c += v >= least; });
     uint32_t sum = c, at = 0;
 #pragma unroll
     for (int off = 1; off < 32; off <<= 1) {
@@ -415,12 +469,12 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
     if (lane == 31) at = atomicAdd(&sh->listed, sum);
     at = __shfl_sync(0xffffffffu, at, 31) + sum - c;
     if (c && at + c <= kListed)
-#pragma unroll 4
-      for (int i = threadIdx.x; i < slice; i += kThreads)
-        if (const float v = x[i]; v >= least) {
+      each_word<T, true>(x, threadIdx.x, kThreads, slice, [&](float v, int i) {
+        if (v >= least) {
           sh->places[at] = static_cast<uint16_t>(i);
           sh->list[at++] = v;
         }
+      });
     __syncthreads();
     listed = sh->listed <= kListed;
   };
@@ -562,8 +616,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
     if (listed) {
       each(take);
     } else {
-#pragma unroll 4
-      for (int i = threadIdx.x; i < slice; i += kThreads) take(x[i]);
+      each_word<T, true>(x, threadIdx.x, kThreads, slice, [&](float v, int) { take(v); });
     }
 #pragma unroll
     for (int k = 0; k < kLevels + 2; ++k) {
@@ -633,7 +686,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
       __syncthreads();
       ties = sh->own[0][threadIdx.x];
     } else {
-      for (int j = 0; j < q.run; ++j) ties += x[first + j] == cut;
+      each_word<T, true>(x + first, 0, 1, q.run, [&](float v, int) { ties += v == cut; });
     }
     u64 all;
     uint32_t ahead = static_cast<uint32_t>(block_scan(ties, sh->scratch, &all)), before;
@@ -646,7 +699,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
     if (ahead < room && room < ahead + ties) {
       uint32_t left = room - ahead;
       for (int j = 0; left > 0; ++j)
-        if (x[first + j] == cut && --left == 0) sh->limit = first + j;
+        if (Logit<T>::load(x[first + j]) == cut && --left == 0) sh->limit = first + j;
     } else if (ahead == room && ties > 0 && ahead > before) {
       // The last one kept lies in an earlier run of this CTA, which ends with it.
       atomicMin(&sh->limit, first - 1);
@@ -662,11 +715,10 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
   };
   u64 mine = 0, total = 0;
   if (cut == -INFINITY) {
-#pragma unroll 4
-    for (int j = 0; j < q.run; ++j) {
-      const u64 w = weight(x[first + j]);
+    each_word<T, true>(x + first, 0, 1, q.run, [&](float v, int) {
+      const u64 w = weight(v);
       mine += w >= least_w ? w : 0;
-    }
+    });
   } else if (listed) {
     // From the list: a run's sum in 16 bits of the weights each.
     for (int i = threadIdx.x; i < 3 * kThreads; i += kThreads) (&sh->own[0][0])[i] = 0;
@@ -682,7 +734,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
     const uint32_t* run = &sh->own[0][threadIdx.x];
     mine = run[0] + (static_cast<u64>(run[kThreads]) << 16) + (static_cast<u64>(run[2 * kThreads]) << 32);
   } else {
-    for (int j = 0; j < q.run; ++j) mine += kept(x[first + j], first + j);
+    each_word<T, true>(x + first, 0, 1, q.run, [&](float v, int j) { mine += kept(v, first + j); });
   }
   u64 before = block_scan(mine, sh->scratch, &total);
   if (threadIdx.x == 0) sh->total = total;
@@ -700,7 +752,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
     before = __shfl_sync(0xffffffffu, before, src);
     const int from = __shfl_sync(0xffffffffu, first, src);
     for (int j0 = 0; j0 < q.run; j0 += 32) {
-      const float v = j0 + lane < q.run ? x[from + j0 + lane] : -INFINITY;
+      const float v = j0 + lane < q.run ? Logit<T>::load(x[from + j0 + lane]) : -INFINITY;
       const u64 w = kept(v, from + j0 + lane);
       u64 sum = w;
 #pragma unroll
@@ -726,15 +778,16 @@ template <typename T>
 cudaError_t launch(const SampleArgs& a, int num_sms, cudaStream_t stream) {
   Params p;
   p.a = a;
-  // CTAs a row: enough for their shared memory to hold 16384 tokens each at
-  // most, and, while they do not fill the GPU, until a CTA has 2048.
+  // CTAs a row: enough for 64 KB of it each at most, so that two CTAs share an
+  // SM, and, while they do not fill the GPU, until a CTA has 2048 tokens.
+  constexpr int kPack = 4 / sizeof(T), kMost = 16384 * kPack;
   int ctas = 1;
-  while (ctas < kMaxCtas && (a.vocab > ctas * 16384 || (static_cast<int64_t>(a.rows) * ctas <= num_sms &&
+  while (ctas < kMaxCtas && (a.vocab > ctas * kMost || (static_cast<int64_t>(a.rows) * ctas <= num_sms &&
                                                         a.vocab > ctas * 2048)))
     ctas *= 2;
   p.ctas = ctas;
-  p.run = ((a.vocab + ctas - 1) / ctas + kThreads - 1) / kThreads | 1;
-  const size_t smem = sizeof(Shared) + static_cast<size_t>(p.run) * kThreads * 4;
+  p.run = kPack * (((a.vocab + ctas - 1) / ctas + kPack * kThreads - 1) / (kPack * kThreads) | 1);
+  const size_t smem = sizeof(Shared) + static_cast<size_t>(p.run) * kThreads * sizeof(T);
   static int configured[64] = {0};
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);

@@ -31,8 +31,10 @@ def sample_tokens(logits: torch.Tensor, uniform: torch.Tensor, *, temperature: t
     token is the first, by index, whose running sum of kept w exceeds uniform
     times their sum; its logprob is that of this draw. A temperature of 0 (or
     less) takes the largest logit, with logprob 0. NaN counts as -inf; a row
-    without a logit above -inf gives -1 and NaN. The same inputs give the same
-    tokens: sums are exact (64-bit integers), whatever their order.
+    without a logit above -inf gives -1 and NaN. A ``uniform`` below 0, or NaN,
+    counts as 0; from 1 on it takes the last token kept. The same inputs give the
+    same tokens: each w is rounded once (2^-31 of itself, or 2^-45) and sums are of
+    64-bit integers, whatever their order.
 
     Each parameter is a number (taken as fp32; top_k as int32), or a tensor of one a
     row of these types."""

@@ -1,12 +1,12 @@
 """The draw of tokens on the GPU against the 64-bit restatement on the CPU.
 
-The kernel's weights are rounded to 2^-45 and their sums exact, the
-restatement's sums are off by up to n 2^-53: over a row of n <= 2^18 tokens a
-running sum differs by less than 2^-26 of the largest weight (2^-33 for n <=
-2^11), and a token can differ only where uniform * total falls that near a
-border. The draws here keep away from borders by that much (checked), so tokens
-are equal. Logprobs are formed in 64 bits and rounded once: 2^-24 relative, and
-2^-25 for what the sums are off.
+The kernel's weights are exact to 2^-31 of themselves and rounded to 2^-45, their
+sums exact; the restatement's sums are off by up to n 2^-53. So a running sum
+differs by less than 2^-31 of itself and n 2^-45 of the largest weight (2^-27 for
+n = 2^18), and a token can differ only where uniform * total, or top_p * total,
+falls that near a border: for a random draw that is a chance of about n 2^-30.
+With the fixed seeds here none does, so tokens are equal. Logprobs are formed in 64 bits and rounded
+once: 2^-24 relative, and 2^-25 for what the sums are off.
 """
 
 from __future__ import annotations
