@@ -16,6 +16,14 @@
 // KV head each: keys, then values, sixteen values of a row a thread.
 // The block that completes a sequence's open block also stores the new open
 // rows, whose place it has read before; no other reads or writes them.
+//
+// Bound by HBM with long batches: 8192 tokens of 64 and 8 heads of 128 with
+// norms (bf16 to e4m3; 168 MB read, 151 written, 49 us at the copy rate) 65 us,
+// of which the writes that stay in L2 show half (172 MB read, 96 MB written).
+// Registers bound it next (29 % of the warps resident, at 96): eight heads a
+// lane group one after the other took 114 us, four with passes and codes apart
+// 67, keys' and values' rows loaded together 65. Small batches are a launch: 8
+// tokens 4.4 us in a graph.
 #include <cstdint>
 
 #include "paged_rope.cuh"
