@@ -179,7 +179,8 @@ int dqg_expand_pages(const dqg_quantized_kv* kv, const int32_t* block_table, int
   if (n_pages > 0 && ((rc = check_ptr(k_out, 16, "k_out")) != DQG_OK || (rc = check_ptr(v_out, 16, "v_out")) != DQG_OK))
     return rc;
   const cudaError_t e =
-      dqg::launch_expand_pages(pool, seqs, n_pages, k_out, v_out, table_out, nullptr, 0, static_cast<cudaStream_t>(stream));
+      dqg::launch_expand_pages(pool, seqs, n_pages, k_out, v_out, table_out, nullptr, 0, 0.f,
+                               static_cast<cudaStream_t>(stream));
   if (e != cudaSuccess) return api_cuda_fail(e, "expand_pages launch");
   return api_ok();
 }
@@ -189,7 +190,7 @@ int dqg_expand_pages(const dqg_quantized_kv* kv, const int32_t* block_table, int
 namespace {
 // What a prompt call leaves between its kernels.
 struct PromptScratch {
-  uint64_t k, v, table, scales, pieces, bytes;  // offsets, and all of it
+  uint64_t k, v, table, factors, pieces, bytes;  // offsets, and all of it
   int64_t scale_stride, n_pages;
 };
 PromptScratch prompt_scratch(const dqg::QuantizedPool& pool, int64_t n_seqs, int64_t table_width, int64_t n_pages,
@@ -203,8 +204,8 @@ PromptScratch prompt_scratch(const dqg::QuantizedPool& pool, int64_t n_seqs, int
   s.k = 0;
   s.v = pages;
   s.table = 2 * pages;
-  s.scales = s.table + up(static_cast<uint64_t>(n_seqs) * table_width * 4);
-  s.pieces = s.scales + up(static_cast<uint64_t>(s.scale_stride) * pool.n_kv_heads * 4);
+  s.factors = s.table + up(static_cast<uint64_t>(n_seqs) * table_width * 4);
+  s.pieces = s.factors + up(static_cast<uint64_t>(s.scale_stride) * pool.n_kv_heads * 16);
   s.bytes = s.pieces + dqg::prompt_workspace(pool.D, sms);
   return s;
 }
@@ -267,9 +268,10 @@ int dqg_quantized_prompt_attention(const void* q, int64_t q_stride_row, int64_t 
   CUtensorMap qmap, kmap, vmap;
   if ((rc = query_map(q, pages, T, n_q_heads, q_stride_row, q_stride_head, &qmap)) != DQG_OK) return rc;
   if ((rc = pool_maps(pages, dqg::prompt_box_rows(pages.page_size), &kmap, &vmap)) != DQG_OK) return rc;
-  float* scales = reinterpret_cast<float*>(ws + s.scales);
-  cudaError_t e = dqg::launch_expand_pages(pool, seqs, s.n_pages, ws + s.k, ws + s.v, table, scales, s.scale_stride,
-                                           static_cast<cudaStream_t>(stream));
+  float* factors = reinterpret_cast<float*>(ws + s.factors);
+  const float scale_log2 = static_cast<float>(scale * kLog2e);
+  cudaError_t e = dqg::launch_expand_pages(pool, seqs, s.n_pages, ws + s.k, ws + s.v, table, factors, s.scale_stride,
+                                           scale_log2, static_cast<cudaStream_t>(stream));
   if (e != cudaSuccess) return api_cuda_fail(e, "quantized_prompt_attention launch");
   dqg::PromptArgs a;
   std::memset(&a, 0, sizeof(a));
@@ -284,8 +286,8 @@ int dqg_quantized_prompt_attention(const void* q, int64_t q_stride_row, int64_t 
   a.T = static_cast<int>(T);
   a.hq = static_cast<int>(n_q_heads);
   a.causal = causal != 0;
-  a.scale_log2 = static_cast<float>(scale * kLog2e);
-  a.k_scales = scales;
+  a.scale_log2 = scale_log2;
+  a.factors = factors;
   a.scale_stride = s.scale_stride;
   e = dqg::launch_prompt(pages, qmap, kmap, vmap, a, sms, static_cast<cudaStream_t>(stream));
   if (e != cudaSuccess) return api_cuda_fail(e, "quantized_prompt_attention launch");

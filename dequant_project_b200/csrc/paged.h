@@ -86,10 +86,13 @@ struct PromptArgs {
   // A prefix: T rows see the same prefix_len keys of one table row; the
   // pieces go to the workspace as PrefixPieces describes. 0: a prompt.
   int prefix_len;
-  // Keys that are codes: fp32 scales, one for every sixteen positions, of KV
-  // head h at h * scale_stride and of sequence b from
-  // scaled_keys_begin(table[b][0], page size, b) on. Null: none.
-  const float* k_scales;
+  // Keys that are codes, and values that are but for a factor f: three fp32
+  // numbers for every sixteen positions, the keys' scale, log2(f) / scale_log2
+  // and 1 / f. 128 positions have 32 numbers: eight of each kind, and eight that
+  // nothing uses. Position t of sequence b has number s = scaled_keys_begin(
+  // table[b][0], page size, b) + t / 16 of its KV head, whose 32 begin at
+  // 4 * (h * scale_stride + s / 8 * 8). Null: none.
+  const float* factors;
   int64_t scale_stride;
 };
 // (Multiples of eight, and apart for sequences whose pages follow one another.)

@@ -104,7 +104,7 @@ struct Params {
   uint32_t g_magic;                   // ceil(2^32 / g), 0 for g = 1
   bool n_units32;                     // the units of any lengths fit 31 bits
   int prefix_len, splits, n_pieces;   // a shared prefix: splits > 0
-  const float* k_scales;              // scaled keys: see PromptArgs
+  const float* factors;               // keys and values as codes: see PromptArgs
   int64_t scale_stride;
 };
 
@@ -191,15 +191,6 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
       "fma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
       : "=f"(d.x), "=f"(d.y)
       : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
-  return d;
-}
-__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
-  float2 d;
-  asm("{\n\t.reg .b64 a, b, d;\n\t"
-      "mov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
-      "mul.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
-      : "=f"(d.x), "=f"(d.y)
-      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
   return d;
 }
 __device__ __forceinline__ float2 add2(float2 a, float2 b) {
@@ -867,15 +858,20 @@ __global__ void __launch_bounds__(kThreads, 1)
       float m = -INFINITY, l = 0.f;
       for (int j = 0; j < n; ++j) {
         const int k0 = (x0 + j) * kBlock;
-        float4 ks[2] = {};
+        const float4* factors = nullptr;
+        float4 ks[2] = {}, vs[2] = {};
         if (kScaled) {
-          // Keys are codes: their scales, one for every sixteen, go to the scores.
+          // Keys are codes, and values but for a power of two: what is left of
+          // the scales, for every sixteen positions, goes to the scores and, as
+          // its logarithm, to the weights of the values.
           // (A sequence whose pages found no room may point anywhere.)
           const int64_t at = static_cast<int64_t>(g.scales) + k0 / 16;
           if (at >= 0 && at + 8 <= p.scale_stride) {
-            const float4* from = reinterpret_cast<const float4*>(p.k_scales + g.kvh * p.scale_stride + at);
-            ks[0] = __ldg(from);
-            ks[1] = __ldg(from + 1);
+            factors = reinterpret_cast<const float4*>(p.factors + 4 * (g.kvh * p.scale_stride + at));
+            ks[0] = __ldg(factors);
+            ks[1] = __ldg(factors + 1);
+            vs[0] = __ldg(factors + 2);
+            vs[1] = __ldg(factors + 3);
           }
         }
         if (!warp_wait(s_full + t, scores & 1)) {
@@ -895,11 +891,15 @@ __global__ void __launch_bounds__(kThreads, 1)
           // (Before any score is hidden: a block that the row does not see may
           // have any scale. Applied to groups' maxima and in the weights' first
           // product instead, the scales would be fewer instructions, but more
-          // registers than there are: 2048 tokens 82 us instead of 74.)
+          // registers than there are: 2048 tokens 82 us instead of 74. Without
+          // the values' part, so with values rounded as they are expanded, a
+          // call took 2 us less and was off by half as much again.)
           const float f[8] = {ks[0].x, ks[0].y, ks[0].z, ks[0].w, ks[1].x, ks[1].y, ks[1].z, ks[1].w};
+          const float a[8] = {vs[0].x, vs[0].y, vs[0].z, vs[0].w, vs[1].x, vs[1].y, vs[1].z, vs[1].w};
 #pragma unroll
           for (int i = 0; i < kBlock; i += 2) {
-            const float2 x = mul2(make_float2(s[i], s[i + 1]), make_float2(f[i / 16], f[i / 16]));
+            const float2 x = fma2(make_float2(s[i], s[i + 1]), make_float2(f[i / 16], f[i / 16]),
+                                  make_float2(a[i / 16], a[i / 16]));
             s[i] = x.x;
             s[i + 1] = x.y;
           }
@@ -946,6 +946,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         const float ref = m == -INFINITY ? 0.f : fmaf(m, p.scale_log2, -kHeadroom);
         const float2 ref2 = make_float2(-ref, -ref);
         float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+        float4 inv[2] = {};
+        if (kScaled && factors) {
+          inv[0] = __ldg(factors + 4);
+          inv[1] = __ldg(factors + 5);
+        }
+        const float per[8] = {inv[0].x, inv[0].y, inv[0].z, inv[0].w, inv[1].x, inv[1].y, inv[1].z, inv[1].w};
+        float2 part;
         // The products take the first kEarly weights while the rest is formed.
         auto weigh = [&](int from, uint32_t* w, int n) {
 #pragma unroll
@@ -953,8 +960,14 @@ __global__ void __launch_bounds__(kThreads, 1)
             float2 x = fma2(make_float2(s[from + 2 * i], s[from + 2 * i + 1]), scale2, ref2);
             x.x = exp2_approx(x.x);
             x.y = exp2_approx(x.y);
-            sum[i & 1] = add2(sum[i & 1], x);
             w[i] = Elem<E>::pack(x.x, x.y);
+            if (kScaled) {  // (the softmax's sum is of the weights without the values' factor)
+              part = i % 8 == 0 ? x : add2(part, x);
+              const float f = per[(from + 2 * i) / 16];
+              if (i % 8 == 7) sum[0] = fma2(part, make_float2(f, f), sum[0]);
+            } else {
+              sum[i & 1] = add2(sum[i & 1], x);
+            }
           }
         };
         {
@@ -1254,9 +1267,9 @@ cudaError_t launch_prompt(const PagedPool& pool, const CUtensorMap& qmap, const 
   p.part = static_cast<float4*>(a.workspace);
   p.ml = reinterpret_cast<float*>(p.part + slots * 64 * pool.D);
   p.desc = reinterpret_cast<Desc*>(p.ml + slots * 512);
-  p.k_scales = a.k_scales;
+  p.factors = a.factors;
   p.scale_stride = a.scale_stride;
-  return a.k_scales ? launch_for<true>(p, pool, qmap, kmap, vmap, num_sms, stream)
+  return a.factors ? launch_for<true>(p, pool, qmap, kmap, vmap, num_sms, stream)
                     : launch_for<false>(p, pool, qmap, kmap, vmap, num_sms, stream);
 }
 

@@ -54,8 +54,8 @@ cudaError_t launch_quantized_append(const QuantizedPool& pool, const QuantizedSe
                                     const QuantizedAppendArgs& a, int num_sms, cudaStream_t stream);
 
 cudaError_t launch_expand_pages(const QuantizedPool& pool, const QuantizedSeqs& seqs, int64_t n_pages,
-                                void* k_out, void* v_out, int32_t* table_out, float* k_scales, int64_t scale_stride,
-                                cudaStream_t stream);
+                                void* k_out, void* v_out, int32_t* table_out, float* factors, int64_t scale_stride,
+                                float scale_log2, cudaStream_t stream);
 
 struct QuantizedAttentionArgs {
   const void* q;  // [B, hq, D], strides in elements

@@ -210,7 +210,8 @@ def quantized_prompt_attention(q: torch.Tensor, cache: QuantizedCache, block_tab
                                workspace: torch.Tensor | None = None) -> torch.Tensor:
     """``paged_ops.prompt_attention`` over an 8-bit cache, whose positions are
     first expanded once to 16-bit pages (as ``expanded_pages``, which says what
-    ``n_pages`` is; but keys stay codes, and their scales go to the scores).
+    ``n_pages`` is; but keys stay codes and values codes times a power of two, exact
+    in 16 bits, and the rest of the scales goes to the scores and weights in fp32).
     ``workspace``: ``quantized_prompt_workspace``, mostly n_pages * 4 * Hkv *
     page size * D bytes; calls that share one must not overlap. Everything else
     as ``prompt_attention``."""
@@ -224,7 +225,7 @@ def quantized_prompt_attention(q: torch.Tensor, cache: QuantizedCache, block_tab
         lo, hi, n = int(q_starts[b]), int(q_starts[b + 1]), int(kv_lens[b])
         ends = n - (hi - lo) + torch.arange(hi - lo) + 1 if causal else torch.full((hi - lo,), n)
         k, v = (_rows(cache, w, block_table[b], int(open_slots[b]), n) for w in (0, 1))
-        out[lo:hi] = paged._cpu_attention(q[lo:hi].float(), k, v.to(q.dtype).float(), ends, scale).to(q.dtype)
+        out[lo:hi] = paged._cpu_attention(q[lo:hi].float(), k, v, ends, scale).to(q.dtype)
     return out
 
 

@@ -490,7 +490,8 @@ typedef struct dqg_quantized_kv {
  * rounded to nearest; rows of a block that is not go to the open block. A
  * block that holds a value that is not finite gets the scale NaN. A sequence
  * whose rows are out of order or range, or more than its length, is not
- * stored, and sets bit 1 of dqg_device_status.
+ * stored, and sets bit 1 of dqg_device_status (starts out of order may leave out
+ * rows of other sequences too).
  */
 int dqg_rope_quantized_append(const void *qkv, int64_t T, int64_t qkv_stride, int64_t n_q_heads,
                               const float *cos_table, const float *sin_table, int64_t n_positions,
@@ -519,8 +520,8 @@ int dqg_expand_pages(const dqg_quantized_kv *kv, const int32_t *block_table, int
 /*
  * dqg_prompt_attention over such a cache. The sequences' positions are first
  * expanded once, into the workspace, as dqg_expand_pages does, but with keys as
- * codes, which are exact in 16 bits; their scales are applied to the scores in
- * fp32. n_pages as there; what sequences give that it leaves pages of out is
+ * codes and values as codes times a power of two, which are exact in 16 bits; the
+ * rest of the scales is applied to scores and weights in fp32. n_pages as there; what sequences give that it leaves pages of out is
  * undefined. Workspace: dqg_quantized_prompt_workspace's bytes (mostly n_pages
  * pages of n_kv_heads * page_size * head_dim * 4 bytes), 16-byte aligned, of any
  * contents; calls that share one must not overlap.
@@ -572,9 +573,10 @@ int dqg_debug_quantized_starved(const void *q, int64_t q_stride_seq, int64_t q_s
  * logprob the logarithm of its w over that sum. A temperature of 0 (or less,
  * or NaN) takes the largest logit of lowest index, with logprob 0. NaN counts
  * as -inf; where the largest logit is +inf only such are kept; a row without
- * a logit above -inf gives token -1 and logprob NaN. The sums are taken over
- * 64-bit integers (w in units of 2^-44), so that they do not depend on an
- * order. Each parameter is an array of `rows` (temperatures, top_ks, top_ps,
+ * a logit above -inf gives token -1 and logprob NaN. A random number below 0, or
+ * NaN, counts as 0, a temperature below 1e-37 as that. The sums are taken over
+ * 64-bit integers (w in units of 2^-44, exact to about 2^-31 of itself), so that
+ * they do not depend on an order. Each parameter is an array of `rows` (temperatures, top_ks, top_ps,
  * min_ps on the device) or, where that is NULL, the value beside it.
  */
 enum { DQG_FP32 = 2 };
