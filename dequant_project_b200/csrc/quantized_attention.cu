@@ -33,7 +33,8 @@
 // Open rows go through products of their own type.
 //
 // HBM bounds the large calls: 64 sequences of 0 to 16000 positions (64 and 8
-// heads of 128, int8, 0.63 GB) take 116 us, joining included, 5.4 TB/s; 64 of
+// heads of 128, int8, 0.63 GB) take 116 us, joining included, 5.4 TB/s (127 in a
+// stream of tens of ms, where the power cap lowers the clock to 1.78 GHz); 64 of
 // 8000 (1 GB) 178 us, 5.9 TB/s, and e4m3 174 us, 6.0 TB/s. What is left between is
 // items' starts and ends and the second kernel. Short calls are latency: one
 // sequence of 2049 positions of 32 heads 12.2 us for 2.6 us of bytes. Steps that
