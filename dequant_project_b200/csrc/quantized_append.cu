@@ -218,7 +218,9 @@ __device__ __forceinline__ void store_block(const Params<E>& p, int b, const Seq
     const float largest = fmaxf(two.x, two.y), range = e4m3 ? E4m3::kMost : Int8::kMost;
     const bool tiny = largest / range < 1.17549435e-38f;
     const float scale = finite ? (tiny ? 1.17549435e-38f : largest / range) : NAN;
-    const float up = tiny ? 8.50705917e37f : range, down = tiny ? 1.f : largest, inv = 1.f / down;  // (2^126)
+    // (Large values by 2^-64 of themselves: bf16's largest times L is no number.)
+    const float less = largest > 1e30f ? 5.42101086e-20f : 1.f;
+    const float up = tiny ? 8.50705917e37f : range * less, down = tiny ? 1.f : largest * less, inv = 1.f / down;  // (2^126)
     if (page < 0) continue;
     if (threadIdx.x == 0) {
       float* to = (which ? p.pool.v_scale : p.pool.k_scale) + page * p.pool.scale_page_stride +

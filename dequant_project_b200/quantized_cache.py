@@ -84,7 +84,10 @@ def quantize_block(x: torch.Tensor, codes: torch.dtype) -> tuple:
     x = x.float()
     most = x.abs().amax((-1, -2))
     scale = torch.where(torch.isfinite(most), (most / MOST[codes]).clamp(min=LEAST_SCALE), float("nan"))
-    # (L x) / max |x|, the product exact: x / scale without the scale's rounding.
+    # (L x) / max |x|, the product exact: x / scale without the scale's rounding
+    # (large values by 2^-64 of themselves: bf16's largest times L is no number).
+    less = torch.where(most > 1e30, 2.0 ** -64, 1.0)
+    x, most = x * less[..., None, None], most * less
     tiny = (scale <= LEAST_SCALE)[..., None, None]
     y = torch.where(tiny, x * 2.0 ** 126, x * MOST[codes] / most[..., None, None])
     y = torch.where(torch.isfinite(scale)[..., None, None], y, 0.0)

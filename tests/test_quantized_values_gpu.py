@@ -109,3 +109,4 @@ def test_softmax_scales_of_any_size(cuda_device, scale):
         e = scale * 2.0 ** -18 * float(q.double().abs().sum(-1).max()) * float(k.abs().max())
         lim = u * ref.abs() + (2 * u + 2.0 ** -13 + math.expm1(2 * e)) * most + 1e-7
         assert bool(((out.double() - ref).abs() <= lim).all())
+
