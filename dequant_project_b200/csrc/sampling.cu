@@ -636,20 +636,20 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
     for (int k = 0; k < kLevels + 2; ++k) sums[k] = cluster_reduce(&sh->parts[k], ctas, u64(0), plus);
     const u64 left_out = all_at ? 0 : (sums[kLevels + 1] - room) * weight(cut);
     const double target = static_cast<double>(top_p) * static_cast<double>(sums[kLevels] - left_out);
+    // From here on the search begins: the same in all CTAs, whether their tokens
+    // are listed or not. Some room for the rounding of the logit that goes with a
+    // weight.
     float least = cut;
-    if (!listed) {
-      // Some room for the rounding of the logit that goes with a weight.
 #pragma unroll
-      for (int k = kLevels - 1; k >= 0; --k)
-        if (static_cast<double>(sums[k]) >= target)
-          least = fmaxf(cut, m - heat * (0.6931472f * 1.0001f) * (3 * k + 4) - fabsf(m) * 1e-5f);
-      if (least > cut) {
-        make_list(least);
-        // (Behind a top-k that is not the whole row's its ties would count too.)
-        if (cut == -INFINITY && draw_listed(sums[kLevels])) {
-          cluster_sync();
-          return;
-        }
+    for (int k = kLevels - 1; k >= 0; --k)
+      if (static_cast<double>(sums[k]) >= target)
+        least = fmaxf(cut, m - heat * (0.6931472f * 1.0001f) * (3 * k + 4) - fabsf(m) * 1e-5f);
+    if (least > cut) {
+      if (!listed) make_list(least);
+      // (Behind a top-k that is not the whole row's its ties would count too.)
+      if (cut == -INFINITY && draw_listed(sums[kLevels])) {
+        cluster_sync();
+        return;
       }
     }
     u64 before, inside;
