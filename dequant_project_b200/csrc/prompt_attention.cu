@@ -860,7 +860,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int k0 = (x0 + j) * kBlock;
         const float4* factors = nullptr;
         float4 ks[2] = {}, vs[2] = {};
-        if (kScaled) {
+        if (kScaled && kv > 0) {  // (a sequence without positions has no factors)
           // Keys are codes, and values but for a power of two: what is left of
           // the scales, for every sixteen positions, goes to the scores and, as
           // its logarithm, to the weights of the values.

@@ -38,3 +38,26 @@ def test_rows_without_keys_behind_values_that_are_not_numbers(cuda_device, eight
         assert bool(attend(q, ints(0, n), ints(n)).isnan().all())  # on every SM
         out = attend(q[:rows], ints(0, rows), ints(0))
         assert bool((out == 0).all())
+
+
+@pytest.mark.parametrize("fill", [0, 0x3c, 0x7e, 255])
+@pytest.mark.parametrize("hq,hkv,d", [(32, 2, 64), (16, 8, 128), (1, 1, 64)])
+def test_rows_without_keys_on_scratch_of_any_contents(cuda_device, hq, hkv, d, fill):
+    cache = qc.QuantizedCache.empty(4, hkv, 64, d, 3, block=32, device=cuda_device)
+    gen = torch.Generator(device=cuda_device).manual_seed(hq)
+    for x in cache[4:]:
+        x.copy_(torch.randn(x.shape, generator=gen, device=cuda_device))
+    q = torch.randn((8, hq, d), generator=gen, device=cuda_device).half()
+
+    def ints(*values):
+        return torch.tensor(values, dtype=torch.int32, device=cuda_device)
+
+    table = ints(0, 1, 2)[:, None]
+    for starts, lens, pages in (((0, 3, 3, 8), (0, 0, 0), 0), ((0, 3, 4, 8), (0, 1, 0), 1), ((0, 1, 4, 8), (5, 0, 7), 2)):
+        ws = qc.quantized_prompt_workspace(cache, 3, 1, pages).fill_(fill)
+        out = qc.quantized_prompt_attention(q, cache, table, ints(0, 1, 2), ints(*starts), ints(*lens), pages,
+                                            workspace=ws)
+        assert bool(out.isfinite().all())
+        for b, n in enumerate(lens):
+            if n == 0:
+                assert bool((out[starts[b]:starts[b + 1]] == 0).all())
