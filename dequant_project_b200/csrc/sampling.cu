@@ -26,9 +26,9 @@
 // the whole row's last (barriers are the largest stall: 6.8 cycles a warp's
 // instruction): 64 rows of 128256 in fp16 with all parameters 31 us (16.4 MB,
 // 2.5 us), up to 50 where the cuts fall in flat places, one row of 32000 13 us,
-// 256 rows of 32000 in fp32 33 us. Top-k alone (50) takes 18 us for the 64 rows;
-// top-p of 0.9 over normal logits (deviation 3), whose cut lies among tens of
-// thousands of tokens, 114. A row a CTA with a 64-bit exp took 412 us, clusters
+// 256 rows of 32000 in fp32 33 us. Top-k alone (50) takes 17 us for the 64 rows;
+// top-p of 0.9 over normal logits (deviation 3), whose cut lies among ten thousand
+// tokens, 72 (114 with lists of 2048 a CTA, which do not hold them). A row a CTA with a 64-bit exp took 412 us, clusters
 // 116, weights in pairs 61, short lists 42; rows kept in their own type, so that
 // half the CTAs hold one and all 64 rows run at once, 31.
 #include <cstdint>
@@ -50,7 +50,7 @@ constexpr int kWarps = kThreads / 32;
 constexpr int kMaxCtas = 8;
 constexpr int kBins = 1024;
 constexpr int kPer = kBins / kThreads;  // bins a thread
-constexpr int kListed = 2048;           // tokens that a CTA's list holds
+constexpr int kListed = 6144;           // tokens that a CTA's list holds
 constexpr int kDirect = 256;            // tokens of a row's lists that one CTA ranks
 constexpr int kLevels = 5;              // weights 2^-4, 2^-7, 2^-10, 2^-13, 2^-16
 
@@ -156,8 +156,7 @@ struct alignas(16) Shared {
   // The cluster's, of the bins that this CTA holds (every ctas-th; a CTA alone
   // has its own histogram), in turn: numbers, or 24 bits of the weights each.
   uint32_t sum[3][3][kBins / 2];
-  float list[kListed];        // logits,
-  uint16_t places[kListed];   // and their places in the CTA's part of the row
+  uint16_t list[kListed];     // places in the CTA's part of the row
   u64 scratch[kWarps];
   u64 wide[kLevels + 2][kWarps];
   u64 parts[kLevels + 2];     // of sums and of a number of ties, read by the peers
@@ -450,7 +449,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
   int round = 0;
   auto each = [&](auto f) {
     if (listed) {
-      for (int i = threadIdx.x, c = sh->listed; i < c; i += kThreads) f(sh->list[i]);
+      for (int i = threadIdx.x, c = sh->listed; i < c; i += kThreads) f(Logit<T>::load(x[sh->list[i]]));
     } else {
       each_word<T, false>(x, threadIdx.x, kThreads, n, [&](float v, int) { f(v); });
     }
@@ -470,10 +469,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
     at = __shfl_sync(0xffffffffu, at, 31) + sum - c;
     if (c && at + c <= kListed)
       each_word<T, true>(x, threadIdx.x, kThreads, slice, [&](float v, int i) {
-        if (v >= least) {
-          sh->places[at] = static_cast<uint16_t>(i);
-          sh->list[at++] = v;
-        }
+        if (v >= least) sh->list[at++] = static_cast<uint16_t>(i);
       });
     __syncthreads();
     listed = sh->listed <= kListed;
@@ -490,10 +486,11 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
     Ranks* half = reinterpret_cast<Ranks*>(all + kDirect);
     static_assert(kDirect * (sizeof(Ranked) + sizeof(Ranks)) <= sizeof(sh->own), "lists");
     for (uint32_t i = threadIdx.x; i < sh->listed; i += kThreads) {
-      const float v = sh->list[i];
+      const int place = sh->list[i];
+      const float v = Logit<T>::load(x[place]);
       const uint32_t to = map_to_rank(all + before + i, 0);
       asm volatile("st.shared::cluster.v2.b64 [%0], {%1, %2};" ::"r"(to), "l"(weight(v)),
-                   "l"(static_cast<u64>(base + sh->places[i]) << 32 | __float_as_uint(v))
+                   "l"(static_cast<u64>(base + place) << 32 | __float_as_uint(v))
                    : "memory");
     }
     cluster_sync();
@@ -682,7 +679,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
       for (int i = threadIdx.x; i < kThreads; i += kThreads) sh->own[0][i] = 0;
       __syncthreads();
       for (int i = threadIdx.x, c = sh->listed; i < c; i += kThreads)
-        if (sh->list[i] == cut) atomicAdd(&sh->own[0][sh->places[i] / q.run], 1u);
+        if (Logit<T>::load(x[sh->list[i]]) == cut) atomicAdd(&sh->own[0][sh->list[i] / q.run], 1u);
       __syncthreads();
       ties = sh->own[0][threadIdx.x];
     } else {
@@ -724,8 +721,9 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
     for (int i = threadIdx.x; i < 3 * kThreads; i += kThreads) (&sh->own[0][0])[i] = 0;
     __syncthreads();
     for (int i = threadIdx.x, c = sh->listed; i < c; i += kThreads) {
-      const u64 w = kept(sh->list[i], sh->places[i]);
-      uint32_t* run = &sh->own[0][sh->places[i] / q.run];
+      const int place = sh->list[i];
+      const u64 w = kept(Logit<T>::load(x[place]), place);
+      uint32_t* run = &sh->own[0][place / q.run];
       if (const uint32_t part = static_cast<uint32_t>(w) & 0xffffu) atomicAdd(run, part);
       if (const uint32_t part = static_cast<uint32_t>(w >> 16) & 0xffffu) atomicAdd(run + kThreads, part);
       if (const uint32_t part = static_cast<uint32_t>(w >> 32)) atomicAdd(run + 2 * kThreads, part);
