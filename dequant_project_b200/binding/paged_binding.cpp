@@ -1,6 +1,7 @@
 // Python binding of the paged-cache operators (dequant_project_b200/paged_ops.py,
-// quantized_cache.py) and of the token draw (sampling.py): tensor checks, outputs and scratch memory from torch's caching allocator, and
-// the call of the C ABI (include/dequant_b200.h) on torch's current stream. A
+// quantized_cache.py) and of the token draw (sampling.py): tensor checks,
+// outputs and scratch memory from torch's caching allocator, and the call of the
+// C ABI (include/dequant_b200.h) on torch's current stream. A
 // step of a small batch runs in a few microseconds on the GPU, and checking ten
 // tensors and packing twenty arguments in Python takes longer than that (13 us a
 // call through ctypes), so these operators are bound natively. The library's

@@ -1,5 +1,6 @@
 // extern "C" entry points of the operators over a cache held in 8 bits (declared
-// in include/dequant_b200.h): argument checks and launches. Nothing here allocates device memory, synchronises or throws.
+// in include/dequant_b200.h): argument checks and launches. Nothing here allocates
+// device memory, synchronises or throws.
 #include <cstdint>
 #include <cstring>
 #include <cuda_runtime.h>

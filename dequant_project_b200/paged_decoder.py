@@ -10,8 +10,9 @@ prompts of any lengths through every layer at once (``rope_paged_append``, then
 with the prefix that ``set_prefix`` has cached once), ``free`` returns a
 sequence's pages, ``sample`` draws the next tokens (``sample_tokens``). With
 ``codes`` the cache is held in 8 bits (``quantized_cache``: half the bytes a
-decode step reads, twice the positions in the same memory). Linear layers go through the fused GEMV up to eight rows and
-through dequantize and a matrix product above, as ``QuantLinear`` does.
+decode step reads, twice the positions in the same memory). Linear layers go
+through the fused GEMV up to eight rows and through dequantize and a matrix
+product above, as ``QuantLinear`` does.
 
 The reference models the decode step's bytes
 (KrishnaI2424/Dequant_Project ``dequant/byte_model.py:179-251``) and has no
