@@ -19,7 +19,7 @@
 // 9.4 us instead of 12.0), sixteen keys and values a thread at a time. 2048
 // positions of 32 heads of 128 (17 MB read, 34 written) take 11 us in a stream of
 // calls, 4.5 TB/s, 30000 of 8 heads 35 us, 5.3 TB/s: the writes stay in L2 at
-// first, the loads' latency bounds the short ones (12 cycles a warp's instruction).
+// first, the loads' latency bounds the short ones (7 cycles a warp's instruction).
 #include <cstdint>
 
 #include "paged_rope.cuh"

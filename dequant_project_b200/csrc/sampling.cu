@@ -23,7 +23,7 @@
 // are not searched at all, but ranked by one CTA that compares each with all.
 //
 // Neither HBM nor arithmetic bounds it, but the chain of steps that each need
-// the whole row's last (barriers are the largest stall: 6.8 cycles a warp's
+// the whole row's last (barriers are the largest stall: 5 cycles a warp's
 // instruction): 64 rows of 128256 in fp16 with all parameters 31 us (16.4 MB,
 // 2.5 us), up to 50 where the cuts fall in flat places, one row of 32000 13 us,
 // 256 rows of 32000 in fp32 33 us. Top-k alone (50) takes 17 us for the 64 rows;
