@@ -30,7 +30,8 @@
 // largest p s_v met, whatever the blocks' scales are. Both references move, and
 // the sums are rescaled, only when a slice exceeds one by more than 2^kMaxGrowth;
 // of fp16's range (2^-24 to 2^16) a weight loses below 2^-32 of the largest.
-// Open rows go through products of their own type.
+// Open rows go through products of their own type, with weights relative to their
+// own largest.
 //
 // HBM bounds the large calls: 64 sequences of 0 to 16000 positions (64 and 8
 // heads of 128, int8, 0.63 GB) take 116 us, joining included, 5.4 TB/s (127 in a
@@ -58,7 +59,7 @@ constexpr int kOpen = 48;              // open rows per tile: their keys fit the
 constexpr int kThreads = 32 * (kWarps + 1);
 constexpr int kQuerySlots = 4;         // items whose queries are held at most
 constexpr int kMergeRows = 4;          // query heads per round of the warps' merge
-constexpr float kMaxGrowth = 8.f, kHeadroom = 7.f;  // log2 units
+constexpr float kMaxGrowth = 8.f, kHeadroom = 7.f, kOpenTop = 14.f;  // log2 units
 
 struct Params : DecodeParams {
   const float* k_scale;
@@ -578,12 +579,9 @@ __global__ void __launch_bounds__(kThreads, Layout<D, NB>::kCtasPerSm)
             // Open rows, in their own type: rows of the products are the tile's.
             const uint32_t kst = ring + at, vst = kst + L::kTileBytes;
             const int rows = i.len - done - (x - whole) * kOpen - p0;  // of this warp's 16, or more
-            float sc[NB][4], f[NB][2];
+            float sc[NB][4];
 #pragma unroll
-            for (int nb = 0; nb < NB; ++nb) {
-              sc[nb][0] = sc[nb][1] = sc[nb][2] = sc[nb][3] = 0.f;
-              f[nb][0] = f[nb][1] = p.scale_log2;
-            }
+            for (int nb = 0; nb < NB; ++nb) sc[nb][0] = sc[nb][1] = sc[nb][2] = sc[nb][3] = 0.f;
 #pragma unroll
             for (int k = 0; k < D / 16; ++k) {
               const uint32_t off = (k / 4) * 128 + c * 32 + (k % 4) * 8;
@@ -599,7 +597,35 @@ __global__ void __launch_bounds__(kThreads, Layout<D, NB>::kCtasPerSm)
             for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
               for (int e = 0; e < 4; ++e) sc[nb][e] = gid + 8 * (e >> 1) < rows ? sc[nb][e] : -INFINITY;
-            weigh(sc, f, 0.f);
+            // Their weights refer to their own largest, 2^kOpenTop, and the products
+            // are added to the sums in fp32: relative to a block's weights, which have
+            // its scale in them (and int8's 2^24), fp16 would not hold them beside
+            // values thousands of times theirs. (The bias of int8 sums goes out
+            // first, so that it takes no bits of what is added.)
+            float g[NB][2], keep[NB][2];
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb) {
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                float mx = fmaxf(sc[nb][e], sc[nb][e + 2]) * p.scale_log2;
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+                mx = max3(mx, __shfl_xor_sync(0xffffffffu, mx, 16), -3.4e38f);
+                if (mx - kHeadroom - ref[nb][e] > kMaxGrowth) {
+                  l[nb][e] *= exp2_approx(ref[nb][e] - (mx - kHeadroom));
+                  ref[nb][e] = mx - kHeadroom;
+                }
+                const float own = mx - kOpenTop, to = fmaxf(ref_v[nb][e], own);
+                keep[nb][e] = exp2_approx(ref_v[nb][e] - to);
+                g[nb][e] = exp2_approx(own - to);
+                ref_v[nb][e] = to;
+#pragma unroll
+                for (int r = 0; r < 4; r += 2) {
+                  l[nb][e] += exp2_approx(fmaf(sc[nb][e + r], p.scale_log2, -ref[nb][e]));
+                  sc[nb][e + r] = exp2_approx(fmaf(sc[nb][e + r], p.scale_log2, -own));
+                }
+              }
+            }
             uint32_t pf[NB][2];
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb) {
@@ -623,7 +649,19 @@ __global__ void __launch_bounds__(kThreads, Layout<D, NB>::kCtasPerSm)
               const uint32_t v[4] = {prmt(w[0], w[1], 0x5410), prmt(w[0], w[1], 0x7632), prmt(w[2], w[3], 0x5410),
                                      prmt(w[2], w[3], 0x7632)};
 #pragma unroll
-              for (int nb = 0; nb < NB; ++nb) Elem<E>::mma(o[nb][k], v, pf[nb][0], pf[nb][1]);
+              for (int nb = 0; nb < NB; ++nb) {
+                float d[4] = {0.f, 0.f, 0.f, 0.f};
+                Elem<E>::mma(d, v, pf[nb][0], pf[nb][1]);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  const float before = o[nb][k][e] - (Pair::kInteger ? o[nb][kSums - 1][e & 1] : 0.f);
+                  o[nb][k][e] = fmaf(d[e], g[nb][e & 1], before * keep[nb][e & 1]);
+                }
+              }
+            }
+            if (Pair::kInteger) {
+#pragma unroll
+              for (int nb = 0; nb < NB; ++nb) o[nb][kSums - 1][0] = o[nb][kSums - 1][1] = 0.f;
             }
           }
           __syncwarp();

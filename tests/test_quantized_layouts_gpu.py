@@ -297,3 +297,30 @@ def test_starved_rejects_bad_arguments(cuda_device):
     for mask in (0, 256):
         with pytest.raises(RuntimeError, match="starved must be"):
             starved_call(q, cache, one[None], one, one, q, q, mask)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("codes", CODES, ids=str)
+@pytest.mark.parametrize("n,block", [(127, 32), (700, 64), (63, 64), (40, 16)])
+def test_open_rows_beside_blocks_of_large_values(cuda_device, n, block, codes, dtype):
+    """One channel's values are thousands of times the others', whose codes are
+    zero beside it: what the other channels hold in the open rows is not lost. So
+    check_attention's bound holds with a channel's own largest value (sums of zero
+    codes are exact, those of int8 codes plus 128 too once as much is taken off)."""
+    gen = torch.Generator(device=cuda_device).manual_seed(n)
+    cache, table, slots = make_cache(gen, [n], 2, 128, 64, block, codes, dtype, cuda_device)
+    cache.v.view(torch.uint8).fill_(0)
+    cache.v.view(torch.uint8)[..., 5] = 0x7f if codes == torch.int8 else 0x7e
+    cache.v_scale.fill_(60000 / qc.MOST[codes])
+    opened = cache.v_open[int(slots[0]), :, :n % block]
+    opened.copy_(1 + 0.2 * torch.randn(opened.shape, generator=gen, device=cuda_device))
+    opened[..., 5] = 60000
+    # (So many sequences, all of them this one, that no item is cut between the two.)
+    many = 400
+    q = torch.randn((many, 8, 128), generator=gen, device=cuda_device).to(dtype)
+    out = qc.quantized_attention(q, cache, table.expand(many, -1).contiguous(), slots.expand(many).contiguous(),
+                                 ints([n] * many, cuda_device))
+    k, v = (rows64(cache, w, table[0], slots[0].long(), n) for w in (0, 1))
+    ref = attend64(q, k, v, torch.full((many,), n, device=cuda_device), 1 / math.sqrt(128))
+    channel = v.abs().amax(0).repeat_interleave(4, 0).clamp(min=1.0)
+    check_attention(out.double() / channel, ref / channel, 1.0, dtype, query_rounding(q, cache, table, slots, [n]))
