@@ -203,10 +203,11 @@ __device__ __forceinline__ int64_t whole_row(const DecodeParams& p, int b, int h
 // Joins an item's pieces, R query heads a block: those that the CTAs of the
 // decode kernel left, and the shared prefix's behind them. The pieces are
 // dealt to groups of threads (several loads of each in flight), whose results
-// are joined in order.
+// are joined in order. kMeans: a piece is the mean of its values (which may be as
+// large as fp32 goes), not their sum, and counts by its weights' sum.
 constexpr int kJoinThreads = 256;
 
-template <typename E, int D, int R>
+template <typename E, int D, int R, bool kMeans>
 __global__ void __launch_bounds__(kJoinThreads)
     paged_join_kernel(const __grid_constant__ DecodeParams p) {
   constexpr int kCells = R * (D / 4), kGroups = kJoinThreads / kCells;
@@ -270,11 +271,27 @@ __global__ void __launch_bounds__(kJoinThreads)
       const float mu = mx == -INFINITY ? 0.f : mx;
       float f = exp2_approx(m - mu);
       l *= f;
+      if constexpr (kMeans) {
+        f = l;
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) {
+          pl[u] *= exp2_approx(pm[u] - mu);
+          l += pl[u];
+        }
+        const float per = l == 0.f ? 0.f : __fdividef(1.f, l);
+        f *= per;
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) pl[u] *= per;
+      }
       num.x *= f; num.y *= f; num.z *= f; num.w *= f;
 #pragma unroll
       for (int u = 0; u < kBatch; ++u) {
-        f = exp2_approx(pm[u] - mu);
-        l = fmaf(pl[u], f, l);
+        if constexpr (kMeans) {
+          f = pl[u];
+        } else {
+          f = exp2_approx(pm[u] - mu);
+          l = fmaf(pl[u], f, l);
+        }
         num.x = fmaf(v[u].x, f, num.x);
         num.y = fmaf(v[u].y, f, num.y);
         num.z = fmaf(v[u].z, f, num.z);
@@ -293,22 +310,31 @@ __global__ void __launch_bounds__(kJoinThreads)
     const float mu = m == -INFINITY ? 0.f : m;
     l = 0.f;
     num = make_float4(0.f, 0.f, 0.f, 0.f);
+    float per = 0.f;
+    if constexpr (kMeans) {
+#pragma unroll
+      for (int k = 0; k < kGroups; ++k) l = fmaf(s_ml[k][cell].y, exp2_approx(s_ml[k][cell].x - mu), l);
+      per = l == 0.f ? 0.f : __fdividef(1.f, l);
+    }
 #pragma unroll
     for (int k = 0; k < kGroups; ++k) {
-      const float f = exp2_approx(s_ml[k][cell].x - mu);
+      float f = exp2_approx(s_ml[k][cell].x - mu);
       const float4 v = s_num[k][cell];
-      l = fmaf(s_ml[k][cell].y, f, l);
+      if constexpr (kMeans)
+        f *= s_ml[k][cell].y * per;
+      else
+        l = fmaf(s_ml[k][cell].y, f, l);
       num.x = fmaf(v.x, f, num.x);
       num.y = fmaf(v.y, f, num.y);
       num.z = fmaf(v.z, f, num.z);
       num.w = fmaf(v.w, f, num.w);
     }
   }
-  if (row < rows) store4<E, D>(p, d.b, kvh * p.g + rb * 16 + row, d4, l, num);
+  if (row < rows) store4<E, D>(p, d.b, kvh * p.g + rb * 16 + row, d4, kMeans ? 1.f : l, num);
 }
 
 // Launches it behind the first kernel (cfg: that one's stream and attributes).
-template <typename E, int D>
+template <typename E, int D, bool kMeans = false>
 cudaError_t launch_join(const DecodeParams& p, cudaLaunchConfig_t cfg) {
   // Query heads a join block takes: few, so that the pieces of a small batch
   // spread over many threads, but one where there is one.
@@ -318,8 +344,8 @@ cudaError_t launch_join(const DecodeParams& p, cudaLaunchConfig_t cfg) {
   cfg.gridDim = dim3(static_cast<unsigned>(items), (rows + per - 1) / per);
   cfg.blockDim = dim3(kJoinThreads);
   cfg.dynamicSmemBytes = 0;
-  return per == 1 ? cudaLaunchKernelEx(&cfg, paged_join_kernel<E, D, 1>, p)
-                  : cudaLaunchKernelEx(&cfg, paged_join_kernel<E, D, 4>, p);
+  return per == 1 ? cudaLaunchKernelEx(&cfg, paged_join_kernel<E, D, 1, kMeans>, p)
+                  : cudaLaunchKernelEx(&cfg, paged_join_kernel<E, D, 4, kMeans>, p);
 }
 
 }  // namespace

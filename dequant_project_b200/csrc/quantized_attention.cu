@@ -59,7 +59,8 @@ constexpr int kOpen = 48;              // open rows per tile: their keys fit the
 constexpr int kThreads = 32 * (kWarps + 1);
 constexpr int kQuerySlots = 4;         // items whose queries are held at most
 constexpr int kMergeRows = 4;          // query heads per round of the warps' merge
-constexpr float kMaxGrowth = 8.f, kHeadroom = 7.f, kOpenTop = 14.f;  // log2 units
+constexpr float kMaxGrowth = 8.f, kHeadroom = 7.f;  // log2 units
+constexpr float kOpenTop = 14.f;  // of fp16 open rows' weights, the largest
 
 struct Params : DecodeParams {
   const float* k_scale;
@@ -597,11 +598,34 @@ __global__ void __launch_bounds__(kThreads, Layout<D, NB>::kCtasPerSm)
             for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
               for (int e = 0; e < 4; ++e) sc[nb][e] = gid + 8 * (e >> 1) < rows ? sc[nb][e] : -INFINITY;
-            // Their weights refer to their own largest, 2^kOpenTop, and the products
-            // are added to the sums in fp32: relative to a block's weights, which have
-            // its scale in them (and int8's 2^24), fp16 would not hold them beside
-            // values thousands of times theirs. (The bias of int8 sums goes out
-            // first, so that it takes no bits of what is added.)
+            // Their weights refer to their own largest, and the products are added to
+            // the sums in fp32: relative to a block's weights, which have its scale in
+            // them (and int8's 2^24), fp16 would not hold them beside values thousands
+            // of times theirs. (The bias of int8 sums goes out first, so that it takes
+            // no bits of what is added.)
+            auto value_pair = [&](int k, int r) {
+              // What lies behind the last row may be anything: a zero weight
+              // times an infinity would not be zero.
+              const int row = 2 * c + (r & 1) + (r & 2 ? 8 : 0);
+              uint32_t w = 0;
+              if (row < rows)
+                asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w) : "r"(vst + (p0 + row) * (D * 2) + gid * (D / 4) + k * 4));
+              return w;
+            };
+            float top = kOpenTop;
+            if constexpr (Elem<E>::kFormat == 1) {
+              // bf16: 2^64 over the largest value's power of two, so that sums of
+              // values of any size are fp32 numbers (and weights normal ones).
+              uint32_t most = 0;
+#pragma unroll
+              for (int k = 0; k < D / 16; ++k)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) most = __vmaxu2(most, value_pair(k, r) & 0x7fff7fffu);
+#pragma unroll
+              for (int off = 16; off >= 1; off >>= 1) most = __vmaxu2(most, __shfl_xor_sync(0xffffffffu, most, off));
+              most = max(most & 0xffffu, most >> 16);
+              top = static_cast<float>(min(64 + 127 - static_cast<int>(most >> 7), 120));
+            }
             float g[NB][2], keep[NB][2];
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb) {
@@ -615,7 +639,7 @@ __global__ void __launch_bounds__(kThreads, Layout<D, NB>::kCtasPerSm)
                   l[nb][e] *= exp2_approx(ref[nb][e] - (mx - kHeadroom));
                   ref[nb][e] = mx - kHeadroom;
                 }
-                const float own = mx - kOpenTop, to = fmaxf(ref_v[nb][e], own);
+                const float own = mx - top, to = fmaxf(ref_v[nb][e], own);
                 keep[nb][e] = exp2_approx(ref_v[nb][e] - to);
                 g[nb][e] = exp2_approx(own - to);
                 ref_v[nb][e] = to;
@@ -634,18 +658,7 @@ __global__ void __launch_bounds__(kThreads, Layout<D, NB>::kCtasPerSm)
             }
 #pragma unroll
             for (int k = 0; k < D / 16; ++k) {
-              uint32_t w[4];
-#pragma unroll
-              for (int r = 0; r < 4; ++r) {
-                // What lies behind the last row may be anything: a zero weight
-                // times an infinity would not be zero.
-                const int row = 2 * c + (r & 1) + (r & 2 ? 8 : 0);
-                w[r] = 0;
-                if (row < rows)
-                  asm volatile("ld.shared.b32 %0, [%1];"
-                               : "=r"(w[r])
-                               : "r"(vst + (p0 + row) * (D * 2) + gid * (D / 4) + k * 4));
-              }
+              const uint32_t w[4] = {value_pair(k, 0), value_pair(k, 1), value_pair(k, 2), value_pair(k, 3)};
               const uint32_t v[4] = {prmt(w[0], w[1], 0x5410), prmt(w[0], w[1], 0x7632), prmt(w[2], w[3], 0x5410),
                                      prmt(w[2], w[3], 0x7632)};
 #pragma unroll
@@ -715,18 +728,26 @@ __global__ void __launch_bounds__(kThreads, Layout<D, NB>::kCtasPerSm)
       const bool all = i.x0 == 0 && i.x1 == i.tiles;
       const int64_t row0 = (2 * static_cast<int64_t>(blockIdx.x) + (i.x0 > 0 ? 0 : 1)) * p.rows;
       if (threadIdx.x < i.rows) {
-        // A head's maximum, its sum, and what each warp's part is multiplied by.
+        // A head's maximum, its sum, what each warp's part is multiplied by, and
+        // what their sum is, to be the mean of the values: the sum's reciprocal and
+        // the power of two between the references, in two halves since all of it
+        // may be no fp32 number (a scale is up to 2^121).
         const int row = threadIdx.x;
-        float mx = -INFINITY, den = 0.f;
+        float mx = -INFINITY, mv = -INFINITY, den = 0.f;
 #pragma unroll
-        for (int w = 0; w < kWarps; ++w) mx = fmaxf(mx, ms[w * 16 + row]);
-        const float mu = mx == -INFINITY ? 0.f : mx;
+        for (int w = 0; w < kWarps; ++w) {
+          mx = fmaxf(mx, ms[w * 16 + row]);
+          mv = fmaxf(mv, vs[w * 16 + row]);
+        }
+        const float mu = mx == -INFINITY ? 0.f : mx, nu = mv == -INFINITY ? mu : mv;
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) {
           den = fmaf(ls[w * 16 + row], exp2_approx(ms[w * 16 + row] - mu), den);
-          vs[w * 16 + row] = exp2_approx(vs[w * 16 + row] - mu);
+          vs[w * 16 + row] = exp2_approx(vs[w * 16 + row] - nu);
         }
-        ls[row] = den;
+        const float half = exp2_approx(0.5f * (nu - mu));
+        ls[row] = den == 0.f ? 0.f : half * __frcp_rn(den);
+        ms[row] = half;
         if (!all) {
           p.m[row0 + row] = mx;
           p.l[row0 + row] = den;
@@ -768,8 +789,10 @@ __global__ void __launch_bounds__(kThreads, Layout<D, NB>::kCtasPerSm)
               num.z = fmaf(v.z, f, num.z);
               num.w = fmaf(v.w, f, num.w);
             }
+            const float f = ls[row], half = ms[row];
+            num = make_float4(num.x * f * half, num.y * f * half, num.z * f * half, num.w * f * half);
             if (all)
-              store4<E, D>(p, s.b, i.head0 + row, d4, ls[row], num);
+              store4<E, D>(p, s.b, i.head0 + row, d4, 1.f, num);
             else
               *reinterpret_cast<float4*>(p.part + (row0 + row) * D + d4 * 4) = num;
           }
@@ -808,7 +831,7 @@ cudaError_t launch(Params p, const CUtensorMap& kmap, const CUtensorMap& vmap, i
   cfg.numAttrs = 1;
   e = cudaLaunchKernelEx(&cfg, quantized_decode_kernel<E, Code, D, NB>, p, kmap, vmap);
   if (e != cudaSuccess) return e;
-  return launch_join<E, D>(p, cfg);
+  return launch_join<E, D, true>(p, cfg);
 }
 
 template <typename E, class Code>

@@ -61,3 +61,60 @@ def test_kernel(cuda_device, codes):
     qc.rope_quantized_append(qkv, cos, sin, at, cache, table, ints(range(n)),
                              ints(range(0, 16 * n + 1, 16)), ints([16] * n), 1)
     check_large(cache.v[:, 0], cache.v_scale[:, 0, 0], x)
+
+
+def appended(device, n, g, page, block, most, codes, d=64, hkv=2):
+    """A bf16 sequence of n positions whose values are up to ``most``, appended:
+    the queries, the cache and what goes with it, and its 64-bit keys and values."""
+    from test_quantized_cache_gpu import ints, rows64
+
+    gen = torch.Generator(device=device).manual_seed(n)
+    cache = qc.QuantizedCache.empty(-(-n // page), hkv, page, d, 1, block=block, codes=codes, dtype=torch.bfloat16,
+                                    device=device)
+    qkv = torch.randn((n, (g + 2) * hkv * d), generator=gen, device=device)
+    qkv[:, -hkv * d:].uniform_(-1, 1, generator=gen).mul_(most)
+    qkv[n // 2, -hkv * d:] = -most
+    cos, sin = torch.ones((1, d // 2), device=device), torch.zeros((1, d // 2), device=device)
+    table = torch.randperm(-(-n // page), generator=gen, device=device).int()[None]
+    slot = ints([0], device)
+    q = qc.rope_quantized_append(qkv.bfloat16(), cos, sin, torch.zeros(n, dtype=torch.int64, device=device), cache,
+                                 table, slot, ints([0, n], device), ints([n], device), g * hkv)
+    return q, cache, table, slot, *(rows64(cache, w, table[0], 0, n) for w in (0, 1))
+
+
+SIZES = [(37, 1, 16, 16), (9, 4, 64, 64), (64, 8, 64, 64), (3000, 12, 128, 32)]  # n, heads a KV head, page, block
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("codes", CODES, ids=str)
+@pytest.mark.parametrize("most", LARGE + [1e34, 1e-30])
+@pytest.mark.parametrize("n,g,page,block", SIZES)
+def test_decode_over_large_values(cuda_device, n, g, page, block, most, codes):
+    """|out - ref| <= u |ref| + (u + 2^-13) max|v| as for ordinary values (and, for
+    queries beside int8 codes, what 2^-16 of their largest moves), for a sequence
+    cut into pieces and for many that are not."""
+    from test_quantized_cache_gpu import attend64, check_attention, ints, query_rounding
+
+    q, cache, table, slot, k, v = appended(cuda_device, n, g, page, block, most, codes)
+    unit = float(v.abs().max())
+    for rows in (1, min(n, 400)):
+        last = q[-rows:].contiguous()
+        out = qc.quantized_attention(last, cache, table.expand(rows, -1).contiguous(), slot.expand(rows).contiguous(),
+                                     ints([n] * rows, cuda_device))
+        ref = attend64(last, k, v, torch.full((rows,), n, device=cuda_device), 0.125)
+        check_attention(out.double() / unit, ref / unit, 1.0, torch.bfloat16,
+                        query_rounding(last, cache, table, slot, [n]))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("codes", CODES, ids=str)
+def test_values_of_zero_scales_and_low_scores(cuda_device, codes):
+    """Blocks whose values' scales are zero read as zeros, whatever the scores are."""
+    from test_quantized_cache_gpu import ints
+
+    q, cache, table, slot, _, _ = appended(cuda_device, 64, 2, 16, 16, 1.0, codes)
+    cache.v_scale.zero_()
+    cache.k_scale.fill_(1.0)
+    cache.k.view(torch.uint8).fill_(0x81 if codes == torch.int8 else 0xfe)  # the most negative
+    out = qc.quantized_attention(torch.full_like(q[:1], 100.0), cache, table, slot, ints([64], cuda_device))
+    assert bool((out == 0).all())
