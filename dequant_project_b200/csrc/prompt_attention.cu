@@ -75,7 +75,11 @@ constexpr int kMmaWarp = 8, kCopyWarp = 9, kValueWarp = 10, kValueWarps = 2;
 // exceeds by kMaxGrowth at most (log2 units): 2^15 at most, so that of fp16's
 // range (2^-24 to 2^16) what lies above 1 is used too, and what a weight loses at
 // the lower end is below 2^-32 of the largest one.
-constexpr float kMaxGrowth = 8.f, kHeadroom = 7.f;
+constexpr float kMaxGrowth = 8.f;
+// (Over an 8-bit cache's bf16 values, which reach that type's largest, weights are
+// 2^-12 at most, so that sums stay finite: bf16 has the exponents for it.)
+template <typename E, bool kScaled>
+constexpr float kHeadroom = kScaled && Elem<E>::kFormat == 1 ? -20.f : 7.f;
 constexpr int kEarly = 96;          // keys whose weights are handed over first
 // An item's start and end, in keys' time: 8192 tokens, 64/8 heads of 128, 1061 us
 // with 128, 991 with 256, 981 with 512; 2048 tokens, 32 heads of 128, 57.1, 54.5,
@@ -943,7 +947,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           l *= f;
           if (grow) m = m_new;
         }
-        const float ref = m == -INFINITY ? 0.f : fmaf(m, p.scale_log2, -kHeadroom);
+        const float ref = m == -INFINITY ? 0.f : fmaf(m, p.scale_log2, -kHeadroom<E, kScaled>);
         const float2 ref2 = make_float2(-ref, -ref);
         float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
         float4 inv[2] = {};
@@ -1045,7 +1049,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         } else {
           const int64_t slot = g.slot;
-          p.ml[slot * 512 + t * 128 + r] = n > 0 && m != -INFINITY ? fmaf(m, p.scale_log2, -kHeadroom) : -INFINITY;
+          p.ml[slot * 512 + t * 128 + r] = n > 0 && m != -INFINITY ? fmaf(m, p.scale_log2, -kHeadroom<E, kScaled>) : -INFINITY;
           p.ml[slot * 512 + 256 + t * 128 + r] = l;
 #pragma unroll
           for (int q = 0; q < D / 32; ++q) {

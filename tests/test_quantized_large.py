@@ -118,3 +118,20 @@ def test_values_of_zero_scales_and_low_scores(cuda_device, codes):
     cache.k.view(torch.uint8).fill_(0x81 if codes == torch.int8 else 0xfe)  # the most negative
     out = qc.quantized_attention(torch.full_like(q[:1], 100.0), cache, table, slot, ints([64], cuda_device))
     assert bool((out == 0).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("codes", CODES, ids=str)
+@pytest.mark.parametrize("most", LARGE + [1e34, 1e-30])
+@pytest.mark.parametrize("n,g,page,block", SIZES)
+def test_prompts_over_large_values(cuda_device, n, g, page, block, most, codes):
+    """|out - ref| <= u |ref| + (u + 2^-13) max|v|, as for ordinary values."""
+    from test_quantized_cache_gpu import attend64, check_attention, ints
+
+    q, cache, table, slot, k, v = appended(cuda_device, n, g, page, block, most, codes)
+    unit, rows = float(v.abs().max()), min(n, 200)
+    ends = n - rows + 1 + torch.arange(rows, device=cuda_device)
+    last = q[-rows:].contiguous()
+    out = qc.quantized_prompt_attention(last, cache, table, slot, ints([0, rows], cuda_device), ints([n], cuda_device),
+                                        -(-n // page))
+    check_attention(out.double() / unit, attend64(last, k, v, ends, 0.125) / unit, 1.0, torch.bfloat16)
