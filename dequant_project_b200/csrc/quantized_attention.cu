@@ -122,11 +122,13 @@ __device__ __forceinline__ void cp_async_arrive(uint64_t* bar) {
 // integer instructions a pair; the bias goes out of the sums again (a product
 // more per slice sums 128 p). Bytes put into the fraction of 1024 and made small
 // again by an addition took 64 more instructions of about 430 a slice.
-// Keys: e4m3 the same way. int8 codes enter integer products as they are; the
-// queries are rounded to 2^-16 of their head's largest, in two int8 digits, which
-// takes all instructions but the products away. (2049 positions, fp16: outputs
-// are 2.2e-4 off, 2.1e-4 of it by their own rounding, as beside e4m3; 2.4e-4, at
-// worst 3.6e-4, with digits of seven bits.)
+// Keys: e4m3 the same way. int8 codes enter integer products as they are, beside
+// the queries as integers of 23 bits, relative to their head's largest, in three int8
+// digits: what that loses is below 2^-24 of the largest, so that a channel far above
+// the others takes nothing that matters from them. (Two digits, 2^-17, took 1 to 2 %
+// less time, and a channel of 4000 made outputs 0.04 of a value off. Codes as fp16
+// numbers, as the values, beside the queries' own took 9 % more: 64 sequences of 8000
+// 195 us instead of 180 in a graph.)
 template <class Code>
 struct Pairs;
 template <>
@@ -158,6 +160,7 @@ __device__ __forceinline__ void mma_s8(int* d, uint32_t a0, uint32_t a1, uint32_
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 constexpr int kIntZero = 0x4b400000;  // 1.5 * 2^23
+constexpr float kDigitMost = 4161407.f;  // 63, 127, 127 in digits of eight bits
 __device__ __forceinline__ float int_sum(int bits) { return __int_as_float(bits) - 12582912.f; }
 
 // Row of a tile that row n of a product takes: conflict-free reads of sixteen
@@ -328,6 +331,7 @@ __global__ void __launch_bounds__(kThreads, Layout<D, NB>::kCtasPerSm)
   } else {
     using Pair = Pairs<Code>;
     constexpr int kSums = D / 16 + (Pair::kInteger ? 1 : 0);  // products a slice; the last one sums the bias
+    constexpr int kDigits = Pair::kInteger ? 3 : 2;  // words of queries a product takes
     const int gid = lane >> 2, c = lane & 3;
     const uint32_t ring = smem_u32(smem);
     const int p0 = warp * 16;
@@ -356,7 +360,7 @@ __global__ void __launch_bounds__(kThreads, Layout<D, NB>::kCtasPerSm)
       await(q_full + qi, (item / q_slots) & 1);
       // Queries as B fragments: columns are heads; a lane holds the values at
       // 64 h + 16 c to + 15, four a product (fp16) or eight (digits).
-      uint32_t qf[NB][D / 16][2];  // digits: [word][high, low]
+      uint32_t qf[NB][D / 16][kDigits];  // digits: [word][high, middle, low]
       float unit[NB][2];           // what scores of heads 2 c and 2 c + 1 are multiplied by, but for the block's scale
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb) {
@@ -378,22 +382,22 @@ __global__ void __launch_bounds__(kThreads, Layout<D, NB>::kCtasPerSm)
         most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
         float f = p.scale_log2;
         if constexpr (Pair::kInteger) {
-          // (A largest value that is not finite makes the head's unit so.)
-          const float largest = Elem<E>::unpack(most).x, up = fminf(32639.f / largest, 1e38f);
-          f *= largest > 1e-30f ? largest / 32639.f : (largest == largest ? 1e-38f : NAN);
+          // Digits by a sum with 1.5 * 2^23, whose last bits are the integer, and with
+          // 128 in each digit's place, which makes all three positive bytes. (A
+          // largest value that is not finite makes the head's unit so.)
+          const float largest = Elem<E>::unpack(most).x, up = fminf(kDigitMost / largest, 1e38f);
+          f *= up < 1e38f ? largest / kDigitMost : (largest == largest ? 1e-38f : NAN);
 #pragma unroll
           for (int k = 0; k < D / 16; ++k) {
             const float2 x = Elem<E>::unpack(w[2 * k]), y = Elem<E>::unpack(w[2 * k + 1]);
             const float v[4] = {x.x, x.y, y.x, y.y};
-            int high[4], low[4];
+            uint32_t n[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const int n = __float2int_rn(v[e] * up);
-              high[e] = (n + 128) >> 8;
-              low[e] = n - high[e] * 256;
-            }
-            qf[nb][k][0] = prmt(prmt(high[0], high[1], 0x0040), prmt(high[2], high[3], 0x0040), 0x5410);
-            qf[nb][k][1] = prmt(prmt(low[0], low[1], 0x0040), prmt(low[2], low[3], 0x0040), 0x5410);
+            for (int e = 0; e < 4; ++e) n[e] = __float_as_uint(fmaf(v[e], up, 12582912.f)) + (0x808080u - kIntZero);
+            const uint32_t a = prmt(n[0], n[1], 0x5140), b = prmt(n[2], n[3], 0x5140);
+            qf[nb][k][0] = prmt(prmt(n[0], n[1], 0x0062), prmt(n[2], n[3], 0x0062), 0x5410) ^ 0x80808080u;
+            qf[nb][k][1] = prmt(a, b, 0x7632) ^ 0x80808080u;
+            qf[nb][k][kDigits - 1] = prmt(a, b, 0x5410) ^ 0x80808080u;
           }
         } else {
           if (Elem<E>::kFormat == 1) {
@@ -491,7 +495,7 @@ __global__ void __launch_bounds__(kThreads, Layout<D, NB>::kCtasPerSm)
               const float2 both = *reinterpret_cast<const float2*>(scales + (stage * kWarps + warp) * 2);
               const float ks = both.x, lv = log2_approx(both.y) + Pair::kUnit;
               float sc[NB][4], f[NB][2];
-              int sums[NB][2][4];
+              int sums[NB][3][4];
 #pragma unroll
               for (int nb = 0; nb < NB; ++nb) {
                 f[nb][0] = unit[nb][0] * ks;
@@ -499,7 +503,8 @@ __global__ void __launch_bounds__(kThreads, Layout<D, NB>::kCtasPerSm)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                   sc[nb][e] = 0.f;
-                  sums[nb][0][e] = sums[nb][1][e] = kIntZero;
+                  sums[nb][0][e] = kIntZero;
+                  sums[nb][1][e] = sums[nb][2][e] = 0;
                 }
               }
 #pragma unroll
@@ -512,7 +517,7 @@ __global__ void __launch_bounds__(kThreads, Layout<D, NB>::kCtasPerSm)
 #pragma unroll
                     for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-                      for (int e = 0; e < 2; ++e)
+                      for (int e = 0; e < kDigits; ++e)
                         mma_s8(sums[nb][e], aw[k], bw[k], aw[k + 1], bw[k + 1], qf[nb][4 * h + k][e],
                                qf[nb][4 * h + k + 1][e]);
                 } else {
@@ -532,29 +537,36 @@ __global__ void __launch_bounds__(kThreads, Layout<D, NB>::kCtasPerSm)
                 for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
                   for (int e = 0; e < 4; ++e)
-                    sc[nb][e] = fmaf(int_sum(sums[nb][0][e]), 256.f, int_sum(sums[nb][1][e]));
+                    sc[nb][e] = fmaf(int_sum(sums[nb][0][e]), 65536.f, __int2float_rn(sums[nb][1][e] * 256 + sums[nb][2][e]));
               }
               // A lane's D / 8 values of four rows: a word of each gives two
               // products' halves.
               constexpr uint32_t kLow = Pair::kStride == 2 ? 0x5410 : 0x5140;
               constexpr uint32_t kHigh = Pair::kStride == 2 ? 0x7632 : 0x7362;
               uint32_t vw[4][D / 32];
+              auto load_values = [&] {
 #pragma unroll
-              for (int r = 0; r < 4; ++r) {
-                const uint32_t from = v_at[r & 1] + at;
-                if (D == 128) {
-                  const uint4 v = r & 2 ? lds128<8 * D>(from) : lds128(from);
-                  vw[r][0] = v.x;
-                  vw[r][1] = v.y;
-                  vw[r][2 % (D / 32)] = v.z;
-                  vw[r][3 % (D / 32)] = v.w;
-                } else {
-                  const uint2 v = r & 2 ? lds64<8 * D>(from) : lds64(from);
-                  vw[r][0] = v.x;
-                  vw[r][1] = v.y;
+                for (int r = 0; r < 4; ++r) {
+                  const uint32_t from = v_at[r & 1] + at;
+                  if (D == 128) {
+                    const uint4 v = r & 2 ? lds128<8 * D>(from) : lds128(from);
+                    vw[r][0] = v.x;
+                    vw[r][1] = v.y;
+                    vw[r][2 % (D / 32)] = v.z;
+                    vw[r][3 % (D / 32)] = v.w;
+                  } else {
+                    const uint2 v = r & 2 ? lds64<8 * D>(from) : lds64(from);
+                    vw[r][0] = v.x;
+                    vw[r][1] = v.y;
+                  }
                 }
-              }
+              };
+              // (Ahead of the weights where there are registers for it: with three
+              // digits of queries and 128 registers 64 sequences took 2 % longer.)
+              constexpr bool kLate = Pair::kInteger && NB == 1;
+              if (!kLate) load_values();
               weigh(sc, f, lv);
+              if (kLate) load_values();
               uint32_t pf[NB][2];
 #pragma unroll
               for (int nb = 0; nb < NB; ++nb) {
@@ -700,7 +712,7 @@ __global__ void __launch_bounds__(kThreads, Layout<D, NB>::kCtasPerSm)
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-          for (int k = 0; k < D / 16; ++k) x ^= qf[nb][k][0] ^ qf[nb][k][1];
+          for (int k = 0; k < D / 16; ++k) for (int t = 0; t < kDigits; ++t) x ^= qf[nb][k][t];
         asm volatile("" ::"r"(x) : "memory");
       }
       __syncwarp();

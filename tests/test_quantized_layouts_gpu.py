@@ -324,3 +324,28 @@ def test_open_rows_beside_blocks_of_large_values(cuda_device, n, block, codes, d
     ref = attend64(q, k, v, torch.full((many,), n, device=cuda_device), 1 / math.sqrt(128))
     channel = v.abs().amax(0).repeat_interleave(4, 0).clamp(min=1.0)
     check_attention(out.double() / channel, ref / channel, 1.0, dtype, query_rounding(q, cache, table, slots, [n]))
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("codes", CODES, ids=str)
+@pytest.mark.parametrize("d,g", [(128, 4), (64, 12)])
+def test_a_query_channel_far_above_the_others(cuda_device, d, g, codes, dtype):
+    """Queries with one value of 4000 among ordinary ones, over keys of zero
+    there: nothing of the other channels is lost. Scores are fp32 sums of products
+    with code + 128 at most, some ten in a row: e = scale s 2^-21 sum |q| (|code| +
+    128)."""
+    gen = torch.Generator(device=cuda_device).manual_seed(d)
+    kl, hkv = [48, 63, 16, 7], 2
+    cache, table, slots = make_cache(gen, kl, hkv, d, 16, 16, codes, dtype, cuda_device, spread=0.0)
+    cache.k.view(torch.uint8)[..., 9] = 0
+    cache.k_open[..., 9] = 0
+    q = torch.randn((4, g * hkv, d), generator=gen, device=cuda_device).to(dtype)
+    q[..., 9] = 4000
+    out = qc.quantized_attention(q, cache, table, slots, ints(kl, cuda_device))
+    ref = reference(q, cache, table, slots, kl, 1 / math.sqrt(d))
+    most = 128 + qc.MOST[codes]
+    step = float(cache.k_scale[table[0, 0].long()].max())
+    e = 2.0 ** -21 * step * float(q.float().abs().sum(-1).max()) * most / math.sqrt(d)
+    for b in range(4):
+        one = table[b:b + 1], slots[b:b + 1], kl[b:b + 1]
+        check_attention(out[b:b + 1], ref[b:b + 1], largest_value(cache, *one), dtype, e)
