@@ -402,7 +402,7 @@ __global__ void __launch_bounds__(kThreads, Layout<D, NB>::kCtasPerSm)
         } else {
           if (Elem<E>::kFormat == 1) {
             // bf16 to fp16, times a power of two for the head.
-            const int e = min(max(static_cast<int>(most >> 7), 20), 240);  // exponent of the largest, biased
+            const int e = min(max(static_cast<int>(most >> 7), 15), 254);  // exponent of the largest, biased
             const float up = __uint_as_float(static_cast<uint32_t>(127 + 14 + 127 - e) << 23);  // 2^(14 - (e - 127))
 #pragma unroll
             for (int h = 0; h < D / 8; ++h) {

@@ -349,3 +349,24 @@ def test_a_query_channel_far_above_the_others(cuda_device, d, g, codes, dtype):
     for b in range(4):
         one = table[b:b + 1], slots[b:b + 1], kl[b:b + 1]
         check_attention(out[b:b + 1], ref[b:b + 1], largest_value(cache, *one), dtype, e)
+
+
+@pytest.mark.parametrize("power", [-110, -60, 60, 110, 118, 123])
+@pytest.mark.parametrize("codes", CODES, ids=str)
+def test_queries_of_any_size(cuda_device, codes, power):
+    """bf16 queries times a power of two over keys (of blocks and open rows) by
+    its inverse: the same scores, and the same result but for fp32 roundings."""
+    gen = torch.Generator(device=cuda_device).manual_seed(3)
+    kl, d = [600, 45, 7], 128
+    cache, table, slots = make_cache(gen, kl, 2, d, 32, 16, codes, torch.bfloat16, cuda_device)
+    lens, q = ints(kl, cuda_device), torch.randn((3, 8, d), generator=gen, device=cuda_device).bfloat16()
+    q[0, 1, 3] = q[1, 5, 100] = 13.0
+    c = clone(cache)
+    c.k_scale.mul_(2.0 ** -power)
+    c.k_open.mul_(2.0 ** -power)
+    out = qc.quantized_attention(q * 2.0 ** power, c, table, slots, lens)
+    ref = reference(q, cache, table, slots, kl, 1 / math.sqrt(d))
+    for b in range(3):
+        one = table[b:b + 1], slots[b:b + 1], kl[b:b + 1]
+        check_attention(out[b:b + 1], ref[b:b + 1], largest_value(cache, *one), torch.bfloat16,
+                        query_rounding(q[b:b + 1], cache, *one))
