@@ -360,8 +360,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
   const float heat = p.temperatures ? __ldg(p.temperatures + row) : p.temperature;
   const int top_k = p.top_ks ? __ldg(p.top_ks + row) : p.top_k;
   const float top_p = p.top_ps ? __ldg(p.top_ps + row) : p.top_p;
-  float min_p = p.min_ps ? __ldg(p.min_ps + row) : p.min_p;
-  min_p = min_p > 0.f ? fminf(min_p, 1.f) : 0.f;
+  const float min_p = p.min_ps ? __ldg(p.min_ps + row) : p.min_p;
 
   // The row's part into shared memory; NaN becomes -inf.
   float largest;
@@ -405,7 +404,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
     cluster_sync();  // no CTA leaves while a peer reads from it
     return;
   }
-  if (!(heat > 0.f)) {
+  if (!(heat > 0.f) || min_p > 1.f) {  // (no w is above one: the first token alone is kept)
     uint32_t at = 0xffffffffu;
     for (int j = q.run - 1; j >= 0; --j)
       if (Logit<T>::load(x[first + j]) == m) at = base + first + j;

@@ -568,7 +568,7 @@ int dqg_debug_quantized_starved(const void *q, int64_t q_stride_seq, int64_t q_s
  * exp((l_i - m) / T); tokens rank by logit, the lower index first. Kept are
  * those of rank below top_k (0 or less: all), with min_p <= w_i, and with the
  * w of those that top_k keeps and that rank before them below top_p of top_k's
- * sum (1 or more: all). The token is the first, by index, whose running sum of
+ * sum (1 or more: all); and always the first. The token is the first, by index, whose running sum of
  * kept w exceeds uniform * their sum (the last kept one if none does), and
  * logprob the logarithm of its w over that sum. A temperature of 0 (or less,
  * or NaN) takes the largest logit of lowest index, with logprob 0. NaN counts

@@ -185,3 +185,20 @@ def test_refusals(cuda_device):
             sample_tokens(*args, **params)
     tokens, logprobs = sample_tokens(x[:0], u[:0])
     assert tokens.shape == (0,) and logprobs.shape == (0,)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+def test_min_p_above_one_keeps_the_first_of_equal_logits(cuda_device, dtype):
+    logits = torch.zeros((5, 3000), dtype=dtype, device=cuda_device)
+    logits[1, 70:] = 2.0
+    logits[2, [5, 2999]] = float("inf")
+    logits[3] = float("nan")
+    logits[4, 2000:] = -1.0
+    for u in (0.0, 0.5, 0.99):
+        uniform = torch.full((5,), u, device=cuda_device)
+        for params in (dict(min_p=5.0), dict(min_p=1.0 + 2.0 ** -23, temperature=0.7), dict(min_p=2.0, top_k=100),
+                       dict(min_p=float("inf"), top_p=0.5)):
+            assert compare(logits, uniform, **params).tolist() == [0, 70, 5, -1, 0]
+        assert compare(logits, uniform, min_p=1.0)[4] == int(u * 2000)
+    each = torch.tensor([5.0, 1.0, 0.5, 2.0, 3.0], device=cuda_device)
+    assert compare(logits, torch.full((5,), 0.99, device=cuda_device), min_p=each)[0] == 0
