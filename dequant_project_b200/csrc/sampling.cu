@@ -388,10 +388,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
     }
   }
   float m = block_reduce(largest, sh->scratch, [](float a, float b) { return fmaxf(a, b); });
-  if (threadIdx.x == 0) {
-    sh->largest = m;
-    sh->listed = 0;
-  }
+  if (threadIdx.x == 0) sh->largest = m;
   cluster_sync();
   m = cluster_reduce(&sh->largest, ctas, -INFINITY, [](float a, float b) { return fmaxf(a, b); });
 
@@ -454,7 +451,11 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
     }
   };
   // Lists this CTA's tokens from `least` on; a list that they do not fit is not used.
+  // (A second list is made where they did not fit the first; the peers have read its
+  // length by the cluster's barrier between.)
   auto make_list = [&](float least) {
+    if (threadIdx.x == 0) sh->listed = 0;
+    __syncthreads();
     // (Counted first, so that a warp takes its places in the list at once.)
     uint32_t c = 0;
     each_word<T, true>(x, threadIdx.x, kThreads, slice, [&](float v, int) { c += v >= least; });

@@ -38,3 +38,22 @@ def test_candidates_in_one_part_of_the_row(cuda_device, skew):
     for params in (dict(top_p=0.3), dict(top_p=0.9, temperature=0.5), dict(top_k=1500, top_p=0.7),
                    dict(top_k=3000, top_p=0.95, min_p=0.01), dict(top_k=40000)):
         compare(logits, uniform, **params)
+
+
+@pytest.mark.parametrize("rows,vocab,dtype", [(64, 128256, torch.float16), (40, 131072, torch.bfloat16),
+                                              (150, 16384, torch.float32), (160, 32768, torch.float32)], ids=str)
+@pytest.mark.parametrize("top_p", [0.05, 0.5, 0.9])
+def test_a_list_for_top_p_where_top_k_has_overflowed(cuda_device, rows, vocab, dtype, top_p):
+    """top_k of nearly as many tokens as there are threads, some of which have but
+    unlikely tokens, so that no list holds the candidates; and few tokens that have
+    top_p of the sum."""
+    gen = torch.Generator(device=cuda_device).manual_seed(rows)
+    threads = 512 * -(-vocab // (16384 if dtype == torch.float32 else 32768))
+    logits = (3 * torch.randn((rows, vocab), generator=gen, device=cuda_device)).abs().to(dtype)
+    size = logits.element_size()
+    # (What five threads of a CTA read: of every 8192 bytes 16 each.)
+    logits[:, torch.arange(vocab, device=cuda_device) % (8192 // size) < 80 // size] = 2.0
+    logits[::3] = torch.round(logits[::3])  # ties, thousands at the cut
+    uniform = torch.rand(rows, generator=gen, device=cuda_device)
+    for params in (dict(), dict(temperature=0.5), dict(temperature=2.0, min_p=0.01)):
+        compare(logits, uniform, top_k=threads - 3, top_p=top_p, **params)
