@@ -107,12 +107,21 @@ class PagedDecoder:
         both = self._linear(x, gu).view(x.shape[0], -1, 2, 8)
         return ops.silu_mul(both.transpose(1, 2).reshape(x.shape[0], -1))
 
+    def _embed(self, tokens: torch.Tensor) -> torch.Tensor:
+        """Rows of the embedding. A token below 0, which ``sample`` draws from
+        logits that are not numbers, is NaN, not another token's row: its sequence's
+        logits are not numbers either, and its further draws -1."""
+        if not tokens.is_cuda:
+            return self.dec.embed[tokens]
+        h = self.dec.embed[tokens.clamp(min=0)]
+        return h.masked_fill_((tokens < 0)[:, None], float("nan"))
+
     def _forward(self, tokens, store, attend, last) -> torch.Tensor:
         """All layers over packed tokens: ``store(layer, qkv)`` rotates, puts
         keys and values into the cache and gives the queries, ``attend(layer,
         q)`` is the attention. Logits of rows ``last``."""
         dec, cfg = self.dec, self.dec.cfg
-        h = dec.embed[tokens]
+        h = self._embed(tokens)
         pending = None
         for layer, w in enumerate(dec.layers):
             x = ops.add_rms_norm(h, pending, dec.attn_norm[layer], cfg.eps)
@@ -308,7 +317,9 @@ class PagedDecoder:
         """The next tokens of rows of logits: ``sample_tokens`` with ``params``
         (temperature, top_k, top_p, min_p) and random numbers of ``generator``
         (of the model's device; at world > 1 one is needed that every rank has
-        seeded alike). Without params the largest logits."""
+        seeded alike). Without params the largest logits. A row without a logit
+        above -inf draws -1: ``step`` takes that on the GPU as a token of no
+        value (the sequence's logits become NaN), and refuses it on the host."""
         if not params:
             return logits.argmax(-1)
         if self.dec.world > 1 and generator is None:

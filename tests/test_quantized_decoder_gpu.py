@@ -135,3 +135,30 @@ def test_a_step_captured_in_a_graph_serves_other_lengths(cuda_device):
         torch.cuda.synchronize()
         assert torch.equal(o, want[i][0]) and torch.equal(t, want[i][1])
     assert _native.device_status(dev.index, reset=True) == 0
+
+
+@pytest.mark.parametrize("codes", [None, torch.int8], ids=str)
+def test_a_draw_from_no_numbers_is_not_another_token(cuda_device, codes):
+    """-1, drawn from logits that are NaN, gives its sequence NaN and nothing to
+    the others, whose steps are those beside an ordinary token, bit for bit."""
+    dec = TPDecoder(CFG, QCFG, seed=3, device=cuda_device, batch=4, kv_len=0)
+    gen = torch.Generator().manual_seed(9)
+    prompts = [torch.randint(0, CFG.vocab, (n,), generator=gen) for n in (4, 20, 17)]
+    both = []
+    for bad in (True, False):
+        serve = PagedDecoder(dec, n_pages=64, page_size=16, max_positions=256, codes=codes)
+        ids, logits = serve.add(prompts)
+        if bad:
+            logits[1] = float("nan")
+        drawn = serve.sample(logits, torch.Generator(device=cuda_device).manual_seed(2), temperature=0.9, top_p=0.9)
+        assert (int(drawn[1]) == -1) == bad
+        steps = []
+        for _ in range(20):
+            logits = serve.step(ids, drawn)
+            steps.append(logits[[0, 2]])
+            assert bool(logits[1].isnan().all()) == bad and bool(steps[-1].isfinite().all())
+            drawn = serve.sample(logits, temperature=0.9, top_k=1)
+            assert (int(drawn[1]) == -1) == bad
+        both.append(torch.stack(steps))
+    assert torch.equal(*both)
+    assert _native.device_status(cuda_device.index, reset=True) == 0
