@@ -357,7 +357,7 @@ Quantized quantized(PyObject* const* a) {
 }
 
 void forward_only_cache(const at::Tensor& x, const Quantized& c) {
-  forward_only({&x, c.t[2], c.t[3], c.t[4], c.t[5]});
+  forward_only({&x, c.t[0], c.t[1], c.t[2], c.t[3], c.t[4], c.t[5]});
 }
 
 // (qkv, cos, sin, positions, cache: 6, block_table, open_slots, q_starts,
@@ -517,8 +517,10 @@ PyObject* sample(PyObject* const* a, Py_ssize_t n) {
       uniform.get_device() != logits.get_device() || !uniform.is_contiguous())
     reject("uniform must be a contiguous float32 tensor of %lld rows on cuda:%d", static_cast<long long>(rows),
            static_cast<int>(logits.get_device()));
-  if (at::GradMode::is_enabled() && logits.requires_grad())
-    reject("a draw has no gradient: the logits require one (call it under torch.no_grad())");
+  if (at::GradMode::is_enabled())
+    for (int i = 0; i < 6; ++i)
+      if (THPVariable_Check(a[i]) && THPVariable_Unpack(a[i]).requires_grad())
+        reject("a draw has no gradient: an input requires one (call it under torch.no_grad())");
   dqg_sampling s;
   parameter(a[2], logits, "temperature", &s.temperatures, &s.temperature);
   parameter(a[3], logits, "top_k", &s.top_ks, &s.top_k);

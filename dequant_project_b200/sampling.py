@@ -42,8 +42,9 @@ def sample_tokens(logits: torch.Tensor, uniform: torch.Tensor, *, temperature: t
                            0.0 if min_p is None else min_p)
     if logits.is_cuda:
         return paged._binding().sample_tokens(logits, uniform, temperature, top_k, top_p, min_p)
-    if torch.is_grad_enabled() and logits.requires_grad:
-        raise RuntimeError("a draw has no gradient: the logits require one (call it under torch.no_grad())")
+    inputs = (logits, uniform, temperature, top_k, top_p, min_p)
+    if torch.is_grad_enabled() and any(isinstance(x, torch.Tensor) and x.requires_grad for x in inputs):
+        raise RuntimeError("a draw has no gradient: an input requires one (call it under torch.no_grad())")
     rows, vocab = logits.shape
 
     def column(p, dtype):

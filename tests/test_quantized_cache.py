@@ -103,3 +103,13 @@ def test_draws_by_hand():
     assert token(0.9, temperature=0.0) == (2, 1.0) and token(0.9, top_p=0.0) == (2, 1.0)
     assert token(0.32, temperature=0.5)[0] == 2                               # weights 1, 4, 16, 1 of 22
     assert token(0.22, temperature=0.5)[0] == 1
+
+
+@pytest.mark.parametrize("name", ["uniform", "temperature", "top_p", "min_p"])
+def test_draws_refuse_parameters_that_require_a_gradient(name):
+    args = dict(uniform=torch.full((2,), 0.5), temperature=torch.ones(2), top_p=torch.ones(2), min_p=torch.zeros(2))
+    args[name].requires_grad_()
+    with pytest.raises(RuntimeError, match="no gradient"):
+        sample_tokens(torch.zeros((2, 4)), **args)
+    with torch.no_grad():
+        assert sample_tokens(torch.zeros((2, 4)), **args)[0].tolist() == [2, 2]

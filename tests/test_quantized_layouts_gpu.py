@@ -370,3 +370,29 @@ def test_queries_of_any_size(cuda_device, codes, power):
         one = table[b:b + 1], slots[b:b + 1], kl[b:b + 1]
         check_attention(out[b:b + 1], ref[b:b + 1], largest_value(cache, *one), torch.bfloat16,
                         query_rounding(q[b:b + 1], cache, *one))
+
+
+def test_inputs_that_require_a_gradient_are_refused(cuda_device):
+    """Codes in e4m3 as well, and a draw's parameters."""
+    from dequant_project_b200.sampling import sample_tokens
+
+    q, one, starts = torch.zeros((1, 4, 64), device=cuda_device).half(), ints([0], cuda_device), ints([0, 1], cuda_device)
+    cos, sin = paged_ops.rope_scaled_tables(64, 1e4, 8, cuda_device)
+    qkv = torch.zeros((1, 8 * 64), device=cuda_device).half()
+    for which in range(6):
+        cache = qc.QuantizedCache.empty(4, 2, 32, 64, 2, codes=torch.float8_e4m3fn, device=cuda_device)
+        cache[which].requires_grad_()
+        for call in (lambda: qc.quantized_attention(q, cache, one[None], one, one),
+                     lambda: qc.quantized_prompt_attention(q, cache, one[None], one, starts, one, 1),
+                     lambda: qc.expanded_pages(cache, one[None], one, one, 1),
+                     lambda: qc.rope_quantized_append(qkv, cos, sin, one.long(), cache, one[None], one, starts,
+                                                      one + 1, 4)):
+            with pytest.raises(RuntimeError, match="forward only"):
+                call()
+    logits = torch.zeros((1, 4), device=cuda_device)
+    args = dict(uniform=torch.zeros(1, device=cuda_device), temperature=torch.ones(1, device=cuda_device),
+                top_p=torch.ones(1, device=cuda_device), min_p=torch.zeros(1, device=cuda_device))
+    for name in args:
+        with pytest.raises(RuntimeError, match="no gradient"):
+            sample_tokens(logits, **{**args, name: args[name].clone().requires_grad_()})
+    sample_tokens(logits, **args)
