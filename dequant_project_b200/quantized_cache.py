@@ -19,7 +19,7 @@ position or row start out of range is left out and reported by
 CUDA tensors go through the sm_100a kernels of libdequant_b200.so on torch's
 current stream (``binding/paged_binding.cpp``); if it is missing these calls
 raise. CPU tensors take the same formulas in torch: that branch exists for the
-host-logic tests and is never taken for a CUDA tensor.
+host-logic tests and is never taken where a cache or its queries are on a GPU.
 
 The reference has none of this; it models the cache's bytes
 (KrishnaI2424/Dequant_Project ``dequant/byte_model.py:214-219``).
@@ -138,7 +138,7 @@ def rope_quantized_append(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tenso
     [B, pages]) and to its open block. Rows behind the last sequence are rotated
     and not stored. Keys and values are rounded to the 16-bit type first, as a
     16-bit cache holds them. Everything else as ``rope_paged_append``."""
-    if qkv.is_cuda:
+    if qkv.is_cuda or cache.k.is_cuda:
         return paged._binding().rope_quantized_append(qkv, cos, sin, positions, *cache, block_table, open_slots,
                                                       q_starts, kv_lens, n_q_heads, interleaved, q_norm, k_norm, eps)
     paged._forward_only(qkv, cos, sin, *cache, q_norm, k_norm)
@@ -164,7 +164,7 @@ def quantized_attention(q: torch.Tensor, cache: QuantizedCache, block_table: tor
     a sequence without positions. Codes enter the products exactly, scales in
     fp32. ``workspace``: ``quantized_attention_workspace``; calls that share one
     must not overlap."""
-    if q.is_cuda:
+    if q.is_cuda or cache.k.is_cuda:
         return paged._binding().quantized_attention(q, *cache, block_table, open_slots, kv_lens, scale, workspace)
     paged._forward_only(q, *cache)
     scale = 1.0 / math.sqrt(q.shape[2]) if scale is None else scale
@@ -218,7 +218,7 @@ def quantized_prompt_attention(q: torch.Tensor, cache: QuantizedCache, block_tab
     ``workspace``: ``quantized_prompt_workspace``, mostly n_pages * 4 * Hkv *
     page size * D bytes; calls that share one must not overlap. Everything else
     as ``prompt_attention``."""
-    if q.is_cuda:
+    if q.is_cuda or cache.k.is_cuda:
         return paged._binding().quantized_prompt_attention(q, *cache, block_table, open_slots, q_starts, kv_lens,
                                                            n_pages, causal, scale, workspace)
     paged._forward_only(q, *cache)

@@ -396,3 +396,18 @@ def test_inputs_that_require_a_gradient_are_refused(cuda_device):
         with pytest.raises(RuntimeError, match="no gradient"):
             sample_tokens(logits, **{**args, name: args[name].clone().requires_grad_()})
     sample_tokens(logits, **args)
+
+
+def test_queries_on_the_host_beside_a_cache_on_the_gpu_are_refused(cuda_device):
+    cache = qc.QuantizedCache.empty(4, 2, 32, 64, 2, device=cuda_device)
+    q, one, starts = torch.zeros((1, 4, 64)).half(), ints([0], cuda_device), ints([0, 1], cuda_device)
+    cos, sin = paged_ops.rope_scaled_tables(64, 1e4, 8, cuda_device)
+    for call, name in ((lambda: qc.quantized_attention(q, cache, one[None], one, one), "q"),
+                       (lambda: qc.quantized_prompt_attention(q, cache, one[None], one, starts, one, 1), "q"),
+                       (lambda: qc.rope_quantized_append(torch.zeros((1, 8 * 64)).half(), cos, sin, one.long(), cache,
+                                                         one[None], one, starts, one + 1, 4), "qkv")):
+        with pytest.raises(RuntimeError, match=f"^{name} must be float16 on cuda"):
+            call()
+    host = qc.QuantizedCache.empty(4, 2, 32, 64, 2, device="cpu")
+    with pytest.raises(RuntimeError, match="k must be a CUDA tensor"):
+        qc.quantized_attention(q.to(cuda_device), host, one[None], one, one)
