@@ -116,3 +116,39 @@ def test_generate_draws_what_its_generator_says():
     serve.dec.world = 2
     with pytest.raises(ValueError, match="seeded alike"):
         serve.sample(torch.zeros((1, 5)), temperature=1.0)
+
+
+def _serve(world):
+    import socket
+
+    import torch.multiprocessing as mp
+
+    import paged_workers
+    with socket.socket() as s:
+        s.bind(("127.0.0.1", 0))
+        port = s.getsockname()[1]
+    ctx = mp.get_context("spawn")
+    queue = ctx.Queue()
+    procs = [ctx.Process(target=paged_workers.serve_quantized, args=(r, world, port, queue)) for r in range(world)]
+    for p in procs:
+        p.start()
+    got = {}
+    for _ in procs:
+        rank, results, err = queue.get(timeout=120)
+        assert err is None, err
+        got[rank] = [torch.from_numpy(x) for x in results]
+    for p in procs:
+        p.join(timeout=60)
+        assert p.exitcode == 0
+    return got
+
+
+def test_two_ranks_serve_what_one_does():
+    """Heads over two gloo ranks, each with open blocks of its own: both gather
+    the same logits and draw the same tokens. One rank's logits differ by the order
+    of sums, which can turn a code over: as much as rounding to codes does at most."""
+    one, two = _serve(1)[0], _serve(2)
+    assert torch.equal(two[0][0], two[1][0]) and torch.equal(two[0][1], two[1][1])
+    assert max_rel_err(two[0][0], one[0]) < BOUND[torch.int8]
+    for _, draws in (one, two[0]):
+        assert draws.shape == (2, 8) and bool(((draws >= 0) & (draws < 1001)).all())
