@@ -18,6 +18,7 @@ struct Desc {    // an item that is joined later
 };
 
 struct DecodeParams {
+  static constexpr bool kPrefix = true;  // whether a call may have a shared prefix
   const void* q;
   void* out;
   const int32_t* table;
@@ -71,7 +72,7 @@ template <class P>
 __device__ __forceinline__ Share find_share(const P& p, int cta, int n_ctas) {
   const int lane = threadIdx.x & 31;
   const int hv = p.hkv * p.nrb;
-  const long long pre = static_cast<long long>(p.pre_items) * (p.pre_tiles + p.item_tiles);
+  const long long pre = P::kPrefix ? static_cast<long long>(p.pre_items) * (p.pre_tiles + p.item_tiles) : 0;
   auto cost = [&](int b) {
     return b < p.B ? tiles_of(p, clamped_len(p.lens, b, p.len_limit)) + p.item_tiles : 0;
   };
@@ -97,7 +98,7 @@ __device__ __forceinline__ Share find_share(const P& p, int cta, int n_ctas) {
     s.count = min(total, pos + each) - pos;
     uint32_t per = p.pre_tiles + p.item_tiles, in = pos;
     s.b = -1;
-    if (pos >= ahead) {
+    if (!P::kPrefix || pos >= ahead) {
       const unsigned past = __ballot_sync(0xffffffffu, sum * hv > pos - ahead);
       const int l = past ? __ffs(past) - 1 : 0;
       per = max(1u, __shfl_sync(0xffffffffu, c, l));
@@ -121,7 +122,7 @@ __device__ __forceinline__ Share find_share(const P& p, int cta, int n_ctas) {
   if (s.count == 0) return s;
   long long before = 0;
   int per = p.pre_tiles + p.item_tiles;
-  if (s.pos >= pre) {  // (prefix items come first, as sequence -1)
+  if (!P::kPrefix || s.pos >= pre) {  // (prefix items come first, as sequence -1)
     before = pre;
 #pragma unroll 1
     for (int b0 = 0; b0 < p.B; b0 += 32) {
@@ -157,7 +158,7 @@ struct Item {
 template <class P>
 __device__ __forceinline__ Item item_of(const P& p, const Share& s) {
   Item i;
-  if (s.b < 0) {
+  if (P::kPrefix && s.b < 0) {
     const int blocks = p.pre_items / p.hkv;
     i.kvh = s.hv / blocks;
     i.first = (s.hv - i.kvh * blocks) * p.pre_seqs;
@@ -182,11 +183,12 @@ __device__ __forceinline__ Item item_of(const P& p, const Share& s) {
   return i;
 }
 // Behind n units of the item at hand.
-__device__ __forceinline__ void advance(const DecodeParams& p, Share& s, int n) {
+template <class P>
+__device__ __forceinline__ void advance(const P& p, Share& s, int n) {
   s.pos += n;
   s.count -= n;
   s.x = 0;
-  if (++s.hv == (s.b < 0 ? p.pre_items : p.hkv * p.nrb)) {
+  if (++s.hv == (P::kPrefix && s.b < 0 ? p.pre_items : p.hkv * p.nrb)) {
     s.hv = 0;
     ++s.b;
   }
@@ -204,7 +206,8 @@ __device__ __forceinline__ int64_t whole_row(const DecodeParams& p, int b, int h
 // decode kernel left, and the shared prefix's behind them. The pieces are
 // dealt to groups of threads (several loads of each in flight), whose results
 // are joined in order. kMeans: a piece is the mean of its values (which may be as
-// large as fp32 goes), not their sum, and counts by its weights' sum.
+// large as fp32 goes), not their sum, and counts by its weights' sum; no call has a
+// prefix then.
 constexpr int kJoinThreads = 256;
 
 template <typename E, int D, int R, bool kMeans>
@@ -225,21 +228,21 @@ __global__ void __launch_bounds__(kJoinThreads)
   // A streamed prefix's pieces are described as an item's are.
   Desc f{0, 0, 0, 0};
   int f_row = 0;
-  if (p.pre_items) {
+  if (!kMeans && p.pre_items) {
     const int pid = kvh * (p.pre_items / p.hkv) + d.b / p.pre_seqs;
     const int4 t = __ldcg(reinterpret_cast<const int4*>(p.desc + gridDim.x + pid));
     f = Desc{t.x, t.y, t.z, t.w};
     f_row = d.b % p.pre_seqs * p.g + row;
   }
-  const int own = d.pieces, all = own + p.prefix.S + f.pieces;
+  const int own = d.pieces, all = kMeans ? own : own + p.prefix.S + f.pieces;
   // Piece 0 lies in its CTA's second place, piece i > 0 in CTA + i's first; a
   // whole result in the item's own.
   auto row_of = [&](const Desc& e, int i) {
-    return e.cta < 0 ? whole_row(p, e.b, e.hv)
+    return !kMeans && e.cta < 0 ? whole_row(p, e.b, e.hv)
                      : (2 * (static_cast<int64_t>(e.cta) + i) + (i == 0 ? 1 : 0)) * p.rows;
   };
-  const int64_t pre = p.prefix.S ? prefix_first(p.prefix, p.hkv, d.b, kvh) : 0;
-  const int pre_row = p.prefix.S ? prefix_row(p.prefix, p.g, d.b, rb * 16 + row) : 0;
+  const int64_t pre = !kMeans && p.prefix.S ? prefix_first(p.prefix, p.hkv, d.b, kvh) : 0;
+  const int pre_row = !kMeans && p.prefix.S ? prefix_row(p.prefix, p.g, d.b, rb * 16 + row) : 0;
   float m = -INFINITY, l = 0.f;
   float4 num = make_float4(0.f, 0.f, 0.f, 0.f);
   if (row < rows) {
@@ -253,12 +256,12 @@ __global__ void __launch_bounds__(kJoinThreads)
         pm[u] = -INFINITY;
         pl[u] = 0.f;
         v[u] = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (i < own || (i < all && p.pre_items)) {
+        if (i < own || (!kMeans && i < all && p.pre_items)) {
           const int64_t at = i < own ? row_of(d, i) + row : row_of(f, i - own) + f_row;
           pm[u] = __ldcg(p.m + at);
           pl[u] = __ldcg(p.l + at);
           v[u] = __ldcg(reinterpret_cast<const float4*>(p.part + at * D) + d4);
-        } else if (i < all) {
+        } else if (!kMeans && i < all) {
           const int64_t s = pre + i - own;
           pm[u] = __ldcg(p.prefix.ml + s * 512 + pre_row);
           pl[u] = __ldcg(p.prefix.ml + s * 512 + 256 + pre_row);
@@ -339,7 +342,7 @@ cudaError_t launch_join(const DecodeParams& p, cudaLaunchConfig_t cfg) {
   // Query heads a join block takes: few, so that the pieces of a small batch
   // spread over many threads, but one where there is one.
   const int rows = p.g < 16 ? p.g : 16, per = rows == 1 ? 1 : 4;
-  const int64_t items = p.prefix.S || p.pre_items ? static_cast<int64_t>(p.B) * p.hkv * p.nrb : p.n_ctas;
+  const int64_t items = !kMeans && (p.prefix.S || p.pre_items) ? static_cast<int64_t>(p.B) * p.hkv * p.nrb : p.n_ctas;
   if (items > 0x7fffffff) return cudaErrorInvalidValue;
   cfg.gridDim = dim3(static_cast<unsigned>(items), (rows + per - 1) / per);
   cfg.blockDim = dim3(kJoinThreads);

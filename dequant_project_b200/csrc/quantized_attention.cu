@@ -63,6 +63,7 @@ constexpr float kMaxGrowth = 8.f, kHeadroom = 7.f;  // log2 units
 constexpr float kOpenTop = 14.f;  // of fp16 open rows' weights, the largest
 
 struct Params : DecodeParams {
+  static constexpr bool kPrefix = false;
   const float* k_scale;
   const float* v_scale;
   const void* k_open;
@@ -890,7 +891,6 @@ cudaError_t launch_quantized_attention(const QuantizedPool& pool, const Quantize
   p.m = p.part + s.rows * pool.D;
   p.l = p.m + s.rows;
   p.rows = s.per_piece;
-  p.pre_seqs = 1;
   p.q_stride_seq = a.q_stride_seq;
   p.q_stride_head = a.q_stride_head;
   p.table_stride = seqs.table_stride;
