@@ -8,11 +8,13 @@
 // goes this way too, with keys as codes (exact in 16 bits) whose scales the
 // prompt kernel applies to its scores: key values rounded to bf16 would move a
 // score by 2^-9 of itself. Values become codes times the power of two at or below
-// the scale, exact too; what is left of the scale, in [1, 2), goes to the softmax's
-// weights (rounded values cost as much precision as the weights' rounding does:
-// fp16 error 3.2e-4 instead of 2.5e-4). In the product loop the codes would be expanded once
-// for every 256 rows (and by warps that share their issue slots with the
-// softmax that bounds it), here once for all.
+// the scale, exact too but for small ones in fp16: powers below 2^-24 (int8) or
+// 2^-15 (e4m3, whose least code is 2^-9) give numbers below its normal ones, off by
+// up to 2^-25. What is left of the scale, in [1, 2), goes to the softmax's weights
+// (rounded values cost as much precision as the weights' rounding does: fp16 error
+// 3.2e-4 instead of 2.5e-4). In the product loop the codes would be expanded once
+// for every 256 rows (and by warps that share their issue slots with the softmax
+// that bounds it), here once for all.
 //
 // Bound by HBM: a byte read and two written a value. A block takes one page of
 // as many heads as give its threads work (7000 positions of 8 heads in pages of 16
@@ -86,9 +88,10 @@ __device__ __forceinline__ void look_over(const Params& p, uint32_t* scratch) {
   if (bad) atomicOr(&g_status, kStatusBadIndex);
 }
 
-// (Eight blocks an SM. With six the expansion alone would be faster, 10.6 us
-// instead of 11.2 for 2048 positions of 32 heads, but the prompt kernel behind it
-// starts later: 78.3 us a call instead of 76.1.)
+// (Eight blocks an SM, so 32 registers, for which int8's four variants spill 12
+// bytes. With six the expansion alone would be faster, 10.6 us instead of 11.2 for
+// 2048 positions of 32 heads, but the prompt kernel behind it starts later: 78.3 us
+// a call instead of 76.1.)
 template <typename E, class Code, int D>
 __global__ void __launch_bounds__(kThreads, 8) expand_pages_kernel(const __grid_constant__ Params p) {
   __shared__ uint32_t scratch[kThreads / 32 + 2];

@@ -22,8 +22,11 @@
 // of which the writes that stay in L2 show half (172 MB read, 96 MB written).
 // Registers bound it next (29 % of the warps resident, at 96): eight heads a
 // lane group one after the other took 114 us, four with passes and codes apart
-// 67, keys' and values' rows loaded together 65. Small batches are a launch: 8
-// tokens 4.4 us in a graph.
+// 67, keys' and values' rows loaded together 65. (Of the 30 variants the five of
+// uneven rotations in two or four passes spill, 16 to 60 bytes.) With heads of 64
+// and blocks of 16 half of a block's threads have no row: 1754 tokens in ragged
+// chunks, of 32 and 8 such heads, take 9.9 us. Small batches are a launch: 8 tokens
+// 4.3 us in a graph.
 #include <cstdint>
 
 #include "paged_rope.cuh"

@@ -24,24 +24,28 @@
 // registers, exactly (Pairs), in whatever order of the summed index that gives,
 // the queries' being the same. Beside e4m3 codes bf16 queries become fp16 times
 // a power of two for each head, the largest between 2^14 and 2^15: what that
-// loses is below 2^-39 of the largest. Scores are scaled in fp32. So are the weights: besides
-// the softmax's reference (of the scores) the sum over values has one of its
-// own, of the score plus log2 s_v, so that a 16-bit weight is relative to the
-// largest p s_v met, whatever the blocks' scales are. Both references move, and
-// the sums are rescaled, only when a slice exceeds one by more than 2^kMaxGrowth;
-// of fp16's range (2^-24 to 2^16) a weight loses below 2^-32 of the largest.
-// Open rows go through products of their own type, with weights relative to their
-// own largest.
+// loses is below 2^-39 of the largest; beside int8 codes they are digits (Pairs).
+// Scores are scaled in fp32. So are the weights: besides the softmax's reference
+// (of the scores) the sum over values has one of its own, of the score plus log2
+// s_v, so that a 16-bit weight is relative to the largest p s_v met, whatever the
+// blocks' scales are. Both references move, and the sums are rescaled, only when a
+// slice exceeds one by more than 2^kMaxGrowth; of fp16's range (2^-24 to 2^16) a
+// weight loses below 2^-32 of the largest. (A weight's one rounding to fp16 adds up
+// to a tenth to the output's own error: 2.2e-4 instead of 2.1e-4 for 2049 positions
+// in fp16.) Open rows go through products of their own type, with weights relative
+// to their own largest. The warps' parts, and the pieces of cut items, are merged as
+// means of the values, so that what is finite in the cache gives a finite result.
 //
 // HBM bounds the large calls: 64 sequences of 0 to 16000 positions (64 and 8
-// heads of 128, int8, 0.63 GB) take 116 us, joining included, 5.4 TB/s (127 in a
-// stream of tens of ms, where the power cap lowers the clock to 1.78 GHz); 64 of
-// 8000 (1 GB) 178 us, 5.9 TB/s, and e4m3 174 us, 6.0 TB/s. What is left between is
-// items' starts and ends and the second kernel. Short calls are latency: one
-// sequence of 2049 positions of 32 heads 12.2 us for 2.6 us of bytes. Steps that
-// counted, 64 sequences: a warp a position on plain lanes 4154 us; tensor
-// products 147; seven consumer warps at 128 registers, two CTAs, 136; integer
-// products of the keys and the merge in rounds of four heads 119.
+// heads of 128, int8, 0.63 GB) take 117 to 119 us, joining included, 5.3 TB/s (124
+// to 129 in a longer stream, where the power cap lowers the clock); 64 of 8000 (1
+// GB) 180 us, 5.8 TB/s, and e4m3 171 us, 6.1 TB/s (200 and 188 in a stream of 0.4
+// s). What is left between is items' starts and ends and the second kernel. Short
+// calls are latency: one sequence of 2049 positions of 32 heads 11.5 us for 2.6 us of
+// bytes. Steps that counted, 64 sequences: a warp a position on plain lanes 4154 us;
+// tensor products 147; seven consumer warps at 128 registers, two CTAs, 136; integer
+// products of the keys and the merge in rounds of four heads 119; a third digit of
+// the queries 2 % more; no code for a prefix 1 % less (2049 positions 12.5 -> 11.5).
 //
 // Waits are bounded, as in paged_attention.cu: a consumer warp whose wait ran
 // out goes on without data and makes its results NaN.
@@ -125,8 +129,8 @@ __device__ __forceinline__ void cp_async_arrive(uint64_t* bar) {
 // again by an addition took 64 more instructions of about 430 a slice.
 // Keys: e4m3 the same way. int8 codes enter integer products as they are, beside
 // the queries as integers of 23 bits, relative to their head's largest, in three int8
-// digits: what that loses is below 2^-24 of the largest, so that a channel far above
-// the others takes nothing that matters from them. (Two digits, 2^-17, took 1 to 2 %
+// digits: what that loses is at most 2^-23 of the largest, so that a channel far above
+// the others takes nothing that matters from them. (Two digits, 2^-16, took 1 to 2 %
 // less time, and a channel of 4000 made outputs 0.04 of a value off. Codes as fp16
 // numbers, as the values, beside the queries' own took 9 % more: 64 sequences of 8000
 // 195 us instead of 180 in a graph.)

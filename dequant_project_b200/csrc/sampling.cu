@@ -6,9 +6,10 @@
 //
 // Ranks are by logit, the lower index first. All sums are of 64-bit integers:
 // exact, so that neither the order of summation nor the number of threads or
-// CTAs changes a token. A W is exact to about 2^-31 of itself: the exponent is
-// formed in pairs of fp32 numbers, its fraction in 64ths from a table and the rest
-// by a polynomial (a 64-bit exp took more than half of the time).
+// CTAs changes a token. A w is rounded once: by 2^-31 of itself, or by 2^-45 where
+// that is more (half of a W's unit). The exponent is formed in pairs of fp32
+// numbers, its fraction in 64ths from a table and the rest by a polynomial (a 64-bit
+// exp took more than half of the time).
 //
 // A cluster of up to eight CTAs takes a row; each holds a part of it in shared
 // memory, and a thread a run of consecutive tokens of that. The logit at which
@@ -24,13 +25,15 @@
 //
 // Neither HBM nor arithmetic bounds it, but the chain of steps that each need
 // the whole row's last (barriers are the largest stall: 5 cycles a warp's
-// instruction): 64 rows of 128256 in fp16 with all parameters 31 us (16.4 MB,
-// 2.5 us), up to 50 where the cuts fall in flat places, one row of 32000 13 us,
-// 256 rows of 32000 in fp32 33 us. Top-k alone (50) takes 17 us for the 64 rows;
-// top-p of 0.9 over normal logits (deviation 3), whose cut lies among ten thousand
-// tokens, 72 (114 with lists of 2048 a CTA, which do not hold them). A row a CTA with a 64-bit exp took 412 us, clusters
-// 116, weights in pairs 61, short lists 42; rows kept in their own type, so that
-// half the CTAs hold one and all 64 rows run at once, 31.
+// instruction): 64 rows of 128256 in fp16 with all parameters 29 to 37 us by
+// the rows drawn (16.4 MB, 2.5 us), up to 50 where the cuts fall in flat places, one
+// row of 32000 9 to 13 us, 256 rows of 32000 in fp32 33 us (without a cut: occupancy
+// bounds that, two CTAs an SM and so two waves of them). Top-k alone (50) takes 17 us
+// for the 64 rows; top-p of 0.9 over normal logits (deviation 3), whose cut lies among
+// ten thousand tokens, 72 (114 with lists of 2048 a CTA, which do not hold them). A
+// row a CTA with a 64-bit exp took 412 us, clusters 116, weights in pairs 61, short
+// lists 42; rows kept in their own type, so that half the CTAs hold one and all 64
+// rows run at once, 31.
 #include <cstdint>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>

@@ -58,8 +58,13 @@ class PagedDecoder:
     (this rank's heads), ``page_size`` positions each, for sequences of up to
     ``max_positions`` positions. ``codes`` (int8 or float8_e4m3fn; default: 16
     bits) holds the cache in 8 bits, with a scale for every ``block`` positions
-    of a head and open blocks for ``max_seqs`` sequences. At world > 1 every
-    rank makes the same calls."""
+    of a head and open blocks for ``max_seqs`` sequences (4 * block * head_dim
+    bytes a head of keys and values, layer and sequence). A pass over prompts then
+    takes scratch memory of 4 * head_dim bytes a head for every position that its
+    sequences have, twice what the codes take; and a prefix is shared in the pages
+    alone: ``add`` expands it, and ``step`` reads it, once for every sequence, where
+    the 16-bit cache's is read once a batch. At world > 1 every rank makes the same
+    calls."""
 
     def __init__(self, dec: TPDecoder, n_pages: int, page_size: int = 16, max_positions: int = 4096,
                  rope_scaling: dict | None = None, *, codes: torch.dtype | None = None, block: int = 16,

@@ -8,6 +8,9 @@ sequence, a row of page numbers in ``block_table``: position t lies in page
 strided views (of one allocation for keys and values, say) as long as both have
 the same strides and D is contiguous.
 
+Sums of weights times values are fp32, of weights up to 2^15 (fp16's range): bf16
+values above about 2^100 may overflow them. (Over an 8-bit cache they do not.)
+
 Forward only: an input that requires a gradient is refused while gradients are
 recorded (``torch.no_grad()`` allows it). ``rope_paged_append`` writes the pages
 in place.

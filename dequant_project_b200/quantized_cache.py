@@ -161,9 +161,10 @@ def quantized_attention(q: torch.Tensor, cache: QuantizedCache, block_table: tor
                         workspace: torch.Tensor | None = None) -> torch.Tensor:
     """``paged_ops.paged_attention`` over an 8-bit cache: one query token per
     sequence, q [B, Hq, D] (strides free, D contiguous) -> [B, Hq, D]; zeros for
-    a sequence without positions. Codes enter the products exactly, scales in
-    fp32. ``workspace``: ``quantized_attention_workspace``; calls that share one
-    must not overlap."""
+    a sequence without positions. Codes enter the products exactly (int8 ones
+    beside queries to 2^-23 of their head's largest value), scales in fp32.
+    ``workspace``: ``quantized_attention_workspace``; calls that share one must not
+    overlap."""
     if q.is_cuda or cache.k.is_cuda:
         return paged._binding().quantized_attention(q, *cache, block_table, open_slots, kv_lens, scale, workspace)
     paged._forward_only(q, *cache)
@@ -187,9 +188,10 @@ def expanded_pages(cache: QuantizedCache, block_table: torch.Tensor, open_slots:
     ``(k_pages, v_pages, table)``, pools of ``n_pages`` pages and a table as
     ``block_table``. One sequence's pages follow the other's; each value is
     rounded once to the 16-bit type, and places behind a sequence's end are
-    zeros. ``n_pages`` is the number that the sequences take (sum of
-    ceil(len / page size)) or more; what has no room is left out and reported,
-    pages that nothing takes are undefined."""
+    zeros; the table's entries behind a sequence's pages are undefined. ``n_pages``
+    is the number that the sequences take (sum of ceil(len / page size)) or more;
+    what has no room is left out and reported, pages that nothing takes are
+    undefined."""
     if cache.k.is_cuda:
         return paged._binding().expand_pages(*cache, block_table, open_slots, kv_lens, n_pages)
     paged._forward_only(*cache)
@@ -214,7 +216,8 @@ def quantized_prompt_attention(q: torch.Tensor, cache: QuantizedCache, block_tab
     """``paged_ops.prompt_attention`` over an 8-bit cache, whose positions are
     first expanded once to 16-bit pages (as ``expanded_pages``, which says what
     ``n_pages`` is; but keys stay codes and values codes times a power of two, exact
-    in 16 bits, and the rest of the scales goes to the scores and weights in fp32).
+    in 16 bits but for the smallest in fp16, off by up to 2^-24; and the rest of the
+    scales goes to the scores and weights in fp32).
     ``workspace``: ``quantized_prompt_workspace``, mostly n_pages * 4 * Hkv *
     page size * D bytes; calls that share one must not overlap. Everything else
     as ``prompt_attention``."""

@@ -32,8 +32,9 @@ def sample_tokens(logits: torch.Tensor, uniform: torch.Tensor, *, temperature: t
     times their sum; its logprob is that of this draw. A temperature of 0 (or
     less) takes the largest logit, with logprob 0. NaN counts as -inf; a row
     without a logit above -inf gives -1 and NaN. A ``uniform`` below 0, or NaN,
-    counts as 0; from 1 on it takes the last token kept. The same inputs give the
-    same tokens: each w is rounded once (2^-31 of itself, or 2^-45) and sums are of
+    counts as 0; from 1 on it takes the last token kept. (Logits further below the
+    largest than fp32's largest number weigh nothing, whatever the temperature.) The
+    same inputs give the same tokens: each w is rounded once (2^-31 of itself, or 2^-45) and sums are of
     64-bit integers, whatever their order.
 
     Each parameter is a number (taken as fp32; top_k as int32), or a tensor of one a

@@ -520,9 +520,10 @@ int dqg_expand_pages(const dqg_quantized_kv *kv, const int32_t *block_table, int
 /*
  * dqg_prompt_attention over such a cache. The sequences' positions are first
  * expanded once, into the workspace, as dqg_expand_pages does, but with keys as
- * codes and values as codes times a power of two, which are exact in 16 bits; the
- * rest of the scales is applied to scores and weights in fp32. n_pages as there; what sequences give that it leaves pages of out is
- * undefined. Workspace: dqg_quantized_prompt_workspace's bytes (mostly n_pages
+ * codes and values as codes times a power of two, which are exact in 16 bits (but
+ * in fp16 for values below 2^-14 of small scales: off by up to 2^-25 before the rest
+ * of the scale); the rest of the scales is applied to scores and weights in fp32.
+ * n_pages as there; what sequences give that it leaves pages of out is undefined. Workspace: dqg_quantized_prompt_workspace's bytes (mostly n_pages
  * pages of n_kv_heads * page_size * head_dim * 4 bytes), 16-byte aligned, of any
  * contents; calls that share one must not overlap.
  */
@@ -538,7 +539,8 @@ int dqg_quantized_prompt_attention(const void *q, int64_t q_stride_row, int64_t 
 
 /*
  * dqg_paged_attention over such a cache. Products use the codes as they are
- * (exact in 16 bits); scales are applied to scores and weights in fp32.
+ * (exact in 16 bits; beside int8 codes queries to 2^-23 of their head's largest);
+ * scales are applied to scores and weights in fp32.
  */
 int dqg_quantized_attention_workspace(int64_t n_seqs, int64_t n_q_heads, int64_t n_kv_heads,
                                       int64_t head_dim, uint64_t *bytes);
@@ -574,10 +576,12 @@ int dqg_debug_quantized_starved(const void *q, int64_t q_stride_seq, int64_t q_s
  * or NaN) takes the largest logit of lowest index, with logprob 0. NaN counts
  * as -inf; where the largest logit is +inf only such are kept; a row without
  * a logit above -inf gives token -1 and logprob NaN. A random number below 0, or
- * NaN, counts as 0, a temperature below 1e-37 as that. The sums are taken over
- * 64-bit integers (w in units of 2^-44, exact to about 2^-31 of itself), so that
- * they do not depend on an order. Each parameter is an array of `rows` (temperatures, top_ks, top_ps,
- * min_ps on the device) or, where that is NULL, the value beside it.
+ * NaN, counts as 0, a temperature below 1e-37 as that; logits further below m than
+ * fp32's largest number weigh nothing, whatever the temperature. The sums are taken
+ * over 64-bit integers (w in units of 2^-44, rounded once: by 2^-31 of itself or by
+ * 2^-45), so that they do not depend on an order. Each parameter is an array of
+ * `rows` (temperatures, top_ks, top_ps, min_ps on the device) or, where that is NULL,
+ * the value beside it.
  */
 enum { DQG_FP32 = 2 };
 typedef struct dqg_sampling {

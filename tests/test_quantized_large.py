@@ -91,8 +91,8 @@ SIZES = [(37, 1, 16, 16), (9, 4, 64, 64), (64, 8, 64, 64), (3000, 12, 128, 32)] 
 @pytest.mark.parametrize("n,g,page,block", SIZES)
 def test_decode_over_large_values(cuda_device, n, g, page, block, most, codes):
     """|out - ref| <= u |ref| + (u + 2^-13) max|v| as for ordinary values (and, for
-    queries beside int8 codes, what 2^-16 of their largest moves), for a sequence
-    cut into pieces and for many that are not."""
+    queries beside int8 codes, what test_quantized_cache_gpu.py allows), for a
+    sequence cut into pieces and for many that are not."""
     from test_quantized_cache_gpu import attend64, check_attention, ints, query_rounding
 
     q, cache, table, slot, k, v = appended(cuda_device, n, g, page, block, most, codes)
