@@ -37,7 +37,7 @@
 // means of the values, so that what is finite in the cache gives a finite result.
 //
 // HBM bounds the large calls: 64 sequences of 0 to 16000 positions (64 and 8
-// heads of 128, int8, 0.63 GB) take 117 to 119 us, joining included, 5.3 TB/s (124
+// heads of 128, int8, 0.63 GB) take 117 to 119 us, joining included, 5.3 TB/s (122
 // to 129 in a longer stream, where the power cap lowers the clock); 64 of 8000 (1
 // GB) 180 us, 5.8 TB/s, and e4m3 171 us, 6.1 TB/s (200 and 188 in a stream of 0.4
 // s). What is left between is items' starts and ends and the second kernel. Short
